@@ -226,6 +226,115 @@ int ivc_device_properties(int device_ordinal, ivc_device_props *out);
 void ivc_f32_to_f16(const float *in, uint16_t *out, size_t n);
 void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
 
+/* ------------------------------------------------------------------------
+ * Language-model operators: rotary positions, a paged key/value cache held in
+ * 8 bits, and the attention over it, for a decoder that follows a network of
+ * this library (its outputs become tokens).  Inference only.
+ *
+ * All tensors are device memory of the handle's device; nothing is copied and
+ * no call waits for the device.  `stream` is a cudaStream_t; NULL is the
+ * legacy default stream.  Argument errors that the host can see come back as
+ * IVC_ERR_ARGUMENT.  What only the device sees (a page number outside the
+ * cache, offsets or lengths that do not fit, a position beyond the rotary
+ * table) is skipped by the kernels, which set the handle's status word:
+ * ivc_kv_synchronize then returns IVC_ERR_KERNEL and clears it.
+ *
+ * Calls may be captured into a CUDA graph once the stream has had one call of
+ * ivc_kv_attend or ivc_kv_reserve (each stream has its own workspace, so calls
+ * on several streams may run at the same time). */
+typedef struct ivc_kv ivc_kv;
+
+typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1 } ivc_dtype;
+
+/* [tokens][heads][head_dim] of the call's dtype; strides in elements, the last
+ * dimension dense.  Any 2-byte alignment works; 16-byte alignment of data and
+ * strides takes the vector path. */
+typedef struct ivc_rows {
+  void *data;
+  int64_t token_stride, head_stride;
+} ivc_rows;
+
+/* One layer's cache, in the caller's memory.  Codes [pages][kv_heads]
+ * [page_size][head_dim] in -127..127; a value is code * scale, one scale (a
+ * power of two, as ivc_kv_append writes it) for each IVC_KV_BLOCK tokens of a
+ * page and head: [pages][kv_heads][page_size / IVC_KV_BLOCK].  page_size is a
+ * multiple of IVC_KV_BLOCK, head_dim 64 or 128, k and v 16-byte aligned. */
+#define IVC_KV_BLOCK 16
+typedef struct ivc_kv_cache {
+  int8_t *k, *v;
+  float *k_scale, *v_scale;
+  int64_t pages;
+  int page_size, kv_heads, head_dim;
+} ivc_kv_cache;
+
+/* The sequences of a call.  Sequence b owns the packed tokens offsets[b] ..
+ * offsets[b + 1] - 1 (offsets [batch + 1], from 0, not falling; none or more
+ * each).  at[b]: append and read: the cache position of the first of them;
+ * attend: how many tokens the cache holds, the call's own included (they are
+ * the last ones).  The token at position p is in page
+ * pages[b * pages_per_seq + p / page_size].  Device memory, int32. */
+typedef struct ivc_kv_seqs {
+  int batch;
+  int64_t tokens;
+  const int32_t *offsets, *at, *pages;
+  int pages_per_seq;
+} ivc_kv_seqs;
+
+/* Rotary positions with `axes` (1..4) position numbers for each token, e.g.
+ * time, height, width: pos[a * pos_stride + token].  Pair i of a head, of
+ * `pairs` (2 * pairs <= head_dim; the rest of the head is left as it is), is
+ * elements (i, i + pairs), or (2i, 2i + 1) if interleaved.  It turns by the
+ * angle whose cosine and sine are table[position on axis axis_of[i]][i]:
+ * table [positions][pairs][2], device memory.  axis_of: host memory [pairs],
+ * or NULL for axis 0 throughout. */
+#define IVC_KV_MAX_PAIRS 128
+typedef struct ivc_rotary {
+  const float *table;
+  int64_t positions;
+  int pairs, axes, interleaved;
+  const int32_t *pos;
+  int64_t pos_stride;
+  const uint8_t *axis_of;
+} ivc_rotary;
+
+int ivc_kv_create(int device_ordinal, ivc_kv **out);
+void ivc_kv_destroy(ivc_kv *h);
+/* Message of the last failed call on `h`; with h == NULL, of the last failed ivc_kv_create. */
+const char *ivc_kv_last_error(const ivc_kv *h);
+/* Waits for `stream` and reports what the kernels found wrong. */
+int ivc_kv_synchronize(ivc_kv *h, void *stream);
+/* Allocates the stream's attention workspace (else its first ivc_kv_attend does). */
+int ivc_kv_reserve(ivc_kv *h, void *stream);
+
+/* Fills a rotary table: the angle of position p and pair i is p * inv_freq[i]
+ * (host memory [pairs]), computed in 64 bits and rounded once. */
+int ivc_kv_rope_table(ivc_kv *h, const double *inv_freq, int pairs, int64_t positions, float *table, void *stream);
+/* out = x with its pairs turned, in f32, rounded once; out may be x. */
+int ivc_kv_rope(ivc_kv *h, int dtype, int64_t tokens, int heads, int head_dim, const ivc_rows *x, const ivc_rows *out,
+                const ivc_rotary *rotary, void *stream);
+/* Appends keys (turned by `rotary`, unless NULL) and values to the cache, and
+ * turns q into q_out (q_heads 0: no queries) in the same launch.
+ * A block's exponent is the least e with |x| <= 127 * 2^e (in -120..121) over
+ * its new tokens; if the block already holds tokens of the sequence, their
+ * exponent if that is larger, and when e grows their codes c become
+ * round(c * 2^(old - e)), ties to even, as the new codes are round(x * 2^-e).
+ * So growth costs at most one rounding each time and the errors of all add up
+ * to less than one final step.  NaN is held as 0, an infinity as the largest
+ * code of its sign; neither takes part in e. */
+int ivc_kv_append(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int dtype, const ivc_rows *k,
+                  const ivc_rows *v, const ivc_rotary *rotary, int q_heads, const ivc_rows *q, const ivc_rows *q_out,
+                  void *stream);
+/* The cache's values of the sequences' tokens into k and v (either may be NULL). */
+int ivc_kv_read(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int dtype, const ivc_rows *k,
+                const ivc_rows *v, void *stream);
+/* out = softmax(scale * q k^T) v over the cache.  The query at position p sees
+ * the keys j <= p, with window > 0 only those with p - j < window or
+ * j < sinks.  q_heads is a multiple of kv_heads; query head h reads kv head
+ * h / (q_heads / kv_heads).  A row that sees nothing gives 0.  max_new: at
+ * least the largest number of new tokens of one sequence. */
+int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int dtype, int q_heads, int max_new,
+                  const ivc_rows *q, const ivc_rows *out, float scale, int window, int sinks, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -67,6 +67,16 @@ SIGNATURES = {
     "ivc_device_properties": (_i32, [_i32, _vp]),
     "ivc_f32_to_f16": (None, [_vp, _vp, _sz]),
     "ivc_f16_to_f32": (None, [_vp, _vp, _sz]),
+    "ivc_kv_create": (_i32, [_i32, _P(_vp)]),
+    "ivc_kv_destroy": (None, [_vp]),
+    "ivc_kv_last_error": (_cp, [_vp]),
+    "ivc_kv_synchronize": (_i32, [_vp, _vp]),
+    "ivc_kv_reserve": (_i32, [_vp, _vp]),
+    "ivc_kv_rope_table": (_i32, [_vp, _P(_f64), _i32, _i64, _vp, _vp]),
+    "ivc_kv_rope": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "ivc_kv_append": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "ivc_kv_read": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "ivc_kv_attend": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _i32, _i32, _vp]),
 }
 
 class Preprocess(ctypes.Structure):
@@ -74,6 +84,29 @@ class Preprocess(ctypes.Structure):
     _fields_ = [("letterbox", ctypes.c_int), ("to_rgb", ctypes.c_int), ("normalize", ctypes.c_int),
                 ("n_mean", ctypes.c_int), ("n_std", ctypes.c_int), ("mean", ctypes.c_float * 3),
                 ("std", ctypes.c_float * 3)]
+
+
+class Rows(ctypes.Structure):
+    """ivc_rows."""
+    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class KvCache(ctypes.Structure):
+    """ivc_kv_cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("page_size", _i32),
+                ("kv_heads", _i32), ("head_dim", _i32)]
+
+
+class KvSeqs(ctypes.Structure):
+    """ivc_kv_seqs."""
+    _fields_ = [("batch", _i32), ("tokens", _i64), ("offsets", _vp), ("at", _vp), ("pages", _vp),
+                ("pages_per_seq", _i32)]
+
+
+class Rotary(ctypes.Structure):
+    """ivc_rotary."""
+    _fields_ = [("table", _vp), ("positions", _i64), ("pairs", _i32), ("axes", _i32), ("interleaved", _i32),
+                ("pos", _vp), ("pos_stride", _i64), ("axis_of", _cp)]
 
 
 _lib = None

@@ -1,0 +1,412 @@
+// Rotary positions and the paged 8-bit key/value cache: the table, the rotation,
+// the append (rotation, block scales and codes in one pass) and the read.
+//
+// All four move bytes: a few operations for each element that is read and
+// written once.  Sixteen elements (eight pairs) of a row are a thread's share;
+// a warp reads whole 128-byte lines of the two halves of a head.
+#include <algorithm>
+
+#include "kv_common.cuh"
+
+namespace ivb {
+
+namespace {
+
+// cos and sin of the eight pairs 8g.. of `token`.
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ bool load_turn(const KvRotary &r, int g, long long token, Turn &t, int *status) {
+  bool ok = true;
+  if ((r.one_axis >> g) & 1u) {
+    long long p = r.pos[(long long)r.axis[8 * g] * r.pos_stride + token];
+    if (p < 0 || p >= r.positions) ok = false, p = 0;
+    const float4 *row = reinterpret_cast<const float4 *>(r.table + p * r.pairs + 8 * g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = __ldg(row + i);
+      t.c[2 * i] = v.x, t.s[2 * i] = v.y, t.c[2 * i + 1] = v.z, t.s[2 * i + 1] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      long long p = r.pos[(long long)r.axis[8 * g + i] * r.pos_stride + token];
+      if (p < 0 || p >= r.positions) ok = false, p = 0;
+      const float2 v = __ldg(r.table + p * r.pairs + 8 * g + i);
+      t.c[i] = v.x, t.s[i] = v.y;
+    }
+  }
+  if (!ok) kv_flag(status, kStatusKvPosition);
+  return ok;
+}
+
+// Where the two vectors of group g of a row begin: the halves of eight pairs
+// (side by side when they are interleaved), or sixteen elements behind the
+// rotated ones.
+__device__ __forceinline__ void group_at(int g, int pairs, int interleaved, int &a, int &b) {
+  if (8 * g < pairs && !interleaved) {
+    a = 8 * g;
+    b = pairs + 8 * g;
+  } else {
+    a = 16 * g;
+    b = 16 * g + 8;
+  }
+}
+
+// Turns eight pairs in place.  Products and sums are rounded one by one (no
+// fused multiply-add), so any IEEE evaluation of the formula gives the same
+// bits, and with them the same codes in the cache.
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const Turn &t, int interleaved) {
+  if (interleaved) {  // a: pairs 0..3, b: pairs 4..7, each (x, y) side by side
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float(&h)[8] = i < 4 ? a : b;
+      const int j = 2 * (i & 3);
+      const float x = h[j], y = h[j + 1];
+      h[j] = __fsub_rn(__fmul_rn(x, t.c[i]), __fmul_rn(y, t.s[i]));
+      h[j + 1] = __fadd_rn(__fmul_rn(y, t.c[i]), __fmul_rn(x, t.s[i]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = __fsub_rn(__fmul_rn(x, t.c[i]), __fmul_rn(y, t.s[i]));
+      b[i] = __fadd_rn(__fmul_rn(y, t.c[i]), __fmul_rn(x, t.s[i]));
+    }
+  }
+}
+
+__global__ void kv_rope_table_k(const __grid_constant__ KvRopeFreq f, int pairs, long long n, float2 *table) {
+  pdl_wait_and_release();
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const long long p = i / pairs;
+    double s, c;
+    sincos((double)p * f.inv[i - p * pairs], &s, &c);
+    table[i] = make_float2((float)c, (float)s);
+  }
+}
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeHeads = 4;  // heads a thread turns by the same angles at once
+
+// Turns the rows of token tile `tile`.  A token takes hs * (dim / 16) threads;
+// thread (head h0, group g) turns heads h0, h0 + hs, ...
+template <bool BF16>
+__device__ __forceinline__ void rope_tile(long long tile, long long tokens, int heads, int dim, int hs, int per_block,
+                                          const KvRows &x, const KvRows &out, const KvRotary &rot, int *status) {
+  const int groups = dim / 16, upt = hs * groups;
+  for (int u = threadIdx.x; u < upt * per_block; u += kRopeThreads) {
+    const int tl = u / upt, r = u - tl * upt, h0 = r / groups, g = r - h0 * groups;
+    const long long token = tile * per_block + tl;
+    if (token >= tokens) break;
+    const bool turned = 8 * g < rot.pairs;
+    int ea, eb;
+    group_at(g, rot.pairs, rot.interleaved, ea, eb);
+    Turn t;
+    if (turned && !load_turn(rot, g, token, t, status)) continue;
+    const uint16_t *xr = static_cast<const uint16_t *>(x.p) + token * x.ts;
+    uint16_t *yr = static_cast<uint16_t *>(out.p) + token * out.ts;
+    for (int h = h0; h < heads; h += kRopeHeads * hs) {
+      uint4 ua[kRopeHeads], ub[kRopeHeads];
+#pragma unroll
+      for (int i = 0; i < kRopeHeads; ++i)
+        if (h + i * hs < heads) {
+          ua[i] = load8(xr + (h + i * hs) * x.hs + ea, x.vec);
+          ub[i] = load8(xr + (h + i * hs) * x.hs + eb, x.vec);
+        }
+#pragma unroll
+      for (int i = 0; i < kRopeHeads; ++i)
+        if (h + i * hs < heads) {
+          if (turned) {
+            float a[8], b[8];
+            unpack8<BF16>(ua[i], a);
+            unpack8<BF16>(ub[i], b);
+            turn8(a, b, t, rot.interleaved);
+            ua[i] = pack8<BF16>(a);
+            ub[i] = pack8<BF16>(b);
+          }
+          store8(yr + (h + i * hs) * out.hs + ea, ua[i], out.vec);
+          store8(yr + (h + i * hs) * out.hs + eb, ub[i], out.vec);
+        }
+    }
+  }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kRopeThreads)
+    kv_rope_k(long long tokens, int heads, int dim, int hs, int per_block, const __grid_constant__ KvRows x,
+              const __grid_constant__ KvRows out, const __grid_constant__ KvRotary rot, int *status) {
+  pdl_wait_and_release();
+  rope_tile<BF16>(blockIdx.x, tokens, heads, dim, hs, per_block, x, out, rot, status);
+}
+
+// ---------------------------------------------------------------- append
+
+struct AppendArgs {
+  KvCache c;
+  KvSeqs s;
+  KvRows k, v, q, q_out;
+  KvRotary rot;
+  int q_heads, q_hs, q_per_block;
+  int window;             // packed tokens an append CTA looks at
+  int append_ctas;
+  int *status;
+};
+
+// The least e with m <= 127 * 2^e, m >= 0 finite: m = f * 2^x with f in [1, 2),
+// and 127 = 1.984375 * 2^6.
+__device__ __forceinline__ int scale_exponent(float m) {
+  const uint32_t u = __float_as_uint(m);
+  const int x = (int)(u >> 23) - 127;
+  const int e = x - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  return max(kKvMinExp, min(kKvMaxExp, e));  // (zero and subnormals: below the range)
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ int quantise(float x, float inv) {
+  // NaN becomes 0, infinities the largest code
+  return __float2int_rn(fminf(fmaxf(x == x ? x * inv : 0.f, -127.f), 127.f));
+}
+__device__ __forceinline__ uint2 quantise8(const float (&f)[8], float inv) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)quantise(f[i], inv) & 0xffu) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ uint32_t requantise4(uint32_t w, float ratio) {
+  uint32_t o = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = (int)(int8_t)(w >> (8 * i));
+    o |= ((uint32_t)__float2int_rn((float)c * ratio) & 0xffu) << (8 * i);
+  }
+  return o;
+}
+
+// One warp: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
+// tokens from t0) of one head, keys or values.  Lane (row l / groups, group
+// l % groups) holds sixteen elements of every (32 / groups)-th row.
+template <bool BF16, int DIM>
+__device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &x, bool turn, int8_t *codes,
+                                             float *scale_at, int head, int r0, int r1, long long t0) {
+  constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows;
+  const int lane = threadIdx.x & 31, g = lane % kGroups, rl = lane / kGroups;
+  const int pairs = turn ? a.rot.pairs : 0;
+  int ea, eb;
+  group_at(g, pairs, a.rot.interleaved, ea, eb);
+  float f[kSteps][2][8];
+  float most = 0.f;
+  const uint16_t *xh = static_cast<const uint16_t *>(x.p) + head * x.hs;
+  uint4 ua[kSteps], ub[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = i * kRows + rl;
+    ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
+    if (r >= r0 && r < r1) {
+      const uint16_t *row = xh + (t0 + r - r0) * x.ts;
+      ua[i] = load8(row + ea, x.vec);
+      ub[i] = load8(row + eb, x.vec);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = i * kRows + rl;
+    unpack8<BF16>(ua[i], f[i][0]);
+    unpack8<BF16>(ub[i], f[i][1]);
+    if (r >= r0 && r < r1 && 8 * g < pairs) {
+      Turn t;
+      if (load_turn(a.rot, g, t0 + r - r0, t, a.status)) turn8(f[i][0], f[i][1], t, a.rot.interleaved);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float m = fabsf(f[i][j >> 3][j & 7]);
+      most = fmaxf(most, m <= 3.402823466e38f ? m : 0.f);  // (a NaN compares false)
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  int e = scale_exponent(most);
+  if (r0 > 0) {  // tokens before: their codes follow the scale if it grows
+    const float before = *scale_at;
+    const int eo = max(kKvMinExp, min(kKvMaxExp, (int)((__float_as_uint(before) >> 23) & 0xffu) - 127));
+    if (e > eo) {
+      const float ratio = e - eo > 60 ? 0.f : exp2i(eo - e);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int r = i * kRows + rl;
+        if (r < r0) {
+          uint4 *p = reinterpret_cast<uint4 *>(codes + r * DIM + 16 * g);
+          const uint4 w = *p;
+          *p = make_uint4(requantise4(w.x, ratio), requantise4(w.y, ratio), requantise4(w.z, ratio),
+                          requantise4(w.w, ratio));
+        }
+      }
+    }
+    e = max(e, eo);
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale_at = exp2i(e);
+  const float inv = exp2i(-e);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = i * kRows + rl;
+    if (r >= r0 && r < r1) {
+      *reinterpret_cast<uint2 *>(codes + r * DIM + ea) = quantise8(f[i][0], inv);
+      *reinterpret_cast<uint2 *>(codes + r * DIM + eb) = quantise8(f[i][1], inv);
+    }
+  }
+}
+
+// CTA c of the first `append_ctas` takes the blocks whose first new token is
+// among packed tokens c * window .. + window - 1; its warps take (block, head,
+// keys or values) in turn.  A block is one warp's alone, so nothing is atomic
+// and the result does not depend on any order.  The other CTAs turn queries.
+template <bool BF16, int DIM>
+__global__ void __launch_bounds__(kRopeThreads) kv_append_k(const __grid_constant__ AppendArgs a) {
+  pdl_wait_and_release();
+  if ((int)blockIdx.x >= a.append_ctas) {
+    rope_tile<BF16>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs, a.q_per_block, a.q, a.q_out,
+                    a.rot, a.status);
+    return;
+  }
+  const long long first = (long long)blockIdx.x * a.window;
+  const int seq0 = kv_seq_of(a.s, first);
+  const int warp = threadIdx.x >> 5;
+  int task = warp;                // (block, head, half) tasks, this warp's next
+  int seq = seq0, base = 0;
+  const int per_block = 2 * a.c.heads;
+  for (int i = 0; i < a.window; ++i) {
+    const long long t = first + i;
+    if (t >= a.s.tokens) break;
+    while (seq < a.s.batch && a.s.offsets[seq + 1] <= t) ++seq;
+    if (seq >= a.s.batch) break;  // tokens behind the last sequence: not the call's
+    const long long o = a.s.offsets[seq], end = a.s.offsets[seq + 1];
+    const int start = a.s.at[seq];
+    if (t < o || o < 0 || start < 0) {
+      kv_flag(a.status, kStatusKvSeqs);
+      continue;
+    }
+    const long long pos = start + (t - o);
+    if (t != o && pos % kKvBlock != 0) continue;
+    // a block begins here
+    if (task < base + per_block && pos < 0x7fffffffLL) {
+      const int page = kv_page_of(a.c, a.s, seq, (int)pos, a.status);
+      if (page >= 0) {
+        const int r0 = (int)(pos % kKvBlock);
+        const int r1 = (int)min((long long)kKvBlock, r0 + min(end, a.s.tokens) - t);
+        const int slot = (int)pos % a.c.page - r0;
+        for (; task < base + per_block; task += kRopeThreads / 32) {
+          const int head = (task - base) >> 1;
+          const long long ca = kv_code_at(a.c, page, head, slot), sa = kv_scale_at(a.c, page, head, slot);
+          if ((task - base) & 1)
+            append_block<BF16, DIM>(a, a.v, false, a.c.v + ca, a.c.vs + sa, head, r0, r1, t);
+          else
+            append_block<BF16, DIM>(a, a.k, a.rot.table != nullptr, a.c.k + ca, a.c.ks + sa, head, r0, r1, t);
+        }
+      }
+    }
+    base += per_block;
+    while (task < base) task += kRopeThreads / 32;
+  }
+}
+
+// ---------------------------------------------------------------- read
+
+// Sixteen values a thread: a CTA takes `window` packed tokens, all heads.
+template <bool BF16, int DIM>
+__global__ void __launch_bounds__(256)
+    kv_read_k(const __grid_constant__ KvCache c, const __grid_constant__ KvSeqs s, const __grid_constant__ KvRows k,
+              const __grid_constant__ KvRows v, int window, int *status) {
+  pdl_wait_and_release();
+  constexpr int kGroups = DIM / 16;
+  const long long first = (long long)blockIdx.x * window;
+  int seq = kv_seq_of(s, first);
+  const int halves = (k.p ? 1 : 0) + (v.p ? 1 : 0);
+  for (int i = 0; i < window; ++i) {
+    const long long t = first + i;
+    if (t >= s.tokens) break;
+    while (seq < s.batch && s.offsets[seq + 1] <= t) ++seq;
+    if (seq >= s.batch) break;
+    const long long o = s.offsets[seq];
+    const long long pos = s.at[seq] + (t - o);
+    if (t < o || o < 0 || pos < 0 || pos >= 0x7fffffffLL) {
+      kv_flag(status, kStatusKvSeqs);
+      continue;
+    }
+    const int page = kv_page_of(c, s, seq, (int)pos, status);
+    if (page < 0) continue;
+    const int slot = (int)pos % c.page;
+    for (int u = threadIdx.x; u < halves * c.heads * kGroups; u += blockDim.x) {
+      const int g = u % kGroups, hh = u / kGroups, head = hh % c.heads;
+      const bool val = hh / c.heads == 1 || !k.p;
+      const KvRows &y = val ? v : k;
+      const long long ca = kv_code_at(c, page, head, slot) + 16 * g;
+      const float sc = (val ? c.vs : c.ks)[kv_scale_at(c, page, head, slot)];
+      const uint4 w = *reinterpret_cast<const uint4 *>((val ? c.v : c.k) + ca);
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+      uint16_t *row = static_cast<uint16_t *>(y.p) + t * y.ts + head * y.hs + 16 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(ws[2 * h + (j >> 2)] >> (8 * (j & 3))) * sc;
+        store8(row + 8 * h, pack8<BF16>(f), y.vec);
+      }
+    }
+  }
+}
+
+// Head groups of the rotation: one head a thread while that leaves SMs free,
+// kRopeHeads (angles loaded once for them) from there on.
+void rope_shape(long long tokens, int heads, int dim, int &hs, int &per_block) {
+  const int groups = dim / 16;
+  const bool many = tokens * heads * groups >= 148LL * 2048;
+  hs = many ? (heads + kRopeHeads - 1) / kRopeHeads : heads;
+  per_block = std::max(1, kRopeThreads / (hs * groups));
+}
+
+}  // namespace
+
+cudaError_t launch_kv_rope_table(const KvRopeFreq &f, int pairs, long long positions, float2 *table, cudaStream_t st) {
+  const long long n = positions * pairs;
+  const int grid = (int)std::min<long long>((n + 255) / 256, 148 * 8);
+  return launch_kernel(kv_rope_table_k, dim3(grid), dim3(256), 0, st, f, pairs, n, table);
+}
+
+cudaError_t launch_kv_rope(bool bf16, long long tokens, int heads, int dim, const KvRows &x, const KvRows &out,
+                           const KvRotary &rot, int *status, cudaStream_t st) {
+  int hs, per_block;
+  rope_shape(tokens, heads, dim, hs, per_block);
+  const dim3 grid((unsigned)((tokens + per_block - 1) / per_block));
+  return launch_kernel(bf16 ? kv_rope_k<true> : kv_rope_k<false>, grid, dim3(kRopeThreads), 0, st, tokens, heads, dim,
+                       hs, per_block, x, out, rot, status);
+}
+
+cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v,
+                             const KvRotary &rot, int q_heads, const KvRows &q, const KvRows &q_out, int *status,
+                             cudaStream_t st) {
+  AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, status};
+  // A CTA for each token while they are few (decode: each begins a block);
+  // sixteen for each CTA beyond that (a prompt begins a block every sixteen).
+  a.window = s.tokens <= 1024 ? 1 : kKvBlock;
+  a.append_ctas = (int)((s.tokens + a.window - 1) / a.window);
+  long long grid = a.append_ctas;
+  if (q_heads) {
+    rope_shape(s.tokens, q_heads, c.dim, a.q_hs, a.q_per_block);
+    grid += (s.tokens + a.q_per_block - 1) / a.q_per_block;
+  }
+  auto kern = c.dim == 64 ? (bf16 ? kv_append_k<true, 64> : kv_append_k<false, 64>)
+                          : (bf16 ? kv_append_k<true, 128> : kv_append_k<false, 128>);
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(kRopeThreads), 0, st, a);
+}
+
+cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v, int *status,
+                           cudaStream_t st) {
+  const int window = s.tokens <= 1024 ? 1 : 8;
+  const dim3 grid((unsigned)((s.tokens + window - 1) / window));
+  auto kern = c.dim == 64 ? (bf16 ? kv_read_k<true, 64> : kv_read_k<false, 64>)
+                          : (bf16 ? kv_read_k<true, 128> : kv_read_k<false, 128>);
+  return launch_kernel(kern, grid, dim3(256), 0, st, c, s, k, v, window, status);
+}
+
+}  // namespace ivb

@@ -1,0 +1,65 @@
+"""The language-model operators' descriptors and refusals that need no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import infvino_b200 as ivb
+from infvino_b200 import _native
+
+
+def tensors(pages=3, heads=2, page=32, dim=64):
+    codes = [torch.zeros((pages, heads, page, dim), dtype=torch.int8) for _ in range(2)]
+    return codes + [torch.zeros((pages, heads, page // 16)) for _ in range(2)]
+
+
+def test_cache_descriptor():
+    c = ivb.KvCache(*tensors())
+    assert (c.pages, c.kv_heads, c.page_size, c.head_dim) == (3, 2, 32, 64)
+    k, v, ks, vs = tensors()
+    for bad in ((k.float(), v, ks, vs), (k, v[:2], ks, vs), (k, v, ks[..., :1], vs), (k.transpose(2, 3), v, ks, vs), (k, v, ks.double(), vs)):
+        with pytest.raises(ValueError):
+            ivb.KvCache(*bad)
+
+
+def test_rotary_descriptor():
+    table = torch.zeros((10, 16, 2))
+    r = ivb.Rotary(table, [0] * 8 + [2] * 8)
+    assert r.axes == 3
+    c = r.at(torch.zeros((3, 5), dtype=torch.int32), 5)
+    assert c.axes == 3 and c.pos_stride == 5 and c.pairs == 16 and c.positions == 10
+    for pos in (torch.zeros((2, 5), dtype=torch.int32), torch.zeros(5, dtype=torch.int32), torch.zeros((3, 4), dtype=torch.int32),
+                torch.zeros((3, 5), dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            r.at(pos, 5)
+    with pytest.raises(ValueError):
+        ivb.Rotary(table, [0] * 15)
+    with pytest.raises(ValueError):
+        ivb.Rotary(table.double())
+
+
+def test_structs_match_the_header(tmp_path):
+    """The ctypes structures have the C compiler's sizes and offsets."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    pairs = [("ivc_rows", _native.Rows), ("ivc_kv_cache", _native.KvCache), ("ivc_kv_seqs", _native.KvSeqs), ("ivc_rotary", _native.Rotary)]
+    lines = []
+    for name, s in pairs:
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        lines += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in s._fields_]
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "infvino_b200.h"\nint main(void) {' + "".join(lines) + "return 0;}")
+    exe = str(tmp_path / "s")
+    subprocess.run(["gcc", str(src), "-I" + os.path.join(root, "include"), "-o", exe], check=True)
+    got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    want = [n for _, s in pairs for n in [ctypes.sizeof(s)] + [getattr(s, f[0]).offset for f in s._fields_]]
+    assert got == want
+
+
+def test_null_handles_are_refused():
+    L = _native.lib()
+    assert L.ivc_kv_create(0, None) == 1
+    assert L.ivc_kv_synchronize(None, None) == 1
+    assert L.ivc_kv_attend(None, None, None, 0, 1, 1, None, None, 1.0, 0, 0, None) == 1
+    L.ivc_kv_destroy(None)
