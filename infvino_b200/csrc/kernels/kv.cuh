@@ -63,6 +63,10 @@ cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const
                              cudaStream_t st);
 cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v, int *status,
                            cudaStream_t st);
-cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, cudaStream_t st);
+// The workspace of a stream's attention calls: counters (zeroed once, they
+// return to zero by themselves), then partial results.
+constexpr size_t kKvCounterBytes = 1 << 14;
+size_t kv_workspace_bytes(int sms);
+cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
 
 }  // namespace ivb

@@ -12,7 +12,7 @@
 #include "kernels/kv.cuh"
 
 struct ivc_kv {
-  int device = 0;
+  int device = 0, sms = 0;
   std::mutex mu;
   std::string err;
   int *status = nullptr;
@@ -81,6 +81,26 @@ int guarded(ivc_kv *h, const char *call, F &&f) {
   } catch (...) {
   }
   return code;
+}
+
+// The stream's attention workspace, allocated and zeroed (in the stream's order) at its first use.
+void *workspace(ivc_kv *h, cudaStream_t st) {
+  const auto it = h->workspace.find(st);
+  if (it != h->workspace.end()) return it->second;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cuda(cudaStreamIsCapturing(st, &cap), "stream");
+  need(cap == cudaStreamCaptureStatusNone, "a stream's first call cannot be captured: call ivc_kv_reserve before");
+  const size_t bytes = ivb::kv_workspace_bytes(h->sms);
+  void *p = nullptr;
+  cuda(cudaMalloc(&p, bytes), "workspace");
+  try {
+    cuda(cudaMemsetAsync(p, 0, ivb::kKvCounterBytes, st), "workspace");
+    h->workspace[st] = p;
+  } catch (...) {
+    (void)cudaFree(p);
+    throw;
+  }
+  return p;
 }
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -174,6 +194,7 @@ int ivc_kv_create(int device_ordinal, ivc_kv **out) {
     need(major == 10, "the kernels are built for sm_100a");
     h = new ivc_kv;
     h->device = device_ordinal;
+    cuda(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device_ordinal), "device attribute");
     Scope scope(device_ordinal);
     cuda(cudaMalloc(&h->status, sizeof(int)), "status word");
     cuda(cudaMemset(h->status, 0, sizeof(int)), "status word");
@@ -236,7 +257,7 @@ int ivc_kv_synchronize(ivc_kv *h, void *stream) {
 }
 
 int ivc_kv_reserve(ivc_kv *h, void *stream) {
-  return guarded(h, "ivc_kv_reserve", [&] { (void)stream; });
+  return guarded(h, "ivc_kv_reserve", [&] { workspace(h, static_cast<cudaStream_t>(stream)); });
 }
 
 int ivc_kv_rope_table(ivc_kv *h, const double *inv_freq, int pairs, int64_t positions, float *table, void *stream) {
@@ -327,7 +348,8 @@ int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
     a.sinks = sinks;
     a.status = h->status;
     if (a.seqs.tokens == 0) return;
-    cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, static_cast<cudaStream_t>(stream)), "launch");
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
   });
 }
 
