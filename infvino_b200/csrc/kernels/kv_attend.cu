@@ -6,7 +6,7 @@
 // in one pass with a running maximum m.  A decode step reads every visible
 // code once and does a few operations for each, so the cache's bytes bound it.
 //
-// An item is a tile of 16 query rows (token, head of the group) of one
+// An item is a tile of 8, 16 or 32 query rows (token, head of the group) of one
 // sequence and kv head; its units are the key blocks (16 keys that share a
 // scale).  All units of the launch are divided evenly over the CTAs, whatever
 // the sequences' lengths: a CTA's share is the rest of one item, some whole
@@ -17,11 +17,16 @@
 //
 // A warp takes whole blocks: it copies 16 rows of key and value codes to its
 // ring in shared memory (cp.async, swizzled so that the reads below do not
-// conflict), and multiplies with m16n8k16 tensor instructions: codes become
-// halves exactly (1024 + code + 128 by a byte permutation, minus 1152), the
-// order of head elements and keys inside the products is chosen so that every
-// lane reads whole 16-byte (64-wide heads: 8-byte) pieces of a row and the
-// scores leave one product in the registers that the next one wants.
+// conflict), and multiplies with m16n8k16 tensor instructions, transposed
+// (keys, then head elements, are the 16 rows; queries the 8 columns), so that
+// a handful of queries fills an instruction and a code is converted once for
+// all of them.  Codes become halves exactly (1024 + code + 128 by a byte
+// permutation, minus 1152).  The order of head elements and keys inside the
+// products is chosen so that every lane reads whole 16-byte (64-wide heads:
+// 8-byte) pieces of a row; the weights turn into the second product's operand
+// by transposing 8 x 8 pieces in registers.
+#include <algorithm>
+
 #include "kv_attend.cuh"
 
 namespace ivb {
@@ -29,10 +34,11 @@ namespace ivb {
 namespace {
 
 constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps;
-constexpr int kStepRows = 16;
-constexpr int kStepStages = 4;
-constexpr int kStepCtasPerSm = 3;
-constexpr int kStepMinBlocks = kStepWarps;  // of a CTA's share: a block for each warp
+constexpr int kStepStages = 4;  // blocks of a warp's ring; two are worked on at once
+constexpr int kStepMinBlocks = 2 * kStepWarps;  // of a CTA's share: two blocks for each warp
+// A row's maximum follows its scores only when one is kStepSlack above it: the
+// sums are rescaled rarely, and weights stay below 2^(kStepBits + kStepSlack).
+constexpr float kStepSlack = 4.f, kStepBits = kWeightBits - kStepSlack;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -50,6 +56,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of halves, a row's two halves a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // Two codes (+ 128, in bytes LO, LO + 1 of w) as halves.
@@ -72,33 +85,36 @@ __device__ __forceinline__ uint32_t tile_swizzle(uint32_t o) {
   return o ^ (f << 4);
 }
 
-template <int DIM>
+template <int DIM, int NT>
 struct StepSlot {  // partial sums of a cut item: accumulators lane by lane, then per row maximum and sum
-  float acc[DIM / 2 * 32];
-  float m[kStepRows], l[kStepRows];
+  float acc[NT * DIM / 4 * 32];
+  float m[8 * NT], l[8 * NT];
   float vref;
   float pad[31];
 };
 
-template <int DIM>
+template <int DIM, int NT>
 struct StepShared {
   alignas(128) uint8_t ring[kStepWarps][kStepStages][2][kKvBlock * DIM];
   float2 scales[kStepWarps][kStepStages];
-  float m[kStepWarps][kStepRows], l[kStepWarps][kStepRows], vref[kStepWarps];
+  float m[kStepWarps][8 * NT], l[kStepWarps][8 * NT], vref[kStepWarps];
   long long scan[kStepWarps];
-  long long total, base;
+  long long base;
   int seq;
   int last;
 };
 
-template <bool BF16, int DIM>
-__global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
-    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM> *slots, unsigned *counters) {
+// NT: 8-row tiles of queries that share the codes of an item.
+template <bool BF16, int DIM, int NT>
+__global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
+    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters) {
   extern __shared__ uint8_t smem_raw[];
-  StepShared<DIM> &sh = *reinterpret_cast<StepShared<DIM> *>(smem_raw);
-  constexpr int kAcc = DIM / 2;         // accumulators a lane (16 x DIM over 32 lanes)
-  constexpr int kTiles = DIM / 8;       // 8-wide column tiles of the output
-  constexpr int kSteps = DIM / 16;      // 16-deep steps of the score product
+  StepShared<DIM, NT> &sh = *reinterpret_cast<StepShared<DIM, NT> *>(smem_raw);
+  constexpr int kRows = 8 * NT;
+  constexpr int kTiles = DIM / 16;      // 16-row tiles of head elements (output), 16-deep steps (scores)
+  constexpr int kPiece = DIM / 8;       // head elements of a lane's piece
+  constexpr int kAcc = NT * DIM / 4;    // accumulators a lane
+  constexpr int kTile = kKvBlock * DIM;  // bytes of a block's keys or values
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait_and_release();
 
@@ -108,7 +124,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
   for (int b = b_lo; b < b_hi; ++b) {
     const KvSpan s = kv_span(a, b);
-    mine += (long long)s.blocks * ((s.n * a.group + kStepRows - 1) / kStepRows) * a.cache.heads;
+    mine += (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
   }
   long long incl = mine;
 #pragma unroll
@@ -136,7 +152,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
     int b = b_lo;
     for (;; ++b) {
       const KvSpan s = kv_span(a, b);
-      const long long w = (long long)s.blocks * ((s.n * a.group + kStepRows - 1) / kStepRows) * a.cache.heads;
+      const long long w = (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
       if (u < at + w) break;
       at += w;
     }
@@ -147,11 +163,17 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
   int b = sh.seq;
   long long base = sh.base;  // first unit of sequence b
 
-  const float qscale = a.scale * kLog2e;
+  // ---- this lane's places in a tile of codes
+  const uint32_t ring = smem_u32(&sh.ring[warp][0][0][0]);
+  const uint32_t put0 = tile_swizzle<DIM>((uint32_t)lane * 16u), put1 = tile_swizzle<DIM>(512u + (uint32_t)lane * 16u);
+  const uint32_t key_at = tile_swizzle<DIM>((uint32_t)(g * DIM + 16 * t4));  // row g, its second half: ^ 64
+  const uint32_t val_at0 = tile_swizzle<DIM>((uint32_t)(2 * t4 * DIM + g * kPiece)),
+                 val_at1 = tile_swizzle<DIM>((uint32_t)((2 * t4 + 1) * DIM + g * kPiece));
+
   while (u < u_end) {
     // ---- the segment: blocks k0 .. k1 - 1 of item (b, head, row tile)
     const KvSpan s = kv_span(a, b);
-    const int row_tiles = (s.n * a.group + kStepRows - 1) / kStepRows;
+    const int row_tiles = (s.n * a.group + kRows - 1) / kRows;
     const long long units = (long long)s.blocks * row_tiles * a.cache.heads;
     if (u >= base + units) {
       base += units;
@@ -163,199 +185,223 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
     const long long item_begin = base + item * s.blocks, item_end = item_begin + s.blocks;
     const int k0 = (int)(u - item_begin), k1 = (int)(min(u_end, item_end) - item_begin);
 
-    // ---- this lane's rows g and g + 8: positions and queries
-    int pos[2];
-    float rs[2];
-    uint32_t q[kSteps][4];
+    // ---- blocks k0 + warp, + kStepWarps, ...; lane i knows the i-th of the next 32
+    const int count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
+    const int first_block = k0 + warp;
+    long long where = -1;  // this lane's block's codes, -1: none
+    float2 sc_mine = make_float2(0.f, -1.f);
+    int looked = 0;
+    // A block is looked up 32 at a time and copied kStepStages ahead of the
+    // products; its scales wait beside its codes (a value scale below 0:
+    // nothing to see).
+    auto fetch = [&](int it) {
+      if (it < count) {
+        if (it == looked) {
+          looked += 32;
+          where = -1;
+          sc_mine = make_float2(0.f, -1.f);
+          if (it + lane < count) {
+            const int key = s.block(first_block + (it + lane) * kStepWarps) * kKvBlock;
+            if (key < s.len) {
+              const int page = kv_page_of(a.cache, a.seqs, b, key, a.status);
+              if (page >= 0) {
+                const int slot = key % a.cache.page;
+                where = kv_code_at(a.cache, page, head, slot);
+                const long long sa = kv_scale_at(a.cache, page, head, slot);
+                sc_mine = make_float2(a.cache.ks[sa], a.cache.vs[sa]);
+              }
+            }
+          }
+        }
+        const long long from = __shfl_sync(0xffffffffu, where, it & 31);
+        if (lane == (it & 31)) sh.scales[warp][it % kStepStages] = sc_mine;
+        if (from >= 0) {
+          const uint32_t dst = ring + (uint32_t)(it % kStepStages) * (2u * kTile);
+          const int8_t *kp = a.cache.k + from + lane * 16, *vp = a.cache.v + from + lane * 16;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = rt * kStepRows + g + 8 * h, i = r / a.group;
-      pos[h] = i < s.n ? s.len - s.n + i : -1;
+          for (int i = 0; i < kTile / 512; ++i)
+            cp_async16(dst + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), kp + i * 512);
+#pragma unroll
+          for (int i = 0; i < kTile / 512; ++i)
+            cp_async16(dst + kTile + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), vp + i * 512);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStepStages; ++i) fetch(i);
+
+    // ---- queries: column g of tile t for the products, columns 2 t4, + 1 for the scores
+    uint32_t q[NT][kTiles][2];
+    int pos[NT][2];
+    float rs[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = rt * kRows + 8 * t + g, i = r / a.group;
       const uint16_t *row = static_cast<const uint16_t *>(a.q.p) + (long long)(s.first + i) * a.q.ts +
                             (long long)(head * a.group + r - i * a.group) * a.q.hs;
-      uint32_t w[2 * kSteps];
+      uint32_t w[2 * kTiles];
 #pragma unroll
       for (int c = 0; c < DIM / 64; ++c) {
-        const uint4 x = pos[h] >= 0 ? load8(row + 64 * c + 16 * t4, a.q.vec) : make_uint4(0, 0, 0, 0);
-        const uint4 y = pos[h] >= 0 ? load8(row + 64 * c + 16 * t4 + 8, a.q.vec) : make_uint4(0, 0, 0, 0);
+        const uint4 x = i < s.n ? load8(row + 64 * c + 16 * t4, a.q.vec) : make_uint4(0, 0, 0, 0);
+        const uint4 y = i < s.n ? load8(row + 64 * c + 16 * t4 + 8, a.q.vec) : make_uint4(0, 0, 0, 0);
         w[8 * c] = x.x, w[8 * c + 1] = x.y, w[8 * c + 2] = x.z, w[8 * c + 3] = x.w;
         w[8 * c + 4] = y.x, w[8 * c + 5] = y.y, w[8 * c + 6] = y.z, w[8 * c + 7] = y.w;
       }
-      rs[h] = qscale;
+      float up = a.scale * kLog2e;
       if (BF16) {
         // bf16 queries become halves: the row is scaled by a power of two so
         // that its largest element lies in 2^0 .. 2^1 (its eight bits stay)
         float most = 0.f;
 #pragma unroll
-        for (int i2 = 0; i2 < 2 * kSteps; ++i2) {
-          const float2 f = unpack2<true>(w[i2]);
+        for (int k = 0; k < 2 * kTiles; ++k) {
+          const float2 f = unpack2<true>(w[k]);
           most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
         const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        rs[h] *= __uint_as_float((uint32_t)e << 23);
+        up *= __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-        for (int i2 = 0; i2 < 2 * kSteps; ++i2) {
-          const float2 f = unpack2<true>(w[i2]);
-          w[i2] = pack2<false>(f.x * down, f.y * down);
+        for (int k = 0; k < 2 * kTiles; ++k) {
+          const float2 f = unpack2<true>(w[k]);
+          w[k] = pack2<false>(f.x * down, f.y * down);
         }
       }
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        q[k][h] = w[2 * k];
-        q[k][2 + h] = w[2 * k + 1];
+      for (int k = 0; k < kTiles; ++k) q[t][k][0] = w[2 * k], q[t][k][1] = w[2 * k + 1];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int rc = rt * kRows + 8 * t + 2 * t4 + c, ic = rc / a.group;
+        pos[t][c] = ic < s.n ? s.len - s.n + ic : -1;
+        rs[t][c] = BF16 ? __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4) : up;  // (lane of column 2 t4 + c)
       }
     }
-    const int p_lo = s.len - s.n + rt * kStepRows / a.group;                              // first row's position
-    const int p_hi = s.len - s.n + min(s.n - 1, (rt * kStepRows + kStepRows - 1) / a.group);  // last row's
+    const int p_lo = s.len - s.n + rt * kRows / a.group;                                  // first row's position
+    const int p_hi = s.len - s.n + min(s.n - 1, (rt * kRows + kRows - 1) / a.group);      // last row's
 
-    float acc[kTiles][4];
+    float acc[NT][kTiles][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.f;
+    }
     float vref = 0.f, vinv = 0.f;  // acc is in units of vref, the largest value scale so far
 
-    // ---- blocks k0 + warp, + kStepWarps, ...; lane i knows the i-th of the next 32
-    const int count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
-    const uint32_t ring = smem_u32(&sh.ring[warp][0][0][0]);
-    long long where = -1;  // this lane's block's codes, -1: none
-    float ksc = 0.f, vsc = 0.f;
-    int looked = 0;
-    auto look_up = [&](int it) {  // for iterations it .. it + 31
-      where = -1;
-      ksc = vsc = 0.f;
-      if (it + lane < count) {
-        const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
-        if (key < s.len) {
-          const int page = kv_page_of(a.cache, a.seqs, b, key, a.status);
-          if (page >= 0) {
-            const int slot = key % a.cache.page;
-            where = kv_code_at(a.cache, page, head, slot);
-            const long long sa = kv_scale_at(a.cache, page, head, slot);
-            ksc = a.cache.ks[sa];
-            vsc = a.cache.vs[sa];
-          }
-        }
-      }
-    };
-    auto copy = [&](int it, long long from) {
-      if (from >= 0) {
-        const uint32_t dst = ring + (uint32_t)(it % kStepStages) * (2u * kKvBlock * DIM);
-#pragma unroll
-        for (int i = 0; i < kKvBlock * DIM / 512; ++i) {
-          const uint32_t o = (uint32_t)(i * 32 + lane) * 16u;
-          cp_async16(dst + tile_swizzle<DIM>(o), a.cache.k + from + o);
-        }
-#pragma unroll
-        for (int i = 0; i < kKvBlock * DIM / 512; ++i) {
-          const uint32_t o = (uint32_t)(i * 32 + lane) * 16u;
-          cp_async16(dst + kKvBlock * DIM + tile_swizzle<DIM>(o), a.cache.v + from + o);
-        }
-      }
-      cp_async_commit();
-    };
-    // the look-up runs kStepStages - 1 blocks ahead of the products: a block's
-    // scales wait beside its codes (a value scale below 0: nothing to see)
-    auto fetch = [&](int it) {
-      long long from = -1;
-      if (it < count) {
-        if (it == looked) {
-          look_up(it);
-          looked += 32;
-        }
-        from = __shfl_sync(0xffffffffu, where, it & 31);
-        if (lane == (it & 31)) sh.scales[warp][it % kStepStages] = make_float2(ksc, where >= 0 ? vsc : -1.f);
-      }
-      copy(it, from);
-    };
-#pragma unroll
-    for (int i = 0; i < kStepStages - 1; ++i) fetch(i);
-    for (int it = 0; it < count; ++it) {
+    for (int it = 0; it < count; it += 2) {
       cp_async_wait<kStepStages - 2>();
       __syncwarp();
-      const int st = it % kStepStages;
-      const float2 scales = sh.scales[warp][st];
-      const float bk = scales.x, bv = scales.y;
-      if (bv >= 0.f) {
-        const uint8_t *kt = sh.ring[warp][st][0], *vt = sh.ring[warp][st][1];
-        // scores of keys 8j + 2 t4, + 1 (j = 0, 1) for rows g, g + 8
-        float sc[2][4];
+      const int st = it % kStepStages;  // (even: the pair is st, st + 1)
+      const bool two = it + 1 < count;
+      // scores of keys g, g + 8 of both blocks
+      float sc[2][NT][4];
+      float vs[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      for (int z = 0; z < 2; ++z) {
+        const float2 scales = sh.scales[warp][st + z];
+        vs[z] = z == 0 || two ? scales.y : -1.f;
+        if (vs[z] < 0.f) {
 #pragma unroll
-          for (int c = 0; c < DIM / 64; ++c) {
-            const uint4 w4 =
-                *reinterpret_cast<const uint4 *>(kt + tile_swizzle<DIM>((uint32_t)((8 * j + g) * DIM + 64 * c + 16 * t4)));
-            const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+          for (int t = 0; t < NT; ++t) sc[z][t][0] = sc[z][t][1] = sc[z][t][2] = sc[z][t][3] = -INFINITY;
+          continue;
+        }
+        const uint8_t *kt = sh.ring[warp][st + z][0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = 4 * c + i;
-              mma16816(sc[j], q[k][0], q[k][1], q[k][2], q[k][3], codes2<0x4140>(w[i]), codes2<0x4342>(w[i]));
-            }
+        for (int t = 0; t < NT; ++t) sc[z][t][0] = sc[z][t][1] = sc[z][t][2] = sc[z][t][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DIM / 64; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(kt + (key_at ^ (64u * c)));
+          const uint4 y = *reinterpret_cast<const uint4 *>(kt + (key_at ^ (64u * c)) + 8 * DIM);
+          const uint32_t xw[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+          const uint32_t yw[4] = {y.x ^ 0x80808080u, y.y ^ 0x80808080u, y.z ^ 0x80808080u, y.w ^ 0x80808080u};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a0 = codes2<0x4140>(xw[i]), a1 = codes2<0x4140>(yw[i]), a2 = codes2<0x4342>(xw[i]),
+                           a3 = codes2<0x4342>(yw[i]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma16816(sc[z][t], a0, a1, a2, a3, q[t][4 * c + i][0], q[t][4 * c + i][1]);
           }
         }
-        const int key0 = s.block(k0 + warp + it * kStepWarps) * kKvBlock;
-        const bool masked = key0 + kKvBlock - 1 > p_lo ||
-                            (a.window > 0 && p_hi - key0 >= a.window && key0 + kKvBlock > a.sinks);
-        float mx[2] = {m[0], m[1]};
+        const int key0 = s.block(first_block + (it + z) * kStepWarps) * kKvBlock;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int h = e >> 1;
-            float x = sc[j][e] * (rs[h] * bk);
-            if (masked && !kv_sees(a, pos[h], key0 + 8 * j + 2 * t4 + (e & 1))) x = -INFINITY;
-            sc[j][e] = x;
-            mx[h] = fmaxf(mx[h], x);
-          }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        for (int t = 0; t < NT; ++t) {
+          const float f0 = rs[t][0] * scales.x, f1 = rs[t][1] * scales.x;
+          sc[z][t][0] *= f0, sc[z][t][1] *= f1, sc[z][t][2] *= f0, sc[z][t][3] *= f1;
         }
-        const float vnew = fmaxf(vref, bv);
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1]) || vnew > vref) {
-          const float vr = vref > 0.f ? __fdividef(vref, vnew) : 0.f;
+        if (key0 + kKvBlock - 1 > p_lo || (a.window > 0 && p_hi - key0 >= a.window && key0 + kKvBlock > a.sinks)) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float f = mx[h] > m[h] ? fast_exp2(m[h] - mx[h]) : 1.f;
-            l[h] *= f;
-            m[h] = mx[h];
-            const float fo = f * vr;
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!kv_sees(a, pos[t][e & 1], key0 + g + 8 * (e >> 1))) sc[z][t][e] = -INFINITY;
+        }
+      }
+      // the rows' maxima, where a score is well above them, and the value scale
+      float mx[NT][2];
+      bool above = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          mx[t][c] = fmaxf(fmaxf(sc[0][t][c], sc[0][t][c + 2]), fmaxf(sc[1][t][c], sc[1][t][c + 2]));
+          above = above || mx[t][c] > m[t][c] + kStepSlack;
+        }
+      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[1]));
+      if (__any_sync(0xffffffffu, above) || vnew > vref) {
+        const float vr = vref > 0.f ? __fdividef(vref, vnew) : 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = fmaxf(m[t][c], mx[t][c]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const float f = x > m[t][c] ? fast_exp2(m[t][c] - x) : 1.f;
+            l[t][c] *= f;
+            m[t][c] = x;
 #pragma unroll
             for (int j = 0; j < kTiles; ++j) {
-              acc[j][2 * h] *= fo;
-              acc[j][2 * h + 1] *= fo;
+              acc[t][j][c] *= f * vr;
+              acc[t][j][c + 2] *= f * vr;
             }
           }
-          vref = vnew;
-          vinv = vref > 0.f ? 1.f / vref : 0.f;
-        }
-        const float bf = bv * vinv;
-        uint32_t p[4];
+        vref = vnew;
+        vinv = vref > 0.f ? 1.f / vref : 0.f;
+      }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float base_m = m[h] == -INFINITY ? 0.f : m[h] - kWeightBits;
+      for (int z = 0; z < 2; ++z) {
+        if (vs[z] < 0.f) continue;
+        const float vf = vs[z] * vinv;
+        uint32_t p[NT][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float x = fast_exp2(sc[j][2 * h] - base_m), y = fast_exp2(sc[j][2 * h + 1] - base_m);
-            l[h] += x + y;
-            p[2 * j + h] = pack2<false>(x * bf, y * bf);  // rounded to 11 bits; summed in 32
+        for (int t = 0; t < NT; ++t) {
+          float w[4];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float shift = m[t][c] == -INFINITY ? 0.f : m[t][c] - kStepBits;
+            w[c] = fast_exp2(sc[z][t][c] - shift);
+            w[c + 2] = fast_exp2(sc[z][t][c + 2] - shift);
+            l[t][c] += w[c] + w[c + 2];
           }
+          // rounded to 11 bits; summed in 32
+          p[t][0] = transpose8x8(pack2<false>(w[0] * vf, w[1] * vf));
+          p[t][1] = transpose8x8(pack2<false>(w[2] * vf, w[3] * vf));
         }
-        // values: keys 2 t4, + 1, + 8, + 9; column tile j is byte j of the lane's piece of a row
+        // values of keys 2 t4, + 1, + 8, + 9; rows g, g + 8 of tile j are bytes 2j, 2j + 1 of the lane's piece
+        const uint8_t *vt = sh.ring[warp][st + z][1];
         uint32_t vw[4][DIM / 32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t o = (uint32_t)((8 * (i >> 1) + 2 * t4 + (i & 1)) * DIM + g * (DIM / 8));
+          const uint8_t *at = vt + (i & 1 ? val_at1 : val_at0) + (i >> 1) * 8 * DIM;
           if (DIM == 128) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(vt + tile_swizzle<DIM>(o));
+            const uint4 x = *reinterpret_cast<const uint4 *>(at);
             vw[i][0] = x.x, vw[i][1] = x.y, vw[i][DIM / 32 - 2] = x.z, vw[i][DIM / 32 - 1] = x.w;
           } else {
-            const uint2 x = *reinterpret_cast<const uint2 *>(vt + tile_swizzle<DIM>(o));
+            const uint2 x = *reinterpret_cast<const uint2 *>(at);
             vw[i][0] = x.x, vw[i][1] = x.y;
           }
         }
@@ -363,50 +409,60 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
         for (int w = 0; w < DIM / 32; ++w) {
           const uint32_t x0 = vw[0][w] ^ 0x80808080u, x1 = vw[1][w] ^ 0x80808080u, x2 = vw[2][w] ^ 0x80808080u,
                          x3 = vw[3][w] ^ 0x80808080u;
-          const uint32_t a0 = __byte_perm(x0, x1, 0x5140), a1 = __byte_perm(x0, x1, 0x7362);
-          const uint32_t c0 = __byte_perm(x2, x3, 0x5140), c1 = __byte_perm(x2, x3, 0x7362);
-          mma16816(acc[4 * w], p[0], p[1], p[2], p[3], codes2<0x4140>(a0), codes2<0x4140>(c0));
-          mma16816(acc[4 * w + 1], p[0], p[1], p[2], p[3], codes2<0x4342>(a0), codes2<0x4342>(c0));
-          mma16816(acc[4 * w + 2], p[0], p[1], p[2], p[3], codes2<0x4140>(a1), codes2<0x4140>(c1));
-          mma16816(acc[4 * w + 3], p[0], p[1], p[2], p[3], codes2<0x4342>(a1), codes2<0x4342>(c1));
+          const uint32_t lo = __byte_perm(x0, x1, 0x5140), hi = __byte_perm(x0, x1, 0x7362);
+          const uint32_t lo8 = __byte_perm(x2, x3, 0x5140), hi8 = __byte_perm(x2, x3, 0x7362);
+          const uint32_t a0 = codes2<0x4140>(lo), a1 = codes2<0x4342>(lo), a2 = codes2<0x4140>(lo8),
+                         a3 = codes2<0x4342>(lo8);
+          const uint32_t b0 = codes2<0x4140>(hi), b1 = codes2<0x4342>(hi), b2 = codes2<0x4140>(hi8),
+                         b3 = codes2<0x4342>(hi8);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma16816(acc[t][2 * w], a0, a1, a2, a3, p[t][0], p[t][1]);
+            mma16816(acc[t][2 * w + 1], b0, b1, b2, b3, p[t][0], p[t][1]);
+          }
         }
       }
-      __syncwarp();  // the slot that the next copy overwrites has been read
-      fetch(it + kStepStages - 1);
+      __syncwarp();  // the pair's places have been read
+      fetch(it + kStepStages);
+      fetch(it + kStepStages + 1);
     }
     cp_async_wait<0>();
 
     // ---- join the warps: row maxima, then sums in a common scale
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (t4 == 0) {
-        sh.m[warp][g + 8 * h] = m[h];
-        sh.l[warp][g + 8 * h] = l[h];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[t][c] += __shfl_xor_sync(0xffffffffu, l[t][c], o);
+        if (g == 0) {
+          sh.m[warp][8 * t + 2 * t4 + c] = m[t][c];
+          sh.l[warp][8 * t + 2 * t4 + c] = l[t][c];
+        }
       }
-    }
     if (lane == 0) sh.vref[warp] = vref;
     __syncthreads();
-    float all_m[2], all_v = 0.f, f[2];
+    float all_v = 0.f;
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w) all_v = fmaxf(all_v, sh.vref[w]);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      all_m[h] = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) all_m[h] = fmaxf(all_m[h], sh.m[w][g + 8 * h]);
-      f[h] = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - all_m[h]) * (all_v > 0.f ? __fdividef(vref, all_v) : 0.f);
-    }
-    // accumulators lane by lane: [row half][column half][tile], so that eight
-    // neighbours of a lane are eight neighbouring outputs
+    // accumulators lane by lane, [row tile][row of two][head element of the
+    // piece]: eight neighbours of a lane are eight neighbouring outputs
     float *part = reinterpret_cast<float *>(&sh.ring[warp][0][0][0]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) part[((2 * h + c) * kTiles + j) * 32 + lane] = acc[j][2 * h + c] * f[h];
+        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][8 * t + 2 * t4 + c]);
+        const float f = m[t][c] == -INFINITY
+                            ? 0.f
+                            : fast_exp2(m[t][c] - top) * (all_v > 0.f ? __fdividef(vref, all_v) : 0.f);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) part[((2 * t + c) * kPiece + 2 * j + h) * 32 + lane] = acc[t][j][2 * h + c] * f;
+      }
     __syncthreads();
     const bool whole = k0 == 0 && k1 == s.blocks;
     const int first_cta = share_of(total, ctas, item_begin), last_cta = share_of(total, ctas, item_end - 1);
@@ -418,13 +474,13 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
         for (int w = 0; w < kStepWarps; ++w) x += reinterpret_cast<const float *>(&sh.ring[w][0][0][0])[e];
         __stcg(&slots[slot].acc[e], x);
       }
-      if (threadIdx.x < kStepRows) {
+      if (threadIdx.x < kRows) {
         const int r = threadIdx.x;
-        float am = -INFINITY, x = 0.f;
-        for (int w = 0; w < kStepWarps; ++w) am = fmaxf(am, sh.m[w][r]);
+        float top = -INFINITY, x = 0.f;
+        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]);
         for (int w = 0; w < kStepWarps; ++w)
-          if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) x += sh.l[w][r] * fast_exp2(sh.m[w][r] - am);
-        __stcg(&slots[slot].m[r], am);
+          if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) x += sh.l[w][r] * fast_exp2(sh.m[w][r] - top);
+        __stcg(&slots[slot].m[r], top);
         __stcg(&slots[slot].l[r], x);
         if (r == 0) __stcg(&slots[slot].vref, all_v);
       }
@@ -443,8 +499,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
       // eight neighbouring outputs a thread
       for (int e = threadIdx.x; e < kAcc / 8 * 32; e += kStepThreads) {
         const int ln = e & 31, i0 = (e >> 5) * 8;  // accumulators i0 .. i0 + 7 of lane ln
-        const int h = i0 / (2 * kTiles), c = i0 / kTiles % 2, j0 = i0 % kTiles;
-        const int r = (ln >> 2) + 8 * h;
+        const int rc = i0 / kPiece, d0 = i0 % kPiece;
+        const int r = 8 * (rc >> 1) + 2 * (ln & 3) + (rc & 1);
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f, top = -INFINITY, vr = 0.f;
         if (whole) {
           for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]);
@@ -457,12 +513,12 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
           }
         } else {
           for (int z = first_cta; z <= last_cta; ++z) {
-            const StepSlot<DIM> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
+            const StepSlot<DIM, NT> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
             top = fmaxf(top, __ldcg(&sl.m[r]));
             vr = fmaxf(vr, __ldcg(&sl.vref));
           }
           for (int z = first_cta; z <= last_cta; ++z) {
-            const StepSlot<DIM> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
+            const StepSlot<DIM, NT> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
             const float zm = __ldcg(&sl.m[r]), zl = __ldcg(&sl.l[r]);
             if (zm == -INFINITY && zl == 0.f) continue;  // this part of the keys was hidden from the row
             const float w = fast_exp2(zm - top), wv = vr > 0.f ? w * __fdividef(__ldcg(&sl.vref), vr) : 0.f;
@@ -471,14 +527,14 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
             for (int k = 0; k < 8; ++k) x[k] += __ldcg(&sl.acc[(i0 + k) * 32 + ln]) * wv;
           }
         }
-        const int row = rt * kStepRows + r, i = row / a.group;
+        const int row = rt * kRows + r, i = row / a.group;
         if (i < s.n) {
           const float y = sum != 0.f ? vr / sum : 0.f;  // (a NaN sum stays NaN)
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] *= y;
           uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(s.first + i) * a.out.ts +
                         (long long)(head * a.group + row - i * a.group) * a.out.hs;
-          store8(o + (2 * (ln & 3) + c) * kTiles + j0, pack8<BF16>(x), a.out.vec);
+          store8(o + (ln >> 2) * kPiece + d0, pack8<BF16>(x), a.out.vec);
         }
       }
     }
@@ -487,27 +543,37 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm)
   }
 }
 
-template <bool BF16, int DIM>
+template <bool BF16, int DIM, int NT>
 cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   static std::atomic<bool> attr_set[kAttrMaxDevices];
-  const int bytes = (int)sizeof(StepShared<DIM>);
-  const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM>, bytes, attr_set);
+  const int bytes = (int)sizeof(StepShared<DIM, NT>);
+  const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT>, bytes, attr_set);
   if (e != cudaSuccess) return e;
-  const int grid = sms * kStepCtasPerSm;
-  return launch_kernel(kv_step_k<BF16, DIM>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
-                       reinterpret_cast<StepSlot<DIM> *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
+  const int grid = sms * (NT == 4 ? 2 : 3);
+  return launch_kernel(kv_step_k<BF16, DIM, NT>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
+                       reinterpret_cast<StepSlot<DIM, NT> *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
                        static_cast<unsigned *>(workspace));
+}
+
+template <bool BF16, int DIM>
+cudaError_t launch_step_rows(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  const long long rows = (long long)a.max_new * a.group;
+  if (rows <= 8) return launch_step<BF16, DIM, 1>(a, workspace, sms, st);
+  if (rows <= 16) return launch_step<BF16, DIM, 2>(a, workspace, sms, st);
+  return launch_step<BF16, DIM, 4>(a, workspace, sms, st);
 }
 
 }  // namespace
 
 // Counters (zero before the first call and after each), then two slots a CTA.
-size_t kv_workspace_bytes(int sms) { return kKvCounterBytes + sizeof(StepSlot<128>) * 2 * (size_t)sms * kStepCtasPerSm; }
+size_t kv_workspace_bytes(int sms) {
+  return kKvCounterBytes + std::max(sizeof(StepSlot<128, 4>) * 4, sizeof(StepSlot<128, 2>) * 6) * (size_t)sms;
+}
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   if (a.cache.dim == 64)
-    return bf16 ? launch_step<true, 64>(a, workspace, sms, st) : launch_step<false, 64>(a, workspace, sms, st);
-  return bf16 ? launch_step<true, 128>(a, workspace, sms, st) : launch_step<false, 128>(a, workspace, sms, st);
+    return bf16 ? launch_step_rows<true, 64>(a, workspace, sms, st) : launch_step_rows<false, 64>(a, workspace, sms, st);
+  return bf16 ? launch_step_rows<true, 128>(a, workspace, sms, st) : launch_step_rows<false, 128>(a, workspace, sms, st);
 }
 
 }  // namespace ivb
