@@ -67,6 +67,9 @@ cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const K
 // return to zero by themselves), then partial results.
 constexpr size_t kKvCounterBytes = 1 << 14;
 size_t kv_workspace_bytes(int sms);
+size_t kv_prompt_workspace_bytes(int sms);  // the part that kv_prompt.cu needs
+bool kv_prompt_takes(const KvAttend &a);
+cudaError_t launch_kv_prompt(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
 
 }  // namespace ivb

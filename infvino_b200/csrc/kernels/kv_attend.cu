@@ -567,10 +567,12 @@ cudaError_t launch_step_rows(const KvAttend &a, void *workspace, int sms, cudaSt
 
 // Counters (zero before the first call and after each), then two slots a CTA.
 size_t kv_workspace_bytes(int sms) {
-  return kKvCounterBytes + std::max(sizeof(StepSlot<128, 4>) * 4, sizeof(StepSlot<128, 2>) * 6) * (size_t)sms;
+  const size_t step = std::max(sizeof(StepSlot<128, 4>) * 4, sizeof(StepSlot<128, 2>) * 6) * (size_t)sms;
+  return kKvCounterBytes + std::max(step, kv_prompt_workspace_bytes(sms));
 }
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  if ((long long)a.max_new * a.group > 32 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, a, workspace, sms, st);
   if (a.cache.dim == 64)
     return bf16 ? launch_step_rows<true, 64>(a, workspace, sms, st) : launch_step_rows<false, 64>(a, workspace, sms, st);
   return bf16 ? launch_step_rows<true, 128>(a, workspace, sms, st) : launch_step_rows<false, 128>(a, workspace, sms, st);

@@ -1,0 +1,769 @@
+// Attention over the paged 8-bit cache for many queries a sequence (prompts,
+// chunks of prompts): the same formula as the step kernel's, on tcgen05.
+//
+// A key serves hundreds of query rows here, so arithmetic bounds it: 4 * DIM
+// operations for each visible (row, key) pair on the tensor cores, and one
+// exponential on the special function units, which takes as long (at DIM 128:
+// 16 exponentials and 8192 operations a clock and SM).
+//
+// An item is 256 query rows (token, head of the group) of one sequence and kv
+// head, two M tiles of 128; its units are tiles of 128 keys (8 blocks of 16,
+// the sinks' blocks first where there is a window).  Units are divided evenly
+// over the CTAs, one an SM; items that the division cuts are joined by the
+// last of their CTAs to arrive, in the order of the keys.
+//
+// Sixteen warps a CTA:
+//   0-3, 4-7  softmax of M tile 0 and 1, a thread a row: scores from TMEM, the
+//             weights back into the scores' columns as the next product's
+//             operand; O is rescaled in TMEM, rarely (a row's maximum follows
+//             only scores kSlack above it); at the end O goes out
+//   8-11      key and value codes from the cache through registers into shared
+//             memory as halves (exact), one tile ahead in registers and two in
+//             shared memory; the blocks' scales beside them
+//   12        issues the products: S_i = Q_i K^T (operands K-major in shared
+//             memory) and O_i += P_i V (P_i from TMEM, V row-major as it lies
+//             in the cache), i alternating, so that one tile's softmax runs
+//             under the other tile's products
+// Every wait is bounded: a timeout sets the status word and an abort flag,
+// all roles run out, and TMEM is released.
+#include <algorithm>
+
+#include "kv_attend.cuh"
+
+namespace ivb {
+
+namespace {
+
+constexpr int kKeys = 128, kTileBlocks = kKeys / kKvBlock;
+constexpr int kRows = 256;
+constexpr int kThreads = 512;
+constexpr int kMeta = 4;          // rings: scales of a tile live until both softmaxes are done
+constexpr float kSlack = 4.f, kBits = kWeightBits - kSlack;
+constexpr float kFarBelow = -40.f;  // value scales are taken as at least 2^-40 of the largest so far
+constexpr int kNoKey = 0x3fffffff;
+constexpr int kMaxSeqs = 8192;    // sequences of a call that the start-up scan has room for
+
+struct TileMeta {
+  float kc[kTileBlocks];    // ks * |scale| * log2 e
+  float lvf[kTileBlocks];   // log2 (vs / vref)
+  float ivf[kTileBlocks];   // vref / vs
+  int key0[kTileBlocks];    // first key, kNoKey behind the end
+  float vr, vref;           // vref before / vref of this tile; vref: the largest value scale so far
+  float pad[2];
+};
+
+template <int DIM>
+struct PromptShared {
+  static constexpr int kSlabs = DIM / 64;
+  uint8_t q[2][kSlabs][128 * 128];  // 128 rows of 64 halves, 16-byte pieces exchanged by row % 8
+  uint8_t k[2][kSlabs][kKeys * 128];
+  uint8_t v[2][kSlabs][kKeys * 128];
+  TileMeta meta[kMeta];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], odone[2], qfull[2], drained;
+  uint32_t tmem;
+  volatile int abort;
+  int last[2];
+  long long scan[kThreads / 32];
+  long long base;
+  int seq, rt;
+};
+
+struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4], row maximum and sum
+  float acc[128 * 128];
+  float m[128], l[128];
+  float vref;
+  float pad[31];
+};
+
+// What an item's rows see: like KvSpan, for rows r0 .. r0 + 255 of a sequence.
+struct RowSpan {
+  int sink_blocks, first_block, blocks, tiles;
+};
+__device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, int rt) {
+  RowSpan s;
+  const int i0 = rt * kRows / a.group, i1 = min(n - 1, (rt * kRows + kRows - 1) / a.group);
+  const int p_lo = len - n + i0, p_hi = len - n + i1;
+  const int all = p_hi >= 0 ? p_hi / kKvBlock + 1 : 0;
+  s.first_block = s.sink_blocks = 0;
+  if (a.window > 0) {
+    const long long lo = (long long)p_lo - a.window + 1;
+    s.first_block = lo > 0 ? (int)(lo / kKvBlock) : 0;
+    s.sink_blocks = min(s.first_block, a.sinks / kKvBlock + (a.sinks % kKvBlock != 0));
+  }
+  s.blocks = max(0, s.sink_blocks + all - s.first_block);
+  s.tiles = max(1, (s.blocks + kTileBlocks - 1) / kTileBlocks);
+  return s;
+}
+
+// The CTA's share of the units, segment after segment; every role walks it by itself.
+struct Walk {
+  long long u, u_end, base, total;  // base: first unit of (b, rt)
+  int ctas, b, rt;
+  KvSpan s;
+  // the segment
+  RowSpan r;
+  int row_tiles, head, k0, k1;
+  long long item_begin;
+
+  __device__ __forceinline__ bool next(const KvAttend &a) {
+    while (u < u_end) {
+      const long long units = (long long)r.tiles * a.cache.heads;
+      if (s.n > 0 && u < base + units) {
+        head = (int)((u - base) / r.tiles);
+        item_begin = base + (long long)head * r.tiles;
+        k0 = (int)(u - item_begin);
+        k1 = (int)(min(u_end, item_begin + r.tiles) - item_begin);
+        u += k1 - k0;
+        return true;
+      }
+      if (s.n > 0) base += units;
+      if (s.n > 0 && rt + 1 < row_tiles) {
+        ++rt;
+      } else {
+        rt = 0;
+        s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+        row_tiles = (s.n * a.group + kRows - 1) / kRows;
+      }
+      if (s.n > 0) r = row_span(a, s.n, s.len, rt);
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == r.tiles; }
+};
+
+__device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+#define KV_R8(r, o) "=f"(r[o]), "=f"(r[o + 1]), "=f"(r[o + 2]), "=f"(r[o + 3]), "=f"(r[o + 4]), "=f"(r[o + 5]), "=f"(r[o + 6]), "=f"(r[o + 7])
+#define KV_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+
+// 32 columns of the thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : KV_R8(r, 0), KV_R8(r, 8), KV_R8(r, 16), KV_R8(r, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      KV_W8(r, 0), KV_W8(r, 8)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// O (+)= P V with P from TMEM.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 bd;\n\t"
+      "mov.b64 bd, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Two codes (+ 128, in bytes of w) as halves: 1024 + u, minus 1152.
+template <int SEL>
+__device__ __forceinline__ uint32_t halves(uint32_t w) {
+  const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x64806480u));
+  return r;
+}
+
+// Sixteen codes of row r, from element 16 c, into a tile of halves.
+template <int DIM>
+__device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 w4) {
+  const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+  const uint4 lo = make_uint4(halves<0x4140>(w[0]), halves<0x4342>(w[0]), halves<0x4140>(w[1]), halves<0x4342>(w[1]));
+  const uint4 hi = make_uint4(halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
+  uint8_t *row = tile + (c >> 2) * (128 * 128) + r * 128;
+  const int p = 2 * (c & 3), x = r & 7;
+  // lanes of the second 64 elements store their halves in the other order:
+  // eight lanes (a row) then meet eight different 16-byte banks
+  const bool swap = DIM == 128 && c >= 4;
+  *reinterpret_cast<uint4 *>(row + (((swap ? p + 1 : p) ^ x) << 4)) = swap ? hi : lo;
+  *reinterpret_cast<uint4 *>(row + (((swap ? p : p + 1) ^ x) << 4)) = swap ? lo : hi;
+}
+
+template <bool BF16, int DIM>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters) {
+  extern __shared__ uint8_t smem_raw[];
+  using Shared = PromptShared<DIM>;
+  Shared &sh = *reinterpret_cast<Shared *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  constexpr int kSlabs = DIM / 64;
+  constexpr long long kLimit = kConvWaitLimitDefault;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.kfull[i]), 4);
+      mbar_init(smem_u32(&sh.vfull[i]), 4);
+      mbar_init(smem_u32(&sh.kempty[i]), 1);
+      mbar_init(smem_u32(&sh.vempty[i]), 1);
+      mbar_init(smem_u32(&sh.sfull[i]), 1);
+      mbar_init(smem_u32(&sh.odone[i]), 1);
+      mbar_init(smem_u32(&sh.pready[i]), 4);
+      mbar_init(smem_u32(&sh.qfull[i]), 4);
+    }
+    mbar_init(smem_u32(&sh.drained), 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(&sh.tmem), 512);
+    tmem_relinquish();
+  }
+  pdl_wait_and_release();
+
+  // ---- all units, and where this CTA's share begins.  A warp adds up a
+  // sequence's row tiles; the sequences' sums wait where the tiles will be.
+  long long *sums = reinterpret_cast<long long *>(&sh.q[0][0][0]);
+  for (int b0 = warp * 32; b0 < a.seqs.batch; b0 += kThreads) {
+    int n = 0, len = 0;
+    if (b0 + lane < a.seqs.batch) {
+      const KvSpan s = kv_span(a, b0 + lane);
+      n = s.n, len = s.len;
+    }
+    for (int j = 0; j < min(32, a.seqs.batch - b0); ++j) {
+      const int nj = __shfl_sync(0xffffffffu, n, j), lj = __shfl_sync(0xffffffffu, len, j);
+      const int rts = (nj * a.group + kRows - 1) / kRows;
+      long long sum = 0;
+      for (int rt = lane; rt < rts; rt += 32) sum += row_span(a, nj, lj, rt).tiles;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) sums[b0 + j] = sum * a.cache.heads;
+    }
+  }
+  __syncthreads();
+  const int per = (a.seqs.batch + kThreads - 1) / kThreads;
+  const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
+  long long mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += sums[b];
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh.scan[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sh.scan[w];
+    total += sh.scan[w];
+  }
+  Walk walk;
+  walk.total = total;
+  walk.ctas = (int)(total < (long long)gridDim.x ? total : (long long)gridDim.x);
+  const bool works = (int)blockIdx.x < walk.ctas;
+  walk.u = works ? share_begin(total, walk.ctas, blockIdx.x) : 0;
+  walk.u_end = works ? share_begin(total, walk.ctas, blockIdx.x + 1) : 0;
+  const long long excl = before + incl - mine;
+  if (works && walk.u >= excl && walk.u < excl + mine) {
+    long long at = excl;
+    int b = b_lo;
+    while (walk.u >= at + sums[b]) at += sums[b++];
+    sh.seq = b;
+    sh.base = at;
+  }
+  __syncthreads();
+  if (works && warp == 0) {  // the row tile: 32 at a time
+    const KvSpan s = kv_span(a, sh.seq);
+    const int rts = (s.n * a.group + kRows - 1) / kRows;
+    long long at = sh.base;
+    for (int r0 = 0; r0 < rts; r0 += 32) {
+      long long w = r0 + lane < rts ? (long long)row_span(a, s.n, s.len, r0 + lane).tiles * a.cache.heads : 0;
+      long long in = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += v;
+      }
+      const bool here = walk.u >= at + in - w && walk.u < at + in;
+      const unsigned vote = __ballot_sync(0xffffffffu, here);
+      if (here) {
+        sh.rt = r0 + lane;
+        sh.base = at + in - w;
+      }
+      if (vote) break;
+      at += __shfl_sync(0xffffffffu, in, 31);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  if (works) {
+    walk.b = sh.seq;
+    walk.rt = sh.rt;
+    walk.base = sh.base;
+    walk.s = kv_span(a, walk.b);
+    walk.row_tiles = (walk.s.n * a.group + kRows - 1) / kRows;
+    walk.r = row_span(a, walk.s.n, walk.s.len, walk.rt);
+  }
+  __syncthreads();  // the sums' room is the tiles' from here on
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax of M tile i
+    reg_inc<184>();
+    const int i = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + 128u * i, o_at = tmem + lanes + 256u + 128u * i;
+    const uint32_t sfull = smem_u32(&sh.sfull[i]), odone = smem_u32(&sh.odone[i]), pready = smem_u32(&sh.pready[i]);
+    int done = 0;   // tiles so far, all segments
+    int tile = 0;   // tiles of both M tiles so far: the place of the scales
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
+      return ok;
+    };
+    while (walk.next(a)) {
+      const int first_row = walk.rt * kRows + 128 * i, rows = min(128, walk.s.n * a.group - first_row);
+      const int tiles = walk.k1 - walk.k0;
+      if (rows <= 0) {
+        tile += tiles;
+        continue;
+      }
+      // ---- the query row: halves, K-major
+      const int tok = (first_row + row) / a.group, qh = walk.head * a.group + first_row + row - tok * a.group;
+      const bool real = row < rows;
+      const int p = real ? walk.s.len - walk.s.n + tok : -1;
+      const int p_lo = walk.s.len - walk.s.n + first_row / a.group;
+      const int p_hi = walk.s.len - walk.s.n + (first_row + rows - 1) / a.group;
+      float rf = 1.f;
+      {
+        const uint16_t *src = static_cast<const uint16_t *>(a.q.p) + (long long)(walk.s.first + tok) * a.q.ts + (long long)qh * a.q.hs;
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // |scale| is in the keys' factor
+        uint4 w[DIM / 8];
+#pragma unroll
+        for (int c = 0; c < DIM / 8; ++c) {
+          w[c] = real ? load8(src + 8 * c, a.q.vec) : make_uint4(0, 0, 0, 0);
+          w[c].x ^= flip, w[c].y ^= flip, w[c].z ^= flip, w[c].w ^= flip;
+        }
+        if (BF16) {
+          // bf16 queries become halves: scaled by a power of two so that the
+          // row's largest element lies in 2^0 .. 2^1 (its eight bits stay)
+          float most = 0.f;
+#pragma unroll
+          for (int c = 0; c < DIM / 8; ++c) {
+            float f[8];
+            unpack8<true>(w[c], f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
+          }
+          const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
+          const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+          rf = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+          for (int c = 0; c < DIM / 8; ++c) {
+            float f[8];
+            unpack8<true>(w[c], f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] *= down;
+            w[c] = pack8<false>(f);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < DIM / 8; ++c)
+          *reinterpret_cast<uint4 *>(&sh.q[i][c >> 3][row * 128 + (((c & 7) ^ (row & 7)) << 4)]) = w[c];
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.qfull[i]));
+
+      float m = -INFINITY, l = 0.f, vref = 0.f;
+      for (int t = 0; t < tiles; ++t, ++done, ++tile) {
+        if (!wait(sfull, done & 1, kStatusTimeoutAcc)) continue;
+        tc_fence_after();
+        float s[kKeys];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
+        const TileMeta &me = sh.meta[tile % kMeta];
+        // hidden keys: behind the row, before its window, behind the end
+        bool masked = me.key0[kTileBlocks - 1] + kKvBlock - 1 > p_lo;
+        if (a.window > 0) {
+#pragma unroll
+          for (int b = 0; b < kTileBlocks; ++b)
+            masked = masked || (p_hi - me.key0[b] >= a.window && me.key0[b] + kKvBlock > a.sinks);
+        }
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < kTileBlocks; ++b) {
+            const int k0 = me.key0[b];
+            const int hi = p - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.window > 0 ? a.sinks - k0 : 0;
+#pragma unroll
+            for (int k = 0; k < kKvBlock; ++k)
+              if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * b + k] = -INFINITY;
+          }
+        }
+        float c[kTileBlocks];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) {
+          c[b] = fmaxf(BF16 ? me.kc[b] * rf : me.kc[b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
+          float x = s[kKvBlock * b];
+#pragma unroll
+          for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
+          mx = fmaxf(mx, x * c[b]);
+        }
+        const float vr = me.vr;
+        vref = me.vref;
+        if (__any_sync(0xffffffffu, mx > m + kSlack) || vr != 1.f) {
+          const float top = fmaxf(m, mx);
+          const float f = top > m ? fast_exp2(m - top) : 1.f;
+          m = top;
+          l *= f;
+          if (t > 0) {
+            if (!wait(odone, (done - 1) & 1, kStatusTimeoutDrain)) continue;
+            tc_fence_after();
+            const float fo = f * vr;
+#pragma unroll
+            for (int h = 0; h < DIM / 32; ++h) {
+              float o[32];
+              tmem_ld32(o_at + 32 * h, o);
+              tmem_ld_wait();
+              uint32_t w[32];
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                asm volatile("" : "+f"(o[k]));
+                w[k] = __float_as_uint(o[k] * fo);
+              }
+              tmem_st16(o_at + 32 * h, w);
+              tmem_st16(o_at + 32 * h + 16, w + 16);
+            }
+          }
+        }
+        // weights 2^(s c - m + kBits) vs / vref, sums without the last factor
+        const float shift = m == -INFINITY ? 0.f : kBits - m;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int b = 2 * q + h;
+            const float add = shift + me.lvf[b];
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kKvBlock; k += 2) {
+              const float x = fast_exp2(fmaf(s[kKvBlock * b + k], c[b], add));
+              const float y = fast_exp2(fmaf(s[kKvBlock * b + k + 1], c[b], add));
+              sum += x + y;
+              w[8 * h + k / 2] = pack2<false>(x, y);
+            }
+            l = fmaf(sum, me.ivf[b], l);
+          }
+          tmem_st16(s_at + 16 * q, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pready);
+      }
+
+      // ---- O
+      wait(odone, (done - 1) & 1, kStatusTimeoutDrain);
+      tc_fence_after();
+      const bool whole = walk.whole();
+      const int first_cta = share_of(walk.total, walk.ctas, walk.item_begin),
+                last_cta = share_of(walk.total, walk.ctas, walk.item_begin + walk.r.tiles - 1);
+      uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(walk.s.first + tok) * a.out.ts + (long long)qh * a.out.hs;
+      if (whole) {
+        const float y = l != 0.f ? vref / l : 0.f;  // (a NaN sum stays NaN)
+#pragma unroll
+        for (int h = 0; h < DIM / 32; ++h) {
+          float o[32];
+          if (ok) tmem_ld32(o_at + 32 * h, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
+          if (real && ok) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float f[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] = l != 0.f ? o[k + j] * y : 0.f;
+              store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
+            }
+          }
+        }
+      } else {
+        PromptSlot &slot = slots[2 * (2 * (int)blockIdx.x + (walk.k0 == 0 ? 1 : 0)) + i];
+#pragma unroll
+        for (int h = 0; h < DIM / 32; ++h) {
+          float o[32];
+          if (ok) tmem_ld32(o_at + 32 * h, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            __stcg(reinterpret_cast<float4 *>(&slot.acc[((32 * h + k) / 4 * 128 + row) * 4]),
+                   make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+        }
+        __stcg(&slot.m[row], m);
+        __stcg(&slot.l[row], l);
+        if (row == 0) __stcg(&slot.vref, vref);
+        __threadfence();
+        wg_sync(1 + i);
+        if (row == 0) {
+          const unsigned parts = (unsigned)(last_cta - first_cta + 1);
+          const unsigned old = atomicAdd(&counters[2 * first_cta + i], 1u);
+          sh.last[i] = old == parts - 1;
+          if (old == parts - 1) atomicExch(&counters[2 * first_cta + i], 0u);
+          __threadfence();
+        }
+        wg_sync(1 + i);
+        if (sh.last[i] && real && ok) {
+          float top = -INFINITY, vmax = 0.f, sum = 0.f;
+          for (int z = first_cta; z <= last_cta; ++z) {
+            const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
+            top = fmaxf(top, __ldcg(&sl.m[row]));
+            vmax = fmaxf(vmax, __ldcg(&sl.vref));
+          }
+          for (int h = 0; h < DIM / 32; ++h) {
+            float x[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = 0.f;
+            sum = 0.f;
+            for (int z = first_cta; z <= last_cta; ++z) {
+              const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
+              const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]);
+              if (zm == -INFINITY && zl == 0.f) continue;  // this part of the keys was hidden from the row
+              const float w = fast_exp2(zm - top), wv = vmax > 0.f ? w * __fdividef(__ldcg(&sl.vref), vmax) : 0.f;
+              sum += zl * w;
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[((32 * h + k) / 4 * 128 + row) * 4]));
+                x[k] += v.x * wv, x[k + 1] += v.y * wv, x[k + 2] += v.z * wv, x[k + 3] += v.w * wv;
+              }
+            }
+            const float y = sum != 0.f ? vmax / sum : 0.f;
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float f[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y;
+              store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ codes to halves
+    reg_dec<96>();
+    constexpr int kParts = DIM / 16;        // 16-code pieces of a row
+    constexpr int kStep = 32 / kParts;      // rows a warp takes at once
+    constexpr int kEach = 32 / kStep;       // pieces a lane holds of the warp's 32 rows
+    const int w = warp - 8, c = lane % kParts, r_in = lane / kParts;
+    const float kc_all = fabsf(a.scale) * kLog2e;
+    uint4 kreg[kEach], vreg[kEach];
+    int tile = 0;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, kStatusTimeoutEmpty, kLimit));
+      return ok;
+    };
+    float vref = 0.f;
+    // lane j < 8 knows block j of a tile: where its codes are, its scales
+    struct Blocks {
+      long long at;
+      int key0;
+      float ks, vs;
+    };
+    auto look_up = [&](int t) {
+      Blocks x{-1, kNoKey, 0.f, 0.f};
+      const int bi = t * kTileBlocks + lane;
+      if (lane < kTileBlocks && t < walk.k1 && bi < walk.r.blocks) {
+        const int key = (bi < walk.r.sink_blocks ? bi : bi - walk.r.sink_blocks + walk.r.first_block) * kKvBlock;
+        const int page = kv_page_of(a.cache, a.seqs, walk.b, key, a.status);
+        if (page >= 0) {
+          const int slot = key % a.cache.page;
+          x.key0 = key;
+          x.at = kv_code_at(a.cache, page, walk.head, slot);
+          const long long sa = kv_scale_at(a.cache, page, walk.head, slot);
+          x.ks = a.cache.ks[sa];
+          x.vs = a.cache.vs[sa];
+        }
+      }
+      return x;
+    };
+    auto load = [&](const int8_t *codes, const Blocks &x, uint4(&reg)[kEach]) {
+      const long long at0 = __shfl_sync(0xffffffffu, x.at, 2 * w), at1 = __shfl_sync(0xffffffffu, x.at, 2 * w + 1);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int r = e * kStep + r_in;  // of the warp's 32: blocks 2 w and 2 w + 1
+        const long long at = e * kStep < kKvBlock ? at0 : at1;
+        reg[e] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(codes + at + (r & 15) * DIM + 16 * c)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    while (walk.next(a)) {
+      vref = 0.f;
+      Blocks now = look_up(walk.k0), ahead = look_up(walk.k0 + 1);
+      load(a.cache.k, now, kreg);
+      load(a.cache.v, now, vreg);
+      for (int t = walk.k0; t < walk.k1; ++t, ++tile) {
+        const int st = tile & 1;
+        const bool reused = tile >= 2;
+        if (reused) wait(smem_u32(&sh.kempty[st]), ((tile >> 1) - 1) & 1);
+        if (w == 0) {  // the scales
+          float vmax = now.vs;
+#pragma unroll
+          for (int o = 4; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+          vmax = fmaxf(vref, __shfl_sync(0xffffffffu, vmax, 0));
+          TileMeta &me = sh.meta[tile % kMeta];
+          if (lane < kTileBlocks) {
+            const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(log2f(now.vs) - log2f(vmax), kFarBelow) : kFarBelow;
+            me.kc[lane] = now.ks * kc_all;
+            me.lvf[lane] = lv;
+            me.ivf[lane] = exp2f(-lv);
+            me.key0[lane] = now.key0;
+          }
+          if (lane == 0) {
+            me.vr = vmax > vref ? vref / vmax : 1.f;
+            me.vref = vmax;
+          }
+          vref = vmax;
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) put_codes<DIM>(&sh.k[st][0][0], 32 * w + e * kStep + r_in, c, kreg[e]);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.kfull[st]));
+        load(a.cache.k, ahead, kreg);
+        if (reused) wait(smem_u32(&sh.vempty[st]), ((tile >> 1) - 1) & 1);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) put_codes<DIM>(&sh.v[st][0][0], 32 * w + e * kStep + r_in, c, vreg[e]);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.vfull[st]));
+        load(a.cache.v, ahead, vreg);
+        now = ahead;
+        ahead = look_up(t + 2);
+      }
+    }
+  } else {
+    reg_dec<40>();
+    if (warp == 12) {
+      // ---------------------------------------------------------- products
+      const bool leader = elect_one();
+      const uint32_t idesc_s = idesc_f16_f32(128, kKeys);
+      const uint32_t idesc_o = idesc_f16_f32(128, DIM) | (1u << 16);  // V: rows are keys (its N side is dense)
+      const uint64_t qd = smem_desc_kmajor(smem_u32(&sh.q[0][0][0]), 128), kd = smem_desc_kmajor(smem_u32(&sh.k[0][0][0]), 128);
+      // V: 64 head elements a row of 128 bytes; 8 keys 1024 bytes on, the next 64 elements a slab on
+      const uint64_t vd = (uint64_t)((smem_u32(&sh.v[0][0][0]) & 0x3FFFFu) >> 4) | ((uint64_t)(128 * 128 >> 4) << 16) |
+                          ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+      constexpr uint32_t kTileUnits = kSlabs * 128 * 128 / 16, kSlabUnits = 128 * 128 / 16;
+      int tile = 0, seg[2] = {0, 0}, done[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
+        return ok;
+      };
+      auto scores = [&](int i, int st, bool last) {
+        tc_fence_after();
+        if (leader) {
+          const uint32_t q_lo = (uint32_t)qd + (uint32_t)i * kTileUnits, k_lo = (uint32_t)kd + (uint32_t)st * kTileUnits;
+#pragma unroll
+          for (int k = 0; k < DIM / 16; ++k) {
+            const uint32_t o = (uint32_t)(k >> 2) * kSlabUnits + 2u * (k & 3);
+            umma_f16_lh(tmem + 128u * i, q_lo + o, (uint32_t)(qd >> 32), k_lo + o, (uint32_t)(kd >> 32), idesc_s, k > 0);
+          }
+          umma_commit(smem_u32(&sh.sfull[i]));
+          if (last) umma_commit(smem_u32(&sh.kempty[st]));
+        }
+        __syncwarp();
+      };
+      auto values = [&](int i, int st, bool begin, bool last) {
+        tc_fence_after();
+        if (leader) {
+          const uint32_t v_lo = (uint32_t)vd + (uint32_t)st * kTileUnits;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_f16_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * k, v_lo + (2048u / 16u) * k, (uint32_t)(vd >> 32), idesc_o,
+                        !begin || k > 0);
+          umma_commit(smem_u32(&sh.odone[i]));
+          if (last) umma_commit(smem_u32(&sh.vempty[st]));
+        }
+        __syncwarp();
+      };
+      while (walk.next(a)) {
+        const int tiles = walk.k1 - walk.k0;
+        const int m_tiles = walk.s.n * a.group - walk.rt * kRows > 128 ? 2 : 1;
+        if (!ok) break;
+        wait(smem_u32(&sh.kfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
+        for (int i = 0; i < m_tiles && ok; ++i) {
+          if (wait(smem_u32(&sh.qfull[i]), seg[i] & 1, kStatusTimeoutFull)) scores(i, tile & 1, i == m_tiles - 1);
+          ++seg[i];
+        }
+        for (int t = 0; t < tiles && ok; ++t, ++tile) {
+          for (int i = 0; i < m_tiles && ok; ++i) {
+            if (i == 0) wait(smem_u32(&sh.vfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
+            if (!wait(smem_u32(&sh.pready[i]), done[i] & 1, kStatusTimeoutAccEmpty)) break;
+            values(i, tile & 1, t == 0, i == m_tiles - 1);
+            ++done[i];
+            if (t + 1 < tiles) {
+              if (i == 0) wait(smem_u32(&sh.kfull[(tile + 1) & 1]), ((tile + 1) >> 1) & 1, kStatusTimeoutFull);
+              if (ok) scores(i, (tile + 1) & 1, i == m_tiles - 1);
+            }
+          }
+        }
+      }
+      // every product retires before TMEM is released
+      volatile int no_abort = 0;
+      if (leader) umma_commit(smem_u32(&sh.drained));
+      __syncwarp();
+      mbar_wait_bounded(smem_u32(&sh.drained), 0, &no_abort, a.status, kStatusTimeoutDrain, 400000000LL);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool BF16, int DIM>
+cudaError_t launch_prompt(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  static std::atomic<bool> attr_set[kAttrMaxDevices];
+  const int bytes = (int)sizeof(PromptShared<DIM>) + 1024;
+  const cudaError_t e = ensure_dynamic_smem(kv_prompt_k<BF16, DIM>, bytes, attr_set);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kv_prompt_k<BF16, DIM>, dim3(sms), dim3(kThreads), (size_t)bytes, st, a,
+                       reinterpret_cast<PromptSlot *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
+                       static_cast<unsigned *>(workspace));
+}
+
+}  // namespace
+
+size_t kv_prompt_workspace_bytes(int sms) { return sizeof(PromptSlot) * 4 * (size_t)sms; }
+
+bool kv_prompt_takes(const KvAttend &a) { return a.seqs.batch <= kMaxSeqs; }
+
+cudaError_t launch_kv_prompt(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  if (a.cache.dim == 64)
+    return bf16 ? launch_prompt<true, 64>(a, workspace, sms, st) : launch_prompt<false, 64>(a, workspace, sms, st);
+  return bf16 ? launch_prompt<true, 128>(a, workspace, sms, st) : launch_prompt<false, 128>(a, workspace, sms, st);
+}
+
+}  // namespace ivb
