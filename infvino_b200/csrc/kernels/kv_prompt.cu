@@ -41,6 +41,7 @@ constexpr int kMeta = 4;          // rings: scales of a tile live until both sof
 constexpr float kSlack = 4.f, kBits = kWeightBits - kSlack;
 constexpr float kFarBelow = -40.f;  // value scales are taken as at least 2^-40 of the largest so far
 constexpr int kNoKey = 0x3fffffff;
+constexpr int kItemCost = 2;      // what an item costs besides its tiles, in tiles: queries in, outputs out
 constexpr int kMaxSeqs = 8192;    // sequences of a call that the start-up scan has room for
 
 struct TileMeta {
@@ -50,29 +51,6 @@ struct TileMeta {
   int key0[kTileBlocks];    // first key, kNoKey behind the end
   float vr, vref;           // vref before / vref of this tile; vref: the largest value scale so far
   float pad[2];
-};
-
-template <int DIM>
-struct PromptShared {
-  static constexpr int kSlabs = DIM / 64;
-  uint8_t q[2][kSlabs][128 * 128];  // 128 rows of 64 halves, 16-byte pieces exchanged by row % 8
-  uint8_t k[2][kSlabs][kKeys * 128];
-  uint8_t v[2][kSlabs][kKeys * 128];
-  TileMeta meta[kMeta];
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], odone[2], qfull[2], drained;
-  uint32_t tmem;
-  volatile int abort;
-  int last[2];
-  long long scan[kThreads / 32];
-  long long base;
-  int seq, rt;
-};
-
-struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4], row maximum and sum
-  float acc[128 * 128];
-  float m[128], l[128];
-  float vref;
-  float pad[31];
 };
 
 // What an item's rows see: like KvSpan, for rows r0 .. r0 + 255 of a sequence.
@@ -95,25 +73,39 @@ __device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, i
   return s;
 }
 
-// The CTA's share of the units, segment after segment; every role walks it by itself.
+// The CTA's share of the units, segment after segment.  Every warp walks it by
+// itself, with its place in shared memory (registers are the softmax's).
 struct Walk {
   long long u, u_end, base, total;  // base: first unit of (b, rt)
   int ctas, b, rt;
   KvSpan s;
   // the segment
   RowSpan r;
-  int row_tiles, head, k0, k1;
-  long long item_begin;
+  int row_tiles, head, k0, k1, first_cta, last_cta;
 
+  // One warp's step, by its lane 0.
   __device__ __forceinline__ bool next(const KvAttend &a) {
+    __syncwarp();
+    bool more = false;
+    if ((threadIdx.x & 31) == 0) more = advance(a);
+    return __shfl_sync(0xffffffffu, more, 0);  // (and the place is the warp's to read)
+  }
+  __device__ __forceinline__ bool advance(const KvAttend &a) {
     while (u < u_end) {
-      const long long units = (long long)r.tiles * a.cache.heads;
+      const int each = r.tiles + kItemCost;
+      const long long units = (long long)each * a.cache.heads;
       if (s.n > 0 && u < base + units) {
-        head = (int)((u - base) / r.tiles);
-        item_begin = base + (long long)head * r.tiles;
-        k0 = (int)(u - item_begin);
-        k1 = (int)(min(u_end, item_begin + r.tiles) - item_begin);
-        u += k1 - k0;
+        head = (int)((uint32_t)(u - base) / (uint32_t)each);  // (tiles < 2^24, heads at most 2^8)
+        const long long item = base + (long long)head * each, end = min(u_end, item + each);
+        k0 = max(0, (int)(u - item) - kItemCost);
+        k1 = (int)(end - item) - kItemCost;
+        u = end;
+        if (k1 <= k0) continue;  // the share ends before the item's first tile
+        first_cta = last_cta = 0;
+        if (!whole()) {
+          first_cta = share_of(total, ctas, item + kItemCost);
+          last_cta = share_of(total, ctas, item + each - 1);
+        }
         return true;
       }
       if (s.n > 0) base += units;
@@ -129,6 +121,30 @@ struct Walk {
     return false;
   }
   __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == r.tiles; }
+};
+
+template <int DIM>
+struct PromptShared {
+  static constexpr int kSlabs = DIM / 64;
+  uint8_t q[2][kSlabs][128 * 128];  // 128 rows of 64 halves, 16-byte pieces exchanged by row % 8
+  uint8_t k[2][kSlabs][kKeys * 128];
+  uint8_t v[2][kSlabs][kKeys * 128];
+  TileMeta meta[kMeta];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], odone[2], qfull[2], drained;
+  uint32_t tmem;
+  volatile int abort;
+  int last[2];
+  Walk walks[13];  // softmax, codes, products: a warp each
+  long long scan[kThreads / 32];
+  long long base;
+  int seq, rt;
+};
+
+struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4], row maximum and sum
+  float acc[128 * 128];
+  float m[128], l[128];
+  float vref;
+  float pad[31];
 };
 
 __device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
@@ -154,6 +170,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float *r) {
       : KV_R8(r, 0), KV_R8(r, 8), KV_R8(r, 16), KV_R8(r, 24)
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld_done(float (&r)[32]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(r[k]));  // uses stay after the wait
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -162,6 +183,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 
 // O (+)= P V with P from TMEM.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
@@ -243,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nj = __shfl_sync(0xffffffffu, n, j), lj = __shfl_sync(0xffffffffu, len, j);
       const int rts = (nj * a.group + kRows - 1) / kRows;
       long long sum = 0;
-      for (int rt = lane; rt < rts; rt += 32) sum += row_span(a, nj, lj, rt).tiles;
+      for (int rt = lane; rt < rts; rt += 32) sum += row_span(a, nj, lj, rt).tiles + kItemCost;
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) sums[b0 + j] = sum * a.cache.heads;
@@ -267,17 +308,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
-  Walk walk;
-  walk.total = total;
-  walk.ctas = (int)(total < (long long)gridDim.x ? total : (long long)gridDim.x);
-  const bool works = (int)blockIdx.x < walk.ctas;
-  walk.u = works ? share_begin(total, walk.ctas, blockIdx.x) : 0;
-  walk.u_end = works ? share_begin(total, walk.ctas, blockIdx.x + 1) : 0;
+  // (a share is at least an item's cost and a tile, or no CTA would have the tiles between two of them)
+  const long long most = max(1LL, total / (kItemCost + 1));
+  const int ctas = total == 0 ? 0 : (int)(most < (long long)gridDim.x ? most : (long long)gridDim.x);
+  const bool works = (int)blockIdx.x < ctas;
+  const long long u = works ? share_begin(total, ctas, blockIdx.x) : 0;
   const long long excl = before + incl - mine;
-  if (works && walk.u >= excl && walk.u < excl + mine) {
+  if (works && u >= excl && u < excl + mine) {
     long long at = excl;
     int b = b_lo;
-    while (walk.u >= at + sums[b]) at += sums[b++];
+    while (u >= at + sums[b]) at += sums[b++];
     sh.seq = b;
     sh.base = at;
   }
@@ -287,14 +327,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rts = (s.n * a.group + kRows - 1) / kRows;
     long long at = sh.base;
     for (int r0 = 0; r0 < rts; r0 += 32) {
-      long long w = r0 + lane < rts ? (long long)row_span(a, s.n, s.len, r0 + lane).tiles * a.cache.heads : 0;
+      long long w = r0 + lane < rts ? (long long)(row_span(a, s.n, s.len, r0 + lane).tiles + kItemCost) * a.cache.heads : 0;
       long long in = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, in, o);
         if (lane >= o) in += v;
       }
-      const bool here = walk.u >= at + in - w && walk.u < at + in;
+      const bool here = u >= at + in - w && u < at + in;
       const unsigned vote = __ballot_sync(0xffffffffu, here);
       if (here) {
         sh.rt = r0 + lane;
@@ -308,13 +348,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  if (works) {
-    walk.b = sh.seq;
-    walk.rt = sh.rt;
-    walk.base = sh.base;
-    walk.s = kv_span(a, walk.b);
-    walk.row_tiles = (walk.s.n * a.group + kRows - 1) / kRows;
-    walk.r = row_span(a, walk.s.n, walk.s.len, walk.rt);
+  Walk &walk = sh.walks[min(warp, 12)];
+  if (lane == 0 && warp < 13) {
+    walk.total = total;
+    walk.ctas = ctas;
+    walk.u = u;
+    walk.u_end = works ? share_begin(total, ctas, blockIdx.x + 1) : 0;
+    if (works) {
+      walk.b = sh.seq;
+      walk.rt = sh.rt;
+      walk.base = sh.base;
+      walk.s = kv_span(a, walk.b);
+      walk.row_tiles = (walk.s.n * a.group + kRows - 1) / kRows;
+      walk.r = row_span(a, walk.s.n, walk.s.len, walk.rt);
+    }
   }
   __syncthreads();  // the sums' room is the tiles' from here on
 
@@ -332,70 +379,83 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
       return ok;
     };
-    while (walk.next(a)) {
-      const int first_row = walk.rt * kRows + 128 * i, rows = min(128, walk.s.n * a.group - first_row);
-      const int tiles = walk.k1 - walk.k0;
-      if (rows <= 0) {
-        tile += tiles;
-        continue;
-      }
-      // ---- the query row: halves, K-major
-      const int tok = (first_row + row) / a.group, qh = walk.head * a.group + first_row + row - tok * a.group;
-      const bool real = row < rows;
-      const int p = real ? walk.s.len - walk.s.n + tok : -1;
-      const int p_lo = walk.s.len - walk.s.n + first_row / a.group;
-      const int p_hi = walk.s.len - walk.s.n + (first_row + rows - 1) / a.group;
-      float rf = 1.f;
-      {
-        const uint16_t *src = static_cast<const uint16_t *>(a.q.p) + (long long)(walk.s.first + tok) * a.q.ts + (long long)qh * a.q.hs;
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // |scale| is in the keys' factor
-        uint4 w[DIM / 8];
+    // ---- the warp's 32 query rows of the walk's segment: halves, K-major.
+    // DIM / 8 lanes a row; rf of a row's owner is what its halves were divided by.
+    float rf = 1.f;
+    auto load_q = [&]() {
+      constexpr int kLanes = DIM / 8, kAtOnce = 32 / kLanes;
+      const int c = lane % kLanes, first_row = walk.rt * kRows + 128 * i + 32 * (warp & 3);
+      const int all_rows = walk.s.n * a.group, head0 = walk.head * a.group;
+      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // |scale| is in the keys' factor
+      const uint16_t *src = static_cast<const uint16_t *>(a.q.p) + (long long)walk.s.first * a.q.ts + 8 * c;
+#pragma unroll 1
+      for (int e0 = 0; e0 < kLanes; e0 += 8) {
+        uint4 w[8];
 #pragma unroll
-        for (int c = 0; c < DIM / 8; ++c) {
-          w[c] = real ? load8(src + 8 * c, a.q.vec) : make_uint4(0, 0, 0, 0);
-          w[c].x ^= flip, w[c].y ^= flip, w[c].z ^= flip, w[c].w ^= flip;
+        for (int e = 0; e < 8; ++e) {
+          const int r = first_row + (e0 + e) * kAtOnce + lane / kLanes, tok = r / a.group;
+          w[e] = r < all_rows ? load8(src + (long long)tok * a.q.ts + (long long)(head0 + r - tok * a.group) * a.q.hs, a.q.vec)
+                              : make_uint4(0, 0, 0, 0);
         }
-        if (BF16) {
-          // bf16 queries become halves: scaled by a power of two so that the
-          // row's largest element lies in 2^0 .. 2^1 (its eight bits stay)
-          float most = 0.f;
 #pragma unroll
-          for (int c = 0; c < DIM / 8; ++c) {
-            float f[8];
-            unpack8<true>(w[c], f);
+        for (int e = 0; e < 8; ++e) {
+          const int rw = (e0 + e) * kAtOnce + lane / kLanes;  // of the warp's rows
+          w[e].x ^= flip, w[e].y ^= flip, w[e].z ^= flip, w[e].w ^= flip;
+          if (BF16) {
+            // bf16 queries become halves: scaled by a power of two so that the
+            // row's largest element lies in 2^0 .. 2^1 (its eight bits stay)
+            float f[8], most = 0.f;
+            unpack8<true>(w[e], f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
-          }
-          const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
-          const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-          rf = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-          for (int c = 0; c < DIM / 8; ++c) {
-            float f[8];
-            unpack8<true>(w[c], f);
+            for (int o = kLanes / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int x = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
+            const float down = __uint_as_float((uint32_t)(254 - x) << 23);
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] *= down;
-            w[c] = pack8<false>(f);
+            w[e] = pack8<false>(f);
+            const int own = (lane % kAtOnce) * kLanes;  // (lane / kAtOnce = (e0 + e): the row is this lane's)
+            const float up = __shfl_sync(0xffffffffu, __uint_as_float((uint32_t)x << 23), own);
+            if (lane / kAtOnce == e0 + e) rf = up;
           }
+          const int row = 32 * (warp & 3) + rw;
+          *reinterpret_cast<uint4 *>(&sh.q[i][c >> 3][row * 128 + (((c & 7) ^ (row & 7)) << 4)]) = w[e];
         }
-#pragma unroll
-        for (int c = 0; c < DIM / 8; ++c)
-          *reinterpret_cast<uint4 *>(&sh.q[i][c >> 3][row * 128 + (((c & 7) ^ (row & 7)) << 4)]) = w[c];
       }
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.qfull[i]));
-
+    };
+    // the next segment with rows for this M tile; its queries follow at once,
+    // before the outputs of the one that is ending
+    auto advance = [&]() {
+      while (walk.next(a)) {
+        if (walk.s.n * a.group > walk.rt * kRows + 128 * i) {
+          load_q();
+          return true;
+        }
+        tile += walk.k1 - walk.k0;
+      }
+      return false;
+    };
+    bool more = advance();
+    while (more) {
+      const int first_row = walk.rt * kRows + 128 * i, rows = min(128, walk.s.n * a.group - first_row);
+      const int tiles = walk.k1 - walk.k0;
+      const int tok = (first_row + row) / a.group;
+      const bool real = row < rows;
+      const int p = real ? walk.s.len - walk.s.n + tok : -1;
+      const int p_lo = walk.s.len - walk.s.n + first_row / a.group;
+      const int p_hi = walk.s.len - walk.s.n + (first_row + rows - 1) / a.group;
+      const bool whole = walk.whole(), head_part = walk.k0 == 0;
+      const int first_cta = walk.first_cta, last_cta = walk.last_cta;
+      uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(walk.s.first + tok) * a.out.ts +
+                      (long long)(walk.head * a.group + first_row + row - tok * a.group) * a.out.hs;
       float m = -INFINITY, l = 0.f, vref = 0.f;
       for (int t = 0; t < tiles; ++t, ++done, ++tile) {
         if (!wait(sfull, done & 1, kStatusTimeoutAcc)) continue;
         tc_fence_after();
-        float s[kKeys];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
-        tmem_ld_wait();
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
         const TileMeta &me = sh.meta[tile % kMeta];
         // hidden keys: behind the row, before its window, behind the end
         bool masked = me.key0[kTileBlocks - 1] + kKvBlock - 1 > p_lo;
@@ -404,25 +464,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int b = 0; b < kTileBlocks; ++b)
             masked = masked || (p_hi - me.key0[b] >= a.window && me.key0[b] + kKvBlock > a.sinks);
         }
-        if (masked) {
+        auto hide = [&](int c, float(&s)[32]) {
 #pragma unroll
-          for (int b = 0; b < kTileBlocks; ++b) {
-            const int k0 = me.key0[b];
+          for (int h = 0; h < 2; ++h) {
+            const int k0 = me.key0[2 * c + h];
             const int hi = p - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.window > 0 ? a.sinks - k0 : 0;
 #pragma unroll
             for (int k = 0; k < kKvBlock; ++k)
-              if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * b + k] = -INFINITY;
+              if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * h + k] = -INFINITY;
           }
-        }
-        float c[kTileBlocks];
+        };
+        // the scores are read twice, 32 columns at a time, the next 32 on
+        // their way: once for the maximum, once for the weights
+        float s0[32], s1[32];
         float mx = -INFINITY;
+        auto factor = [&](int b) { return fmaxf(BF16 ? me.kc[b] * rf : me.kc[b], 0x1p-120f); };  // (never 0: hidden keys stay at -inf)
+        auto top32 = [&](int c, float(&s)[32]) {
+          if (masked) hide(c, s);
 #pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b) {
-          c[b] = fmaxf(BF16 ? me.kc[b] * rf : me.kc[b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
-          float x = s[kKvBlock * b];
+          for (int h = 0; h < 2; ++h) {
+            float x = s[kKvBlock * h];
 #pragma unroll
-          for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
-          mx = fmaxf(mx, x * c[b]);
+            for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * h + k]);
+            mx = fmaxf(mx, x * factor(2 * c + h));
+          }
+        };
+        tmem_ld32(s_at, s0);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_done(s0);
+          tmem_ld32(s_at + 32 * c + 32, s1);
+          top32(c, s0);
+          tmem_ld_done(s1);
+          tmem_ld32(s_at + (c == 0 ? 64 : 0), s0);
+          top32(c + 1, s1);
         }
         const float vr = me.vr;
         vref = me.vref;
@@ -435,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait(odone, (done - 1) & 1, kStatusTimeoutDrain)) continue;
             tc_fence_after();
             const float fo = f * vr;
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < DIM / 32; ++h) {
               float o[32];
               tmem_ld32(o_at + 32 * h, o);
@@ -453,24 +528,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // weights 2^(s c - m + kBits) vs / vref, sums without the last factor
         const float shift = m == -INFINITY ? 0.f : kBits - m;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        auto weights32 = [&](int c, float(&s)[32]) {
+          if (masked) hide(c, s);
           uint32_t w[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int b = 2 * q + h;
-            const float add = shift + me.lvf[b];
-            float sum = 0.f;
+            const int b = 2 * c + h;
+            const float f = factor(b), add = shift + me.lvf[b];
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < kKvBlock; k += 2) {
-              const float x = fast_exp2(fmaf(s[kKvBlock * b + k], c[b], add));
-              const float y = fast_exp2(fmaf(s[kKvBlock * b + k + 1], c[b], add));
-              sum += x + y;
-              w[8 * h + k / 2] = pack2<false>(x, y);
+              float2 x = fma2(make_float2(s[kKvBlock * h + k], s[kKvBlock * h + k + 1]), make_float2(f, f), make_float2(add, add));
+              x.x = fast_exp2(x.x);
+              x.y = fast_exp2(x.y);
+              sum = add2(sum, x);
+              w[8 * h + k / 2] = pack2<false>(x.x, x.y);
             }
-            l = fmaf(sum, me.ivf[b], l);
+            l = fmaf(sum.x + sum.y, me.ivf[b], l);
           }
-          tmem_st16(s_at + 16 * q, w);
+          tmem_st16(s_at + 16 * c, w);  // (columns whose scores have been read)
+        };
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_done(s0);
+          tmem_ld32(s_at + 32 * c + 32, s1);
+          weights32(c, s0);
+          tmem_ld_done(s1);
+          if (c == 0) tmem_ld32(s_at + 64, s0);
+          weights32(c + 1, s1);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -479,22 +564,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 
       // ---- O
+      more = advance();
       wait(odone, (done - 1) & 1, kStatusTimeoutDrain);
       tc_fence_after();
-      const bool whole = walk.whole();
-      const int first_cta = share_of(walk.total, walk.ctas, walk.item_begin),
-                last_cta = share_of(walk.total, walk.ctas, walk.item_begin + walk.r.tiles - 1);
-      uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(walk.s.first + tok) * a.out.ts + (long long)qh * a.out.hs;
-      if (whole) {
+      if (!ok) {  // (the slot keeps whatever it holds: the status word says that the result is not valid)
+      } else if (whole) {
         const float y = l != 0.f ? vref / l : 0.f;  // (a NaN sum stays NaN)
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < DIM / 32; ++h) {
           float o[32];
-          if (ok) tmem_ld32(o_at + 32 * h, o);
+          tmem_ld32(o_at + 32 * h, o);
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
-          if (real && ok) {
+          if (real) {
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
               float f[8];
@@ -505,11 +588,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        PromptSlot &slot = slots[2 * (2 * (int)blockIdx.x + (walk.k0 == 0 ? 1 : 0)) + i];
-#pragma unroll
+        PromptSlot &slot = slots[2 * (2 * (int)blockIdx.x + (head_part ? 1 : 0)) + i];
+#pragma unroll 1
         for (int h = 0; h < DIM / 32; ++h) {
           float o[32];
-          if (ok) tmem_ld32(o_at + 32 * h, o);
+          tmem_ld32(o_at + 32 * h, o);
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
@@ -522,6 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __stcg(&slot.l[row], l);
         if (row == 0) __stcg(&slot.vref, vref);
         __threadfence();
+      }
+      if (!whole) {
         wg_sync(1 + i);
         if (row == 0) {
           const unsigned parts = (unsigned)(last_cta - first_cta + 1);
@@ -538,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             top = fmaxf(top, __ldcg(&sl.m[row]));
             vmax = fmaxf(vmax, __ldcg(&sl.vref));
           }
+#pragma unroll 1
           for (int h = 0; h < DIM / 32; ++h) {
             float x[32];
 #pragma unroll

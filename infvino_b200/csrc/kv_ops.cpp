@@ -160,7 +160,7 @@ ivb::KvCache check_cache(const ivc_kv_cache *c) {
   need(c->pages > 0 && c->pages <= 0x7fffffffLL, "cache pages: 1 to 2^31 - 1");
   need(c->page_size > 0 && c->page_size % IVC_KV_BLOCK == 0 && c->page_size <= (1 << 20),
        "page_size is a multiple of IVC_KV_BLOCK");
-  need(c->kv_heads > 0 && c->kv_heads <= 1024, "kv_heads: 1 to 1024");
+  need(c->kv_heads > 0 && c->kv_heads <= 256, "kv_heads: 1 to 256");
   need(c->head_dim == 64 || c->head_dim == 128, "the cache's head_dim is 64 or 128");
   return ivb::KvCache{c->k, c->v, c->k_scale, c->v_scale, c->pages, c->page_size, c->kv_heads, c->head_dim};
 }
