@@ -38,7 +38,8 @@ constexpr int kKeys = 128, kTileBlocks = kKeys / kKvBlock;
 constexpr int kRows = 256;
 constexpr int kThreads = 512;
 constexpr int kMeta = 4;          // rings: scales of a tile live until both softmaxes are done
-constexpr float kSlack = 4.f, kBits = kWeightBits - kSlack;
+constexpr int kSub = 64;          // keys of a score tile: two in turn for each M tile and key tile
+constexpr float kSlack = 6.f, kBits = kWeightBits - kSlack;
 constexpr float kFarBelow = -40.f;  // value scales are taken as at least 2^-40 of the largest so far
 constexpr int kNoKey = 0x3fffffff;
 constexpr int kItemCost = 2;      // what an item costs besides its tiles, in tiles: queries in, outputs out
@@ -130,7 +131,7 @@ struct PromptShared {
   uint8_t k[2][kSlabs][kKeys * 128];
   uint8_t v[2][kSlabs][kKeys * 128];
   TileMeta meta[kMeta];
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], odone[2], qfull[2], drained;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2][2], pready[2][2], odone[2][2], qfull[2], drained;
   uint32_t tmem;
   volatile int abort;
   int last[2];
@@ -225,19 +226,13 @@ __device__ __forceinline__ uint32_t halves(uint32_t w) {
   return r;
 }
 
-// Sixteen codes of row r, from element 16 c, into a tile of halves.
-template <int DIM>
-__device__ __forceinline__ void put_codes(uint8_t *tile, int r, int c, uint4 w4) {
+// Sixteen codes as halves, to two 16-byte pieces of a row.
+__device__ __forceinline__ void put_codes(uint8_t *lo_at, uint8_t *hi_at, uint4 w4) {
   const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
-  const uint4 lo = make_uint4(halves<0x4140>(w[0]), halves<0x4342>(w[0]), halves<0x4140>(w[1]), halves<0x4342>(w[1]));
-  const uint4 hi = make_uint4(halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
-  uint8_t *row = tile + (c >> 2) * (128 * 128) + r * 128;
-  const int p = 2 * (c & 3), x = r & 7;
-  // lanes of the second 64 elements store their halves in the other order:
-  // eight lanes (a row) then meet eight different 16-byte banks
-  const bool swap = DIM == 128 && c >= 4;
-  *reinterpret_cast<uint4 *>(row + (((swap ? p + 1 : p) ^ x) << 4)) = swap ? hi : lo;
-  *reinterpret_cast<uint4 *>(row + (((swap ? p : p + 1) ^ x) << 4)) = swap ? lo : hi;
+  *reinterpret_cast<uint4 *>(lo_at) =
+      make_uint4(halves<0x4140>(w[0]), halves<0x4342>(w[0]), halves<0x4140>(w[1]), halves<0x4342>(w[1]));
+  *reinterpret_cast<uint4 *>(hi_at) =
+      make_uint4(halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
 }
 
 template <bool BF16, int DIM>
@@ -256,9 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&sh.vfull[i]), 4);
       mbar_init(smem_u32(&sh.kempty[i]), 1);
       mbar_init(smem_u32(&sh.vempty[i]), 1);
-      mbar_init(smem_u32(&sh.sfull[i]), 1);
-      mbar_init(smem_u32(&sh.odone[i]), 1);
-      mbar_init(smem_u32(&sh.pready[i]), 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_u32(&sh.sfull[i][h]), 1);
+        mbar_init(smem_u32(&sh.pready[i][h]), 4);
+        mbar_init(smem_u32(&sh.odone[i][h]), 1);
+      }
       mbar_init(smem_u32(&sh.qfull[i]), 4);
     }
     mbar_init(smem_u32(&sh.drained), 1);
@@ -370,8 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     reg_inc<184>();
     const int i = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + 128u * i, o_at = tmem + lanes + 256u + 128u * i;
-    const uint32_t sfull = smem_u32(&sh.sfull[i]), odone = smem_u32(&sh.odone[i]), pready = smem_u32(&sh.pready[i]);
+    const uint32_t o_at = tmem + lanes + 256u + 128u * i;
     int done = 0;   // tiles so far, all segments
     int tile = 0;   // tiles of both M tiles so far: the place of the scales
     bool ok = true;
@@ -454,118 +450,105 @@ __global__ void __launch_bounds__(kThreads, 1)
                       (long long)(walk.head * a.group + first_row + row - tok * a.group) * a.out.hs;
       float m = -INFINITY, l = 0.f, vref = 0.f;
       for (int t = 0; t < tiles; ++t, ++done, ++tile) {
-        if (!wait(sfull, done & 1, kStatusTimeoutAcc)) continue;
-        tc_fence_after();
         const TileMeta &me = sh.meta[tile % kMeta];
-        // hidden keys: behind the row, before its window, behind the end
-        bool masked = me.key0[kTileBlocks - 1] + kKvBlock - 1 > p_lo;
-        if (a.window > 0) {
-#pragma unroll
-          for (int b = 0; b < kTileBlocks; ++b)
-            masked = masked || (p_hi - me.key0[b] >= a.window && me.key0[b] + kKvBlock > a.sinks);
-        }
-        auto hide = [&](int c, float(&s)[32]) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k0 = me.key0[2 * c + h];
-            const int hi = p - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.window > 0 ? a.sinks - k0 : 0;
-#pragma unroll
-            for (int k = 0; k < kKvBlock; ++k)
-              if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * h + k] = -INFINITY;
-          }
-        };
-        // the scores are read twice, 32 columns at a time, the next 32 on
-        // their way: once for the maximum, once for the weights
-        float s0[32], s1[32];
-        float mx = -INFINITY;
-        auto factor = [&](int b) { return fmaxf(BF16 ? me.kc[b] * rf : me.kc[b], 0x1p-120f); };  // (never 0: hidden keys stay at -inf)
-        auto top32 = [&](int c, float(&s)[32]) {
-          if (masked) hide(c, s);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = s[kKvBlock * h];
-#pragma unroll
-            for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * h + k]);
-            mx = fmaxf(mx, x * factor(2 * c + h));
-          }
-        };
-        tmem_ld32(s_at, s0);
 #pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          tmem_ld_done(s0);
-          tmem_ld32(s_at + 32 * c + 32, s1);
-          top32(c, s0);
-          tmem_ld_done(s1);
-          tmem_ld32(s_at + (c == 0 ? 64 : 0), s0);
-          top32(c + 1, s1);
-        }
-        const float vr = me.vr;
-        vref = me.vref;
-        if (__any_sync(0xffffffffu, mx > m + kSlack) || vr != 1.f) {
-          const float top = fmaxf(m, mx);
-          const float f = top > m ? fast_exp2(m - top) : 1.f;
-          m = top;
-          l *= f;
-          if (t > 0) {
-            if (!wait(odone, (done - 1) & 1, kStatusTimeoutDrain)) continue;
-            tc_fence_after();
-            const float fo = f * vr;
-#pragma unroll 1
-            for (int h = 0; h < DIM / 32; ++h) {
-              float o[32];
-              tmem_ld32(o_at + 32 * h, o);
-              tmem_ld_wait();
-              uint32_t w[32];
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(smem_u32(&sh.sfull[i][h]), done & 1, kStatusTimeoutAcc)) continue;
+          tc_fence_after();
+          const uint32_t s_at = tmem + lanes + (uint32_t)(2 * i + h) * kSub;
+          float s[kSub];
+          tmem_ld32(s_at, s);
+          tmem_ld32(s_at + 32, s + 32);
+          const int b0 = 4 * h;  // its blocks
+          // hidden keys: behind the row, before its window, behind the end
+          bool masked = me.key0[b0 + 3] + kKvBlock - 1 > p_lo;
+          if (a.window > 0) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                asm volatile("" : "+f"(o[k]));
-                w[k] = __float_as_uint(o[k] * fo);
+            for (int b = 0; b < 4; ++b)
+              masked = masked || (p_hi - me.key0[b0 + b] >= a.window && me.key0[b0 + b] + kKvBlock > a.sinks);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < kSub; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
+          if (masked) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const int k0 = me.key0[b0 + b];
+              const int hi = p - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.window > 0 ? a.sinks - k0 : 0;
+#pragma unroll
+              for (int k = 0; k < kKvBlock; ++k)
+                if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * b + k] = -INFINITY;
+            }
+          }
+          float c[4], mx = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            c[b] = fmaxf(BF16 ? me.kc[b0 + b] * rf : me.kc[b0 + b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
+            float x = s[kKvBlock * b];
+#pragma unroll
+            for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
+            mx = fmaxf(mx, x * c[b]);
+          }
+          const float vr = h == 0 ? me.vr : 1.f;
+          vref = me.vref;
+          if (__any_sync(0xffffffffu, mx > m + kSlack) || vr != 1.f) {
+            const float top = fmaxf(m, mx);
+            const float f = top > m ? fast_exp2(m - top) : 1.f;
+            m = top;
+            l *= f;
+            if (t > 0 || h > 0) {
+              // the products before: the other half of the keys, of this tile or the last
+              if (!wait(smem_u32(&sh.odone[i][h ^ 1]), (h == 0 ? done - 1 : done) & 1, kStatusTimeoutDrain)) continue;
+              tc_fence_after();
+              const float fo = f * vr;
+#pragma unroll 1
+              for (int d = 0; d < DIM / 32; ++d) {
+                float o[32];
+                tmem_ld32(o_at + 32 * d, o);
+                tmem_ld_wait();
+                uint32_t w[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  asm volatile("" : "+f"(o[k]));
+                  w[k] = __float_as_uint(o[k] * fo);
+                }
+                tmem_st16(o_at + 32 * d, w);
+                tmem_st16(o_at + 32 * d + 16, w + 16);
               }
-              tmem_st16(o_at + 32 * h, w);
-              tmem_st16(o_at + 32 * h + 16, w + 16);
             }
           }
-        }
-        // weights 2^(s c - m + kBits) vs / vref, sums without the last factor
-        const float shift = m == -INFINITY ? 0.f : kBits - m;
-        auto weights32 = [&](int c, float(&s)[32]) {
-          if (masked) hide(c, s);
-          uint32_t w[16];
+          // weights 2^(s c - m + kBits) vs / vref, sums without the last factor
+          const float shift = m == -INFINITY ? 0.f : kBits - m;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int b = 2 * c + h;
-            const float f = factor(b), add = shift + me.lvf[b];
-            float2 sum = make_float2(0.f, 0.f);
+          for (int q = 0; q < 2; ++q) {
+            uint32_t w[16];
 #pragma unroll
-            for (int k = 0; k < kKvBlock; k += 2) {
-              float2 x = fma2(make_float2(s[kKvBlock * h + k], s[kKvBlock * h + k + 1]), make_float2(f, f), make_float2(add, add));
-              x.x = fast_exp2(x.x);
-              x.y = fast_exp2(x.y);
-              sum = add2(sum, x);
-              w[8 * h + k / 2] = pack2<false>(x.x, x.y);
+            for (int z = 0; z < 2; ++z) {
+              const int b = 2 * q + z;
+              const float f = c[b], add = shift + me.lvf[b0 + b];
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int k = 0; k < kKvBlock; k += 2) {
+                float2 x = fma2(make_float2(s[kKvBlock * b + k], s[kKvBlock * b + k + 1]), make_float2(f, f), make_float2(add, add));
+                x.x = fast_exp2(x.x);
+                x.y = fast_exp2(x.y);
+                sum = add2(sum, x);
+                w[8 * z + k / 2] = pack2<false>(x.x, x.y);
+              }
+              l = fmaf(sum.x + sum.y, me.ivf[b0 + b], l);
             }
-            l = fmaf(sum.x + sum.y, me.ivf[b], l);
+            tmem_st16(s_at + 16 * q, w);
           }
-          tmem_st16(s_at + 16 * c, w);  // (columns whose scores have been read)
-        };
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          tmem_ld_done(s0);
-          tmem_ld32(s_at + 32 * c + 32, s1);
-          weights32(c, s0);
-          tmem_ld_done(s1);
-          if (c == 0) tmem_ld32(s_at + 64, s0);
-          weights32(c + 1, s1);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.pready[i][h]));
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pready);
       }
 
       // ---- O
       more = advance();
-      wait(odone, (done - 1) & 1, kStatusTimeoutDrain);
+      wait(smem_u32(&sh.odone[i][1]), (done - 1) & 1, kStatusTimeoutDrain);
       tc_fence_after();
       if (!ok) {  // (the slot keeps whatever it holds: the status word says that the result is not valid)
       } else if (whole) {
@@ -656,10 +639,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < 12) {
     // ------------------------------------------------------------ codes to halves
     reg_dec<96>();
-    constexpr int kParts = DIM / 16;        // 16-code pieces of a row
-    constexpr int kStep = 32 / kParts;      // rows a warp takes at once
-    constexpr int kEach = 32 / kStep;       // pieces a lane holds of the warp's 32 rows
-    const int w = warp - 8, c = lane % kParts, r_in = lane / kParts;
+    // A warp takes 32 rows (two blocks): eight rows of 64 elements at once, a
+    // lane sixteen codes of one.  (Eight lanes, two rows, meet eight different
+    // 16-byte banks when they store.)
+    constexpr int kEach = 4 * kSlabs;
+    const int w = warp - 8, c = lane & 3, r8 = lane >> 2;
+    const uint32_t put_lo = (uint32_t)((32 * w + r8) * 128 + (((2 * c) ^ r8) << 4)),
+                   put_hi = (uint32_t)((32 * w + r8) * 128 + (((2 * c + 1) ^ r8) << 4));
     const float kc_all = fabsf(a.scale) * kLog2e;
     uint4 kreg[kEach], vreg[kEach];
     int tile = 0;
@@ -669,25 +655,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       return ok;
     };
     float vref = 0.f;
-    // lane j < 8 knows block j of a tile: where its codes are, its scales
+    // Lane j < 8 knows block j of a tile: where its codes are, its scales.  The
+    // page number is asked for a tile before the place and the scales, and
+    // those a tile before the codes, so that no look-up waits for another.
     struct Blocks {
       long long at;
       int key0;
       float ks, vs;
     };
-    auto look_up = [&](int t) {
-      Blocks x{-1, kNoKey, 0.f, 0.f};
+    int key_next = kNoKey, page_next = -1;
+    auto ask_page = [&](int t) {
       const int bi = t * kTileBlocks + lane;
+      key_next = kNoKey;
       if (lane < kTileBlocks && t < walk.k1 && bi < walk.r.blocks) {
-        const int key = (bi < walk.r.sink_blocks ? bi : bi - walk.r.sink_blocks + walk.r.first_block) * kKvBlock;
-        const int page = kv_page_of(a.cache, a.seqs, walk.b, key, a.status);
-        if (page >= 0) {
-          const int slot = key % a.cache.page;
-          x.key0 = key;
-          x.at = kv_code_at(a.cache, page, walk.head, slot);
-          const long long sa = kv_scale_at(a.cache, page, walk.head, slot);
+        key_next = (bi < walk.r.sink_blocks ? bi : bi - walk.r.sink_blocks + walk.r.first_block) * kKvBlock;
+        page_next = a.seqs.pages[(long long)walk.b * a.seqs.pps + key_next / a.cache.page];  // (in the row: kv_span has checked)
+      }
+    };
+    auto look_up = [&]() {
+      Blocks x{-1, kNoKey, 0.f, 0.f};
+      if (key_next != kNoKey) {
+        if ((unsigned)page_next < (unsigned long long)a.cache.pages) {
+          const int slot = key_next % a.cache.page;
+          x.key0 = key_next;
+          x.at = kv_code_at(a.cache, page_next, walk.head, slot);
+          const long long sa = kv_scale_at(a.cache, page_next, walk.head, slot);
           x.ks = a.cache.ks[sa];
           x.vs = a.cache.vs[sa];
+        } else {
+          kv_flag(a.status, kStatusKvPage);
         }
       }
       return x;
@@ -695,15 +691,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto load = [&](const int8_t *codes, const Blocks &x, uint4(&reg)[kEach]) {
       const long long at0 = __shfl_sync(0xffffffffu, x.at, 2 * w), at1 = __shfl_sync(0xffffffffu, x.at, 2 * w + 1);
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int r = e * kStep + r_in;  // of the warp's 32: blocks 2 w and 2 w + 1
-        const long long at = e * kStep < kKvBlock ? at0 : at1;
-        reg[e] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(codes + at + (r & 15) * DIM + 16 * c)) : make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < kEach; ++e) {  // rows 8 (e % 4).., slab e / 4
+        const long long at = e % 4 < 2 ? at0 : at1;
+        reg[e] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(codes + at + (8 * (e % 2) + r8) * DIM + 64 * (e / 4) + 16 * c))
+                         : make_uint4(0, 0, 0, 0);
       }
     };
     while (walk.next(a)) {
       vref = 0.f;
-      Blocks now = look_up(walk.k0), ahead = look_up(walk.k0 + 1);
+      ask_page(walk.k0);
+      Blocks now = look_up();
+      ask_page(walk.k0 + 1);
+      Blocks ahead = look_up();
+      ask_page(walk.k0 + 2);
       load(a.cache.k, now, kreg);
       load(a.cache.v, now, vreg);
       for (int t = walk.k0; t < walk.k1; ++t, ++tile) {
@@ -717,10 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           vmax = fmaxf(vref, __shfl_sync(0xffffffffu, vmax, 0));
           TileMeta &me = sh.meta[tile % kMeta];
           if (lane < kTileBlocks) {
-            const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(log2f(now.vs) - log2f(vmax), kFarBelow) : kFarBelow;
+            const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(__log2f(now.vs) - __log2f(vmax), kFarBelow) : kFarBelow;
             me.kc[lane] = now.ks * kc_all;
             me.lvf[lane] = lv;
-            me.ivf[lane] = exp2f(-lv);
+            me.ivf[lane] = fast_exp2(-lv);
             me.key0[lane] = now.key0;
           }
           if (lane == 0) {
@@ -730,20 +730,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           vref = vmax;
         }
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) put_codes<DIM>(&sh.k[st][0][0], 32 * w + e * kStep + r_in, c, kreg[e]);
+        for (int e = 0; e < kEach; ++e)
+          put_codes(&sh.k[st][e / 4][put_lo + 1024 * (e % 4)], &sh.k[st][e / 4][put_hi + 1024 * (e % 4)], kreg[e]);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.kfull[st]));
         load(a.cache.k, ahead, kreg);
         if (reused) wait(smem_u32(&sh.vempty[st]), ((tile >> 1) - 1) & 1);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) put_codes<DIM>(&sh.v[st][0][0], 32 * w + e * kStep + r_in, c, vreg[e]);
+        for (int e = 0; e < kEach; ++e)
+          put_codes(&sh.v[st][e / 4][put_lo + 1024 * (e % 4)], &sh.v[st][e / 4][put_hi + 1024 * (e % 4)], vreg[e]);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.vfull[st]));
         load(a.cache.v, ahead, vreg);
         now = ahead;
-        ahead = look_up(t + 2);
+        ahead = look_up();
+        ask_page(t + 3);
       }
     }
   } else {
@@ -751,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 12) {
       // ---------------------------------------------------------- products
       const bool leader = elect_one();
-      const uint32_t idesc_s = idesc_f16_f32(128, kKeys);
+      const uint32_t idesc_s = idesc_f16_f32(128, kSub);
       const uint32_t idesc_o = idesc_f16_f32(128, DIM) | (1u << 16);  // V: rows are keys (its N side is dense)
       const uint64_t qd = smem_desc_kmajor(smem_u32(&sh.q[0][0][0]), 128), kd = smem_desc_kmajor(smem_u32(&sh.k[0][0][0]), 128);
       // V: 64 head elements a row of 128 bytes; 8 keys 1024 bytes on, the next 64 elements a slab on
@@ -764,29 +767,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
         return ok;
       };
-      auto scores = [&](int i, int st, bool last) {
+      // (64 keys are 8192 bytes on in the keys' and the values' tiles)
+      auto scores = [&](int i, int h, int st, bool last) {
         tc_fence_after();
         if (leader) {
-          const uint32_t q_lo = (uint32_t)qd + (uint32_t)i * kTileUnits, k_lo = (uint32_t)kd + (uint32_t)st * kTileUnits;
+          const uint32_t q_lo = (uint32_t)qd + (uint32_t)i * kTileUnits, k_lo = (uint32_t)kd + (uint32_t)st * kTileUnits + 512u * h;
 #pragma unroll
           for (int k = 0; k < DIM / 16; ++k) {
             const uint32_t o = (uint32_t)(k >> 2) * kSlabUnits + 2u * (k & 3);
-            umma_f16_lh(tmem + 128u * i, q_lo + o, (uint32_t)(qd >> 32), k_lo + o, (uint32_t)(kd >> 32), idesc_s, k > 0);
+            umma_f16_lh(tmem + (uint32_t)(2 * i + h) * kSub, q_lo + o, (uint32_t)(qd >> 32), k_lo + o, (uint32_t)(kd >> 32), idesc_s, k > 0);
           }
-          umma_commit(smem_u32(&sh.sfull[i]));
+          umma_commit(smem_u32(&sh.sfull[i][h]));
           if (last) umma_commit(smem_u32(&sh.kempty[st]));
         }
         __syncwarp();
       };
-      auto values = [&](int i, int st, bool begin, bool last) {
+      auto values = [&](int i, int h, int st, bool begin, bool last) {
         tc_fence_after();
         if (leader) {
-          const uint32_t v_lo = (uint32_t)vd + (uint32_t)st * kTileUnits;
+          const uint32_t v_lo = (uint32_t)vd + (uint32_t)st * kTileUnits + 512u * h;
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_f16_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * k, v_lo + (2048u / 16u) * k, (uint32_t)(vd >> 32), idesc_o,
-                        !begin || k > 0);
-          umma_commit(smem_u32(&sh.odone[i]));
+          for (int k = 0; k < kSub / 16; ++k)
+            umma_f16_ts(tmem + 256u + 128u * i, tmem + (uint32_t)(2 * i + h) * kSub + 8u * k, v_lo + (2048u / 16u) * k,
+                        (uint32_t)(vd >> 32), idesc_o, !begin || k > 0);
+          umma_commit(smem_u32(&sh.odone[i][h]));
           if (last) umma_commit(smem_u32(&sh.vempty[st]));
         }
         __syncwarp();
@@ -796,21 +800,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int m_tiles = walk.s.n * a.group - walk.rt * kRows > 128 ? 2 : 1;
         if (!ok) break;
         wait(smem_u32(&sh.kfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
-        for (int i = 0; i < m_tiles && ok; ++i) {
-          if (wait(smem_u32(&sh.qfull[i]), seg[i] & 1, kStatusTimeoutFull)) scores(i, tile & 1, i == m_tiles - 1);
-          ++seg[i];
-        }
-        for (int t = 0; t < tiles && ok; ++t, ++tile) {
+        for (int h = 0; h < 2 && ok; ++h)
           for (int i = 0; i < m_tiles && ok; ++i) {
-            if (i == 0) wait(smem_u32(&sh.vfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
-            if (!wait(smem_u32(&sh.pready[i]), done[i] & 1, kStatusTimeoutAccEmpty)) break;
-            values(i, tile & 1, t == 0, i == m_tiles - 1);
-            ++done[i];
-            if (t + 1 < tiles) {
-              if (i == 0) wait(smem_u32(&sh.kfull[(tile + 1) & 1]), ((tile + 1) >> 1) & 1, kStatusTimeoutFull);
-              if (ok) scores(i, (tile + 1) & 1, i == m_tiles - 1);
-            }
+            if (h == 0) wait(smem_u32(&sh.qfull[i]), seg[i]++ & 1, kStatusTimeoutFull);
+            if (ok) scores(i, h, tile & 1, h == 1 && i == m_tiles - 1);
           }
+        for (int t = 0; t < tiles && ok; ++t, ++tile) {
+          const int st = tile & 1, nx = st ^ 1;
+          wait(smem_u32(&sh.vfull[st]), (tile >> 1) & 1, kStatusTimeoutFull);
+          for (int h = 0; h < 2 && ok; ++h)
+            for (int i = 0; i < m_tiles && ok; ++i) {
+              const bool last = h == 1 && i == m_tiles - 1;
+              if (!wait(smem_u32(&sh.pready[i][h]), done[i] & 1, kStatusTimeoutAccEmpty)) break;
+              values(i, h, st, t == 0 && h == 0, last);
+              if (t + 1 < tiles) {
+                if (h == 0 && i == 0) wait(smem_u32(&sh.kfull[nx]), ((tile + 1) >> 1) & 1, kStatusTimeoutFull);
+                if (ok) scores(i, h, nx, last);
+              }
+            }
+          for (int i = 0; i < m_tiles; ++i) ++done[i];
         }
       }
       // every product retires before TMEM is released
