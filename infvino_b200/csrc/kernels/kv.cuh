@@ -5,6 +5,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include "conv_tc.cuh"  // FastDiv
+
 namespace ivb {
 
 constexpr int kKvBlock = 16;       // tokens that share a scale
@@ -50,6 +52,7 @@ struct KvAttend {
   float scale;
   int window, sinks;
   int *status;
+  FastDiv by_group, by_page;
 };
 
 struct KvRopeFreq {

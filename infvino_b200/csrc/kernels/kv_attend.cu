@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
             if (key < s.len) {
               const int page = kv_page_of(a.cache, a.seqs, b, key, a.status);
               if (page >= 0) {
-                const int slot = key % a.cache.page;
+                const int slot = key - fast_div(key, a.by_page) * a.cache.page;
                 where = kv_code_at(a.cache, page, head, slot);
                 const long long sa = kv_scale_at(a.cache, page, head, slot);
                 sc_mine = make_float2(a.cache.ks[sa], a.cache.vs[sa]);
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
     float rs[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int r = rt * kRows + 8 * t + g, i = r / a.group;
+      const int r = rt * kRows + 8 * t + g, i = fast_div(r, a.by_group);
       const uint16_t *row = static_cast<const uint16_t *>(a.q.p) + (long long)(s.first + i) * a.q.ts +
                             (long long)(head * a.group + r - i * a.group) * a.q.hs;
       uint32_t w[2 * kTiles];
@@ -273,13 +273,13 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
       for (int k = 0; k < kTiles; ++k) q[t][k][0] = w[2 * k], q[t][k][1] = w[2 * k + 1];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int rc = rt * kRows + 8 * t + 2 * t4 + c, ic = rc / a.group;
+        const int rc = rt * kRows + 8 * t + 2 * t4 + c, ic = fast_div(rc, a.by_group);
         pos[t][c] = ic < s.n ? s.len - s.n + ic : -1;
         rs[t][c] = BF16 ? __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4) : up;  // (lane of column 2 t4 + c)
       }
     }
-    const int p_lo = s.len - s.n + rt * kRows / a.group;                                  // first row's position
-    const int p_hi = s.len - s.n + min(s.n - 1, (rt * kRows + kRows - 1) / a.group);      // last row's
+    const int p_lo = s.len - s.n + fast_div(rt * kRows, a.by_group);                                  // first row's position
+    const int p_hi = s.len - s.n + min(s.n - 1, fast_div(rt * kRows + kRows - 1, a.by_group));      // last row's
 
     float acc[NT][kTiles][4];
     float m[NT][2], l[NT][2];
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
             for (int k = 0; k < 8; ++k) x[k] += __ldcg(&sl.acc[(i0 + k) * 32 + ln]) * wv;
           }
         }
-        const int row = rt * kRows + r, i = row / a.group;
+        const int row = rt * kRows + r, i = fast_div(row, a.by_group);
         if (i < s.n) {
           const float y = sum != 0.f ? vr / sum : 0.f;  // (a NaN sum stays NaN)
 #pragma unroll

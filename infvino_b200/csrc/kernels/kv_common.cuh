@@ -33,24 +33,29 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Eight consecutive 16-bit elements; element by element where the row is not on 16 bytes.
+// Eight consecutive 16-bit elements; element by element (a small loop, so that
+// every use does not carry eight copies) where the row is not on 16 bytes.
 __device__ __forceinline__ uint4 load8(const uint16_t *p, bool vec) {
   if (vec) return *reinterpret_cast<const uint4 *>(p);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+  for (int i = 7; i >= 0; --i) {
+    hi = (hi << 16) | (lo >> 48);
+    lo = (lo << 16) | p[i];
+  }
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 __device__ __forceinline__ void store8(uint16_t *p, uint4 u, bool vec) {
   if (vec) {
     *reinterpret_cast<uint4 *>(p) = u;
     return;
   }
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p[2 * i] = (uint16_t)w[i];
-    p[2 * i + 1] = (uint16_t)(w[i] >> 16);
+  uint64_t lo = u.x | ((uint64_t)u.y << 32), hi = u.z | ((uint64_t)u.w << 32);
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    p[i] = (uint16_t)lo;
+    lo = (lo >> 16) | (hi << 48);
+    hi >>= 16;
   }
 }
 template <bool BF16>
@@ -90,6 +95,10 @@ __device__ __forceinline__ int kv_page_of(const KvCache &c, const KvSeqs &s, int
     return -1;
   }
   return page;
+}
+
+__device__ __forceinline__ int fast_div(int n, FastDiv f) {  // (0 <= n < 2^31)
+  return (int)(((uint64_t)(uint32_t)n * f.m) >> (31u + f.s));
 }
 
 // How many sequences end at or before packed token t (= the sequence t is in),

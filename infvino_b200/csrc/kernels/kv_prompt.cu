@@ -37,6 +37,7 @@ namespace {
 constexpr int kKeys = 128, kTileBlocks = kKeys / kKvBlock;
 constexpr int kRows = 256;
 constexpr int kThreads = 512;
+constexpr int kSegments = 4;      // ring of segments
 constexpr int kMeta = 4;          // rings: scales of a tile live until both softmaxes are done
 constexpr int kSub = 64;          // keys of a score tile: two in turn for each M tile and key tile
 constexpr float kSlack = 6.f, kBits = kWeightBits - kSlack;
@@ -45,7 +46,7 @@ constexpr int kNoKey = 0x3fffffff;
 constexpr int kItemCost = 2;      // what an item costs besides its tiles, in tiles: queries in, outputs out
 constexpr int kMaxSeqs = 8192;    // sequences of a call that the start-up scan has room for
 
-struct TileMeta {
+struct alignas(16) TileMeta {
   float kc[kTileBlocks];    // ks * |scale| * log2 e
   float lvf[kTileBlocks];   // log2 (vs / vref)
   float ivf[kTileBlocks];   // vref / vs
@@ -60,7 +61,7 @@ struct RowSpan {
 };
 __device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, int rt) {
   RowSpan s;
-  const int i0 = rt * kRows / a.group, i1 = min(n - 1, (rt * kRows + kRows - 1) / a.group);
+  const int i0 = fast_div(rt * kRows, a.by_group), i1 = min(n - 1, fast_div(rt * kRows + kRows - 1, a.by_group));
   const int p_lo = len - n + i0, p_hi = len - n + i1;
   const int all = p_hi >= 0 ? p_hi / kKvBlock + 1 : 0;
   s.first_block = s.sink_blocks = 0;
@@ -74,53 +75,13 @@ __device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, i
   return s;
 }
 
-// The CTA's share of the units, segment after segment.  Every warp walks it by
-// itself, with its place in shared memory (registers are the softmax's).
-struct Walk {
-  long long u, u_end, base, total;  // base: first unit of (b, rt)
-  int ctas, b, rt;
+// A piece of an item: tiles k0 .. k1 - 1 of rows 256 rt .. of sequence b, one kv head.
+struct Segment {
+  int more;                  // 0: there is none, the share is done
+  int b, rt, head, k0, k1;
+  int first_cta, last_cta;   // the CTAs that have tiles of the item
   KvSpan s;
-  // the segment
   RowSpan r;
-  int row_tiles, head, k0, k1, first_cta, last_cta;
-
-  // One warp's step, by its lane 0.
-  __device__ __forceinline__ bool next(const KvAttend &a) {
-    __syncwarp();
-    bool more = false;
-    if ((threadIdx.x & 31) == 0) more = advance(a);
-    return __shfl_sync(0xffffffffu, more, 0);  // (and the place is the warp's to read)
-  }
-  __device__ __forceinline__ bool advance(const KvAttend &a) {
-    while (u < u_end) {
-      const int each = r.tiles + kItemCost;
-      const long long units = (long long)each * a.cache.heads;
-      if (s.n > 0 && u < base + units) {
-        head = (int)((uint32_t)(u - base) / (uint32_t)each);  // (tiles < 2^24, heads at most 2^8)
-        const long long item = base + (long long)head * each, end = min(u_end, item + each);
-        k0 = max(0, (int)(u - item) - kItemCost);
-        k1 = (int)(end - item) - kItemCost;
-        u = end;
-        if (k1 <= k0) continue;  // the share ends before the item's first tile
-        first_cta = last_cta = 0;
-        if (!whole()) {
-          first_cta = share_of(total, ctas, item + kItemCost);
-          last_cta = share_of(total, ctas, item + each - 1);
-        }
-        return true;
-      }
-      if (s.n > 0) base += units;
-      if (s.n > 0 && rt + 1 < row_tiles) {
-        ++rt;
-      } else {
-        rt = 0;
-        s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
-        row_tiles = (s.n * a.group + kRows - 1) / kRows;
-      }
-      if (s.n > 0) r = row_span(a, s.n, s.len, rt);
-    }
-    return false;
-  }
   __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == r.tiles; }
 };
 
@@ -135,7 +96,8 @@ struct PromptShared {
   uint32_t tmem;
   volatile int abort;
   int last[2];
-  Walk walks[13];  // softmax, codes, products: a warp each
+  Segment seg[kSegments];  // written by warp 13, read by the 13 warps that work
+  uint64_t segfull[kSegments], segempty[kSegments];
   long long scan[kThreads / 32];
   long long base;
   int seq, rt;
@@ -147,6 +109,9 @@ struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 row
   float vref;
   float pad[31];
 };
+
+// The lowest n of 16 bits.
+__device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; }
 
 __device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -170,11 +135,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float *r) {
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : KV_R8(r, 0), KV_R8(r, 8), KV_R8(r, 16), KV_R8(r, 24)
       : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld_done(float (&r)[32]) {
-  tmem_ld_wait();
-#pragma unroll
-  for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(r[k]));  // uses stay after the wait
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
@@ -258,6 +218,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mbar_init(smem_u32(&sh.qfull[i]), 4);
     }
+    for (int i = 0; i < kSegments; ++i) {
+      mbar_init(smem_u32(&sh.segfull[i]), 1);
+      mbar_init(smem_u32(&sh.segempty[i]), 13);
+    }
     mbar_init(smem_u32(&sh.drained), 1);
     sh.abort = 0;
     fence_mbar_init();
@@ -271,16 +235,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ---- all units, and where this CTA's share begins.  A warp adds up a
   // sequence's row tiles; the sequences' sums wait where the tiles will be.
   long long *sums = reinterpret_cast<long long *>(&sh.q[0][0][0]);
+#pragma unroll 1
   for (int b0 = warp * 32; b0 < a.seqs.batch; b0 += kThreads) {
     int n = 0, len = 0;
     if (b0 + lane < a.seqs.batch) {
       const KvSpan s = kv_span(a, b0 + lane);
       n = s.n, len = s.len;
     }
+#pragma unroll 1
     for (int j = 0; j < min(32, a.seqs.batch - b0); ++j) {
       const int nj = __shfl_sync(0xffffffffu, n, j), lj = __shfl_sync(0xffffffffu, len, j);
       const int rts = (nj * a.group + kRows - 1) / kRows;
       long long sum = 0;
+#pragma unroll 1
       for (int rt = lane; rt < rts; rt += 32) sum += row_span(a, nj, lj, rt).tiles + kItemCost;
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -291,6 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per = (a.seqs.batch + kThreads - 1) / kThreads;
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
   long long mine = 0;
+#pragma unroll 1
   for (int b = b_lo; b < b_hi; ++b) mine += sums[b];
   long long incl = mine;
 #pragma unroll
@@ -305,11 +273,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
-  // (a share is at least an item's cost and a tile, or no CTA would have the tiles between two of them)
-  const long long most = max(1LL, total / (kItemCost + 1));
-  const int ctas = total == 0 ? 0 : (int)(most < (long long)gridDim.x ? most : (long long)gridDim.x);
-  const bool works = (int)blockIdx.x < ctas;
-  const long long u = works ? share_begin(total, ctas, blockIdx.x) : 0;
+  // (2^31 units would be hours of work; they are counted in 32 bits from here)
+  if (total == 0 || total > 0x7fffffffLL) {
+    if (threadIdx.x == 0 && total) kv_flag(a.status, kStatusKvSeqs);
+  }
+  const bool sane = total > 0 && total <= 0x7fffffffLL;
+  // (a share is more than an item's cost, or no CTA would have the tiles between two of them)
+  const uint32_t size = sane ? max((uint32_t)kItemCost + 1, ((uint32_t)total + gridDim.x - 1) / gridDim.x) : 1u;
+  const bool works = sane && blockIdx.x * size < (uint32_t)total;
+  const uint32_t u_begin = works ? blockIdx.x * size : 0u;
+  const long long u = u_begin;
   const long long excl = before + incl - mine;
   if (works && u >= excl && u < excl + mine) {
     long long at = excl;
@@ -323,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const KvSpan s = kv_span(a, sh.seq);
     const int rts = (s.n * a.group + kRows - 1) / kRows;
     long long at = sh.base;
+#pragma unroll 1
     for (int r0 = 0; r0 < rts; r0 += 32) {
       long long w = r0 + lane < rts ? (long long)(row_span(a, s.n, s.len, r0 + lane).tiles + kItemCost) * a.cache.heads : 0;
       long long in = w;
@@ -345,22 +319,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  Walk &walk = sh.walks[min(warp, 12)];
-  if (lane == 0 && warp < 13) {
-    walk.total = total;
-    walk.ctas = ctas;
-    walk.u = u;
-    walk.u_end = works ? share_begin(total, ctas, blockIdx.x + 1) : 0;
-    if (works) {
-      walk.b = sh.seq;
-      walk.rt = sh.rt;
-      walk.base = sh.base;
-      walk.s = kv_span(a, walk.b);
-      walk.row_tiles = (walk.s.n * a.group + kRows - 1) / kRows;
-      walk.r = row_span(a, walk.s.n, walk.s.len, walk.rt);
-    }
-  }
   __syncthreads();  // the sums' room is the tiles' from here on
+
+  // Waits as a warp.  A wait that is over already costs one test.
+  bool ok = true;
+  auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+    if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
+    return ok;
+  };
+  // A working warp's next segment: leaves the one it has (what it still needs
+  // of it is in registers) and waits for the next.
+  int seg_n = 0;
+  auto next_segment = [&]() -> const Segment * {
+    __syncwarp();
+    if (seg_n > 0 && lane == 0) mbar_arrive(smem_u32(&sh.segempty[(seg_n - 1) % kSegments]));
+    const int at = seg_n % kSegments;
+    wait(smem_u32(&sh.segfull[at]), (seg_n / kSegments) & 1, kStatusTimeoutFull);
+    ++seg_n;
+    return ok && sh.seg[at].more ? &sh.seg[at] : nullptr;
+  };
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax of M tile i
@@ -370,26 +348,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_at = tmem + lanes + 256u + 128u * i;
     int done = 0;   // tiles so far, all segments
     int tile = 0;   // tiles of both M tiles so far: the place of the scales
-    bool ok = true;
-    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
-      return ok;
-    };
+    const Segment *g = nullptr;
     // ---- the warp's 32 query rows of the walk's segment: halves, K-major.
     // DIM / 8 lanes a row; rf of a row's owner is what its halves were divided by.
     float rf = 1.f;
     auto load_q = [&]() {
       constexpr int kLanes = DIM / 8, kAtOnce = 32 / kLanes;
-      const int c = lane % kLanes, first_row = walk.rt * kRows + 128 * i + 32 * (warp & 3);
-      const int all_rows = walk.s.n * a.group, head0 = walk.head * a.group;
+      const int c = lane % kLanes, first_row = g->rt * kRows + 128 * i + 32 * (warp & 3);
+      const int all_rows = g->s.n * a.group, head0 = g->head * a.group;
       const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // |scale| is in the keys' factor
-      const uint16_t *src = static_cast<const uint16_t *>(a.q.p) + (long long)walk.s.first * a.q.ts + 8 * c;
+      const uint16_t *src = static_cast<const uint16_t *>(a.q.p) + (long long)g->s.first * a.q.ts + 8 * c;
 #pragma unroll 1
       for (int e0 = 0; e0 < kLanes; e0 += 8) {
         uint4 w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int r = first_row + (e0 + e) * kAtOnce + lane / kLanes, tok = r / a.group;
+          const int r = first_row + (e0 + e) * kAtOnce + lane / kLanes, tok = fast_div(r, a.by_group);
           w[e] = r < all_rows ? load8(src + (long long)tok * a.q.ts + (long long)(head0 + r - tok * a.group) * a.q.hs, a.q.vec)
                               : make_uint4(0, 0, 0, 0);
         }
@@ -426,29 +400,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the next segment with rows for this M tile; its queries follow at once,
     // before the outputs of the one that is ending
     auto advance = [&]() {
-      while (walk.next(a)) {
-        if (walk.s.n * a.group > walk.rt * kRows + 128 * i) {
+      while ((g = next_segment())) {
+        if (g->s.n * a.group > g->rt * kRows + 128 * i) {
           load_q();
           return true;
         }
-        tile += walk.k1 - walk.k0;
+        tile += g->k1 - g->k0;
       }
       return false;
     };
     bool more = advance();
     while (more) {
-      const int first_row = walk.rt * kRows + 128 * i, rows = min(128, walk.s.n * a.group - first_row);
-      const int tiles = walk.k1 - walk.k0;
-      const int tok = (first_row + row) / a.group;
+      const int first_row = g->rt * kRows + 128 * i, rows = min(128, g->s.n * a.group - first_row);
+      const int tiles = g->k1 - g->k0;
+      const int tok = fast_div(first_row + row, a.by_group);
       const bool real = row < rows;
-      const int p = real ? walk.s.len - walk.s.n + tok : -1;
-      const int p_lo = walk.s.len - walk.s.n + first_row / a.group;
-      const int p_hi = walk.s.len - walk.s.n + (first_row + rows - 1) / a.group;
-      const bool whole = walk.whole(), head_part = walk.k0 == 0;
-      const int first_cta = walk.first_cta, last_cta = walk.last_cta;
-      uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(walk.s.first + tok) * a.out.ts +
-                      (long long)(walk.head * a.group + first_row + row - tok * a.group) * a.out.hs;
+      const int p = real ? g->s.len - g->s.n + tok : -1;
+      const int p_lo = g->s.len - g->s.n + fast_div(first_row, a.by_group);
+      const int p_hi = g->s.len - g->s.n + fast_div(first_row + rows - 1, a.by_group);
+      const bool whole = g->whole(), head_part = g->k0 == 0;
+      const int first_cta = g->first_cta, last_cta = g->last_cta;
+      uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(g->s.first + tok) * a.out.ts +
+                      (long long)(g->head * a.group + first_row + row - tok * a.group) * a.out.hs;
+      // parts (of four blocks) that need no look at single keys: up to part_hi
+      // every row sees the end of it, from part_lo on every row its beginning
+      // (or, before part_sink, all of it are sinks)
+      const RowSpan &rs = g->r;
+      const int part_hi = ((p_lo + 1) / kKvBlock + rs.sink_blocks - rs.first_block) / 4 - 1;
+      int part_lo = 0, part_sink = 0;
+      if (a.window > 0 && p_hi >= a.window) {
+        part_lo = ((p_hi - a.window) / kKvBlock + 1 - rs.first_block + rs.sink_blocks + 3) / 4;
+        part_sink = min(rs.sink_blocks, a.sinks / kKvBlock) / 4;
+      }
+      int part = 2 * g->k0;
       float m = -INFINITY, l = 0.f, vref = 0.f;
+#pragma unroll 1
       for (int t = 0; t < tiles; ++t, ++done, ++tile) {
         const TileMeta &me = sh.meta[tile % kMeta];
 #pragma unroll 1
@@ -460,30 +446,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(s_at, s);
           tmem_ld32(s_at + 32, s + 32);
           const int b0 = 4 * h;  // its blocks
-          // hidden keys: behind the row, before its window, behind the end
-          bool masked = me.key0[b0 + 3] + kKvBlock - 1 > p_lo;
-          if (a.window > 0) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              masked = masked || (p_hi - me.key0[b0 + b] >= a.window && me.key0[b0 + b] + kKvBlock > a.sinks);
-          }
+          const bool masked = part > part_hi || (part < part_lo && part >= part_sink);
+          ++part;
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < kSub; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
-          if (masked) {
+          if (masked) {  // hidden keys: behind the row, before its window, behind the end
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-              const int k0 = me.key0[b0 + b];
-              const int hi = p - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.window > 0 ? a.sinks - k0 : 0;
+              const int hi = p - me.key0[b0 + b];
+              uint32_t seen = low_bits(hi + 1);
+              if (a.window > 0) seen &= ~low_bits(hi - a.window + 1) | low_bits(a.sinks - me.key0[b0 + b]);
 #pragma unroll
               for (int k = 0; k < kKvBlock; ++k)
-                if (k > hi || (k <= lo && k >= sk)) s[kKvBlock * b + k] = -INFINITY;
+                if (!(seen >> k & 1)) s[kKvBlock * b + k] = -INFINITY;
             }
           }
-          float c[4], mx = -INFINITY;
+          const float4 kc4 = *reinterpret_cast<const float4 *>(&me.kc[b0]);
+          const float4 lv4 = *reinterpret_cast<const float4 *>(&me.lvf[b0]), iv4 = *reinterpret_cast<const float4 *>(&me.ivf[b0]);
+          float c[4] = {kc4.x, kc4.y, kc4.z, kc4.w}, mx = -INFINITY;
+          const float lvf[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, ivf[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            c[b] = fmaxf(BF16 ? me.kc[b0 + b] * rf : me.kc[b0 + b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
+            c[b] = fmaxf(BF16 ? c[b] * rf : c[b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
             float x = s[kKvBlock * b];
 #pragma unroll
             for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
@@ -525,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const int b = 2 * q + z;
-              const float f = c[b], add = shift + me.lvf[b0 + b];
+              const float f = c[b], add = shift + lvf[b];
               float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
               for (int k = 0; k < kKvBlock; k += 2) {
@@ -535,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum = add2(sum, x);
                 w[8 * z + k / 2] = pack2<false>(x.x, x.y);
               }
-              l = fmaf(sum.x + sum.y, me.ivf[b0 + b], l);
+              l = fmaf(sum.x + sum.y, ivf[b], l);
             }
             tmem_st16(s_at + 16 * q, w);
           }
@@ -601,6 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         wg_sync(1 + i);
         if (sh.last[i] && real && ok) {
           float top = -INFINITY, vmax = 0.f, sum = 0.f;
+#pragma unroll 1
           for (int z = first_cta; z <= last_cta; ++z) {
             const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
             top = fmaxf(top, __ldcg(&sl.m[row]));
@@ -612,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) x[k] = 0.f;
             sum = 0.f;
+#pragma unroll 1
             for (int z = first_cta; z <= last_cta; ++z) {
               const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
               const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]);
@@ -649,11 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float kc_all = fabsf(a.scale) * kLog2e;
     uint4 kreg[kEach], vreg[kEach];
     int tile = 0;
-    bool ok = true;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, kStatusTimeoutEmpty, kLimit));
-      return ok;
-    };
+    const Segment *g = nullptr;
     float vref = 0.f;
     // Lane j < 8 knows block j of a tile: where its codes are, its scales.  The
     // page number is asked for a tile before the place and the scales, and
@@ -667,19 +650,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto ask_page = [&](int t) {
       const int bi = t * kTileBlocks + lane;
       key_next = kNoKey;
-      if (lane < kTileBlocks && t < walk.k1 && bi < walk.r.blocks) {
-        key_next = (bi < walk.r.sink_blocks ? bi : bi - walk.r.sink_blocks + walk.r.first_block) * kKvBlock;
-        page_next = a.seqs.pages[(long long)walk.b * a.seqs.pps + key_next / a.cache.page];  // (in the row: kv_span has checked)
+      if (lane < kTileBlocks && t < g->k1 && bi < g->r.blocks) {
+        key_next = (bi < g->r.sink_blocks ? bi : bi - g->r.sink_blocks + g->r.first_block) * kKvBlock;
+        page_next = a.seqs.pages[(long long)g->b * a.seqs.pps + fast_div(key_next, a.by_page)];  // (in the row: kv_span has checked)
       }
     };
     auto look_up = [&]() {
       Blocks x{-1, kNoKey, 0.f, 0.f};
       if (key_next != kNoKey) {
         if ((unsigned)page_next < (unsigned long long)a.cache.pages) {
-          const int slot = key_next % a.cache.page;
+          const int slot = key_next - fast_div(key_next, a.by_page) * a.cache.page;
           x.key0 = key_next;
-          x.at = kv_code_at(a.cache, page_next, walk.head, slot);
-          const long long sa = kv_scale_at(a.cache, page_next, walk.head, slot);
+          x.at = kv_code_at(a.cache, page_next, g->head, slot);
+          const long long sa = kv_scale_at(a.cache, page_next, g->head, slot);
           x.ks = a.cache.ks[sa];
           x.vs = a.cache.vs[sa];
         } else {
@@ -697,19 +680,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : make_uint4(0, 0, 0, 0);
       }
     };
-    while (walk.next(a)) {
+    while ((g = next_segment())) {
       vref = 0.f;
-      ask_page(walk.k0);
+      ask_page(g->k0);
       Blocks now = look_up();
-      ask_page(walk.k0 + 1);
+      ask_page(g->k0 + 1);
       Blocks ahead = look_up();
-      ask_page(walk.k0 + 2);
+      ask_page(g->k0 + 2);
       load(a.cache.k, now, kreg);
       load(a.cache.v, now, vreg);
-      for (int t = walk.k0; t < walk.k1; ++t, ++tile) {
+#pragma unroll 1
+      for (int t = g->k0; t < g->k1; ++t, ++tile) {
         const int st = tile & 1;
         const bool reused = tile >= 2;
-        if (reused) wait(smem_u32(&sh.kempty[st]), ((tile >> 1) - 1) & 1);
+        if (reused) wait(smem_u32(&sh.kempty[st]), ((tile >> 1) - 1) & 1, kStatusTimeoutEmpty);
         if (w == 0) {  // the scales
           float vmax = now.vs;
 #pragma unroll
@@ -736,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.kfull[st]));
         load(a.cache.k, ahead, kreg);
-        if (reused) wait(smem_u32(&sh.vempty[st]), ((tile >> 1) - 1) & 1);
+        if (reused) wait(smem_u32(&sh.vempty[st]), ((tile >> 1) - 1) & 1, kStatusTimeoutEmpty);
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
           put_codes(&sh.v[st][e / 4][put_lo + 1024 * (e % 4)], &sh.v[st][e / 4][put_hi + 1024 * (e % 4)], vreg[e]);
@@ -762,11 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
       constexpr uint32_t kTileUnits = kSlabs * 128 * 128 / 16, kSlabUnits = 128 * 128 / 16;
       int tile = 0, seg[2] = {0, 0}, done[2] = {0, 0};
-      bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort, a.status, code, kLimit));
-        return ok;
-      };
+      const Segment *g = nullptr;
       // (64 keys are 8192 bytes on in the keys' and the values' tiles)
       auto scores = [&](int i, int h, int st, bool last) {
         tc_fence_after();
@@ -795,20 +775,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      while (walk.next(a)) {
-        const int tiles = walk.k1 - walk.k0;
-        const int m_tiles = walk.s.n * a.group - walk.rt * kRows > 128 ? 2 : 1;
-        if (!ok) break;
+      while ((g = next_segment())) {
+        const int tiles = g->k1 - g->k0;
+        const int m_tiles = g->s.n * a.group - g->rt * kRows > 128 ? 2 : 1;
         wait(smem_u32(&sh.kfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
+#pragma unroll 1
         for (int h = 0; h < 2 && ok; ++h)
+#pragma unroll 1
           for (int i = 0; i < m_tiles && ok; ++i) {
             if (h == 0) wait(smem_u32(&sh.qfull[i]), seg[i]++ & 1, kStatusTimeoutFull);
             if (ok) scores(i, h, tile & 1, h == 1 && i == m_tiles - 1);
           }
+#pragma unroll 1
         for (int t = 0; t < tiles && ok; ++t, ++tile) {
           const int st = tile & 1, nx = st ^ 1;
           wait(smem_u32(&sh.vfull[st]), (tile >> 1) & 1, kStatusTimeoutFull);
+#pragma unroll 1
           for (int h = 0; h < 2 && ok; ++h)
+#pragma unroll 1
             for (int i = 0; i < m_tiles && ok; ++i) {
               const bool last = h == 1 && i == m_tiles - 1;
               if (!wait(smem_u32(&sh.pready[i][h]), done[i] & 1, kStatusTimeoutAccEmpty)) break;
@@ -826,6 +810,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader) umma_commit(smem_u32(&sh.drained));
       __syncwarp();
       mbar_wait_bounded(smem_u32(&sh.drained), 0, &no_abort, a.status, kStatusTimeoutDrain, 400000000LL);
+    } else if (warp == 13 && lane == 0) {
+      // ---------------------------------------------------------- segments
+      uint32_t u = u_begin;
+      const uint32_t u_end = works ? min((uint32_t)total, u + size) : 0u;
+      uint32_t base = (uint32_t)sh.base;  // first unit of (b, rt)
+      int b = sh.seq, rt = sh.rt, row_tiles = 0;
+      KvSpan s{};
+      RowSpan r{};
+      if (works) {
+        s = kv_span(a, b);
+        row_tiles = (s.n * a.group + kRows - 1) / kRows;
+        r = row_span(a, s.n, s.len, rt);
+      }
+      for (int n = 0;; ++n) {
+        Segment &g = sh.seg[n % kSegments];
+        if (n >= kSegments && !mbar_wait_bounded(smem_u32(&sh.segempty[n % kSegments]), (n / kSegments - 1) & 1, &sh.abort, a.status,
+                                                 kStatusTimeoutEmpty, kLimit))
+          break;
+        bool found = false;
+        while (!found && u < u_end) {
+          if (s.n > 0) {
+            const uint32_t each = (uint32_t)r.tiles + kItemCost, units = each * (uint32_t)a.cache.heads;
+            if (u < base + units) {
+              const uint32_t head = (u - base) / each, item = base + head * each, end = min(u_end, item + each);
+              g.k0 = max(0, (int)(u - item) - kItemCost);
+              g.k1 = (int)(end - item) - kItemCost;
+              u = end;
+              found = g.k1 > g.k0;  // (else the share ends before the item's first tile)
+              if (found) {
+                g.b = b, g.rt = rt, g.head = (int)head;
+                g.first_cta = (int)((item + kItemCost) / size);
+                g.last_cta = (int)((item + each - 1) / size);
+                g.s = s;
+                g.r = r;
+              }
+              continue;
+            }
+            base += units;
+            if (++rt < row_tiles) {
+              r = row_span(a, s.n, s.len, rt);
+              continue;
+            }
+          }
+          rt = 0;
+          s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+          row_tiles = (s.n * a.group + kRows - 1) / kRows;
+          if (s.n > 0) r = row_span(a, s.n, s.len, 0);
+        }
+        g.more = found;
+        mbar_arrive(smem_u32(&sh.segfull[n % kSegments]));
+        if (!found) break;
+      }
     }
   }
   __syncwarp();

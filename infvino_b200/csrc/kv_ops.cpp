@@ -347,6 +347,9 @@ int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
     a.window = window;
     a.sinks = sinks;
     a.status = h->status;
+    need((int64_t)max_new * a.group < (1LL << 30), "max_new * q_heads / kv_heads out of range");
+    a.by_group = ivb::make_fastdiv((uint32_t)a.group);
+    a.by_page = ivb::make_fastdiv((uint32_t)a.cache.page);
     if (a.seqs.tokens == 0) return;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
