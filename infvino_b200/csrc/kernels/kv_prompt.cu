@@ -155,6 +155,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 x, y, w;\n\t"
@@ -491,11 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float o[32];
                 tmem_ld32(o_at + 32 * d, o);
                 tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
                 uint32_t w[32];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                  asm volatile("" : "+f"(o[k]));
-                  w[k] = __float_as_uint(o[k] * fo);
+                for (int k = 0; k < 32; k += 2) {
+                  const float2 x = mul2(make_float2(o[k], o[k + 1]), make_float2(fo, fo));
+                  w[k] = __float_as_uint(x.x);
+                  w[k + 1] = __float_as_uint(x.y);
                 }
                 tmem_st16(o_at + 32 * d, w);
                 tmem_st16(o_at + 32 * d + 16, w + 16);
@@ -747,62 +759,82 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kTileUnits = kSlabs * 128 * 128 / 16, kSlabUnits = 128 * 128 / 16;
       int tile = 0, seg[2] = {0, 0}, done[2] = {0, 0};
       const Segment *g = nullptr;
-      // (64 keys are 8192 bytes on in the keys' and the values' tiles)
-      auto scores = [&](int i, int h, int st, bool last) {
-        tc_fence_after();
-        if (leader) {
-          const uint32_t q_lo = (uint32_t)qd + (uint32_t)i * kTileUnits, k_lo = (uint32_t)kd + (uint32_t)st * kTileUnits + 512u * h;
+      // One lane issues, in one stretch for each part, with every operand
+      // worked out before: between two parts the tensor cores have only a few
+      // products queued.  (64 keys are 8192 bytes on in a tile.)
+      const uint32_t q_hi = (uint32_t)(qd >> 32), k_hi = (uint32_t)(kd >> 32), v_hi = (uint32_t)(vd >> 32);
+      auto scores = [&](int i, int h, uint32_t k_lo) {
 #pragma unroll
-          for (int k = 0; k < DIM / 16; ++k) {
-            const uint32_t o = (uint32_t)(k >> 2) * kSlabUnits + 2u * (k & 3);
-            umma_f16_lh(tmem + (uint32_t)(2 * i + h) * kSub, q_lo + o, (uint32_t)(qd >> 32), k_lo + o, (uint32_t)(kd >> 32), idesc_s, k > 0);
-          }
-          umma_commit(smem_u32(&sh.sfull[i][h]));
-          if (last) umma_commit(smem_u32(&sh.kempty[st]));
+        for (int k = 0; k < DIM / 16; ++k) {
+          const uint32_t o = (uint32_t)(k >> 2) * kSlabUnits + 2u * (k & 3);
+          umma_f16_lh(tmem + (uint32_t)(2 * i + h) * kSub, (uint32_t)qd + (uint32_t)i * kTileUnits + o, q_hi, k_lo + 512u * h + o, k_hi,
+                      idesc_s, k > 0);
         }
-        __syncwarp();
+        umma_commit(smem_u32(&sh.sfull[i][h]));
       };
-      auto values = [&](int i, int h, int st, bool begin, bool last) {
+      // O_i += P_i V over part h, then the scores of the next tile's part h into its place
+      // (the next tile may not be there yet: the products do not wait for it)
+      auto part = [&](int i, int h, uint32_t v_lo, uint32_t k_lo, bool begin, bool more, bool keys_late, bool last, int st) {
+        if (!wait(smem_u32(&sh.pready[i][h]), done[i] & 1, kStatusTimeoutAccEmpty)) return;
         tc_fence_after();
         if (leader) {
-          const uint32_t v_lo = (uint32_t)vd + (uint32_t)st * kTileUnits + 512u * h;
 #pragma unroll
           for (int k = 0; k < kSub / 16; ++k)
-            umma_f16_ts(tmem + 256u + 128u * i, tmem + (uint32_t)(2 * i + h) * kSub + 8u * k, v_lo + (2048u / 16u) * k,
-                        (uint32_t)(vd >> 32), idesc_o, !begin || k > 0);
+            umma_f16_ts(tmem + 256u + 128u * i, tmem + (uint32_t)(2 * i + h) * kSub + 8u * k, v_lo + 512u * h + (2048u / 16u) * k, v_hi,
+                        idesc_o, !begin || k > 0);
           umma_commit(smem_u32(&sh.odone[i][h]));
           if (last) umma_commit(smem_u32(&sh.vempty[st]));
+          if (more && !keys_late) {
+            scores(i, h, k_lo);
+            if (last) umma_commit(smem_u32(&sh.kempty[st ^ 1]));
+          }
         }
         __syncwarp();
+        if (keys_late && more) {
+          if (!wait(smem_u32(&sh.kfull[st ^ 1]), ((tile + 1) >> 1) & 1, kStatusTimeoutFull)) return;
+          tc_fence_after();
+          if (leader) scores(i, h, k_lo);
+          __syncwarp();
+        }
       };
       while ((g = next_segment())) {
         const int tiles = g->k1 - g->k0;
-        const int m_tiles = g->s.n * a.group - g->rt * kRows > 128 ? 2 : 1;
-        wait(smem_u32(&sh.kfull[tile & 1]), (tile >> 1) & 1, kStatusTimeoutFull);
-#pragma unroll 1
-        for (int h = 0; h < 2 && ok; ++h)
-#pragma unroll 1
-          for (int i = 0; i < m_tiles && ok; ++i) {
-            if (h == 0) wait(smem_u32(&sh.qfull[i]), seg[i]++ & 1, kStatusTimeoutFull);
-            if (ok) scores(i, h, tile & 1, h == 1 && i == m_tiles - 1);
+        const bool two = g->s.n * a.group - g->rt * kRows > 128;
+        const int st0 = tile & 1;
+        wait(smem_u32(&sh.kfull[st0]), (tile >> 1) & 1, kStatusTimeoutFull);
+        const uint32_t k0_lo = (uint32_t)kd + (uint32_t)st0 * kTileUnits;
+        wait(smem_u32(&sh.qfull[0]), seg[0]++ & 1, kStatusTimeoutFull);
+        tc_fence_after();
+        if (ok && leader) {
+          scores(0, 0, k0_lo);
+          scores(0, 1, k0_lo);
+        }
+        __syncwarp();
+        if (two) {
+          wait(smem_u32(&sh.qfull[1]), seg[1]++ & 1, kStatusTimeoutFull);
+          tc_fence_after();
+          if (ok && leader) {
+            scores(1, 0, k0_lo);
+            scores(1, 1, k0_lo);
           }
+          __syncwarp();
+        }
+        if (ok && leader) umma_commit(smem_u32(&sh.kempty[st0]));
+        __syncwarp();
 #pragma unroll 1
         for (int t = 0; t < tiles && ok; ++t, ++tile) {
-          const int st = tile & 1, nx = st ^ 1;
+          const int st = tile & 1;
+          const bool more = t + 1 < tiles;
+          const uint32_t v_lo = (uint32_t)vd + (uint32_t)st * kTileUnits, k_lo = (uint32_t)kd + (uint32_t)(st ^ 1) * kTileUnits;
           wait(smem_u32(&sh.vfull[st]), (tile >> 1) & 1, kStatusTimeoutFull);
-#pragma unroll 1
-          for (int h = 0; h < 2 && ok; ++h)
-#pragma unroll 1
-            for (int i = 0; i < m_tiles && ok; ++i) {
-              const bool last = h == 1 && i == m_tiles - 1;
-              if (!wait(smem_u32(&sh.pready[i][h]), done[i] & 1, kStatusTimeoutAccEmpty)) break;
-              values(i, h, st, t == 0 && h == 0, last);
-              if (t + 1 < tiles) {
-                if (h == 0 && i == 0) wait(smem_u32(&sh.kfull[nx]), ((tile + 1) >> 1) & 1, kStatusTimeoutFull);
-                if (ok) scores(i, h, nx, last);
-              }
-            }
-          for (int i = 0; i < m_tiles; ++i) ++done[i];
+          if (!ok) break;
+          const bool late = more && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sh.kfull[st ^ 1]), ((tile + 1) >> 1) & 1));
+          part(0, 0, v_lo, k_lo, t == 0, more, late, false, st);
+          if (two) part(1, 0, v_lo, k_lo, t == 0, more, false, false, st);
+          part(0, 1, v_lo, k_lo, false, more, false, !two, st);
+          if (two) part(1, 1, v_lo, k_lo, false, more, false, true, st);
+          ++done[0];
+          if (two) ++done[1];
         }
       }
       // every product retires before TMEM is released
