@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -86,27 +87,12 @@ class Preprocess(ctypes.Structure):
                 ("std", ctypes.c_float * 3)]
 
 
-class Rows(ctypes.Structure):
-    """ivc_rows."""
-    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
-
-
-class KvCache(ctypes.Structure):
-    """ivc_kv_cache."""
-    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("page_size", _i32),
-                ("kv_heads", _i32), ("head_dim", _i32)]
-
-
-class KvSeqs(ctypes.Structure):
-    """ivc_kv_seqs."""
-    _fields_ = [("batch", _i32), ("tokens", _i64), ("offsets", _vp), ("at", _vp), ("pages", _vp),
-                ("pages_per_seq", _i32)]
-
-
-class Rotary(ctypes.Structure):
-    """ivc_rotary."""
-    _fields_ = [("table", _vp), ("positions", _i64), ("pairs", _i32), ("axes", _i32), ("interleaved", _i32),
-                ("pos", _vp), ("pos_stride", _i64), ("axis_of", _cp)]
+# The structs of the ivc_kv_* calls as packed bytes (a ctypes Structure costs
+# several times as much to fill, and a decode step makes these calls for every layer).
+ROWS = struct.Struct("@Pqq")               # ivc_rows: data, token_stride, head_stride
+KV_CACHE = struct.Struct("@PPPPqiii0q")    # ivc_kv_cache: k, v, k_scale, v_scale, pages, page_size, kv_heads, head_dim
+KV_SEQS = struct.Struct("@iqPPPi0q")       # ivc_kv_seqs: batch, tokens, offsets, at, pages, pages_per_seq
+ROTARY = struct.Struct("@PqiiiPqP")        # ivc_rotary: table, positions, pairs, axes, interleaved, pos, pos_stride, axis_of
 
 
 _lib = None

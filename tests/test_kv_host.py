@@ -1,5 +1,6 @@
 """The language-model operators' descriptors and refusals that need no GPU."""
-import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
@@ -26,8 +27,8 @@ def test_rotary_descriptor():
     table = torch.zeros((10, 16, 2))
     r = ivb.Rotary(table, [0] * 8 + [2] * 8)
     assert r.axes == 3
-    c = r.at(torch.zeros((3, 5), dtype=torch.int32), 5)
-    assert c.axes == 3 and c.pos_stride == 5 and c.pairs == 16 and c.positions == 10
+    c = _native.ROTARY.unpack(r.at(torch.zeros((3, 5), dtype=torch.int32), 5))
+    assert c[1:5] == (10, 16, 3, 0) and c[6] == 5
     for pos in (torch.zeros((2, 5), dtype=torch.int32), torch.zeros(5, dtype=torch.int32), torch.zeros((3, 4), dtype=torch.int32),
                 torch.zeros((3, 5), dtype=torch.int64)):
         with pytest.raises(ValueError):
@@ -39,22 +40,22 @@ def test_rotary_descriptor():
 
 
 def test_structs_match_the_header(tmp_path):
-    """The ctypes structures have the C compiler's sizes and offsets."""
-    import os
-    import subprocess
+    """The packed structures have the C compiler's sizes, and every field its place."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    pairs = [("ivc_rows", _native.Rows), ("ivc_kv_cache", _native.KvCache), ("ivc_kv_seqs", _native.KvSeqs), ("ivc_rotary", _native.Rotary)]
+    fields = {"ivc_rows": (_native.ROWS, "data token_stride head_stride"),
+              "ivc_kv_cache": (_native.KV_CACHE, "k v k_scale v_scale pages page_size kv_heads head_dim"),
+              "ivc_kv_seqs": (_native.KV_SEQS, "batch tokens offsets at pages pages_per_seq"),
+              "ivc_rotary": (_native.ROTARY, "table positions pairs axes interleaved pos pos_stride axis_of")}
     lines = []
-    for name, s in pairs:
-        lines.append(f'printf("%zu\\n", sizeof({name}));')
-        lines += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in s._fields_]
+    for name, (s, names) in fields.items():  # field i holds i + 1 in the struct that this prints byte by byte
+        sets = "".join(f"x.{f} = (__typeof__(x.{f}))(intptr_t){i + 1};" for i, f in enumerate(names.split()))
+        lines.append(f'{{ {name} x; memset(&x, 0, sizeof x); {sets} for (size_t i = 0; i < sizeof x; ++i) printf("%02x", ((unsigned char *)&x)[i]); puts(""); }}')
     src = tmp_path / "s.c"
-    src.write_text('#include <stdio.h>\n#include "infvino_b200.h"\nint main(void) {' + "".join(lines) + "return 0;}")
+    src.write_text('#include <stdio.h>\n#include <string.h>\n#include "infvino_b200.h"\nint main(void) {' + "".join(lines) + "return 0;}")
     exe = str(tmp_path / "s")
     subprocess.run(["gcc", str(src), "-I" + os.path.join(root, "include"), "-o", exe], check=True)
-    got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
-    want = [n for _, s in pairs for n in [ctypes.sizeof(s)] + [getattr(s, f[0]).offset for f in s._fields_]]
-    assert got == want
+    got = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()
+    assert got == [s.pack(*range(1, len(names.split()) + 1)).hex() for s, names in fields.values()]
 
 
 def test_null_handles_are_refused():
