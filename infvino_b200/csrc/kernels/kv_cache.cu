@@ -5,6 +5,7 @@
 // written once.  Sixteen elements (eight pairs) of a row are a thread's share;
 // a warp reads whole 128-byte lines of the two halves of a head.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_common.cuh"
 
@@ -43,8 +44,9 @@ __device__ __forceinline__ bool load_turn(const KvRotary &r, int g, long long to
 // Where the two vectors of group g of a row begin: the halves of eight pairs
 // (side by side when they are interleaved), or sixteen elements behind the
 // rotated ones.
-__device__ __forceinline__ void group_at(int g, int pairs, int interleaved, int &a, int &b) {
-  if (8 * g < pairs && !interleaved) {
+template <bool INTER>
+__device__ __forceinline__ void group_at(int g, int pairs, int &a, int &b) {
+  if (!INTER && 8 * g < pairs) {
     a = 8 * g;
     b = pairs + 8 * g;
   } else {
@@ -56,8 +58,9 @@ __device__ __forceinline__ void group_at(int g, int pairs, int interleaved, int 
 // Turns eight pairs in place.  Products and sums are rounded one by one (no
 // fused multiply-add), so any IEEE evaluation of the formula gives the same
 // bits, and with them the same codes in the cache.
-__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const Turn &t, int interleaved) {
-  if (interleaved) {  // a: pairs 0..3, b: pairs 4..7, each (x, y) side by side
+template <bool INTER>
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const Turn &t) {
+  if (INTER) {  // a: pairs 0..3, b: pairs 4..7, each (x, y) side by side
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float(&h)[8] = i < 4 ? a : b;
@@ -91,7 +94,7 @@ constexpr int kRopeHeads = 4;  // heads a thread turns by the same angles at onc
 
 // Turns the rows of token tile `tile`.  A token takes hs * (dim / 16) threads;
 // thread (head h0, group g) turns heads h0, h0 + hs, ...
-template <bool BF16>
+template <bool BF16, bool INTER>
 __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int heads, int dim, int hs, int per_block,
                                           const KvRows &x, const KvRows &out, const KvRotary &rot, int *status) {
   const int groups = dim / 16, upt = hs * groups;
@@ -101,12 +104,13 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
     if (token >= tokens) break;
     const bool turned = 8 * g < rot.pairs;
     int ea, eb;
-    group_at(g, rot.pairs, rot.interleaved, ea, eb);
-    Turn t;
-    if (turned && !load_turn(rot, g, token, t, status)) continue;
+    group_at<INTER>(g, rot.pairs, ea, eb);
     const uint16_t *xr = static_cast<const uint16_t *>(x.p) + token * x.ts;
     uint16_t *yr = static_cast<uint16_t *>(out.p) + token * out.ts;
+    Turn t;
+    bool ok = true;
     for (int h = h0; h < heads; h += kRopeHeads * hs) {
+      // the rows are on their way before the angles' chain (position, then table) begins
       uint4 ua[kRopeHeads], ub[kRopeHeads];
 #pragma unroll
       for (int i = 0; i < kRopeHeads; ++i)
@@ -114,6 +118,8 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
           ua[i] = load8(xr + (h + i * hs) * x.hs + ea, x.vec);
           ub[i] = load8(xr + (h + i * hs) * x.hs + eb, x.vec);
         }
+      if (h == h0 && turned) ok = load_turn(rot, g, token, t, status);
+      if (!ok) break;
 #pragma unroll
       for (int i = 0; i < kRopeHeads; ++i)
         if (h + i * hs < heads) {
@@ -121,7 +127,7 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
             float a[8], b[8];
             unpack8<BF16>(ua[i], a);
             unpack8<BF16>(ub[i], b);
-            turn8(a, b, t, rot.interleaved);
+            turn8<INTER>(a, b, t);
             ua[i] = pack8<BF16>(a);
             ub[i] = pack8<BF16>(b);
           }
@@ -132,12 +138,12 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
   }
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kRopeThreads)
+template <bool BF16, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, 3)
     kv_rope_k(long long tokens, int heads, int dim, int hs, int per_block, const __grid_constant__ KvRows x,
               const __grid_constant__ KvRows out, const __grid_constant__ KvRotary rot, int *status) {
   pdl_wait_and_release();
-  rope_tile<BF16>(blockIdx.x, tokens, heads, dim, hs, per_block, x, out, rot, status);
+  rope_tile<BF16, INTER>(blockIdx.x, tokens, heads, dim, hs, per_block, x, out, rot, status);
 }
 
 // ---------------------------------------------------------------- append
@@ -186,14 +192,14 @@ __device__ __forceinline__ uint32_t requantise4(uint32_t w, float ratio) {
 // One warp: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
 // tokens from t0) of one head, keys or values.  Lane (row l / groups, group
 // l % groups) holds sixteen elements of every (32 / groups)-th row.
-template <bool BF16, int DIM>
+template <bool BF16, bool INTER, int DIM>
 __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &x, bool turn, int8_t *codes,
                                              float *scale_at, int head, int r0, int r1, long long t0) {
   constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows;
   const int lane = threadIdx.x & 31, g = lane % kGroups, rl = lane / kGroups;
   const int pairs = turn ? a.rot.pairs : 0;
   int ea, eb;
-  group_at(g, pairs, a.rot.interleaved, ea, eb);
+  group_at<INTER>(g, pairs, ea, eb);
   float f[kSteps][2][8];
   float most = 0.f;
   const uint16_t *xh = static_cast<const uint16_t *>(x.p) + head * x.hs;
@@ -215,7 +221,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
     unpack8<BF16>(ub[i], f[i][1]);
     if (r >= r0 && r < r1 && 8 * g < pairs) {
       Turn t;
-      if (load_turn(a.rot, g, t0 + r - r0, t, a.status)) turn8(f[i][0], f[i][1], t, a.rot.interleaved);
+      if (load_turn(a.rot, g, t0 + r - r0, t, a.status)) turn8<INTER>(f[i][0], f[i][1], t);
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -257,56 +263,72 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
   }
 }
 
+// Where a packed token is: its sequence's end, and its page and slot (-1: nowhere).
+struct Place {
+  long long first, end;  // the sequence's packed tokens
+  int pos, page, slot;
+};
+
+// The places of packed tokens first .. first + window - 1, one thread each.
+__device__ __forceinline__ void find_places(const KvCache &c, const KvSeqs &s, long long first, int window, int *status,
+                                            Place *places) {
+  int seq = kv_seq_of(s, first);
+  const int i = threadIdx.x;
+  const long long t = first + i;
+  if (i < window) {
+    Place p{0, 0, -1, -1, 0};
+    if (t < s.tokens) {
+      while (seq < s.batch && s.offsets[seq + 1] <= t) ++seq;
+      if (seq < s.batch) {  // (tokens behind the last sequence are not the call's)
+        p.first = s.offsets[seq];
+        p.end = min((long long)s.offsets[seq + 1], s.tokens);
+        const long long pos = (long long)s.at[seq] + (t - p.first);
+        if (t < p.first || p.first < 0 || s.at[seq] < 0 || pos >= 0x7fffffffLL) {
+          kv_flag(status, kStatusKvSeqs);
+        } else {
+          p.pos = (int)pos;
+          p.page = kv_page_of(c, s, seq, p.pos, status);
+          p.slot = p.pos % c.page;
+        }
+      }
+    }
+    places[i] = p;
+  }
+  __syncthreads();
+}
+
 // CTA c of the first `append_ctas` takes the blocks whose first new token is
 // among packed tokens c * window .. + window - 1; its warps take (block, head,
 // keys or values) in turn.  A block is one warp's alone, so nothing is atomic
 // and the result does not depend on any order.  The other CTAs turn queries.
-template <bool BF16, int DIM>
-__global__ void __launch_bounds__(kRopeThreads) kv_append_k(const __grid_constant__ AppendArgs a) {
+template <bool BF16, bool INTER, int DIM>
+__global__ void __launch_bounds__(kRopeThreads, 2) kv_append_k(const __grid_constant__ AppendArgs a) {
+  __shared__ Place places[kKvBlock];
   pdl_wait_and_release();
   if ((int)blockIdx.x >= a.append_ctas) {
-    rope_tile<BF16>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs, a.q_per_block, a.q, a.q_out,
+    rope_tile<BF16, INTER>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs, a.q_per_block, a.q, a.q_out,
                     a.rot, a.status);
     return;
   }
   const long long first = (long long)blockIdx.x * a.window;
-  const int seq0 = kv_seq_of(a.s, first);
-  const int warp = threadIdx.x >> 5;
-  int task = warp;                // (block, head, half) tasks, this warp's next
-  int seq = seq0, base = 0;
+  find_places(a.c, a.s, first, a.window, a.status, places);
   const int per_block = 2 * a.c.heads;
+  int task = threadIdx.x >> 5, base = 0;  // (block, head, half) tasks, this warp's next
   for (int i = 0; i < a.window; ++i) {
+    const Place p = places[i];
     const long long t = first + i;
-    if (t >= a.s.tokens) break;
-    while (seq < a.s.batch && a.s.offsets[seq + 1] <= t) ++seq;
-    if (seq >= a.s.batch) break;  // tokens behind the last sequence: not the call's
-    const long long o = a.s.offsets[seq], end = a.s.offsets[seq + 1];
-    const int start = a.s.at[seq];
-    if (t < o || o < 0 || start < 0) {
-      kv_flag(a.status, kStatusKvSeqs);
-      continue;
-    }
-    const long long pos = start + (t - o);
-    if (t != o && pos % kKvBlock != 0) continue;
-    // a block begins here
-    if (task < base + per_block && pos < 0x7fffffffLL) {
-      const int page = kv_page_of(a.c, a.s, seq, (int)pos, a.status);
-      if (page >= 0) {
-        const int r0 = (int)(pos % kKvBlock);
-        const int r1 = (int)min((long long)kKvBlock, r0 + min(end, a.s.tokens) - t);
-        const int slot = (int)pos % a.c.page - r0;
-        for (; task < base + per_block; task += kRopeThreads / 32) {
-          const int head = (task - base) >> 1;
-          const long long ca = kv_code_at(a.c, page, head, slot), sa = kv_scale_at(a.c, page, head, slot);
-          if ((task - base) & 1)
-            append_block<BF16, DIM>(a, a.v, false, a.c.v + ca, a.c.vs + sa, head, r0, r1, t);
-          else
-            append_block<BF16, DIM>(a, a.k, a.rot.table != nullptr, a.c.k + ca, a.c.ks + sa, head, r0, r1, t);
-        }
-      }
+    const int r0 = p.slot % kKvBlock;
+    if (p.page < 0 || (t != p.first && r0 != 0)) continue;
+    const int r1 = (int)min((long long)kKvBlock, r0 + (p.end - t));  // a block begins here
+    for (; task < base + per_block; task += kRopeThreads / 32) {
+      const int head = (task - base) >> 1;
+      const long long ca = kv_code_at(a.c, p.page, head, p.slot - r0), sa = kv_scale_at(a.c, p.page, head, p.slot - r0);
+      if ((task - base) & 1)
+        append_block<BF16, INTER, DIM>(a, a.v, false, a.c.v + ca, a.c.vs + sa, head, r0, r1, t);
+      else
+        append_block<BF16, INTER, DIM>(a, a.k, a.rot.table != nullptr, a.c.k + ca, a.c.ks + sa, head, r0, r1, t);
     }
     base += per_block;
-    while (task < base) task += kRopeThreads / 32;
   }
 }
 
@@ -317,43 +339,41 @@ template <bool BF16, int DIM>
 __global__ void __launch_bounds__(256)
     kv_read_k(const __grid_constant__ KvCache c, const __grid_constant__ KvSeqs s, const __grid_constant__ KvRows k,
               const __grid_constant__ KvRows v, int window, int *status) {
+  __shared__ Place places[kKvBlock];
   pdl_wait_and_release();
   constexpr int kGroups = DIM / 16;
   const long long first = (long long)blockIdx.x * window;
-  int seq = kv_seq_of(s, first);
-  const int halves = (k.p ? 1 : 0) + (v.p ? 1 : 0);
-  for (int i = 0; i < window; ++i) {
-    const long long t = first + i;
-    if (t >= s.tokens) break;
-    while (seq < s.batch && s.offsets[seq + 1] <= t) ++seq;
-    if (seq >= s.batch) break;
-    const long long o = s.offsets[seq];
-    const long long pos = s.at[seq] + (t - o);
-    if (t < o || o < 0 || pos < 0 || pos >= 0x7fffffffLL) {
-      kv_flag(status, kStatusKvSeqs);
-      continue;
-    }
-    const int page = kv_page_of(c, s, seq, (int)pos, status);
-    if (page < 0) continue;
-    const int slot = (int)pos % c.page;
-    for (int u = threadIdx.x; u < halves * c.heads * kGroups; u += blockDim.x) {
-      const int g = u % kGroups, hh = u / kGroups, head = hh % c.heads;
-      const bool val = hh / c.heads == 1 || !k.p;
-      const KvRows &y = val ? v : k;
-      const long long ca = kv_code_at(c, page, head, slot) + 16 * g;
-      const float sc = (val ? c.vs : c.ks)[kv_scale_at(c, page, head, slot)];
-      const uint4 w = *reinterpret_cast<const uint4 *>((val ? c.v : c.k) + ca);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-      uint16_t *row = static_cast<uint16_t *>(y.p) + t * y.ts + head * y.hs + 16 * g;
+  find_places(c, s, first, window, status, places);
+  const int halves = (k.p ? 1 : 0) + (v.p ? 1 : 0), each = halves * c.heads * kGroups;
+  for (int u = threadIdx.x; u < window * each; u += blockDim.x) {
+    const int i = u / each, w0 = u - i * each;
+    const int g = w0 % kGroups, hh = w0 / kGroups;
+    const bool val = hh >= c.heads || !k.p;
+    const int head = hh >= c.heads ? hh - c.heads : hh;
+    const Place &p = places[i];
+    if (p.page < 0) continue;
+    const KvRows &y = val ? v : k;
+    const long long ca = kv_code_at(c, p.page, head, p.slot) + 16 * g;
+    const float sc = (val ? c.vs : c.ks)[kv_scale_at(c, p.page, head, p.slot)];
+    const uint4 w = *reinterpret_cast<const uint4 *>((val ? c.v : c.k) + ca);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint16_t *row = static_cast<uint16_t *>(y.p) + (first + i) * y.ts + head * y.hs + 16 * g;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float f[8];
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(ws[2 * h + (j >> 2)] >> (8 * (j & 3))) * sc;
-        store8(row + 8 * h, pack8<BF16>(f), y.vec);
-      }
+      for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(ws[2 * h + (j >> 2)] >> (8 * (j & 3))) * sc;
+      store8(row + 8 * h, pack8<BF16>(f), y.vec);
     }
   }
+}
+
+// Tokens a CTA looks at: one while there are few (decoding: each begins a
+// block), up to a block's sixteen where that still gives every SM some.
+int window_of(long long tokens) {
+  int w = 1;
+  while (w < kKvBlock && tokens / w > 148 * 4) w *= 2;
+  return w;
 }
 
 // Head groups of the rotation: one head a thread while that leaves SMs free,
@@ -378,7 +398,9 @@ cudaError_t launch_kv_rope(bool bf16, long long tokens, int heads, int dim, cons
   int hs, per_block;
   rope_shape(tokens, heads, dim, hs, per_block);
   const dim3 grid((unsigned)((tokens + per_block - 1) / per_block));
-  return launch_kernel(bf16 ? kv_rope_k<true> : kv_rope_k<false>, grid, dim3(kRopeThreads), 0, st, tokens, heads, dim,
+  auto kern = rot.interleaved ? (bf16 ? kv_rope_k<true, true> : kv_rope_k<false, true>)
+                              : (bf16 ? kv_rope_k<true, false> : kv_rope_k<false, false>);
+  return launch_kernel(kern, grid, dim3(kRopeThreads), 0, st, tokens, heads, dim,
                        hs, per_block, x, out, rot, status);
 }
 
@@ -386,23 +408,25 @@ cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const
                              const KvRotary &rot, int q_heads, const KvRows &q, const KvRows &q_out, int *status,
                              cudaStream_t st) {
   AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, status};
-  // A CTA for each token while they are few (decode: each begins a block);
-  // sixteen for each CTA beyond that (a prompt begins a block every sixteen).
-  a.window = s.tokens <= 1024 ? 1 : kKvBlock;
+  a.window = window_of(s.tokens);
   a.append_ctas = (int)((s.tokens + a.window - 1) / a.window);
   long long grid = a.append_ctas;
   if (q_heads) {
     rope_shape(s.tokens, q_heads, c.dim, a.q_hs, a.q_per_block);
     grid += (s.tokens + a.q_per_block - 1) / a.q_per_block;
   }
-  auto kern = c.dim == 64 ? (bf16 ? kv_append_k<true, 64> : kv_append_k<false, 64>)
-                          : (bf16 ? kv_append_k<true, 128> : kv_append_k<false, 128>);
+  auto pick = [&](auto inter) {
+    constexpr bool kInter = decltype(inter)::value;
+    return c.dim == 64 ? (bf16 ? kv_append_k<true, kInter, 64> : kv_append_k<false, kInter, 64>)
+                       : (bf16 ? kv_append_k<true, kInter, 128> : kv_append_k<false, kInter, 128>);
+  };
+  auto kern = rot.interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   return launch_kernel(kern, dim3((unsigned)grid), dim3(kRopeThreads), 0, st, a);
 }
 
 cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v, int *status,
                            cudaStream_t st) {
-  const int window = s.tokens <= 1024 ? 1 : 8;
+  const int window = window_of(s.tokens);
   const dim3 grid((unsigned)((s.tokens + window - 1) / window));
   auto kern = c.dim == 64 ? (bf16 ? kv_read_k<true, 64> : kv_read_k<false, 64>)
                           : (bf16 ? kv_read_k<true, 128> : kv_read_k<false, 128>);
