@@ -155,7 +155,7 @@ struct AppendArgs {
   KvRotary rot;
   int q_heads, q_hs, q_per_block;
   int window;             // packed tokens an append CTA looks at
-  int append_ctas;
+  int slices, append_ctas;
   int *status;
 };
 
@@ -169,15 +169,21 @@ __device__ __forceinline__ int scale_exponent(float m) {
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-__device__ __forceinline__ int quantise(float x, float inv) {
-  // NaN becomes 0, infinities the largest code
-  return __float2int_rn(fminf(fmaxf(x == x ? x * inv : 0.f, -127.f), 127.f));
-}
-__device__ __forceinline__ uint2 quantise8(const float (&f)[8], float inv) {
-  uint32_t w[2] = {0, 0};
+// Four codes.  x * inv is exact (a power of two) and at most 127, so adding
+// 1.5 * 2^23 rounds it to the nearest integer, ties to even, in the low byte.
+__device__ __forceinline__ uint32_t quantise4(const float *x, float inv) {
+  uint32_t t[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)quantise(f[i], inv) & 0xffu) << (8 * (i & 3));
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(fmaf(x[i], inv, 12582912.f));
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+// NaN to 0, infinities (and what the largest scale cannot hold) to the largest code.
+__device__ __forceinline__ float tame(float x, float most) { return x == x ? fminf(fmaxf(x, -most), most) : 0.f; }
+// The larger magnitude; NaN if one is.
+__device__ __forceinline__ float max_abs(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
 }
 __device__ __forceinline__ uint32_t requantise4(uint32_t w, float ratio) {
   uint32_t o = 0;
@@ -189,76 +195,122 @@ __device__ __forceinline__ uint32_t requantise4(uint32_t w, float ratio) {
   return o;
 }
 
-// One warp: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
-// tokens from t0) of one head, keys or values.  Lane (row l / groups, group
-// l % groups) holds sixteen elements of every (32 / groups)-th row.
+constexpr int kPair = 2;                               // warps that share a block
+constexpr int kPairs = kRopeThreads / 32 / kPair;
+
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); }
+
+// Two warps: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
+// tokens from t0), keys or values (`codes`, `scales`: head 0's), of heads
+// head, head + step, ...  A warp takes eight of the rows; lane (row l /
+// groups, group l % groups) holds sixteen elements of every (32 / groups)-th.
+// A token's angles are loaded once for all heads, and a head's rows while the
+// one before is worked on.
 template <bool BF16, bool INTER, int DIM>
 __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &x, bool turn, int8_t *codes,
-                                             float *scale_at, int head, int r0, int r1, long long t0) {
-  constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows;
-  const int lane = threadIdx.x & 31, g = lane % kGroups, rl = lane / kGroups;
+                                             float *scales, int head, int step, int r0, int r1, long long t0,
+                                             float *shared) {
+  constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows / kPair;
+  const int lane = threadIdx.x & 31, g = lane % kGroups, warp = threadIdx.x >> 5, pair = warp / kPair;
+  const int row0 = warp % kPair * (kKvBlock / kPair) + lane / kGroups;
   const int pairs = turn ? a.rot.pairs : 0;
   int ea, eb;
   group_at<INTER>(g, pairs, ea, eb);
-  float f[kSteps][2][8];
-  float most = 0.f;
-  const uint16_t *xh = static_cast<const uint16_t *>(x.p) + head * x.hs;
+  const uint16_t *xt = static_cast<const uint16_t *>(x.p) + t0 * x.ts;
   uint4 ua[kSteps], ub[kSteps];
+  float before = 0.f;
+  auto load = [&](int h) {
+    if (h >= a.c.heads) return;
+    if (r0 > 0) before = scales[(long long)h * (a.c.page / kKvBlock)];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int r = i * kRows + rl;
-    ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
-    if (r >= r0 && r < r1) {
-      const uint16_t *row = xh + (t0 + r - r0) * x.ts;
-      ua[i] = load8(row + ea, x.vec);
-      ub[i] = load8(row + eb, x.vec);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int r = i * kRows + rl;
-    unpack8<BF16>(ua[i], f[i][0]);
-    unpack8<BF16>(ub[i], f[i][1]);
-    if (r >= r0 && r < r1 && 8 * g < pairs) {
-      Turn t;
-      if (load_turn(a.rot, g, t0 + r - r0, t, a.status)) turn8<INTER>(f[i][0], f[i][1], t);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float m = fabsf(f[i][j >> 3][j & 7]);
-      most = fmaxf(most, m <= 3.402823466e38f ? m : 0.f);  // (a NaN compares false)
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  int e = scale_exponent(most);
-  if (r0 > 0) {  // tokens before: their codes follow the scale if it grows
-    const float before = *scale_at;
-    const int eo = max(kKvMinExp, min(kKvMaxExp, (int)((__float_as_uint(before) >> 23) & 0xffu) - 127));
-    if (e > eo) {
-      const float ratio = e - eo > 60 ? 0.f : exp2i(eo - e);
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int r = i * kRows + rl;
-        if (r < r0) {
-          uint4 *p = reinterpret_cast<uint4 *>(codes + r * DIM + 16 * g);
-          const uint4 w = *p;
-          *p = make_uint4(requantise4(w.x, ratio), requantise4(w.y, ratio), requantise4(w.z, ratio),
-                          requantise4(w.w, ratio));
-        }
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
+      if (r >= r0 && r < r1) {
+        const uint16_t *row = xt + (r - r0) * x.ts + h * x.hs;
+        ua[i] = load8(row + ea, x.vec);
+        ub[i] = load8(row + eb, x.vec);
       }
     }
-    e = max(e, eo);
-  }
-  __syncwarp();  // every lane has read the old scale
-  if (lane == 0) *scale_at = exp2i(e);
-  const float inv = exp2i(-e);
+  };
+  // the largest magnitude of the block
+  auto join = [&](float m) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) shared[warp] = m;
+    pair_sync(pair);
+    m = max_abs(shared[pair * kPair], shared[pair * kPair + 1]);
+    pair_sync(pair);
+    return m;
+  };
+  load(head);
+  Turn t[kSteps];
+  bool turned[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int r = i * kRows + rl;
-    if (r >= r0 && r < r1) {
-      *reinterpret_cast<uint2 *>(codes + r * DIM + ea) = quantise8(f[i][0], inv);
-      *reinterpret_cast<uint2 *>(codes + r * DIM + eb) = quantise8(f[i][1], inv);
+    const int r = row0 + i * kRows;
+    turned[i] = r >= r0 && r < r1 && 8 * g < pairs && load_turn(a.rot, g, t0 + r - r0, t[i], a.status);
+  }
+#pragma unroll 1
+  for (; head < a.c.heads; head += step) {
+    float f[kSteps][2][8], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      unpack8<BF16>(ua[i], f[i][0]);
+      unpack8<BF16>(ub[i], f[i][1]);
+      if (turned[i]) turn8<INTER>(f[i][0], f[i][1], t[i]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) most = max_abs(most, f[i][j >> 3][j & 7]);
+    }
+    const float old = before;
+    load(head + step);
+    most = join(most);
+    const bool odd = !(most <= 3.402823466e38f);  // an infinity or a NaN: the scale goes by the others
+    if (odd) {
+      most = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16 * kSteps; ++j) {
+        const float v = fabsf(f[j >> 4][j >> 3 & 1][j & 7]);
+        if (v <= 3.402823466e38f) most = fmaxf(most, v);
+      }
+      most = join(most);
+    }
+    int8_t *ch = codes + (long long)head * a.c.page * DIM;
+    int e = scale_exponent(most);
+    if (r0 > 0) {  // tokens before: their codes follow the scale if it grows
+      const int eo = max(kKvMinExp, min(kKvMaxExp, (int)((__float_as_uint(old) >> 23) & 0xffu) - 127));
+      if (e > eo) {
+        const float ratio = e - eo > 60 ? 0.f : exp2i(eo - e);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int r = row0 + i * kRows;
+          if (r < r0) {
+            uint4 *p = reinterpret_cast<uint4 *>(ch + r * DIM + 16 * g);
+            const uint4 w = *p;
+            *p = make_uint4(requantise4(w.x, ratio), requantise4(w.y, ratio), requantise4(w.z, ratio),
+                            requantise4(w.w, ratio));
+          }
+        }
+      }
+      e = max(e, eo);
+    }
+    if (warp % kPair == 0 && lane == 0) scales[(long long)head * (a.c.page / kKvBlock)] = exp2i(e);  // (both have read the old one)
+    const float inv = exp2i(-e);
+    if (odd || e == kKvMaxExp) {
+      const float top = 127.f * exp2i(e);
+#pragma unroll
+      for (int j = 0; j < 16 * kSteps; ++j) {
+        float &v = f[j >> 4][j >> 3 & 1][j & 7];
+        v = tame(v, top);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      if (r >= r0 && r < r1) {
+        *reinterpret_cast<uint2 *>(ch + r * DIM + ea) = make_uint2(quantise4(f[i][0], inv), quantise4(f[i][0] + 4, inv));
+        *reinterpret_cast<uint2 *>(ch + r * DIM + eb) = make_uint2(quantise4(f[i][1], inv), quantise4(f[i][1] + 4, inv));
+      }
     }
   }
 }
@@ -297,38 +349,35 @@ __device__ __forceinline__ void find_places(const KvCache &c, const KvSeqs &s, l
   __syncthreads();
 }
 
-// CTA c of the first `append_ctas` takes the blocks whose first new token is
-// among packed tokens c * window .. + window - 1; its warps take (block, head,
-// keys or values) in turn.  A block is one warp's alone, so nothing is atomic
-// and the result does not depend on any order.  The other CTAs turn queries.
+// Of the first `append_ctas` CTAs each takes the blocks whose first new token
+// is among `window` packed tokens, and every `slices`-th pair of heads of
+// them: two warps for a head's keys, two for its values.  A block is one
+// pair's alone, so nothing is atomic and the result does not depend on any
+// order.  The other CTAs turn queries.
 template <bool BF16, bool INTER, int DIM>
 __global__ void __launch_bounds__(kRopeThreads, 2) kv_append_k(const __grid_constant__ AppendArgs a) {
   __shared__ Place places[kKvBlock];
+  __shared__ float most[kRopeThreads / 32];
   pdl_wait_and_release();
   if ((int)blockIdx.x >= a.append_ctas) {
     rope_tile<BF16, INTER>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs, a.q_per_block, a.q, a.q_out,
                     a.rot, a.status);
     return;
   }
-  const long long first = (long long)blockIdx.x * a.window;
+  const long long first = (long long)(blockIdx.x / a.slices) * a.window;
   find_places(a.c, a.s, first, a.window, a.status, places);
-  const int per_block = 2 * a.c.heads;
-  int task = threadIdx.x >> 5, base = 0;  // (block, head, half) tasks, this warp's next
+  const int pair = (threadIdx.x >> 5) / kPair, step = kPairs / 2;  // heads a CTA works on at once
+  const int head = (blockIdx.x % a.slices) * step + (pair >> 1);
   for (int i = 0; i < a.window; ++i) {
     const Place p = places[i];
     const long long t = first + i;
     const int r0 = p.slot % kKvBlock;
     if (p.page < 0 || (t != p.first && r0 != 0)) continue;
     const int r1 = (int)min((long long)kKvBlock, r0 + (p.end - t));  // a block begins here
-    for (; task < base + per_block; task += kRopeThreads / 32) {
-      const int head = (task - base) >> 1;
-      const long long ca = kv_code_at(a.c, p.page, head, p.slot - r0), sa = kv_scale_at(a.c, p.page, head, p.slot - r0);
-      if ((task - base) & 1)
-        append_block<BF16, INTER, DIM>(a, a.v, false, a.c.v + ca, a.c.vs + sa, head, r0, r1, t);
-      else
-        append_block<BF16, INTER, DIM>(a, a.k, a.rot.table != nullptr, a.c.k + ca, a.c.ks + sa, head, r0, r1, t);
-    }
-    base += per_block;
+    const long long ca = kv_code_at(a.c, p.page, 0, p.slot - r0), sa = kv_scale_at(a.c, p.page, 0, p.slot - r0);
+    const bool keys = (pair & 1) == 0;
+    append_block<BF16, INTER, DIM>(a, keys ? a.k : a.v, keys && a.rot.table != nullptr, (keys ? a.c.k : a.c.v) + ca,
+                                   (keys ? a.c.ks : a.c.vs) + sa, head, a.slices * step, r0, r1, t, most);
   }
 }
 
@@ -407,9 +456,13 @@ cudaError_t launch_kv_rope(bool bf16, long long tokens, int heads, int dim, cons
 cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v,
                              const KvRotary &rot, int q_heads, const KvRows &q, const KvRows &q_out, int *status,
                              cudaStream_t st) {
-  AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, status};
+  AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, 0, status};
   a.window = window_of(s.tokens);
-  a.append_ctas = (int)((s.tokens + a.window - 1) / a.window);
+  // A CTA loops over the heads where there are blocks enough for two CTAs an
+  // SM; fewer take the heads side by side.
+  const int windows = (int)((s.tokens + a.window - 1) / a.window), most = (2 * c.heads + kPairs - 1) / kPairs;
+  a.slices = std::max(1, std::min(most, 2 * 148 / windows));
+  a.append_ctas = windows * a.slices;
   long long grid = a.append_ctas;
   if (q_heads) {
     rope_shape(s.tokens, q_heads, c.dim, a.q_hs, a.q_per_block);
