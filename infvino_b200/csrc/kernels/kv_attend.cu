@@ -6,7 +6,7 @@
 // in one pass with a running maximum m.  A decode step reads every visible
 // code once and does a few operations for each, so the cache's bytes bound it.
 //
-// An item is a tile of 8, 16 or 32 query rows (token, head of the group) of one
+// An item is a tile of 8 or 16 query rows (token, head of the group) of one
 // sequence and kv head; its units are the key blocks (16 keys that share a
 // scale).  All units of the launch are divided evenly over the CTAs, whatever
 // the sequences' lengths: a CTA's share is the rest of one item, some whole
@@ -85,6 +85,9 @@ __device__ __forceinline__ uint32_t tile_swizzle(uint32_t o) {
   return o ^ (f << 4);
 }
 
+// CTAs an SM, by registers (and, for wide heads, the rings)
+constexpr int step_ctas(int dim, int nt) { return nt == 1 && dim == 64 ? 4 : 3; }
+
 template <int DIM, int NT>
 struct StepSlot {  // partial sums of a cut item: accumulators lane by lane, then per row maximum and sum
   float acc[NT * DIM / 4 * 32];
@@ -106,7 +109,7 @@ struct StepShared {
 
 // NT: 8-row tiles of queries that share the codes of an item.
 template <bool BF16, int DIM, int NT>
-__global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
+__global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters) {
   extern __shared__ uint8_t smem_raw[];
   StepShared<DIM, NT> &sh = *reinterpret_cast<StepShared<DIM, NT> *>(smem_raw);
@@ -115,6 +118,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
   constexpr int kPiece = DIM / 8;       // head elements of a lane's piece
   constexpr int kAcc = NT * DIM / 4;    // accumulators a lane
   constexpr int kTile = kKvBlock * DIM;  // bytes of a block's keys or values
+  constexpr int kZ = 2;                  // blocks worked on at once
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait_and_release();
 
@@ -141,11 +145,14 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
     total += sh.scan[w];
   }
   if (total == 0) return;
-  const long long want = (total + kStepMinBlocks - 1) / kStepMinBlocks;
-  const int ctas = (int)(want < (long long)gridDim.x ? want : (long long)gridDim.x);
-  if ((int)blockIdx.x >= ctas) return;
-  long long u = share_begin(total, ctas, blockIdx.x);
-  const long long u_end = share_begin(total, ctas, blockIdx.x + 1);
+  if (total > 0x7fffffffLL) {  // (hours of work; units are counted in 32 bits from here)
+    if (threadIdx.x == 0) kv_flag(a.status, kStatusKvSeqs);
+    return;
+  }
+  const uint32_t size = max((uint32_t)kStepMinBlocks, ((uint32_t)total + gridDim.x - 1) / gridDim.x);  // units of a share
+  uint32_t u = blockIdx.x * size;
+  if (u >= (uint32_t)total) return;
+  const uint32_t u_end = min((uint32_t)total, u + size);
   const long long excl = before + incl - mine;
   if (u >= excl && u < excl + mine) {
     long long at = excl;
@@ -161,7 +168,9 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
   }
   __syncthreads();
   int b = sh.seq;
-  long long base = sh.base;  // first unit of sequence b
+  uint32_t base = (uint32_t)sh.base;  // first unit of sequence b
+  KvSpan s = kv_span(a, b);
+  int row_tiles = (s.n * a.group + kRows - 1) / kRows;
 
   // ---- this lane's places in a tile of codes
   const uint32_t ring = smem_u32(&sh.ring[warp][0][0][0]);
@@ -170,66 +179,79 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
   const uint32_t val_at0 = tile_swizzle<DIM>((uint32_t)(2 * t4 * DIM + g * kPiece)),
                  val_at1 = tile_swizzle<DIM>((uint32_t)((2 * t4 + 1) * DIM + g * kPiece));
 
-  while (u < u_end) {
-    // ---- the segment: blocks k0 .. k1 - 1 of item (b, head, row tile)
-    const KvSpan s = kv_span(a, b);
-    const int row_tiles = (s.n * a.group + kRows - 1) / kRows;
-    const long long units = (long long)s.blocks * row_tiles * a.cache.heads;
-    if (u >= base + units) {
+  // ---- the segment at u: blocks k0 .. k1 - 1 of item (b, head, row tile), and
+  // this warp's of them, k0 + warp, + kStepWarps, ...
+  int head = 0, rt = 0, k0 = 0, k1 = 0, count = 0, looked = 0;
+  uint32_t item_begin = 0;
+  long long where = -1;  // lane i: where the i-th of the next 32 blocks' codes are, -1: none
+  float2 sc_mine = make_float2(0.f, -1.f);
+  auto locate = [&]() {
+    for (;;) {
+      const uint32_t units = (uint32_t)s.blocks * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
+      if (u < base + units) break;
       base += units;
-      ++b;
-      continue;
+      s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+      row_tiles = (s.n * a.group + kRows - 1) / kRows;
     }
-    const long long item = (u - base) / s.blocks;
-    const int head = (int)(item / row_tiles), rt = (int)(item - (long long)head * row_tiles);
-    const long long item_begin = base + item * s.blocks, item_end = item_begin + s.blocks;
-    const int k0 = (int)(u - item_begin), k1 = (int)(min(u_end, item_end) - item_begin);
-
-    // ---- blocks k0 + warp, + kStepWarps, ...; lane i knows the i-th of the next 32
-    const int count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
-    const int first_block = k0 + warp;
-    long long where = -1;  // this lane's block's codes, -1: none
-    float2 sc_mine = make_float2(0.f, -1.f);
-    int looked = 0;
-    // A block is looked up 32 at a time and copied kStepStages ahead of the
-    // products; its scales wait beside its codes (a value scale below 0:
-    // nothing to see).
-    auto fetch = [&](int it) {
-      if (it < count) {
-        if (it == looked) {
-          looked += 32;
-          where = -1;
-          sc_mine = make_float2(0.f, -1.f);
-          if (it + lane < count) {
-            const int key = s.block(first_block + (it + lane) * kStepWarps) * kKvBlock;
-            if (key < s.len) {
-              const int page = kv_page_of(a.cache, a.seqs, b, key, a.status);
-              if (page >= 0) {
-                const int slot = key - fast_div(key, a.by_page) * a.cache.page;
-                where = kv_code_at(a.cache, page, head, slot);
-                const long long sa = kv_scale_at(a.cache, page, head, slot);
-                sc_mine = make_float2(a.cache.ks[sa], a.cache.vs[sa]);
-              }
+    const uint32_t item = (u - base) / (uint32_t)s.blocks;
+    head = (int)(item / (uint32_t)row_tiles);
+    rt = (int)item - head * row_tiles;
+    item_begin = base + item * (uint32_t)s.blocks;
+    k0 = (int)(u - item_begin);
+    k1 = (int)(min(u_end, item_begin + (uint32_t)s.blocks) - item_begin);
+    count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
+    looked = 0;
+  };
+  // A block is looked up 32 at a time and copied kStepStages ahead of the
+  // products; its scales wait beside its codes (a value scale below 0:
+  // nothing to see).
+  auto fetch = [&](int it) {
+    if (it < count) {
+      if (it == looked) {
+        looked += 32;
+        where = -1;
+        sc_mine = make_float2(0.f, -1.f);
+        if (it + lane < count) {
+          const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
+          if (key < s.len) {
+            const int at = fast_div(key, a.by_page), page = a.seqs.pages[(long long)b * a.seqs.pps + at];
+            if ((unsigned)page < (unsigned long long)a.cache.pages) {
+              const int slot = key - at * a.cache.page;
+              where = kv_code_at(a.cache, page, head, slot);
+              const long long sa = kv_scale_at(a.cache, page, head, slot);
+              sc_mine = make_float2(a.cache.ks[sa], a.cache.vs[sa]);
+            } else {
+              kv_flag(a.status, kStatusKvPage);
             }
           }
         }
-        const long long from = __shfl_sync(0xffffffffu, where, it & 31);
-        if (lane == (it & 31)) sh.scales[warp][it % kStepStages] = sc_mine;
-        if (from >= 0) {
-          const uint32_t dst = ring + (uint32_t)(it % kStepStages) * (2u * kTile);
-          const int8_t *kp = a.cache.k + from + lane * 16, *vp = a.cache.v + from + lane * 16;
-#pragma unroll
-          for (int i = 0; i < kTile / 512; ++i)
-            cp_async16(dst + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), kp + i * 512);
-#pragma unroll
-          for (int i = 0; i < kTile / 512; ++i)
-            cp_async16(dst + kTile + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), vp + i * 512);
-        }
       }
-      cp_async_commit();
-    };
+      const long long from = __shfl_sync(0xffffffffu, where, it & 31);
+      if (lane == (it & 31)) sh.scales[warp][it % kStepStages] = sc_mine;
+      if (from >= 0) {
+        const uint32_t dst = ring + (uint32_t)(it % kStepStages) * (2u * kTile);
+        const int8_t *kp = a.cache.k + from + lane * 16, *vp = a.cache.v + from + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kStepStages; ++i) fetch(i);
+        for (int i = 0; i < kTile / 512; ++i)
+          cp_async16(dst + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), kp + i * 512);
+#pragma unroll
+        for (int i = 0; i < kTile / 512; ++i)
+          cp_async16(dst + kTile + (uint32_t)(i >> 1) * 1024u + (i & 1 ? put1 : put0), vp + i * 512);
+      }
+    }
+    cp_async_commit();
+  };
+  // The join at a segment's end uses the last NT places of the ring; the first
+  // ones hold the next segment's first blocks by then.
+  constexpr int kAhead = kStepStages - NT;
+  locate();
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) fetch(i);
+
+  for (;;) {
+#pragma unroll
+    for (int i = kAhead; i < kStepStages; ++i) fetch(i);
+    const int first_block = k0 + warp;
 
     // ---- queries: column g of tile t for the products, columns 2 t4, + 1 for the scores
     uint32_t q[NT][kTiles][2];
@@ -292,18 +314,17 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
     }
     float vref = 0.f, vinv = 0.f;  // acc is in units of vref, the largest value scale so far
 
-    for (int it = 0; it < count; it += 2) {
-      cp_async_wait<kStepStages - 2>();
+    for (int it = 0; it < count; it += kZ) {
+      cp_async_wait<kStepStages - kZ>();
       __syncwarp();
-      const int st = it % kStepStages;  // (even: the pair is st, st + 1)
-      const bool two = it + 1 < count;
-      // scores of keys g, g + 8 of both blocks
-      float sc[2][NT][4];
-      float vs[2];
+      const int st = it % kStepStages;  // (a multiple of kZ)
+      // scores of keys g, g + 8 of each block
+      float sc[kZ][NT][4];
+      float vs[kZ];
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
+      for (int z = 0; z < kZ; ++z) {
         const float2 scales = sh.scales[warp][st + z];
-        vs[z] = z == 0 || two ? scales.y : -1.f;
+        vs[z] = z == 0 || it + z < count ? scales.y : -1.f;
         if (vs[z] < 0.f) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) sc[z][t][0] = sc[z][t][1] = sc[z][t][2] = sc[z][t][3] = -INFINITY;
@@ -347,10 +368,11 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          mx[t][c] = fmaxf(fmaxf(sc[0][t][c], sc[0][t][c + 2]), fmaxf(sc[1][t][c], sc[1][t][c + 2]));
+          mx[t][c] = fmaxf(sc[0][t][c], sc[0][t][c + 2]);
+          if (kZ == 2) mx[t][c] = fmaxf(mx[t][c], fmaxf(sc[kZ - 1][t][c], sc[kZ - 1][t][c + 2]));
           above = above || mx[t][c] > m[t][c] + kStepSlack;
         }
-      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[1]));
+      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[kZ - 1]));
       if (__any_sync(0xffffffffu, above) || vnew > vref) {
         const float vr = vref > 0.f ? __fdividef(vref, vnew) : 0.f;
 #pragma unroll
@@ -373,7 +395,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
         vinv = vref > 0.f ? 1.f / vref : 0.f;
       }
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
+      for (int z = 0; z < kZ; ++z) {
         if (vs[z] < 0.f) continue;
         const float vf = vs[z] * vinv;
         uint32_t p[NT][2];
@@ -422,11 +444,24 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
           }
         }
       }
-      __syncwarp();  // the pair's places have been read
-      fetch(it + kStepStages);
-      fetch(it + kStepStages + 1);
+      __syncwarp();  // their places have been read
+#pragma unroll
+      for (int z = 0; z < kZ; ++z) fetch(it + kStepStages + z);
     }
     cp_async_wait<0>();
+    __syncwarp();
+
+    // ---- what the join needs of this segment, then the next one's blocks on their way
+    const int n = s.n, first = s.first, head_now = head, rt_now = rt;
+    const bool begins = k0 == 0, whole = begins && k1 == s.blocks;
+    const int first_cta = (int)(item_begin / size), last_cta = (int)((item_begin + (uint32_t)s.blocks - 1u) / size);
+    u += (uint32_t)(k1 - k0);
+    const bool more = u < u_end;
+    if (more) {
+      locate();
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch(i);
+    }
 
     // ---- join the warps: row maxima, then sums in a common scale
 #pragma unroll
@@ -447,7 +482,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
     for (int w = 0; w < kStepWarps; ++w) all_v = fmaxf(all_v, sh.vref[w]);
     // accumulators lane by lane, [row tile][row of two][head element of the
     // piece]: eight neighbours of a lane are eight neighbouring outputs
-    float *part = reinterpret_cast<float *>(&sh.ring[warp][0][0][0]);
+    float *part = reinterpret_cast<float *>(&sh.ring[warp][kAhead][0][0]);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -464,14 +499,12 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
           for (int h = 0; h < 2; ++h) part[((2 * t + c) * kPiece + 2 * j + h) * 32 + lane] = acc[t][j][2 * h + c] * f;
       }
     __syncthreads();
-    const bool whole = k0 == 0 && k1 == s.blocks;
-    const int first_cta = share_of(total, ctas, item_begin), last_cta = share_of(total, ctas, item_end - 1);
-    const int slot = 2 * (int)blockIdx.x + (k0 == 0 ? 1 : 0);
+    const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
     if (!whole) {
       for (int e = threadIdx.x; e < kAcc * 32; e += kStepThreads) {
         float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < kStepWarps; ++w) x += reinterpret_cast<const float *>(&sh.ring[w][0][0][0])[e];
+        for (int w = 0; w < kStepWarps; ++w) x += reinterpret_cast<const float *>(&sh.ring[w][kAhead][0][0])[e];
         __stcg(&slots[slot].acc[e], x);
       }
       if (threadIdx.x < kRows) {
@@ -484,14 +517,16 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
         __stcg(&slots[slot].l[r], x);
         if (r == 0) __stcg(&slots[slot].vref, all_v);
       }
-      __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
+        __threadfence();  // (the CTA's writes, which the barrier has put before this)
         const unsigned parts = (unsigned)(last_cta - first_cta + 1);
-        const unsigned old = atomicAdd(&counters[first_cta], 1u);
-        sh.last = old == parts - 1;
-        if (sh.last) atomicExch(&counters[first_cta], 0u);
-        __threadfence();
+        const bool last = atomicAdd(&counters[first_cta], 1u) == parts - 1;
+        if (last) {
+          atomicExch(&counters[first_cta], 0u);
+          __threadfence();
+        }
+        sh.last = last;
       }
       __syncthreads();
     }
@@ -507,7 +542,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
           vr = all_v;
           for (int w = 0; w < kStepWarps; ++w) {
             if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) sum += sh.l[w][r] * fast_exp2(sh.m[w][r] - top);
-            const float *src = reinterpret_cast<const float *>(&sh.ring[w][0][0][0]) + i0 * 32 + ln;
+            const float *src = reinterpret_cast<const float *>(&sh.ring[w][kAhead][0][0]) + i0 * 32 + ln;
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] += src[32 * k];
           }
@@ -527,19 +562,19 @@ __global__ void __launch_bounds__(kStepThreads, NT == 4 ? 2 : 3)
             for (int k = 0; k < 8; ++k) x[k] += __ldcg(&sl.acc[(i0 + k) * 32 + ln]) * wv;
           }
         }
-        const int row = rt * kRows + r, i = fast_div(row, a.by_group);
-        if (i < s.n) {
+        const int row = rt_now * kRows + r, i = fast_div(row, a.by_group);
+        if (i < n) {
           const float y = sum != 0.f ? vr / sum : 0.f;  // (a NaN sum stays NaN)
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] *= y;
-          uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(s.first + i) * a.out.ts +
-                        (long long)(head * a.group + row - i * a.group) * a.out.hs;
+          uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(first + i) * a.out.ts +
+                        (long long)(head_now * a.group + row - i * a.group) * a.out.hs;
           store8(o + (ln >> 2) * kPiece + d0, pack8<BF16>(x), a.out.vec);
         }
       }
     }
+    if (!more) break;
     __syncthreads();  // the ring and the joins are free again
-    u += k1 - k0;
   }
 }
 
@@ -549,7 +584,7 @@ cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_
   const int bytes = (int)sizeof(StepShared<DIM, NT>);
   const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT>, bytes, attr_set);
   if (e != cudaSuccess) return e;
-  const int grid = sms * (NT == 4 ? 2 : 3);
+  const int grid = sms * step_ctas(DIM, NT);
   return launch_kernel(kv_step_k<BF16, DIM, NT>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
                        reinterpret_cast<StepSlot<DIM, NT> *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
                        static_cast<unsigned *>(workspace));
@@ -557,22 +592,26 @@ cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_
 
 template <bool BF16, int DIM>
 cudaError_t launch_step_rows(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
-  const long long rows = (long long)a.max_new * a.group;
-  if (rows <= 8) return launch_step<BF16, DIM, 1>(a, workspace, sms, st);
-  if (rows <= 16) return launch_step<BF16, DIM, 2>(a, workspace, sms, st);
-  return launch_step<BF16, DIM, 4>(a, workspace, sms, st);
+  // Rows beyond 16 come as further items: their codes are read again, from L2
+  // (24 sequences of 6001, 30 rows of 64 wide heads: 58 us; tiles of 32 rows,
+  // which read them once but leave room for half the warps, 65 us).
+  if ((long long)a.max_new * a.group <= 8) return launch_step<BF16, DIM, 1>(a, workspace, sms, st);
+  return launch_step<BF16, DIM, 2>(a, workspace, sms, st);
 }
 
 }  // namespace
 
 // Counters (zero before the first call and after each), then two slots a CTA.
 size_t kv_workspace_bytes(int sms) {
-  const size_t step = std::max(sizeof(StepSlot<128, 4>) * 4, sizeof(StepSlot<128, 2>) * 6) * (size_t)sms;
+  const size_t step = sizeof(StepSlot<128, 2>) * 2 * 4 * (size_t)sms;  // (the largest slot, the most CTAs)
   return kKvCounterBytes + std::max(step, kv_prompt_workspace_bytes(sms));
 }
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
-  if ((long long)a.max_new * a.group > 32 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, a, workspace, sms, st);
+  // Rows of one sequence and kv head: 24 sequences of up to 6001 tokens take the
+  // kernel for many queries 102 / 98 / 109 us at 64 / 96 / 128 rows (64 wide)
+  // and 144 us at 48 (128 wide), this one 99 / 125 / 173 and 116 us.
+  if ((long long)a.max_new * a.group > 64 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, a, workspace, sms, st);
   if (a.cache.dim == 64)
     return bf16 ? launch_step_rows<true, 64>(a, workspace, sms, st) : launch_step_rows<false, 64>(a, workspace, sms, st);
   return bf16 ? launch_step_rows<true, 128>(a, workspace, sms, st) : launch_step_rows<false, 128>(a, workspace, sms, st);

@@ -1,5 +1,4 @@
-// What the attention kernels share: which keys a sequence's queries see, and
-// the even division of all work over the CTAs of a launch.
+// What the attention kernels share: which keys a sequence's queries see.
 #pragma once
 
 #include "kv_common.cuh"
@@ -59,9 +58,5 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
 __device__ __forceinline__ bool kv_sees(const KvAttend &a, int p, int j) {
   return j <= p && (a.window == 0 || p - j < a.window || j < a.sinks);
 }
-
-// Bounds of CTA i's share of `total` units over n CTAs, and the CTA that has unit u.
-__device__ __forceinline__ long long share_begin(long long total, int n, int i) { return total * i / n; }
-__device__ __forceinline__ int share_of(long long total, int n, long long u) { return (int)(((u + 1) * n - 1) / total); }
 
 }  // namespace ivb
