@@ -195,13 +195,15 @@ __device__ __forceinline__ uint32_t halves(uint32_t w) {
   return r;
 }
 
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 // Sixteen codes as halves, to two 16-byte pieces of a row.
-__device__ __forceinline__ void put_codes(uint8_t *lo_at, uint8_t *hi_at, uint4 w4) {
+__device__ __forceinline__ void put_codes(uint32_t lo_at, uint32_t hi_at, uint4 w4) {
   const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
-  *reinterpret_cast<uint4 *>(lo_at) =
-      make_uint4(halves<0x4140>(w[0]), halves<0x4342>(w[0]), halves<0x4140>(w[1]), halves<0x4342>(w[1]));
-  *reinterpret_cast<uint4 *>(hi_at) =
-      make_uint4(halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
+  st_shared16(lo_at, halves<0x4140>(w[0]), halves<0x4342>(w[0]), halves<0x4140>(w[1]), halves<0x4342>(w[1]));
+  st_shared16(hi_at, halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
 }
 
 template <bool BF16, int DIM>
@@ -705,6 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = g->k0; t < g->k1; ++t, ++tile) {
         const int st = tile & 1;
         const bool reused = tile >= 2;
+        const uint32_t k_at = smem_u32(&sh.k[0][0][0]) + (uint32_t)(st * sizeof(sh.k[0])), v_at = smem_u32(&sh.v[0][0][0]) + (uint32_t)(st * sizeof(sh.v[0]));
         if (reused) wait(smem_u32(&sh.kempty[st]), ((tile >> 1) - 1) & 1, kStatusTimeoutEmpty);
         if (w == 0) {  // the scales
           float vmax = now.vs;
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
-          put_codes(&sh.k[st][e / 4][put_lo + 1024 * (e % 4)], &sh.k[st][e / 4][put_hi + 1024 * (e % 4)], kreg[e]);
+          put_codes(k_at + put_lo + 16384 * (e / 4) + 1024 * (e % 4), k_at + put_hi + 16384 * (e / 4) + 1024 * (e % 4), kreg[e]);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.kfull[st]));
@@ -735,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (reused) wait(smem_u32(&sh.vempty[st]), ((tile >> 1) - 1) & 1, kStatusTimeoutEmpty);
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
-          put_codes(&sh.v[st][e / 4][put_lo + 1024 * (e % 4)], &sh.v[st][e / 4][put_hi + 1024 * (e % 4)], vreg[e]);
+          put_codes(v_at + put_lo + 16384 * (e / 4) + 1024 * (e % 4), v_at + put_hi + 16384 * (e / 4) + 1024 * (e % 4), vreg[e]);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.vfull[st]));
