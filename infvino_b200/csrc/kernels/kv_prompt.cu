@@ -453,26 +453,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait(smem_u32(&sh.sfull[i][h]), done & 1, kStatusTimeoutAcc)) continue;
           tc_fence_after();
           const uint32_t s_at = tmem + lanes + (uint32_t)(2 * i + h) * kSub;
-          float s[kSub];
-          tmem_ld32(s_at, s);
-          tmem_ld32(s_at + 32, s + 32);
           const int b0 = 4 * h;  // its blocks
-          const bool masked = part > part_hi || (part < part_lo && part >= part_sink);
-          ++part;
-          tmem_ld_wait();
-#pragma unroll
-          for (int k = 0; k < kSub; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
-          if (masked) {  // hidden keys: behind the row, before its window, behind the end
-#pragma unroll
+          // Hidden keys (behind the row, before its window, behind the end)
+          // are put out in TMEM, block by block, before the scores are read:
+          // few parts need it, and the code that all parts run stays straight.
+          if (part > part_hi || (part < part_lo && part >= part_sink)) {
+#pragma unroll 1
             for (int b = 0; b < 4; ++b) {
               const int hi = p - me.key0[b0 + b];
               uint32_t seen = low_bits(hi + 1);
               if (a.window > 0) seen &= ~low_bits(hi - a.window + 1) | low_bits(a.sinks - me.key0[b0 + b]);
+              if (__all_sync(0xffffffffu, seen == 0xffffu)) continue;
+              uint32_t w[16];
+              tmem_ld16(s_at + 16 * b, w);
+              tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < kKvBlock; ++k)
-                if (!(seen >> k & 1)) s[kKvBlock * b + k] = -INFINITY;
+              for (int k = 0; k < kKvBlock; ++k) {
+                asm volatile("" : "+r"(w[k]));
+                if (!(seen >> k & 1)) w[k] = 0xff800000u;  // -inf
+              }
+              tmem_st16(s_at + 16 * b, w);
             }
+            tmem_st_wait();
           }
+          ++part;
+          float s[kSub];
+          tmem_ld32(s_at, s);
+          tmem_ld32(s_at + 32, s + 32);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < kSub; ++k) asm volatile("" : "+f"(s[k]));  // uses stay after the wait
           const float4 kc4 = *reinterpret_cast<const float4 *>(&me.kc[b0]);
           const float4 lv4 = *reinterpret_cast<const float4 *>(&me.lvf[b0]), iv4 = *reinterpret_cast<const float4 *>(&me.ivf[b0]);
           float c[4] = {kc4.x, kc4.y, kc4.z, kc4.w}, mx = -INFINITY;
