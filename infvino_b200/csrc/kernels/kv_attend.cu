@@ -20,8 +20,10 @@
 // conflict), and multiplies with m16n8k16 tensor instructions, transposed
 // (keys, then head elements, are the 16 rows; queries the 8 columns), so that
 // a handful of queries fills an instruction and a code is converted once for
-// all of them.  Codes become halves exactly (1024 + code + 128 by a byte
-// permutation, minus 1152).  The order of head elements and keys inside the
+// all of them.  Value codes become halves exactly (1024 + code +
+// 128 by a byte permutation, minus 1152); key codes stay code + 128, and 128
+// times the query's sum comes off the score: an offset far below the score's
+// error bound, where for the values it would cost bits.  The order of head elements and keys inside the
 // products is chosen so that every lane reads whole 16-byte (64-wide heads:
 // 8-byte) pieces of a row; the weights turn into the second product's operand
 // by transposing 8 x 8 pieces in registers.
@@ -65,7 +67,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// Two codes (+ 128, in bytes LO, LO + 1 of w) as halves.
+// Two codes (+ 128, in bytes of w) as halves 2^-24 (code + 128): the bytes are
+// the last bits of subnormal halves, which the tensor cores multiply exactly.
+template <int SEL>
+__device__ __forceinline__ uint32_t tiny2(uint32_t w) {
+  return __byte_perm(w, 0u, SEL);
+}
+constexpr float kTiny = 0x1p-24f;
+
+// Two codes (+ 128, in bytes of w) as halves.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     // ---- queries: column g of tile t for the products, columns 2 t4, + 1 for the scores
     uint32_t q[NT][kTiles][2];
     int pos[NT][2];
-    float rs[NT][2];
+    float rs[NT][2], qo[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = rt * kRows + 8 * t + g, i = fast_div(r, a.by_group);
@@ -270,7 +280,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         w[8 * c] = x.x, w[8 * c + 1] = x.y, w[8 * c + 2] = x.z, w[8 * c + 3] = x.w;
         w[8 * c + 4] = y.x, w[8 * c + 5] = y.y, w[8 * c + 6] = y.z, w[8 * c + 7] = y.w;
       }
-      float up = a.scale * kLog2e;
+      float up = a.scale * kLog2e / kTiny;
       if (BF16) {
         // bf16 queries become halves: the row is scaled by a power of two so
         // that its largest element lies in 2^0 .. 2^1 (its eight bits stay)
@@ -293,11 +303,20 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       }
 #pragma unroll
       for (int k = 0; k < kTiles; ++k) q[t][k][0] = w[2 * k], q[t][k][1] = w[2 * k + 1];
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * kTiles; ++k) {
+        const float2 f = unpack2<false>(w[k]);
+        sum += f.x + f.y;
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int rc = rt * kRows + 8 * t + 2 * t4 + c, ic = fast_div(rc, a.by_group);
         pos[t][c] = ic < s.n ? s.len - s.n + ic : -1;
         rs[t][c] = BF16 ? __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4) : up;  // (lane of column 2 t4 + c)
+        qo[t][c] = __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4) * (-128.f * kTiny);
       }
     }
     const int p_lo = s.len - s.n + fast_div(rt * kRows, a.by_group);                                  // first row's position
@@ -341,8 +360,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
           const uint32_t yw[4] = {y.x ^ 0x80808080u, y.y ^ 0x80808080u, y.z ^ 0x80808080u, y.w ^ 0x80808080u};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t a0 = codes2<0x4140>(xw[i]), a1 = codes2<0x4140>(yw[i]), a2 = codes2<0x4342>(xw[i]),
-                           a3 = codes2<0x4342>(yw[i]);
+            const uint32_t a0 = tiny2<0x4140>(xw[i]), a1 = tiny2<0x4140>(yw[i]), a2 = tiny2<0x4342>(xw[i]),
+                           a3 = tiny2<0x4342>(yw[i]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) mma16816(sc[z][t], a0, a1, a2, a3, q[t][4 * c + i][0], q[t][4 * c + i][1]);
           }
@@ -350,8 +369,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         const int key0 = s.block(first_block + (it + z) * kStepWarps) * kKvBlock;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float f0 = rs[t][0] * scales.x, f1 = rs[t][1] * scales.x;
-          sc[z][t][0] *= f0, sc[z][t][1] *= f1, sc[z][t][2] *= f0, sc[z][t][3] *= f1;
+          // (q . (code + 128) - 128 sum q, in the units of the products)
+          const float f0 = rs[t][0] * scales.x, f1 = rs[t][1] * scales.x, o0 = qo[t][0] * f0, o1 = qo[t][1] * f1;
+          sc[z][t][0] = fmaf(sc[z][t][0], f0, o0);
+          sc[z][t][1] = fmaf(sc[z][t][1], f1, o1);
+          sc[z][t][2] = fmaf(sc[z][t][2], f0, o0);
+          sc[z][t][3] = fmaf(sc[z][t][3], f1, o1);
         }
         if (key0 + kKvBlock - 1 > p_lo || (a.window > 0 && p_hi - key0 >= a.window && key0 + kKvBlock > a.sinks)) {
 #pragma unroll
