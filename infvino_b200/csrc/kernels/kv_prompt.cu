@@ -114,6 +114,17 @@ struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 row
 __device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; }
 
 __device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// Whether all 128 threads say so.
+__device__ __forceinline__ bool wg_all(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
+      "barrier.cta.red.and.pred p, %1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void reg_inc() {
@@ -411,14 +422,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the next segment with rows for this M tile; its queries follow at once,
     // before the outputs of the one that is ending
     auto advance = [&]() {
-      while ((g = next_segment())) {
+      for (;;) {
+        g = next_segment();
+        // (the four warps end together, also where a bounded wait ran out: they share barriers)
+        if (!wg_all(1 + i, g != nullptr)) return false;
         if (g->s.n * a.group > g->rt * kRows + 128 * i) {
           load_q();
           return true;
         }
         tile += g->k1 - g->k0;
       }
-      return false;
     };
     bool more = advance();
     while (more) {
