@@ -522,6 +522,10 @@ def test_refusals(ops):
         ops.attend(cache, q, out, offs.long(), lens, table, max_new=1)
     with pytest.raises(ValueError):
         ops.attend(cache, q[..., ::2], out, offs, lens, table, max_new=1)
+    for args in ((cache, q.cpu(), out, offs, lens, table), (cache, q, out.cpu(), offs, lens, table), (cache, q, out, offs, lens.cpu(), table),
+                 (ivb.KvCache(*[t.cpu() for t in cache_t]), q, out, offs, lens, table)):
+        with pytest.raises(ValueError):  # host memory
+            ops.attend(*args, max_new=1)
     for bad in (dict(max_new=0), dict(max_new=1, window=-1), dict(max_new=1, sinks=-2)):
         with pytest.raises(ivb.NativeError) as e:
             ops.attend(cache, q, out, offs, lens, table, **bad)

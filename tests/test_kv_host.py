@@ -27,12 +27,14 @@ def test_rotary_descriptor():
     table = torch.zeros((10, 16, 2))
     r = ivb.Rotary(table, [0] * 8 + [2] * 8)
     assert r.axes == 3
-    c = _native.ROTARY.unpack(r.at(torch.zeros((3, 5), dtype=torch.int32), 5))
+    c = _native.ROTARY.unpack(r.at(torch.zeros((3, 5), dtype=torch.int32), 5, -1))
     assert c[1:5] == (10, 16, 3, 0) and c[6] == 5
     for pos in (torch.zeros((2, 5), dtype=torch.int32), torch.zeros(5, dtype=torch.int32), torch.zeros((3, 4), dtype=torch.int32),
                 torch.zeros((3, 5), dtype=torch.int64)):
         with pytest.raises(ValueError):
-            r.at(pos, 5)
+            r.at(pos, 5, -1)
+    with pytest.raises(ValueError):  # host memory, for a handle on device 0
+        r.at(torch.zeros((3, 5), dtype=torch.int32), 5, 0)
     with pytest.raises(ValueError):
         ivb.Rotary(table, [0] * 15)
     with pytest.raises(ValueError):
