@@ -609,21 +609,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         __stcg(&slot.m[row], m);
         __stcg(&slot.l[row], l);
         if (row == 0) __stcg(&slot.vref, vref);
-        __threadfence();
       }
       if (!whole) {
         wg_sync(1 + i);
         if (row == 0) {
+          __threadfence();  // (the four warps' writes, which the barrier has put before this)
           const unsigned parts = (unsigned)(last_cta - first_cta + 1);
-          const unsigned old = atomicAdd(&counters[2 * first_cta + i], 1u);
-          sh.last[i] = old == parts - 1;
-          if (old == parts - 1) atomicExch(&counters[2 * first_cta + i], 0u);
-          __threadfence();
+          const bool last = atomicAdd(&counters[2 * first_cta + i], 1u) == parts - 1;
+          if (last) {
+            atomicExch(&counters[2 * first_cta + i], 0u);
+            __threadfence();
+          }
+          sh.last[i] = last;
         }
         wg_sync(1 + i);
         if (sh.last[i] && real && ok) {
           float top = -INFINITY, vmax = 0.f, sum = 0.f;
-#pragma unroll 1
+          // (several parts' loads at once: a short call over a long cache has many)
+#pragma unroll 4
           for (int z = first_cta; z <= last_cta; ++z) {
             const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
             top = fmaxf(top, __ldcg(&sl.m[row]));
@@ -635,12 +638,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) x[k] = 0.f;
             sum = 0.f;
-#pragma unroll 1
+#pragma unroll 2
             for (int z = first_cta; z <= last_cta; ++z) {
               const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
-              const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]);
-              if (zm == -INFINITY && zl == 0.f) continue;  // this part of the keys was hidden from the row
-              const float w = fast_exp2(zm - top), wv = vmax > 0.f ? w * __fdividef(__ldcg(&sl.vref), vmax) : 0.f;
+              const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]), zv = __ldcg(&sl.vref);
+              // (a part of the keys that was hidden from the row: 0)
+              const float w = zm == -INFINITY && zl == 0.f ? 0.f : fast_exp2(zm - top), wv = vmax > 0.f ? w * __fdividef(zv, vmax) : 0.f;
               sum += zl * w;
 #pragma unroll
               for (int k = 0; k < 32; k += 4) {
