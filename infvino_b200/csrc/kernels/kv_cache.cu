@@ -2,8 +2,11 @@
 // the append (rotation, block scales and codes in one pass) and the read.
 //
 // All four move bytes: a few operations for each element that is read and
-// written once.  Sixteen elements (eight pairs) of a row are a thread's share;
-// a warp reads whole 128-byte lines of the two halves of a head.
+// written once, so memory bounds long calls and the chain of dependent loads
+// (sequence, page, position, angles) short ones.  Sixteen elements (eight
+// pairs) of a row are a thread's share; a warp reads whole 128-byte lines of
+// the two halves of a head.  Rows that cannot be read 16 bytes at a time have
+// kernels of their own: the slow path beside the fast one cost the latter 9 %.
 #include <algorithm>
 #include <type_traits>
 
@@ -89,16 +92,20 @@ __global__ void kv_rope_table_k(const __grid_constant__ KvRopeFreq f, int pairs,
   }
 }
 
+// Heads a thread turns by the same angles at once: what hides the chain from
+// position to table row is the rows in flight meanwhile, 2 x 16 bytes a head,
+// more than the number of warps.  16381 tokens, 28 heads of 128: 44 us, 5.3
+// TB/s (floor 36); 4 heads and three CTAs an SM 47, 2 heads and four 50.
 constexpr int kRopeThreads = 256;
-constexpr int kRopeHeads = 4;  // heads a thread turns by the same angles at once
+constexpr int kRopeHeads = 8;
 
 // Turns the rows of token tile `tile`.  A token takes hs * (dim / 16) threads;
 // thread (head h0, group g) turns heads h0, h0 + hs, ...
-template <bool BF16, bool INTER>
+template <bool BF16, bool INTER, bool VEC, int HEADS>
 __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int heads, int dim, int hs, int per_block,
                                           const KvRows &x, const KvRows &out, const KvRotary &rot, int *status) {
   const int groups = dim / 16, upt = hs * groups;
-  for (int u = threadIdx.x; u < upt * per_block; u += kRopeThreads) {
+  for (int u = threadIdx.x; u < upt * per_block; u += (int)blockDim.x) {
     const int tl = u / upt, r = u - tl * upt, h0 = r / groups, g = r - h0 * groups;
     const long long token = tile * per_block + tl;
     if (token >= tokens) break;
@@ -109,19 +116,19 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
     uint16_t *yr = static_cast<uint16_t *>(out.p) + token * out.ts;
     Turn t;
     bool ok = true;
-    for (int h = h0; h < heads; h += kRopeHeads * hs) {
+    for (int h = h0; h < heads; h += HEADS * hs) {
       // the rows are on their way before the angles' chain (position, then table) begins
-      uint4 ua[kRopeHeads], ub[kRopeHeads];
+      uint4 ua[HEADS], ub[HEADS];
 #pragma unroll
-      for (int i = 0; i < kRopeHeads; ++i)
+      for (int i = 0; i < HEADS; ++i)
         if (h + i * hs < heads) {
-          ua[i] = load8(xr + (h + i * hs) * x.hs + ea, x.vec);
-          ub[i] = load8(xr + (h + i * hs) * x.hs + eb, x.vec);
+          ua[i] = load8(xr + (h + i * hs) * x.hs + ea, VEC);
+          ub[i] = load8(xr + (h + i * hs) * x.hs + eb, VEC);
         }
       if (h == h0 && turned) ok = load_turn(rot, g, token, t, status);
       if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < kRopeHeads; ++i)
+      for (int i = 0; i < HEADS; ++i)
         if (h + i * hs < heads) {
           if (turned) {
             float a[8], b[8];
@@ -131,19 +138,19 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
             ua[i] = pack8<BF16>(a);
             ub[i] = pack8<BF16>(b);
           }
-          store8(yr + (h + i * hs) * out.hs + ea, ua[i], out.vec);
-          store8(yr + (h + i * hs) * out.hs + eb, ub[i], out.vec);
+          store8(yr + (h + i * hs) * out.hs + ea, ua[i], VEC);
+          store8(yr + (h + i * hs) * out.hs + eb, ub[i], VEC);
         }
     }
   }
 }
 
-template <bool BF16, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads, 3)
+template <bool BF16, bool INTER, bool VEC>
+__global__ void __launch_bounds__(kRopeThreads, 2)
     kv_rope_k(long long tokens, int heads, int dim, int hs, int per_block, const __grid_constant__ KvRows x,
               const __grid_constant__ KvRows out, const __grid_constant__ KvRotary rot, int *status) {
   pdl_wait_and_release();
-  rope_tile<BF16, INTER>(blockIdx.x, tokens, heads, dim, hs, per_block, x, out, rot, status);
+  rope_tile<BF16, INTER, VEC, kRopeHeads>(blockIdx.x, tokens, heads, dim, hs, per_block, x, out, rot, status);
 }
 
 // ---------------------------------------------------------------- append
@@ -195,24 +202,29 @@ __device__ __forceinline__ uint32_t requantise4(uint32_t w, float ratio) {
   return o;
 }
 
-constexpr int kPair = 2;                               // warps that share a block
-constexpr int kPairs = kRopeThreads / 32 / kPair;
+constexpr int kAppendThreads = 256;
+constexpr int kAppendHeads = 4;  // query heads a thread turns at once: more would cost every CTA its registers
+// Warps that share a block: with DIM / 32 of them a lane has sixteen elements
+// of one of its rows, with half as many of two.
+template <int TEAM>
+__device__ __forceinline__ void team_sync(int team) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
+}
+constexpr int append_ctas(int dim, int team) { return team == dim / 32 ? 3 : 2; }  // an SM, by registers
 
-__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); }
-
-// Two warps: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
+// TEAM warps: the new tokens of one block (rows r0 .. r1 - 1 of its 16, packed
 // tokens from t0), keys or values (`codes`, `scales`: head 0's), of heads
-// head, head + step, ...  A warp takes eight of the rows; lane (row l /
+// head, head + step, ...  A warp takes 16 / TEAM of the rows; lane (row l /
 // groups, group l % groups) holds sixteen elements of every (32 / groups)-th.
 // A token's angles are loaded once for all heads, and a head's rows while the
 // one before is worked on.
-template <bool BF16, bool INTER, int DIM>
+template <bool BF16, bool INTER, int DIM, bool VEC, int TEAM>
 __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &x, bool turn, int8_t *codes,
                                              float *scales, int head, int step, int r0, int r1, long long t0,
                                              float *shared) {
-  constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows / kPair;
-  const int lane = threadIdx.x & 31, g = lane % kGroups, warp = threadIdx.x >> 5, pair = warp / kPair;
-  const int row0 = warp % kPair * (kKvBlock / kPair) + lane / kGroups;
+  constexpr int kGroups = DIM / 16, kRows = 32 / kGroups, kSteps = kKvBlock / kRows / TEAM;
+  const int lane = threadIdx.x & 31, g = lane % kGroups, warp = threadIdx.x >> 5, team = warp / TEAM;
+  const int row0 = warp % TEAM * (kKvBlock / TEAM) + lane / kGroups;
   const int pairs = turn ? a.rot.pairs : 0;
   int ea, eb;
   group_at<INTER>(g, pairs, ea, eb);
@@ -228,8 +240,8 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
       ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
       if (r >= r0 && r < r1) {
         const uint16_t *row = xt + (r - r0) * x.ts + h * x.hs;
-        ua[i] = load8(row + ea, x.vec);
-        ub[i] = load8(row + eb, x.vec);
+        ua[i] = load8(row + ea, VEC);
+        ub[i] = load8(row + eb, VEC);
       }
     }
   };
@@ -238,9 +250,10 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) shared[warp] = m;
-    pair_sync(pair);
-    m = max_abs(shared[pair * kPair], shared[pair * kPair + 1]);
-    pair_sync(pair);
+    team_sync<TEAM>(team);
+#pragma unroll
+    for (int w = 0; w < TEAM; ++w) m = max_abs(m, shared[team * TEAM + w]);
+    team_sync<TEAM>(team);
     return m;
   };
   load(head);
@@ -294,7 +307,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
       }
       e = max(e, eo);
     }
-    if (warp % kPair == 0 && lane == 0) scales[(long long)head * (a.c.page / kKvBlock)] = exp2i(e);  // (both have read the old one)
+    if (warp % TEAM == 0 && lane == 0) scales[(long long)head * (a.c.page / kKvBlock)] = exp2i(e);  // (all have read the old one)
     const float inv = exp2i(-e);
     if (odd || e == kKvMaxExp) {
       const float top = 127.f * exp2i(e);
@@ -350,24 +363,28 @@ __device__ __forceinline__ void find_places(const KvCache &c, const KvSeqs &s, l
 }
 
 // Of the first `append_ctas` CTAs each takes the blocks whose first new token
-// is among `window` packed tokens, and every `slices`-th pair of heads of
-// them: two warps for a head's keys, two for its values.  A block is one
-// pair's alone, so nothing is atomic and the result does not depend on any
+// is among `window` packed tokens, and every `slices`-th set of heads of
+// them: a team of warps for a head's keys, one for its values.  A block is one
+// team's alone, so nothing is atomic and the result does not depend on any
 // order.  The other CTAs turn queries.
-template <bool BF16, bool INTER, int DIM>
-__global__ void __launch_bounds__(kRopeThreads, 2) kv_append_k(const __grid_constant__ AppendArgs a) {
+//
+// Latency bounds it: two joins and a block's loads for each head in turn.  9412
+// tokens, 8 heads of 128 beside 32 of queries: 44 us, 4.8 TB/s (floor 32); 64
+// conversations, a token each: 4.3 us.
+template <bool BF16, bool INTER, int DIM, bool VEC, int TEAM>
+__global__ void __launch_bounds__(kAppendThreads, append_ctas(DIM, TEAM)) kv_append_k(const __grid_constant__ AppendArgs a) {
   __shared__ Place places[kKvBlock];
-  __shared__ float most[kRopeThreads / 32];
+  __shared__ float most[kAppendThreads / 32];
   pdl_wait_and_release();
   if ((int)blockIdx.x >= a.append_ctas) {
-    rope_tile<BF16, INTER>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs, a.q_per_block, a.q, a.q_out,
-                    a.rot, a.status);
+    rope_tile<BF16, INTER, VEC, kAppendHeads>((int)blockIdx.x - a.append_ctas, a.s.tokens, a.q_heads, DIM, a.q_hs,
+                                              a.q_per_block, a.q, a.q_out, a.rot, a.status);
     return;
   }
   const long long first = (long long)(blockIdx.x / a.slices) * a.window;
   find_places(a.c, a.s, first, a.window, a.status, places);
-  const int pair = (threadIdx.x >> 5) / kPair, step = kPairs / 2;  // heads a CTA works on at once
-  const int head = (blockIdx.x % a.slices) * step + (pair >> 1);
+  constexpr int kTeams = kAppendThreads / 32 / TEAM, step = kTeams / 2;  // heads a CTA works on at once
+  const int team = (threadIdx.x >> 5) / TEAM, head = (blockIdx.x % a.slices) * step + (team >> 1);
   for (int i = 0; i < a.window; ++i) {
     const Place p = places[i];
     const long long t = first + i;
@@ -375,44 +392,60 @@ __global__ void __launch_bounds__(kRopeThreads, 2) kv_append_k(const __grid_cons
     if (p.page < 0 || (t != p.first && r0 != 0)) continue;
     const int r1 = (int)min((long long)kKvBlock, r0 + (p.end - t));  // a block begins here
     const long long ca = kv_code_at(a.c, p.page, 0, p.slot - r0), sa = kv_scale_at(a.c, p.page, 0, p.slot - r0);
-    const bool keys = (pair & 1) == 0;
-    append_block<BF16, INTER, DIM>(a, keys ? a.k : a.v, keys && a.rot.table != nullptr, (keys ? a.c.k : a.c.v) + ca,
-                                   (keys ? a.c.ks : a.c.vs) + sa, head, a.slices * step, r0, r1, t, most);
+    const bool keys = (team & 1) == 0;
+    append_block<BF16, INTER, DIM, VEC, TEAM>(a, keys ? a.k : a.v, keys && a.rot.table != nullptr, (keys ? a.c.k : a.c.v) + ca,
+                                        (keys ? a.c.ks : a.c.vs) + sa, head, a.slices * step, r0, r1, t, most);
   }
 }
 
 // ---------------------------------------------------------------- read
 
-// Sixteen values a thread: a CTA takes `window` packed tokens, all heads.
+// A CTA takes `window` packed tokens, all heads.  A thread keeps its place in
+// the rows (keys or values, head, eight elements: 16 bytes out, so that a warp
+// writes whole lines) and goes over the tokens, kReadAhead of them on their way
+// at once.  9412 tokens, 8 heads of 128: 10.2 us, 5.7 TB/s (floor 8.9); sixteen
+// elements a thread, in two stores, 17.4.
+constexpr int kReadAhead = 4, kReadThreads = 256;
 template <bool BF16, int DIM>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kReadThreads)
     kv_read_k(const __grid_constant__ KvCache c, const __grid_constant__ KvSeqs s, const __grid_constant__ KvRows k,
               const __grid_constant__ KvRows v, int window, int *status) {
   __shared__ Place places[kKvBlock];
   pdl_wait_and_release();
-  constexpr int kGroups = DIM / 16;
+  constexpr int kGroups = DIM / 8;
   const long long first = (long long)blockIdx.x * window;
+  const int each = ((k.p ? 1 : 0) + (v.p ? 1 : 0)) * c.heads * kGroups;
+  const int lanes = min(each, kReadThreads), step = kReadThreads / lanes;
+  const int i0 = threadIdx.x / lanes;
   find_places(c, s, first, window, status, places);
-  const int halves = (k.p ? 1 : 0) + (v.p ? 1 : 0), each = halves * c.heads * kGroups;
-  for (int u = threadIdx.x; u < window * each; u += blockDim.x) {
-    const int i = u / each, w0 = u - i * each;
-    const int g = w0 % kGroups, hh = w0 / kGroups;
+  if (i0 >= step) return;
+  for (int u = threadIdx.x - i0 * lanes; u < each; u += lanes) {
+    const int g = u % kGroups, hh = u / kGroups;
     const bool val = hh >= c.heads || !k.p;
     const int head = hh >= c.heads ? hh - c.heads : hh;
-    const Place &p = places[i];
-    if (p.page < 0) continue;
+    const int8_t *codes = (val ? c.v : c.k) + kv_code_at(c, 0, head, 0) + 8 * g;
+    const float *scales = (val ? c.vs : c.ks) + kv_scale_at(c, 0, head, 0);
     const KvRows &y = val ? v : k;
-    const long long ca = kv_code_at(c, p.page, head, p.slot) + 16 * g;
-    const float sc = (val ? c.vs : c.ks)[kv_scale_at(c, p.page, head, p.slot)];
-    const uint4 w = *reinterpret_cast<const uint4 *>((val ? c.v : c.k) + ca);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    uint16_t *row = static_cast<uint16_t *>(y.p) + (first + i) * y.ts + head * y.hs + 16 * g;
+    uint16_t *rows = static_cast<uint16_t *>(y.p) + first * y.ts + head * y.hs + 8 * g;
+    for (int i = i0; i < window; i += kReadAhead * step) {
+      uint2 w[kReadAhead];
+      float sc[kReadAhead];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[8];
+      for (int n = 0; n < kReadAhead; ++n) {
+        const int j = i + n * step;
+        if (j >= window || places[j].page < 0) continue;
+        w[n] = *reinterpret_cast<const uint2 *>(codes + kv_code_at(c, places[j].page, 0, places[j].slot));
+        sc[n] = scales[kv_scale_at(c, places[j].page, 0, places[j].slot)];
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(ws[2 * h + (j >> 2)] >> (8 * (j & 3))) * sc;
-      store8(row + 8 * h, pack8<BF16>(f), y.vec);
+      for (int n = 0; n < kReadAhead; ++n) {
+        const int j = i + n * step;
+        if (j >= window || places[j].page < 0) continue;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)((e < 4 ? w[n].x : w[n].y) >> (8 * (e & 3))) * sc[n];
+        store8(rows + j * y.ts, pack8<BF16>(f), y.vec);
+      }
     }
   }
 }
@@ -426,12 +459,13 @@ int window_of(long long tokens) {
 }
 
 // Head groups of the rotation: one head a thread while that leaves SMs free,
-// kRopeHeads (angles loaded once for them) from there on.
-void rope_shape(long long tokens, int heads, int dim, int &hs, int &per_block) {
+// up to `most` (angles loaded once for them) from there on.
+void rope_shape(long long tokens, int heads, int dim, int most, int threads, int &hs, int &per_block) {
   const int groups = dim / 16;
-  const bool many = tokens * heads * groups >= 148LL * 2048;
-  hs = many ? (heads + kRopeHeads - 1) / kRopeHeads : heads;
-  per_block = std::max(1, kRopeThreads / (hs * groups));
+  const long long work = tokens * heads * groups / 148;
+  const int each = work < 2048 ? 1 : work < 8192 ? std::min(4, most) : most;
+  hs = (heads + each - 1) / each;
+  per_block = std::max(1, threads / (hs * groups));
 }
 
 }  // namespace
@@ -445,10 +479,16 @@ cudaError_t launch_kv_rope_table(const KvRopeFreq &f, int pairs, long long posit
 cudaError_t launch_kv_rope(bool bf16, long long tokens, int heads, int dim, const KvRows &x, const KvRows &out,
                            const KvRotary &rot, int *status, cudaStream_t st) {
   int hs, per_block;
-  rope_shape(tokens, heads, dim, hs, per_block);
+  rope_shape(tokens, heads, dim, kRopeHeads, kRopeThreads, hs, per_block);
   const dim3 grid((unsigned)((tokens + per_block - 1) / per_block));
-  auto kern = rot.interleaved ? (bf16 ? kv_rope_k<true, true> : kv_rope_k<false, true>)
-                              : (bf16 ? kv_rope_k<true, false> : kv_rope_k<false, false>);
+  auto types = [&](auto inter, auto vec) {
+    constexpr bool kInter = decltype(inter)::value, kVec = decltype(vec)::value;
+    return bf16 ? kv_rope_k<true, kInter, kVec> : kv_rope_k<false, kInter, kVec>;
+  };
+  auto pick = [&](auto inter) {
+    return x.vec && out.vec ? types(inter, std::true_type{}) : types(inter, std::false_type{});
+  };
+  auto kern = rot.interleaved ? pick(std::true_type{}) : pick(std::false_type{});
   return launch_kernel(kern, grid, dim3(kRopeThreads), 0, st, tokens, heads, dim,
                        hs, per_block, x, out, rot, status);
 }
@@ -458,23 +498,32 @@ cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const
                              cudaStream_t st) {
   AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, 0, status};
   a.window = window_of(s.tokens);
+  // Two warps a block where most blocks get a token or two (64 conversations, 8
+  // heads: 4.3 us; four warps 5.0), one row a lane where they are filled (9412
+  // tokens: 47 us; 53).
+  const int team = a.window == 1 ? 2 : c.dim / 32, teams = kAppendThreads / 32 / team;
   // A CTA loops over the heads where there are blocks enough for two CTAs an
   // SM; fewer take the heads side by side.
-  const int windows = (int)((s.tokens + a.window - 1) / a.window), most = (2 * c.heads + kPairs - 1) / kPairs;
+  const int windows = (int)((s.tokens + a.window - 1) / a.window), most = (2 * c.heads + teams - 1) / teams;
   a.slices = std::max(1, std::min(most, 2 * 148 / windows));
   a.append_ctas = windows * a.slices;
   long long grid = a.append_ctas;
   if (q_heads) {
-    rope_shape(s.tokens, q_heads, c.dim, a.q_hs, a.q_per_block);
+    rope_shape(s.tokens, q_heads, c.dim, kAppendHeads, kAppendThreads, a.q_hs, a.q_per_block);
     grid += (s.tokens + a.q_per_block - 1) / a.q_per_block;
   }
+  auto dims = [&](auto inter, auto vec, auto type) {
+    constexpr bool kInter = decltype(inter)::value, kVec = decltype(vec)::value, kBf16 = decltype(type)::value;
+    return c.dim == 64 ? kv_append_k<kBf16, kInter, 64, kVec, 2>
+           : team == 2 ? kv_append_k<kBf16, kInter, 128, kVec, 2>
+                       : kv_append_k<kBf16, kInter, 128, kVec, 4>;
+  };
+  auto types = [&](auto inter, auto vec) { return bf16 ? dims(inter, vec, std::true_type{}) : dims(inter, vec, std::false_type{}); };
   auto pick = [&](auto inter) {
-    constexpr bool kInter = decltype(inter)::value;
-    return c.dim == 64 ? (bf16 ? kv_append_k<true, kInter, 64> : kv_append_k<false, kInter, 64>)
-                       : (bf16 ? kv_append_k<true, kInter, 128> : kv_append_k<false, kInter, 128>);
+    return k.vec && v.vec && (!q_heads || (q.vec && q_out.vec)) ? types(inter, std::true_type{}) : types(inter, std::false_type{});
   };
   auto kern = rot.interleaved ? pick(std::true_type{}) : pick(std::false_type{});
-  return launch_kernel(kern, dim3((unsigned)grid), dim3(kRopeThreads), 0, st, a);
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(kAppendThreads), 0, st, a);
 }
 
 cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const KvRows &k, const KvRows &v, int *status,
@@ -483,7 +532,7 @@ cudaError_t launch_kv_read(bool bf16, const KvCache &c, const KvSeqs &s, const K
   const dim3 grid((unsigned)((s.tokens + window - 1) / window));
   auto kern = c.dim == 64 ? (bf16 ? kv_read_k<true, 64> : kv_read_k<false, 64>)
                           : (bf16 ? kv_read_k<true, 128> : kv_read_k<false, 128>);
-  return launch_kernel(kern, grid, dim3(256), 0, st, c, s, k, v, window, status);
+  return launch_kernel(kern, grid, dim3(kReadThreads), 0, st, c, s, k, v, window, status);
 }
 
 }  // namespace ivb
