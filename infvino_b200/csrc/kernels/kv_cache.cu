@@ -5,8 +5,8 @@
 // written once, so memory bounds long calls and the chain of dependent loads
 // (sequence, page, position, angles) short ones.  Sixteen elements (eight
 // pairs) of a row are a thread's share; a warp reads whole 128-byte lines of
-// the two halves of a head.  Rows that cannot be read 16 bytes at a time have
-// kernels of their own: the slow path beside the fast one cost the latter 9 %.
+// the two halves of a head.  Whether rows can be read 16 bytes at a time is
+// settled for a whole launch: a branch at each load cost 9 %.
 #include <algorithm>
 #include <type_traits>
 
