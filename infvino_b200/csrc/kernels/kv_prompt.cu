@@ -645,12 +645,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             vmax = fmaxf(vmax, __ldcg(&sl.vref));
           }
 #pragma unroll 1
-          for (int h = 0; h < DIM / 32; ++h) {
-            float x[32];
+          for (int h = 0; h < DIM / 64; ++h) {
+            float x[64];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = 0.f;
+            for (int k = 0; k < 64; ++k) x[k] = 0.f;
             sum = 0.f;
-#pragma unroll 2
+#pragma unroll 1
             for (int z = first_cta; z <= last_cta; ++z) {
               const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
               const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]), zv = __ldcg(&sl.vref);
@@ -658,18 +658,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float w = zm == -INFINITY && zl == 0.f ? 0.f : fast_exp2(zm - top), wv = vmax > 0.f ? w * __fdividef(zv, vmax) : 0.f;
               sum += zl * w;
 #pragma unroll
-              for (int k = 0; k < 32; k += 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[((32 * h + k) / 4 * 128 + row) * 4]));
+              for (int k = 0; k < 64; k += 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[((64 * h + k) / 4 * 128 + row) * 4]));
                 x[k] += v.x * wv, x[k + 1] += v.y * wv, x[k + 2] += v.z * wv, x[k + 3] += v.w * wv;
               }
             }
             const float y = sum != 0.f ? vmax / sum : 0.f;
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
+            for (int k = 0; k < 64; k += 8) {
               float f[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y;
-              store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
+              store8(out + 64 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
         }
