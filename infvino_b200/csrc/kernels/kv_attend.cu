@@ -32,7 +32,8 @@
 // (a copy reaches 6.5); 48 of up to 16384: 165 us, 6.1 TB/s.  Sliding windows of
 // 1024 over 128 sequences (64 wide): 24 us (floor 10), the start of the shares
 // and their joins; six drafted tokens for 24 sequences, 30 rows: 50 us (floor
-// 14), instructions, since each of two row tiles converts and masks on its own.
+// 14), the latency of conversion, products and softmax in turn, at twelve warps
+// an SM and for two row tiles.
 #include <algorithm>
 
 #include "kv_attend.cuh"
