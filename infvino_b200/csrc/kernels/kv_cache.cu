@@ -368,7 +368,7 @@ __device__ __forceinline__ void find_places(const KvCache &c, const KvSeqs &s, l
 // team's alone, so nothing is atomic and the result does not depend on any
 // order.  The other CTAs turn queries.
 //
-// Latency bounds it: two joins and a block's loads for each head in turn.  9412
+// Latency bounds it: two joins and a block's loads for each head in turn.  9375
 // tokens, 8 heads of 128 beside 32 of queries: 44 us, 4.8 TB/s (floor 32); 64
 // conversations, a token each: 4.3 us.
 template <bool BF16, bool INTER, int DIM, bool VEC, int TEAM>
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kAppendThreads, append_ctas(DIM, TEAM)) kv_app
 // A CTA takes `window` packed tokens, all heads.  A thread keeps its place in
 // the rows (keys or values, head, eight elements: 16 bytes out, so that a warp
 // writes whole lines) and goes over the tokens, kReadAhead of them on their way
-// at once.  9412 tokens, 8 heads of 128: 10.2 us, 5.7 TB/s (floor 8.9); sixteen
+// at once.  9375 tokens, 8 heads of 128: 10.2 us, 5.7 TB/s (floor 8.9); sixteen
 // elements a thread, in two stores, 17.4.
 constexpr int kReadAhead = 4, kReadThreads = 256;
 template <bool BF16, int DIM>
@@ -499,7 +499,7 @@ cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const
   AppendArgs a{c, s, k, v, q, q_out, rot, q_heads, 1, 1, 0, 0, 0, status};
   a.window = window_of(s.tokens);
   // Two warps a block where most blocks get a token or two (64 conversations, 8
-  // heads: 4.3 us; four warps 5.0), one row a lane where they are filled (9412
+  // heads: 4.3 us; four warps 5.0), one row a lane where they are filled (9375
   // tokens: 47 us; 53).
   const int team = a.window == 1 ? 2 : c.dim / 32, teams = kAppendThreads / 32 / team;
   // A CTA loops over the heads where there are blocks enough for two CTAs an
