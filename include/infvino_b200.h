@@ -241,7 +241,10 @@ void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
  *
  * Calls may be captured into a CUDA graph once the stream has had one call of
  * ivc_kv_attend or ivc_kv_reserve (each stream has its own workspace, so calls
- * on several streams may run at the same time). */
+ * on several streams may run at the same time; cudaStreamPerThread is another
+ * stream in every thread).  A graph uses the workspace of the stream that it
+ * was captured on: its replays must not overlap one another, other graphs'
+ * from that stream, or eager calls on it. */
 typedef struct ivc_kv ivc_kv;
 
 typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1 } ivc_dtype;

@@ -6,6 +6,8 @@
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <thread>
+#include <utility>
 
 #include "../../include/infvino_b200.h"
 #include "kernels/common.cuh"
@@ -16,7 +18,8 @@ struct ivc_kv {
   std::mutex mu;
   std::string err;
   int *status = nullptr;
-  std::map<cudaStream_t, void *> workspace;
+  std::map<unsigned long long, void *> workspace;  // by the stream's id
+  std::map<std::pair<cudaStream_t, std::thread::id>, unsigned long long> named;  // ids by handle value (and thread, for cudaStreamPerThread)
 };
 
 namespace {
@@ -84,18 +87,27 @@ int guarded(ivc_kv *h, const char *call, F &&f) {
 }
 
 // The stream's attention workspace, allocated and zeroed (in the stream's order) at its first use.
+// It goes by the stream's id, which tells streams apart that run at the same
+// time.  The handle's value does not: cudaStreamPerThread is one value for a
+// stream of every thread, and a destroyed stream's value may be given out again
+// while its work is pending.  A stream that is being captured does not tell its
+// id; it is the one that its name stood for at the last call outside a capture.
 void *workspace(ivc_kv *h, cudaStream_t st) {
-  const auto it = h->workspace.find(st);
-  if (it != h->workspace.end()) return it->second;
+  const auto name = std::make_pair(st, st == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id());
+  unsigned long long &id = h->named.emplace(name, ~0ull).first->second;  // (~0: none yet)
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   cuda(cudaStreamIsCapturing(st, &cap), "stream");
-  need(cap == cudaStreamCaptureStatusNone, "a stream's first call cannot be captured: call ivc_kv_reserve before");
+  const bool captured = cap != cudaStreamCaptureStatusNone;
+  if (!captured) cuda(cudaStreamGetId(st, &id), "stream");
+  const auto it = h->workspace.find(id);
+  if (it != h->workspace.end()) return it->second;
+  need(!captured, "a stream's first call cannot be captured: call ivc_kv_reserve before");
   const size_t bytes = ivb::kv_workspace_bytes(h->sms);
   void *p = nullptr;
   cuda(cudaMalloc(&p, bytes), "workspace");
   try {
     cuda(cudaMemsetAsync(p, 0, ivb::kKvCounterBytes, st), "workspace");
-    h->workspace[st] = p;
+    h->workspace[id] = p;
   } catch (...) {
     (void)cudaFree(p);
     throw;

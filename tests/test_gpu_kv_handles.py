@@ -1,0 +1,94 @@
+"""Handles of the language-model operators: streams, threads, workspaces, status."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import infvino_b200 as ivb
+
+pytestmark = pytest.mark.gpu
+PER_THREAD = 2  # cudaStreamPerThread
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Call:
+    """An attention call whose items are cut over CTAs, so that its joins use the workspace."""
+
+    def __init__(self, seed, new, lens, heads=2, group=4, dim=64, page=32):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        need = [-(-n // page) for n in lens]
+        order, table, at = np.random.default_rng(seed).permutation(sum(need)), np.full((len(lens), max(need)), -1, np.int32), 0
+        for b, n in enumerate(need):
+            table[b, :n] = order[at:at + n]
+            at += n
+        codes = [torch.randint(-127, 128, (at, heads, page, dim), generator=g, device="cuda").to(torch.int8) for _ in range(2)]
+        scales = [2.0 ** torch.randint(-9, -4, (at, heads, page // 16), generator=g, device="cuda").float() for _ in range(2)]
+        self.cache, self.table, self.max_new = ivb.KvCache(*codes, *scales), ints(table), max(new)
+        self.q = torch.randn((sum(new), heads * group, dim), generator=g, device="cuda").half()
+        self.out = torch.empty_like(self.q)
+        self.offsets, self.lens = ints([0] + list(np.cumsum(new))), ints(lens)
+
+    def run(self, ops, st, out=None):
+        ops.attend(self.cache, self.q, self.out if out is None else out, self.offsets, self.lens, self.table, max_new=self.max_new, stream=st)
+
+    def expected(self):
+        want = torch.empty_like(self.q)
+        with ivb.KvOps(0) as ops:
+            self.run(ops, stream(), want)
+            ops.synchronize(stream())
+        return want
+
+
+def test_per_thread_streams_have_their_own_workspaces():
+    """cudaStreamPerThread is one handle value, but another stream in every thread."""
+    calls = [Call(1, [1, 1], [9000, 5000]), Call(2, [1, 1, 1], [4000, 7000, 100]), Call(3, [300], [3000]), Call(4, [200, 100], [900, 2000])]
+    wants = [c.expected() for c in calls]
+    torch.cuda.synchronize()
+    wrong = []
+    with ivb.KvOps(0) as ops:
+        def work(c, want):
+            outs = [torch.empty_like(c.q) for _ in range(40)]
+            torch.cuda.synchronize()
+            for o in outs:
+                c.run(ops, PER_THREAD, o)
+            ops.synchronize(PER_THREAD)
+            wrong.append(sum(not torch.equal(o, want) for o in outs))
+
+        threads = [threading.Thread(target=work, args=z) for z in zip(calls, wants)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert wrong == [0] * len(calls)
+
+
+def test_a_capture_without_a_call_before_is_refused():
+    c = Call(5, [1, 1], [500, 300])
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with ivb.KvOps(0) as ops:
+        ops.reserve(other.cuda_stream)
+        torch.cuda.synchronize()
+        graph, refused = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(graph, stream=side):
+            try:
+                c.run(ops, side.cuda_stream)
+            except ivb.NativeError as e:
+                refused.append((e.status, e.message))
+            c.out.zero_()  # (a graph of something)
+        assert len(refused) == 1 and refused[0][0] == 1 and "ivc_kv_reserve" in refused[0][1]
+        ops.reserve(side.cuda_stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            c.run(ops, side.cuda_stream)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.out, c.expected())
