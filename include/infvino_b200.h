@@ -308,6 +308,10 @@ const char *ivc_kv_last_error(const ivc_kv *h);
 int ivc_kv_synchronize(ivc_kv *h, void *stream);
 /* Allocates the stream's attention workspace (else its first ivc_kv_attend does). */
 int ivc_kv_reserve(ivc_kv *h, void *stream);
+/* Waits for the stream and frees its attention workspace (some 40 MB; else the
+ * handle keeps it to its end).  To be called before a stream is destroyed.
+ * Graphs captured on the stream must not be replayed after it. */
+int ivc_kv_release(ivc_kv *h, void *stream);
 
 /* Fills a rotary table: the angle of position p and pair i is p * inv_freq[i]
  * (host memory [pairs]), computed in 64 bits and rounded once. */

@@ -2,6 +2,7 @@
 // argument checks, the per-stream workspaces and the status word.  Exceptions
 // never cross the boundary.
 #include <cstring>
+#include <iterator>
 #include <map>
 #include <mutex>
 #include <stdexcept>
@@ -270,6 +271,27 @@ int ivc_kv_synchronize(ivc_kv *h, void *stream) {
 
 int ivc_kv_reserve(ivc_kv *h, void *stream) {
   return guarded(h, "ivc_kv_reserve", [&] { workspace(h, static_cast<cudaStream_t>(stream)); });
+}
+
+int ivc_kv_release(ivc_kv *h, void *stream) {
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void *p = nullptr;
+  const int r = guarded(h, "ivc_kv_release", [&] {
+    unsigned long long id = 0;
+    cuda(cudaStreamGetId(st, &id), "stream");
+    const auto it = h->workspace.find(id);
+    if (it == h->workspace.end()) return;
+    p = it->second;
+    h->workspace.erase(it);
+    for (auto n = h->named.begin(); n != h->named.end();) n = n->second == id ? h->named.erase(n) : std::next(n);
+  });
+  if (!p) return r;
+  // (not under the handle's lock: other threads' calls need not wait for this stream)
+  Scope scope(h->device);
+  (void)cudaStreamSynchronize(st);
+  (void)cudaFree(p);
+  (void)cudaGetLastError();
+  return r;
 }
 
 int ivc_kv_rope_table(ivc_kv *h, const double *inv_freq, int pairs, int64_t positions, float *table, void *stream) {

@@ -160,6 +160,11 @@ class KvOps:
         """Allocates the stream's attention workspace, as its first `attend` would (needed before a graph capture)."""
         self._check(self._L.ivc_kv_reserve(self._h, stream))
 
+    def release(self, stream: int = 0) -> None:
+        """Waits for the stream and frees its attention workspace (some 40 MB), before the stream is destroyed or
+        when it is not used any more; graphs captured on it must not be replayed afterwards."""
+        self._check(self._L.ivc_kv_release(self._h, stream))
+
     def rope_table(self, inv_freq: Sequence[float], table, stream: int = 0) -> None:
         """Fills `table` [positions, pairs, 2] with the angles position * inv_freq[pair]."""
         ptr = _dense(table, "table", "float32", 3, self.device)

@@ -92,3 +92,31 @@ def test_a_capture_without_a_call_before_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(c.out, c.expected())
+
+
+def test_release_gives_the_workspace_back():
+    c = Call(6, [1, 1, 30], [700, 3000, 400])
+    want = c.expected()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    with ivb.KvOps(0) as ops:
+        for s in streams[:1]:  # (what the first call of all brings with it)
+            c.run(ops, s.cuda_stream)
+            ops.release(s.cuda_stream)
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        for _ in range(2):
+            for s in streams:
+                ops.reserve(s.cuda_stream)
+            held = before - torch.cuda.mem_get_info()[0]
+            assert held > 6 << 20
+            for s in streams:
+                c.out.zero_()
+                torch.cuda.synchronize()
+                c.run(ops, s.cuda_stream)
+                ops.release(s.cuda_stream)  # (waits)
+                assert torch.equal(c.out, want)
+                ops.release(s.cuda_stream)  # nothing is left to free
+            assert torch.cuda.mem_get_info()[0] >= before - held // 6
+        c.run(ops, streams[0].cuda_stream)
+        ops.synchronize(streams[0].cuda_stream)
+        assert torch.equal(c.out, want)
