@@ -313,6 +313,13 @@ int ivc_kv_reserve(ivc_kv *h, void *stream);
  * Graphs captured on the stream must not be replayed after it. */
 int ivc_kv_release(ivc_kv *h, void *stream);
 
+/* Diagnostic: with limit_cycles above 0 every other CTA of ivc_kv_attend's
+ * kernel for many queries first waits so many SM clocks (2 M are about 1 ms)
+ * for what never comes, and gives up as after any wait that runs out: the
+ * call's results are not valid, and ivc_kv_synchronize returns IVC_ERR_KERNEL.
+ * Calls after that (0 again) are as if it had not been. */
+int ivc_debug_kv_probe(ivc_kv *h, long long limit_cycles);
+
 /* Fills a rotary table: the angle of position p and pair i is p * inv_freq[i]
  * (host memory [pairs]), computed in 64 bits and rounded once. */
 int ivc_kv_rope_table(ivc_kv *h, const double *inv_freq, int pairs, int64_t positions, float *table, void *stream);

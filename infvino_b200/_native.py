@@ -74,6 +74,7 @@ SIGNATURES = {
     "ivc_kv_synchronize": (_i32, [_vp, _vp]),
     "ivc_kv_reserve": (_i32, [_vp, _vp]),
     "ivc_kv_release": (_i32, [_vp, _vp]),
+    "ivc_debug_kv_probe": (_i32, [_vp, ctypes.c_longlong]),
     "ivc_kv_rope_table": (_i32, [_vp, _P(_f64), _i32, _i64, _vp, _vp]),
     "ivc_kv_rope": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
     "ivc_kv_append": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),

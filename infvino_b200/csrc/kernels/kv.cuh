@@ -53,6 +53,7 @@ struct KvAttend {
   int window, sinks;
   int *status;
   FastDiv by_group, by_page;
+  long long probe;  // above 0: every other CTA of the prompt kernel first waits so many SM clocks for what never comes
 };
 
 struct KvRopeFreq {

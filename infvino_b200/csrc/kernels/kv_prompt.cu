@@ -97,6 +97,55 @@ struct Segment {
   __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == r.tiles; }
 };
 
+// A CTA's share of the units, segment by segment.
+struct Walk {
+  uint32_t u, end, base;  // next unit, the share's end, first unit of (b, rt)
+  int b, rt, row_tiles;
+  KvSpan s;
+  RowSpan r;
+
+  // The share begins at unit `from`, in row tile `rt0` (first unit `at`) of sequence b0; it may be empty.
+  __device__ __forceinline__ void begin(const KvAttend &a, uint32_t from, uint32_t to, uint32_t at, int b0, int rt0) {
+    u = from, end = to, base = at, b = b0, rt = rt0;
+    if (u >= end) return;
+    s = kv_span(a, b);
+    row_tiles = (s.n * a.group + kRows - 1) / kRows;
+    r = row_span(a, s.n, s.len, rt);
+  }
+
+  // The next segment into g (all but `more`); false where the share ends.
+  __device__ __forceinline__ bool next(const KvAttend &a, uint32_t size, Segment &g) {
+    while (u < end) {
+      if (s.n > 0) {
+        const uint32_t each = (uint32_t)r.tiles + kItemCost, units = each * (uint32_t)a.cache.heads;
+        if (u < base + units) {
+          const uint32_t head = (u - base) / each, item = base + head * each, to = min(end, item + each);
+          g.k0 = max(0, (int)(u - item) - kItemCost);
+          g.k1 = (int)(to - item) - kItemCost;
+          u = to;
+          if (g.k1 <= g.k0) continue;  // (the share ends before the item's first tile)
+          g.b = b, g.rt = rt, g.head = (int)head;
+          g.first_cta = (int)((item + kItemCost) / size);
+          g.last_cta = (int)((item + each - 1) / size);
+          g.s = s;
+          g.r = r;
+          return true;
+        }
+        base += units;
+        if (++rt < row_tiles) {
+          r = row_span(a, s.n, s.len, rt);
+          continue;
+        }
+      }
+      rt = 0;
+      s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+      row_tiles = (s.n * a.group + kRows - 1) / kRows;
+      if (s.n > 0) r = row_span(a, s.n, s.len, 0);
+    }
+    return false;
+  }
+};
+
 template <int DIM>
 struct PromptShared {
   static constexpr int kSlabs = DIM / 64;
@@ -104,15 +153,17 @@ struct PromptShared {
   uint8_t k[2][kSlabs][kKeys * 128];
   uint8_t v[2][kSlabs][kKeys * 128];
   TileMeta meta[kMeta];
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2][2], pready[2][2], odone[2][2], qfull[2], drained;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2][2], pready[2][2], odone[2][2], qfull[2], drained, never;
   uint32_t tmem;
   volatile int abort;
   int last[2];
+  int counted[2][2];  // M tile i's part of the item that the share begins in / ends in
   Segment seg[kSegments];  // written by warp 13, read by the 13 warps that work
   uint64_t segfull[kSegments], segempty[kSegments];
   long long scan[kThreads / 32];
   long long base;
   int seq, rt;
+  uint32_t u_begin, u_end, size;  // the share, and how many units one has
 };
 
 struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4], row maximum and sum
@@ -121,6 +172,13 @@ struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 row
   float vref;
   float pad[31];
 };
+
+// Counts a part of an item that CTAs first .. last share; the last one to come sets the counter back.
+__device__ __forceinline__ bool count_part(unsigned *counter, int first, int last) {
+  const bool done = atomicAdd(counter, 1u) == (unsigned)(last - first);
+  if (done) atomicExch(counter, 0u);
+  return done;
+}
 
 // The lowest n of 16 bits.
 __device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; }
@@ -229,6 +287,19 @@ __device__ __forceinline__ void put_codes(uint32_t lo_at, uint32_t hi_at, uint4 
   st_shared16(hi_at, halves<0x4140>(w[2]), halves<0x4342>(w[2]), halves<0x4140>(w[3]), halves<0x4342>(w[3]));
 }
 
+// Counts the parts of cut items that a CTA has not come to, so that the counters
+// are zero again after a launch in which it gave up.  (Not inline: this is rarely run.)
+template <class Shared>
+__device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned *counters) {
+  Walk walk;
+  walk.begin(a, sh.u_begin, sh.u_end, (uint32_t)sh.base, sh.seq, sh.rt);
+  Segment &g = sh.seg[0];
+  while (walk.next(a, sh.size, g))
+    for (int i = 0; i < 2; ++i)
+      if (!g.whole() && g.s.n * a.group > g.rt * kRows + 128 * i && !sh.counted[i][g.k0 == 0])
+        count_part(&counters[2 * g.first_cta + i], g.first_cta, g.last_cta);
+}
+
 template <bool BF16, int DIM>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters) {
@@ -257,7 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&sh.segempty[i]), 13);
     }
     mbar_init(smem_u32(&sh.drained), 1);
+    mbar_init(smem_u32(&sh.never), 1);
     sh.abort = 0;
+    for (int i = 0; i < 4; ++i) sh.counted[i >> 1][i & 1] = 0;
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -316,6 +389,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t size = sane ? max((uint32_t)kItemCost + 1, ((uint32_t)total + gridDim.x - 1) / gridDim.x) : 1u;
   const bool works = sane && blockIdx.x * size < (uint32_t)total;
   const uint32_t u_begin = works ? blockIdx.x * size : 0u;
+  if (threadIdx.x == 0) {
+    sh.u_begin = u_begin;
+    sh.u_end = works ? min((uint32_t)total, u_begin + size) : 0u;
+    sh.size = size;
+  }
   const long long u = u_begin;
   const long long excl = before + incl - mine;
   if (works && u >= excl && u < excl + mine) {
@@ -626,13 +704,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         wg_sync(1 + i);
         if (row == 0) {
           __threadfence();  // (the four warps' writes, which the barrier has put before this)
-          const unsigned parts = (unsigned)(last_cta - first_cta + 1);
-          const bool last = atomicAdd(&counters[2 * first_cta + i], 1u) == parts - 1;
-          if (last) {
-            atomicExch(&counters[2 * first_cta + i], 0u);
-            __threadfence();
-          }
+          const bool last = count_part(&counters[2 * first_cta + i], first_cta, last_cta);
+          if (last) __threadfence();
           sh.last[i] = last;
+          sh.counted[i][head_part] = 1;
         }
         wg_sync(1 + i);
         if (sh.last[i] && real && ok) {
@@ -800,6 +875,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kTileUnits = kSlabs * 128 * 128 / 16, kSlabUnits = 128 * 128 / 16;
       int tile = 0, seg[2] = {0, 0}, done[2] = {0, 0};
       const Segment *g = nullptr;
+      if (a.probe > 0 && blockIdx.x % 2 == 1)
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&sh.never), 0, &sh.abort, a.status, kStatusTimeoutProbe, a.probe));
       // One lane issues, in one stretch for each part, with every operand
       // worked out before: between two parts the tensor cores have only a few
       // products queued.  (64 keys are 8192 bytes on in a tile.)
@@ -885,52 +962,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait_bounded(smem_u32(&sh.drained), 0, &no_abort, a.status, kStatusTimeoutDrain, 400000000LL);
     } else if (warp == 13 && lane == 0) {
       // ---------------------------------------------------------- segments
-      uint32_t u = u_begin;
-      const uint32_t u_end = works ? min((uint32_t)total, u + size) : 0u;
-      uint32_t base = (uint32_t)sh.base;  // first unit of (b, rt)
-      int b = sh.seq, rt = sh.rt, row_tiles = 0;
-      KvSpan s{};
-      RowSpan r{};
-      if (works) {
-        s = kv_span(a, b);
-        row_tiles = (s.n * a.group + kRows - 1) / kRows;
-        r = row_span(a, s.n, s.len, rt);
-      }
+      Walk walk;
+      const uint32_t size = sh.size;
+      walk.begin(a, sh.u_begin, sh.u_end, (uint32_t)sh.base, sh.seq, sh.rt);
       for (int n = 0;; ++n) {
         Segment &g = sh.seg[n % kSegments];
         if (n >= kSegments && !mbar_wait_bounded(smem_u32(&sh.segempty[n % kSegments]), (n / kSegments - 1) & 1, &sh.abort, a.status,
                                                  kStatusTimeoutEmpty, kLimit))
           break;
-        bool found = false;
-        while (!found && u < u_end) {
-          if (s.n > 0) {
-            const uint32_t each = (uint32_t)r.tiles + kItemCost, units = each * (uint32_t)a.cache.heads;
-            if (u < base + units) {
-              const uint32_t head = (u - base) / each, item = base + head * each, end = min(u_end, item + each);
-              g.k0 = max(0, (int)(u - item) - kItemCost);
-              g.k1 = (int)(end - item) - kItemCost;
-              u = end;
-              found = g.k1 > g.k0;  // (else the share ends before the item's first tile)
-              if (found) {
-                g.b = b, g.rt = rt, g.head = (int)head;
-                g.first_cta = (int)((item + kItemCost) / size);
-                g.last_cta = (int)((item + each - 1) / size);
-                g.s = s;
-                g.r = r;
-              }
-              continue;
-            }
-            base += units;
-            if (++rt < row_tiles) {
-              r = row_span(a, s.n, s.len, rt);
-              continue;
-            }
-          }
-          rt = 0;
-          s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
-          row_tiles = (s.n * a.group + kRows - 1) / kRows;
-          if (s.n > 0) r = row_span(a, s.n, s.len, 0);
-        }
+        const bool found = walk.next(a, size, g);
         g.more = found;
         mbar_arrive(smem_u32(&sh.segfull[n % kSegments]));
         if (!found) break;
@@ -943,6 +983,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  } else if (threadIdx.x == 0 && sh.abort) {
+    count_rest(a, sh, counters);
   }
 }
 

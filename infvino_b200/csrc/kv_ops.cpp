@@ -19,6 +19,7 @@ struct ivc_kv {
   std::mutex mu;
   std::string err;
   int *status = nullptr;
+  long long probe = 0;
   std::map<unsigned long long, void *> workspace;  // by the stream's id
   std::map<std::pair<cudaStream_t, std::thread::id>, unsigned long long> named;  // ids by handle value (and thread, for cudaStreamPerThread)
 };
@@ -294,6 +295,13 @@ int ivc_kv_release(ivc_kv *h, void *stream) {
   return r;
 }
 
+int ivc_debug_kv_probe(ivc_kv *h, long long limit_cycles) {
+  return guarded(h, "ivc_debug_kv_probe", [&] {
+    need(limit_cycles >= 0 && limit_cycles <= ivb::kConvWaitLimitDefault, "the limit is from 0 to that of the other waits");
+    h->probe = limit_cycles;
+  });
+}
+
 int ivc_kv_rope_table(ivc_kv *h, const double *inv_freq, int pairs, int64_t positions, float *table, void *stream) {
   return guarded(h, "ivc_kv_rope_table", [&] {
     need(inv_freq && table, "null pointer");
@@ -381,6 +389,7 @@ int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
     a.window = window;
     a.sinks = sinks;
     a.status = h->status;
+    a.probe = h->probe;
     need((int64_t)max_new * a.group < (1LL << 30), "max_new * q_heads / kv_heads out of range");
     a.by_group = ivb::make_fastdiv((uint32_t)a.group);
     a.by_page = ivb::make_fastdiv((uint32_t)a.cache.page);

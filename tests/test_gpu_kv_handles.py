@@ -120,3 +120,29 @@ def test_release_gives_the_workspace_back():
         c.run(ops, streams[0].cuda_stream)
         ops.synchronize(streams[0].cuda_stream)
         assert torch.equal(c.out, want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_calls_after_a_timed_out_one(dim):
+    """Every other CTA of a prompt call gives up: it is reported, and later calls on the same workspace give the bits they would have given."""
+    many = [Call(7, [300], [3000], dim=dim), Call(8, [40, 500, 1], [900, 2000, 3], dim=dim), Call(9, [700], [700], heads=3, group=1, dim=dim),
+            Call(11, [1000], [1500], heads=8, group=8, dim=dim)]  # (the last: shares that end one cut item and begin another)
+    few = Call(10, [1, 1], [9000, 300], dim=dim)
+    wants = [c.expected() for c in many + [few]]
+    L, st = ivb._native.lib(), stream()
+    with ivb.KvOps(0) as ops:
+        for c in many:
+            assert L.ivc_debug_kv_probe(ops._h, 2_000_000) == 0
+            for _ in range(3):  # (odd: of two parts one is missing each time)
+                c.run(ops, st)
+                with pytest.raises(ivb.NativeError) as e:
+                    ops.synchronize(st)
+                assert e.value.status == 5 and "timed out" in e.value.message
+            assert L.ivc_debug_kv_probe(ops._h, 0) == 0
+            for d, want in zip(many + [few], wants):
+                for _ in range(2):
+                    d.out.fill_(float("nan"))
+                    d.run(ops, st)
+                    ops.synchronize(st)
+                    assert torch.equal(d.out, want)
+        assert L.ivc_debug_kv_probe(ops._h, -1) == 1
