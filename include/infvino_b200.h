@@ -234,10 +234,14 @@ void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
  * All tensors are device memory of the handle's device; nothing is copied and
  * no call waits for the device.  `stream` is a cudaStream_t; NULL is the
  * legacy default stream.  Argument errors that the host can see come back as
- * IVC_ERR_ARGUMENT.  What only the device sees (a page number outside the
- * cache, offsets or lengths that do not fit, a position beyond the rotary
- * table) is skipped by the kernels, which set the handle's status word:
- * ivc_kv_synchronize then returns IVC_ERR_KERNEL and clears it.
+ * IVC_ERR_ARGUMENT.  What only the device sees is skipped by the kernels, which
+ * set the handle's status word: ivc_kv_synchronize then returns IVC_ERR_KERNEL
+ * and clears it.  Skipped is: of a token with a position outside the rotary
+ * table everything (no row, code or scale of it is written); of a token without
+ * a place in the cache (a page number outside it, offsets or lengths that do
+ * not fit) the codes, or the row that would be read; of attention, a sequence
+ * whose offsets or length do not fit, and the keys in a page outside the cache,
+ * as if they were hidden.  The others of the call are as they would be alone.
  *
  * Calls may be captured into a CUDA graph once the stream has had one call of
  * ivc_kv_attend or ivc_kv_reserve (each stream has its own workspace, so calls

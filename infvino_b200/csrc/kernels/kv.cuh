@@ -38,8 +38,7 @@ struct KvRotary {
   const float2 *table;  // [positions][pairs] cos, sin; null: no rotation
   long long positions;
   int pairs, interleaved;
-  const int32_t *pos;   // [axes][tokens]
-  long long pos_stride;
+  const int32_t *pos[kKvMaxAxes];  // a token's positions on each axis (one that no pair turns by: another's again)
   uint32_t one_axis;    // bit g: the eight pairs 8g.. share an axis
   uint8_t axis[kKvMaxPairs];
 };

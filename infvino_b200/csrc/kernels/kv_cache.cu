@@ -16,16 +16,37 @@ namespace ivb {
 
 namespace {
 
-// cos and sin of the eight pairs 8g.. of `token`.
+// A token's positions, on the axes that pairs turn by.  If one is outside the
+// table nothing of the token is written.
+struct Positions {
+  int p[kKvMaxAxes];
+};
+__device__ __forceinline__ Positions load_positions(const KvRotary &r, long long token) {
+  Positions x;
+#pragma unroll
+  for (int axis = 0; axis < kKvMaxAxes; ++axis) x.p[axis] = __ldg(r.pos[axis] + token);
+  return x;
+}
+__device__ __forceinline__ bool in_table(const KvRotary &r, int p) { return p >= 0 && p < r.positions; }
+__device__ __forceinline__ bool in_table(const KvRotary &r, const Positions &x) {
+  bool ok = true;
+#pragma unroll
+  for (int axis = 0; axis < kKvMaxAxes; ++axis) ok = ok & in_table(r, x.p[axis]);
+  return ok;
+}
+__device__ __forceinline__ int on_axis(const Positions &x, int axis) {
+  const int lo = axis & 1 ? x.p[1] : x.p[0], hi = axis & 1 ? x.p[3] : x.p[2];
+  return axis & 2 ? hi : lo;
+}
+
+// cos and sin of the eight pairs 8g.. at positions x (of position 0 for one outside the table).
 struct Turn {
   float c[8], s[8];
 };
-__device__ __forceinline__ bool load_turn(const KvRotary &r, int g, long long token, Turn &t, int *status) {
-  bool ok = true;
+__device__ __forceinline__ void load_turn(const KvRotary &r, int g, const Positions &x, Turn &t) {
   if ((r.one_axis >> g) & 1u) {
-    long long p = r.pos[(long long)r.axis[8 * g] * r.pos_stride + token];
-    if (p < 0 || p >= r.positions) ok = false, p = 0;
-    const float4 *row = reinterpret_cast<const float4 *>(r.table + p * r.pairs + 8 * g);
+    const int p = on_axis(x, r.axis[8 * g]);
+    const float4 *row = reinterpret_cast<const float4 *>(r.table + (in_table(r, p) ? (long long)p : 0) * r.pairs + 8 * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 v = __ldg(row + i);
@@ -34,14 +55,11 @@ __device__ __forceinline__ bool load_turn(const KvRotary &r, int g, long long to
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      long long p = r.pos[(long long)r.axis[8 * g + i] * r.pos_stride + token];
-      if (p < 0 || p >= r.positions) ok = false, p = 0;
-      const float2 v = __ldg(r.table + p * r.pairs + 8 * g + i);
+      const int p = on_axis(x, r.axis[8 * g + i]);
+      const float2 v = __ldg(r.table + (in_table(r, p) ? (long long)p : 0) * r.pairs + 8 * g + i);
       t.c[i] = v.x, t.s[i] = v.y;
     }
   }
-  if (!ok) kv_flag(status, kStatusKvPosition);
-  return ok;
 }
 
 // Where the two vectors of group g of a row begin: the halves of eight pairs
@@ -125,7 +143,12 @@ __device__ __forceinline__ void rope_tile(long long tile, long long tokens, int 
           ua[i] = load8(xr + (h + i * hs) * x.hs + ea, VEC);
           ub[i] = load8(xr + (h + i * hs) * x.hs + eb, VEC);
         }
-      if (h == h0 && turned) ok = load_turn(rot, g, token, t, status);
+      if (h == h0) {
+        const Positions at = load_positions(rot, token);
+        ok = in_table(rot, at);
+        if (turned) load_turn(rot, g, at, t);
+        if (!ok) kv_flag(status, kStatusKvPosition);
+      }
       if (!ok) break;
 #pragma unroll
       for (int i = 0; i < HEADS; ++i)
@@ -231,6 +254,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
   const uint16_t *xt = static_cast<const uint16_t *>(x.p) + t0 * x.ts;
   uint4 ua[kSteps], ub[kSteps];
   float before = 0.f;
+  uint32_t rows = (1u << r1) - (1u << r0);  // bit r: row r is written
   auto load = [&](int h) {
     if (h >= a.c.heads) return;
     if (r0 > 0) before = scales[(long long)h * (a.c.page / kKvBlock)];
@@ -238,7 +262,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
     for (int i = 0; i < kSteps; ++i) {
       const int r = row0 + i * kRows;
       ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
-      if (r >= r0 && r < r1) {
+      if ((rows >> r) & 1u) {
         const uint16_t *row = xt + (r - r0) * x.ts + h * x.hs;
         ua[i] = load8(row + ea, VEC);
         ub[i] = load8(row + eb, VEC);
@@ -256,13 +280,36 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
     team_sync<TEAM>(team);
     return m;
   };
+  // lane l looks at the positions of row l % 16 on axes l / 16 and l / 16 + 2
+  int p01 = 0, p23 = 0;
+  if (a.rot.table && ((rows >> (lane & 15)) & 1u)) {
+    const long long token = t0 + (lane & 15) - r0;
+    p01 = __ldg((lane < 16 ? a.rot.pos[0] : a.rot.pos[1]) + token);
+    p23 = __ldg((lane < 16 ? a.rot.pos[2] : a.rot.pos[3]) + token);
+  }
   load(head);
   Turn t[kSteps];
   bool turned[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int r = row0 + i * kRows;
-    turned[i] = r >= r0 && r < r1 && 8 * g < pairs && load_turn(a.rot, g, t0 + r - r0, t[i], a.status);
+    Positions at;
+#pragma unroll
+    for (int axis = 0; axis < kKvMaxAxes; ++axis) at.p[axis] = __shfl_sync(0xffffffffu, axis < 2 ? p01 : p23, 16 * (axis & 1) + r);
+    turned[i] = ((rows >> r) & 1u) && 8 * g < pairs;
+    if (turned[i]) load_turn(a.rot, g, at, t[i]);
+  }
+  const uint32_t bad = a.rot.table ? __ballot_sync(0xffffffffu, !in_table(a.rot, p01) || !in_table(a.rot, p23)) : 0;
+  if (bad) {
+    if (lane == 0) kv_flag(a.status, kStatusKvPosition);
+    rows &= ~(bad | bad >> 16);
+    if (rows == 0) return;  // (for all warps of the team)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if (!((rows >> (row0 + i * kRows)) & 1u)) {
+        ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
+        turned[i] = false;
+      }
   }
 #pragma unroll 1
   for (; head < a.c.heads; head += step) {
@@ -320,7 +367,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const KvRows &
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int r = row0 + i * kRows;
-      if (r >= r0 && r < r1) {
+      if ((rows >> r) & 1u) {
         *reinterpret_cast<uint2 *>(ch + r * DIM + ea) = make_uint2(quantise4(f[i][0], inv), quantise4(f[i][0] + 4, inv));
         *reinterpret_cast<uint2 *>(ch + r * DIM + eb) = make_uint2(quantise4(f[i][1], inv), quantise4(f[i][1] + 4, inv));
       }

@@ -1,6 +1,7 @@
 // C ABI of the language-model operators (include/infvino_b200.h, ivc_kv_*):
 // argument checks, the per-stream workspaces and the status word.  Exceptions
 // never cross the boundary.
+#include <algorithm>
 #include <cstring>
 #include <iterator>
 #include <map>
@@ -151,12 +152,14 @@ ivb::KvRotary rotation(const ivc_rotary *r, int head_dim, int64_t tokens) {
   k.positions = r->positions;
   k.pairs = r->pairs;
   k.interleaved = r->interleaved != 0;
-  k.pos = r->pos;
-  k.pos_stride = r->axes > 1 ? r->pos_stride : 0;
   for (int i = 0; i < r->pairs; ++i) {
     const int a = r->axis_of ? r->axis_of[i] : 0;
     need(a < r->axes, "axis_of names an axis that the positions lack");
     k.axis[i] = (uint8_t)a;
+  }
+  for (int a = 0; a < ivb::kKvMaxAxes; ++a) {
+    const bool used = std::find(k.axis, k.axis + r->pairs, a) != k.axis + r->pairs;
+    k.pos[a] = r->pos + (used ? a : k.axis[0]) * (r->axes > 1 ? r->pos_stride : 0);
   }
   for (int g = 0; g < r->pairs / 8; ++g) {
     bool one = true;

@@ -1,0 +1,138 @@
+"""The language-model operators where only the device sees that input does not
+fit: what is skipped stays as it was, and the rest of the call is right."""
+import numpy as np
+import pytest
+import torch
+
+import infvino_b200 as ivb
+from test_gpu_kv import BLOCK, TYPES, Model, ints, new_cache, offsets_of, page_table, some_axes, stream
+
+pytestmark = pytest.mark.gpu
+IVC_ERR_KERNEL = 5
+
+
+@pytest.fixture(scope="module")
+def ops():
+    with ivb.KvOps(0) as o:
+        yield o
+
+
+def reported(ops):
+    with pytest.raises(ivb.NativeError) as e:
+        ops.synchronize(stream())
+    assert e.value.status == IVC_ERR_KERNEL
+    ops.synchronize(stream())
+
+
+def spoil(pos, tokens, positions, axis):
+    """Puts the tokens' positions outside the table, on one axis."""
+    for i, t in enumerate(tokens):
+        pos[axis, t] = (positions, -1, 2 ** 31 - 1, -2 ** 31)[i % 4]
+
+
+@pytest.mark.parametrize("tokens,heads,dim,pairs,axes,interleaved", [
+    (40, 5, 128, 64, 3, False), (40, 5, 128, 64, 3, True), (33, 3, 80, 24, 4, False), (17, 300, 64, 8, 1, False), (3000, 12, 128, 32, 2, True)])
+@pytest.mark.parametrize("off_grid", [False, True])
+def test_rope_leaves_whole_rows_out(ops, tokens, heads, dim, pairs, axes, interleaved, off_grid):
+    g = torch.Generator(device="cuda").manual_seed(tokens + dim)
+    table = torch.empty((500, pairs, 2), device="cuda")
+    ops.rope_table([100.0 ** (-i / pairs) for i in range(pairs)], table, stream())
+    x = torch.randn(tokens * heads * dim + 8, generator=g, device="cuda").half()[int(off_grid):][:tokens * heads * dim].view(tokens, heads, dim)
+    pos = torch.randint(0, 500, (axes, tokens), generator=g, device="cuda", dtype=torch.int32)
+    rotary = ivb.Rotary(table, some_axes(pairs, axes), interleaved)
+    want = torch.empty_like(x)
+    ops.rope(x, want, rotary, pos, stream())
+    ops.synchronize(stream())
+    for axis in range(axes):
+        bad = sorted({0, 3, 4, tokens // 2 + axis, tokens - 1})
+        p = pos.clone()
+        spoil(p, bad, 500, axis)
+        out = torch.full_like(x, 7.0)
+        ops.rope(x, out, rotary, p, stream())
+        reported(ops)
+        w = want.clone()
+        w[bad] = 7.0
+        assert torch.equal(out, w)
+        y = x.clone()
+        ops.rope(y, y, rotary, p, stream())  # in place: the row stays
+        reported(ops)
+        w[bad] = x[bad]
+        assert torch.equal(y, w)
+    unused = torch.cat([pos, torch.full((4 - axes, tokens), -9, dtype=torch.int32, device="cuda")])  # no pair turns by these
+    out = torch.empty_like(x)
+    ops.rope(x, out, rotary, unused, stream())
+    ops.synchronize(stream())
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,dim,page,axes,first,new,bad", [
+    (2, 64, 16, 1, [5, 0], [30, 1], [0, 7, 29]),           # of a begun block, of whole ones
+    (3, 128, 48, 3, [10, 33], [6, 20], [0, 1, 2, 3, 4, 5, 10]),  # all that a begun block gets
+    (1, 128, 64, 2, [0, 16], [64, 5], list(range(16, 32)) + [64]),  # a whole new block
+    (2, 64, 32, 4, [3] * 9, [1] * 9, [2, 5]),               # single tokens
+    (2, 128, 64, 3, [40, 0], [2000, 900], [0, 100, 1999, 2000, 2899])])
+def test_append_leaves_whole_tokens_out(ops, dtype, heads, dim, page, axes, first, new, bad):
+    batch, dt, positions = len(new), TYPES[dtype], 300
+    lens = [f + n for f, n in zip(first, new)]
+    table, pages = page_table(lens, page, seed=dim)
+    cache_t = new_cache(pages, heads, page, dim)
+    cache, dev_table = ivb.KvCache(*cache_t), ints(table)
+    rot_table = torch.empty((positions, dim // 2, 2), device="cuda")
+    ops.rope_table([100.0 ** (-i / (dim // 2)) for i in range(dim // 2)], rot_table, stream())
+    axis = some_axes(dim // 2, axes)
+    rotary = ivb.Rotary(rot_table, axis)
+    models = [Model(batch, heads, dim, max(lens) + BLOCK) for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(page)
+    for start, count, holes, grow in (([0] * batch, first, [], 1.0), (first, new, bad, 3.0)):
+        t = sum(count)
+        if t == 0:
+            continue
+        k, v, q = (torch.randn((t, h, dim), generator=g, device="cuda").mul_(grow).to(dt) for h in (heads, heads, 2 * heads))
+        for i, h in enumerate(holes):  # what is left out would decide the scale
+            k[h] *= 50.0
+            v[h] *= 50.0
+        pos = torch.randint(0, positions, (axes, t), generator=g, device="cuda", dtype=torch.int32)
+        turned = torch.empty_like(q)
+        ops.rope(q, turned, rotary, pos, stream())
+        x = k.float()
+        cs = torch.stack([rot_table[pos[a].long(), i] for i, a in enumerate(axis)], 1)[:, None]
+        a, b_ = x[..., :dim // 2], x[..., dim // 2:]
+        kr = torch.cat([a * cs[..., 0] - b_ * cs[..., 1], b_ * cs[..., 0] + a * cs[..., 1]], -1).cpu().numpy()
+        spoil(pos, holes, positions, axes - 1)
+        q_out, before = torch.full_like(q, 7.0), [c.clone() for c in cache_t]
+        ops.append(cache, k, v, offsets_of(count), ints(start), dev_table, rotary=rotary, pos=pos, q=q, q_out=q_out, stream=stream())
+        if holes:
+            reported(ops)
+            turned[holes] = 7.0
+        else:
+            ops.synchronize(stream())
+        assert torch.equal(q_out, turned)
+        kr[holes], vr = np.nan, v.float().cpu().numpy()  # (the model takes NaN out of the scale)
+        vr[holes] = np.nan
+        at = 0
+        for b, n in enumerate(count):
+            for model, x in zip(models, (kr, vr)):
+                if n:
+                    model.append(b, start[b], x[at:at + n])
+            at += n
+        at = 0
+        for b, n in enumerate(count):
+            out = np.zeros(start[b] + n, dtype=bool)
+            out[[start[b] + h - at for h in holes if at <= h < at + n]] = True
+            at += n
+            where = np.arange(start[b] + n)
+            page_of, slot = table[b, where // page], where % page
+            blocks = where // BLOCK
+            # a block that gets nothing keeps its scale, whatever that is
+            got = np.array([(~out[(blocks == k) & (where >= start[b])]).any() for k in blocks], dtype=bool)
+            touched = np.array([((blocks == k) & (where >= start[b])).any() for k in blocks], dtype=bool)
+            for model, i in zip(models, (0, 1)):
+                c, s = cache_t[i].cpu().numpy()[page_of, :, slot], cache_t[i + 2].cpu().numpy()[page_of, :, slot // BLOCK]
+                c0, s0 = before[i].cpu().numpy()[page_of, :, slot], before[i + 2].cpu().numpy()[page_of, :, slot // BLOCK]
+                want_s = 2.0 ** model.exp[b, blocks].astype(np.float64)
+                same = touched & ~got
+                assert np.array_equal(s[same], s0[same], equal_nan=True)
+                assert np.array_equal(s[~same], want_s[~same])
+                assert np.array_equal(c[~out], model.codes[b, where[~out]])
+                assert np.array_equal(c[out], c0[out])
