@@ -108,18 +108,16 @@ __device__ __forceinline__ uint32_t tile_swizzle(uint32_t o) {
 constexpr int step_ctas(int dim, int nt) { return nt == 1 && dim == 64 ? 4 : 3; }
 
 template <int DIM, int NT>
-struct StepSlot {  // partial sums of a cut item: accumulators lane by lane, then per row maximum and sum
+struct StepSlot {  // a part of a cut item: accumulators lane by lane in units of 2^t, then each row's m, sum and t
   float acc[NT * DIM / 4 * 32];
-  float m[8 * NT], l[8 * NT];
-  float vref;
-  float pad[31];
+  float m[8 * NT], l[8 * NT], t[8 * NT];
 };
 
 template <int DIM, int NT>
 struct StepShared {
   alignas(128) uint8_t ring[kStepWarps][kStepStages][2][kKvBlock * DIM];
   float2 scales[kStepWarps][kStepStages];
-  float m[kStepWarps][8 * NT], l[kStepWarps][8 * NT], vref[kStepWarps];
+  float m[kStepWarps][8 * NT], l[kStepWarps][8 * NT], lref[kStepWarps];
   long long scan[kStepWarps];
   long long base;
   int seq;
@@ -340,7 +338,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.f;
     }
-    float vref = 0.f, vinv = 0.f;  // acc is in units of vref, the largest value scale so far
+    float vref = 0.f, vinv = 0.f, lref = -INFINITY;  // acc is in units of vref, the largest value scale so far; log2 of it
 
     for (int it = 0; it < count; it += kZ) {
       cp_async_wait<kStepStages - kZ>();
@@ -393,50 +391,59 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
               if (!kv_sees(a, pos[t][e & 1], key0 + g + 8 * (e >> 1))) sc[z][t][e] = -INFINITY;
         }
       }
-      // the rows' maxima, where a score is well above them, and the value scale
+      // the value scale, and the rows' maxima of s + log2 (vs / vref), where one is well above
+      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[kZ - 1]));
+      const float lnew = vnew > vref ? log2_of(vnew) : lref;
+      float lv[kZ];
+#pragma unroll
+      for (int z = 0; z < kZ; ++z) lv[z] = fmaxf(log2_of(vs[z]) - lnew, kFarBelow);  // (a block without keys: any)
       float mx[NT][2];
       bool above = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          mx[t][c] = fmaxf(sc[0][t][c], sc[0][t][c + 2]);
-          if (kZ == 2) mx[t][c] = fmaxf(mx[t][c], fmaxf(sc[kZ - 1][t][c], sc[kZ - 1][t][c + 2]));
+          mx[t][c] = fmaxf(sc[0][t][c], sc[0][t][c + 2]) + lv[0];
+          if (kZ == 2) mx[t][c] = fmaxf(mx[t][c], fmaxf(sc[kZ - 1][t][c], sc[kZ - 1][t][c + 2]) + lv[kZ - 1]);
           above = above || mx[t][c] > m[t][c] + kStepSlack;
         }
-      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[kZ - 1]));
       if (__any_sync(0xffffffffu, above) || vnew > vref) {
-        const float vr = vref > 0.f ? __fdividef(vref, vnew) : 0.f;
+        const float lvr = vnew > vref ? lref - lnew : 0.f;  // in units of the new vref the largest so far is lower by this
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(m[t][c], mx[t][c]);
+            float x = fmaxf(m[t][c] + lvr, mx[t][c]), room = kv_room(l[t][c]);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            const float f = x > m[t][c] ? fast_exp2(m[t][c] - x) : 1.f;
-            l[t][c] *= f;
+            for (int o = 4; o < 32; o <<= 1) {
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+              room = fminf(room, __shfl_xor_sync(0xffffffffu, room, o));
+            }
+            x = fmaxf(x, m[t][c] - room);
+            const float d = x != m[t][c] ? m[t][c] - x : 0.f, f = fast_exp2(d + lvr);
+            l[t][c] = kv_scaled(l[t][c], d);
             m[t][c] = x;
 #pragma unroll
             for (int j = 0; j < kTiles; ++j) {
-              acc[t][j][c] *= f * vr;
-              acc[t][j][c + 2] *= f * vr;
+              acc[t][j][c] *= f;
+              acc[t][j][c + 2] *= f;
             }
           }
         vref = vnew;
+        lref = lnew;
         vinv = vref > 0.f ? 1.f / vref : 0.f;
       }
 #pragma unroll
       for (int z = 0; z < kZ; ++z) {
         if (vs[z] < 0.f) continue;
-        const float vf = vs[z] * vinv;
+        const float vf = vs[z] * vinv * 0x1p64f;  // 2^(lv + kSumBits)
         uint32_t p[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float w[4];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float shift = m[t][c] == -INFINITY ? 0.f : m[t][c] - kStepBits;
+            const float shift = m[t][c] == -INFINITY ? 0.f : m[t][c] - (kStepBits - kSumBits);
             w[c] = fast_exp2(sc[z][t][c] - shift);
             w[c + 2] = fast_exp2(sc[z][t][c + 2] - shift);
             l[t][c] += w[c] + w[c + 2];
@@ -507,11 +514,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
           sh.l[warp][8 * t + 2 * t4 + c] = l[t][c];
         }
       }
-    if (lane == 0) sh.vref[warp] = vref;
+    if (lane == 0) sh.lref[warp] = lref;
     __syncthreads();
-    float all_v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) all_v = fmaxf(all_v, sh.vref[w]);
     // accumulators lane by lane, [row tile][row of two][head element of the
     // piece]: eight neighbours of a lane are eight neighbouring outputs
     float *part = reinterpret_cast<float *>(&sh.ring[warp][kAhead][0][0]);
@@ -521,10 +525,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       for (int c = 0; c < 2; ++c) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][8 * t + 2 * t4 + c]);
-        const float f = m[t][c] == -INFINITY
-                            ? 0.f
-                            : fast_exp2(m[t][c] - top) * (all_v > 0.f ? __fdividef(vref, all_v) : 0.f);
+        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][8 * t + 2 * t4 + c] + sh.lref[w]);
+        const float f = kv_share(m[t][c] + lref, top);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
@@ -541,13 +543,13 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       }
       if (threadIdx.x < kRows) {
         const int r = threadIdx.x;
-        float top = -INFINITY, x = 0.f;
-        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]);
+        float top = -INFINITY, x = 0.f, t = -INFINITY;
+        for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]), t = fmaxf(t, sh.m[w][r] + sh.lref[w]);
         for (int w = 0; w < kStepWarps; ++w)
-          if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) x += sh.l[w][r] * fast_exp2(sh.m[w][r] - top);
+          if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) x += kv_scaled(sh.l[w][r], sh.m[w][r] - top);
         __stcg(&slots[slot].m[r], top);
         __stcg(&slots[slot].l[r], x);
-        if (r == 0) __stcg(&slots[slot].vref, all_v);
+        __stcg(&slots[slot].t[r], t);
       }
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -568,12 +570,11 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         const int ln = e & 31, i0 = (e >> 5) * 8;  // accumulators i0 .. i0 + 7 of lane ln
         const int rc = i0 / kPiece, d0 = i0 % kPiece;
         const int r = 8 * (rc >> 1) + 2 * (ln & 3) + (rc & 1);
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f, top = -INFINITY, vr = 0.f;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f, top = -INFINITY, t = -INFINITY;
         if (whole) {
-          for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]);
-          vr = all_v;
+          for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh.m[w][r]), t = fmaxf(t, sh.m[w][r] + sh.lref[w]);
           for (int w = 0; w < kStepWarps; ++w) {
-            if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) sum += sh.l[w][r] * fast_exp2(sh.m[w][r] - top);
+            if (sh.m[w][r] != -INFINITY || sh.l[w][r] != 0.f) sum += kv_scaled(sh.l[w][r], sh.m[w][r] - top);
             const float *src = reinterpret_cast<const float *>(&sh.ring[w][kAhead][0][0]) + i0 * 32 + ln;
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] += src[32 * k];
@@ -584,24 +585,23 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
           for (int z = first_cta; z <= last_cta; ++z) {
             const StepSlot<DIM, NT> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
             top = fmaxf(top, __ldcg(&sl.m[r]));
-            vr = fmaxf(vr, __ldcg(&sl.vref));
+            t = fmaxf(t, __ldcg(&sl.t[r]));
           }
 #pragma unroll 4
           for (int z = first_cta; z <= last_cta; ++z) {
             const StepSlot<DIM, NT> &sl = slots[2 * z + (z == first_cta ? 1 : 0)];
-            const float zm = __ldcg(&sl.m[r]), zl = __ldcg(&sl.l[r]), zv = __ldcg(&sl.vref);
+            const float zm = __ldcg(&sl.m[r]), zl = __ldcg(&sl.l[r]), wv = kv_share(__ldcg(&sl.t[r]), t);
             // (a part of the keys that was hidden from the row: 0)
-            const float w = zm == -INFINITY && zl == 0.f ? 0.f : fast_exp2(zm - top), wv = vr > 0.f ? w * __fdividef(zv, vr) : 0.f;
-            sum += zl * w;
+            if (zm != -INFINITY || zl != 0.f) sum += kv_scaled(zl, zm - top);
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] += __ldcg(&sl.acc[(i0 + k) * 32 + ln]) * wv;
           }
         }
         const int row = rt_now * kRows + r, i = fast_div(row, a.by_group);
         if (i < n) {
-          const float y = sum != 0.f ? vr / sum : 0.f;  // (a NaN sum stays NaN)
+          const float2 y = kv_norm(fast_exp2(t - top), sum);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] *= y;
+          for (int k = 0; k < 8; ++k) x[k] = x[k] * y.x * y.y;
           uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(first + i) * a.out.ts +
                         (long long)(head_now * a.group + row - i * a.group) * a.out.hs;
           store8(o + (ln >> 2) * kPiece + d0, pack8<BF16>(x), a.out.vec);

@@ -7,8 +7,10 @@ namespace ivb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Weights are 2^(s - m + kWeightBits), at most 2^14: as halves they keep their
-// 11 bits down to 2^-28 of the row's largest, and sums of them fit as well.
+// Weights times value scales are halves of at most 2^kWeightBits.  The largest of
+// a row is at least 2^(kWeightBits - slack), where slack (4 or 6, in the kernels)
+// is how far a row's reference m may lag behind, so halves keep their 11 bits
+// down to 2^-(14 + kWeightBits - slack) of it: 2^-24 or 2^-22.
 constexpr float kWeightBits = 14.f;
 
 // 2^x (relative error about 2^-22; 0 for -inf).
@@ -17,6 +19,38 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+__device__ __forceinline__ float log2_of(float x) {  // (-inf for 0; exact for powers of two)
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A row's reference m is the largest s + lv of the keys that it sees, where lv is
+// log2 (vs / vref): the largest weight times value scale, and not the largest
+// weight, sets what the halves can hold.  vref, the largest value scale so far, is
+// common to the rows of an item; where it grows m is lowered with it, so that
+// keys that are hidden from a row do not count for it.  s - m can be as large as
+// -lv then, so sums of 2^(s - m) are kept in units of 2^-kSumBits.
+constexpr float kSumBits = 64.f;
+constexpr float kFarBelow = -150.f;  // lv is taken as at least this
+// l 2^d, d far below the range of f32's exponents or not.
+__device__ __forceinline__ float kv_scaled(float l, float d) {
+  const float half = fast_exp2(0.5f * d);
+  return l * half * half;
+}
+// How far a row's m may be lowered when its sum is l: until the sum is 2^96.
+__device__ __forceinline__ float kv_room(float l) {
+  return fmaxf(0.f, (float)(96 + 127 - (int)(__float_as_uint(l) >> 23)));
+}
+// vref / (l 2^kSumBits) as a product that stays inside f32's range; 0 for no sum (a NaN sum stays NaN).
+__device__ __forceinline__ float2 kv_norm(float vref, float l) {
+  if (l == 0.f) return make_float2(0.f, 0.f);
+  return l < 1.f ? make_float2(vref / (l * 0x1p64f), 1.f) : make_float2(vref / l, 0x1p-64f);
+}
+
+// What a part's accumulators count beside the largest: t = m + log2 vref of either.
+__device__ __forceinline__ float kv_share(float t, float top) { return t == -INFINITY ? 0.f : fast_exp2(t - top); }
 
 // One sequence of a call: its packed tokens, cache length, and the key blocks
 // (of kKvBlock keys) that its queries see: `sink_blocks` from 0, then the rest

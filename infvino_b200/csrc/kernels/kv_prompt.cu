@@ -53,18 +53,18 @@ constexpr int kSegments = 4;      // ring of segments
 constexpr int kMeta = 4;          // rings: scales of a tile live until both softmaxes are done
 constexpr int kSub = 64;          // keys of a score tile: two in turn for each M tile and key tile
 constexpr float kSlack = 6.f, kBits = kWeightBits - kSlack;
-constexpr float kFarBelow = -40.f;  // value scales are taken as at least 2^-40 of the largest so far
+constexpr float kFar = -80.f;     // blocks with a lower lv (below) are looked at row by row
 constexpr int kNoKey = 0x3fffffff;
 constexpr int kItemCost = 2;      // what an item costs besides its tiles, in tiles: queries in, outputs out
 constexpr int kMaxSeqs = 8192;    // sequences of a call that the start-up scan has room for
 
 struct alignas(16) TileMeta {
   float kc[kTileBlocks];    // ks * |scale| * log2 e
-  float lvf[kTileBlocks];   // log2 (vs / vref)
-  float ivf[kTileBlocks];   // vref / vs
+  float lvf[kTileBlocks];   // lv = log2 (vs / vref)
+  float ivf[kTileBlocks];   // 2^(-lv - kSumBits)
   int key0[kTileBlocks];    // first key, kNoKey behind the end
-  float vr, vref;           // vref before / vref of this tile; vref: the largest value scale so far
-  float pad[2];
+  float vref, lvr;          // vref: the largest value scale so far; log2 (vref before / vref)
+  uint32_t rare[2];         // of half h: bit 4: vref grew; bit j: the lv of its block j is below kFar
 };
 
 // The key blocks that an item's rows see, for rows 256 rt and on of a sequence.
@@ -589,27 +589,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 kc4 = *reinterpret_cast<const float4 *>(&me.kc[b0]);
           const float4 lv4 = *reinterpret_cast<const float4 *>(&me.lvf[b0]), iv4 = *reinterpret_cast<const float4 *>(&me.ivf[b0]);
           float c[4] = {kc4.x, kc4.y, kc4.z, kc4.w}, mx = -INFINITY;
-          const float lvf[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, ivf[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
+          float lvf[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, ivf[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            c[b] = fmaxf(BF16 ? c[b] * rf : c[b], 0x1p-120f);  // (never 0: hidden keys stay at -inf)
+            if (BF16) c[b] = fmaxf(c[b] * rf, 0x1p-120f);  // (never 0: hidden keys stay at -inf)
             float x = s[kKvBlock * b];
 #pragma unroll
             for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
-            mx = fmaxf(mx, x * c[b]);
+            mx = fmaxf(mx, fmaf(x, c[b], lvf[b]));
           }
-          const float vr = h == 0 ? me.vr : 1.f;
-          vref = me.vref;
-          if (__any_sync(0xffffffffu, mx > m + kSlack) || vr != 1.f) {
-            const float top = fmaxf(m, mx);
-            const float f = top > m ? fast_exp2(m - top) : 1.f;
+          const uint32_t rare = me.rare[h];
+          if (__any_sync(0xffffffffu, mx > m + kSlack) || rare != 0) {
+            float lvr = 0.f;
+            if (rare & 16u) {  // in units of the new vref the largest so far is lower by lvr
+              lvr = me.lvr;
+              vref = me.vref;
+            }
+            const float top = fmaxf(fmaxf(m + lvr, mx), m - kv_room(l));
+            const float d = top != m ? m - top : 0.f;
+            l = kv_scaled(l, d);
             m = top;
-            l *= f;
             if (t > 0 || h > 0) {
               // the products before: the other half of the keys, of this tile or the last
               if (!wait(smem_u32(&sh.odone[i][h ^ 1]), (h == 0 ? done - 1 : done) & 1, kStatusTimeoutDrain)) continue;
               tc_fence_after();
-              const float fo = f * vr;
+              const float fo = fast_exp2(d + lvr);
 #pragma unroll 1
               for (int d = 0; d < DIM / 32; ++d) {
                 float o[32];
@@ -629,7 +633,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          // weights 2^(s c - m + kBits) vs / vref, sums without the last factor
+          if (rare & 15u) {
+            // Weights may be too small for numbers here and yet count in the
+            // sum, which has no 2^lv: lv is raised where the values count for
+            // nothing all the same (2^-70 of the row's largest).
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              float x = s[kKvBlock * b];
+#pragma unroll
+              for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
+              lvf[b] = fmaxf(lvf[b], fminf(kFar, m - x * c[b] - 70.f));
+              ivf[b] = fast_exp2(-lvf[b] - kSumBits);
+            }
+          }
+          // weights 2^(s c + lv - m + kBits), sums without 2^lv and in units of 2^-kSumBits
           const float shift = m == -INFINITY ? 0.f : kBits - m;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -664,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       if (!ok) {  // (the slot keeps whatever it holds: the status word says that the result is not valid)
       } else if (whole) {
-        const float y = l != 0.f ? vref / l : 0.f;  // (a NaN sum stays NaN)
+        const float2 y = kv_norm(vref, l);
 #pragma unroll 1
         for (int h = 0; h < DIM / 32; ++h) {
           float o[32];
@@ -677,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 32; k += 8) {
               float f[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = l != 0.f ? o[k + j] * y : 0.f;
+              for (int j = 0; j < 8; ++j) f[j] = l != 0.f ? o[k + j] * y.x * y.y : 0.f;
               store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
@@ -711,13 +728,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         wg_sync(1 + i);
         if (sh.last[i] && real && ok) {
-          float top = -INFINITY, vmax = 0.f, sum = 0.f;
+          float top = -INFINITY, t = -INFINITY, sum = 0.f;
           // (several parts' loads at once: a short call over a long cache has many)
 #pragma unroll 4
           for (int z = first_cta; z <= last_cta; ++z) {
             const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
-            top = fmaxf(top, __ldcg(&sl.m[row]));
-            vmax = fmaxf(vmax, __ldcg(&sl.vref));
+            const float zm = __ldcg(&sl.m[row]);
+            top = fmaxf(top, zm);
+            t = fmaxf(t, zm + log2_of(__ldcg(&sl.vref)));
           }
 #pragma unroll 1
           for (int h = 0; h < DIM / 64; ++h) {
@@ -728,22 +746,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int z = first_cta; z <= last_cta; ++z) {
               const PromptSlot &sl = slots[2 * (2 * z + (z == first_cta ? 1 : 0)) + i];
-              const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]), zv = __ldcg(&sl.vref);
+              const float zm = __ldcg(&sl.m[row]), zl = __ldcg(&sl.l[row]), wv = kv_share(zm + log2_of(__ldcg(&sl.vref)), t);
               // (a part of the keys that was hidden from the row: 0)
-              const float w = zm == -INFINITY && zl == 0.f ? 0.f : fast_exp2(zm - top), wv = vmax > 0.f ? w * __fdividef(zv, vmax) : 0.f;
-              sum += zl * w;
+              if (zm != -INFINITY || zl != 0.f) sum += kv_scaled(zl, zm - top);
 #pragma unroll
               for (int k = 0; k < 64; k += 4) {
                 const float4 v = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[((64 * h + k) / 4 * 128 + row) * 4]));
                 x[k] += v.x * wv, x[k + 1] += v.y * wv, x[k + 2] += v.z * wv, x[k + 3] += v.w * wv;
               }
             }
-            const float y = sum != 0.f ? vmax / sum : 0.f;
+            const float2 y = kv_norm(fast_exp2(t - top), sum);
 #pragma unroll
             for (int k = 0; k < 64; k += 8) {
               float f[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y;
+              for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y.x * y.y;
               store8(out + 64 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
@@ -828,16 +845,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int o = 4; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
           vmax = fmaxf(vref, __shfl_sync(0xffffffffu, vmax, 0));
           TileMeta &me = sh.meta[tile % kMeta];
+          const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(log2_of(now.vs) - log2_of(vmax), kFarBelow) : kFarBelow;
           if (lane < kTileBlocks) {
-            const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(__log2f(now.vs) - __log2f(vmax), kFarBelow) : kFarBelow;
-            me.kc[lane] = now.ks * kc_all;
+            me.kc[lane] = fmaxf(now.ks * kc_all, 0x1p-120f);
             me.lvf[lane] = lv;
-            me.ivf[lane] = fast_exp2(-lv);
+            me.ivf[lane] = fast_exp2(-fmaxf(lv, kFar) - kSumBits);
             me.key0[lane] = now.key0;
           }
+          const uint32_t far = __ballot_sync(0xffffffffu, lane < kTileBlocks && now.key0 != kNoKey && lv < kFar);
           if (lane == 0) {
-            me.vr = vmax > vref ? vref / vmax : 1.f;
+            me.lvr = vmax > vref ? log2_of(vref) - log2_of(vmax) : 0.f;
             me.vref = vmax;
+            me.rare[0] = (far & 15u) | (vmax > vref ? 16u : 0u);
+            me.rare[1] = far >> 4;
           }
           vref = vmax;
         }
