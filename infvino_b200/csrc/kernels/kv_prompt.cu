@@ -845,6 +845,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int o = 4; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
           vmax = fmaxf(vref, __shfl_sync(0xffffffffu, vmax, 0));
           TileMeta &me = sh.meta[tile % kMeta];
+          // (a block in a page outside the cache has no scale: at kFarBelow and
+          // without the row by row look its weights, and what the sums get, are 0)
           const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(log2_of(now.vs) - log2_of(vmax), kFarBelow) : kFarBelow;
           if (lane < kTileBlocks) {
             me.kc[lane] = fmaxf(now.ks * kc_all, 0x1p-120f);

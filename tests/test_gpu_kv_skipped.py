@@ -136,3 +136,60 @@ def test_append_leaves_whole_tokens_out(ops, dtype, heads, dim, page, axes, firs
                 assert np.array_equal(s[~same], want_s[~same])
                 assert np.array_equal(c[~out], model.codes[b, where[~out]])
                 assert np.array_equal(c[out], c0[out])
+
+
+def attention_without(cache_t, table, q, new, lens, window, sinks):
+    """Output and error bound of each row in 64 bits; keys in pages outside the cache are hidden (as test_gpu_kv.attention64 has it else)."""
+    k, v, ks, vs = (c.cpu() for c in cache_t)
+    pages, heads, page, dim = k.shape
+    group, scale, at, outs, bounds = q.shape[1] // heads, dim ** -0.5, 0, [], []
+    for b, n in enumerate(new):
+        at += n
+        if not n:
+            continue
+        have = np.arange(lens[b])
+        page_of = table[b, have // page]
+        inside = torch.from_numpy((page_of >= 0) & (page_of < pages))
+        p_, s_ = np.where(inside, page_of, 0), have % page
+        K, V = ((c[p_, :, s_].double() * s[p_, :, s_ // BLOCK].double()[..., None]).transpose(0, 1) for c, s in ((k, ks), (v, vs)))
+        Q = q[at - n:at].double().cpu().transpose(0, 1).reshape(heads, group, n, dim)
+        p, j = torch.arange(lens[b] - n, lens[b])[:, None], torch.arange(lens[b])
+        seen = (j <= p) & inside
+        if window:
+            seen &= (p - j < window) | (j < sinks)
+        s = torch.einsum("hgnd,hkd->hgnk", Q, K) * scale
+        big = torch.einsum("hgnd,hkd->hgnk", Q.abs(), K.abs()) * scale
+        w = torch.softmax(s.masked_fill(~seen, -torch.inf), -1).nan_to_num(0.0)
+        o, mass = torch.einsum("hgnk,hkd->hgnd", w, V), torch.einsum("hgnk,hkd->hgnd", w, V.abs())
+        off = (big * (dim + 4) * 2.0 ** -24 + s.abs() * 2.0 ** -21).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        bounds.append((mass * (2 * off + 2.0 ** -11 + 2.0 ** -16)).permute(2, 0, 1, 3).reshape(n, heads * group, dim))
+        outs.append(o.permute(2, 0, 1, 3).reshape(n, heads * group, dim))
+    return torch.cat(outs), torch.cat(bounds)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 20)])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [2000, 60, 700]), ([5, 0, 2], [900, 10, 300]), ([300, 40, 1], [1500, 300, 200]), ([700], [700])])
+def test_attend_hides_keys_in_pages_outside_the_cache(ops, dim, window, sinks, new, lens):
+    heads, group, page = 2, 4, 16
+    table, pages = page_table(lens, page, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    cache_t = [torch.randint(-127, 128, (pages, heads, page, dim), generator=g, device="cuda").to(torch.int8) for _ in range(2)]
+    cache_t += [2.0 ** torch.randint(-9, -4, (pages, heads, 1), generator=g, device="cuda").float() for _ in range(2)]
+    q = torch.randn((sum(new), heads * group, dim), generator=g, device="cuda").mul_(2).half()
+    for bad in ([0], [1, 5, 6], [3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14]):  # one block, some, a whole tile of 128 keys
+        t = table.copy()
+        for i, c in enumerate(bad):
+            if c < -(-lens[0] // page):
+                t[0, c] = (pages, -1, 2 ** 31 - 1, -2 ** 31)[i % 4]
+        out = torch.full_like(q, float("nan"))
+        ops.attend(ivb.KvCache(*cache_t), q, out, offsets_of(new), ints(lens), ints(t), max_new=max(new), window=window, sinks=sinks, stream=stream())
+        want, bound = attention_without(cache_t, t, q, new, lens, window, sinks)
+        got = out.double().cpu()
+        assert ((got - want).abs() <= bound * 1.01 + 2.0 ** -11 * want.abs() + 2.0 ** -25).all()
+        read = any((page_first <= lens[0] - 1) and (not window or page_first < sinks or (c + 1) * page - 1 > lens[0] - new[0] - window)
+                   for c in bad for page_first in [c * page])
+        if read:
+            reported(ops)
+        else:
+            ops.synchronize(stream())
