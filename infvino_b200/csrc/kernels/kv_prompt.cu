@@ -642,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float x = s[kKvBlock * b];
 #pragma unroll
               for (int k = 1; k < kKvBlock; ++k) x = fmaxf(x, s[kKvBlock * b + k]);
+              if (lvf[b] == -INFINITY) continue;  // (no block)
               lvf[b] = fmaxf(lvf[b], fminf(kFar, m - x * c[b] - 70.f));
               ivf[b] = fast_exp2(-lvf[b] - kSumBits);
             }
@@ -845,13 +846,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int o = 4; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
           vmax = fmaxf(vref, __shfl_sync(0xffffffffu, vmax, 0));
           TileMeta &me = sh.meta[tile % kMeta];
-          // (a block in a page outside the cache has no scale: at kFarBelow and
-          // without the row by row look its weights, and what the sums get, are 0)
           const float lv = vmax > 0.f && now.vs > 0.f ? fmaxf(log2_of(now.vs) - log2_of(vmax), kFarBelow) : kFarBelow;
           if (lane < kTileBlocks) {
             me.kc[lane] = fmaxf(now.ks * kc_all, 0x1p-120f);
-            me.lvf[lane] = lv;
-            me.ivf[lane] = fast_exp2(-fmaxf(lv, kFar) - kSumBits);
+            // (a block in a page outside the cache: weights and sums of 0)
+            const bool none = now.key0 == kNoKey;
+            me.lvf[lane] = none ? -INFINITY : lv;
+            me.ivf[lane] = none ? 0.f : fast_exp2(-fmaxf(lv, kFar) - kSumBits);
             me.key0[lane] = now.key0;
           }
           const uint32_t far = __ballot_sync(0xffffffffu, lane < kTileBlocks && now.key0 != kNoKey && lv < kFar);

@@ -167,16 +167,19 @@ def attention_without(cache_t, table, q, new, lens, window, sinks):
     return torch.cat(outs), torch.cat(bounds)
 
 
+@pytest.mark.parametrize("tiny", [False, True])  # the least value scale beside the missing blocks
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (300, 20)])
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [2000, 60, 700]), ([5, 0, 2], [900, 10, 300]), ([300, 40, 1], [1500, 300, 200]), ([700], [700])])
-def test_attend_hides_keys_in_pages_outside_the_cache(ops, dim, window, sinks, new, lens):
+def test_attend_hides_keys_in_pages_outside_the_cache(ops, dim, window, sinks, new, lens, tiny):
     heads, group, page = 2, 4, 16
     table, pages = page_table(lens, page, seed=3)
     g = torch.Generator(device="cuda").manual_seed(dim)
     cache_t = [torch.randint(-127, 128, (pages, heads, page, dim), generator=g, device="cuda").to(torch.int8) for _ in range(2)]
     cache_t += [2.0 ** torch.randint(-9, -4, (pages, heads, 1), generator=g, device="cuda").float() for _ in range(2)]
     q = torch.randn((sum(new), heads * group, dim), generator=g, device="cuda").mul_(2).half()
+    if tiny:
+        cache_t[3][table[0, ::2].clip(0)] = 2.0 ** -120
     for bad in ([0], [1, 5, 6], [3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14]):  # one block, some, a whole tile of 128 keys
         t = table.copy()
         for i, c in enumerate(bad):
