@@ -49,7 +49,7 @@ constexpr int kStepStages = 4;  // blocks of a warp's ring; two are worked on at
 constexpr int kStepMinBlocks = 4 * kStepWarps;
 // A row's maximum follows its scores only when one is kStepSlack above it: the
 // sums are rescaled rarely, and weights stay below 2^(kStepBits + kStepSlack).
-constexpr float kStepSlack = 4.f, kStepBits = kWeightBits - kStepSlack;
+constexpr float kStepSlack = 4.f, kStepBits = 10.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -413,13 +413,15 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(m[t][c] + lvr, mx[t][c]), room = kv_room(l[t][c]);
+            float x = mx[t][c], room = kv_room(l[t][c]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
               room = fminf(room, __shfl_xor_sync(0xffffffffu, room, o));
             }
-            x = fmaxf(x, m[t][c] - room);
+            // (a row's m goes by its own scores alone, whichever row brought the warp here)
+            const float md = fmaxf(m[t][c] + lvr, m[t][c] - room);
+            x = x > md + kStepSlack ? x : md;
             const float d = x != m[t][c] ? m[t][c] - x : 0.f, f = fast_exp2(d + lvr);
             l[t][c] = kv_scaled(l[t][c], d);
             m[t][c] = x;

@@ -7,12 +7,6 @@ namespace ivb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Weights times value scales are halves of at most 2^kWeightBits.  The largest of
-// a row is at least 2^(kWeightBits - slack), where slack (4 or 6, in the kernels)
-// is how far a row's reference m may lag behind, so halves keep their 11 bits
-// down to 2^-(14 + kWeightBits - slack) of it: 2^-24 or 2^-22.
-constexpr float kWeightBits = 14.f;
-
 // 2^x (relative error about 2^-22; 0 for -inf).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
@@ -28,7 +22,10 @@ __device__ __forceinline__ float log2_of(float x) {  // (-inf for 0; exact for p
 
 // A row's reference m is the largest s + lv of the keys that it sees, where lv is
 // log2 (vs / vref): the largest weight times value scale, and not the largest
-// weight, sets what the halves can hold.  vref, the largest value scale so far, is
+// weight, sets what the halves can hold.  m lags behind by up to a slack; a row's
+// largest weight times value scale is from 2^bits to 2^(bits + slack) as a half
+// (bits, slack: 10, 4 and 8, 7.5 in the two kernels; halves end at 2^16), so that
+// halves keep their 11 bits down to 2^-24 and 2^-22 of it.  vref, the largest value scale so far, is
 // common to the rows of an item; where it grows m is lowered with it, so that
 // keys that are hidden from a row do not count for it.  s - m can be as large as
 // -lv then, so sums of 2^(s - m) are kept in units of 2^-kSumBits.
