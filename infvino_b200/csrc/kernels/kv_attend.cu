@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       float up = a.scale * kLog2e / kTiny;
       if (BF16) {
         // bf16 queries become halves: the row is scaled by a power of two so
-        // that its largest element lies in 2^0 .. 2^1 (its eight bits stay)
+        // that its largest element lies in 2^15 .. 2^16 (eight bits are exact
+        // down to 2^-32 of it)
         float most = 0.f;
 #pragma unroll
         for (int k = 0; k < 2 * kTiles; ++k) {
@@ -299,9 +300,9 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        up *= __uint_as_float((uint32_t)e << 23);
+        const int e = min(max((int)(__float_as_uint(most) >> 23), 16), 254);  // biased
+        const float down = __uint_as_float((uint32_t)(269 - e) << 23);
+        up *= __uint_as_float((uint32_t)(e - 15) << 23);
 #pragma unroll
         for (int k = 0; k < 2 * kTiles; ++k) {
           const float2 f = unpack2<true>(w[k]);

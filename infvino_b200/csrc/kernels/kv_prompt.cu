@@ -486,20 +486,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           w[e].x ^= flip, w[e].y ^= flip, w[e].z ^= flip, w[e].w ^= flip;
           if (BF16) {
             // bf16 queries become halves: scaled by a power of two so that the
-            // row's largest element lies in 2^0 .. 2^1 (its eight bits stay)
+            // row's largest element lies in 2^15 .. 2^16 (eight bits are exact
+            // down to 2^-32 of it)
             float f[8], most = 0.f;
             unpack8<true>(w[e], f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
 #pragma unroll
             for (int o = kLanes / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const int x = min(max((int)(__float_as_uint(most) >> 23), 1), 253);  // biased
-            const float down = __uint_as_float((uint32_t)(254 - x) << 23);
+            const int x = min(max((int)(__float_as_uint(most) >> 23), 16), 254);  // biased
+            const float down = __uint_as_float((uint32_t)(269 - x) << 23);
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] *= down;
             w[e] = pack8<false>(f);
             const int own = (lane % kAtOnce) * kLanes;  // (lane / kAtOnce = (e0 + e): the row is this lane's)
-            const float up = __shfl_sync(0xffffffffu, __uint_as_float((uint32_t)x << 23), own);
+            const float up = __shfl_sync(0xffffffffu, __uint_as_float((uint32_t)(x - 15) << 23), own);
             if (lane / kAtOnce == e0 + e) rf = up;
           }
           const int row = 32 * (warp & 3) + rw;

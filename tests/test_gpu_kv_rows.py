@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import infvino_b200 as ivb
-from test_gpu_kv import TYPES, filled_cache, ints, offsets_of, page_table, stream
+from test_gpu_kv import HALF_ULP, TINY, TYPES, attention64, filled_cache, ints, offsets_of, page_table, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,25 @@ def test_rows_do_not_depend_on_their_neighbours(dtype, new, lens, heads, group, 
             ops.attend(cache, changed, got, *args, stream=stream(), **kw)
             ops.synchronize(stream())
             assert torch.equal(got[~other], out[~other]), seed
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ratio", [12, 18, 22])
+def test_small_query_elements_beside_a_large_one(dim, ratio):
+    """A bf16 query's largest element meets keys that are 0 there: the others, 2^-ratio of it, decide."""
+    new, lens, heads, group = [200, 90], [400, 90], 2, 2
+    table, pages = page_table(lens, 32)
+    k, v, ks, vs = filled_cache(pages, heads, 32, dim, ratio)
+    k[..., 3] = 0
+    ks = torch.full_like(ks, 2.0 ** (ratio - 8))
+    g = torch.Generator(device="cuda").manual_seed(dim + ratio)
+    q = torch.randn((sum(new), heads * group, dim), generator=g, device="cuda") * 2.0 ** -ratio
+    q[..., 3] = torch.where(torch.rand(q.shape[:2], generator=g, device="cuda") < 0.5, -1.5, 1.9)
+    q = q.to(torch.bfloat16)
+    out = torch.empty_like(q)
+    with ivb.KvOps(0) as ops:
+        ops.attend(ivb.KvCache(k, v, ks, vs), q, out, offsets_of(new), ints(lens), ints(table), max_new=max(new), stream=stream())
+        ops.synchronize(stream())
+    want, bound = attention64((k, v, ks, vs), table, q, new, lens, dim ** -0.5, 0, 0)
+    bound = bound * 1.01 + HALF_ULP["bf16"] * want.abs() + TINY["bf16"]
+    assert ((out.double().cpu() - want).abs() <= bound).all()
