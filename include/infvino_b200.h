@@ -308,7 +308,10 @@ int ivc_kv_create(int device_ordinal, ivc_kv **out);
 void ivc_kv_destroy(ivc_kv *h);
 /* Message of the last failed call on `h`; with h == NULL, of the last failed ivc_kv_create. */
 const char *ivc_kv_last_error(const ivc_kv *h);
-/* Waits for `stream` and reports what the kernels found wrong. */
+/* Waits for `stream` and reports what the kernels found wrong, once.  There is
+ * one status word for a handle: with several streams the first call to come
+ * reports the first error of any of them, and clears the word (use a handle for
+ * each stream where that matters).  Other threads' calls do not wait for it. */
 int ivc_kv_synchronize(ivc_kv *h, void *stream);
 /* Allocates the stream's attention workspace (else its first ivc_kv_attend does). */
 int ivc_kv_reserve(ivc_kv *h, void *stream);

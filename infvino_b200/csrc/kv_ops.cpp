@@ -64,12 +64,10 @@ void cuda(cudaError_t e, const char *what) {
   throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// Runs f on the handle's device; what it throws becomes a status and a message.
 template <class F>
-int guarded(ivc_kv *h, const char *call, F &&f) {
-  if (!h) return IVC_ERR_ARGUMENT;
-  std::lock_guard<std::mutex> lk(h->mu);
+int attempt(ivc_kv *h, std::string &why, F &&f) {
   int code = IVC_ERR_CUDA;
-  std::string why;
   try {
     Scope scope(h->device);
     f();
@@ -82,10 +80,24 @@ int guarded(ivc_kv *h, const char *call, F &&f) {
   } catch (...) {
     why = "unknown error";
   }
+  return code;
+}
+
+// (under the handle's lock)
+void note(ivc_kv *h, const char *call, const std::string &why) {
   try {
     h->err = std::string(call) + ": " + why;
   } catch (...) {
   }
+}
+
+template <class F>
+int guarded(ivc_kv *h, const char *call, F &&f) {
+  if (!h) return IVC_ERR_ARGUMENT;
+  std::lock_guard<std::mutex> lk(h->mu);
+  std::string why;
+  const int code = attempt(h, why, f);
+  if (code != IVC_OK) note(h, call, why);
   return code;
 }
 
@@ -252,8 +264,11 @@ const char *ivc_kv_last_error(const ivc_kv *h) {
 }
 
 int ivc_kv_synchronize(ivc_kv *h, void *stream) {
+  if (!h) return IVC_ERR_ARGUMENT;
   int word = 0;
-  const int r = guarded(h, "ivc_kv_synchronize", [&] {
+  std::string why;
+  // (not under the handle's lock: other threads' calls need not wait for this stream)
+  int r = attempt(h, why, [&] {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cuda(cudaMemcpyAsync(&word, h->status, sizeof(int), cudaMemcpyDeviceToHost, st), "status word");
     cuda(cudaStreamSynchronize(st), "synchronize");
@@ -262,15 +277,19 @@ int ivc_kv_synchronize(ivc_kv *h, void *stream) {
       cuda(cudaStreamSynchronize(st), "synchronize");
     }
   });
-  if (r != IVC_OK || word == 0) return r;
-  std::lock_guard<std::mutex> lk(h->mu);
-  h->err = std::string("ivc_kv_synchronize: ") +
-           (word == 16   ? "a page number outside the cache"
-            : word == 17 ? "offsets, positions or lengths that do not fit the call"
-            : word == 18 ? "a position outside the rotary table"
-                         : "a kernel's bounded wait timed out") +
-           " (status " + std::to_string(word) + ")";
-  return IVC_ERR_KERNEL;
+  if (r == IVC_OK && word != 0) {
+    r = IVC_ERR_KERNEL;
+    why = std::string(word == 16   ? "a page number outside the cache"
+                      : word == 17 ? "offsets, positions or lengths that do not fit the call"
+                      : word == 18 ? "a position outside the rotary table"
+                                   : "a kernel's bounded wait timed out") +
+          " (status " + std::to_string(word) + ")";
+  }
+  if (r != IVC_OK) {
+    std::lock_guard<std::mutex> lk(h->mu);
+    note(h, "ivc_kv_synchronize", why);
+  }
+  return r;
 }
 
 int ivc_kv_reserve(ivc_kv *h, void *stream) {

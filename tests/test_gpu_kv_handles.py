@@ -1,5 +1,6 @@
 """Handles of the language-model operators: streams, threads, workspaces, status."""
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -146,3 +147,32 @@ def test_calls_after_a_timed_out_one(dim):
                     ops.synchronize(st)
                     assert torch.equal(d.out, want)
         assert L.ivc_debug_kv_probe(ops._h, -1) == 1
+
+
+def test_waiting_for_one_stream_does_not_hold_up_calls_on_another():
+    c = Call(12, [1, 1], [500, 300])
+    want = c.expected()
+    slow, fast = torch.cuda.Stream(), torch.cuda.Stream()
+    with ivb.KvOps(0) as ops:
+        c.run(ops, fast.cuda_stream)  # (its workspace)
+        c.out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(slow):
+            torch.cuda._sleep(2_000_000_000)  # about a second
+        entered, done = threading.Event(), threading.Event()
+
+        def wait():
+            entered.set()
+            ops.synchronize(slow.cuda_stream)
+            done.set()
+
+        t = threading.Thread(target=wait)
+        t.start()
+        entered.wait()
+        time.sleep(0.1)
+        c.run(ops, fast.cuda_stream)
+        fast.synchronize()
+        first = not done.is_set()
+        t.join()
+        assert first, "the call waited for the other stream"
+        assert torch.equal(c.out, want)
