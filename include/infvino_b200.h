@@ -306,7 +306,9 @@ typedef struct ivc_rotary {
 
 int ivc_kv_create(int device_ordinal, ivc_kv **out);
 void ivc_kv_destroy(ivc_kv *h);
-/* Message of the last failed call on `h`; with h == NULL, of the last failed ivc_kv_create. */
+/* Message of the calling thread's last failed call on `h` (for a thread without
+ * one, of any thread's); with h == NULL, of its last failed ivc_kv_create.  Valid
+ * until the thread's next call of this function. */
 const char *ivc_kv_last_error(const ivc_kv *h);
 /* Waits for `stream` and reports what the kernels found wrong, once.  There is
  * one status word for a handle: with several streams the first call to come

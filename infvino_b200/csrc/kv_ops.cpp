@@ -17,8 +17,9 @@
 
 struct ivc_kv {
   int device = 0, sms = 0;
-  std::mutex mu;
-  std::string err;
+  mutable std::mutex mu;
+  std::string err;                              // of the last failed call,
+  std::map<std::thread::id, std::string> errs;  // and of each thread's
   int *status = nullptr;
   long long probe = 0;
   std::map<unsigned long long, void *> workspace;  // by the stream's id
@@ -27,8 +28,8 @@ struct ivc_kv {
 
 namespace {
 
-std::string g_kv_create_err;
-std::mutex g_kv_create_mu;
+thread_local std::string g_kv_create_err;
+thread_local std::string g_kv_shown_err;  // what this thread's ivc_kv_last_error has returned: no other thread writes it
 
 // The handle's device for the length of a call, and launches with programmatic
 // dependent launch whatever an engine on this thread last chose.
@@ -87,6 +88,7 @@ int attempt(ivc_kv *h, std::string &why, F &&f) {
 void note(ivc_kv *h, const char *call, const std::string &why) {
   try {
     h->err = std::string(call) + ": " + why;
+    h->errs[std::this_thread::get_id()] = h->err;
   } catch (...) {
   }
 }
@@ -237,7 +239,6 @@ int ivc_kv_create(int device_ordinal, ivc_kv **out) {
   }
   ivc_kv_destroy(h);
   try {
-    std::lock_guard<std::mutex> lk(g_kv_create_mu);
     g_kv_create_err = "ivc_kv_create: " + why;
   } catch (...) {
   }
@@ -256,11 +257,15 @@ void ivc_kv_destroy(ivc_kv *h) {
 }
 
 const char *ivc_kv_last_error(const ivc_kv *h) {
-  if (!h) {
-    std::lock_guard<std::mutex> lk(g_kv_create_mu);
-    return g_kv_create_err.c_str();
+  if (!h) return g_kv_create_err.c_str();
+  std::lock_guard<std::mutex> lk(h->mu);
+  try {
+    const auto it = h->errs.find(std::this_thread::get_id());
+    g_kv_shown_err = it != h->errs.end() ? it->second : h->err;
+  } catch (...) {
+    return "";
   }
-  return h->err.c_str();
+  return g_kv_shown_err.c_str();
 }
 
 int ivc_kv_synchronize(ivc_kv *h, void *stream) {

@@ -176,3 +176,39 @@ def test_waiting_for_one_stream_does_not_hold_up_calls_on_another():
         t.join()
         assert first, "the call waited for the other stream"
         assert torch.equal(c.out, want)
+
+
+def test_threads_share_a_handle():
+    """Calls, errors and waits from several threads at once, each on a stream of its own."""
+    calls = [Call(20 + i, [1, 1, 40], [3000, 500, 900]) for i in range(4)]
+    wants = [c.expected() for c in calls]
+    wrong = []
+    with ivb.KvOps(0) as ops:
+        def work(c, want):
+            try:
+                calls_of(c, want)
+            except Exception as e:
+                wrong.append(repr(e))
+
+        def calls_of(c, want):
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(30):
+                    c.out.zero_()
+                    c.run(ops, s.cuda_stream)
+                    try:
+                        ops.attend(c.cache, c.q, c.out, c.offsets, c.lens, c.table, max_new=0, stream=s.cuda_stream)
+                        wrong.append("not refused")
+                    except ivb.NativeError as e:
+                        if e.status != 1 or "max_new" not in e.message:
+                            wrong.append(str(e))
+                    ops.synchronize(s.cuda_stream)
+                    if not torch.equal(c.out, want):
+                        wrong.append("other bits")
+
+        threads = [threading.Thread(target=work, args=z) for z in zip(calls, wants)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert not wrong, wrong[:3]
