@@ -228,7 +228,14 @@ int ivc_kv_create(int device_ordinal, ivc_kv **out) {
     cuda(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device_ordinal), "device attribute");
     Scope scope(device_ordinal);
     cuda(cudaMalloc(&h->status, sizeof(int)), "status word");
-    cuda(cudaMemset(h->status, 0, sizeof(int)), "status word");
+    // Zero before any stream's kernel can set it: in a stream of its own, for the
+    // legacy stream's order means nothing to streams that do not block.
+    cudaStream_t st = nullptr;
+    cuda(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking), "status word");
+    cudaError_t e = cudaMemsetAsync(h->status, 0, sizeof(int), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    (void)cudaStreamDestroy(st);
+    cuda(e, "status word");
     *out = h;
     return IVC_OK;
   } catch (const Bad &e) {

@@ -212,3 +212,21 @@ def test_threads_share_a_handle():
         for t in threads:
             t.join()
     assert not wrong, wrong[:3]
+
+
+def test_a_new_handle_keeps_errors_while_the_default_stream_is_busy():
+    table = torch.zeros((4, 32, 2), device="cuda")
+    x, pos = torch.zeros((1, 1, 64), dtype=torch.float16, device="cuda"), ints([9])
+    side = torch.cuda.Stream()
+    with ivb.KvOps(0) as ops:  # (what the first calls of all bring with them)
+        ops.rope(x, x, ivb.Rotary(table), ints([1]), stream=side.cuda_stream)
+        ops.synchronize(side.cuda_stream)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(600_000_000)  # some 0.3 s of the default stream
+    with ivb.KvOps(0) as ops:
+        ops.rope(x, x, ivb.Rotary(table), pos, stream=side.cuda_stream)
+        side.synchronize()
+        torch.cuda.synchronize()
+        with pytest.raises(ivb.NativeError) as e:
+            ops.synchronize(side.cuda_stream)
+        assert e.value.status == 5 and "rotary table" in e.value.message
