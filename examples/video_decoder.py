@@ -98,10 +98,10 @@ class Decoder:
 
     def generate(self, frames_tokens: torch.Tensor, steps: int):
         """Greedy tokens and each step's logits: the prompt, then one captured step replayed."""
-        logits, at = self.prompt(frames_tokens)
         length = frames_tokens.shape[0]
         if length + steps > self.max_len:
             raise ValueError(f"{length} prompt tokens and {steps} steps exceed max_len {self.max_len}")
+        logits, at = self.prompt(frames_tokens)
         token = logits.argmax(-1)
         start = torch.tensor([length], dtype=torch.int32, device="cuda")
         lens, pos = start + 1, torch.full((3, 1), at, dtype=torch.int32, device="cuda")

@@ -78,3 +78,17 @@ def test_decoder_refuses_what_does_not_fit(tmp_path):
     d = m.Decoder(layers=1, max_len=64)
     with pytest.raises(ValueError):
         d.generate(torch.zeros((60, 576), dtype=torch.float16, device="cuda"), 5)
+
+
+@pytest.mark.gpu
+def test_decoder_is_as_before_after_a_refusal():
+    """A prompt that is too long is refused before any of it runs."""
+    d = load().Decoder(layers=1, max_len=64)
+    x = torch.randn((40, 576), generator=torch.Generator().manual_seed(3)).half().cuda()
+    tokens, logits = d.generate(x, 5)
+    for count, steps in ((70, 5), (64, 1)):
+        with pytest.raises(ValueError):
+            d.generate(torch.zeros((count, 576), dtype=torch.float16, device="cuda"), steps)
+        d.ops.synchronize(d.stream())
+        again, same = d.generate(x, 5)
+        assert again == tokens and torch.equal(same, logits)
