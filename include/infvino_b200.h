@@ -255,7 +255,7 @@ typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1 } ivc_dtype;
 
 /* [tokens][heads][head_dim] of the call's dtype; strides in elements, the last
  * dimension dense.  Any 2-byte alignment works; 16-byte alignment of data and
- * strides takes the vector path. */
+ * strides takes the vector path.  Rows that are written do not overlap. */
 typedef struct ivc_rows {
   void *data;
   int64_t token_stride, head_stride;

@@ -149,6 +149,14 @@ ivb::KvRows rows(const ivc_rows *r, const char *what, int64_t tokens, int heads)
   return k;
 }
 
+// Rows that are written: no two may share elements.
+ivb::KvRows out_rows(const ivc_rows *r, const char *what, int64_t tokens, int heads, int dim) {
+  const ivb::KvRows k = rows(r, what, tokens, heads);
+  need((tokens <= 1 || k.ts >= dim || k.ts <= -dim) && (heads <= 1 || k.hs >= dim || k.hs <= -dim),
+       "rows that are written overlap");
+  return k;
+}
+
 void check_dtype(int dtype) { need(dtype == IVC_F16 || dtype == IVC_BF16, "dtype is IVC_F16 or IVC_BF16"); }
 
 ivb::KvRotary rotation(const ivc_rotary *r, int head_dim, int64_t tokens) {
@@ -359,7 +367,7 @@ int ivc_kv_rope(ivc_kv *h, int dtype, int64_t tokens, int heads, int head_dim, c
     need(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256, "head_dim: a multiple of 16, at most 256");
     need(rotary != nullptr, "no rotary");
     const ivb::KvRotary rot = rotation(rotary, head_dim, tokens);
-    const ivb::KvRows a = rows(x, "x is null", tokens, heads), b = rows(out, "out is null", tokens, heads);
+    const ivb::KvRows a = rows(x, "x is null", tokens, heads), b = out_rows(out, "out is null", tokens, heads, head_dim);
     if (tokens == 0) return;
     cuda(ivb::launch_kv_rope(dtype == IVC_BF16, tokens, heads, head_dim, a, b, rot, h->status,
                              static_cast<cudaStream_t>(stream)),
@@ -381,7 +389,7 @@ int ivc_kv_append(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
     ivb::KvRows qr{}, qo{};
     if (q_heads) {
       qr = rows(q, "q is null", s.tokens, q_heads);
-      qo = rows(q_out, "q_out is null", s.tokens, q_heads);
+      qo = out_rows(q_out, "q_out is null", s.tokens, q_heads, c.dim);
     }
     if (s.tokens == 0) return;
     cuda(ivb::launch_kv_append(dtype == IVC_BF16, c, s, kr, vr, rot, q_heads, qr, qo, h->status,
@@ -397,8 +405,8 @@ int ivc_kv_read(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, i
     const ivb::KvCache c = check_cache(cache);
     const ivb::KvSeqs s = check_seqs(seqs);
     ivb::KvRows kr{}, vr{};
-    if (k) kr = rows(k, "k is null", s.tokens, c.heads);
-    if (v) vr = rows(v, "v is null", s.tokens, c.heads);
+    if (k) kr = out_rows(k, "k is null", s.tokens, c.heads, c.dim);
+    if (v) vr = out_rows(v, "v is null", s.tokens, c.heads, c.dim);
     if (s.tokens == 0 || (!k && !v)) return;
     cuda(ivb::launch_kv_read(dtype == IVC_BF16, c, s, kr, vr, h->status, static_cast<cudaStream_t>(stream)), "launch");
   });
@@ -415,7 +423,7 @@ int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
     need(max_new >= 0 && (max_new > 0 || a.seqs.tokens == 0), "max_new is at least 1");
     need(window >= 0 && sinks >= 0, "window and sinks are not negative");
     a.q = rows(q, "q is null", a.seqs.tokens, q_heads);
-    a.out = rows(out, "out is null", a.seqs.tokens, q_heads);
+    a.out = out_rows(out, "out is null", a.seqs.tokens, q_heads, a.cache.dim);
     a.q_heads = q_heads;
     a.group = q_heads / a.cache.heads;
     a.max_new = max_new;

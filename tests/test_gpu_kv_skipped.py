@@ -196,3 +196,26 @@ def test_attend_hides_keys_in_pages_outside_the_cache(ops, dim, window, sinks, n
             reported(ops)
         else:
             ops.synchronize(stream())
+
+
+def test_overlapping_outputs_are_refused(ops):
+    t, heads, dim = 6, 4, 64
+    x = torch.randn((t, heads, dim), device="cuda").half()
+    rotary, pos = ivb.Rotary(torch.zeros((8, 32, 2), device="cuda")), ints(list(range(t)))
+    table, pages = page_table([t], 16)
+    cache = ivb.KvCache(*[torch.zeros((pages, heads, 16, dim), dtype=torch.int8, device="cuda") for _ in range(2)],
+                        *[torch.ones((pages, heads, 1), device="cuda") for _ in range(2)])
+    seqs = (offsets_of([t]), ints([0]), ints(table))
+    one = torch.zeros((t, heads, dim), dtype=torch.float16, device="cuda")
+    for bad in (one[:1].expand(t, heads, dim), one[:, :1].expand(t, heads, dim), one.view(-1).as_strided((t, heads, dim), (heads * 32, 32, 1))):
+        for call in (lambda: ops.rope(x, bad, rotary, pos, stream()), lambda: ops.read(cache, bad, None, *seqs, stream()),
+                     lambda: ops.read(cache, None, bad, *seqs, stream()),
+                     lambda: ops.append(cache, x, x, *seqs, rotary=rotary, pos=pos, q=x, q_out=bad, stream=stream()),
+                     lambda: ops.attend(cache, x, bad, seqs[0], ints([t]), seqs[2], max_new=t, stream=stream())):
+            with pytest.raises(ivb.NativeError) as e:
+                call()
+            assert e.value.status == 1 and "overlap" in e.value.message
+    ops.rope(x[:1].expand(t, heads, dim), one, rotary, pos, stream())  # inputs may
+    ops.attend(cache, x[:, :1].expand(t, heads, dim), one.transpose(0, 1).contiguous().transpose(0, 1), seqs[0], ints([t]), seqs[2], max_new=t, stream=stream())
+    ops.rope(x[:1], one.expand(1, t, heads, dim)[0][:1], rotary, pos[:1], stream())
+    ops.synchronize(stream())
