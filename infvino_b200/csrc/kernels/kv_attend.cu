@@ -49,7 +49,7 @@ constexpr int kStepStages = 4;  // blocks of a warp's ring; two are worked on at
 constexpr int kStepMinBlocks = 4 * kStepWarps;
 // A row's maximum follows its scores only when one is kStepSlack above it: the
 // sums are rescaled rarely, and weights stay below 2^(kStepBits + kStepSlack).
-constexpr float kStepSlack = 4.f, kStepBits = 10.f;
+constexpr float kStepSlack = 3.5f, kStepBits = 12.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

@@ -24,8 +24,8 @@ __device__ __forceinline__ float log2_of(float x) {  // (-inf for 0; exact for p
 // log2 (vs / vref): the largest weight times value scale, and not the largest
 // weight, sets what the halves can hold.  m lags behind by up to a slack; a row's
 // largest weight times value scale is from 2^bits to 2^(bits + slack) as a half
-// (bits, slack: 10, 4 and 8, 7.5 in the two kernels; halves end at 2^16), so that
-// halves keep their 11 bits down to 2^-24 and 2^-22 of it.  vref, the largest value scale so far, is
+// (bits, slack: 12, 3.5 and 8, 7.5 in the two kernels; halves end at 2^16), so that
+// halves keep their 11 bits down to 2^-26 and 2^-22 of it.  vref, the largest value scale so far, is
 // common to the rows of an item; where it grows m is lowered with it, so that
 // keys that are hidden from a row do not count for it.  s - m can be as large as
 // -lv then, so sums of 2^(s - m) are kept in units of 2^-kSumBits.
