@@ -410,16 +410,17 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         }
       if (__any_sync(0xffffffffu, above) || vnew > vref) {
         const float lvr = vnew > vref ? lref - lnew : 0.f;  // in units of the new vref the largest so far is lower by this
+        float most = 0.f;  // (fmaxf passes over NaN)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) most = fmaxf(most, fmaxf(l[t][0], l[t][1]));
+        const float room = kv_room(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))));
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = mx[t][c], room = kv_room(l[t][c]);
+            float x = mx[t][c];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-              room = fminf(room, __shfl_xor_sync(0xffffffffu, room, o));
-            }
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
             // (a row's m goes by its own scores alone, whichever row brought the warp here)
             const float md = fmaxf(m[t][c] + lvr, m[t][c] - room);
             x = x > md + kStepSlack ? x : md;
