@@ -49,6 +49,7 @@ constexpr int kStepStages = 4;  // blocks of a warp's ring; two are worked on at
 constexpr int kStepMinBlocks = 4 * kStepWarps;
 // A row's maximum follows its scores only when one is kStepSlack above it: the
 // sums are rescaled rarely, and weights stay below 2^(kStepBits + kStepSlack).
+constexpr float kNoValue = -1000.f;  // log2 of a value scale of 0
 constexpr float kStepSlack = 3.5f, kStepBits = 12.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
@@ -116,7 +117,7 @@ struct StepSlot {  // a part of a cut item: accumulators lane by lane in units o
 template <int DIM, int NT>
 struct StepShared {
   alignas(128) uint8_t ring[kStepWarps][kStepStages][2][kKvBlock * DIM];
-  float2 scales[kStepWarps][kStepStages];
+  float2 scales[kStepWarps][kStepStages];  // key scale, log2 of the value scale (-inf: no block)
   float m[kStepWarps][8 * NT], l[kStepWarps][8 * NT], lref[kStepWarps];
   long long scan[kStepWarps];
   long long base;
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   int head = 0, rt = 0, k0 = 0, k1 = 0, count = 0, looked = 0;
   uint32_t item_begin = 0;
   long long where = -1;  // lane i: where the i-th of the next 32 blocks' codes are, -1: none
-  float2 sc_mine = make_float2(0.f, -1.f);
+  float2 sc_mine = make_float2(0.f, -INFINITY);
   auto locate = [&]() {
     for (;;) {
       const uint32_t units = (uint32_t)s.blocks * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       if (it == looked) {
         looked += 32;
         where = -1;
-        sc_mine = make_float2(0.f, -1.f);
+        sc_mine = make_float2(0.f, -INFINITY);
         if (it + lane < count) {
           const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
           if (key < s.len) {
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
               const int slot = key - at * a.cache.page;
               where = kv_code_at(a.cache, page, head, slot);
               const long long sa = kv_scale_at(a.cache, page, head, slot);
-              sc_mine = make_float2(a.cache.ks[sa], a.cache.vs[sa]);
+              sc_mine = make_float2(a.cache.ks[sa], fmaxf(log2_of(a.cache.vs[sa]), kNoValue));
             } else {
               kv_flag(a.status, kStatusKvPage);
             }
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.f;
     }
-    float vref = 0.f, vinv = 0.f, lref = -INFINITY;  // acc is in units of vref, the largest value scale so far; log2 of it
+    float lref = -INFINITY;  // acc is in units of vref, the largest value scale so far: log2 of it
 
     for (int it = 0; it < count; it += kZ) {
       cp_async_wait<kStepStages - kZ>();
@@ -347,12 +348,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       const int st = it % kStepStages;  // (a multiple of kZ)
       // scores of keys g, g + 8 of each block
       float sc[kZ][NT][4];
-      float vs[kZ];
+      float lv[kZ];
 #pragma unroll
       for (int z = 0; z < kZ; ++z) {
         const float2 scales = sh.scales[warp][st + z];
-        vs[z] = z == 0 || it + z < count ? scales.y : -1.f;
-        if (vs[z] < 0.f) {
+        lv[z] = z == 0 || it + z < count ? scales.y : -INFINITY;
+        if (lv[z] == -INFINITY) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) sc[z][t][0] = sc[z][t][1] = sc[z][t][2] = sc[z][t][3] = -INFINITY;
           continue;
@@ -393,11 +394,10 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         }
       }
       // the value scale, and the rows' maxima of s + log2 (vs / vref), where one is well above
-      const float vnew = fmaxf(vref, fmaxf(vs[0], vs[kZ - 1]));
-      const float lnew = vnew > vref ? log2_of(vnew) : lref;
-      float lv[kZ];
+      const float lnew = fmaxf(lref, fmaxf(lv[0], lv[kZ - 1]));
+      const bool there[2] = {lv[0] != -INFINITY, lv[kZ - 1] != -INFINITY};
 #pragma unroll
-      for (int z = 0; z < kZ; ++z) lv[z] = fmaxf(log2_of(vs[z]) - lnew, kFarBelow);  // (a block without keys: any)
+      for (int z = 0; z < kZ; ++z) lv[z] = fmaxf(lv[z] - lnew, kFarBelow);
       float mx[NT][2];
       bool above = false;
 #pragma unroll
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
           if (kZ == 2) mx[t][c] = fmaxf(mx[t][c], fmaxf(sc[kZ - 1][t][c], sc[kZ - 1][t][c + 2]) + lv[kZ - 1]);
           above = above || mx[t][c] > m[t][c] + kStepSlack;
         }
-      if (__any_sync(0xffffffffu, above) || vnew > vref) {
-        const float lvr = vnew > vref ? lref - lnew : 0.f;  // in units of the new vref the largest so far is lower by this
+      if (__any_sync(0xffffffffu, above) || lnew > lref) {
+        const float lvr = lnew > lref ? lref - lnew : 0.f;  // in units of the new vref the largest so far is lower by this
         float most = 0.f;  // (fmaxf passes over NaN)
 #pragma unroll
         for (int t = 0; t < NT; ++t) most = fmaxf(most, fmaxf(l[t][0], l[t][1]));
@@ -433,14 +433,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
               acc[t][j][c + 2] *= f;
             }
           }
-        vref = vnew;
         lref = lnew;
-        vinv = vref > 0.f ? 1.f / vref : 0.f;
       }
 #pragma unroll
       for (int z = 0; z < kZ; ++z) {
-        if (vs[z] < 0.f) continue;
-        const float vf = vs[z] * vinv * 0x1p64f;  // 2^(lv + kSumBits)
+        if (!there[z]) continue;
+        const float vf = fast_exp2(lv[z] + kSumBits);
         uint32_t p[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
