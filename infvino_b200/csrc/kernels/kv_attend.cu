@@ -105,8 +105,10 @@ __device__ __forceinline__ uint32_t tile_swizzle(uint32_t o) {
   return o ^ (f << 4);
 }
 
-// CTAs an SM, by registers (and, for wide heads, the rings)
-constexpr int step_ctas(int dim, int nt) { return nt == 1 && dim == 64 ? 4 : 3; }
+// CTAs an SM, by registers (and, for wide heads, the rings).  16 rows of 128-wide
+// heads take 240 registers, three CTAs leave 168: 24 sequences of up to 6001
+// tokens, 8 kv heads, at 16, 32, 64 rows 78, 130, 241 us, two CTAs 66, 115, 209.
+constexpr int step_ctas(int dim, int nt) { return dim == 128 ? (nt == 1 ? 3 : 2) : (nt == 1 ? 4 : 3); }
 
 template <int DIM, int NT>
 struct StepSlot {  // a part of a cut item: accumulators lane by lane in units of 2^t, then each row's m, sum and t
