@@ -3,8 +3,9 @@
 //
 // For a query at position p and the visible keys j (codes kc, vc; scales ks, vs):
 //   s_j = scale * ks_j * (q . kc_j),  o = sum_j e^(s_j - m) vs_j vc_j / sum_j e^(s_j - m)
-// in one pass with a running maximum m.  A decode step reads every visible
-// code once and does a few operations for each, so the cache's bytes bound it.
+// in one pass with a running reference m (the largest weight times value scale).
+// A decode step reads every visible code once and does a few operations for each,
+// so the cache's bytes bound it.
 //
 // An item is a tile of 8 or 16 query rows (token, head of the group) of one
 // sequence and kv head; its units are the key blocks (16 keys that share a
@@ -22,18 +23,21 @@
 // a handful of queries fills an instruction and a code is converted once for
 // all of them.  Value codes become halves exactly (1024 + code + 128 by a byte
 // permutation, minus 1152); key codes stay code + 128, and 128 times the
-// query's sum comes off the score: an offset far below the score's error
-// bound, where for the values it would cost bits.  The order of head elements
-// and keys inside the products is chosen so that every lane reads whole 16-byte
-// (64-wide heads: 8-byte) pieces of a row; the weights turn into the second
-// product's operand by transposing 8 x 8 pieces in registers.
+// query's sum comes off the score (16 sequences of 131072: 660 us, 688 with exact
+// codes).  A score's rounding error then goes by 2^-24 scale ks sum |q| (|code| +
+// 128) and not |q code|: below 1 / 1000 of what rounding the keys to codes has
+// cost, unless a query element is some 2^14 times the others where codes are small.
+// The order of head elements and keys inside the products is chosen so that every
+// lane reads whole 16-byte (64-wide heads: 8-byte) pieces of a row; the weights turn
+// into the second product's operand by transposing 8 x 8 pieces in registers.
 //
-// 16 sequences of 131072 tokens, 8 heads of 128: 660 to 717 us, 6.0 to 6.5 TB/s
-// (a copy reaches 6.5); 48 of up to 16384: 165 us, 6.1 TB/s.  Sliding windows of
-// 1024 over 128 sequences (64 wide): 24 us (floor 10), the start of the shares
-// and their joins; six drafted tokens for 24 sequences, 30 rows: 50 us (floor
-// 14), the latency of conversion, products and softmax in turn, at twelve warps
-// an SM and for two row tiles.
+// 16 sequences of 131072 tokens, 8 heads of 128: 650 to 720 us, 6.0 to 6.6 TB/s
+// (a copy reaches 6.5); 48 of up to 16384: 165 us, 6.1 TB/s (186 after a flush of
+// the L2, which else holds a fifth of them).  Sliding windows of 1024 over 128
+// sequences (64 wide): 23 us (floor 10), the start of the shares and their joins;
+// six drafted tokens for 24 sequences, 30 rows: 50 us (floor 14), the latency of
+// conversion, products and softmax in turn, at twelve warps an SM and for two row
+// tiles.
 #include <algorithm>
 
 #include "kv_attend.cuh"
@@ -632,8 +636,9 @@ cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_
 template <bool BF16, int DIM>
 cudaError_t launch_step_rows(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   // Rows beyond 16 come as further items: their codes are read again, from L2
-  // (24 sequences of 6001, 30 rows of 64 wide heads: 58 us; tiles of 32 rows,
-  // which read them once but leave room for half the warps, 65 us).
+  // (24 sequences of 6001, 30 rows of 64 wide heads: 58 us when it was compared,
+  // 50 now; tiles of 32 rows, which read them once but leave room for half the
+  // warps, 65 us).
   if ((long long)a.max_new * a.group <= 8) return launch_step<BF16, DIM, 1>(a, workspace, sms, st);
   return launch_step<BF16, DIM, 2>(a, workspace, sms, st);
 }
@@ -647,9 +652,16 @@ size_t kv_workspace_bytes(int sms) {
 }
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
-  // Rows of one sequence and kv head: 24 sequences of up to 6001 tokens take the
-  // kernel for many queries 102 / 98 / 109 us at 64 / 96 / 128 rows (64 wide)
-  // and 144 us at 48 (128 wide), this one 99 / 125 / 173 and 116 us.
+  // Rows of one sequence and kv head (max_new has to do for all sequences).  Us in
+  // this kernel / in the one for many queries, 8 kv heads, at 32, 48, 64 rows:
+  //   24 sequences of up to 6001 tokens   64 wide   74/119  106/118  134/118
+  //                                      128 wide  115/180  163/180  210/181
+  //   one of 8192                         64 wide   26/27    21/28    23/28
+  //                                      128 wide   29/38    29/38    30/38
+  //   4 of 2000                           64 wide   19/22    19/22    20/22
+  //                                      128 wide   23/28    26/29    28/29
+  // At 96 and 128 rows (64 wide, 24 sequences) it was 125/98 and 173/109: few
+  // sequences gain from this one up to 64 rows and beyond, many up to some 50.
   if ((long long)a.max_new * a.group > 64 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, a, workspace, sms, st);
   if (a.cache.dim == 64)
     return bf16 ? launch_step_rows<true, 64>(a, workspace, sms, st) : launch_step_rows<false, 64>(a, workspace, sms, st);

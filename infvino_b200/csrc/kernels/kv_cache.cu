@@ -112,7 +112,7 @@ __global__ void kv_rope_table_k(const __grid_constant__ KvRopeFreq f, int pairs,
 
 // Heads a thread turns by the same angles at once: what hides the chain from
 // position to table row is the rows in flight meanwhile, 2 x 16 bytes a head,
-// more than the number of warps.  16381 tokens, 28 heads of 128: 44 us, 5.3
+// more than the number of warps.  16381 tokens, 28 heads of 128: 44.5 us, 5.3
 // TB/s (floor 36); 4 heads and three CTAs an SM 47, 2 heads and four 50.
 constexpr int kRopeThreads = 256;
 constexpr int kRopeHeads = 8;
@@ -416,7 +416,7 @@ __device__ __forceinline__ void find_places(const KvCache &c, const KvSeqs &s, l
 // order.  The other CTAs turn queries.
 //
 // Latency bounds it: two joins and a block's loads for each head in turn.  9375
-// tokens, 8 heads of 128 beside 32 of queries: 44 us, 4.8 TB/s (floor 32); 64
+// tokens, 8 heads of 128 beside 32 of queries: 45 us, 4.7 TB/s (floor 32); 64
 // conversations, a token each: 4.3 us.
 template <bool BF16, bool INTER, int DIM, bool VEC, int TEAM>
 __global__ void __launch_bounds__(kAppendThreads, append_ctas(DIM, TEAM)) kv_append_k(const __grid_constant__ AppendArgs a) {
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(kAppendThreads, append_ctas(DIM, TEAM)) kv_app
 // A CTA takes `window` packed tokens, all heads.  A thread keeps its place in
 // the rows (keys or values, head, eight elements: 16 bytes out, so that a warp
 // writes whole lines) and goes over the tokens, kReadAhead of them on their way
-// at once.  9375 tokens, 8 heads of 128: 10.2 us, 5.7 TB/s (floor 8.9); sixteen
-// elements a thread, in two stores, 17.4.
+// at once.  9375 tokens, 8 heads of 128: 10.4 us with the codes in the L2, 14.6
+// after a flush of it (floor 8.9); sixteen elements a thread, in two stores, 17.4.
 constexpr int kReadAhead = 4, kReadThreads = 256;
 template <bool BF16, int DIM>
 __global__ void __launch_bounds__(kReadThreads)
@@ -547,7 +547,7 @@ cudaError_t launch_kv_append(bool bf16, const KvCache &c, const KvSeqs &s, const
   a.window = window_of(s.tokens);
   // Two warps a block where most blocks get a token or two (64 conversations, 8
   // heads: 4.3 us; four warps 5.0), one row a lane where they are filled (9375
-  // tokens: 47 us; 53).
+  // tokens, when it was compared: 47 us; two warps 53).
   const int team = a.window == 1 ? 2 : c.dim / 32, teams = kAppendThreads / 32 / team;
   // A CTA loops over the heads where there are blocks enough for two CTAs an
   // SM; fewer take the heads side by side.

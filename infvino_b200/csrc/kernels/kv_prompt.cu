@@ -15,8 +15,8 @@
 // Sixteen warps a CTA:
 //   0-3, 4-7  softmax of M tile 0 and 1, a thread a row: scores from TMEM, the
 //             weights back into the scores' columns as the next product's
-//             operand; O is rescaled in TMEM, rarely (a row's maximum follows
-//             only scores kSlack above it); at the end O goes out
+//             operand; O is rescaled in TMEM, rarely (a row's reference follows
+//             only what is kSlack above it); at the end O goes out
 //   8-11      key and value codes from the cache through registers into shared
 //             memory as halves (exact), one tile ahead in registers and two in
 //             shared memory; the blocks' scales beside them
@@ -26,18 +26,20 @@
 //             under the other tile's products
 //   13        walks the CTA's share and publishes its segments, ahead of the rest
 //
-// A causal prompt of 8191 tokens, 32 heads of 128 over 8 of the cache: 710 us,
-// 0.78 PFLOP/s of visible pairs (floor 335).  The products of 64 keys and 128
-// rows take 512 clocks by the pipe's rate, 572 when nothing else runs and 650 to
-// 720 from issue to end here; their exponentials another 512; a CTA ends such a
-// part every 1250 or so.  Without exponentials 14 % of the time goes, without
-// seven of eight products another 10 %, without operand stores another 16 %: the
-// hand-over between the roles is the rest, and no one of them bounds it.  An
-// item costs some 8 us of filling and emptying the pipeline, which short and
-// windowed prompts feel.
+// A causal prompt of 8191 tokens, 32 heads of 128 over 8 of the cache: 722 us by
+// itself, 0.76 PFLOP/s of visible pairs (floor 335), 750 back to back, where the
+// card's power counts.  Rows that go by their own scores and value scales cost
+// 2 to 3 % of it.  Measured before that: the products of 64 keys and 128 rows take
+// 512 clocks by the pipe's rate, 572 when nothing else runs and 650 to 720 from
+// issue to end here; their exponentials another 512; a CTA ends such a part every
+// 1250 or so.  Without exponentials 14 % of the time goes, without seven of eight
+// products another 10 %, without operand stores another 16 %: the hand-over between
+// the roles is the rest, and no one of them bounds it.  An item costs some 8 us of
+// filling and emptying the pipeline, which short and windowed prompts feel.
 //
-// Every wait is bounded: a timeout sets the status word and an abort flag,
-// all roles run out, and TMEM is released.
+// Every wait is bounded: a timeout sets the status word and an abort flag, all
+// roles run out, TMEM is released, and parts of cut items that the CTA has not come
+// to are counted, so that the next call finds the counters at zero.
 #include <algorithm>
 
 #include "kv_attend.cuh"
@@ -167,7 +169,7 @@ struct PromptShared {
   uint32_t u_begin, u_end, size;  // the share, and how many units one has
 };
 
-struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4], row maximum and sum
+struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4] in units of 2^m vref, row's m and sum
   float acc[128 * 128];
   float m[128], l[128];
   float vref;
