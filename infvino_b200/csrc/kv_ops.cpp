@@ -103,28 +103,41 @@ int guarded(ivc_kv *h, const char *call, F &&f) {
   return code;
 }
 
-// The stream's attention workspace, allocated and zeroed (in the stream's order) at its first use.
-// It goes by the stream's id, which tells streams apart that run at the same
-// time.  The handle's value does not: cudaStreamPerThread is one value for a
-// stream of every thread, and a destroyed stream's value may be given out again
-// while its work is pending.  A stream that is being captured does not tell its
-// id; it is the one that its name stood for at the last call outside a capture.
-void *workspace(ivc_kv *h, cudaStream_t st) {
+// A stream's id tells it apart from others that run at the same time.  The
+// handle's value does not: cudaStreamPerThread is one value for a stream of every
+// thread, and a destroyed stream's value may be given out again while its work is
+// pending.  A stream that is being captured does not tell its id; it is the one
+// that its name stood for at the last call outside a capture (~0: none yet).  The
+// legacy stream is never captured, and while others are it cannot be asked.
+struct StreamName {
+  unsigned long long &id;
+  bool captured;
+};
+StreamName stream_name(ivc_kv *h, cudaStream_t st) {
+  constexpr unsigned long long kLegacy = ~1ull;
+  if (st == cudaStreamLegacy) st = nullptr;
   const auto name = std::make_pair(st, st == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id());
-  unsigned long long &id = h->named.emplace(name, ~0ull).first->second;  // (~0: none yet)
+  unsigned long long &id = h->named.emplace(name, st ? ~0ull : kLegacy).first->second;
+  if (!st) return {id, false};
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   cuda(cudaStreamIsCapturing(st, &cap), "stream");
   const bool captured = cap != cudaStreamCaptureStatusNone;
   if (!captured) cuda(cudaStreamGetId(st, &id), "stream");
-  const auto it = h->workspace.find(id);
+  return {id, captured};
+}
+
+// The stream's attention workspace, allocated and zeroed (in the stream's order) at its first use.
+void *workspace(ivc_kv *h, cudaStream_t st) {
+  const StreamName name = stream_name(h, st);
+  const auto it = h->workspace.find(name.id);
   if (it != h->workspace.end()) return it->second;
-  need(!captured, "a stream's first call cannot be captured: call ivc_kv_reserve before");
+  need(!name.captured, "a stream's first call cannot be captured: call ivc_kv_reserve before");
   const size_t bytes = ivb::kv_workspace_bytes(h->sms);
   void *p = nullptr;
   cuda(cudaMalloc(&p, bytes), "workspace");
   try {
     cuda(cudaMemsetAsync(p, 0, ivb::kKvCounterBytes, st), "workspace");
-    h->workspace[id] = p;
+    h->workspace[name.id] = p;
   } catch (...) {
     (void)cudaFree(p);
     throw;
@@ -320,8 +333,9 @@ int ivc_kv_release(ivc_kv *h, void *stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   void *p = nullptr;
   const int r = guarded(h, "ivc_kv_release", [&] {
-    unsigned long long id = 0;
-    cuda(cudaStreamGetId(st, &id), "stream");
+    const StreamName name = stream_name(h, st);
+    need(!name.captured, "a stream that is being captured keeps its workspace");
+    const unsigned long long id = name.id;
     const auto it = h->workspace.find(id);
     if (it == h->workspace.end()) return;
     p = it->second;

@@ -230,3 +230,30 @@ def test_a_new_handle_keeps_errors_while_the_default_stream_is_busy():
         with pytest.raises(ivb.NativeError) as e:
             ops.synchronize(side.cuda_stream)
         assert e.value.status == 5 and "rotary table" in e.value.message
+
+
+@pytest.mark.parametrize("other", [0, 1])  # the legacy stream's two names
+def test_the_default_stream_while_another_is_captured(other):
+    """A call on the default stream beside a capture runs; release of the captured stream is refused and does no harm."""
+    c, d = Call(30, [1, 1], [900, 300]), Call(31, [50], [400])
+    wants = [c.expected(), d.expected()]
+    side = torch.cuda.Stream()
+    with ivb.KvOps(0) as ops:
+        c.run(ops, 0)
+        ops.reserve(side.cuda_stream)
+        torch.cuda.synchronize()
+        c.out.zero_()
+        torch.cuda.synchronize()
+        graph, errors = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(graph, stream=side):
+            d.run(ops, side.cuda_stream)
+            for what in (lambda: c.run(ops, other), lambda: ops.release(side.cuda_stream)):
+                try:
+                    what()
+                    errors.append(None)
+                except ivb.NativeError as e:
+                    errors.append(e.status)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert errors == [None, 1]
+        assert torch.equal(c.out, wants[0]) and torch.equal(d.out, wants[1])
