@@ -54,7 +54,7 @@ class Decoder:
         self.blocks = [{"qkv": weight(dim, (q_heads + 2 * kv_heads) * head_dim), "o": weight(q_heads * head_dim, dim),
                         "up": weight(dim, 4 * dim), "down": weight(2 * dim, dim)} for _ in range(layers)]
         self.head = weight(dim, vocab)
-        self.ops = ivb.KvOps(0)
+        self.ops, self.side = ivb.KvOps(0), torch.cuda.Stream()  # (captures are made on one stream: each has a workspace)
         pairs = head_dim // 2
         table = torch.empty((max_len, pairs, 2), device="cuda")
         self.ops.rope_table([10000.0 ** (-i / pairs) for i in range(pairs)], table, self.stream())
@@ -106,11 +106,10 @@ class Decoder:
         start = torch.tensor([length], dtype=torch.int32, device="cuda")
         lens, pos = start + 1, torch.full((3, 1), at, dtype=torch.int32, device="cuda")
         offsets = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
-        side = torch.cuda.Stream()
-        self.ops.reserve(side.cuda_stream)
+        self.ops.reserve(self.side.cuda_stream)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=side):
+        with torch.cuda.graph(graph, stream=self.side):
             out = self.forward(self.embed[token], pos, offsets, start, lens)
         tokens, seen = [], []
         for _ in range(steps):

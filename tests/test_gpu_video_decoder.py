@@ -92,3 +92,17 @@ def test_decoder_is_as_before_after_a_refusal():
         d.ops.synchronize(d.stream())
         again, same = d.generate(x, 5)
         assert again == tokens and torch.equal(same, logits)
+
+
+@pytest.mark.gpu
+def test_decoder_holds_one_capture_workspace():
+    """Generation after generation takes no more memory."""
+    d = load().Decoder(layers=1, max_len=64)
+    x = torch.randn((20, 576), generator=torch.Generator().manual_seed(3)).half().cuda()
+    d.generate(x, 2)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(6):
+        d.generate(x, 2)
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] < 60 << 20  # (a workspace is some 40 MB: five more were 200)
