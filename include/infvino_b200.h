@@ -263,8 +263,9 @@ typedef struct ivc_rows {
 
 /* One layer's cache, in the caller's memory.  Codes [pages][kv_heads]
  * [page_size][head_dim] in -127..127; a value is code * scale, one scale (a
- * power of two, as ivc_kv_append writes it) for each IVC_KV_BLOCK tokens of a
- * page and head: [pages][kv_heads][page_size / IVC_KV_BLOCK].  page_size is a
+ * power of two, as ivc_kv_append writes it; never negative, infinite or NaN where
+ * it is read) for each IVC_KV_BLOCK tokens of a page and head:
+ * [pages][kv_heads][page_size / IVC_KV_BLOCK].  page_size is a
  * multiple of IVC_KV_BLOCK, head_dim 64 or 128, k and v 16-byte aligned. */
 #define IVC_KV_BLOCK 16
 typedef struct ivc_kv_cache {
