@@ -145,6 +145,8 @@ class KvOps:
         self.close()
 
     def _fail(self, status: int) -> None:
+        if not self._h:
+            raise ValueError("the handle is closed")
         raise NativeError(status, (self._L.ivc_kv_last_error(self._h) or b"").decode())
 
     def _check(self, status: int) -> None:
@@ -201,6 +203,7 @@ class KvOps:
         name, tokens, d = _kind(k, "k"), k.shape[0], self.device
         sh = (tokens, cache.kv_heads, cache.head_dim)
         _need((rotary is None) == (pos is None), "rotary and pos go together")
+        _need((q is None) == (q_out is None), "q and q_out go together")
         rot = rotary.at(pos, tokens, d) if rotary is not None else None
         heads, qr, qo = 0, None, None
         if q is not None:

@@ -257,3 +257,17 @@ def test_the_default_stream_while_another_is_captured(other):
         torch.cuda.synchronize()
         assert errors == [None, 1]
         assert torch.equal(c.out, wants[0]) and torch.equal(d.out, wants[1])
+
+
+def test_closed_handles_and_lone_queries_are_refused():
+    c = Call(40, [1], [40])
+    k = torch.zeros((1, 2, 64), dtype=torch.float16, device="cuda")
+    rotary, pos = ivb.Rotary(torch.zeros((50, 32, 2), device="cuda")), ints([39])
+    ops = ivb.KvOps(0)
+    for lone in (dict(q=c.q), dict(q_out=c.out)):
+        with pytest.raises(ValueError, match="q_out"):
+            ops.append(c.cache, k, k, c.offsets, ints([39]), c.table, rotary=rotary, pos=pos, stream=stream(), **lone)
+    ops.close()
+    for call in (lambda: c.run(ops, stream()), lambda: ops.synchronize(stream()), lambda: ops.rope(k, k, rotary, pos, stream()), lambda: ops.release(stream())):
+        with pytest.raises(ValueError, match="closed"):
+            call()
