@@ -251,7 +251,7 @@ void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
  * from that stream, or eager calls on it. */
 typedef struct ivc_kv ivc_kv;
 
-typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1 } ivc_dtype;
+typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1, IVC_F32 = 2 /* logits only */ } ivc_dtype;
 
 /* [tokens][heads][head_dim] of the call's dtype; strides in elements, the last
  * dimension dense.  Any 2-byte alignment works; 16-byte alignment of data and
@@ -358,6 +358,82 @@ int ivc_kv_read(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, i
  * least the largest number of new tokens of one sequence. */
 int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int dtype, int q_heads, int max_new,
                   const ivc_rows *q, const ivc_rows *out, float scale, int window, int sinks, void *stream);
+
+/* Sequences that begin alike: group g is the sequences first[g] ..
+ * first[g + 1] - 1 of a call (first [count + 1], from 0 to batch, rising), and
+ * their first shared[g] tokens (whole pages; 0: none) are in the pages that the
+ * group's first sequence has for them.  Device memory, int32. */
+typedef struct ivc_kv_groups {
+  int count;
+  const int32_t *first, *shared;
+} ivc_kv_groups;
+/* ivc_kv_attend without a window, for groups of sequences with a common
+ * beginning (samples or questions over the same frames): its keys and values are
+ * read once for all of a group's queries.  Every sequence's new tokens come
+ * after it (lens[b] - new tokens >= shared[g]); a sequence's own pages for the
+ * first shared[g] tokens are not looked at.  A group whose sequences, or whose
+ * shared[g], do not fit is skipped, as is a sequence that ends inside the
+ * beginning.  scratch: at least tokens * q_heads * (head_dim + 2) floats, 16-byte
+ * aligned, of nobody else until the call has run. */
+int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, const ivc_kv_groups *groups,
+                         int dtype, int q_heads, int max_new, const ivc_rows *q, const ivc_rows *out, float scale,
+                         float *scratch, int64_t scratch_floats, void *stream);
+
+/* The next token of each row of logits [rows][vocab] (IVC_F16, IVC_BF16 or
+ * IVC_F32, rows row_stride elements apart, vocab at most 2^20). */
+typedef struct ivc_logits {
+  const void *data;
+  int dtype;
+  int64_t rows, vocab, row_stride;
+} ivc_logits;
+/* For each row, device memory: a random number u in [0, 1), a temperature, and the
+ * filters; those that are NULL are off (temperature: 1). */
+typedef struct ivc_sampling {
+  const float *u, *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+} ivc_sampling;
+/* Token i has the weight w_i = e^((x_i - x_max) / temperature), and the tokens are
+ * ordered by their logits, equal ones by their numbers.  Kept are, one filter after
+ * the other, the first top_k (0 and below: all); of them the shortest beginning
+ * with at least top_p of their weight (1 and above, NaN: all); of them those with
+ * w_i >= min_p (0 and below, NaN: all); always the first.  tokens[row] is the least
+ * i for which the weights of the kept tokens up to i exceed u times the weight of
+ * all kept ones, probs[row] (NULL: not wanted) its share of that.  With a
+ * temperature that is not above 0 it is the first in order, with probability 1.
+ * A logit of NaN counts as -inf; where one is +inf, only those have a weight; a
+ * row of -inf alone gives token -1 with probability 0.  Sums are in 64 bits;
+ * weights below 2^-60 count as 0.  u is taken into [0, 1) (NaN: 0). */
+int ivc_kv_sample(ivc_kv *h, const ivc_logits *logits, const ivc_sampling *how, int32_t *tokens, float *probs,
+                  void *stream);
+
+/* A matrix [rows][width] of microscaled 4-bit numbers (the OCP format MXFP4),
+ * width a multiple of 32.  codes [rows][width / 2], the lower four bits first:
+ * sign, two bits of exponent, one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6).
+ * Scales are powers of two, 2^(e - 127), for each IVC_MX4_BLOCK values of a row
+ * (e = 255: NaN), laid out as the tensor cores read them: the byte e of block b
+ * of row r is scales[r / 128][b / 4][r % 32][r % 128 / 32][b % 4], of
+ * [ceil(rows / 128)][ceil(width / 128)][32][4][4]; bytes without a row or block
+ * are 0.  Device memory; both 16-byte aligned. */
+#define IVC_MX4_BLOCK 32
+typedef struct ivc_mx4 {
+  uint8_t *codes, *scales;
+  int64_t rows, width;
+} ivc_mx4;
+/* m = x [rows][width] (IVC_F16 or IVC_BF16, rows x_stride elements apart), its
+ * first `rows` rows: e - 127 is the exponent of a block's largest magnitude less 2
+ * (at least -127), and codes are x 2^(127 - e), rounded to the nearest, ties to
+ * even, at most 6.  NaN is held as 0, an infinity as the largest code of its sign;
+ * neither takes part in e. */
+int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *m,
+                        void *stream);
+/* out = the values of m's first `rows` rows, rounded once (out_stride elements apart). */
+int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *out, int64_t out_stride, void *stream);
+/* out [rows][w->rows] = X W^T, summed in f32 and rounded once: W is w; X is the
+ * first `rows` rows of xq, which x [rows][width] (x_dtype) is quantised into first
+ * unless it is NULL.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
+int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
+                      const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream);
 
 #ifdef __cplusplus
 }

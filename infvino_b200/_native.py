@@ -80,6 +80,11 @@ SIGNATURES = {
     "ivc_kv_append": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "ivc_kv_read": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "ivc_kv_attend": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _i32, _i32, _vp]),
+    "ivc_kv_attend_shared": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, ctypes.c_float, _vp, _i64, _vp]),
+    "ivc_kv_sample": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "ivc_kv_mx4_quantize": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _vp]),
+    "ivc_kv_mx4_read": (_i32, [_vp, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "ivc_kv_mx4_linear": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _vp]),
 }
 
 class Preprocess(ctypes.Structure):
@@ -95,6 +100,10 @@ ROWS = struct.Struct("@Pqq")               # ivc_rows: data, token_stride, head_
 KV_CACHE = struct.Struct("@PPPPqiii0q")    # ivc_kv_cache: k, v, k_scale, v_scale, pages, page_size, kv_heads, head_dim
 KV_SEQS = struct.Struct("@iqPPPi0q")       # ivc_kv_seqs: batch, tokens, offsets, at, pages, pages_per_seq
 ROTARY = struct.Struct("@PqiiiPqP")        # ivc_rotary: table, positions, pairs, axes, interleaved, pos, pos_stride, axis_of
+KV_GROUPS = struct.Struct("@iPP")          # ivc_kv_groups: count, first, shared
+LOGITS = struct.Struct("@Piqqq")           # ivc_logits: data, dtype, rows, vocab, row_stride
+SAMPLING = struct.Struct("@PPPPP")         # ivc_sampling: u, temperature, top_k, top_p, min_p
+MX4 = struct.Struct("@PPqq")               # ivc_mx4: codes, scales, rows, width
 
 
 _lib = None

@@ -1,0 +1,40 @@
+// Host-visible declarations of the kernels for matrices of microscaled 4-bit numbers.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace ivb {
+
+constexpr int kMx4Block = 32;  // values that share a scale
+
+// codes [rows][width / 2], the lower four bits first; scale bytes
+// [ceil(rows / 128)][ceil(width / 128)][32][4][4] (mx4_scale_at).
+struct Mx4 {
+  uint8_t *codes, *scales;
+  long long rows, width;
+};
+
+// Where the scale byte of block b of row r is; `chunks` = ceil(width / 128).
+__host__ __device__ inline long long mx4_scale_at(long long r, long long b, long long chunks) {
+  return ((r >> 7) * chunks + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
+}
+
+cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long long stride, const Mx4 &m,
+                                cudaStream_t st);
+cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st);
+struct Mx4Linear {
+  Mx4 x, w;         // x.rows: the rows that are used
+  void *out;
+  long long stride;
+  bool bf16;
+  bool fresh;       // x has just been quantised by a launch that waited for what came before it
+  void *workspace;
+  int *status;
+  int sms;
+};
+size_t mx4_workspace_bytes(int sms);
+// (why: what was wrong, when the launch could not be described)
+cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st);
+
+}  // namespace ivb

@@ -14,6 +14,8 @@
 #include "../../include/infvino_b200.h"
 #include "kernels/common.cuh"
 #include "kernels/kv.cuh"
+#include "kernels/mx4.cuh"
+#include "kernels/sample.cuh"
 
 struct ivc_kv {
   int device = 0, sms = 0;
@@ -132,7 +134,7 @@ void *workspace(ivc_kv *h, cudaStream_t st) {
   const auto it = h->workspace.find(name.id);
   if (it != h->workspace.end()) return it->second;
   need(!name.captured, "a stream's first call cannot be captured: call ivc_kv_reserve before");
-  const size_t bytes = ivb::kv_workspace_bytes(h->sms);
+  const size_t bytes = std::max(ivb::kv_workspace_bytes(h->sms), ivb::mx4_workspace_bytes(h->sms));
   void *p = nullptr;
   cuda(cudaMalloc(&p, bytes), "workspace");
   try {
@@ -226,6 +228,47 @@ ivb::KvSeqs check_seqs(const ivc_kv_seqs *s) {
   need(aligned(s->offsets, 4) && aligned(s->at, 4) && aligned(s->pages, 4), "offsets, at and pages are int32");
   need(s->pages_per_seq >= 1 || s->batch == 0, "pages_per_seq is at least 1");
   return ivb::KvSeqs{s->batch, s->tokens, s->offsets, s->at, s->pages, s->pages_per_seq};
+}
+
+ivb::KvAttend attention(const ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int q_heads, int max_new,
+                        const ivc_rows *q, const ivc_rows *out, float scale, int window, int sinks) {
+  ivb::KvAttend a{};
+  a.cache = check_cache(cache);
+  a.seqs = check_seqs(seqs);
+  need(q_heads > 0 && q_heads <= 65536 && q_heads % a.cache.heads == 0, "q_heads is a multiple of kv_heads");
+  need(max_new >= 0 && (max_new > 0 || a.seqs.tokens == 0), "max_new is at least 1");
+  need(window >= 0 && sinks >= 0, "window and sinks are not negative");
+  a.q = rows(q, "q is null", a.seqs.tokens, q_heads);
+  a.out = out_rows(out, "out is null", a.seqs.tokens, q_heads, a.cache.dim);
+  a.q_heads = q_heads;
+  a.group = q_heads / a.cache.heads;
+  a.max_new = max_new;
+  a.scale = scale;
+  a.window = window;
+  a.sinks = sinks;
+  a.status = h->status;
+  a.probe = h->probe;
+  need((int64_t)max_new * a.group < (1LL << 30), "max_new * q_heads / kv_heads out of range");
+  a.by_group = ivb::make_fastdiv((uint32_t)a.group);
+  a.by_page = ivb::make_fastdiv((uint32_t)a.cache.page);
+  return a;
+}
+
+ivb::Mx4 check_mx4(const ivc_mx4 *m) {
+  need(m != nullptr, "no 4-bit matrix");
+  need(m->rows >= 0 && m->rows <= 0x7fffffffLL, "rows of a 4-bit matrix: at most 2^31 - 1");
+  need(m->width > 0 && m->width % IVC_MX4_BLOCK == 0 && m->width <= (1 << 24), "width of a 4-bit matrix: a multiple of IVC_MX4_BLOCK");
+  need(m->rows == 0 || (m->codes && m->scales), "a 4-bit matrix has a null pointer");
+  need(aligned(m->codes, 16) && aligned(m->scales, 16), "codes and scales are 16-byte aligned");
+  return ivb::Mx4{m->codes, m->scales, m->rows, m->width};
+}
+
+void check_matrix(int dtype, const void *p, int64_t rows, int64_t width, int64_t stride, bool written) {
+  check_dtype(dtype);
+  need(rows >= 0 && rows <= kMaxTokens, "rows out of range");
+  need(p != nullptr || rows == 0, "a matrix is null");
+  need(aligned(p, 2), "rows are 2-byte aligned");
+  need(!written || rows <= 1 || stride >= width || stride <= -width, "rows that are written overlap");
 }
 
 }  // namespace
@@ -430,28 +473,103 @@ int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs,
                   const ivc_rows *q, const ivc_rows *out, float scale, int window, int sinks, void *stream) {
   return guarded(h, "ivc_kv_attend", [&] {
     check_dtype(dtype);
-    ivb::KvAttend a{};
-    a.cache = check_cache(cache);
-    a.seqs = check_seqs(seqs);
-    need(q_heads > 0 && q_heads <= 65536 && q_heads % a.cache.heads == 0, "q_heads is a multiple of kv_heads");
-    need(max_new >= 0 && (max_new > 0 || a.seqs.tokens == 0), "max_new is at least 1");
-    need(window >= 0 && sinks >= 0, "window and sinks are not negative");
-    a.q = rows(q, "q is null", a.seqs.tokens, q_heads);
-    a.out = out_rows(out, "out is null", a.seqs.tokens, q_heads, a.cache.dim);
-    a.q_heads = q_heads;
-    a.group = q_heads / a.cache.heads;
-    a.max_new = max_new;
-    a.scale = scale;
-    a.window = window;
-    a.sinks = sinks;
-    a.status = h->status;
-    a.probe = h->probe;
-    need((int64_t)max_new * a.group < (1LL << 30), "max_new * q_heads / kv_heads out of range");
-    a.by_group = ivb::make_fastdiv((uint32_t)a.group);
-    a.by_page = ivb::make_fastdiv((uint32_t)a.cache.page);
+    const ivb::KvAttend a = attention(h, cache, seqs, q_heads, max_new, q, out, scale, window, sinks);
     if (a.seqs.tokens == 0) return;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
+  });
+}
+
+int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, const ivc_kv_groups *groups,
+                         int dtype, int q_heads, int max_new, const ivc_rows *q, const ivc_rows *out, float scale,
+                         float *scratch, int64_t scratch_floats, void *stream) {
+  return guarded(h, "ivc_kv_attend_shared", [&] {
+    check_dtype(dtype);
+    ivb::KvAttend a = attention(h, cache, seqs, q_heads, max_new, q, out, scale, 0, 0);
+    need(groups != nullptr, "no groups");
+    need(groups->count >= 0 && groups->count <= a.seqs.batch, "groups: at most one for each sequence");
+    need(groups->count > 0 || a.seqs.batch == 0, "sequences without a group");
+    need(groups->count == 0 || (groups->first && groups->shared), "the groups have a null pointer");
+    need(aligned(groups->first, 4) && aligned(groups->shared, 4), "first and shared are int32");
+    need(aligned(scratch, 16), "scratch is 16-byte aligned");
+    need(a.seqs.tokens == 0 || (scratch && scratch_floats >= a.seqs.tokens * q_heads * (a.cache.dim + 2)),
+         "scratch: at least tokens * q_heads * (head_dim + 2) floats");
+    if (a.seqs.tokens == 0) return;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
+  });
+}
+
+int ivc_kv_sample(ivc_kv *h, const ivc_logits *logits, const ivc_sampling *how, int32_t *tokens, float *probs,
+                  void *stream) {
+  return guarded(h, "ivc_kv_sample", [&] {
+    need(logits && how, "null pointer");
+    need(logits->dtype == IVC_F16 || logits->dtype == IVC_BF16 || logits->dtype == IVC_F32, "logits are IVC_F16, IVC_BF16 or IVC_F32");
+    need(logits->rows >= 0 && logits->rows <= (1 << 24), "rows out of range");
+    need(logits->vocab >= 1 && logits->vocab <= ivb::kSampleMaxVocab, "vocab: 1 to 2^20");
+    if (logits->rows == 0) return;
+    need(logits->data && how->u && tokens, "null pointer");
+    need(aligned(logits->data, logits->dtype == IVC_F32 ? 4 : 2), "logits are aligned to their type");
+    need(aligned(how->u, 4) && aligned(how->temperature, 4) && aligned(how->top_k, 4) && aligned(how->top_p, 4) &&
+             aligned(how->min_p, 4) && aligned(tokens, 4) && aligned(probs, 4),
+         "the rows' numbers are 4-byte aligned");
+    ivb::Sample s{};
+    s.x = logits->data;
+    s.rows = logits->rows;
+    s.stride = logits->row_stride;
+    s.vocab = (int)logits->vocab;
+    s.dtype = logits->dtype;
+    s.u = how->u, s.temperature = how->temperature, s.top_k = how->top_k, s.top_p = how->top_p, s.min_p = how->min_p;
+    s.tokens = tokens;
+    s.probs = probs;
+    cuda(ivb::launch_sample(s, h->sms, static_cast<cudaStream_t>(stream)), "launch");
+  });
+}
+
+int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *m,
+                        void *stream) {
+  return guarded(h, "ivc_kv_mx4_quantize", [&] {
+    const ivb::Mx4 q = check_mx4(m);
+    check_matrix(dtype, x, rows, q.width, x_stride, false);
+    need(rows <= q.rows, "the 4-bit matrix has fewer rows");
+    if (rows == 0) return;
+    cuda(ivb::launch_mx4_quantize(dtype == IVC_BF16, x, rows, x_stride, q, static_cast<cudaStream_t>(stream)), "launch");
+  });
+}
+
+int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *out, int64_t out_stride, void *stream) {
+  return guarded(h, "ivc_kv_mx4_read", [&] {
+    const ivb::Mx4 q = check_mx4(m);
+    check_matrix(dtype, out, rows, q.width, out_stride, true);
+    need(rows <= q.rows, "the 4-bit matrix has fewer rows");
+    if (rows == 0) return;
+    cuda(ivb::launch_mx4_read(dtype == IVC_BF16, q, rows, out, out_stride, static_cast<cudaStream_t>(stream)), "launch");
+  });
+}
+
+int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
+                      const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream) {
+  return guarded(h, "ivc_kv_mx4_linear", [&] {
+    ivb::Mx4Linear a{};
+    a.x = check_mx4(xq);
+    a.w = check_mx4(w);
+    need(a.x.width == a.w.width, "the matrices differ in width");
+    need(a.w.rows <= (1 << 26), "rows of the weights out of range");
+    check_matrix(out_dtype, out, rows, a.w.rows, out_stride, true);
+    if (x) check_matrix(x_dtype, x, rows, a.x.width, x_stride, false);
+    need(rows <= a.x.rows, "the 4-bit matrix has fewer rows");
+    if (rows == 0 || a.w.rows == 0) return;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    a.workspace = workspace(h, st);
+    if (x) cuda(ivb::launch_mx4_quantize(x_dtype == IVC_BF16, x, rows, x_stride, a.x, st), "launch");
+    a.x.rows = rows;
+    a.out = out;
+    a.stride = out_stride;
+    a.bf16 = out_dtype == IVC_BF16;
+    a.fresh = x != nullptr;
+    a.status = h->status;
+    a.sms = h->sms;
+    cuda(ivb::launch_mx4_linear(a, st), "launch");
   });
 }
 

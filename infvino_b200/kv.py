@@ -1,5 +1,6 @@
 """Language-model operators over device tensors: rotary positions with several
-axes, a paged key/value cache held in 8 bits, and the attention over it
+axes, a paged key/value cache held in 8 bits, the attention over it, products
+with matrices in microscaled 4-bit numbers, and the choice of the next token
 (include/infvino_b200.h, ivc_kv_*), for a decoder behind a `PlanModel`.
 
 Tensors are anything with torch's `data_ptr()`, `shape`, `stride()`, `dim()`,
@@ -15,10 +16,12 @@ from typing import Optional, Sequence
 from . import _native
 from ._native import NativeError, lib
 
-__all__ = ["KvOps", "KvCache", "Rotary"]
+__all__ = ["KvOps", "KvCache", "Rotary", "Mx4"]
 
 BLOCK = 16  # tokens that share a scale (IVC_KV_BLOCK)
+GROUP = 32  # values of a 4-bit matrix that share a scale (IVC_MX4_BLOCK)
 _DTYPES = {"float16": 0, "bfloat16": 1}
+_LOGITS = {**_DTYPES, "float32": 2}
 _names: dict = {}  # dtype object -> its name
 
 
@@ -113,6 +116,42 @@ class KvCache:
         self._c = _native.KV_CACHE.pack(*ptrs, self.pages, self.page_size, self.kv_heads, self.head_dim)
 
 
+def _matrix(t, name: str, device: int, shape=None):
+    """Address, row stride and dtype of a float16 or bfloat16 [rows, width] tensor whose last dimension is dense."""
+    kind = _name(t)
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a tensor on CUDA device {device}")
+    if kind not in _DTYPES or t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name}: expected float16 or bfloat16 {'[rows, width]' if shape is None else tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    st = t.stride()
+    if st[1] != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name}: the last dimension must be dense")
+    return t.data_ptr(), st[0], _DTYPES[kind]
+
+
+class Mx4:
+    """A matrix of microscaled 4-bit numbers (OCP MXFP4) over the caller's tensors:
+    codes uint8 [rows, width / 2], scales uint8 [ceil(rows / 128),
+    ceil(width / 128), 32, 4, 4] (the exponent byte of block b of row r is at
+    [r // 128, b // 4, r % 32, r % 128 // 32, b % 4])."""
+
+    def __init__(self, codes, scales):
+        c, s = _dense(codes, "codes", "uint8", 2), _dense(scales, "scales", "uint8", 5)
+        self.rows, half = codes.shape
+        self.width = 2 * half
+        _need(half % (GROUP // 2) == 0 and half > 0, "codes: expected [rows, width / 2], width a multiple of 32")
+        want = self.scales_shape(self.rows, self.width)
+        _need(tuple(scales.shape) == want, f"scales: expected shape {want}, got {tuple(scales.shape)}")
+        self.device = codes.get_device()
+        _need(scales.get_device() == self.device, "codes and scales are on different devices")
+        self._keep = (codes, scales)
+        self._m = _native.MX4.pack(c, s, self.rows, self.width)
+
+    @staticmethod
+    def scales_shape(rows: int, width: int):
+        return (-(-rows // 128), -(-width // 128), 32, 4, 4)
+
+
 class KvOps:
     """A handle of the operators on one CUDA device."""
 
@@ -124,6 +163,7 @@ class KvOps:
             raise NativeError(st, (L.ivc_kv_last_error(None) or b"").decode())
         self._h, self._L = h, L
         self._rope, self._append, self._read, self._attend = L.ivc_kv_rope, L.ivc_kv_append, L.ivc_kv_read, L.ivc_kv_attend
+        self._shared, self._sample, self._linear = L.ivc_kv_attend_shared, L.ivc_kv_sample, L.ivc_kv_mx4_linear
         self.device = device
 
     def close(self) -> None:
@@ -240,5 +280,94 @@ class KvOps:
         st = self._attend(self._h, cache._c, self._seqs(tokens, cache, offsets, lens, pages), _DTYPES[name], heads, max_new,
                           _rows(q, "q", name, sh, d), _rows(out, "out", name, sh, d), dim ** -0.5 if scale is None else scale, window, sinks,
                           stream)
+        if st:
+            self._fail(st)
+
+    def attend_shared(self, cache: KvCache, q, out, offsets, lens, pages, groups, shared, scratch, max_new: int, scale: Optional[float] = None,
+                      stream: int = 0) -> None:
+        """`attend` for groups of sequences that begin alike: the sequences
+        groups[g] .. groups[g + 1] - 1 (groups int32 [count + 1], from 0 to batch)
+        have their first shared[g] tokens (int32 [count], whole pages) in common, in
+        the pages of the group's first sequence, and those are read once for all of
+        the group.  scratch: float32, at least tokens * q_heads * (head_dim + 2)."""
+        name, sh, d = _kind(q, "q"), q.shape, self.device
+        tokens, heads, dim = sh
+        if dim != cache.head_dim:
+            raise ValueError(f"q: expected head_dim {cache.head_dim}, got {dim}")
+        f, n, w = _dense(groups, "groups", "int32", 1, d), _dense(shared, "shared", "int32", 1, d), _dense(scratch, "scratch", "float32", 1, d)
+        count = shared.shape[0]
+        _need(groups.shape[0] == count + 1, "groups: one entry more than shared")
+        st = self._shared(self._h, cache._c, self._seqs(tokens, cache, offsets, lens, pages), _native.KV_GROUPS.pack(count, f, n), _DTYPES[name],
+                          heads, max_new, _rows(q, "q", name, sh, d), _rows(out, "out", name, sh, d), dim ** -0.5 if scale is None else scale, w,
+                          scratch.shape[0], stream)
+        if st:
+            self._fail(st)
+
+    def sample(self, logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int = 0) -> None:
+        """tokens int32 [rows] (and probs float32 [rows]: their probabilities) from
+        logits [rows, vocab] (float16, bfloat16 or float32) by the random numbers u
+        float32 [rows]: weights e^((x - max) / temperature); of the tokens in falling
+        order the first top_k (int32; 0: all), of them the fewest with top_p of the
+        weight, of them those with at least min_p of the largest; of these the least
+        i whose weights up to i exceed u times all.  The filters are tensors [rows]
+        or None; a temperature of 0 takes the first of the largest logits; a row of
+        -inf gives -1."""
+        d = self.device
+        if logits.get_device() != d:
+            raise ValueError(f"logits: expected a tensor on CUDA device {d}")
+        kind = _name(logits)
+        if kind not in _LOGITS or logits.dim() != 2:
+            raise ValueError(f"logits: expected float16, bfloat16 or float32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+        (rows, vocab), st = logits.shape, logits.stride()
+        _need(st[1] == 1 or vocab == 1, "logits: the last dimension must be dense")
+
+        def each(t, name, dtype):
+            if t is None:
+                return 0
+            p = _dense(t, name, dtype, 1, d)
+            _need(t.shape[0] == rows, f"{name}: expected {rows} entries, got {t.shape[0]}")
+            return p
+
+        how = _native.SAMPLING.pack(each(u, "u", "float32"), each(temperature, "temperature", "float32"), each(top_k, "top_k", "int32"),
+                                    each(top_p, "top_p", "float32"), each(min_p, "min_p", "float32"))
+        st = self._sample(self._h, _native.LOGITS.pack(logits.data_ptr(), _LOGITS[kind], rows, vocab, st[0]), how,
+                          each(tokens, "tokens", "int32"), each(probs, "probs", "float32"), stream)
+        if st:
+            self._fail(st)
+
+    def _mx4(self, m: Mx4, name: str) -> bytes:
+        if m.device != self.device:
+            raise ValueError(f"{name}: expected tensors on CUDA device {self.device}")
+        return m._m
+
+    def mx4_quantize(self, x, m: Mx4, stream: int = 0) -> None:
+        """The first rows of m = x [rows, width] (float16 or bfloat16), width m's, rows at most m's."""
+        p, st, dt = _matrix(x, "x", self.device)
+        _need(x.shape[1] == m.width and x.shape[0] <= m.rows, f"x: expected width {m.width} and at most {m.rows} rows, got {tuple(x.shape)}")
+        self._check(self._L.ivc_kv_mx4_quantize(self._h, dt, p, x.shape[0], st, self._mx4(m, "m"), stream))
+
+    def mx4_read(self, m: Mx4, out, stream: int = 0) -> None:
+        """out [rows, width] (float16 or bfloat16) = the values of m's first rows."""
+        p, st, dt = _matrix(out, "out", self.device)
+        _need(out.shape[1] == m.width and out.shape[0] <= m.rows, f"out: expected width {m.width} and at most {m.rows} rows, got {tuple(out.shape)}")
+        self._check(self._L.ivc_kv_mx4_read(self._h, self._mx4(m, "m"), out.shape[0], dt, p, st, stream))
+
+    def mx4_linear(self, x, w: Mx4, out, scratch: Optional[Mx4] = None, stream: int = 0) -> None:
+        """out [rows, w.rows] = x w^T with both in 4 bits: x is an `Mx4`, or a
+        float16 / bfloat16 tensor [rows, width] that is first quantised into
+        `scratch`.  Sums are in 32 bits."""
+        o, ost, odt = _matrix(out, "out", self.device)
+        rows = out.shape[0]
+        if isinstance(x, Mx4):
+            p, st, dt, xq = None, 0, 0, x
+            _need(scratch is None, "scratch: x is quantised already")
+        else:
+            p, st, dt = _matrix(x, "x", self.device)
+            _need(scratch is not None, "scratch: an Mx4 that x is quantised into")
+            _need(tuple(x.shape) == (rows, w.width), f"x: expected {(rows, w.width)}, got {tuple(x.shape)}")
+            xq = scratch
+        _need(xq.width == w.width and xq.rows >= rows, f"x: expected width {w.width} and at least {rows} rows, got {(xq.rows, xq.width)}")
+        _need(out.shape[1] == w.rows, f"out: expected {w.rows} columns, got {out.shape[1]}")
+        st = self._linear(self._h, dt, p, rows, st, self._mx4(xq, "x"), self._mx4(w, "w"), odt, o, ost, stream)
         if st:
             self._fail(st)

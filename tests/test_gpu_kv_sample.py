@@ -1,0 +1,257 @@
+"""KvOps.sample against the definition in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import infvino_b200 as ivb
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+INF, NAN = math.inf, math.nan
+
+
+@pytest.fixture(scope="module")
+def ops():
+    with ivb.KvOps(0) as o:
+        yield o
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def choose(x, u, t=1.0, k=0, p=1.0, least=0.0):
+    """The token of one row of float64 logits, its probability, and how near u is to a border of it."""
+    x = np.where(np.isnan(x), -INF, x) + 0.0
+    top = x.max()
+    if top == -INF:
+        return -1, 0.0, 1.0
+    best = int(np.argmax(x))
+    if not t > 0:
+        return best, 1.0, 1.0
+    with np.errstate(all="ignore"):
+        w = np.where(x == top, 1.0, np.where(x == -INF, 0.0, np.exp((x - top) / t)))
+    w = np.nan_to_num(w, nan=0.0)
+    w[w <= 2.0 ** -60] = 0
+    order = np.lexsort((np.arange(len(x)), -x))
+    if k > 0:
+        order = order[:k]
+    if p < 1:
+        c = np.cumsum(w[order])
+        order = order[:int(np.argmax(c >= max(p, 0.0) * c[-1])) + 1]
+    if least > 0:
+        order = order[(w[order] >= least) | (x[order] == top)]
+    keep = np.zeros(len(x), bool)
+    keep[order] = True
+    w = w * keep
+    c = np.cumsum(w)
+    u = min(max(u, 0.0), 1 - 2.0 ** -24) if u == u else 0.0
+    i = int(np.argmax(c > u * c[-1]))
+    return i, w[i] / c[-1], min(c[i] - u * c[-1], u * c[-1] - (c[i] - w[i])) / c[-1]
+
+
+def check(ops, x, u, temperature=None, top_k=None, top_p=None, min_p=None, probs=True):
+    rows = x.shape[0]
+    dev = {n: None if v is None else torch.tensor(v, dtype=torch.int32 if n == "k" else torch.float32, device="cuda")
+           for n, v in (("u", u), ("t", temperature), ("k", top_k), ("p", top_p), ("m", min_p))}
+    tokens = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    pr = torch.full((rows,), NAN, device="cuda") if probs else None
+    ops.sample(x, dev["u"], tokens, pr, temperature=dev["t"], top_k=dev["k"], top_p=dev["p"], min_p=dev["m"], stream=stream())
+    ops.synchronize(stream())
+    host, got, f = x.double().cpu().numpy(), tokens.tolist(), {n: None if v is None else v.tolist() for n, v in dev.items()}
+    for r in range(rows):
+        want, share, margin = choose(host[r], f["u"][r], *(d if f[n] is None else f[n][r] for n, d in (("t", 1.0), ("k", 0), ("p", 1.0), ("m", 0.0))))
+        # (sums of 2^20 weights in 64 bits are good to some 2^-33 whatever their order: nearer to a border than that nothing is asked)
+        assert got[r] == want or abs(margin) < 2.0 ** -33, (r, got[r], want, margin)
+        if probs and got[r] == want:
+            assert abs(float(pr[r]) - share) <= 2.0 ** -23 * share, (r, float(pr[r]), share)  # one rounding to f32, and 64-bit sums
+    return got
+
+
+def logits(rows, vocab, dtype, seed=0, spread=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, vocab), generator=g, device="cuda").mul_(spread)
+    some = torch.randint(vocab, (rows, 12), generator=g, device="cuda")
+    return x.scatter_add_(1, some, torch.rand((rows, 12), generator=g, device="cuda") * 9).to(TYPES[dtype])
+
+
+def uniform(rows, seed):
+    return np.random.default_rng(seed).random(rows, dtype=np.float32)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 33), (5, 1000), (1, 32003), (300, 777), (40, 50021), (2, 262144), (1, 1 << 20)])
+@pytest.mark.parametrize("filters", ["none", "temperature", "top_k", "top_p", "min_p", "all"])
+def test_sample(ops, dtype, rows, vocab, filters):
+    r = np.random.default_rng(rows + vocab)
+    f = {}
+    if filters in ("temperature", "all"):
+        f["temperature"] = r.choice([0.0, 0.3, 0.7, 1.0, 1.9], rows)
+    if filters in ("top_k", "all"):
+        f["top_k"] = r.choice([-1, 0, 1, 2, 17, 50, 1000, 1025, 3000, 1 << 30], rows)
+    if filters in ("top_p", "all"):
+        f["top_p"] = r.choice([0.0, 0.1, 0.5, 0.9, 0.99, 1.0], rows)
+    if filters in ("min_p", "all"):
+        f["min_p"] = r.choice([0.0, 0.001, 0.05, 1.0], rows)
+    check(ops, logits(rows, vocab, dtype, vocab), uniform(rows, vocab), **f)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [40, 5000, 70000])
+def test_ties(ops, dtype, vocab):
+    """Few distinct logits: cuts lie inside runs of equal ones, which go by their numbers."""
+    rows = 24
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randint(-2, 3, (rows, vocab), generator=g, device="cuda").to(TYPES[dtype])
+    x[3] = 1.5
+    x[4] = -0.0
+    x[4, ::2] = 0.0
+    r = np.random.default_rng(1)
+    u = uniform(rows, 5)
+    check(ops, x, u)
+    check(ops, x, u, top_k=r.integers(1, vocab, rows))
+    check(ops, x, u, top_p=r.random(rows))
+    check(ops, x, u, temperature=r.random(rows) + 0.5, top_k=r.integers(1, vocab, rows), top_p=r.random(rows), min_p=r.random(rows) * 0.5)
+    check(ops, x, u, temperature=[0.0] * rows)
+
+
+@pytest.mark.parametrize("vocab", [3000, 60000])
+def test_logits_that_one_bin_holds(ops, vocab):
+    """An outlier, or values on scales that differ by many powers of two, leave most logits in one bin, again and again."""
+    rows = 8
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn((rows, vocab), generator=g, device="cuda")
+    x[0] *= 1e-4
+    x[0, 77] = 30.0
+    x[1] = torch.exp2(-40.0 * torch.rand(vocab, generator=g, device="cuda"))
+    x[2] = -torch.exp2(-60.0 * torch.rand(vocab, generator=g, device="cuda"))
+    x[3] = 5.0 + 1e-6 * x[3]
+    x[4] *= 1e30
+    x[5] *= 1e-38
+    x[6, 5:] = x[6, 5]
+    t = [1000.0, 1.0, 0.5, 1e-6, 1e30, 1e-38, 1.0, INF]
+    u = uniform(rows, 9)
+    for k, p in ((None, None), (2000, None), (None, 0.6), (2500, 0.7), (5, 0.9)):
+        check(ops, x, u, temperature=t, top_k=None if k is None else [k] * rows, top_p=None if p is None else [p] * rows)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_masked_and_not_finite(ops, dtype):
+    vocab = 5003
+    x = logits(9, vocab, dtype, 3)
+    x[0] = -INF                       # nothing is allowed
+    x[1] = -INF
+    x[1, 4999] = -3.0                 # one token is
+    x[2, ::2] = -INF
+    x[3] = torch.finfo(x.dtype).min   # a mask of the type's lowest value
+    x[3, 100:110] = 1.0
+    x[4, 17] = NAN
+    x[4, 5:9] = NAN
+    x[5] = NAN
+    x[6, [30, 4000]] = INF
+    x[7] = INF
+    x[8] = torch.finfo(x.dtype).min
+    u = uniform(9, 1)
+    got = check(ops, x, u)
+    assert got[0] == -1 and got[1] == 4999 and got[5] == -1 and got[6] in (30, 4000)
+    check(ops, x, u, top_k=[20] * 9, top_p=[0.8] * 9, min_p=[0.01] * 9)
+    check(ops, x, u, top_k=[3000] * 9, top_p=[0.99] * 9)
+    check(ops, x, u, temperature=[0.0] * 9)
+    check(ops, x, u, temperature=[INF] * 9)
+    check(ops, x, u, temperature=[NAN] * 9, top_p=[NAN] * 9, min_p=[NAN] * 9)
+    check(ops, x, u, top_p=[NAN] * 9, min_p=[NAN] * 9, top_k=[-5] * 9)
+
+
+def test_borders_of_u(ops):
+    x = torch.zeros((7, 1000), device="cuda")
+    got = check(ops, x, [0.0, 1 - 2.0 ** -24, 0.5, 0.25, -3.0, 7.0, NAN])
+    assert got == [0, 999, 500, 250, 0, 999, 0]  # equal weights: the first with more than u of them
+    assert check(ops, x, [0.999, 0.0, 0.5, 0.1, 0.1, 0.1, 0.1], top_k=[10, 1, 2, 3, 4, 5, 6]) == [9, 0, 1, 0, 0, 0, 0]
+
+
+def test_layouts_and_outputs(ops):
+    """Rows of a wider buffer, odd strides and addresses; nothing else is written; probabilities may be left out."""
+    base = logits(6, 4001, "f16", 11)
+    u = uniform(6, 2)
+    wide = torch.zeros((6, 5003), dtype=torch.float16, device="cuda")
+    for at in (0, 1, 8):
+        wide[:, at:at + 4001] = base
+        check(ops, wide[:, at:at + 4001], u, top_p=[0.9] * 6, probs=at != 1)
+    flipped = torch.empty_like(base)
+    flipped[:] = base.flip(0)
+    one = base[2:3].expand(6, -1)  # (the same row six times)
+    check(ops, one, u)
+    tokens = torch.full((10,), -7, dtype=torch.int32, device="cuda")
+    ops.sample(base, torch.tensor(u, device="cuda"), tokens[2:8], stream=stream())
+    assert tokens[:2].tolist() == [-7, -7] and tokens[8:].tolist() == [-7, -7] and (tokens[2:8] >= 0).all()
+    ops.sample(base[:0], torch.empty(0, device="cuda"), tokens[:0], stream=stream())  # no rows
+
+
+def test_a_row_does_not_depend_on_how_many_there_are(ops):
+    x, u = logits(400, 20011, "bf16", 8), torch.tensor(uniform(400, 8), device="cuda")
+    many, one = torch.empty(400, dtype=torch.int32, device="cuda"), torch.empty(400, dtype=torch.int32, device="cuda")
+    p = torch.full((400,), 0.95, device="cuda")
+    ops.sample(x, u, many, top_p=p, stream=stream())
+    for r in range(0, 400, 13):
+        ops.sample(x[r:r + 1], u[r:r + 1], one[r:r + 1], top_p=p[r:r + 1], stream=stream())
+    assert torch.equal(many[::13], one[::13])
+
+
+def test_same_bits_again(ops):
+    x, u = logits(64, 131072, "f32", 5), torch.tensor(uniform(64, 5), device="cuda")
+    k = torch.full((64,), 2000, dtype=torch.int32, device="cuda")
+    p = torch.full((64,), 0.97, device="cuda")
+    seen = []
+    for _ in range(4):
+        t, q = torch.empty(64, dtype=torch.int32, device="cuda"), torch.empty(64, device="cuda")
+        ops.sample(x, u, t, q, top_k=k, top_p=p, stream=stream())
+        seen.append((t, q))
+    assert all(torch.equal(a, seen[0][0]) and torch.equal(b, seen[0][1]) for a, b in seen)
+
+
+def test_graph_and_streams(ops):
+    """Captured once (no call before it is needed) and replayed with other logits and numbers, beside calls on another stream."""
+    x, u, t = logits(3, 9001, "f16", 1), torch.tensor(uniform(3, 1), device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    temp = torch.full((3,), 0.8, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.sample(x, u, t, temperature=temp, top_p=temp, stream=side.cuda_stream)
+    for seed in range(3):
+        x.copy_(logits(3, 9001, "f16", seed + 10))
+        u.copy_(torch.tensor(uniform(3, seed + 10)))
+        other = torch.empty(3, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        graph.replay()
+        ops.sample(x, u, other, temperature=temp, top_p=temp, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(t, other)
+        want = [choose(x[r].double().cpu().numpy(), float(u[r]), float(temp[r]), 0, float(temp[r]))[0] for r in range(3)]
+        assert t.tolist() == want
+
+
+def test_how_often(ops):
+    """Tokens come as often as their probabilities say."""
+    rows = 20000
+    x = torch.tensor([0.0, 1.0, -1.0, 2.0, -INF, 0.5], device="cuda").expand(rows, -1)
+    u = torch.rand(rows, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    t = torch.empty(rows, dtype=torch.int32, device="cuda")
+    ops.sample(x, u, t, stream=stream())
+    p = torch.softmax(x[0].double(), 0).cpu()
+    got = torch.bincount(t.long(), minlength=6).double().cpu() / rows
+    assert got[4] == 0 and ((got - p).abs() <= 5 * (p * (1 - p) / rows).sqrt()).all()  # five standard deviations
+
+
+def test_refusals(ops):
+    x, u, t = logits(4, 100, "f16"), torch.rand(4, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda")
+    for bad in (dict(logits=x.double()), dict(logits=x[0]), dict(logits=x.cpu()), dict(logits=x.t()[:4]), dict(u=u[:3]), dict(u=u.double()),
+                dict(u=u.cpu()), dict(tokens=t.long()), dict(tokens=t[:3]), dict(probs=u[:2]), dict(top_k=u), dict(top_p=t), dict(min_p=u[::2]),
+                dict(temperature=u.half()), dict(logits=torch.empty((4, 0), device="cuda"))):
+        args = {"logits": x, "u": u, "tokens": t, **bad}
+        with pytest.raises((ValueError, ivb.NativeError)):
+            ops.sample(stream=stream(), **args)
+    with pytest.raises(ivb.NativeError):
+        ops.sample(torch.empty((1, (1 << 20) + 1), dtype=torch.float16, device="cuda"), u[:1], t[:1], stream=stream())
