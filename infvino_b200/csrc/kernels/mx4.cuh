@@ -34,7 +34,6 @@ struct Mx4Linear {
   int sms;
 };
 size_t mx4_workspace_bytes(int sms);
-// (why: what was wrong, when the launch could not be described)
 cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st);
 
 }  // namespace ivb

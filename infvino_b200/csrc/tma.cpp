@@ -60,4 +60,24 @@ bool encode_tiled_f16(CUtensorMap *map, int rank, const void *base, const uint64
   return true;
 }
 
+bool encode_tiled_bytes(CUtensorMap *map, const void *base, uint64_t row_bytes, uint64_t rows, uint64_t pitch,
+                        uint32_t box_rows, std::string *err) {
+  EncodeFn fn = get_encode(err);
+  if (!fn) return false;
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || pitch % 16 != 0) {
+    if (err) *err = "tensor map base and pitch are multiples of 16 bytes";
+    return false;
+  }
+  const cuuint64_t dims[2] = {row_bytes, rows}, strides[1] = {pitch};
+  const cuuint32_t box[2] = {128, box_rows}, steps[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    if (err) *err = "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r);
+    return false;
+  }
+  return true;
+}
+
 }  // namespace ivb
