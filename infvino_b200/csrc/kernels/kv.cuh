@@ -53,6 +53,10 @@ struct KvAttend {
   int *status;
   FastDiv by_group, by_page;
   long long probe;  // above 0: every other CTA of the prompt kernel first waits so many SM clocks for what never comes
+  // groups of sequences with a common beginning (kv_attend.cuh, KvMode)
+  const int32_t *first, *shared;
+  int groups, sequences;
+  float *scratch;
 };
 
 struct KvRopeFreq {
@@ -72,7 +76,8 @@ constexpr size_t kKvCounterBytes = 1 << 14;
 size_t kv_workspace_bytes(int sms);
 size_t kv_prompt_workspace_bytes(int sms);  // the part that kv_prompt.cu needs
 bool kv_prompt_takes(const KvAttend &a);
-cudaError_t launch_kv_prompt(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
+cudaError_t launch_kv_prompt(bool bf16, int mode, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
+cudaError_t launch_kv_attend_shared(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st);
 
 }  // namespace ivb

@@ -132,9 +132,9 @@ struct StepShared {
 };
 
 // NT: 8-row tiles of queries that share the codes of an item.
-template <bool BF16, int DIM, int NT>
+template <bool BF16, int DIM, int NT, int MODE>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
-    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters) {
+    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters, const PromptSlot *begun) {
   extern __shared__ uint8_t smem_raw[];
   StepShared<DIM, NT> &sh = *reinterpret_cast<StepShared<DIM, NT> *>(smem_raw);
   constexpr int kRows = 8 * NT;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   long long mine = 0;
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
   for (int b = b_lo; b < b_hi; ++b) {
-    const KvSpan s = kv_span(a, b);
+    const KvSpan s = kv_span<MODE>(a, b);
     mine += (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
   }
   long long incl = mine;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     long long at = excl;
     int b = b_lo;
     for (;; ++b) {
-      const KvSpan s = kv_span(a, b);
+      const KvSpan s = kv_span<MODE>(a, b);
       const long long w = (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
       if (u < at + w) break;
       at += w;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   __syncthreads();
   int b = sh.seq;
   uint32_t base = (uint32_t)sh.base;  // first unit of sequence b
-  KvSpan s = kv_span(a, b);
+  KvSpan s = kv_span<MODE>(a, b);
   int row_tiles = (s.n * a.group + kRows - 1) / kRows;
 
   // ---- this lane's places in a tile of codes
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       const uint32_t units = (uint32_t)s.blocks * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
       if (u < base + units) break;
       base += units;
-      s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+      s = kv_span<MODE>(a, ++b);  // (units are left, so there is a next sequence)
       row_tiles = (s.n * a.group + kRows - 1) / kRows;
     }
     const uint32_t item = (u - base) / (uint32_t)s.blocks;
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         if (it + lane < count) {
           const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
           if (key < s.len) {
-            const int at = fast_div(key, a.by_page), page = a.seqs.pages[(long long)b * a.seqs.pps + at];
+            const int at = fast_div(key, a.by_page), page = a.seqs.pages[kv_page_row<MODE>(a, b) + at];
             if ((unsigned)page < (unsigned long long)a.cache.pages) {
               const int slot = key - at * a.cache.page;
               where = kv_code_at(a.cache, page, head, slot);
@@ -329,13 +329,13 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int rc = rt * kRows + 8 * t + 2 * t4 + c, ic = fast_div(rc, a.by_group);
-        pos[t][c] = ic < s.n ? s.len - s.n + ic : -1;
+        pos[t][c] = ic < s.n ? kv_position<MODE>(s, ic) : -1;
         rs[t][c] = BF16 ? __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4) : up;  // (lane of column 2 t4 + c)
         qo[t][c] = __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4) * (-128.f * kTiny);
       }
     }
-    const int p_lo = s.len - s.n + fast_div(rt * kRows, a.by_group);                                  // first row's position
-    const int p_hi = s.len - s.n + min(s.n - 1, fast_div(rt * kRows + kRows - 1, a.by_group));      // last row's
+    const int p_lo = kv_position<MODE>(s, fast_div(rt * kRows, a.by_group));                               // first row's position
+    const int p_hi = kv_position<MODE>(s, min(s.n - 1, fast_div(rt * kRows + kRows - 1, a.by_group)));  // last row's
 
     float acc[NT][kTiles][4];
     float m[NT][2], l[NT][2];
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 
     // ---- what the join needs of this segment, then the next one's blocks on their way
     const int n = s.n, first = s.first, head_now = head, rt_now = rt;
-    const bool begins = k0 == 0, whole = begins && k1 == s.blocks;
+    const bool begins = k0 == 0, whole = begins && k1 == s.blocks, joins = MODE == kRest && s.first_block > 0;
     const int first_cta = (int)(item_begin / size), last_cta = (int)((item_begin + (uint32_t)s.blocks - 1u) / size);
     u += (uint32_t)(k1 - k0);
     const bool more = u < u_end;
@@ -610,9 +610,18 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
           const float2 y = kv_norm(fast_exp2(t - top), sum);
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] = x[k] * y.x * y.y;
-          uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(first + i) * a.out.ts +
-                        (long long)(head_now * a.group + row - i * a.group) * a.out.hs;
-          store8(o + (ln >> 2) * kPiece + d0, pack8<BF16>(x), a.out.vec);
+          const int d = (ln >> 2) * kPiece + d0, h = head_now * a.group + row - i * a.group;
+          const long long at = (long long)(first + i) * a.q_heads + h;
+          if (MODE == kBegin) {
+            float4 *o = reinterpret_cast<float4 *>(kv_part(a, at) + d);
+            __stcg(o, make_float4(x[0], x[1], x[2], x[3]));
+            __stcg(o + 1, make_float4(x[4], x[5], x[6], x[7]));
+            if (d == 0) __stcg(kv_part_sums(a, at), make_float2(top, sum));
+            continue;
+          }
+          if (joins) kv_join(a, begun, at, d, x, top, sum);
+          uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(first + i) * a.out.ts + (long long)h * a.out.hs;
+          store8(o + d, pack8<BF16>(x), a.out.vec);
         }
       }
     }
@@ -621,34 +630,51 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   }
 }
 
-template <bool BF16, int DIM, int NT>
-cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+template <bool BF16, int DIM, int NT, int MODE>
+cudaError_t launch_step(const KvAttend &a, void *workspace, size_t at, int sms, cudaStream_t st) {
   static std::atomic<bool> attr_set[kAttrMaxDevices];
   const int bytes = (int)sizeof(StepShared<DIM, NT>);
-  const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT>, bytes, attr_set);
+  const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT, MODE>, bytes, attr_set);
   if (e != cudaSuccess) return e;
   const int grid = sms * step_ctas(DIM, NT);
-  return launch_kernel(kv_step_k<BF16, DIM, NT>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
-                       reinterpret_cast<StepSlot<DIM, NT> *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
-                       static_cast<unsigned *>(workspace));
+  uint8_t *const slots = static_cast<uint8_t *>(workspace) + kKvCounterBytes;
+  return launch_kernel(kv_step_k<BF16, DIM, NT, MODE>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
+                       reinterpret_cast<StepSlot<DIM, NT> *>(slots + at), static_cast<unsigned *>(workspace),
+                       reinterpret_cast<const PromptSlot *>(slots));
 }
 
-template <bool BF16, int DIM>
-cudaError_t launch_step_rows(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+// `at`: where the parts' room in the workspace begins.
+template <bool BF16, int DIM, int MODE = kWhole>
+cudaError_t launch_step_rows(const KvAttend &a, long long rows, void *workspace, size_t at, int sms, cudaStream_t st) {
   // Rows beyond 16 come as further items: their codes are read again, from L2
   // (24 sequences of 6001, 30 rows of 64 wide heads: 58 us when it was compared,
   // 50 now; tiles of 32 rows, which read them once but leave room for half the
   // warps, 65 us).
-  if ((long long)a.max_new * a.group <= 8) return launch_step<BF16, DIM, 1>(a, workspace, sms, st);
-  return launch_step<BF16, DIM, 2>(a, workspace, sms, st);
+  if (rows <= 8) return launch_step<BF16, DIM, 1, MODE>(a, workspace, at, sms, st);
+  return launch_step<BF16, DIM, 2, MODE>(a, workspace, at, sms, st);
+}
+
+template <bool BF16, int DIM>
+cudaError_t launch_shared(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  // Rows of a group: of all sequences, one group like another.
+  KvAttend b = a;
+  b.seqs.batch = a.groups;
+  const long long rows = (a.seqs.tokens + a.groups - 1) / a.groups * a.group;
+  const cudaError_t e = rows > 64 && kv_prompt_takes(b) ? launch_kv_prompt(BF16, kBegin, b, workspace, sms, st)
+                                                        : launch_step_rows<BF16, DIM, kBegin>(b, rows, workspace, 0, sms, st);
+  if (e != cudaSuccess) return e;
+  const long long own = (long long)a.max_new * a.group;
+  if (own > 64 && kv_prompt_takes(a)) return launch_kv_prompt(BF16, kRest, a, workspace, sms, st);
+  return launch_step_rows<BF16, DIM, kRest>(a, own, workspace, kv_prompt_workspace_bytes(sms), sms, st);
 }
 
 }  // namespace
 
-// Counters (zero before the first call and after each), then two slots a CTA.
+// Counters (zero before the first call and after each), then two slots a CTA; twice, for
+// the parts of a common beginning wait while the sequences' own keys are read.
 size_t kv_workspace_bytes(int sms) {
   const size_t step = sizeof(StepSlot<128, 2>) * 2 * 4 * (size_t)sms;  // (the largest slot, the most CTAs)
-  return kKvCounterBytes + std::max(step, kv_prompt_workspace_bytes(sms));
+  return kKvCounterBytes + kv_prompt_workspace_bytes(sms) + std::max(step, kv_prompt_workspace_bytes(sms));
 }
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
@@ -662,10 +688,16 @@ cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int 
   //                                      128 wide   23/28    26/29    28/29
   // At 96 and 128 rows (64 wide, 24 sequences) it was 125/98 and 173/109: few
   // sequences gain from this one up to 64 rows and beyond, many up to some 50.
-  if ((long long)a.max_new * a.group > 64 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, a, workspace, sms, st);
+  const long long rows = (long long)a.max_new * a.group;
+  if (rows > 64 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, kWhole, a, workspace, sms, st);
   if (a.cache.dim == 64)
-    return bf16 ? launch_step_rows<true, 64>(a, workspace, sms, st) : launch_step_rows<false, 64>(a, workspace, sms, st);
-  return bf16 ? launch_step_rows<true, 128>(a, workspace, sms, st) : launch_step_rows<false, 128>(a, workspace, sms, st);
+    return bf16 ? launch_step_rows<true, 64>(a, rows, workspace, 0, sms, st) : launch_step_rows<false, 64>(a, rows, workspace, 0, sms, st);
+  return bf16 ? launch_step_rows<true, 128>(a, rows, workspace, 0, sms, st) : launch_step_rows<false, 128>(a, rows, workspace, 0, sms, st);
+}
+
+cudaError_t launch_kv_attend_shared(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  if (a.cache.dim == 64) return bf16 ? launch_shared<true, 64>(a, workspace, sms, st) : launch_shared<false, 64>(a, workspace, sms, st);
+  return bf16 ? launch_shared<true, 128>(a, workspace, sms, st) : launch_shared<false, 128>(a, workspace, sms, st);
 }
 
 }  // namespace ivb

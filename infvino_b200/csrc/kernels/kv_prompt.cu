@@ -74,13 +74,21 @@ struct alignas(16) TileMeta {
 struct RowSpan {
   int sink_blocks, first_block, blocks, tiles;
 };
-__device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, int rt) {
+template <int MODE>
+__device__ __forceinline__ RowSpan row_span(const KvAttend &a, int n, int len, int first_block, int rt) {
   RowSpan s;
+  if (MODE == kBegin) {  // every row sees all
+    s.first_block = s.sink_blocks = 0;
+    s.blocks = len / kKvBlock;
+    s.tiles = max(1, (s.blocks + kTileBlocks - 1) / kTileBlocks);
+    return s;
+  }
   const int i0 = fast_div(rt * kRows, a.by_group), i1 = min(n - 1, fast_div(rt * kRows + kRows - 1, a.by_group));
   const int p_lo = len - n + i0, p_hi = len - n + i1;
   const int all = p_hi >= 0 ? p_hi / kKvBlock + 1 : 0;
-  s.first_block = s.sink_blocks = 0;
-  if (a.window > 0) {
+  s.first_block = MODE == kRest ? first_block : 0;
+  s.sink_blocks = 0;
+  if (MODE == kWhole && a.window > 0) {
     const long long lo = (long long)p_lo - a.window + 1;
     s.first_block = lo > 0 ? (int)(lo / kKvBlock) : 0;
     s.sink_blocks = min(s.first_block, a.sinks / kKvBlock + (a.sinks % kKvBlock != 0));
@@ -101,6 +109,7 @@ struct Segment {
 };
 
 // A CTA's share of the units, segment by segment.
+template <int MODE>
 struct Walk {
   uint32_t u, end, base;  // next unit, the share's end, first unit of (b, rt)
   int b, rt, row_tiles;
@@ -111,9 +120,9 @@ struct Walk {
   __device__ __forceinline__ void begin(const KvAttend &a, uint32_t from, uint32_t to, uint32_t at, int b0, int rt0) {
     u = from, end = to, base = at, b = b0, rt = rt0;
     if (u >= end) return;
-    s = kv_span(a, b);
+    s = kv_span<MODE>(a, b);
     row_tiles = (s.n * a.group + kRows - 1) / kRows;
-    r = row_span(a, s.n, s.len, rt);
+    r = row_span<MODE>(a, s.n, s.len, s.first_block, rt);
   }
 
   // The next segment into g (all but `more`); false where the share ends.
@@ -136,14 +145,14 @@ struct Walk {
         }
         base += units;
         if (++rt < row_tiles) {
-          r = row_span(a, s.n, s.len, rt);
+          r = row_span<MODE>(a, s.n, s.len, s.first_block, rt);
           continue;
         }
       }
       rt = 0;
-      s = kv_span(a, ++b);  // (units are left, so there is a next sequence)
+      s = kv_span<MODE>(a, ++b);  // (units are left, so there is a next sequence)
       row_tiles = (s.n * a.group + kRows - 1) / kRows;
-      if (s.n > 0) r = row_span(a, s.n, s.len, 0);
+      if (s.n > 0) r = row_span<MODE>(a, s.n, s.len, s.first_block, 0);
     }
     return false;
   }
@@ -167,13 +176,6 @@ struct PromptShared {
   long long base;
   int seq, rt;
   uint32_t u_begin, u_end, size;  // the share, and how many units one has
-};
-
-struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4] in units of 2^m vref, row's m and sum
-  float acc[128 * 128];
-  float m[128], l[128];
-  float vref;
-  float pad[31];
 };
 
 // Counts a part of an item that CTAs first .. last share; the last one to come sets the counter back.
@@ -292,9 +294,9 @@ __device__ __forceinline__ void put_codes(uint32_t lo_at, uint32_t hi_at, uint4 
 
 // Counts the parts of cut items that a CTA has not come to, so that the counters
 // are zero again after a launch in which it gave up.  (Not inline: this is rarely run.)
-template <class Shared>
+template <int MODE, class Shared>
 __device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned *counters) {
-  Walk walk;
+  Walk<MODE> walk;
   walk.begin(a, sh.u_begin, sh.u_end, (uint32_t)sh.base, sh.seq, sh.rt);
   Segment &g = sh.seg[0];
   while (walk.next(a, sh.size, g))
@@ -303,9 +305,9 @@ __device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned 
         count_part(&counters[2 * g.first_cta + i], g.first_cta, g.last_cta);
 }
 
-template <bool BF16, int DIM>
+template <bool BF16, int DIM, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters) {
+    kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters, const PromptSlot *begun) {
   extern __shared__ uint8_t smem_raw[];
   using Shared = PromptShared<DIM>;
   Shared &sh = *reinterpret_cast<Shared *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -347,18 +349,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   long long *sums = reinterpret_cast<long long *>(&sh.q[0][0][0]);
 #pragma unroll 1
   for (int b0 = warp * 32; b0 < a.seqs.batch; b0 += kThreads) {
-    int n = 0, len = 0;
+    int n = 0, len = 0, block = 0;
     if (b0 + lane < a.seqs.batch) {
-      const KvSpan s = kv_span(a, b0 + lane);
-      n = s.n, len = s.len;
+      const KvSpan s = kv_span<MODE>(a, b0 + lane);
+      n = s.n, len = s.len, block = s.first_block;
     }
 #pragma unroll 1
     for (int j = 0; j < min(32, a.seqs.batch - b0); ++j) {
       const int nj = __shfl_sync(0xffffffffu, n, j), lj = __shfl_sync(0xffffffffu, len, j);
+      const int bj = MODE == kRest ? __shfl_sync(0xffffffffu, block, j) : 0;
       const int rts = (nj * a.group + kRows - 1) / kRows;
       long long sum = 0;
 #pragma unroll 1
-      for (int rt = lane; rt < rts; rt += 32) sum += row_span(a, nj, lj, rt).tiles + kItemCost;
+      for (int rt = lane; rt < rts; rt += 32) sum += row_span<MODE>(a, nj, lj, bj, rt).tiles + kItemCost;
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) sums[b0 + j] = sum * a.cache.heads;
@@ -408,12 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (works && warp == 0) {  // the row tile: 32 at a time
-    const KvSpan s = kv_span(a, sh.seq);
+    const KvSpan s = kv_span<MODE>(a, sh.seq);
     const int rts = (s.n * a.group + kRows - 1) / kRows;
     long long at = sh.base;
 #pragma unroll 1
     for (int r0 = 0; r0 < rts; r0 += 32) {
-      long long w = r0 + lane < rts ? (long long)(row_span(a, s.n, s.len, r0 + lane).tiles + kItemCost) * a.cache.heads : 0;
+      long long w = r0 + lane < rts ? (long long)(row_span<MODE>(a, s.n, s.len, s.first_block, r0 + lane).tiles + kItemCost) * a.cache.heads : 0;
       long long in = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -533,20 +536,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = g->k1 - g->k0;
       const int tok = fast_div(first_row + row, a.by_group);
       const bool real = row < rows;
-      const int p = real ? g->s.len - g->s.n + tok : -1;
-      const int p_lo = g->s.len - g->s.n + fast_div(first_row, a.by_group);
-      const int p_hi = g->s.len - g->s.n + fast_div(first_row + rows - 1, a.by_group);
+      const int p = real ? kv_position<MODE>(g->s, tok) : -1;
+      const int p_lo = kv_position<MODE>(g->s, fast_div(first_row, a.by_group));
+      const int p_hi = kv_position<MODE>(g->s, fast_div(first_row + rows - 1, a.by_group));
       const bool whole = g->whole(), head_part = g->k0 == 0;
       const int first_cta = g->first_cta, last_cta = g->last_cta;
       uint16_t *out = static_cast<uint16_t *>(a.out.p) + (long long)(g->s.first + tok) * a.out.ts +
                       (long long)(g->head * a.group + first_row + row - tok * a.group) * a.out.hs;
+      // (of kBegin and kRest: the row's place in the scratch, and whether there is a beginning)
+      const long long at = (long long)(g->s.first + tok) * a.q_heads + g->head * a.group + first_row + row - tok * a.group;
+      const bool joins = MODE == kRest && g->s.first_block > 0;
       // parts (of four blocks) that need no look at single keys: up to part_hi
       // every row sees the end of it, from part_lo on every row its beginning
       // (or, before part_sink, all of it are sinks)
       const RowSpan &rs = g->r;
       const int part_hi = ((p_lo + 1) / kKvBlock + rs.sink_blocks - rs.first_block) / 4 - 1;
       int part_lo = 0, part_sink = 0;
-      if (a.window > 0 && p_hi >= a.window) {
+      if (MODE == kWhole && a.window > 0 && p_hi >= a.window) {
         part_lo = ((p_hi - a.window) / kKvBlock + 1 - rs.first_block + rs.sink_blocks + 3) / 4;
         part_sink = min(rs.sink_blocks, a.sinks / kKvBlock) / 4;
       }
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b = 0; b < 4; ++b) {
               const int hi = p - me.key0[b0 + b];
               uint32_t seen = low_bits(hi + 1);
-              if (a.window > 0) seen &= ~low_bits(hi - a.window + 1) | low_bits(a.sinks - me.key0[b0 + b]);
+              if (MODE == kWhole && a.window > 0) seen &= ~low_bits(hi - a.window + 1) | low_bits(a.sinks - me.key0[b0 + b]);
               if (__all_sync(0xffffffffu, seen == 0xffffu)) continue;
               uint32_t w[16];
               tmem_ld16(s_at + 16 * b, w);
@@ -701,10 +707,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               float f[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) f[j] = l != 0.f ? o[k + j] * y.x * y.y : 0.f;
+              if (MODE == kBegin) {
+                float4 *to = reinterpret_cast<float4 *>(kv_part(a, at) + 32 * h + k);
+                __stcg(to, make_float4(f[0], f[1], f[2], f[3]));
+                __stcg(to + 1, make_float4(f[4], f[5], f[6], f[7]));
+                continue;
+              }
+              if (joins) kv_join(a, begun, at, 32 * h + k, f, m, l * kPromptToPart);
               store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
         }
+        if (MODE == kBegin && real) __stcg(kv_part_sums(a, at), make_float2(m, l * kPromptToPart));
       } else {
         PromptSlot &slot = slots[2 * (2 * (int)blockIdx.x + (head_part ? 1 : 0)) + i];
 #pragma unroll 1
@@ -722,8 +736,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         __stcg(&slot.m[row], m);
         __stcg(&slot.l[row], l);
         if (row == 0) __stcg(&slot.vref, vref);
+        if (MODE == kBegin && head_part && real) {  // (the parts are joined where they are used, by many CTAs)
+          __stcg(reinterpret_cast<int4 *>(kv_part(a, at)), make_int4(first_cta, last_cta, 128 * i + row, 0));
+          __stcg(kv_part_sums(a, at), make_float2(0.f, -1.f));
+        }
       }
-      if (!whole) {
+      if (MODE != kBegin && !whole) {
         wg_sync(1 + i);
         if (row == 0) {
           __threadfence();  // (the four warps' writes, which the barrier has put before this)
@@ -767,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float f[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y.x * y.y;
+              if (joins) kv_join(a, begun, at, 64 * h + k, f, top, sum * kPromptToPart);
               store8(out + 64 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
@@ -802,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       key_next = kNoKey;
       if (lane < kTileBlocks && t < g->k1 && bi < g->r.blocks) {
         key_next = (bi < g->r.sink_blocks ? bi : bi - g->r.sink_blocks + g->r.first_block) * kKvBlock;
-        page_next = a.seqs.pages[(long long)g->b * a.seqs.pps + fast_div(key_next, a.by_page)];  // (in the row: kv_span has checked)
+        page_next = a.seqs.pages[kv_page_row<MODE>(a, g->b) + fast_div(key_next, a.by_page)];  // (in the row: kv_span has checked)
       }
     };
     auto look_up = [&]() {
@@ -990,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait_bounded(smem_u32(&sh.drained), 0, &no_abort, a.status, kStatusTimeoutDrain, 400000000LL);
     } else if (warp == 13 && lane == 0) {
       // ---------------------------------------------------------- segments
-      Walk walk;
+      Walk<MODE> walk;
       const uint32_t size = sh.size;
       walk.begin(a, sh.u_begin, sh.u_end, (uint32_t)sh.base, sh.seq, sh.rt);
       for (int n = 0;; ++n) {
@@ -1011,20 +1030,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
-  } else if (threadIdx.x == 0 && sh.abort) {
-    count_rest(a, sh, counters);
+  } else if (MODE != kBegin && threadIdx.x == 0 && sh.abort) {
+    count_rest<MODE>(a, sh, counters);
   }
 }
 
-template <bool BF16, int DIM>
+template <bool BF16, int DIM, int MODE>
 cudaError_t launch_prompt(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   static std::atomic<bool> attr_set[kAttrMaxDevices];
   const int bytes = (int)sizeof(PromptShared<DIM>) + 1024;
-  const cudaError_t e = ensure_dynamic_smem(kv_prompt_k<BF16, DIM>, bytes, attr_set);
+  const cudaError_t e = ensure_dynamic_smem(kv_prompt_k<BF16, DIM, MODE>, bytes, attr_set);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kv_prompt_k<BF16, DIM>, dim3(sms), dim3(kThreads), (size_t)bytes, st, a,
-                       reinterpret_cast<PromptSlot *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
-                       static_cast<unsigned *>(workspace));
+  PromptSlot *const slots = reinterpret_cast<PromptSlot *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes);
+  return launch_kernel(kv_prompt_k<BF16, DIM, MODE>, dim3(sms), dim3(kThreads), (size_t)bytes, st, a,
+                       MODE == kRest ? slots + 4 * (size_t)sms : slots, static_cast<unsigned *>(workspace),
+                       static_cast<const PromptSlot *>(slots));
+}
+
+template <int MODE>
+cudaError_t launch_mode(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  if (a.cache.dim == 64)
+    return bf16 ? launch_prompt<true, 64, MODE>(a, workspace, sms, st) : launch_prompt<false, 64, MODE>(a, workspace, sms, st);
+  return bf16 ? launch_prompt<true, 128, MODE>(a, workspace, sms, st) : launch_prompt<false, 128, MODE>(a, workspace, sms, st);
 }
 
 }  // namespace
@@ -1033,10 +1060,10 @@ size_t kv_prompt_workspace_bytes(int sms) { return sizeof(PromptSlot) * 4 * (siz
 
 bool kv_prompt_takes(const KvAttend &a) { return a.seqs.batch <= kMaxSeqs; }
 
-cudaError_t launch_kv_prompt(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
-  if (a.cache.dim == 64)
-    return bf16 ? launch_prompt<true, 64>(a, workspace, sms, st) : launch_prompt<false, 64>(a, workspace, sms, st);
-  return bf16 ? launch_prompt<true, 128>(a, workspace, sms, st) : launch_prompt<false, 128>(a, workspace, sms, st);
+cudaError_t launch_kv_prompt(bool bf16, int mode, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
+  if (mode == kBegin) return launch_mode<kBegin>(bf16, a, workspace, sms, st);
+  if (mode == kRest) return launch_mode<kRest>(bf16, a, workspace, sms, st);
+  return launch_mode<kWhole>(bf16, a, workspace, sms, st);
 }
 
 }  // namespace ivb

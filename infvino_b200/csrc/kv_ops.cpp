@@ -494,9 +494,15 @@ int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs
     need(aligned(scratch, 16), "scratch is 16-byte aligned");
     need(a.seqs.tokens == 0 || (scratch && scratch_floats >= a.seqs.tokens * q_heads * (a.cache.dim + 2)),
          "scratch: at least tokens * q_heads * (head_dim + 2) floats");
+    need(a.seqs.tokens * a.group < (1LL << 30), "tokens * q_heads / kv_heads out of range");
     if (a.seqs.tokens == 0) return;
+    a.first = groups->first;
+    a.shared = groups->shared;
+    a.groups = groups->count;
+    a.sequences = a.seqs.batch;
+    a.scratch = scratch;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cuda(ivb::launch_kv_attend(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
+    cuda(ivb::launch_kv_attend_shared(dtype == IVC_BF16, a, workspace(h, st), h->sms, st), "launch");
   });
 }
 
