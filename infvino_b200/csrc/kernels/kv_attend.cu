@@ -129,12 +129,13 @@ struct StepShared {
   long long base;
   int seq;
   int last;
+  unsigned items, each;  // of kRest: items, and blocks of one
 };
 
 // NT: 8-row tiles of queries that share the codes of an item.
 template <bool BF16, int DIM, int NT, int MODE>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
-    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters, const PromptSlot *begun) {
+    kv_step_k(const __grid_constant__ KvAttend a, StepSlot<DIM, NT> *slots, unsigned *counters) {
   extern __shared__ uint8_t smem_raw[];
   StepShared<DIM, NT> &sh = *reinterpret_cast<StepShared<DIM, NT> *>(smem_raw);
   constexpr int kRows = 8 * NT;
@@ -150,9 +151,15 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   const int per = (a.seqs.batch + kStepThreads - 1) / kStepThreads;
   long long mine = 0;
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
+  if (MODE == kRest) {
+    if (threadIdx.x == 0) sh.items = 0;
+    __syncthreads();
+  }
   for (int b = b_lo; b < b_hi; ++b) {
     const KvSpan s = kv_span<MODE>(a, b);
-    mine += (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
+    const int tiles = (s.n * a.group + kRows - 1) / kRows;
+    mine += (long long)s.blocks * tiles * a.cache.heads;
+    if (MODE == kRest && tiles) atomicAdd(&sh.items, (unsigned)(tiles * a.cache.heads));
   }
   long long incl = mine;
 #pragma unroll
@@ -169,11 +176,16 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     total += sh.scan[w];
   }
   if (total == 0) return;
+  // (what a sequence has of its own may be a block or two: a share is an item then, not several in turn)
+  if (MODE == kRest && threadIdx.x == 0) sh.each = (uint32_t)min(total / max(sh.items, 1u) + 1, (long long)kStepMinBlocks);
+  if (MODE == kRest) __syncthreads();
   if (total > 0x7fffffffLL) {  // (hours of work; units are counted in 32 bits from here)
     if (threadIdx.x == 0) kv_flag(a.status, kStatusKvSeqs);
     return;
   }
-  const uint32_t size = max((uint32_t)kStepMinBlocks, ((uint32_t)total + gridDim.x - 1) / gridDim.x);  // units of a share
+  uint32_t at_least = kStepMinBlocks;
+  if (MODE == kRest) at_least = min(at_least, sh.each);
+  const uint32_t size = max(at_least, ((uint32_t)total + gridDim.x - 1) / gridDim.x);  // units of a share
   uint32_t u = blockIdx.x * size;
   if (u >= (uint32_t)total) return;
   const uint32_t u_end = min((uint32_t)total, u + size);
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         if (it + lane < count) {
           const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
           if (key < s.len) {
-            const int at = fast_div(key, a.by_page), page = a.seqs.pages[kv_page_row<MODE>(a, b) + at];
+            const int at = fast_div(key, a.by_page), page = a.seqs.pages[kv_page_at<MODE>(a, s, b, key, at)];
             if ((unsigned)page < (unsigned long long)a.cache.pages) {
               const int slot = key - at * a.cache.page;
               where = kv_code_at(a.cache, page, head, slot);
@@ -619,7 +631,11 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
             if (d == 0) __stcg(kv_part_sums(a, at), make_float2(top, sum));
             continue;
           }
-          if (joins) kv_join(a, begun, at, d, x, top, sum);
+          if (joins) {
+            const float4 *o = reinterpret_cast<const float4 *>(kv_part(a, at) + d);
+            const float4 v0 = __ldcg(o), v1 = __ldcg(o + 1);
+            kv_joined(kv_join(a, at, top, sum), v0, v1, x);
+          }
           uint16_t *o = static_cast<uint16_t *>(a.out.p) + (long long)(first + i) * a.out.ts + (long long)h * a.out.hs;
           store8(o + d, pack8<BF16>(x), a.out.vec);
         }
@@ -631,28 +647,28 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 }
 
 template <bool BF16, int DIM, int NT, int MODE>
-cudaError_t launch_step(const KvAttend &a, void *workspace, size_t at, int sms, cudaStream_t st) {
+cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   static std::atomic<bool> attr_set[kAttrMaxDevices];
   const int bytes = (int)sizeof(StepShared<DIM, NT>);
   const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT, MODE>, bytes, attr_set);
   if (e != cudaSuccess) return e;
   const int grid = sms * step_ctas(DIM, NT);
-  uint8_t *const slots = static_cast<uint8_t *>(workspace) + kKvCounterBytes;
   return launch_kernel(kv_step_k<BF16, DIM, NT, MODE>, dim3(grid), dim3(kStepThreads), (size_t)bytes, st, a,
-                       reinterpret_cast<StepSlot<DIM, NT> *>(slots + at), static_cast<unsigned *>(workspace),
-                       reinterpret_cast<const PromptSlot *>(slots));
+                       reinterpret_cast<StepSlot<DIM, NT> *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes),
+                       static_cast<unsigned *>(workspace));
 }
 
-// `at`: where the parts' room in the workspace begins.
 template <bool BF16, int DIM, int MODE = kWhole>
-cudaError_t launch_step_rows(const KvAttend &a, long long rows, void *workspace, size_t at, int sms, cudaStream_t st) {
+cudaError_t launch_step_rows(const KvAttend &a, long long rows, void *workspace, int sms, cudaStream_t st) {
   // Rows beyond 16 come as further items: their codes are read again, from L2
   // (24 sequences of 6001, 30 rows of 64 wide heads: 58 us when it was compared,
   // 50 now; tiles of 32 rows, which read them once but leave room for half the
   // warps, 65 us).
-  if (rows <= 8) return launch_step<BF16, DIM, 1, MODE>(a, workspace, at, sms, st);
-  return launch_step<BF16, DIM, 2, MODE>(a, workspace, at, sms, st);
+  if (rows <= 8) return launch_step<BF16, DIM, 1, MODE>(a, workspace, sms, st);
+  return launch_step<BF16, DIM, 2, MODE>(a, workspace, sms, st);
 }
+
+constexpr long long kOnePass = 48 << 20;  // bytes of codes
 
 template <bool BF16, int DIM>
 cudaError_t launch_shared(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
@@ -660,21 +676,28 @@ cudaError_t launch_shared(const KvAttend &a, void *workspace, int sms, cudaStrea
   KvAttend b = a;
   b.seqs.batch = a.groups;
   const long long rows = (a.seqs.tokens + a.groups - 1) / a.groups * a.group;
-  const cudaError_t e = rows > 64 && kv_prompt_takes(b) ? launch_kv_prompt(BF16, kBegin, b, workspace, sms, st)
-                                                        : launch_step_rows<BF16, DIM, kBegin>(b, rows, workspace, 0, sms, st);
-  if (e != cudaSuccess) return e;
   const long long own = (long long)a.max_new * a.group;
+  // Few keys: every sequence reads the beginning for itself, in one launch (TODO us).
+  const long long keys = (long long)a.sequences * a.seqs.pps * a.cache.page;
+  if (own <= 64 && keys * a.cache.heads * 2 * DIM <= kOnePass) return launch_step_rows<BF16, DIM, kOne>(a, own, workspace, sms, st);
+  cudaError_t e;
+  if (rows > 64 && kv_prompt_takes(b)) {
+    e = launch_kv_prompt(BF16, kBegin, b, workspace, sms, st);
+    if (e == cudaSuccess) e = launch_kv_parts(a, workspace, sms, st);
+  } else {
+    e = launch_step_rows<BF16, DIM, kBegin>(b, rows, workspace, sms, st);
+  }
+  if (e != cudaSuccess) return e;
   if (own > 64 && kv_prompt_takes(a)) return launch_kv_prompt(BF16, kRest, a, workspace, sms, st);
-  return launch_step_rows<BF16, DIM, kRest>(a, own, workspace, kv_prompt_workspace_bytes(sms), sms, st);
+  return launch_step_rows<BF16, DIM, kRest>(a, own, workspace, sms, st);
 }
 
 }  // namespace
 
-// Counters (zero before the first call and after each), then two slots a CTA; twice, for
-// the parts of a common beginning wait while the sequences' own keys are read.
+// Counters (zero before the first call and after each), then two slots a CTA.
 size_t kv_workspace_bytes(int sms) {
   const size_t step = sizeof(StepSlot<128, 2>) * 2 * 4 * (size_t)sms;  // (the largest slot, the most CTAs)
-  return kKvCounterBytes + kv_prompt_workspace_bytes(sms) + std::max(step, kv_prompt_workspace_bytes(sms));
+  return kKvCounterBytes + std::max(step, kv_prompt_workspace_bytes(sms));
 }
 
 cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
@@ -691,8 +714,8 @@ cudaError_t launch_kv_attend(bool bf16, const KvAttend &a, void *workspace, int 
   const long long rows = (long long)a.max_new * a.group;
   if (rows > 64 && kv_prompt_takes(a)) return launch_kv_prompt(bf16, kWhole, a, workspace, sms, st);
   if (a.cache.dim == 64)
-    return bf16 ? launch_step_rows<true, 64>(a, rows, workspace, 0, sms, st) : launch_step_rows<false, 64>(a, rows, workspace, 0, sms, st);
-  return bf16 ? launch_step_rows<true, 128>(a, rows, workspace, 0, sms, st) : launch_step_rows<false, 128>(a, rows, workspace, 0, sms, st);
+    return bf16 ? launch_step_rows<true, 64>(a, rows, workspace, sms, st) : launch_step_rows<false, 64>(a, rows, workspace, sms, st);
+  return bf16 ? launch_step_rows<true, 128>(a, rows, workspace, sms, st) : launch_step_rows<false, 128>(a, rows, workspace, sms, st);
 }
 
 cudaError_t launch_kv_attend_shared(bool bf16, const KvAttend &a, void *workspace, int sms, cudaStream_t st) {

@@ -57,20 +57,28 @@ struct KvSpan {
   int first;          // packed token
   int n, len;         // new tokens; tokens in the cache, those included
   int sink_blocks, first_block, blocks;
+  int lead, common;   // of kOne: the sequence whose pages have the first `common` tokens
   __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : i - sink_blocks + first_block; }
 };
 
 // What a launch works on: whole sequences; or, of sequences in groups with a common
 // beginning, first the groups (all queries of a group over the beginning, whose
 // results wait in the scratch: kv_part below), then each sequence's own keys, with
-// those results joined in.
-enum KvMode { kWhole = 0, kBegin = 1, kRest = 2 };
+// those results joined in; or both in one pass, each sequence reading the beginning.
+enum KvMode { kWhole = 0, kBegin = 1, kRest = 2, kOne = 3 };
 
-// The first sequence of a group, the one behind its last, and how many tokens are common; false (status set) if that does not fit.
-__device__ __forceinline__ bool kv_group(const KvAttend &a, int g, int &s0, int &s1, int &len) {
-  s0 = a.first[g], s1 = a.first[g + 1], len = a.shared[g];
-  const bool fits = s0 >= 0 && s1 >= s0 && s1 <= a.sequences && len >= 0 && len <= (long long)a.seqs.pps * a.cache.page &&
-                    len == fast_div(len, a.by_page) * a.cache.page;
+// A group's sequences s0 .. s1 - 1, its packed tokens o .. e - 1, and how many are common; false (status set) if that does not fit.
+struct KvGroup {
+  int s0, s1, o, e, len;
+};
+__device__ __forceinline__ bool kv_group(const KvAttend &a, int g, KvGroup &r) {
+  r.s0 = a.first[g], r.s1 = a.first[g + 1], r.len = a.shared[g];
+  bool fits = r.s0 >= 0 && r.s1 >= r.s0 && r.s1 <= a.sequences && r.len >= 0 && r.len <= (long long)a.seqs.pps * a.cache.page &&
+              r.len == fast_div(r.len, a.by_page) * a.cache.page;
+  if (fits) {
+    r.o = a.seqs.offsets[r.s0], r.e = a.seqs.offsets[r.s1];
+    fits = r.o >= 0 && r.e >= r.o && r.e <= a.seqs.tokens;
+  }
   if (!fits) kv_flag(a.status, kStatusKvSeqs);
   return fits;
 }
@@ -80,19 +88,16 @@ template <int MODE>
 __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
   KvSpan s;
   s.sink_blocks = s.first_block = s.blocks = 0;
+  s.lead = s.common = 0;
   if (MODE == kBegin) {
-    int s0, s1, len;
+    KvGroup r;
     s.first = s.n = s.len = 0;
-    if (!kv_group(a, b, s0, s1, len) || s0 == s1 || len == 0) return s;
-    const int o = a.seqs.offsets[s0], e = a.seqs.offsets[s1];
-    if (o < 0 || e < o || e > a.seqs.tokens) {
-      kv_flag(a.status, kStatusKvSeqs);
-      return s;
-    }
-    s.first = o;
-    s.n = e - o;
-    s.len = len;
-    s.blocks = max(1, len / kKvBlock);
+    if (!kv_group(a, b, r) || r.o == r.e || r.len == 0) return s;
+    s.first = r.o;
+    s.n = r.e - r.o;
+    s.lead = r.s0;
+    s.len = r.len;
+    s.blocks = r.len / kKvBlock;
     return s;
   }
   const int o = a.seqs.offsets[b], e = a.seqs.offsets[b + 1];
@@ -107,7 +112,7 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
   }
   if (s.n == 0) return s;
   const int all = (s.len + kKvBlock - 1) / kKvBlock;
-  if (MODE == kRest) {
+  if (MODE == kRest || MODE == kOne) {
     int g = 0, end = a.groups;  // the last group that begins at or before b
     while (end - g > 1) {
       const int mid = (g + end) / 2;
@@ -116,13 +121,16 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
       else
         end = mid;
     }
-    int s0, s1, len;
-    if (!kv_group(a, g, s0, s1, len) || b < s0 || b >= s1 || s.len - s.n < len) {
+    // (its tokens are the group's: their results over the beginning are there)
+    KvGroup r;
+    if (!kv_group(a, g, r) || b < r.s0 || b >= r.s1 || o < r.o || e > r.e || s.len - s.n < r.len) {
       kv_flag(a.status, kStatusKvSeqs);
       s.n = 0;
       return s;
     }
-    s.first_block = len / kKvBlock;
+    if (MODE == kRest) s.first_block = r.len / kKvBlock;
+    s.lead = r.s0;
+    s.common = r.len;
   } else if (a.window > 0) {
     // the first query's first window key; blocks before it only for the sinks
     const long long lo = (long long)s.len - s.n - a.window + 1;
@@ -133,10 +141,11 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
   return s;
 }
 
-// The row of the page table that b's pages are in.
+// Where the page of block `at` (from 0) of sequence b's pages is named, for key `key`.
 template <int MODE>
-__device__ __forceinline__ long long kv_page_row(const KvAttend &a, int b) {
-  return (long long)(MODE == kBegin ? a.first[b] : b) * a.seqs.pps;
+__device__ __forceinline__ long long kv_page_at(const KvAttend &a, const KvSpan &s, int b, int key, int at) {
+  const int row = MODE == kBegin ? s.lead : MODE == kOne && key < s.common ? s.lead : b;
+  return (long long)row * a.seqs.pps + at;
 }
 // The last key that query i of s sees.
 template <int MODE>
@@ -151,9 +160,9 @@ __device__ __forceinline__ bool kv_sees(const KvAttend &a, int p, int j) {
 
 // ---- results over a common beginning, for every packed token and head: DIM floats
 // each, then each one's m and l (the sum of weights 2^(s - m), in units of
-// 2^(kPartBits - kSumBits)).  An item that was cut over CTAs has l = -1: its first
-// words say which CTAs' slots have its parts, and its row in them.
-constexpr float kPartBits = 12.f;
+// 2^(12 - kSumBits)).  An item of the prompt kernel that was cut over CTAs has
+// l = -1 at first: its first words say which CTAs' slots have its parts, and its row
+// in them, for kv_parts_k.
 struct PromptSlot {  // one M tile of a cut item: accumulators [DIM / 4][128 rows][4] in units of 2^m vref, row's m and sum
   float acc[128 * 128];
   float m[128], l[128];
@@ -167,49 +176,20 @@ __device__ __forceinline__ float2 *kv_part_sums(const KvAttend &a, long long row
   return reinterpret_cast<float2 *>(a.scratch + a.seqs.tokens * a.q_heads * a.cache.dim) + row;
 }
 
-// x, eight elements from d0 on of a row's result over its own keys (with its m, and l in
-// units as above), becomes the result over these and the beginning.
-__device__ __forceinline__ void kv_join(const KvAttend &a, const PromptSlot *slots, long long row, int d0, float (&x)[8], float m, float l) {
+// How much a row's result over the beginning and that over its own keys (with its m,
+// and l in units as above) count.
+__device__ __forceinline__ float2 kv_join(const KvAttend &a, long long row, float m, float l) {
   const float2 ml = __ldcg(kv_part_sums(a, row));
-  float m1 = ml.x, l1 = ml.y, o[8];
-  const float4 *at = reinterpret_cast<const float4 *>(kv_part(a, row));
-  if (l1 == -1.f) {
-    const int4 where = __ldcg(reinterpret_cast<const int4 *>(at));
-    const int i = where.z >> 7, r = where.z & 127;
-    float t = -INFINITY;
-    m1 = -INFINITY, l1 = 0.f;
-#pragma unroll 8
-    for (int z = where.x; z <= where.y; ++z) {
-      const PromptSlot &sl = slots[2 * (2 * z + (z == where.x ? 1 : 0)) + i];
-      const float zm = __ldcg(&sl.m[r]);
-      m1 = fmaxf(m1, zm);
-      t = fmaxf(t, zm + log2_of(__ldcg(&sl.vref)));
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = 0.f;
-#pragma unroll 4
-    for (int z = where.x; z <= where.y; ++z) {
-      const PromptSlot &sl = slots[2 * (2 * z + (z == where.x ? 1 : 0)) + i];
-      const float zm = __ldcg(&sl.m[r]), zl = __ldcg(&sl.l[r]), wv = kv_share(zm + log2_of(__ldcg(&sl.vref)), t);
-      const float4 u = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[(d0 / 4 * 128 + r) * 4])),
-                   v = __ldcg(reinterpret_cast<const float4 *>(&sl.acc[((d0 / 4 + 1) * 128 + r) * 4]));
-      if (zm != -INFINITY || zl != 0.f) l1 += kv_scaled(zl, zm - m1);
-      o[0] += u.x * wv, o[1] += u.y * wv, o[2] += u.z * wv, o[3] += u.w * wv;
-      o[4] += v.x * wv, o[5] += v.y * wv, o[6] += v.z * wv, o[7] += v.w * wv;
-    }
-    const float2 y = kv_norm(fast_exp2(t - m1), l1);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = o[k] * y.x * y.y;
-    l1 *= kPromptToPart;
-  } else {
-    const float4 u = __ldcg(at + d0 / 4), v = __ldcg(at + d0 / 4 + 1);
-    o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w, o[4] = v.x, o[5] = v.y, o[6] = v.z, o[7] = v.w;
-  }
-  const float top = fmaxf(m, m1);
+  const float m1 = ml.x, l1 = ml.y, top = fmaxf(m, m1);
   const float w1 = l1 != 0.f ? kv_scaled(l1, m1 - top) : 0.f, w = l != 0.f ? kv_scaled(l, m - top) : 0.f;
-  const float sum = w1 + w, f1 = sum != 0.f ? w1 / sum : 0.f, f = sum != 0.f ? w / sum : 0.f;
+  const float sum = w1 + w;
+  return sum != 0.f ? make_float2(w1 / sum, w / sum) : make_float2(0.f, 0.f);
+}
+// x, eight elements of a row's result over its own keys, becomes the result over these and the beginning (u, v).
+__device__ __forceinline__ void kv_joined(float2 f, float4 u, float4 v, float (&x)[8]) {
+  const float o[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] = (f1 != 0.f ? o[k] * f1 : 0.f) + (f != 0.f ? x[k] * f : 0.f);
+  for (int k = 0; k < 8; ++k) x[k] = (f.x != 0.f ? o[k] * f.x : 0.f) + (f.y != 0.f ? x[k] * f.y : 0.f);
 }
 
 }  // namespace ivb

@@ -178,6 +178,12 @@ struct PromptShared {
   uint32_t u_begin, u_end, size;  // the share, and how many units one has
 };
 
+// Whether the last CTA of a cut item adds its parts up.  Of kBegin items with many, kv_parts_k does.
+template <int MODE>
+__device__ __forceinline__ bool few_parts(int first_cta, int last_cta) {
+  return MODE != kBegin || last_cta - first_cta < 3;
+}
+
 // Counts a part of an item that CTAs first .. last share; the last one to come sets the counter back.
 __device__ __forceinline__ bool count_part(unsigned *counter, int first, int last) {
   const bool done = atomicAdd(counter, 1u) == (unsigned)(last - first);
@@ -301,13 +307,13 @@ __device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned 
   Segment &g = sh.seg[0];
   while (walk.next(a, sh.size, g))
     for (int i = 0; i < 2; ++i)
-      if (!g.whole() && g.s.n * a.group > g.rt * kRows + 128 * i && !sh.counted[i][g.k0 == 0])
+      if (!g.whole() && few_parts<MODE>(g.first_cta, g.last_cta) && g.s.n * a.group > g.rt * kRows + 128 * i && !sh.counted[i][g.k0 == 0])
         count_part(&counters[2 * g.first_cta + i], g.first_cta, g.last_cta);
 }
 
 template <bool BF16, int DIM, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters, const PromptSlot *begun) {
+    kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters) {
   extern __shared__ uint8_t smem_raw[];
   using Shared = PromptShared<DIM>;
   Shared &sh = *reinterpret_cast<Shared *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -694,8 +700,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) {  // (the slot keeps whatever it holds: the status word says that the result is not valid)
       } else if (whole) {
         const float2 y = kv_norm(vref, l);
+        float2 shares = make_float2(0.f, 1.f);
+        if (joins && real) shares = kv_join(a, at, m, l * kPromptToPart);
 #pragma unroll 1
         for (int h = 0; h < DIM / 32; ++h) {
+          float4 u[8];
+          if (joins && real) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = __ldcg(reinterpret_cast<const float4 *>(kv_part(a, at) + 32 * h) + k);
+          }
           float o[32];
           tmem_ld32(o_at + 32 * h, o);
           tmem_ld_wait();
@@ -713,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __stcg(to + 1, make_float4(f[4], f[5], f[6], f[7]));
                 continue;
               }
-              if (joins) kv_join(a, begun, at, 32 * h + k, f, m, l * kPromptToPart);
+              if (joins) kv_joined(shares, u[k / 4], u[k / 4 + 1], f);
               store8(out + 32 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
@@ -736,12 +749,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         __stcg(&slot.m[row], m);
         __stcg(&slot.l[row], l);
         if (row == 0) __stcg(&slot.vref, vref);
-        if (MODE == kBegin && head_part && real) {  // (the parts are joined where they are used, by many CTAs)
+        if (MODE == kBegin && !few_parts<MODE>(first_cta, last_cta) && head_part && real) {
           __stcg(reinterpret_cast<int4 *>(kv_part(a, at)), make_int4(first_cta, last_cta, 128 * i + row, 0));
           __stcg(kv_part_sums(a, at), make_float2(0.f, -1.f));
         }
       }
-      if (MODE != kBegin && !whole) {
+      if (!whole && few_parts<MODE>(first_cta, last_cta)) {
         wg_sync(1 + i);
         if (row == 0) {
           __threadfence();  // (the four warps' writes, which the barrier has put before this)
@@ -753,6 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         wg_sync(1 + i);
         if (sh.last[i] && real && ok) {
           float top = -INFINITY, t = -INFINITY, sum = 0.f;
+          float2 shares = make_float2(0.f, 1.f);
           // (several parts' loads at once: a short call over a long cache has many)
 #pragma unroll 4
           for (int z = first_cta; z <= last_cta; ++z) {
@@ -780,12 +794,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             const float2 y = kv_norm(fast_exp2(t - top), sum);
+            if (joins && h == 0) shares = kv_join(a, at, top, sum * kPromptToPart);
+            if (MODE == kBegin && h == 0) __stcg(kv_part_sums(a, at), make_float2(top, sum * kPromptToPart));
 #pragma unroll
             for (int k = 0; k < 64; k += 8) {
               float f[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) f[j] = x[k + j] * y.x * y.y;
-              if (joins) kv_join(a, begun, at, 64 * h + k, f, top, sum * kPromptToPart);
+              float4 *part = reinterpret_cast<float4 *>(kv_part(a, at) + 64 * h + k);
+              if (MODE == kBegin) {
+                __stcg(part, make_float4(f[0], f[1], f[2], f[3]));
+                __stcg(part + 1, make_float4(f[4], f[5], f[6], f[7]));
+                continue;
+              }
+              if (joins) kv_joined(shares, __ldcg(part), __ldcg(part + 1), f);
               store8(out + 64 * h + k, pack8<BF16>(f), a.out.vec);
             }
           }
@@ -821,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       key_next = kNoKey;
       if (lane < kTileBlocks && t < g->k1 && bi < g->r.blocks) {
         key_next = (bi < g->r.sink_blocks ? bi : bi - g->r.sink_blocks + g->r.first_block) * kKvBlock;
-        page_next = a.seqs.pages[kv_page_row<MODE>(a, g->b) + fast_div(key_next, a.by_page)];  // (in the row: kv_span has checked)
+        page_next = a.seqs.pages[kv_page_at<MODE>(a, g->s, g->b, key_next, fast_div(key_next, a.by_page))];  // (in the row: kv_span has checked)
       }
     };
     auto look_up = [&]() {
@@ -1030,9 +1052,64 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
-  } else if (MODE != kBegin && threadIdx.x == 0 && sh.abort) {
+  } else if (threadIdx.x == 0 && sh.abort) {
     count_rest<MODE>(a, sh, counters);
   }
+}
+
+// The parts of items that kBegin cut among many CTAs, added up in the order of their
+// keys: eight rows a block, a thread four elements of one.  (A few rows over long
+// beginnings have a part in every CTA; with 18 parts of 256 rows, the last CTA alone
+// took as long for them as for the keys.)
+constexpr int kPartsMost = 256;  // CTAs that a launch has at most
+template <int DIM>
+__global__ void __launch_bounds__(2 * DIM) kv_parts_k(const __grid_constant__ KvAttend a, const PromptSlot *slots, int ctas) {
+  __shared__ float ms[8][kPartsMost + 1], ls[8][kPartsMost + 1], ts[8][kPartsMost + 1];
+  constexpr int kThreadsRow = DIM / 4, kAtOnce = 8;
+  const int rr = threadIdx.x & 7, c = threadIdx.x >> 3;
+  const long long row = (long long)blockIdx.x * 8 + rr;
+  pdl_wait_and_release();
+  const bool marked = row < a.seqs.tokens * a.q_heads && __ldcg(kv_part_sums(a, row)).y == -1.f;
+  if (!__syncthreads_or(marked)) return;
+  const int4 w = marked ? __ldcg(reinterpret_cast<const int4 *>(kv_part(a, row))) : make_int4(0, -1, 0, 0);
+  // (rows of no group are as the caller left them)
+  const bool there = marked && w.x >= 0 && w.y >= w.x && w.y < ctas && (unsigned)w.z < kRows;
+  const int i = w.z >> 7, r = w.z & 127, parts = there ? w.y - w.x + 1 : 0;
+  auto slot = [&](int k) -> const PromptSlot & { return slots[2 * (2 * (w.x + k) + (k == 0 ? 1 : 0)) + i]; };
+  auto load = [&](int k) {
+    return k < parts ? __ldcg(reinterpret_cast<const float4 *>(&slot(k).acc[(c * 128 + r) * 4])) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float4 u[kAtOnce];
+#pragma unroll
+  for (int k = 0; k < kAtOnce; ++k) u[k] = load(k);
+  for (int k = c; k < parts; k += kThreadsRow) {
+    const float zm = __ldcg(&slot(k).m[r]);
+    ms[rr][k] = zm;
+    ls[rr][k] = __ldcg(&slot(k).l[r]);
+    ts[rr][k] = zm + log2_of(__ldcg(&slot(k).vref));
+  }
+  __syncthreads();  // (also: every thread has read the row's marks)
+  if (!there) return;
+  float m = -INFINITY, t = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < parts; ++k) {
+    m = fmaxf(m, ms[rr][k]);
+    t = fmaxf(t, ts[rr][k]);
+  }
+  for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (k0 + k < parts) {
+        const float zm = ms[rr][k0 + k], zl = ls[rr][k0 + k], wv = kv_share(ts[rr][k0 + k], t);
+        if (zm != -INFINITY || zl != 0.f) l += kv_scaled(zl, zm - m);
+        o[0] += u[k].x * wv, o[1] += u[k].y * wv, o[2] += u[k].z * wv, o[3] += u[k].w * wv;
+      }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) u[k] = load(k0 + kAtOnce + k);
+  }
+  const float2 y = kv_norm(fast_exp2(t - m), l);
+  __stcg(reinterpret_cast<float4 *>(kv_part(a, row) + 4 * c),
+         make_float4(o[0] * y.x * y.y, o[1] * y.x * y.y, o[2] * y.x * y.y, o[3] * y.x * y.y));
+  if (c == 0) __stcg(kv_part_sums(a, row), make_float2(m, l * kPromptToPart));
 }
 
 template <bool BF16, int DIM, int MODE>
@@ -1042,9 +1119,8 @@ cudaError_t launch_prompt(const KvAttend &a, void *workspace, int sms, cudaStrea
   const cudaError_t e = ensure_dynamic_smem(kv_prompt_k<BF16, DIM, MODE>, bytes, attr_set);
   if (e != cudaSuccess) return e;
   PromptSlot *const slots = reinterpret_cast<PromptSlot *>(static_cast<uint8_t *>(workspace) + kKvCounterBytes);
-  return launch_kernel(kv_prompt_k<BF16, DIM, MODE>, dim3(sms), dim3(kThreads), (size_t)bytes, st, a,
-                       MODE == kRest ? slots + 4 * (size_t)sms : slots, static_cast<unsigned *>(workspace),
-                       static_cast<const PromptSlot *>(slots));
+  return launch_kernel(kv_prompt_k<BF16, DIM, MODE>, dim3(sms), dim3(kThreads), (size_t)bytes, st, a, slots,
+                       static_cast<unsigned *>(workspace));
 }
 
 template <int MODE>
@@ -1057,6 +1133,14 @@ cudaError_t launch_mode(bool bf16, const KvAttend &a, void *workspace, int sms, 
 }  // namespace
 
 size_t kv_prompt_workspace_bytes(int sms) { return sizeof(PromptSlot) * 4 * (size_t)sms; }
+
+cudaError_t launch_kv_parts(const KvAttend &a, const void *workspace, int sms, cudaStream_t st) {
+  if (sms > kPartsMost) return cudaErrorInvalidValue;
+  const PromptSlot *slots = reinterpret_cast<const PromptSlot *>(static_cast<const uint8_t *>(workspace) + kKvCounterBytes);
+  const unsigned grid = (unsigned)((a.seqs.tokens * a.q_heads + 7) / 8);
+  if (a.cache.dim == 64) return launch_kernel(kv_parts_k<64>, dim3(grid), dim3(128), 0, st, a, slots, sms);
+  return launch_kernel(kv_parts_k<128>, dim3(grid), dim3(256), 0, st, a, slots, sms);
+}
 
 bool kv_prompt_takes(const KvAttend &a) { return a.seqs.batch <= kMaxSeqs; }
 
