@@ -56,6 +56,7 @@ struct KvAttend {
   // groups of sequences with a common beginning (kv_attend.cuh, KvMode)
   const int32_t *first, *shared;
   int groups, sequences;
+  int many_parts;  // a launch of launch_kv_parts follows
   float *scratch;
 };
 

@@ -682,8 +682,10 @@ cudaError_t launch_shared(const KvAttend &a, void *workspace, int sms, cudaStrea
   if (own <= 64 && keys * a.cache.heads * 2 * DIM <= kOnePass) return launch_step_rows<BF16, DIM, kOne>(a, own, workspace, sms, st);
   cudaError_t e;
   if (rows > 64 && kv_prompt_takes(b)) {
+    // Items of 256 rows: fewer than CTAs, and an item is cut over several of them.
+    b.many_parts = (a.seqs.tokens * a.group + 255) / 256 * a.cache.heads < sms;
     e = launch_kv_prompt(BF16, kBegin, b, workspace, sms, st);
-    if (e == cudaSuccess) e = launch_kv_parts(a, workspace, sms, st);
+    if (e == cudaSuccess && b.many_parts) e = launch_kv_parts(a, workspace, sms, st);
   } else {
     e = launch_step_rows<BF16, DIM, kBegin>(b, rows, workspace, sms, st);
   }

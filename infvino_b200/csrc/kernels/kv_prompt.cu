@@ -180,8 +180,8 @@ struct PromptShared {
 
 // Whether the last CTA of a cut item adds its parts up.  Of kBegin items with many, kv_parts_k does.
 template <int MODE>
-__device__ __forceinline__ bool few_parts(int first_cta, int last_cta) {
-  return MODE != kBegin || last_cta - first_cta < 3;
+__device__ __forceinline__ bool few_parts(const KvAttend &a, int first_cta, int last_cta) {
+  return MODE != kBegin || !a.many_parts || last_cta - first_cta < 3;
 }
 
 // Counts a part of an item that CTAs first .. last share; the last one to come sets the counter back.
@@ -307,7 +307,7 @@ __device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned 
   Segment &g = sh.seg[0];
   while (walk.next(a, sh.size, g))
     for (int i = 0; i < 2; ++i)
-      if (!g.whole() && few_parts<MODE>(g.first_cta, g.last_cta) && g.s.n * a.group > g.rt * kRows + 128 * i && !sh.counted[i][g.k0 == 0])
+      if (!g.whole() && few_parts<MODE>(a, g.first_cta, g.last_cta) && g.s.n * a.group > g.rt * kRows + 128 * i && !sh.counted[i][g.k0 == 0])
         count_part(&counters[2 * g.first_cta + i], g.first_cta, g.last_cta);
 }
 
@@ -749,12 +749,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         __stcg(&slot.m[row], m);
         __stcg(&slot.l[row], l);
         if (row == 0) __stcg(&slot.vref, vref);
-        if (MODE == kBegin && !few_parts<MODE>(first_cta, last_cta) && head_part && real) {
+        if (MODE == kBegin && !few_parts<MODE>(a, first_cta, last_cta) && head_part && real) {
           __stcg(reinterpret_cast<int4 *>(kv_part(a, at)), make_int4(first_cta, last_cta, 128 * i + row, 0));
           __stcg(kv_part_sums(a, at), make_float2(0.f, -1.f));
         }
       }
-      if (!whole && few_parts<MODE>(first_cta, last_cta)) {
+      if (!whole && few_parts<MODE>(a, first_cta, last_cta)) {
         wg_sync(1 + i);
         if (row == 0) {
           __threadfence();  // (the four warps' writes, which the barrier has put before this)

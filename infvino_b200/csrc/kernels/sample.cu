@@ -8,10 +8,14 @@
 // one that is goes by sums next to a border, so weights and sums are in 64 bits,
 // added in an order that is fixed for a size and a number of rows.
 //
-// A row belongs to a cluster of CTAs, each with a slice of it in shared memory.
-// A cut is found by counting logits in bins of equal width and looking closer at
-// the bin where it must be: up to kList of them are put in order, more of them are
-// binned again, equal ones by their numbers.
+// Two kernels.  sample_count_k, for logits in 16 bits: a CTA a row counts how often
+// each of the 65536 values occurs, in shared memory.  A value's weight is then worked
+// out once for all its tokens, every cut follows from the counts, and only tokens
+// that are kept are weighed one by one, where the running sums need them.
+// sample_k, for the others and for few long rows: a cluster of CTAs a row, each with
+// a slice of it in shared memory.  It counts logits in bins of equal width, up to the
+// bin where the cut must be; if these are at most kList, one CTA puts them in order
+// and does the rest; if not, the bin is binned again, equal logits by their numbers.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -31,20 +35,46 @@ constexpr int kBins = 2048, kList = 1024;
 constexpr int kMaxRanks = 8;
 constexpr double kFar = 41.588830833596715;  // 60 ln 2: what is further below the largest has no weight
 
+// 2^(j / 64), j below 64, by the first threads of a block.
+constexpr int kPowers = 64;
+__device__ __forceinline__ void fill_powers(double *powers) {
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2(threadIdx.x / (double)kPowers);
+}
+// e^((v - top) / T) with by = 64 log2(e) / T: 2^(n / 64) from the table, and the first
+// terms of the series of 2^(r / 64), r at most a half (the rest is below 2^-44 of it).
+__device__ __forceinline__ double weight_of(float v, float top, double by, const double *powers) {
+  if (v == top) return 1.0;
+  const double t = ((double)v - (double)top) * by;
+  if (!(t > -60.0 * kPowers)) return 0.0;
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: what is added to it is rounded to a whole number
+  const double s = t + kRound;
+  const double r = t - (s - kRound);
+  const int n = __double2loint(s);
+  constexpr double c = 0.6931471805599453 / kPowers;
+  double p = c * c * c * c / 24.0;
+  p = fma(p, r, c * c * c / 6.0);
+  p = fma(p, r, c * c / 2.0);
+  p = fma(p, r, c);
+  p = fma(p, r, 1.0);
+  const double w = p * powers[n & (kPowers - 1)];
+  return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
+}
+
 struct Cut {  // kept: x > this one's, or x equal and number at most this one's
   float x;
   int i;
 };
 
 struct SampleShared {
+  double powers[kPowers];
   unsigned hist[kBins];
   unsigned long long key[kList];  // (order of x, number), rising
-  double mass[kList];
+  double mass[kList], wt[kList];  // running sums, weights
   double part[2][kMaxRanks][2];   // what CTAs tell one another, two exchanges in turn
   double red[2][kWarps];
   unsigned cnt[kWarps];
   unsigned listed;
-  int found;
+  int found, kept, reached;
   unsigned before, in_bin;
   Cut cut;
   double seg[kWarps];
@@ -62,15 +92,38 @@ __device__ __forceinline__ float logit(T v) {
   float x = (float)v;
   return x != x ? -INFINITY : x + 0.f;  // (-0 is 0)
 }
+// What a row asks for.
+struct Want {
+  int k;               // 0: all
+  float t, p, min_p, u;
+  __device__ __forceinline__ Want(const Sample &a, long long r) {
+    t = a.temperature ? a.temperature[r] : 1.f;
+    k = a.top_k ? a.top_k[r] : 0;
+    k = !(t > 0.f) ? 1 : k > 0 && k < a.vocab ? k : 0;
+    p = a.top_p && t > 0.f ? fmaxf(a.top_p[r], 0.f) : 1.f;
+    if (!(a.top_p && a.top_p[r] < 1.f)) p = 1.f;
+    min_p = a.min_p ? a.min_p[r] : 0.f;
+    u = a.u[r];
+    u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  }
+  // Logits below this weigh less than min_p, by more than any rounding.
+  __device__ __forceinline__ float floor(float top) const {
+    if (!(min_p > 0.f) || !(t > 0.f)) return -INFINITY;
+    const double x = (double)top + (fmin(log((double)min_p), 0.0) - 1e-6) * (double)t;
+    return (float)(x - 2e-7 * fabs(x));
+  }
+  __device__ __forceinline__ bool enough(double w, bool top) const { return !(min_p > 0.f) || top || w >= (double)min_p; }
+};
 
 template <class T>
 struct Row {
   SampleShared &sh;
   const T *x;      // this CTA's slice
+  bool vec;        // on 16 bytes
   int n, first;    // its length, the number of its first token
   int ranks, rank;
   float top;       // the largest logit
-  double inv_t;
+  double by;       // 64 log2(e) / T
   Cut cut;
   int turn = 0;    // of `part`
 
@@ -87,11 +140,7 @@ struct Row {
     return ranks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
   }
 
-  __device__ __forceinline__ double weight(float v) const {
-    if (v == top) return 1.0;
-    const double z = ((double)v - (double)top) * inv_t;
-    return z > -kFar ? exp(z) : 0.0;
-  }
+  __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, by, sh.powers); }
   __device__ __forceinline__ bool keeps(float v, int i) const { return v > cut.x || (v == cut.x && i <= cut.i); }
 
   // Sum (or maximum) of a and b over the cluster, to all its threads.
@@ -124,10 +173,31 @@ struct Row {
     }
   }
 
-  // f(logit, number) for each of the slice.
+  // Four logits from j on (a multiple of 4; -inf behind the slice's end).
+  __device__ __forceinline__ void load4(int j, float (&v)[4]) const {
+    T t[4];
+    if (vec && j + 3 < n) {
+      if (sizeof(T) == 4)
+        *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(x + j);
+      else
+        *reinterpret_cast<uint2 *>(t) = *reinterpret_cast<const uint2 *>(x + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = logit(t[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = j + i < n ? logit(x[j + i]) : -INFINITY;
+    }
+  }
+  // f(logit, number) for each of the slice (and for some -inf behind it).
   template <class F>
   __device__ __forceinline__ void each(F &&f) {
-    for (int j = threadIdx.x; j < n; j += kThreads) f(logit(x[j]), first + j);
+#pragma unroll 2
+    for (int j = 4 * threadIdx.x; j < n; j += 4 * kThreads) {
+      float v[4];
+      load4(j, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f(v[i], first + j + i);
+    }
   }
 
   // Counts into sh.hist, over the cluster, what bin(logit, number) says (below 0: nothing).
@@ -221,6 +291,7 @@ struct Row {
     return n;
   }
 
+  // Rising, padded with ~0 to a power of two.  Steps over at most 32 stay inside a warp's 64 keys.
   __device__ void sort(unsigned n) {
     unsigned size = 2;
     while (size < n) size <<= 1;
@@ -233,8 +304,99 @@ struct Row {
           const unsigned long long s = sh.key[a], t = sh.key[b];
           if ((s > t) == ((a & k) == 0)) sh.key[a] = t, sh.key[b] = s;
         }
-        __syncthreads();
+        if (j > 32 || (j == 1 && k >= 64))
+          __syncthreads();
+        else
+          __syncwarp();
       }
+    __syncthreads();
+  }
+
+  // Running sums of two doubles a thread over the block, and their total.
+  __device__ __forceinline__ double scan(double &x0, double &x1) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    double s = x0 + x1;
+    const double mine = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    __syncthreads();
+    if (lane == 31) sh.red[0][warp] = s;
+    __syncthreads();
+    double before = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) before = all;
+      all += sh.red[0][w];
+    }
+    const double a0 = x0;
+    x0 = before + (s - mine) + a0;
+    x1 = before + s;
+    return all;
+  }
+
+  // Of the n logits in sh.key, in order: what is kept, and the token; CTA 0.  mass: of
+  // all tokens (top_p of them is meant where there is no top_k).  False: top_p is not reached.
+  __device__ bool finish(unsigned n, const Want &want, double mass, const Sample &a, long long r) {
+    static_assert(kList == 2 * kThreads, "two a thread");
+    const int e0 = 2 * threadIdx.x;
+    double w[2], c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = e0 + i < (int)n ? weight(from_falling((uint32_t)(sh.key[e0 + i] >> 32))) : 0.0;
+      sh.wt[e0 + i] = w[i];
+      c[i] = w[i];
+    }
+    scan(c[0], c[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sh.mass[e0 + i] = c[i];
+    const int m = want.k ? min(want.k, (int)n) : (int)n;
+    if (threadIdx.x == 0) sh.kept = m, sh.reached = 0;
+    __syncthreads();
+    if (want.p < 1.f) {
+      const double target = (double)want.p * (want.k ? sh.mass[m - 1] : mass);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (e0 + i < (int)n && c[i] >= target) {
+          atomicMin(&sh.kept, e0 + i + 1);
+          sh.reached = 1;
+          break;
+        }
+    }
+#pragma unroll
+    for (int i = 1; i >= 0; --i)
+      if (e0 + i < (int)n && !want.enough(w[i], from_falling((uint32_t)(sh.key[e0 + i] >> 32)) == top)) atomicMin(&sh.kept, e0 + i);
+    __syncthreads();
+    if (want.p < 1.f && !want.k && !sh.reached) return false;
+    const unsigned kept = (unsigned)sh.kept;
+    // by number
+    unsigned long long by_number[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) by_number[i] = (sh.key[e0 + i] << 32) | (unsigned)(e0 + i);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (e0 + i < (int)kept) sh.key[e0 + i] = by_number[i];
+    if (threadIdx.x == 0) sh.found = (int)kept - 1;
+    __syncthreads();
+    sort(kept);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c[i] = e0 + i < (int)kept ? sh.wt[(uint32_t)sh.key[e0 + i]] : 0.0;
+    const double all = scan(c[0], c[1]), target = (double)want.u * all;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (e0 + i < (int)kept && c[i] > target) {
+        atomicMin(&sh.found, e0 + i);
+        break;
+      }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const unsigned long long key = sh.key[sh.found];
+      a.tokens[r] = (int)(key >> 32);
+      if (a.probs) a.probs[r] = (float)(sh.wt[(uint32_t)key] / all);
+    }
+    return true;
   }
 
   // CTA 0's choice becomes every CTA's cut.
@@ -265,6 +427,24 @@ struct Row {
     cut_at(sh.key[at]);
   }
 
+  // Bins of equal width from hi down to lo; -1 for what is outside, or not kept.
+  struct Bins {
+    float hi, lo, fscale;
+    double scale;
+    bool wide;
+    __device__ __forceinline__ Bins(float h, float l) : hi(h), lo(l) {
+      scale = kBins * 0.99999 / ((double)h - (double)l);
+      fscale = (float)scale;
+      wide = !(fscale < 1e30f && fscale > 1e-30f && h - l < 1e30f);
+    }
+    __device__ __forceinline__ int operator()(float v) const {
+      if (v > hi || v < lo) return -1;
+      const float b = wide ? (float)(((double)hi - (double)v) * scale) : (hi - v) * fscale;
+      return min(kBins - 1, (int)b);
+    }
+    __device__ __forceinline__ float middle(int k) const { return (float)fmin((double)hi - (k + 0.5) / scale, (double)hi); }
+  };
+
   // Cuts where `target` is reached: of how many are kept (COUNT) or of what they weigh.
   template <bool COUNT>
   __device__ void select(double target, float least, int vocab) {
@@ -278,14 +458,8 @@ struct Row {
         cut_equal(hi, (unsigned)fmin(fmax(r, 1.0), 2147483647.0), vocab);
         return;
       }
-      const double scale = kBins * 0.99999 / ((double)hi - (double)lo);
-      const float fhi = hi, fscale = (float)scale;
-      const bool wide = !(fscale < 1e30f && fscale > 1e-30f && hi - lo < 1e30f);
-      auto bin = [&](float v, int i) {
-        if (v > hi || v < lo || !keeps(v, i)) return -1;
-        const float b = wide ? (float)(((double)hi - (double)v) * scale) : (fhi - v) * fscale;
-        return min(kBins - 1, (int)b);
-      };
+      const Bins bins(hi, lo);
+      auto bin = [&](float v, int i) { return keeps(v, i) ? bins(v) : -1; };
       count(bin);
       int b;
       if (COUNT) {
@@ -295,7 +469,7 @@ struct Row {
         base += sh.before;
       } else {
         // a guess by the weights of the bins' middles, then sums
-        find(target - base, [&](int k) { return sh.hist[k] ? sh.hist[k] * exp(fmax(((double)hi - (k + 0.5) / scale - top) * inv_t, -kFar)) : 0.0; });
+        find(target - base, [&](int k) { return sh.hist[k] ? sh.hist[k] * weight(bins.middle(k)) : 0.0; });
         b = sh.found;
         int from = 0, to = kBins - 1;
         for (int tries = 0;; ++tries) {
@@ -360,132 +534,219 @@ struct Row {
       hi = (float)h, lo = (float)-l;
     }
   }
+
+  // The row's token.  x, n, first, ranks and rank are set, sh.powers filled, high the
+  // largest logit and low the smallest above -inf negated, of the whole row.
+  __device__ void run(const Sample &a, long long r, double high, double low) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    top = (float)high;
+    const bool writes = rank == 0 && threadIdx.x == 0;
+    if (high == -INFINITY) {
+      if (writes) {
+        a.tokens[r] = -1;
+        if (a.probs) a.probs[r] = 0.f;
+      }
+      return;
+    }
+    const Want want(a, r);
+    if (!(want.t > 0.f)) {
+      double best = -INFINITY, none = 0;
+      each([&](float v, int i) {
+        if (v == top) best = fmax(best, -(double)i);
+      });
+      reduce<true>(best, none);
+      if (writes) {
+        a.tokens[r] = (int)-best;
+        if (a.probs) a.probs[r] = 1.f;
+      }
+      return;
+    }
+    by = kPowers * 1.4426950408889634 / (double)want.t;
+    cut = Cut{-INFINITY, -1};  // (-inf weighs nothing)
+    // logits below this have no weight
+    const float least = high == INFINITY ? top : (float)fmax(-low, high - kFar * (double)want.t);
+    double mass = 0, none = 0;
+    if (want.p < 1.f && !want.k) {
+      each([&](float v, int) { mass += v > -INFINITY ? weight(v) : 0.0; });
+      reduce<false>(mass, none);
+    }
+    if ((want.p < 1.f || want.k) && want.k <= kList && least < top) {
+      // what is kept, if it is not much, goes through one list
+      const Bins bins(top, least);
+      count([&](float v, int) { return bins(v); });
+      if (want.k)
+        find((double)want.k, [&](int b) { return (double)sh.hist[b]; });
+      else
+        find((double)want.p * mass, [&](int b) { return sh.hist[b] ? sh.hist[b] * weight(bins.middle(b)) : 0.0; });
+      int b = sh.found;
+      unsigned many = sh.before + sh.in_bin;
+      if (!want.k) {  // (the bins' middles are a guess: two more)
+        for (int more = 0; more < 2 && b + 1 < kBins; ++more) many += sh.hist[++b];
+      }
+      __syncthreads();
+      if (many <= kList) {
+        const unsigned n = gather([&](float v, int) { return (unsigned)bins(v) <= (unsigned)b; });
+        bool done = true;
+        if (rank == 0) done = finish(n, want, mass, a, r);
+        if (want.k) return;
+        if (rank == 0 && threadIdx.x < ranks) *at(&sh.reached, (int)threadIdx.x) = done;
+        sync();
+        if (sh.reached) return;
+      }
+    }
+    if (want.k) select<true>((double)want.k, least, a.vocab);
+    if (want.p < 1.f) {
+      if (want.k) {
+        mass = 0;
+        each([&](float v, int i) { mass += keeps(v, i) ? weight(v) : 0.0; });
+        reduce<false>(mass, none);
+      }
+      select<false>((double)want.p * mass, least, a.vocab);
+    }
+    // ---- running sums, by number: a warp has a piece of the slice, in steps of 128
+    const float lowest = want.floor(top);
+    auto kept = [&](float v, int i) {
+      if (!keeps(v, i) || v < lowest) return 0.0;
+      const double w = weight(v);
+      return want.enough(w, v == top) ? w : 0.0;
+    };
+    const int piece = (a.slice + 128 * kWarps - 1) / (128 * kWarps) * 128;
+    const int j0 = min(warp * piece, n), j1 = min(j0 + piece, n);
+    double mine = 0;
+    for (int j = j0 + 4 * lane; j < j1; j += 128) {
+      float v[4];
+      load4(j, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine += kept(v[i], first + j + i);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sh.seg[warp] = mine;
+    __syncthreads();
+    mass = threadIdx.x < kWarps ? sh.seg[threadIdx.x] : 0.0;
+    reduce<false>(mass, none);
+    const double target = (double)want.u * mass;
+    // the CTA, then the warp, where the sum passes the target
+    double before = 0;
+    int q = 0;
+    for (; q + 1 < ranks; ++q) {
+      const double s = sh.part[turn][q][0];
+      if (before + s > target) break;
+      before += s;
+    }
+    // (a last CTA without weight, by a rounding: the last one with some)
+    while (q > 0 && sh.part[turn][q][0] == 0) --q;
+    if (q != rank) return;
+    int w = 0;
+    for (; w + 1 < kWarps; ++w) {
+      if (before + sh.seg[w] > target) break;
+      before += sh.seg[w];
+    }
+    while (w > 0 && sh.seg[w] == 0) --w;
+    if (w != warp) return;
+    int token = -1;
+    double share = 0;
+    for (int j = j0; j < j1; j += 128) {
+      float v[4];
+      double c[4], s = 0;
+      load4(j + 4 * lane, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = j + 4 * lane < j1 ? kept(v[i], first + j + 4 * lane + i) : 0.0, s += c[i];
+      const double sum = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += x;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, sum > 0), over = __ballot_sync(0xffffffffu, sum > 0 && before + s > target);
+      if (some) {
+        const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
+        // the last of the lane's that weighs something, or the first that passes
+        double run = before + (s - sum);
+        int at = -1;
+        double sh_at = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (c[i] > 0 && (at < 0 || !(run > target))) at = i, sh_at = c[i];
+          run += c[i];
+        }
+        token = __shfl_sync(0xffffffffu, first + j + 4 * lane + at, l);
+        share = __shfl_sync(0xffffffffu, sh_at, l);
+      }
+      if (over) break;
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) {
+      a.tokens[r] = token;
+      if (a.probs) a.probs[r] = (float)(share / mass);
+    }
+  }
 };
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) sample_k(const __grid_constant__ Sample a) {
   extern __shared__ __align__(16) uint8_t slice_raw[];
   __shared__ SampleShared sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Row<T> row(sh);
   row.ranks = a.ranks;
   row.rank = a.ranks > 1 ? (int)(blockIdx.x % a.ranks) : 0;
   const long long r = blockIdx.x / a.ranks;
   row.first = min(row.rank * a.slice, a.vocab);
   row.n = min(a.slice, a.vocab - row.first);
+  fill_powers(sh.powers);
   pdl_wait_and_release();
   const T *x = static_cast<const T *>(a.x) + r * a.stride + row.first;
   row.x = x;
-  double high = -INFINITY, low = -INFINITY;  // the largest logit, and the smallest above -inf negated
-  for (int j = threadIdx.x; j < row.n; j += kThreads) {
-    const T v = x[j];
-    if (a.resident) reinterpret_cast<T *>(slice_raw)[j] = v;
+  row.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  float high = -INFINITY, low = -INFINITY;  // the largest logit, and the smallest above -inf negated
+  T *const slice = reinterpret_cast<T *>(slice_raw);
+  constexpr int kEach = 16 / sizeof(T);
+  auto look = [&](T v) {
     const float f = logit(v);
-    high = fmax(high, (double)f);
-    if (f > -INFINITY) low = fmax(low, -(double)f);
-  }
-  if (a.resident) row.x = reinterpret_cast<const T *>(slice_raw);
-  row.template reduce<true>(high, low);  // (and the slice is in place)
-  row.top = (float)high;
-  const bool writes = row.rank == 0 && threadIdx.x == 0;
-  if (high == -INFINITY) {
-    if (writes) {
-      a.tokens[r] = -1;
-      if (a.probs) a.probs[r] = 0.f;
-    }
-    return;
-  }
-  const float t = a.temperature ? a.temperature[r] : 1.f;
-  if (!(t > 0.f)) {
-    double best = -INFINITY, none = 0;
-    row.each([&](float v, int i) {
-      if (v == row.top) best = fmax(best, -(double)i);
-    });
-    row.template reduce<true>(best, none);
-    if (writes) {
-      a.tokens[r] = (int)-best;
-      if (a.probs) a.probs[r] = 1.f;
-    }
-    return;
-  }
-  row.inv_t = 1.0 / (double)t;
-  row.cut = Cut{-INFINITY, -1};  // (-inf weighs nothing)
-  // logits below this have no weight
-  const float least = high == INFINITY ? row.top : (float)fmax(-low, high - kFar * (double)t);
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f, min_p = a.min_p ? a.min_p[r] : 0.f;
-  if (k > 0 && k < a.vocab) row.template select<true>((double)k, least, a.vocab);
-  if (p < 1.f) {
-    double z = 0, none = 0;
-    row.each([&](float v, int i) { z += row.keeps(v, i) ? row.weight(v) : 0.0; });
-    row.template reduce<false>(z, none);
-    row.template select<false>(fmax((double)p, 0.0) * z, least, a.vocab);
-  }
-  // ---- running sums, by number: a warp has a piece of the slice
-  auto kept = [&](float v, int i) {
-    if (!row.keeps(v, i)) return 0.0;
-    const double w = row.weight(v);
-    return w >= (double)min_p || v == row.top || !(min_p > 0.f) ? w : 0.0;
+    high = fmaxf(high, f);
+    if (f > -INFINITY) low = fmaxf(low, -f);
   };
-  const int piece = (a.slice + kThreads - 1) / kThreads * 32;
-  const int j0 = min(warp * piece, row.n), j1 = min(j0 + piece, row.n);
-  double mine = 0;
-  for (int j = j0 + lane; j < j1; j += 32) mine += kept(logit(row.x[j]), row.first + j);
+  if (row.vec && a.resident) {
+    constexpr int kAtOnce = 4;
+    for (int j0 = threadIdx.x * kEach; j0 < row.n; j0 += kAtOnce * kThreads * kEach) {
+      uint4 w[kAtOnce];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sh.seg[warp] = mine;
-  __syncthreads();
-  double mass = threadIdx.x < kWarps ? sh.seg[threadIdx.x] : 0.0, none = 0;
-  row.template reduce<false>(mass, none);
-  float u = a.u[r];
-  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  const double target = (double)u * mass;
-  // the CTA, then the warp, where the sum passes the target
-  double before = 0;
-  int rank = 0;
-  for (; rank + 1 < a.ranks; ++rank) {
-    const double s = sh.part[row.turn][rank][0];
-    if (before + s > target) break;
-    before += s;
-  }
-  // (a last CTA without weight, by a rounding: the last one with some)
-  while (rank > 0 && sh.part[row.turn][rank][0] == 0) --rank;
-  if (rank != row.rank) return;
-  int w = 0;
-  for (; w + 1 < kWarps; ++w) {
-    if (before + sh.seg[w] > target) break;
-    before += sh.seg[w];
-  }
-  while (w > 0 && sh.seg[w] == 0) --w;
-  if (w != warp) return;
-  int token = -1;
-  double share = 0;
-  for (int j = j0; j < j1; j += 32) {
-    const double v = j + lane < j1 ? kept(logit(row.x[j + lane]), row.first + j + lane) : 0.0;
-    double s = v;
+      for (int q = 0; q < kAtOnce; ++q)
+        if (j0 + q * kThreads * kEach + kEach <= row.n) w[q] = __ldg(reinterpret_cast<const uint4 *>(x + j0 + q * kThreads * kEach));
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double q = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += q;
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int j = j0 + q * kThreads * kEach;
+        if (j + kEach <= row.n) {
+          *reinterpret_cast<uint4 *>(slice + j) = w[q];
+          T t[kEach];
+          *reinterpret_cast<uint4 *>(t) = w[q];
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) look(t[i]);
+        } else {
+          for (int i = j; i < row.n; ++i) {
+            const T v = x[i];
+            slice[i] = v;
+            look(v);
+          }
+        }
+      }
     }
-    const unsigned some = __ballot_sync(0xffffffffu, v > 0), over = __ballot_sync(0xffffffffu, v > 0 && before + s > target);
-    if (some) {
-      const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
-      token = row.first + j + l;
-      share = __shfl_sync(0xffffffffu, v, l);
+  } else {
+    for (int j = threadIdx.x; j < row.n; j += kThreads) {
+      const T v = x[j];
+      if (a.resident) slice[j] = v;
+      look(v);
     }
-    if (over) break;
-    before += __shfl_sync(0xffffffffu, s, 31);
   }
-  if (lane == 0) {
-    a.tokens[r] = token;
-    if (a.probs) a.probs[r] = (float)(share / mass);
-  }
+  if (a.resident) row.x = slice, row.vec = true;
+  double h = high, l = low;
+  row.template reduce<true>(h, l);  // (and the slice is in place)
+  row.run(a, r, h, l);
 }
 
 template <class T>
 cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
-  constexpr int kResident = 200 << 10;  // bytes of a slice that is kept
+  constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
   Sample s = a;
   const long long bytes = (long long)a.vocab * sizeof(T);
   s.ranks = 1;
