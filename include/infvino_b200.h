@@ -380,7 +380,7 @@ int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs
                          float *scratch, int64_t scratch_floats, void *stream);
 
 /* The next token of each row of logits [rows][vocab] (IVC_F16, IVC_BF16 or
- * IVC_F32, rows row_stride elements apart, vocab at most 2^20). */
+ * IVC_F32, rows row_stride elements apart, vocab at most 500000). */
 typedef struct ivc_logits {
   const void *data;
   int dtype;

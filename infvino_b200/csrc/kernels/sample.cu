@@ -20,6 +20,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sample.cuh"
@@ -30,7 +31,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kClusterThreads = 512;
+constexpr int kMostWarps = 32;
 constexpr int kBins = 2048, kList = 1024;
 constexpr int kMaxRanks = 8;
 constexpr double kFar = 41.588830833596715;  // 60 ln 2: what is further below the largest has no weight
@@ -71,13 +73,13 @@ struct SampleShared {
   unsigned long long key[kList];  // (order of x, number), rising
   double mass[kList], wt[kList];  // running sums, weights
   double part[2][kMaxRanks][2];   // what CTAs tell one another, two exchanges in turn
-  double red[2][kWarps];
-  unsigned cnt[kWarps];
+  double red[2][kMostWarps];
+  unsigned cnt[kMostWarps];
   unsigned listed;
   int found, kept, reached;
   unsigned before, in_bin;
   Cut cut;
-  double seg[kWarps];
+  double seg[kMostWarps];
 };
 
 // Order of floats as unsigned numbers, falling (no NaN, no -0).
@@ -115,8 +117,9 @@ struct Want {
   __device__ __forceinline__ bool enough(double w, bool top) const { return !(min_p > 0.f) || top || w >= (double)min_p; }
 };
 
-template <class T>
+template <class T, int THREADS>
 struct Row {
+  static constexpr int kThreads = THREADS, kWarps = THREADS / 32, kPer = kList / THREADS;
   SampleShared &sh;
   const T *x;      // this CTA's slice
   bool vec;        // on 16 bytes
@@ -312,11 +315,13 @@ struct Row {
     __syncthreads();
   }
 
-  // Running sums of two doubles a thread over the block, and their total.
-  __device__ __forceinline__ double scan(double &x0, double &x1) {
+  // Running sums of kPer doubles a thread over the block, and their total.
+  __device__ __forceinline__ double scan(double (&x)[kPer]) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    double s = x0 + x1;
-    const double mine = s;
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) x[i] += x[i - 1];
+    const double mine = x[kPer - 1];
+    double s = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double v = __shfl_up_sync(0xffffffffu, s, o);
@@ -330,34 +335,33 @@ struct Row {
       if (w == warp) before = all;
       all += sh.red[0][w];
     }
-    const double a0 = x0;
-    x0 = before + (s - mine) + a0;
-    x1 = before + s;
+    before += s - mine;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] += before;
     return all;
   }
 
   // Of the n logits in sh.key, in order: what is kept, and the token; CTA 0.  mass: of
   // all tokens (top_p of them is meant where there is no top_k).  False: top_p is not reached.
   __device__ bool finish(unsigned n, const Want &want, double mass, const Sample &a, long long r) {
-    static_assert(kList == 2 * kThreads, "two a thread");
-    const int e0 = 2 * threadIdx.x;
-    double w[2], c[2];
+    const int e0 = kPer * threadIdx.x;
+    double w[kPer], c[kPer];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPer; ++i) {
       w[i] = e0 + i < (int)n ? weight(from_falling((uint32_t)(sh.key[e0 + i] >> 32))) : 0.0;
       sh.wt[e0 + i] = w[i];
       c[i] = w[i];
     }
-    scan(c[0], c[1]);
+    scan(c);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) sh.mass[e0 + i] = c[i];
+    for (int i = 0; i < kPer; ++i) sh.mass[e0 + i] = c[i];
     const int m = want.k ? min(want.k, (int)n) : (int)n;
     if (threadIdx.x == 0) sh.kept = m, sh.reached = 0;
     __syncthreads();
     if (want.p < 1.f) {
       const double target = (double)want.p * (want.k ? sh.mass[m - 1] : mass);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kPer; ++i)
         if (e0 + i < (int)n && c[i] >= target) {
           atomicMin(&sh.kept, e0 + i + 1);
           sh.reached = 1;
@@ -365,27 +369,27 @@ struct Row {
         }
     }
 #pragma unroll
-    for (int i = 1; i >= 0; --i)
+    for (int i = kPer - 1; i >= 0; --i)
       if (e0 + i < (int)n && !want.enough(w[i], from_falling((uint32_t)(sh.key[e0 + i] >> 32)) == top)) atomicMin(&sh.kept, e0 + i);
     __syncthreads();
     if (want.p < 1.f && !want.k && !sh.reached) return false;
     const unsigned kept = (unsigned)sh.kept;
     // by number
-    unsigned long long by_number[2];
+    unsigned long long by_number[kPer];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) by_number[i] = (sh.key[e0 + i] << 32) | (unsigned)(e0 + i);
+    for (int i = 0; i < kPer; ++i) by_number[i] = (sh.key[e0 + i] << 32) | (unsigned)(e0 + i);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kPer; ++i)
       if (e0 + i < (int)kept) sh.key[e0 + i] = by_number[i];
     if (threadIdx.x == 0) sh.found = (int)kept - 1;
     __syncthreads();
     sort(kept);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) c[i] = e0 + i < (int)kept ? sh.wt[(uint32_t)sh.key[e0 + i]] : 0.0;
-    const double all = scan(c[0], c[1]), target = (double)want.u * all;
+    for (int i = 0; i < kPer; ++i) c[i] = e0 + i < (int)kept ? sh.wt[(uint32_t)sh.key[e0 + i]] : 0.0;
+    const double all = scan(c), target = (double)want.u * all;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kPer; ++i)
       if (e0 + i < (int)kept && c[i] > target) {
         atomicMin(&sh.found, e0 + i);
         break;
@@ -684,10 +688,11 @@ struct Row {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) sample_k(const __grid_constant__ Sample a) {
+__global__ void __launch_bounds__(kClusterThreads) sample_k(const __grid_constant__ Sample a) {
   extern __shared__ __align__(16) uint8_t slice_raw[];
   __shared__ SampleShared sh;
-  Row<T> row(sh);
+  constexpr int kThreads = kClusterThreads;
+  Row<T, kThreads> row(sh);
   row.ranks = a.ranks;
   row.rank = a.ranks > 1 ? (int)(blockIdx.x % a.ranks) : 0;
   const long long r = blockIdx.x / a.ranks;
@@ -744,9 +749,634 @@ __global__ void __launch_bounds__(kThreads) sample_k(const __grid_constant__ Sam
   row.run(a, r, h, l);
 }
 
+// ---------------------------------------------------------------- by counting values
+//
+// Keys are the bits of a logit, turned so that larger logits come first: 16 bits, or
+// the upper 16 of 32.  Counters are 16 bits too, two a word; their sum tells whether
+// one of them ran over (more than 65535 equal logits), and such a row goes the other
+// kernel's way.  A cut of 32-bit logits lies inside a bin: the bin's logits are
+// counted again by their lower 16 bits.
+constexpr int kCountThreads = 1024, kCountWarps = kCountThreads / 32;
+constexpr int kWords = 32768, kGroups = 2048;     // two counters a word; 32 counters a group
+constexpr int kSpan = 256;                        // tokens of a running sum's entry
+constexpr int kWindow = 16;                       // bins whose weight is added up one by one
+
+struct CountShared {
+  union {
+    unsigned hist[kWords];
+    SampleShared other;
+  };
+  double sum[kGroups];
+  unsigned cnt[kGroups];
+  double powers[kPowers];
+  unsigned long long window[kWindow];
+  double red[kCountWarps];
+  unsigned redc[kCountWarps];
+  unsigned bin, before;
+  double mass;
+};
+
+template <class T>
+struct Key;
+template <>
+struct Key<float> {
+  static constexpr int kBits = 32;
+  static __device__ __forceinline__ float value(uint32_t k) { return from_falling(k); }
+};
+template <int MANTISSA>
+struct Key16 {
+  static constexpr int kBits = 16;
+  static constexpr uint32_t kInf = 0x7fffu & ~((1u << MANTISSA) - 1u);
+  static __device__ __forceinline__ uint32_t bits(uint32_t k) { return k >> 31 ? k >> 16 : 0x7fffu ^ (k >> 16); }
+};
+template <>
+struct Key<__half> : Key16<10> {
+  static __device__ __forceinline__ float value(uint32_t k) { return __half2float(__ushort_as_half((unsigned short)bits(k))); }
+};
+template <>
+struct Key<__nv_bfloat16> : Key16<7> {
+  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(bits(k) << 16); }
+};
+constexpr uint32_t kDead = 0xffffffffu;  // -inf, NaN
+
+// The key of a logit given by its bits (16-bit ones in the lower half).
+template <class T>
+__device__ __forceinline__ uint32_t key_of(uint32_t b) {
+  if (sizeof(T) == 4) {
+    const float x = __uint_as_float(b) + 0.f;
+    return x > -INFINITY ? falling(x) : kDead;
+  }
+  constexpr uint32_t inf = sizeof(T) == 2 && Key<T>::kBits == 16 ? Key16<sizeof(T) == 2 && std::is_same<T, __half>::value ? 10 : 7>::kInf : 0u;
+  uint32_t k = b >> 15 ? b : 0x7fffu ^ b;
+  k -= k == 0x8000u;                                   // -0 is 0
+  return k - (0x7fffu ^ inf) < 0x8000u + inf - (0x7fffu ^ inf) ? k << 16 : kDead;
+}
+
+template <class T>
+struct Counter {
+  static constexpr int kEach = 16 / sizeof(T);
+  static constexpr bool kWide = sizeof(T) == 4;
+  CountShared &sh;
+  const T *x;
+  int vocab, skip;            // skip: how many elements before the row its first 16-byte piece begins
+  float top;
+  double by;
+  uint32_t cut = kDead - 1;   // kept: smaller keys, and the first `room` (by number) of this one
+  unsigned room = 0xffffffffu;
+
+  __device__ Counter(CountShared &s) : sh(s) {}
+
+  __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, by, sh.powers); }
+  __device__ __forceinline__ double weight_at(uint32_t k) const { return weight(Key<T>::value(k)); }
+
+  // The keys of piece c of the row (16 bytes, in order).
+  __device__ __forceinline__ void keys(int c, uint32_t (&k)[kEach]) const {
+    const int j0 = c * kEach - skip;
+    if (j0 >= 0 && j0 + kEach <= vocab) {
+      unpack(__ldg(reinterpret_cast<const uint4 *>(x + j0)), k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        k[i] = kDead;
+        if (j0 + i >= 0 && j0 + i < vocab)
+          k[i] = key_of<T>(sizeof(T) == 4 ? __float_as_uint(*reinterpret_cast<const float *>(x + j0 + i)) : *reinterpret_cast<const uint16_t *>(x + j0 + i));
+      }
+    }
+  }
+  static __device__ __forceinline__ void unpack(uint4 u, uint32_t (&k)[kEach]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kWide) {
+        k[i] = key_of<T>(w[i]);
+      } else {
+        k[2 * i % kEach] = key_of<T>(w[i] & 0xffffu);
+        k[(2 * i + 1) % kEach] = key_of<T>(w[i] >> 16);
+      }
+    }
+  }
+  __device__ __forceinline__ int pieces() const { return (skip + vocab + kEach - 1) / kEach; }
+  // f(keys of a piece) for every piece, several in flight.
+  template <class F>
+  __device__ __forceinline__ void each(F &&f) const {
+    constexpr int kAtOnce = 4;
+    const int n = pieces();
+    for (int c0 = threadIdx.x; c0 < n; c0 += kAtOnce * kCountThreads) {
+      uint4 u[kAtOnce];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int j0 = (c0 + q * kCountThreads) * kEach - skip;
+        if (j0 >= 0 && j0 + kEach <= vocab) u[q] = __ldg(reinterpret_cast<const uint4 *>(x + j0));
+      }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int c = c0 + q * kCountThreads, j0 = c * kEach - skip;
+        if (c >= n) break;
+        uint32_t k[kEach];
+        if (j0 >= 0 && j0 + kEach <= vocab)
+          unpack(u[q], k);
+        else
+          keys(c, k);
+        f(k);
+      }
+    }
+  }
+
+  __device__ double total(double v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh.red[0];
+    for (int w = 1; w < kCountWarps; ++w) v += sh.red[w];
+    return v;
+  }
+  __device__ unsigned total(unsigned v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.redc[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kCountWarps; ++w) v += sh.redc[w];
+    return v;
+  }
+
+  __device__ __forceinline__ void clear() {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kWords / 4; i += kCountThreads) reinterpret_cast<uint4 *>(sh.hist)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add(uint32_t b) { atomicAdd(&sh.hist[b >> 1], 1u << (16 * (b & 1))); }
+  __device__ __forceinline__ unsigned counter(uint32_t b) const { return sh.hist[b >> 1] >> (16 * (b & 1)) & 0xffffu; }
+
+  // Counts of the groups of 32 counters, and with MASS their weights: key(b) stands for counter b.  The counters' sum.
+  template <bool MASS, class F>
+  __device__ unsigned groups(F &&key) {
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned all = 0;
+    for (int g = warp; g < kGroups; g += kCountWarps) {
+      const unsigned c = counter(32 * g + lane);
+      const unsigned n = __reduce_add_sync(0xffffffffu, c);
+      all += n;
+      if (lane == 0) sh.cnt[g] = n;
+      if (MASS) {
+        double w = 0;
+        if (n) {
+          if (c) w = (double)c * weight_at(key(32 * g + lane));
+#pragma unroll
+          for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        }
+        if (lane == 0) sh.sum[g] = w;
+      }
+    }
+    return total(lane == 0 ? all : 0u);
+  }
+
+  // Running sums over the groups, two a thread: of counts and (MASS) of weights; the
+  // first counter where they reach the target into sh.bin, what lies before it into
+  // sh.before and sh.mass.  False: they do not reach it.
+  template <bool MASS, class F>
+  __device__ bool locate(double target, F &&key) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g0 = 2 * threadIdx.x;
+    unsigned c[2] = {sh.cnt[g0], sh.cnt[g0 + 1]};
+    double m[2] = {MASS ? sh.sum[g0] : (double)c[0], MASS ? sh.sum[g0 + 1] : (double)c[1]};
+    double s = m[0] + m[1];
+    unsigned n = c[0] + c[1];
+    const double s0 = s;
+    const unsigned n0 = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, s, o);
+      const unsigned u = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) s += t, n += u;
+    }
+    __syncthreads();
+    if (lane == 31) sh.red[warp] = s, sh.redc[warp] = n;
+    if (threadIdx.x == 0) sh.bin = kGroups;
+    __syncthreads();
+    double before = 0;
+    unsigned nb = 0;
+    for (int w = 0; w < warp; ++w) before += sh.red[w], nb += sh.redc[w];
+    before += s - s0;
+    nb += n - n0;
+    const int at = before + m[0] >= target ? 0 : before + m[0] + m[1] >= target ? 1 : 2;
+    if (at < 2) atomicMin(&sh.bin, (unsigned)(g0 + at));
+    __syncthreads();
+    const unsigned g = sh.bin;
+    __syncthreads();
+    if (g == kGroups) return false;
+    if (g / 2 == threadIdx.x) {
+      sh.mass = before + (at ? m[0] : 0.0);
+      sh.before = nb + (at ? c[0] : 0u);
+    }
+    __syncthreads();
+    if (warp == 0) {  // inside the group
+      const unsigned k = counter(32 * g + lane);
+      double v = MASS ? (k ? (double)k * weight_at(key(32 * g + lane)) : 0.0) : (double)k;
+      const double v0 = v;
+      unsigned q = k;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, v, o);
+        const unsigned u = __shfl_up_sync(0xffffffffu, q, o);
+        if (lane >= o) v += t, q += u;
+      }
+      // (the last counter that is not empty, where the sums in this order fall short by a rounding)
+      const unsigned some = __ballot_sync(0xffffffffu, k > 0), over = __ballot_sync(0xffffffffu, k > 0 && sh.mass + v >= target);
+      const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
+      const double base = sh.mass;
+      const unsigned nbase = sh.before;
+      __syncwarp();
+      if (lane == l) {
+        sh.bin = 32 * g + lane;
+        sh.mass = base + (v - v0);
+        sh.before = nbase + (q - k);
+      }
+    }
+    __syncthreads();
+    return true;
+  }
+
+  // How many of n equal ones, weighing w each, it takes from `base` to the target.
+  static __device__ __forceinline__ unsigned enough(double target, double base, double w, unsigned n) {
+    const double r = ceil((target - base) / w);
+    return r > 1.0 ? (unsigned)fmin(r, (double)n) : 1u;
+  }
+
+  // Counts the lower halves of the keys of bin b.  False: a counter ran over.
+  __device__ bool count_inside(uint32_t b, unsigned n) {
+    clear();
+    each([&](const uint32_t(&k)[kEach]) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (k[i] >> 16 == b && k[i] != kDead) add(k[i] & 0xffffu);
+    });
+    return groups<false>([](uint32_t) { return 0u; }) == n;
+  }
+
+  // Counts the upper halves of all keys; how many logits there are, and the first key.
+  __device__ bool count_all(unsigned &live, uint32_t &first) {
+    clear();
+    unsigned n = 0;
+    uint32_t least = kDead;
+    each([&](const uint32_t(&k)[kEach]) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (k[i] != kDead) {
+          add(k[i] >> 16);
+          least = min(least, k[i]);
+          ++n;
+        }
+    });
+    least = __reduce_min_sync(0xffffffffu, least);
+    live = total(n);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.redc[threadIdx.x >> 5] = least;
+    __syncthreads();
+    first = sh.redc[0];
+    for (int w = 1; w < kCountWarps; ++w) first = min(first, sh.redc[w]);
+    return groups<false>([](uint32_t) { return 0u; }) == live;
+  }
+
+  // The cut.  False: a counter ran over, or a guess was too far off.
+  __device__ bool select(const Want &want, unsigned live, uint32_t first) {
+    auto upper = [](uint32_t b) { return b << 16; };
+    // (of a bin of 32-bit logits the middle, but no more than the largest logit)
+    auto middle = [first](uint32_t b) { return kWide ? max(b << 16 | 0x8000u, first) : b << 16; };
+    if (want.k && (unsigned)want.k < live) {
+      locate<false>((double)want.k, upper);
+      const uint32_t b = sh.bin;
+      unsigned need = want.k - sh.before;
+      const unsigned in_bin = counter(b);
+      if (kWide) {
+        if (!count_inside(b, in_bin)) return false;
+        locate<false>((double)need, upper);
+        need -= sh.before;
+        cut = b << 16 | sh.bin;
+        if (want.p < 1.f) {
+          unsigned n;
+          uint32_t f;
+          if (!count_all(n, f)) return false;
+        }
+      } else {
+        cut = b << 16;
+      }
+      room = need;
+    }
+    if (!(want.p < 1.f)) return true;
+    // weights of the bins up to the cut (the cut's own bin: as much as there is room for)
+    groups<true>(middle);
+    const double wc = cut < kDead - 1 ? weight_at(cut) : 0.0;
+    double mass;
+    if (cut < kDead - 1) {
+      // what lies before the cut's bin
+      const uint32_t b = cut >> 16;
+      double m = 0;
+      for (uint32_t g = threadIdx.x; g < b / 32; g += kCountThreads) m += sh.sum[g];
+      if (threadIdx.x < b % 32) {
+        const unsigned c = counter((b & ~31u) + threadIdx.x);
+        m += c ? (double)c * weight_at(middle((b & ~31u) + threadIdx.x)) : 0.0;
+      }
+      mass = total(m) + room * wc;
+    } else {
+      double m = 0;
+      for (int g = threadIdx.x; g < kGroups; g += kCountThreads) m += sh.sum[g];
+      mass = total(m);
+    }
+    constexpr double kLeast = 1e-300;  // (something is kept, also with top_p 0)
+    double target = fmax((double)want.p * mass, kLeast);
+    if (!kWide) {
+      if (!locate<true>(target, middle)) return true;  // (p is 1, but for a rounding)
+      const uint32_t b = sh.bin;
+      if ((b << 16) > cut) return true;
+      const unsigned r = enough(target, sh.mass, weight_at(b << 16), counter(b));
+      room = (b << 16) < cut ? r : min(room, r);
+      cut = b << 16;
+      return true;
+    }
+    // The middles gave a guess of the bin; the weights up to a window around it are added up one by one.
+    uint32_t b = locate<true>(target, middle) ? sh.bin : 0xffffu;
+    for (int tries = 0; tries < 4; ++tries) {
+      const uint32_t from = b > kWindow / 2 ? min(b - kWindow / 2, 0x10000u - kWindow) : 0u;
+      __syncthreads();
+      if (threadIdx.x < kWindow) sh.window[threadIdx.x] = 0;
+      __syncthreads();
+      double below = 0, above = 0;
+      each([&](const uint32_t(&k)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (k[i] < cut) {
+            const double w = weight_at(k[i]);
+            const uint32_t at = (k[i] >> 16) - from;
+            if (k[i] >> 16 < from)
+              below += w;
+            else if (at >= kWindow)
+              above += w;
+            else
+              atomicAdd(&sh.window[at], __double2ull_rn(w * 0x1p44));  // (whole numbers: the order does not matter)
+          }
+      });
+      below = total(below);
+      above = total(above);
+      double in[kWindow], all = below + above + room * wc;
+      if (!(cut < kDead - 1)) all = below + above;
+#pragma unroll
+      for (int i = 0; i < kWindow; ++i) in[i] = (double)sh.window[i] * 0x1p-44, all += in[i];
+      const uint32_t at = (cut >> 16) - from;
+      target = fmax((double)want.p * all, kLeast);
+      if (target <= below && from > 0) {
+        b = from > kWindow / 2 ? from - kWindow / 2 : 0;
+        continue;
+      }
+      double base = below;
+      int hit = -1;
+#pragma unroll
+      for (int i = 0; i < kWindow; ++i) {
+        const double m = in[i] + ((uint32_t)i == at && cut < kDead - 1 ? room * wc : 0.0);
+        if (hit < 0 && base + m >= target) hit = i;
+        if (hit < 0) base += m;
+      }
+      if (hit < 0) {
+        if (from + kWindow > cut >> 16) return true;  // (p is 1, but for a rounding)
+        b = from + kWindow + kWindow / 2;
+        continue;
+      }
+      const uint32_t bin = from + hit;
+      const unsigned in_bin = counter(bin);
+      if (in_bin == 0 || !count_inside(bin, in_bin)) return false;
+      auto inside = [bin](uint32_t l) { return bin << 16 | l; };
+      groups<true>(inside);
+      if (!locate<true>(target - base, inside)) return true;
+      const uint32_t key = bin << 16 | sh.bin;
+      if (key > cut) return true;
+      const unsigned r = enough(target - base, sh.mass, weight_at(key), counter(sh.bin));
+      room = key < cut ? r : min(room, r);
+      cut = key;
+      return true;
+    }
+    return false;
+  }
+
+  // The running sums of the kept tokens, by number, and the token where they pass u of them all.
+  __device__ void choose(const Want &want, const Sample &a, long long r) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float lowest = want.floor(top);
+    const double wc = weight_at(cut);
+    const bool cut_counts = cut < kDead - 1 && want.enough(wc, Key<T>::value(cut) == top);
+    constexpr int kLanePieces = kSpan / 32 / kEach;  // pieces of a lane in an entry
+    const int n = pieces(), entries = (n + 32 * kLanePieces - 1) / (32 * kLanePieces);
+    auto before_cut = [&](uint32_t k) {
+      if (k >= cut) return 0.0;
+      const float v = Key<T>::value(k);
+      if (v < lowest) return 0.0;
+      const double w = weight(v);
+      return want.enough(w, v == top) ? w : 0.0;
+    };
+    __syncthreads();
+    for (int e = threadIdx.x; e < kGroups; e += kCountThreads) sh.sum[e] = 0.0, sh.cnt[e] = 0;
+    __syncthreads();
+    constexpr int kAtOnce = 2;
+    for (int e0 = warp; e0 < entries; e0 += kAtOnce * kCountWarps) {
+      uint32_t k[kAtOnce][kLanePieces][kEach];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+        for (int z = 0; z < kLanePieces; ++z) {
+          const int c = ((e0 + q * kCountWarps) * 32 + lane) * kLanePieces + z;
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) k[q][z][i] = kDead;
+          if (e0 + q * kCountWarps < entries && c < n) keys(c, k[q][z]);
+        }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        uint32_t least = kDead;
+#pragma unroll
+        for (int z = 0; z < kLanePieces; ++z)
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) least = min(least, k[q][z][i]);
+        if (!__any_sync(0xffffffffu, least <= cut)) continue;
+        double s = 0;
+        unsigned equal = 0;
+        if (least <= cut) {
+#pragma unroll
+          for (int z = 0; z < kLanePieces; ++z)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+              s += before_cut(k[q][z][i]);
+              equal += k[q][z][i] == cut;
+            }
+        }
+        equal = __reduce_add_sync(0xffffffffu, equal);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
+      }
+    }
+    __syncthreads();
+    // two entries a thread: how many equal to the cut come before, then sums
+    const int e0 = 2 * threadIdx.x;
+    const unsigned c[2] = {sh.cnt[e0], sh.cnt[e0 + 1]};
+    unsigned nq = c[0] + c[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned t = __shfl_up_sync(0xffffffffu, nq, o);
+      if (lane >= o) nq += t;
+    }
+    if (lane == 31) sh.redc[warp] = nq;
+    __syncthreads();
+    unsigned have = nq - c[0] - c[1];
+    for (int w = 0; w < warp; ++w) have += sh.redc[w];
+    const unsigned have0 = min(have, room), have1 = min(have + c[0], room), have2 = min(have + c[0] + c[1], room);
+    const double v0 = sh.sum[e0] + (have1 > have0 ? (have1 - have0) * wc : 0.0), v1 = sh.sum[e0 + 1] + (have2 > have1 ? (have2 - have1) * wc : 0.0);
+    double s = v0 + v1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    if (lane == 31) sh.red[warp] = s;
+    if (threadIdx.x == 0) sh.bin = kGroups, sh.before = 0;
+    __syncthreads();
+    double start = 0, all = 0;
+    for (int w = 0; w < kCountWarps; ++w) {
+      if (w == warp) start = all;
+      all += sh.red[w];
+    }
+    start += s - v0 - v1;
+    const double target = (double)want.u * all;
+    const int at = v0 > 0 && start + v0 > target ? 0 : v1 > 0 && start + v0 + v1 > target ? 1 : 2;
+    if (at < 2) atomicMin(&sh.bin, (unsigned)(e0 + at));
+    if (v0 > 0 || v1 > 0) atomicMax(&sh.before, (unsigned)(v1 > 0 ? e0 + 1 : e0));  // the last with some weight
+    __syncthreads();
+    const unsigned e = sh.bin < kGroups ? sh.bin : sh.before;
+    __syncthreads();
+    if (e / 2 == threadIdx.x) {
+      sh.mass = e & 1 ? start + v0 : start;
+      sh.before = e & 1 ? have1 : have0;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    // the entry, a lane's tokens one after the other
+    uint32_t k[kLanePieces * kEach];
+#pragma unroll
+    for (int z = 0; z < kLanePieces; ++z) {
+      const int p = ((int)e * 32 + lane) * kLanePieces + z;
+      uint32_t t[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) t[i] = kDead;
+      if (p < n) keys(p, t);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) k[z * kEach + i] = t[i];
+    }
+    unsigned equal = 0;
+#pragma unroll
+    for (int i = 0; i < kLanePieces * kEach; ++i) equal += cut_counts && k[i] == cut;
+    unsigned eq = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned t = __shfl_up_sync(0xffffffffu, eq, o);
+      if (lane >= o) eq += t;
+    }
+    unsigned used = sh.before + eq - equal;
+    double w[kLanePieces * kEach], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kLanePieces * kEach; ++i) {
+      w[i] = before_cut(k[i]);
+      if (cut_counts && k[i] == cut && used++ < room) w[i] = wc;
+      mine += w[i];
+    }
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const double base = sh.mass;
+    const unsigned some = __ballot_sync(0xffffffffu, mine > 0), over = __ballot_sync(0xffffffffu, mine > 0 && base + incl > target);
+    const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
+    if (lane == l) {
+      double run = base + (incl - mine), share = 0;
+      int hit = -1;
+#pragma unroll
+      for (int i = 0; i < kLanePieces * kEach; ++i) {
+        if (w[i] > 0 && (hit < 0 || !(run > target))) hit = i, share = w[i];
+        run += w[i];
+      }
+      a.tokens[r] = ((int)e * 32 + lane) * kLanePieces * kEach + hit - skip;
+      if (a.probs) a.probs[r] = (float)(share / all);
+    }
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kCountThreads, 1) sample_count_k(const __grid_constant__ Sample a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  CountShared &sh = *reinterpret_cast<CountShared *>(smem_raw);
+  Counter<T> c(sh);
+  const long long r = blockIdx.x;
+  fill_powers(sh.powers);
+  pdl_wait_and_release();
+  c.x = static_cast<const T *>(a.x) + r * a.stride;
+  c.vocab = a.vocab;
+  c.skip = (int)(reinterpret_cast<uintptr_t>(c.x) % 16 / sizeof(T));
+  unsigned live;
+  uint32_t first;
+  bool fits = c.count_all(live, first);
+  if (live == 0) {
+    if (threadIdx.x == 0) {
+      a.tokens[r] = -1;
+      if (a.probs) a.probs[r] = 0.f;
+    }
+    return;
+  }
+  const Want want(a, r);
+  c.top = Key<T>::value(first);
+  c.by = want.t > 0.f ? kPowers * 1.4426950408889634 / (double)want.t : 0.0;
+  if (!(want.t > 0.f)) {  // the first of the largest
+    c.cut = first;
+    c.room = 1;
+    fits = true;
+  } else if (fits) {
+    fits = c.select(want, live, first);
+  }
+  if (fits) {
+    c.choose(want, a, r);
+    return;
+  }
+  // the other kernel's way, from global memory
+  __syncthreads();
+  Row<T, kCountThreads> row(sh.other);
+  row.ranks = 1, row.rank = 0;
+  row.x = c.x, row.n = a.vocab, row.first = 0;
+  row.vec = c.skip == 0;
+  fill_powers(sh.other.powers);
+  __syncthreads();
+  double high = -INFINITY, low = -INFINITY;
+  row.each([&](float v, int) {
+    if (v > -INFINITY) high = fmax(high, (double)v), low = fmax(low, -(double)v);
+  });
+  row.template reduce<true>(high, low);
+  row.run(a, r, high, low);
+}
+
+template <class T>
+cudaError_t launch_count(const Sample &a, cudaStream_t st) {
+  static std::atomic<bool> attr_set[kAttrMaxDevices];
+  const cudaError_t e = ensure_dynamic_smem(sample_count_k<T>, (int)sizeof(CountShared), attr_set);
+  if (e != cudaSuccess) return e;
+  Sample s = a;
+  s.ranks = 1;
+  s.slice = a.vocab;
+  return launch_kernel(sample_count_k<T>, dim3((unsigned)a.rows), dim3(kCountThreads), sizeof(CountShared), st, s);
+}
+
 template <class T>
 cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
+  const char *env = getenv("IVB_SAMPLE");
+  if (env ? env[0] == 'c' : a.rows >= 100) return launch_count<T>(a, st);
   Sample s = a;
   const long long bytes = (long long)a.vocab * sizeof(T);
   s.ranks = 1;
@@ -759,7 +1389,7 @@ cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * s.ranks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = s.resident ? (size_t)need : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];

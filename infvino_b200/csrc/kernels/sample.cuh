@@ -6,7 +6,7 @@
 
 namespace ivb {
 
-constexpr long long kSampleMaxVocab = 1 << 20;
+constexpr long long kSampleMaxVocab = 500000;
 
 struct Sample {
   const void *x;             // [rows][vocab], 16 or 32 bits

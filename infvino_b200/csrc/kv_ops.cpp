@@ -512,7 +512,7 @@ int ivc_kv_sample(ivc_kv *h, const ivc_logits *logits, const ivc_sampling *how, 
     need(logits && how, "null pointer");
     need(logits->dtype == IVC_F16 || logits->dtype == IVC_BF16 || logits->dtype == IVC_F32, "logits are IVC_F16, IVC_BF16 or IVC_F32");
     need(logits->rows >= 0 && logits->rows <= (1 << 24), "rows out of range");
-    need(logits->vocab >= 1 && logits->vocab <= ivb::kSampleMaxVocab, "vocab: 1 to 2^20");
+    need(logits->vocab >= 1 && logits->vocab <= ivb::kSampleMaxVocab, "vocab: 1 to 500000");
     if (logits->rows == 0) return;
     need(logits->data && how->u && tokens, "null pointer");
     need(aligned(logits->data, logits->dtype == IVC_F32 ? 4 : 2), "logits are aligned to their type");

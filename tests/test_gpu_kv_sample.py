@@ -63,7 +63,7 @@ def check(ops, x, u, temperature=None, top_k=None, top_p=None, min_p=None, probs
     host, got, f = x.double().cpu().numpy(), tokens.tolist(), {n: None if v is None else v.tolist() for n, v in dev.items()}
     for r in range(rows):
         want, share, margin = choose(host[r], f["u"][r], *(d if f[n] is None else f[n][r] for n, d in (("t", 1.0), ("k", 0), ("p", 1.0), ("m", 0.0))))
-        # (sums of 2^20 weights in 64 bits are good to some 2^-33 whatever their order: nearer to a border than that nothing is asked)
+        # (sums of 500000 weights in 64 bits are good to some 2^-33 whatever their order: nearer to a border than that nothing is asked)
         assert got[r] == want or abs(margin) < 2.0 ** -33, (r, got[r], want, margin)
         if probs and got[r] == want:
             assert abs(float(pr[r]) - share) <= 2.0 ** -23 * share, (r, float(pr[r]), share)  # one rounding to f32, and 64-bit sums
@@ -82,7 +82,7 @@ def uniform(rows, seed):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 33), (5, 1000), (1, 32003), (300, 777), (40, 50021), (2, 262144), (1, 1 << 20)])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 33), (5, 1000), (1, 32003), (300, 777), (40, 50021), (2, 262144), (1, 500000)])
 @pytest.mark.parametrize("filters", ["none", "temperature", "top_k", "top_p", "min_p", "all"])
 def test_sample(ops, dtype, rows, vocab, filters):
     r = np.random.default_rng(rows + vocab)
@@ -254,4 +254,4 @@ def test_refusals(ops):
         with pytest.raises((ValueError, ivb.NativeError)):
             ops.sample(stream=stream(), **args)
     with pytest.raises(ivb.NativeError):
-        ops.sample(torch.empty((1, (1 << 20) + 1), dtype=torch.float16, device="cuda"), u[:1], t[:1], stream=stream())
+        ops.sample(torch.empty((1, 500001), dtype=torch.float16, device="cuda"), u[:1], t[:1], stream=stream())
