@@ -35,6 +35,7 @@ constexpr int kClusterThreads = 512;
 constexpr int kMostWarps = 32;
 constexpr int kBins = 2048, kList = 1024;
 constexpr int kMaxRanks = 8;
+constexpr int kWindow = 16;  // bins around a guess
 constexpr double kFar = 41.588830833596715;  // 60 ln 2: what is further below the largest has no weight
 
 // 2^(j / 64), j below 64, by the first threads of a block.
@@ -80,6 +81,7 @@ struct SampleShared {
   unsigned before, in_bin;
   Cut cut;
   double seg[kMostWarps];
+  unsigned long long window[kWindow];
 };
 
 // Order of floats as unsigned numbers, falling (no NaN, no -0).
@@ -276,6 +278,22 @@ struct Row {
     __syncthreads();
   }
 
+  // The sum of f over the first n bins.
+  template <class F>
+  __device__ double guessed(int n, F &&f) {
+    double m = 0;
+    for (int k = threadIdx.x; k < n; k += kThreads) m += f(k);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.red[0][threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = sh.red[0][0];
+    for (int w = 1; w < kWarps; ++w) m += sh.red[0][w];
+    __syncthreads();
+    return m;
+  }
+
   // Puts those of which in(logit, number) holds (at most kList) in order, in CTA 0: sh.key; how many there are is returned there.
   template <class F>
   __device__ unsigned gather(F &&in) {
@@ -451,10 +469,10 @@ struct Row {
 
   // Cuts where `target` is reached: of how many are kept (COUNT) or of what they weigh.
   template <bool COUNT>
-  __device__ void select(double target, float least, int vocab) {
+  __device__ void select(double target, float least, int vocab, bool counted) {
     float hi = top, lo = least;
     double base = 0;
-    for (;;) {
+    for (;; counted = false) {
       if (!(lo < hi)) {
         // equal ones: as many as it takes
         const double w = COUNT ? 1.0 : weight(hi);
@@ -464,7 +482,7 @@ struct Row {
       }
       const Bins bins(hi, lo);
       auto bin = [&](float v, int i) { return keeps(v, i) ? bins(v) : -1; };
-      count(bin);
+      if (!counted) count(bin);
       int b;
       if (COUNT) {
         find(target - base, [&](int k) { return (double)sh.hist[k]; });
@@ -472,30 +490,56 @@ struct Row {
         if (base + sh.before + sh.in_bin < target) return;  // there are not so many
         base += sh.before;
       } else {
-        // a guess by the weights of the bins' middles, then sums
-        find(target - base, [&](int k) { return sh.hist[k] ? sh.hist[k] * weight(bins.middle(k)) : 0.0; });
+        // a guess by the weights of the bins' middles; then the weights up to a window
+        // around it are added up one by one
+        auto guess = [&](int k) { return sh.hist[k] ? sh.hist[k] * weight(bins.middle(k)) : 0.0; };
+        find(target - base, guess);
         b = sh.found;
-        int from = 0, to = kBins - 1;
-        for (int tries = 0;; ++tries) {
-          double a = 0, in = 0;
+        int from = 0, to = kBins - 1;  // the bin is one of these
+        for (;;) {
+          const int w0 = max(from, min(b - kWindow / 2, to + 1 - kWindow));
+          __syncthreads();
+          if (threadIdx.x < kWindow) sh.window[threadIdx.x] = 0;
+          __syncthreads();
+          double a = 0, none = 0;
           each([&](float v, int i) {
-            const int k = bin(v, i);
-            if (k < 0 || k > b) return;
+            const int k = bin(v, i) - w0;
+            if (k >= kWindow || k + w0 < 0) return;
             const double w = weight(v);
-            if (k < b)
+            if (k < 0)
               a += w;
             else
-              in += w;
+              atomicAdd(&sh.window[k], __double2ull_rn(w * 0x1p44));  // (whole numbers: the order does not matter)
           });
-          reduce<false>(a, in);
-          if (base + a >= target && b > from) {
-            to = b - 1;
-            b = tries < 2 ? to : (from + to) / 2;
-          } else if (base + a + in < target && b < to) {
-            from = b + 1;
-            b = tries < 2 ? from : (from + to) / 2;
+          reduce<false>(a, none);  // (and the windows are complete)
+          if (threadIdx.x < kWindow) {
+            unsigned long long u = 0;
+            for (int r = 0; r < ranks; ++r) u += *at(&sh.window[threadIdx.x], r);
+            sh.mass[threadIdx.x] = (double)u * 0x1p-44;
+          }
+          __syncthreads();
+          double sum = base + a;
+          int hit = -1;
+          for (int k = 0; k < kWindow && hit < 0; ++k) {
+            const double m = sh.mass[k];
+            if (sum + m >= target || w0 + k == to)
+              hit = k;
+            else
+              sum += m;
+          }
+          sync();  // (the windows have been read)
+          // (the next guess begins at the window's edge, where the sum is known)
+          if (base + a >= target && w0 > from) {
+            to = w0 - 1;
+            find(guessed(w0, guess) - (base + a - target), guess);
+            b = sh.found;
+          } else if (hit < 0) {
+            from = w0 + kWindow;
+            find(guessed(from, guess) + (target - sum), guess);
+            b = sh.found;
           } else {
-            base += a;
+            b = w0 + hit;
+            base = sum;
             break;
           }
         }
@@ -574,10 +618,12 @@ struct Row {
       each([&](float v, int) { mass += v > -INFINITY ? weight(v) : 0.0; });
       reduce<false>(mass, none);
     }
+    bool counted = false;
     if ((want.p < 1.f || want.k) && want.k <= kList && least < top) {
       // what is kept, if it is not much, goes through one list
       const Bins bins(top, least);
       count([&](float v, int) { return bins(v); });
+      counted = true;
       if (want.k)
         find((double)want.k, [&](int b) { return (double)sh.hist[b]; });
       else
@@ -598,14 +644,14 @@ struct Row {
         if (sh.reached) return;
       }
     }
-    if (want.k) select<true>((double)want.k, least, a.vocab);
+    if (want.k) select<true>((double)want.k, least, a.vocab, counted);
     if (want.p < 1.f) {
       if (want.k) {
         mass = 0;
         each([&](float v, int i) { mass += keeps(v, i) ? weight(v) : 0.0; });
         reduce<false>(mass, none);
       }
-      select<false>((double)want.p * mass, least, a.vocab);
+      select<false>((double)want.p * mass, least, a.vocab, counted && !want.k);
     }
     // ---- running sums, by number: a warp has a piece of the slice, in steps of 128
     const float lowest = want.floor(top);
@@ -688,7 +734,7 @@ struct Row {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kClusterThreads) sample_k(const __grid_constant__ Sample a) {
+__global__ void __launch_bounds__(kClusterThreads, 2) sample_k(const __grid_constant__ Sample a) {
   extern __shared__ __align__(16) uint8_t slice_raw[];
   __shared__ SampleShared sh;
   constexpr int kThreads = kClusterThreads;
@@ -759,7 +805,6 @@ __global__ void __launch_bounds__(kClusterThreads) sample_k(const __grid_constan
 constexpr int kCountThreads = 1024, kCountWarps = kCountThreads / 32;
 constexpr int kWords = 32768, kGroups = 2048;     // two counters a word; 32 counters a group
 constexpr int kSpan = 256;                        // tokens of a running sum's entry
-constexpr int kWindow = 16;                       // bins whose weight is added up one by one
 
 struct CountShared {
   union {
@@ -780,12 +825,11 @@ template <class T>
 struct Key;
 template <>
 struct Key<float> {
-  static constexpr int kBits = 32;
+  static constexpr uint32_t kInf = 0;
   static __device__ __forceinline__ float value(uint32_t k) { return from_falling(k); }
 };
 template <int MANTISSA>
 struct Key16 {
-  static constexpr int kBits = 16;
   static constexpr uint32_t kInf = 0x7fffu & ~((1u << MANTISSA) - 1u);
   static __device__ __forceinline__ uint32_t bits(uint32_t k) { return k >> 31 ? k >> 16 : 0x7fffu ^ (k >> 16); }
 };
@@ -806,7 +850,7 @@ __device__ __forceinline__ uint32_t key_of(uint32_t b) {
     const float x = __uint_as_float(b) + 0.f;
     return x > -INFINITY ? falling(x) : kDead;
   }
-  constexpr uint32_t inf = sizeof(T) == 2 && Key<T>::kBits == 16 ? Key16<sizeof(T) == 2 && std::is_same<T, __half>::value ? 10 : 7>::kInf : 0u;
+  constexpr uint32_t inf = Key<T>::kInf;
   uint32_t k = b >> 15 ? b : 0x7fffu ^ b;
   k -= k == 0x8000u;                                   // -0 is 0
   return k - (0x7fffu ^ inf) < 0x8000u + inf - (0x7fffu ^ inf) ? k << 16 : kDead;
@@ -842,6 +886,20 @@ struct Counter {
           k[i] = key_of<T>(sizeof(T) == 4 ? __float_as_uint(*reinterpret_cast<const float *>(x + j0 + i)) : *reinterpret_cast<const uint16_t *>(x + j0 + i));
       }
     }
+  }
+  // Piece c as it lies in memory, with NaN where it is not the row's.
+  __device__ __forceinline__ uint4 piece(int c) const {
+    const int j0 = c * kEach - skip;
+    if (j0 >= 0 && j0 + kEach <= vocab) return __ldg(reinterpret_cast<const uint4 *>(x + j0));
+    uint32_t w[4] = {kDead, kDead, kDead, kDead};
+    if (!kWide)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + i >= 0 && j0 + i < vocab) {
+          const uint32_t b = *reinterpret_cast<const uint16_t *>(x + j0 + i);
+          w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | b << 16 : (w[i / 2] & 0xffff0000u) | b;
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
   static __device__ __forceinline__ void unpack(uint4 u, uint32_t (&k)[kEach]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -910,28 +968,54 @@ struct Counter {
   __device__ __forceinline__ void add(uint32_t b) { atomicAdd(&sh.hist[b >> 1], 1u << (16 * (b & 1))); }
   __device__ __forceinline__ unsigned counter(uint32_t b) const { return sh.hist[b >> 1] >> (16 * (b & 1)) & 0xffffu; }
 
-  // Counts of the groups of 32 counters, and with MASS their weights: key(b) stands for counter b.  The counters' sum.
-  template <bool MASS, class F>
-  __device__ unsigned groups(F &&key) {
+  // Counts of the groups of 32 counters: their sum.
+  __device__ unsigned group_counts() {
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned all = 0;
-    for (int g = warp; g < kGroups; g += kCountWarps) {
-      const unsigned c = counter(32 * g + lane);
-      const unsigned n = __reduce_add_sync(0xffffffffu, c);
-      all += n;
-      if (lane == 0) sh.cnt[g] = n;
-      if (MASS) {
-        double w = 0;
-        if (n) {
-          if (c) w = (double)c * weight_at(key(32 * g + lane));
 #pragma unroll
-          for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-        }
+    for (int z = 0; z < kGroups / kCountThreads; ++z) {
+      const int g = threadIdx.x + z * kCountThreads;
+      unsigned n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // (the lanes begin at different quarters: no two meet in a bank)
+        const uint4 u = reinterpret_cast<const uint4 *>(sh.hist)[4 * g + ((i + (threadIdx.x >> 1)) & 3)];
+        n += (u.x & 0xffffu) + (u.x >> 16) + (u.y & 0xffffu) + (u.y >> 16) + (u.z & 0xffffu) + (u.z >> 16) + (u.w & 0xffffu) + (u.w >> 16);
+      }
+      sh.cnt[g] = n;
+      all += n;
+    }
+    return total(all);  // (barriers: the counts are in place)
+  }
+  // Weights of the groups; key(b) stands for counter b.
+  template <class F>
+  __device__ void group_weights(F &&key) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int g0 = 0; g0 < kGroups; g0 += 32 * kCountWarps) {
+      const int mine = g0 + warp + kCountWarps * lane;
+      unsigned some = __ballot_sync(0xffffffffu, sh.cnt[mine] != 0);
+      if (!(some >> lane & 1)) sh.sum[mine] = 0.0;
+      for (; some; some &= some - 1) {
+        const int g = g0 + warp + kCountWarps * (__ffs(some) - 1);
+        const unsigned c = counter(32 * g + lane);
+        double w = c ? (double)c * weight_at(key(32 * g + lane)) : 0.0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
         if (lane == 0) sh.sum[g] = w;
       }
     }
-    return total(lane == 0 ? all : 0u);
+    __syncthreads();
+  }
+
+  // What the counters before counter b weigh.
+  template <class F>
+  __device__ double weight_before(uint32_t b, F &&key) {
+    double m = 0;
+    for (uint32_t g = threadIdx.x; g < b / 32; g += kCountThreads) m += sh.sum[g];
+    if (threadIdx.x < b % 32) {
+      const uint32_t k = (b & ~31u) + threadIdx.x;
+      if (counter(k)) m += (double)counter(k) * weight_at(key(k));
+    }
+    return total(m);
   }
 
   // Running sums over the groups, two a thread: of counts and (MASS) of weights; the
@@ -1013,31 +1097,130 @@ struct Counter {
       for (int i = 0; i < kEach; ++i)
         if (k[i] >> 16 == b && k[i] != kDead) add(k[i] & 0xffffu);
     });
-    return groups<false>([](uint32_t) { return 0u; }) == n;
+    return group_counts() == n;
   }
+
+  static __device__ __forceinline__ float2 values2(uint32_t w) {
+    if (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  // Two 16-bit keys from two logits (-0 is not 0 here).
+  static __device__ __forceinline__ uint32_t keys2(uint32_t w) {
+    return w ^ 0x7fff7fffu ^ ((w >> 15 & 0x00010001u) * 0x7fffu);
+  }
+  // The same with -0 as 0.
+  static __device__ __forceinline__ uint32_t keys2_zero(uint32_t w) {
+    const uint32_t k = keys2(w);
+    return k - (__vcmpeq2(k, 0x80008000u) & 0x00010001u);
+  }
+  static constexpr uint32_t kInf = Key<T>::kInf, kFirst16 = 0x7fffu - kInf, kEnd16 = 0x8000u + kInf;  // keys of logits: kFirst16 .. kEnd16 - 1
 
   // Counts the upper halves of all keys; how many logits there are, and the first key.
   __device__ bool count_all(unsigned &live, uint32_t &first) {
     clear();
     unsigned n = 0;
     uint32_t least = kDead;
-    each([&](const uint32_t(&k)[kEach]) {
+    if constexpr (kWide) {
+      each([&](const uint32_t(&k)[kEach]) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (k[i] != kDead) {
-          add(k[i] >> 16);
-          least = min(least, k[i]);
-          ++n;
-        }
-    });
-    least = __reduce_min_sync(0xffffffffu, least);
+        for (int i = 0; i < kEach; ++i)
+          if (k[i] != kDead) {
+            add(k[i] >> 16);
+            least = min(least, k[i]);
+            ++n;
+          }
+      });
+    } else {
+      auto two = [&](uint32_t w) {
+        const uint32_t k = keys2(w), lo = k & 0xffffu, hi = k >> 16;
+        // (NaN with the sign bit and -inf are left out here, the other NaN and -0 below)
+        if (lo < kEnd16) add(lo), ++n;
+        if (hi < kEnd16) add(hi), ++n;
+      };
+      constexpr int kAtOnce = 4;
+      const int c1 = pieces() - 1;
+      for (int c0 = threadIdx.x; c0 <= c1; c0 += kAtOnce * kCountThreads) {
+        uint4 u[kAtOnce];
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) u[q] = piece(c0 + q * kCountThreads);
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q)
+          if (c0 + q * kCountThreads <= c1) two(u[q].x), two(u[q].y), two(u[q].z), two(u[q].w);
+      }
+      __syncthreads();
+      unsigned out = 0;
+      for (uint32_t b = threadIdx.x; b < kFirst16; b += kCountThreads) out += counter(b);
+      out = total(out);  // (a barrier: all have looked)
+      for (uint32_t b = threadIdx.x; b < kFirst16 / 2; b += kCountThreads) sh.hist[b] = 0;
+      if (threadIdx.x == 0) {
+        if (kFirst16 & 1) sh.hist[kFirst16 / 2] &= 0xffff0000u;
+        const unsigned zero = counter(0x8000u);
+        sh.hist[0x4000] -= zero;
+        // (should the sum run over, the total tells)
+        sh.hist[0x3fff] += zero << 16;
+      }
+      if (threadIdx.x == 1) n -= out;
+    }
     live = total(n);
+    if constexpr (kWide) {
+      least = __reduce_min_sync(0xffffffffu, least);
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) sh.redc[threadIdx.x >> 5] = least;
+      __syncthreads();
+      first = sh.redc[0];
+      for (int w = 1; w < kCountWarps; ++w) first = min(first, sh.redc[w]);
+    }
+    const bool fits = group_counts() == live;
+    if constexpr (!kWide) {
+      // the first counter that is not empty
+      __syncthreads();
+      if (threadIdx.x == 0) sh.bin = kGroups;
+      __syncthreads();
+      for (int g = threadIdx.x; g < kGroups; g += kCountThreads)
+        if (sh.cnt[g]) {
+          atomicMin(&sh.bin, (unsigned)g);
+          break;
+        }
+      __syncthreads();
+      const unsigned g = min(sh.bin, (unsigned)kGroups - 1);
+      const unsigned some = __ballot_sync(0xffffffffu, counter(32 * g + (threadIdx.x & 31)) != 0);
+      first = (32 * g + __ffs(some) - 1) << 16;
+    }
+    return fits;
+  }
+
+  // The first key alone (kDead: there are no logits).
+  __device__ uint32_t first_key() {
+    uint32_t least = kDead;
+    if constexpr (kWide) {
+      each([&](const uint32_t(&k)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) least = min(least, k[i]);
+      });
+    } else {
+      constexpr int kAtOnce = 4;
+      constexpr uint32_t kBefore = kFirst16 * 0x10001u;  // (NaN without the sign bit goes behind all others)
+      const int c1 = pieces() - 1;
+      uint32_t two = kDead;
+      for (int c0 = threadIdx.x; c0 <= c1; c0 += kAtOnce * kCountThreads) {
+        uint4 u[kAtOnce];
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) u[q] = c0 + q * kCountThreads <= c1 ? piece(c0 + q * kCountThreads) : make_uint4(kDead, kDead, kDead, kDead);
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q)
+          two = __vminu2(two, __vminu2(__vminu2(__vsub2(keys2_zero(u[q].x), kBefore), __vsub2(keys2_zero(u[q].y), kBefore)),
+                                       __vminu2(__vsub2(keys2_zero(u[q].z), kBefore), __vsub2(keys2_zero(u[q].w), kBefore))));
+      }
+      const uint32_t k = min(two & 0xffffu, two >> 16);
+      least = k < kEnd16 - kFirst16 ? (k + kFirst16) << 16 : kDead;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.redc[threadIdx.x >> 5] = least;
     __syncthreads();
-    first = sh.redc[0];
-    for (int w = 1; w < kCountWarps; ++w) first = min(first, sh.redc[w]);
-    return groups<false>([](uint32_t) { return 0u; }) == live;
+    least = sh.redc[0];
+    for (int w = 1; w < kCountWarps; ++w) least = min(least, sh.redc[w]);
+    return least;
   }
 
   // The cut.  False: a counter ran over, or a guess was too far off.
@@ -1066,25 +1249,11 @@ struct Counter {
       room = need;
     }
     if (!(want.p < 1.f)) return true;
-    // weights of the bins up to the cut (the cut's own bin: as much as there is room for)
-    groups<true>(middle);
+    group_weights(middle);
     const double wc = cut < kDead - 1 ? weight_at(cut) : 0.0;
     double mass;
-    if (cut < kDead - 1) {
-      // what lies before the cut's bin
-      const uint32_t b = cut >> 16;
-      double m = 0;
-      for (uint32_t g = threadIdx.x; g < b / 32; g += kCountThreads) m += sh.sum[g];
-      if (threadIdx.x < b % 32) {
-        const unsigned c = counter((b & ~31u) + threadIdx.x);
-        m += c ? (double)c * weight_at(middle((b & ~31u) + threadIdx.x)) : 0.0;
-      }
-      mass = total(m) + room * wc;
-    } else {
-      double m = 0;
-      for (int g = threadIdx.x; g < kGroups; g += kCountThreads) m += sh.sum[g];
-      mass = total(m);
-    }
+    // (the cut's own bin: as much as there is room for)
+    mass = cut < kDead - 1 ? weight_before(cut >> 16, middle) + room * wc : weight_before(0x10000u, middle);
     constexpr double kLeast = 1e-300;  // (something is kept, also with top_p 0)
     double target = fmax((double)want.p * mass, kLeast);
     if (!kWide) {
@@ -1098,8 +1267,9 @@ struct Counter {
     }
     // The middles gave a guess of the bin; the weights up to a window around it are added up one by one.
     uint32_t b = locate<true>(target, middle) ? sh.bin : 0xffffu;
-    for (int tries = 0; tries < 4; ++tries) {
-      const uint32_t from = b > kWindow / 2 ? min(b - kWindow / 2, 0x10000u - kWindow) : 0u;
+    uint32_t lo = 0, hi = 0xffffu;  // the bin is one of these
+    for (;;) {
+      const uint32_t from = min(max(b > kWindow / 2 ? b - kWindow / 2 : 0u, lo), max(lo, hi + 1 > kWindow ? hi + 1 - kWindow : 0u));
       __syncthreads();
       if (threadIdx.x < kWindow) sh.window[threadIdx.x] = 0;
       __syncthreads();
@@ -1126,8 +1296,9 @@ struct Counter {
       for (int i = 0; i < kWindow; ++i) in[i] = (double)sh.window[i] * 0x1p-44, all += in[i];
       const uint32_t at = (cut >> 16) - from;
       target = fmax((double)want.p * all, kLeast);
-      if (target <= below && from > 0) {
-        b = from > kWindow / 2 ? from - kWindow / 2 : 0;
+      if (target <= below && from > lo) {  // (the next guess begins at the window's edge, where the sum is known)
+        hi = from - 1;
+        b = locate<true>(fmax(weight_before(from, middle) - (below - target), kLeast), middle) ? sh.bin : hi;
         continue;
       }
       double base = below;
@@ -1139,15 +1310,16 @@ struct Counter {
         if (hit < 0) base += m;
       }
       if (hit < 0) {
-        if (from + kWindow > cut >> 16) return true;  // (p is 1, but for a rounding)
-        b = from + kWindow + kWindow / 2;
+        lo = from + kWindow;
+        if (lo > min(hi, cut >> 16)) return true;  // (p is 1, but for a rounding)
+        b = locate<true>(weight_before(lo, middle) + (target - base), middle) ? sh.bin : hi;
         continue;
       }
       const uint32_t bin = from + hit;
       const unsigned in_bin = counter(bin);
       if (in_bin == 0 || !count_inside(bin, in_bin)) return false;
       auto inside = [bin](uint32_t l) { return bin << 16 | l; };
-      groups<true>(inside);
+      group_weights(inside);
       if (!locate<true>(target - base, inside)) return true;
       const uint32_t key = bin << 16 | sh.bin;
       if (key > cut) return true;
@@ -1156,11 +1328,10 @@ struct Counter {
       cut = key;
       return true;
     }
-    return false;
   }
 
   // The running sums of the kept tokens, by number, and the token where they pass u of them all.
-  __device__ void choose(const Want &want, const Sample &a, long long r) {
+  __device__ void choose(const Want &want, const Sample &a, long long r, uint32_t first) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float lowest = want.floor(top);
     const double wc = weight_at(cut);
@@ -1176,42 +1347,123 @@ struct Counter {
     };
     __syncthreads();
     for (int e = threadIdx.x; e < kGroups; e += kCountThreads) sh.sum[e] = 0.0, sh.cnt[e] = 0;
-    __syncthreads();
-    constexpr int kAtOnce = 2;
-    for (int e0 = warp; e0 < entries; e0 += kAtOnce * kCountWarps) {
-      uint32_t k[kAtOnce][kLanePieces][kEach];
+    if constexpr (kWide) {
+      __syncthreads();
+      constexpr int kAtOnce = 2;
+      for (int e0 = warp; e0 < entries; e0 += kAtOnce * kCountWarps) {
+        uint32_t k[kAtOnce][kLanePieces][kEach];
 #pragma unroll
-      for (int q = 0; q < kAtOnce; ++q)
+        for (int q = 0; q < kAtOnce; ++q)
 #pragma unroll
-        for (int z = 0; z < kLanePieces; ++z) {
-          const int c = ((e0 + q * kCountWarps) * 32 + lane) * kLanePieces + z;
+          for (int z = 0; z < kLanePieces; ++z) {
+            const int c = ((e0 + q * kCountWarps) * 32 + lane) * kLanePieces + z;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) k[q][z][i] = kDead;
-          if (e0 + q * kCountWarps < entries && c < n) keys(c, k[q][z]);
-        }
+            for (int i = 0; i < kEach; ++i) k[q][z][i] = kDead;
+            if (e0 + q * kCountWarps < entries && c < n) keys(c, k[q][z]);
+          }
 #pragma unroll
-      for (int q = 0; q < kAtOnce; ++q) {
-        uint32_t least = kDead;
-#pragma unroll
-        for (int z = 0; z < kLanePieces; ++z)
-#pragma unroll
-          for (int i = 0; i < kEach; ++i) least = min(least, k[q][z][i]);
-        if (!__any_sync(0xffffffffu, least <= cut)) continue;
-        double s = 0;
-        unsigned equal = 0;
-        if (least <= cut) {
+        for (int q = 0; q < kAtOnce; ++q) {
+          uint32_t least = kDead;
 #pragma unroll
           for (int z = 0; z < kLanePieces; ++z)
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-              s += before_cut(k[q][z][i]);
-              equal += k[q][z][i] == cut;
-            }
-        }
-        equal = __reduce_add_sync(0xffffffffu, equal);
+            for (int i = 0; i < kEach; ++i) least = min(least, k[q][z][i]);
+          if (!__any_sync(0xffffffffu, least <= cut)) continue;
+          double s = 0;
+          unsigned equal = 0;
+          if (least <= cut) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
+            for (int z = 0; z < kLanePieces; ++z)
+#pragma unroll
+              for (int i = 0; i < kEach; ++i) {
+                s += before_cut(k[q][z][i]);
+                equal += k[q][z][i] == cut;
+              }
+          }
+          equal = __reduce_add_sync(0xffffffffu, equal);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (lane == 0) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
+        }
+      }
+    } else if ((cut >> 16) - (first >> 16) > sizeof(sh.hist) / sizeof(double)) {
+      // more values than a table holds (or everything) is kept: weights from the logits as they are
+      __syncthreads();
+      constexpr int kAtOnce = 4;
+      const bool bounded = want.min_p > 0.f, all_kept = cut == kDead - 1;
+      const float last = all_kept ? -INFINITY : Key<T>::value(cut);
+      for (int e0 = warp; e0 < entries; e0 += kAtOnce * kCountWarps) {
+        uint4 u[kAtOnce];
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const int c = (e0 + q * kCountWarps) * 32 + lane;
+          u[q] = c < n ? piece(c) : make_uint4(kDead, kDead, kDead, kDead);
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          if (e0 + q * kCountWarps >= entries) break;
+          const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+          double s = 0;
+          unsigned equal = 0;
+          auto weigh = [&](float v) {
+            if (!(v > last)) {
+              equal += v == last;
+            } else if (!bounded || v >= lowest) {
+              const double w = weight(v);
+              s += !bounded || want.enough(w, v == top) ? w : 0.0;
+            }
+          };
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = values2(w[i]);
+            weigh(f.x);
+            weigh(f.y);
+          }
+          equal = __reduce_add_sync(0xffffffffu, equal);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (lane == 0) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
+        }
+      }
+    } else {
+      // the weights of the first kept values, in the counters' place
+      const uint32_t k0 = first >> 16, end = cut >> 16;  // (k0 .. end are kept)
+      double *const table = reinterpret_cast<double *>(sh.hist);
+      for (uint32_t i = threadIdx.x; k0 + i < end; i += kCountThreads) table[i] = before_cut((k0 + i) << 16);
+      __syncthreads();
+      auto weigh = [&](uint32_t k, double &s, unsigned &equal) {
+        if (k < end) s += table[k - k0];
+        equal += k == end;
+      };
+      constexpr int kAtOnce = 4;
+      for (int e0 = warp; e0 < entries; e0 += kAtOnce * kCountWarps) {
+        uint4 u[kAtOnce];
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const int c = (e0 + q * kCountWarps) * 32 + lane;
+          u[q] = c < n ? piece(c) : make_uint4(kDead, kDead, kDead, kDead);
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const uint32_t k[4] = {keys2_zero(u[q].x), keys2_zero(u[q].y), keys2_zero(u[q].z), keys2_zero(u[q].w)};
+          const uint32_t m = __vminu2(__vminu2(k[0], k[1]), __vminu2(k[2], k[3])), least = min(m & 0xffffu, m >> 16);
+          // (a NaN without the sign bit has a smaller key than any logit: it passes here, and weighs nothing below)
+          if (!__any_sync(0xffffffffu, least <= end)) continue;
+          double s = 0;
+          unsigned equal = 0;
+          if (least <= end) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t lo = k[i] & 0xffffu, hi = k[i] >> 16;
+              if (lo >= k0) weigh(lo, s, equal);
+              if (hi >= k0) weigh(hi, s, equal);
+            }
+          }
+          equal = __reduce_add_sync(0xffffffffu, equal);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (lane == 0 && e0 + q * kCountWarps < entries) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
+        }
       }
     }
     __syncthreads();
@@ -1321,9 +1573,17 @@ __global__ void __launch_bounds__(kCountThreads, 1) sample_count_k(const __grid_
   c.x = static_cast<const T *>(a.x) + r * a.stride;
   c.vocab = a.vocab;
   c.skip = (int)(reinterpret_cast<uintptr_t>(c.x) % 16 / sizeof(T));
-  unsigned live;
+  const Want want(a, r);
+  const bool filtered = want.t > 0.f && (want.k || want.p < 1.f);
+  unsigned live = 0;
   uint32_t first;
-  bool fits = c.count_all(live, first);
+  bool fits = true;
+  if (filtered) {
+    fits = c.count_all(live, first);
+  } else {
+    first = c.first_key();
+    live = first != kDead;
+  }
   if (live == 0) {
     if (threadIdx.x == 0) {
       a.tokens[r] = -1;
@@ -1331,18 +1591,16 @@ __global__ void __launch_bounds__(kCountThreads, 1) sample_count_k(const __grid_
     }
     return;
   }
-  const Want want(a, r);
   c.top = Key<T>::value(first);
   c.by = want.t > 0.f ? kPowers * 1.4426950408889634 / (double)want.t : 0.0;
   if (!(want.t > 0.f)) {  // the first of the largest
     c.cut = first;
     c.room = 1;
-    fits = true;
-  } else if (fits) {
+  } else if (fits && filtered) {
     fits = c.select(want, live, first);
   }
   if (fits) {
-    c.choose(want, a, r);
+    c.choose(want, a, r, first);
     return;
   }
   // the other kernel's way, from global memory
@@ -1375,8 +1633,11 @@ cudaError_t launch_count(const Sample &a, cudaStream_t st) {
 template <class T>
 cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
-  const char *env = getenv("IVB_SAMPLE");
-  if (env ? env[0] == 'c' : a.rows >= 100) return launch_count<T>(a, st);
+  // A CTA a row is enough where there are many.  Us in a cluster / by counting, rows of
+  // 131072, with top p / with top k, top p and min p: 16-bit logits, 16 rows 82/68 and
+  // 66/45, 64 rows 154/68 and 123/47; 32 bits, 64 rows 153/156 and 87/170, 148 rows
+  // 285/160 and 164/156.  (One row of 32003: 21/23 and 21/23.)
+  if (a.rows >= (sizeof(T) == 2 ? 24 : 100)) return launch_count<T>(a, st);
   Sample s = a;
   const long long bytes = (long long)a.vocab * sizeof(T);
   s.ranks = 1;
