@@ -38,66 +38,88 @@ __device__ __forceinline__ float mx4_scale(uint32_t e) {  // 2^(e - 127)
   return e == 255 ? __uint_as_float(0x7fc00000u) : e == 0 ? 0x1p-127f : __uint_as_float(e << 23);
 }
 
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 256, kQuantRows = kQuantThreads / 32;
 
-// A thread takes eight values, four lanes a block of 32, a warp 256 of a row.
-// Memory bounds it: 2 + 17 / 32 bytes a value.
-template <bool BF16>
-__global__ void __launch_bounds__(kQuantThreads) mx4_quantize_k(const uint16_t *x, long long rows, long long stride,
-                                                               int vec, Mx4 m, int pieces, long long units) {
-  const int lane = threadIdx.x & 31;
-  const long long chunks = (m.width + 127) / 128;
+// A warp takes N pieces of 256 of a row (one after another in a launch's x), a thread eight
+// values of each, four lanes a block of 32; a CTA eight rows.  Memory bounds it (2 + 17 /
+// 32 bytes a value), if few instructions are spent on a value: maxima go by the bits,
+// two values an instruction, and a block with a NaN or an infinity takes another path.
+// (8191 x 8192: TODO us.)
+template <bool BF16, int N>
+__global__ void __launch_bounds__(kQuantThreads) mx4_quantize_k(const uint16_t *x, long long rows, long long padded,
+                                                               long long stride, int vec, Mx4 m) {
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+  const int lane = threadIdx.x & 31, width = (int)m.width, chunks = (width + 127) / 128;
+  const int c0 = blockIdx.x * (256 * N) + lane * 8;
   pdl_wait_and_release();
-  for (long long u = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units;
-       u += (long long)gridDim.x * (kQuantThreads / 32)) {
-    const long long r = u / pieces;
-    const long long c0 = (u - r * pieces) * 256 + lane * 8;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const bool there = r < rows && c0 < m.width;
-    if (there) unpack8<BF16>(load8(x + r * stride + c0, vec), f);
-    float most = 0.f;
+  for (long long r = (long long)blockIdx.y * kQuantRows + (threadIdx.x >> 5); r < padded; r += (long long)gridDim.y * kQuantRows) {
+    uint4 w[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (f[i] != f[i]) f[i] = 0.f;
-      if (fabsf(f[i]) < INFINITY) most = fmaxf(most, fabsf(f[i]));
+    for (int q = 0; q < N; ++q) w[q] = r < rows && c0 + 256 * q < width ? load8(x + r * stride + c0 + 256 * q, vec) : make_uint4(0, 0, 0, 0);
+    uint32_t *const codes = reinterpret_cast<uint32_t *>(m.codes + r * (width / 2) + c0 / 2);
+    uint8_t *const scales = m.scales + mx4_scale_at(r, c0 / 32, chunks);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      uint32_t two = __vmaxu2(__vmaxu2(w[q].x & 0x7fff7fffu, w[q].y & 0x7fff7fffu), __vmaxu2(w[q].z & 0x7fff7fffu, w[q].w & 0x7fff7fffu));
+      two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 1));
+      two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 2));
+      uint32_t top = max(two & 0xffffu, two >> 16);
+      float f[8];
+      unpack8<BF16>(w[q], f);
+      if (__any_sync(0xffffffffu, top >= kInf)) {  // (the largest finite one; NaN is 0)
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = fabsf(f[i]);
+          most = fmaxf(most, a < INFINITY ? a : 0.f);
+          f[i] = f[i] != f[i] ? 0.f : f[i];
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        top = pack2<BF16>(most, 0.f) & 0xffffu;
+      }
+      const float most = BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+      const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
+      const float by = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= by;
+      if (r < rows && c0 + 256 * q < width) codes[32 * q] = mx4_codes(f);
+      // four blocks' bytes in one word
+      uint32_t word = (uint32_t)e << (8 * ((lane >> 2) & 3));
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if ((lane & 15) == 0 && c0 + 256 * q < chunks * 128) *reinterpret_cast<uint32_t *>(scales + 1024 * q) = word;
     }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
-    const float by = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= by;
-    if (there) *reinterpret_cast<uint32_t *>(m.codes + r * (m.width / 2) + c0 / 2) = mx4_codes(f);
-    // four blocks' bytes in one word
-    uint32_t word = (uint32_t)e << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    if ((lane & 15) == 0 && c0 < chunks * 128)
-      *reinterpret_cast<uint32_t *>(m.scales + mx4_scale_at(r, c0 / 32, chunks)) = word;
   }
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kQuantThreads) mx4_read_k(Mx4 m, long long rows, uint16_t *out, long long stride,
-                                                           int vec, int pieces, long long units) {
-  const int lane = threadIdx.x & 31;
-  const long long chunks = (m.width + 127) / 128;
+template <bool BF16, int N>
+__global__ void __launch_bounds__(kQuantThreads) mx4_read_k(Mx4 m, long long rows, uint16_t *out, long long stride, int vec) {
+  const int lane = threadIdx.x & 31, width = (int)m.width, chunks = (width + 127) / 128;
+  const int c0 = blockIdx.x * (256 * N) + lane * 8;
   pdl_wait_and_release();
-  for (long long u = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); u < units;
-       u += (long long)gridDim.x * (kQuantThreads / 32)) {
-    const long long r = u / pieces;
-    const long long c0 = (u - r * pieces) * 256 + lane * 8;
-    if (c0 >= m.width) continue;
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(m.codes + r * (m.width / 2) + c0 / 2);
-    const float s = mx4_scale(m.scales[mx4_scale_at(r, c0 / 32, chunks)]);
-    float f[8];
+  for (long long r = (long long)blockIdx.y * kQuantRows + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.y * kQuantRows) {
+    const uint32_t *const codes = reinterpret_cast<const uint32_t *>(m.codes + r * (width / 2) + c0 / 2);
+    const uint8_t *const scales = m.scales + mx4_scale_at(r, c0 / 32, chunks);
+    uint32_t w[N], e[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = mx4_pair(w >> (8 * i));
-      f[2 * i] = p.x * s;
-      f[2 * i + 1] = p.y * s;
+    for (int q = 0; q < N; ++q) {
+      const bool there = c0 + 256 * q < width;
+      w[q] = there ? codes[32 * q] : 0u;
+      e[q] = there ? scales[1024 * q] : 0u;
     }
-    store8(out + r * stride + c0, pack8<BF16>(f), vec);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const float s = mx4_scale(e[q]);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 p = mx4_pair(w[q] >> (8 * i));
+        f[2 * i] = p.x * s;
+        f[2 * i + 1] = p.y * s;
+      }
+      if (c0 + 256 * q < width) store8(out + r * stride + c0 + 256 * q, pack8<BF16>(f), vec);
+    }
   }
 }
 
@@ -470,21 +492,30 @@ cudaError_t linear_rows(const Mx4Linear &l, cudaStream_t st) {
   return linear_tiles<192, BF16>(l, st);
 }
 
+// Pieces of a warp, and the grid: few values go to many warps.
+dim3 quant_grid(long long width, long long rows, bool &four) {
+  const long long blocks = (rows + kQuantRows - 1) / kQuantRows;
+  four = width > 256 && blocks * ((width + 1023) / 1024) >= 148 * 2;
+  const long long x = (width + (four ? 1023 : 255)) / (four ? 1024 : 256);
+  return dim3((unsigned)x, (unsigned)std::min(blocks, std::max(1ll, 148 * 8 / x)));
+}
+
 template <bool BF16>
 cudaError_t quantize(const void *x, long long rows, long long stride, const Mx4 &m, cudaStream_t st) {
-  const int pieces = (int)((m.width + 255) / 256);
-  const long long units = (rows + 127) / 128 * 128 * pieces;  // (scale bytes of rows that are not there are 0)
-  const long long grid = std::min<long long>((units + kQuantThreads / 32 - 1) / (kQuantThreads / 32), 148 * 8);
-  return launch_kernel(mx4_quantize_k<BF16>, dim3((unsigned)grid), dim3(kQuantThreads), 0, st, static_cast<const uint16_t *>(x), rows,
-                       stride, (int)rows_vec(x, stride), m, pieces, units);
+  const long long padded = (rows + 127) / 128 * 128;  // (scale bytes of rows that are not there are 0)
+  bool four;
+  const dim3 grid = quant_grid(m.width, padded, four);
+  const uint16_t *p = static_cast<const uint16_t *>(x);
+  if (four) return launch_kernel(mx4_quantize_k<BF16, 4>, grid, dim3(kQuantThreads), 0, st, p, rows, padded, stride, (int)rows_vec(x, stride), m);
+  return launch_kernel(mx4_quantize_k<BF16, 1>, grid, dim3(kQuantThreads), 0, st, p, rows, padded, stride, (int)rows_vec(x, stride), m);
 }
 template <bool BF16>
 cudaError_t read(const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st) {
-  const int pieces = (int)((m.width + 255) / 256);
-  const long long units = rows * pieces;
-  const long long grid = std::min<long long>((units + kQuantThreads / 32 - 1) / (kQuantThreads / 32), 148 * 8);
-  return launch_kernel(mx4_read_k<BF16>, dim3((unsigned)grid), dim3(kQuantThreads), 0, st, m, rows, static_cast<uint16_t *>(out), stride,
-                       (int)rows_vec(out, stride), pieces, units);
+  bool four;
+  const dim3 grid = quant_grid(m.width, rows, four);
+  uint16_t *p = static_cast<uint16_t *>(out);
+  if (four) return launch_kernel(mx4_read_k<BF16, 4>, grid, dim3(kQuantThreads), 0, st, m, rows, p, stride, (int)rows_vec(out, stride));
+  return launch_kernel(mx4_read_k<BF16, 1>, grid, dim3(kQuantThreads), 0, st, m, rows, p, stride, (int)rows_vec(out, stride));
 }
 
 }  // namespace

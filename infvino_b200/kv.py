@@ -116,17 +116,16 @@ class KvCache:
         self._c = _native.KV_CACHE.pack(*ptrs, self.pages, self.page_size, self.kv_heads, self.head_dim)
 
 
-def _matrix(t, name: str, device: int, shape=None):
+def _matrix(t, name: str, device: int, rows=None, width=None):
     """Address, row stride and dtype of a float16 or bfloat16 [rows, width] tensor whose last dimension is dense."""
-    kind = _name(t)
-    if t.get_device() != device:
-        raise ValueError(f"{name}: expected a tensor on CUDA device {device}")
-    if kind not in _DTYPES or t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name}: expected float16 or bfloat16 {'[rows, width]' if shape is None else tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    st = t.stride()
-    if st[1] != 1 and t.shape[1] > 1:
-        raise ValueError(f"{name}: the last dimension must be dense")
-    return t.data_ptr(), st[0], _DTYPES[kind]
+    kind, sh, st = _DTYPES.get(_names.get(t.dtype) or _name(t)), t.shape, t.stride()
+    if kind is None or t.get_device() != device or len(sh) != 2 or st[1] != 1 or (rows is not None and (sh[0] != rows or sh[1] != width)):
+        _need(t.get_device() == device, f"{name}: expected a tensor on CUDA device {device}")
+        want = "[rows, width]" if rows is None else [rows, width]
+        ok = kind is not None and len(sh) == 2 and (rows is None or (sh[0] == rows and sh[1] == width))
+        _need(ok, f"{name}: expected float16 or bfloat16 {want}, got {t.dtype} {tuple(sh)}")
+        _need(sh[1] <= 1, f"{name}: the last dimension must be dense")
+    return t.data_ptr(), st[0], kind
 
 
 class Mx4:
@@ -135,21 +134,24 @@ class Mx4:
     ceil(width / 128), 32, 4, 4] (the exponent byte of block b of row r is at
     [r // 128, b // 4, r % 32, r % 128 // 32, b % 4])."""
 
+    __slots__ = ("rows", "width", "device", "_keep", "_m")
+
     def __init__(self, codes, scales):
         c, s = _dense(codes, "codes", "uint8", 2), _dense(scales, "scales", "uint8", 5)
-        self.rows, half = codes.shape
-        self.width = 2 * half
-        _need(half % (GROUP // 2) == 0 and half > 0, "codes: expected [rows, width / 2], width a multiple of 32")
-        want = self.scales_shape(self.rows, self.width)
-        _need(tuple(scales.shape) == want, f"scales: expected shape {want}, got {tuple(scales.shape)}")
-        self.device = codes.get_device()
-        _need(scales.get_device() == self.device, "codes and scales are on different devices")
+        rows, half = codes.shape
+        if half % (GROUP // 2) or not half:
+            raise ValueError("codes: expected [rows, width / 2], width a multiple of 32")
+        if scales.shape != ((rows + 127) >> 7, (half + 63) >> 6, 32, 4, 4):
+            raise ValueError(f"scales: expected shape {self.scales_shape(rows, 2 * half)}, got {tuple(scales.shape)}")
+        self.rows, self.width, self.device = rows, 2 * half, codes.get_device()
+        if scales.get_device() != self.device:
+            raise ValueError("codes and scales are on different devices")
         self._keep = (codes, scales)
-        self._m = _native.MX4.pack(c, s, self.rows, self.width)
+        self._m = _native.MX4.pack(c, s, rows, 2 * half)
 
     @staticmethod
     def scales_shape(rows: int, width: int):
-        return (-(-rows // 128), -(-width // 128), 32, 4, 4)
+        return ((rows + 127) // 128, (width + 127) // 128, 32, 4, 4)
 
 
 class KvOps:
@@ -163,7 +165,8 @@ class KvOps:
             raise NativeError(st, (L.ivc_kv_last_error(None) or b"").decode())
         self._h, self._L = h, L
         self._rope, self._append, self._read, self._attend = L.ivc_kv_rope, L.ivc_kv_append, L.ivc_kv_read, L.ivc_kv_attend
-        self._shared, self._sample, self._linear = L.ivc_kv_attend_shared, L.ivc_kv_sample, L.ivc_kv_mx4_linear
+        self._shared, self._sample = L.ivc_kv_attend_shared, L.ivc_kv_sample
+        self._quantize, self._mx4_read, self._linear = L.ivc_kv_mx4_quantize, L.ivc_kv_mx4_read, L.ivc_kv_mx4_linear
         self.device = device
 
     def close(self) -> None:
@@ -313,61 +316,67 @@ class KvOps:
         or None; a temperature of 0 takes the first of the largest logits; a row of
         -inf gives -1."""
         d = self.device
-        if logits.get_device() != d:
-            raise ValueError(f"logits: expected a tensor on CUDA device {d}")
-        kind = _name(logits)
-        if kind not in _LOGITS or logits.dim() != 2:
-            raise ValueError(f"logits: expected float16, bfloat16 or float32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
-        (rows, vocab), st = logits.shape, logits.stride()
-        _need(st[1] == 1 or vocab == 1, "logits: the last dimension must be dense")
-
-        def each(t, name, dtype):
+        kind, sh = _LOGITS.get(_names.get(logits.dtype) or _name(logits)), logits.shape
+        if kind is None or len(sh) != 2 or logits.get_device() != d:
+            _need(logits.get_device() == d, f"logits: expected a tensor on CUDA device {d}")
+            raise ValueError(f"logits: expected float16, bfloat16 or float32 [rows, vocab], got {logits.dtype} {tuple(sh)}")
+        (rows, vocab), st = sh, logits.stride()
+        if st[1] != 1 and vocab != 1:
+            raise ValueError("logits: the last dimension must be dense")
+        each = []
+        for t, name, dtype in ((u, "u", "float32"), (temperature, "temperature", "float32"), (top_k, "top_k", "int32"), (top_p, "top_p", "float32"),
+                               (min_p, "min_p", "float32"), (tokens, "tokens", "int32"), (probs, "probs", "float32")):
             if t is None:
-                return 0
-            p = _dense(t, name, dtype, 1, d)
-            _need(t.shape[0] == rows, f"{name}: expected {rows} entries, got {t.shape[0]}")
-            return p
-
-        how = _native.SAMPLING.pack(each(u, "u", "float32"), each(temperature, "temperature", "float32"), each(top_k, "top_k", "int32"),
-                                    each(top_p, "top_p", "float32"), each(min_p, "min_p", "float32"))
-        st = self._sample(self._h, _native.LOGITS.pack(logits.data_ptr(), _LOGITS[kind], rows, vocab, st[0]), how,
-                          each(tokens, "tokens", "int32"), each(probs, "probs", "float32"), stream)
+                each.append(0)
+                continue
+            each.append(_dense(t, name, dtype, 1, d))
+            if t.shape[0] != rows:
+                raise ValueError(f"{name}: expected {rows} entries, got {t.shape[0]}")
+        st = self._sample(self._h, _native.LOGITS.pack(logits.data_ptr(), kind, rows, vocab, st[0]), _native.SAMPLING.pack(*each[:5]), each[5], each[6],
+                          stream)
         if st:
             self._fail(st)
 
-    def _mx4(self, m: Mx4, name: str) -> bytes:
-        if m.device != self.device:
-            raise ValueError(f"{name}: expected tensors on CUDA device {self.device}")
-        return m._m
+    def _rows_of(self, t, name: str, m: Mx4):
+        p, st, dt = _matrix(t, name, self.device)
+        rows, width = t.shape
+        if width != m.width or rows > m.rows or m.device != self.device:
+            _need(m.device == self.device, f"m: expected tensors on CUDA device {self.device}")
+            raise ValueError(f"{name}: expected width {m.width} and at most {m.rows} rows, got {tuple(t.shape)}")
+        return p, rows, st, dt
 
     def mx4_quantize(self, x, m: Mx4, stream: int = 0) -> None:
         """The first rows of m = x [rows, width] (float16 or bfloat16), width m's, rows at most m's."""
-        p, st, dt = _matrix(x, "x", self.device)
-        _need(x.shape[1] == m.width and x.shape[0] <= m.rows, f"x: expected width {m.width} and at most {m.rows} rows, got {tuple(x.shape)}")
-        self._check(self._L.ivc_kv_mx4_quantize(self._h, dt, p, x.shape[0], st, self._mx4(m, "m"), stream))
+        p, rows, st, dt = self._rows_of(x, "x", m)
+        st = self._quantize(self._h, dt, p, rows, st, m._m, stream)
+        if st:
+            self._fail(st)
 
     def mx4_read(self, m: Mx4, out, stream: int = 0) -> None:
         """out [rows, width] (float16 or bfloat16) = the values of m's first rows."""
-        p, st, dt = _matrix(out, "out", self.device)
-        _need(out.shape[1] == m.width and out.shape[0] <= m.rows, f"out: expected width {m.width} and at most {m.rows} rows, got {tuple(out.shape)}")
-        self._check(self._L.ivc_kv_mx4_read(self._h, self._mx4(m, "m"), out.shape[0], dt, p, st, stream))
+        p, rows, st, dt = self._rows_of(out, "out", m)
+        st = self._mx4_read(self._h, m._m, rows, dt, p, st, stream)
+        if st:
+            self._fail(st)
 
     def mx4_linear(self, x, w: Mx4, out, scratch: Optional[Mx4] = None, stream: int = 0) -> None:
         """out [rows, w.rows] = x w^T with both in 4 bits: x is an `Mx4`, or a
-        float16 / bfloat16 tensor [rows, width] that is first quantised into
-        `scratch`.  Sums are in 32 bits."""
-        o, ost, odt = _matrix(out, "out", self.device)
+        float16 / bfloat16 tensor [rows, width], which is quantised on the way;
+        `scratch` is room for that (an Mx4 of at least as many rows, whose contents
+        are not defined afterwards).  Sums are in 32 bits."""
+        d, width = self.device, w.width
         rows = out.shape[0]
-        if isinstance(x, Mx4):
-            p, st, dt, xq = None, 0, 0, x
+        o, ost, odt = _matrix(out, "out", d, rows, w.rows)
+        if x.__class__ is Mx4:
             _need(scratch is None, "scratch: x is quantised already")
+            p, st, dt, xq = None, 0, 0, x
         else:
-            p, st, dt = _matrix(x, "x", self.device)
             _need(scratch is not None, "scratch: an Mx4 that x is quantised into")
-            _need(tuple(x.shape) == (rows, w.width), f"x: expected {(rows, w.width)}, got {tuple(x.shape)}")
+            p, st, dt = _matrix(x, "x", d, rows, width)
             xq = scratch
-        _need(xq.width == w.width and xq.rows >= rows, f"x: expected width {w.width} and at least {rows} rows, got {(xq.rows, xq.width)}")
-        _need(out.shape[1] == w.rows, f"out: expected {w.rows} columns, got {out.shape[1]}")
-        st = self._linear(self._h, dt, p, rows, st, self._mx4(xq, "x"), self._mx4(w, "w"), odt, o, ost, stream)
+        if xq.width != width or xq.rows < rows or xq.device != d or w.device != d:
+            _need(xq.device == d and w.device == d, f"w, x and scratch: expected tensors on CUDA device {d}")
+            raise ValueError(f"x: expected width {width} and at least {rows} rows, got {(xq.rows, xq.width)}")
+        st = self._linear(self._h, dt, p, rows, st, xq._m, w._m, odt, o, ost, stream)
         if st:
             self._fail(st)
