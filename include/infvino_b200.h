@@ -430,8 +430,9 @@ int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64
 /* out = the values of m's first `rows` rows, rounded once (out_stride elements apart). */
 int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *out, int64_t out_stride, void *stream);
 /* out [rows][w->rows] = X W^T, summed in f32 and rounded once: W is w; X is the
- * first `rows` rows of xq, which x [rows][width] (x_dtype) is quantised into first
- * unless it is NULL.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
+ * first `rows` rows of xq if x is NULL, else x [rows][width] (x_dtype), quantised as
+ * ivc_kv_mx4_quantize does it: xq is room for that then, and what it holds
+ * afterwards is not defined.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
 int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
                       const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream);
 

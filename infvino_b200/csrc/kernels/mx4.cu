@@ -38,17 +38,48 @@ __device__ __forceinline__ float mx4_scale(uint32_t e) {  // 2^(e - 127)
   return e == 255 ? __uint_as_float(0x7fc00000u) : e == 0 ? 0x1p-127f : __uint_as_float(e << 23);
 }
 
+// Eight values of a block of 32, four neighbouring lanes each, as codes; the scale's
+// byte is returned.  Maxima go by the bits, two values an instruction; a block with a
+// NaN or an infinity takes another path.
+template <bool BF16>
+__device__ __forceinline__ int mx4_block(uint4 w, uint32_t &codes) {
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+  uint32_t two = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+  two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 1));
+  two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 2));
+  uint32_t top = max(two & 0xffffu, two >> 16);
+  float f[8];
+  unpack8<BF16>(w, f);
+  if (__any_sync(0xffffffffu, top >= kInf)) {  // (the largest finite one; NaN is 0)
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = fabsf(f[i]);
+      most = fmaxf(most, a < INFINITY ? a : 0.f);
+      f[i] = f[i] != f[i] ? 0.f : f[i];
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    top = pack2<BF16>(most, 0.f) & 0xffffu;
+  }
+  const float most = BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+  const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
+  const float by = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] *= by;
+  codes = mx4_codes(f);
+  return e;
+}
+
 constexpr int kQuantThreads = 256, kQuantRows = kQuantThreads / 32;
 
 // A warp takes N pieces of 256 of a row (one after another in a launch's x), a thread eight
 // values of each, four lanes a block of 32; a CTA eight rows.  Memory bounds it (2 + 17 /
-// 32 bytes a value), if few instructions are spent on a value: maxima go by the bits,
-// two values an instruction, and a block with a NaN or an infinity takes another path.
-// (8191 x 8192: TODO us.)
+// 32 bytes a value), if few instructions are spent on a value (8191 x 8192: 33 us, 5.2
+// TB/s; with maxima in f32 and a row and column for each piece 61).
 template <bool BF16, int N>
 __global__ void __launch_bounds__(kQuantThreads) mx4_quantize_k(const uint16_t *x, long long rows, long long padded,
                                                                long long stride, int vec, Mx4 m) {
-  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
   const int lane = threadIdx.x & 31, width = (int)m.width, chunks = (width + 127) / 128;
   const int c0 = blockIdx.x * (256 * N) + lane * 8;
   pdl_wait_and_release();
@@ -60,32 +91,11 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quantize_k(const uint16_t *
     uint8_t *const scales = m.scales + mx4_scale_at(r, c0 / 32, chunks);
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      uint32_t two = __vmaxu2(__vmaxu2(w[q].x & 0x7fff7fffu, w[q].y & 0x7fff7fffu), __vmaxu2(w[q].z & 0x7fff7fffu, w[q].w & 0x7fff7fffu));
-      two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 1));
-      two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 2));
-      uint32_t top = max(two & 0xffffu, two >> 16);
-      float f[8];
-      unpack8<BF16>(w[q], f);
-      if (__any_sync(0xffffffffu, top >= kInf)) {  // (the largest finite one; NaN is 0)
-        float most = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = fabsf(f[i]);
-          most = fmaxf(most, a < INFINITY ? a : 0.f);
-          f[i] = f[i] != f[i] ? 0.f : f[i];
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        top = pack2<BF16>(most, 0.f) & 0xffffu;
-      }
-      const float most = BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
-      const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
-      const float by = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= by;
-      if (r < rows && c0 + 256 * q < width) codes[32 * q] = mx4_codes(f);
+      uint32_t word;
+      const int e = mx4_block<BF16>(w[q], word);
+      if (r < rows && c0 + 256 * q < width) codes[32 * q] = word;
       // four blocks' bytes in one word
-      uint32_t word = (uint32_t)e << (8 * ((lane >> 2) & 3));
+      word = (uint32_t)e << (8 * ((lane >> 2) & 3));
       word |= __shfl_xor_sync(0xffffffffu, word, 4);
       word |= __shfl_xor_sync(0xffffffffu, word, 8);
       if ((lane & 15) == 0 && c0 + 256 * q < chunks * 128) *reinterpret_cast<uint32_t *>(scales + 1024 * q) = word;
@@ -138,36 +148,55 @@ bool rows_vec(const void *p, long long stride) { return reinterpret_cast<uintptr
 //   warp 0     brings a stage's codes (TMA, 128-byte swizzled lines) and scales (as they
 //              lie in memory: 512 bytes for 128 rows x 128 of the width)
 //   warp 1     copies a stage's scales into TMEM and issues its products
-//   warps 2-5  take a finished tile out of TMEM: a thread a weight row
-// Two accumulators: a tile's products run while the one before it goes out.
+//   warps 2 .. take a finished tile out of TMEM: a thread a weight row
+// Two sets of accumulators: a tile's products run while the one before it goes out.
 //
 // Every wait is bounded: a timeout sets the status word and an abort flag, all
 // roles run out, and parts of cut tiles are counted all the same.
-constexpr int kMm = 128;             // weight rows of a tile
+constexpr int kMm = 128;             // weight rows of an instruction
 constexpr int kStageK = 256;         // of the width
-constexpr int kLinearThreads = 192;
-constexpr int kMaxTokens = 192;      // of a tile
+constexpr int kFuseWarps = 4;
 
-template <int TN>
+// MT: weight tiles of 128 rows that share a stage's tokens.  What an SM gets from the L2 in
+// a clock (some 38 bytes when all ask) bounds products with many tokens, and weights,
+// from memory, queue up behind tokens in the copies of those with some: two weight tiles
+// halve the tokens' part.
+template <int TN, int MT>
 struct Tile {
-  static constexpr int kRowTiles = (TN + 127) / 128;       // 128-row scale pieces a stage may touch
-  static constexpr uint32_t kA = kMm * 128, kB = TN * 128, kSa = 1024, kSb = 1024 * kRowTiles;
+  static constexpr int kRows = 128 * MT;                   // weight rows of a tile
+  static constexpr int kRowTiles = (TN + 127) / 128;       // 128-row scale pieces of the tokens that a stage may touch
+  static constexpr uint32_t kA = kRows * 128, kB = TN * 128, kSa = 1024 * MT, kSb = 1024 * kRowTiles;
   static constexpr uint32_t kStage = kA + kB + kSa + kSb;
-  static constexpr int kStages = TN == 16 ? 10 : TN == 32 ? 9 : TN == 64 ? 8 : TN == 128 ? 6 : 5;
+  // Up to 64 tokens two CTAs fit on an SM: the next launch's CTAs set themselves up, and ask for
+  // their weights, while this one's end.
+  static constexpr int kCtas = TN <= 64 && MT == 1 ? 2 : 1;
+  static constexpr int kStages = MT == 2 ? (TN == 64 ? 5 : 3) : TN == 16 ? 5 : TN <= 64 ? 4 : TN == 128 ? 6 : 5;
   static constexpr int kD = TN < 32 ? 32 : TN;             // columns of an accumulator
-  static constexpr int kScaleCols = 8 + 8 * kRowTiles;     // columns of a stage's scales
+  // Two sets of accumulators where they fit.  (256 x 192: one; the loads go on while it is emptied.)
+  static constexpr int kBufs = MT == 2 && TN > 64 ? 1 : 2;
+  static constexpr int kScaleCols = 8 * (MT + kRowTiles);  // columns of a stage's scales
+  static constexpr int kTmem = 512 / kCtas;
   static constexpr int kSmem = kStage * kStages + 1024;
-  static_assert(2 * kD + kStages * kScaleCols <= 512, "TMEM");
+  static constexpr int kThreads = 64 + 128 * MT;           // loads, products, and four warps for each weight tile's results
+  // Many tokens: X and W change places (X's rows are the lanes), so that a thread has
+  // neighbouring outputs of a token and stores 32 bytes at once.
+  static constexpr bool kSwap = MT == 2 && TN > 64;
+  static_assert(kBufs * MT * kD + kStages * kScaleCols <= kTmem, "TMEM");
+  static_assert(kSmem * kCtas <= 224 << 10, "shared memory");
 };
 
 struct LinearArgs {
-  CUtensorMap wmap, xmap;
-  const uint8_t *ws, *xs;   // scales
+  CUtensorMap wmap, xmap;   // of the lanes' matrix (W, or X where they change places), of the columns'
+  const uint16_t *x;        // FUSED: rows that are quantised on the way
+  long long x_stride;
+  int x_vec;
+  const uint8_t *ws, *xs;   // their scales
   uint16_t *out;
   long long stride;
+  int out_vec;              // rows of outputs on 32 bytes
   long long chunks;         // 128-wide scale pieces of a row
   int rows, outputs, width;
-  int m_tiles, ks;          // weight tiles; stages of a tile
+  int m_tiles, ks;          // tiles of lanes; stages of a tile
   uint32_t units, size;     // in all; of a CTA's share
   int fresh;
   float *slots;
@@ -198,6 +227,14 @@ struct LinearWalk {
   }
 };
 
+__device__ __forceinline__ void prefetch_2d(const void *map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ unsigned count_acq_rel(unsigned *p) {  // (what the block's barrier has put before it is released too)
+  unsigned v;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                : "memory");
@@ -216,26 +253,47 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
       : "memory");
 }
 
-template <int TN, bool BF16>
-__global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_constant__ LinearArgs a) {
-  using S = Tile<TN>;
+// FUSE: 0: X comes from memory in 4 bits; 1, 2: from halves / bf16 rows, which the CTA
+// quantises itself, with kFuseWarps more warps.  Few rows: every CTA does it for its
+// stages again, but a launch is saved, and the weights are on their way meanwhile.
+// Sixteen outputs of a token, the first n of them.
+template <bool BF16>
+__device__ __forceinline__ void store_outputs(uint16_t *out, const float (&v)[16], int n, bool vec) {
+  if (n >= 16 && vec) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack2<BF16>(v[2 * i], v[2 * i + 1]);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < n) out[i] = (uint16_t)pack2<BF16>(v[i], v[i]);
+}
+
+template <int TN, int MT, bool BF16, int FUSE>
+__global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWarps : 0), Tile<TN, MT>::kCtas)
+    mx4_linear_k(const __grid_constant__ LinearArgs a) {
+  using S = Tile<TN, MT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages], accfull[2], accempty[2], drained;
   __shared__ uint32_t tmem_sh;
   __shared__ volatile int abort_sh;
-  __shared__ int last_sh;
+  __shared__ int last_sh[MT];
   constexpr long long kLimit = kConvWaitLimitDefault;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&full[i]), 1), mbar_init(smem_u32(&empty[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&accfull[i]), 1), mbar_init(smem_u32(&accempty[i]), 4);
+    for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&full[i]), FUSE ? 2 : 1), mbar_init(smem_u32(&empty[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&accfull[i]), 1), mbar_init(smem_u32(&accempty[i]), 4 * MT);
     mbar_init(smem_u32(&drained), 1);
     abort_sh = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_sh), 512);
+    tmem_alloc(smem_u32(&tmem_sh), S::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -245,7 +303,15 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
 
   if (warp == 0) {
     // ---- loads
-    if (!a.fresh) pdl_wait();
+    if (!a.fresh) {
+      // (into the L2 for now, which is no reading: what comes before this launch may still write them)
+      LinearWalk w(a);
+      int left = S::kStages;
+      while (left > 0 && w.next(a))
+        for (int k = w.k0; k < w.k1 && left > 0; ++k, --left)
+          if (elect_one()) prefetch_2d(&a.wmap, k * 128, w.m * S::kRows);
+      pdl_wait();
+    }
     // (after a fresh quantisation the weights are there already: their first stages come before it has ended)
     bool waited = !a.fresh;
     if (waited) pdl_release();
@@ -254,6 +320,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
     bool more = tokens.next(a);
     int tk = tokens.k0;
     auto load_tokens = [&](uint32_t i) {
+      if (FUSE) return;
       const uint32_t s = i % S::kStages, at = ring + s * S::kStage, bar = smem_u32(&full[s]);
       const int chunks = (int)min(2ll, a.chunks - 2 * tk);
       const long long rt = (long long)tokens.t * TN / 128;
@@ -261,7 +328,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
         tma_load_2d(at + S::kA, &a.xmap, bar, tk * 128, tokens.t * TN);
 #pragma unroll
         for (int r = 0; r < S::kRowTiles; ++r)
-          if ((rt + r) * 128 < a.rows)
+          if ((rt + r) * 128 < (S::kSwap ? a.outputs : a.rows))
             bulk_load(at + S::kA + S::kB + S::kSa + 1024u * r, a.xs + ((rt + r) * a.chunks + 2 * tk) * 512, 512u * chunks, bar);
       }
       if (++tk == tokens.k1 && (more = tokens.next(a))) tk = tokens.k0;
@@ -283,13 +350,16 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
         const uint32_t at = ring + s * S::kStage, bar = smem_u32(&full[s]);
         const int chunks = (int)min(2ll, a.chunks - 2 * k);
         const long long rt = (long long)w.t * TN / 128;
-        uint32_t pieces = 1;
+        const long long mt0 = (long long)w.m * MT;
+        const int mts = MT == 1 || (mt0 + 1) * kMm < (S::kSwap ? a.rows : a.outputs) ? MT : 1;
+        uint32_t pieces = (uint32_t)mts;
 #pragma unroll
-        for (int r = 0; r < S::kRowTiles; ++r) pieces += (rt + r) * 128 < a.rows;
+        for (int r = 0; r < S::kRowTiles; ++r) pieces += !FUSE && (rt + r) * 128 < (S::kSwap ? a.outputs : a.rows);
         if (elect_one()) {
-          mbar_expect_tx(bar, S::kA + S::kB + 512u * chunks * pieces);
-          tma_load_2d(at, &a.wmap, bar, k * 128, w.m * kMm);
-          bulk_load(at + S::kA + S::kB, a.ws + ((long long)w.m * a.chunks + 2 * k) * 512, 512u * chunks, bar);
+          mbar_expect_tx(bar, S::kA + (FUSE ? 0 : S::kB) + 512u * chunks * pieces);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) tma_load_2d(at + m * (kMm * 128), &a.wmap, bar, k * 128, w.m * S::kRows + m * kMm);
+          for (int m = 0; m < mts; ++m) bulk_load(at + S::kA + S::kB + 1024u * m, a.ws + ((mt0 + m) * a.chunks + 2 * k) * 512, 512u * chunks, bar);
         }
         __syncwarp();
         if (waited)
@@ -318,12 +388,12 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
     LinearWalk w(a);
     bool ok = true;
     while (ok && w.next(a)) {
-      const uint32_t buf = tile & 1u, use = tile >> 1;
+      const uint32_t buf = tile % S::kBufs, use = tile / S::kBufs;
       if (use > 0) ok = mbar_wait_bounded(smem_u32(&accempty[buf]), (use - 1u) & 1u, &abort_sh, a.status, kStatusTimeoutAccEmpty, kLimit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem + buf * S::kD;
+      const uint32_t d = tmem + buf * (MT * S::kD);
       const uint32_t group = (uint32_t)(((long long)w.t * TN % 128) / 32);  // first 32 tokens of the tile in their scale piece
       for (int k = w.k0; k < w.k1; ++k, ++n) {
         const uint32_t s = n % S::kStages;
@@ -332,21 +402,24 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
         if (!ok) break;
         tc_fence_after();
         const uint32_t at = ring + s * S::kStage;
-        const uint32_t sc = tmem + 2 * S::kD + s * S::kScaleCols;
+        const uint32_t sa = tmem + S::kBufs * MT * S::kD + s * S::kScaleCols, sb = sa + 8 * MT;  // (four columns for each 128 rows and 128 of the width)
         const int steps = min(kStageK / 64, (a.width - k * kStageK + 63) / 64);
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            scales_to_tmem(sc + 4 * c, at + S::kA + S::kB + 512 * c);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) scales_to_tmem(sa + 8 * m + 4 * c, at + S::kA + S::kB + 1024 * m + 512 * c);
 #pragma unroll
             for (int r = 0; r < S::kRowTiles; ++r)
-              scales_to_tmem(sc + 8 + 4 * S::kRowTiles * c + 4 * r, at + S::kA + S::kB + S::kSa + 1024 * r + 512 * c);
+              scales_to_tmem(sb + 4 * S::kRowTiles * c + 4 * r, at + S::kA + S::kB + S::kSa + 1024 * r + 512 * c);
           }
           const uint64_t ad = smem_desc_kmajor(at, 128), bd = smem_desc_kmajor(at + S::kA, 128);
           for (int i = 0; i < steps; ++i) {
             const uint32_t id = (uint32_t)(i & 1) * 2u, c = (uint32_t)i >> 1;  // which two of the four scales of 128
-            umma_mxf4(d, ad + 2 * i, bd + 2 * i, kIdesc | (id << 29) | (id << 4), sc + 4 * c, sc + 8 + 4 * S::kRowTiles * c + group,
-                      k > w.k0 || i > 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              umma_mxf4(d + m * S::kD, ad + m * (kMm * 128 / 16) + 2 * i, bd + 2 * i, kIdesc | (id << 29) | (id << 4), sa + 8 * m + 4 * c,
+                        sb + 4 * S::kRowTiles * c + group, k > w.k0 || i > 0);
           }
           umma_commit(smem_u32(&empty[s]));
           if (k == w.k1 - 1) umma_commit(smem_u32(&accfull[buf]));
@@ -359,27 +432,78 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
     if (elect_one()) umma_commit(smem_u32(&drained));
     __syncwarp();
     (void)mbar_wait_poll(smem_u32(&drained), 0, kLimit);
+  } else if (FUSE && warp >= 2 + 4 * MT) {
+    // ---- tokens: a warp every kFuseWarps-th stage, its rows as mx4_quantize_k takes them.
+    // (A wait tells one phase of a barrier from the next, not from the one after that.
+    // The warp has waited for the place of the stage kFuseWarps before, so that with at
+    // most kStages warps the phase before the one that it waits for is over.)
+    static_assert(!FUSE || kFuseWarps <= S::kStages, "phases");
+    constexpr bool XB = FUSE == 2;
+    constexpr int kEach = 8;  // rows in flight
+    const uint32_t mine = (uint32_t)warp - (2 + 4 * MT);
+    pdl_wait();
+    uint32_t n = 0;
+    LinearWalk w(a);
+    bool ok = true;
+    while (ok && w.next(a)) {
+      for (int k = w.k0; k < w.k1; ++k, ++n) {
+        if (n % kFuseWarps != mine) continue;
+        const uint32_t s = n % S::kStages, wrap = n / S::kStages;
+        uint8_t *const at = smem_raw + (ring - smem_u32(smem_raw)) + s * S::kStage + S::kA;
+        const int c = k * kStageK + lane * 8;
+        for (int r0 = 0; r0 < a.rows; r0 += kEach) {
+          uint4 now[kEach];
+#pragma unroll
+          for (int i = 0; i < kEach; ++i)
+            now[i] = r0 + i < a.rows && c < a.width ? load8(a.x + (r0 + i) * a.x_stride + c, a.x_vec) : make_uint4(0, 0, 0, 0);
+          if (r0 == 0 && wrap > 0) {
+            ok = mbar_wait_bounded(smem_u32(&empty[s]), (wrap - 1u) & 1u, &abort_sh, a.status, kStatusTimeoutEmpty, kLimit);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            const int r = r0 + i;
+            if (r >= a.rows) break;
+            uint32_t codes;
+            const int e = mx4_block<XB>(now[i], codes);
+            *reinterpret_cast<uint32_t *>(at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
+            uint32_t word = (uint32_t)e << (8 * ((lane >> 2) & 3));
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            word |= __shfl_xor_sync(0xffffffffu, word, 8);
+            if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(at + S::kB + S::kSa + (lane >> 4) * 512 + r * 16) = word;
+          }
+        }
+        if (!ok) break;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&full[s]));
+      }
+    }
   } else {
     // ---- results: thread = weight row, four warps the four lane quarters
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int quarter = warp & 3, row = quarter * 32 + lane, mt = (warp - 2) >> 2;
+    auto team_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + mt) : "memory"); };
     pdl_wait();
     uint32_t tile = 0;
     LinearWalk w(a);
     bool ok = true;
     constexpr int kStep = 16;
     while (w.next(a)) {
-      const uint32_t buf = tile & 1u, use = tile >> 1;
+      const uint32_t buf = tile % S::kBufs, use = tile / S::kBufs;
       if (ok) ok = mbar_wait_bounded(smem_u32(&accfull[buf]), use & 1u, &abort_sh, a.status, kStatusTimeoutAcc, kLimit);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const uint32_t d = tmem + buf * S::kD + ((uint32_t)quarter << 21);
-      const int t0 = w.t * TN, count = min(TN, a.rows - t0);
-      const long long n = (long long)w.m * kMm + row;
+      const uint32_t d = tmem + (buf * MT + mt) * S::kD + ((uint32_t)quarter << 21);
+      const int t0 = w.t * TN, count = min(TN, (S::kSwap ? a.outputs : a.rows) - t0);
+      const long long n = (long long)w.m * S::kRows + mt * kMm + row;
       const bool whole = w.k0 == 0 && w.k1 == a.ks;
-      uint16_t *out = a.out + (long long)t0 * a.stride + n;
+      // (swapped: the lanes are tokens, the columns outputs)
+      const long long lanes = S::kSwap ? a.rows : a.outputs;
+      uint16_t *out = S::kSwap ? a.out + n * a.stride + t0 : a.out + (long long)t0 * a.stride + n;
       bool last = false;
       if (!whole) {
-        float *slot = a.slots + (size_t)(2 * blockIdx.x + (w.k0 == 0)) * (kMm * TN);
+        float *slot = a.slots + ((size_t)(2 * blockIdx.x + (w.k0 == 0)) * MT + mt) * (kMm * TN);
         if (ok) {
 #pragma unroll 1
           for (int c = 0; c < count; c += kStep) {
@@ -391,20 +515,15 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
               if (c + i < count) __stcg(&slot[(c + i) * kMm + row], __uint_as_float(r[i]));
           }
         }
-        __threadfence();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (threadIdx.x == 64) {
-          __threadfence();
+        team_sync();
+        if (quarter == 0 && lane == 0) {
           const unsigned parts = (unsigned)(w.last_cta - w.first_cta + 1);
-          const bool done = atomicAdd(&a.counters[w.first_cta], 1u) == parts - 1;
-          if (done) {
-            atomicExch(&a.counters[w.first_cta], 0u);
-            __threadfence();
-          }
-          last_sh = done;
+          const bool done = count_acq_rel(&a.counters[w.first_cta * MT + mt]) == parts - 1;
+          if (done) atomicExch(&a.counters[w.first_cta * MT + mt], 0u);
+          last_sh[mt] = done;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        last = last_sh != 0;
+        team_sync();
+        last = last_sh[mt] != 0;
       }
       if (ok && (whole || last)) {
 #pragma unroll 1
@@ -419,17 +538,22 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
           } else {
 #pragma unroll
             for (int i = 0; i < kStep; ++i) v[i] = 0.f;
+#pragma unroll 4
             for (int z = w.first_cta; z <= w.last_cta; ++z) {
-              const float *slot = a.slots + (size_t)(2 * z + (z == w.first_cta)) * (kMm * TN);
+              const float *slot = a.slots + ((size_t)(2 * z + (z == w.first_cta)) * MT + mt) * (kMm * TN);
 #pragma unroll
               for (int i = 0; i < kStep; ++i)
                 if (c + i < count) v[i] += __ldcg(&slot[(c + i) * kMm + row]);
             }
           }
-          if (n < a.outputs) {
+          if (n < lanes) {
+            if constexpr (S::kSwap) {
+              store_outputs<BF16>(out + c, v, count - c, a.out_vec);
+            } else {
 #pragma unroll
-            for (int i = 0; i < kStep; ++i)
-              if (c + i < count) out[(c + i) * a.stride] = (uint16_t)pack2<BF16>(v[i], v[i]);
+              for (int i = 0; i < kStep; ++i)
+                if (c + i < count) out[(c + i) * a.stride] = (uint16_t)pack2<BF16>(v[i], v[i]);
+            }
           }
         }
       }
@@ -437,59 +561,106 @@ __global__ void __launch_bounds__(kLinearThreads, 1) mx4_linear_k(const __grid_c
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&accempty[buf]));
-      if (!whole) asm volatile("bar.sync 1, 128;" ::: "memory");  // (last_sh has been read)
+      if (!whole) team_sync();  // (last_sh has been read)
       ++tile;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, S::kTmem);
 }
 
-template <int TN, bool BF16>
-cudaError_t linear_tiles(const Mx4Linear &l, cudaStream_t st) {
-  using S = Tile<TN>;
+// How a product is divided: tokens and weight tiles of a tile, and whether tiles are cut over CTAs.
+struct LinearPlan {
+  int tn, mt;
+  uint32_t units, size;
+  int grid;
+};
+LinearPlan linear_plan(const Mx4Linear &l) {
+  const long long ks = (l.w.width + kStageK - 1) / kStageK;
+  LinearPlan best{};
+  double least = 1e300;
+  struct Form {
+    int tn, mt;
+  };
+  for (const Form f : {Form{16, 1}, Form{32, 1}, Form{64, 1}, Form{64, 2}, Form{128, 1}, Form{192, 1}, Form{192, 2}}) {
+    const int tn = f.tn, mt = f.mt;
+    if (tn < 64 && l.x.rows > tn) continue;
+    if (least < 1e300 && tn / 2 >= l.x.rows && tn > 64) continue;
+    const bool swap = mt == 2 && tn > 64;  // (Tile::kSwap)
+    const long long lanes = swap ? l.x.rows : l.w.rows, columns = swap ? l.w.rows : l.x.rows;
+    const long long tiles = (lanes + 128 * mt - 1) / (128 * mt) * ((columns + tn - 1) / tn);
+    if (tiles * ks > 0x7fffffffLL) continue;
+    // Us of a stage: bytes that come from the L2 (some 73 GB/s to an SM), the weights' from
+    // memory (44 GB/s).
+    const double weights = mt * kMm * 136.0, tokens = tn * 128.0 + 1024;
+    const double stage = tn < 128 ? weights / 44e3 + tokens / 46e3 : (weights + tokens) / 73e3;
+    const long long turns = (tiles + l.sms - 1) / l.sms;
+    for (int cut = 0; cut < (mt == 2 && tn > 64 ? 1 : 2); ++cut) {
+      const long long size = cut ? (tiles * ks + l.sms - 1) / l.sms : turns * ks;
+      if (cut && size >= turns * ks) continue;
+      const double us = size * stage + (cut ? 2.5 + 0.03 * tn : 0.0);
+      if (us < least) {
+        least = us;
+        best = LinearPlan{tn, mt, (uint32_t)(tiles * ks), (uint32_t)size, (int)((tiles * ks + size - 1) / size)};
+      }
+    }
+  }
+  return best;
+}
+
+template <int TN, int MT, bool BF16, int FUSE>
+cudaError_t linear_tiles(const Mx4Linear &l, const LinearPlan &plan, cudaStream_t st) {
+  using S = Tile<TN, MT>;
   LinearArgs a;
   std::string err;
   const uint64_t pitch = (uint64_t)l.w.width / 2;
-  if (!encode_tiled_bytes(&a.wmap, l.w.codes, pitch, (uint64_t)l.w.rows, pitch, kMm, &err) ||
-      !encode_tiled_bytes(&a.xmap, l.x.codes, pitch, (uint64_t)l.x.rows, pitch, TN, &err))
-    return cudaErrorInvalidValue;
-  a.ws = l.w.scales, a.xs = l.x.scales;
+  const Mx4 &lanes = S::kSwap ? l.x : l.w, &columns = S::kSwap ? l.w : l.x;
+  if (!encode_tiled_bytes(&a.wmap, lanes.codes, pitch, (uint64_t)lanes.rows, pitch, kMm, &err)) return cudaErrorInvalidValue;
+  if (!FUSE && !encode_tiled_bytes(&a.xmap, columns.codes, pitch, (uint64_t)columns.rows, pitch, TN, &err)) return cudaErrorInvalidValue;
+  a.x = static_cast<const uint16_t *>(l.rows);
+  a.x_stride = l.x_stride;
+  a.x_vec = rows_vec(l.rows, l.x_stride);
+  a.ws = lanes.scales, a.xs = columns.scales;
   a.out = static_cast<uint16_t *>(l.out);
   a.stride = l.stride;
+  a.out_vec = reinterpret_cast<uintptr_t>(l.out) % 32 == 0 && l.stride % 16 == 0;
   a.chunks = (l.w.width + 127) / 128;
   a.rows = (int)l.x.rows, a.outputs = (int)l.w.rows, a.width = (int)l.w.width;
-  a.m_tiles = (int)((l.w.rows + kMm - 1) / kMm);
+  a.m_tiles = (int)((lanes.rows + S::kRows - 1) / S::kRows);
   a.ks = (int)((l.w.width + kStageK - 1) / kStageK);
-  const long long tiles = (long long)a.m_tiles * ((l.x.rows + TN - 1) / TN);
-  if (tiles * a.ks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  a.units = (uint32_t)(tiles * a.ks);
-  // whole tiles where they fill the CTAs evenly enough
-  const long long turns = (tiles + l.sms - 1) / l.sms;
-  if (tiles * 10 >= turns * l.sms * 9)
-    a.size = (uint32_t)(turns * a.ks);
-  else
-    a.size = (uint32_t)((a.units + l.sms - 1) / l.sms);
-  const int grid = (int)((a.units + a.size - 1) / a.size);
-  a.fresh = l.fresh;
+  a.units = plan.units;
+  a.size = plan.size;
+  a.fresh = l.rows && !FUSE && !S::kSwap;
   a.counters = static_cast<unsigned *>(l.workspace);
   a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(l.workspace) + kKvCounterBytes);
   a.status = l.status;
   static std::atomic<bool> attr_set[kAttrMaxDevices];
-  const cudaError_t e = ensure_dynamic_smem(mx4_linear_k<TN, BF16>, S::kSmem, attr_set);
+  const cudaError_t e = ensure_dynamic_smem(mx4_linear_k<TN, MT, BF16, FUSE>, S::kSmem, attr_set);
   if (e != cudaSuccess) return e;
-  return launch_kernel(mx4_linear_k<TN, BF16>, dim3((unsigned)grid), dim3(kLinearThreads), (size_t)S::kSmem, st, a);
+  return launch_kernel(mx4_linear_k<TN, MT, BF16, FUSE>, dim3((unsigned)plan.grid), dim3(S::kThreads + (FUSE ? 32 * kFuseWarps : 0)),
+                       (size_t)S::kSmem, st, a);
 }
 
 template <bool BF16>
 cudaError_t linear_rows(const Mx4Linear &l, cudaStream_t st) {
-  if (l.x.rows <= 16) return linear_tiles<16, BF16>(l, st);
-  if (l.x.rows <= 32) return linear_tiles<32, BF16>(l, st);
-  if (l.x.rows <= 64) return linear_tiles<64, BF16>(l, st);
-  if (l.x.rows <= 128) return linear_tiles<128, BF16>(l, st);
-  return linear_tiles<192, BF16>(l, st);
+  const LinearPlan p = linear_plan(l);
+  if (!p.tn) return cudaErrorInvalidValue;
+  if (p.tn == 16 && l.rows && l.x.rows <= 16)
+    return l.x_bf16 ? linear_tiles<16, 1, BF16, 2>(l, p, st) : linear_tiles<16, 1, BF16, 1>(l, p, st);
+  if (l.rows) {
+    const cudaError_t e = launch_mx4_quantize(l.x_bf16, l.rows, l.x.rows, l.x_stride, l.x, st);
+    if (e != cudaSuccess) return e;
+  }
+  switch (p.tn * p.mt) {
+    case 16: return linear_tiles<16, 1, BF16, 0>(l, p, st);
+    case 32: return linear_tiles<32, 1, BF16, 0>(l, p, st);
+    case 64: return linear_tiles<64, 1, BF16, 0>(l, p, st);
+    case 128: return p.mt == 2 ? linear_tiles<64, 2, BF16, 0>(l, p, st) : linear_tiles<128, 1, BF16, 0>(l, p, st);
+    case 192: return linear_tiles<192, 1, BF16, 0>(l, p, st);
+    default: return linear_tiles<192, 2, BF16, 0>(l, p, st);
+  }
 }
 
 // Pieces of a warp, and the grid: few values go to many warps.
@@ -530,7 +701,7 @@ cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, 
 }
 
 // Counters (zero before the first call and after each), then two parts of tiles a CTA.
-size_t mx4_workspace_bytes(int sms) { return kKvCounterBytes + sizeof(float) * 2 * (size_t)sms * kMm * kMaxTokens; }
+size_t mx4_workspace_bytes(int sms) { return kKvCounterBytes + sizeof(float) * 2 * (size_t)sms * kMm * 192; }  // (most: 128 x 192)
 
 cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st) {
   return a.bf16 ? linear_rows<true>(a, st) : linear_rows<false>(a, st);

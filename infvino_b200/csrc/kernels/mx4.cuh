@@ -25,10 +25,12 @@ cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long l
 cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st);
 struct Mx4Linear {
   Mx4 x, w;         // x.rows: the rows that are used
+  const void *rows;  // if not null: 16-bit rows that X is quantised from, x is room for it
+  long long x_stride;
+  bool x_bf16;
   void *out;
   long long stride;
   bool bf16;
-  bool fresh;       // x has just been quantised by a launch that waited for what came before it
   void *workspace;
   int *status;
   int sms;

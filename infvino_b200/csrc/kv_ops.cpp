@@ -567,12 +567,13 @@ int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64
     if (rows == 0 || a.w.rows == 0) return;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     a.workspace = workspace(h, st);
-    if (x) cuda(ivb::launch_mx4_quantize(x_dtype == IVC_BF16, x, rows, x_stride, a.x, st), "launch");
+    a.rows = x;
+    a.x_stride = x_stride;
+    a.x_bf16 = x_dtype == IVC_BF16;
     a.x.rows = rows;
     a.out = out;
     a.stride = out_stride;
     a.bf16 = out_dtype == IVC_BF16;
-    a.fresh = x != nullptr;
     a.status = h->status;
     a.sms = h->sms;
     cuda(ivb::launch_mx4_linear(a, st), "launch");

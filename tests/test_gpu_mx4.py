@@ -172,6 +172,27 @@ def test_linear(ops, dtype, rows, width, outputs):
     close(out, want, mass, width, dtype)
 
 
+@pytest.mark.parametrize("rows,width,outputs", [(1, 8192, 20500), (16, 4096, 19000), (20, 14336, 4100), (1, 14336, 4096), (50, 8192, 20500), (128, 8192, 8300)])
+def test_linear_long_shares(ops, rows, width, outputs):
+    """Every CTA has many stages, of several tiles: rings go round, quantised on the way or before."""
+    x = inputs(rows, width, "f16", 7)
+    w = (torch.randn((outputs, width), generator=torch.Generator(device="cuda").manual_seed(8), device="cuda") * width ** -0.5).bfloat16()
+    m, xq = ivb.Mx4(*empty(outputs, width)), ivb.Mx4(*empty(rows, width))
+    ops.mx4_quantize(w, m, stream=stream())
+    ops.mx4_quantize(x, xq, stream=stream())
+    vx, vw = torch.empty_like(x), torch.empty_like(w)  # (their values need at most two bits: exact)
+    ops.mx4_read(xq, vx, stream=stream())
+    ops.mx4_read(m, vw, stream=stream())
+    vx, vw = vx.double(), vw.double()
+    want, mass = (vx @ vw.t()).cpu(), (vx.abs() @ vw.abs().t()).cpu()
+    out, again = (torch.full((rows, outputs), math.nan, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.mx4_linear(xq, m, out, stream=stream())
+    ops.mx4_linear(x, m, again, scratch=ivb.Mx4(*empty(rows, width)), stream=stream())
+    ops.synchronize(stream())
+    close(out, want, mass, width, "f16")
+    assert torch.equal(out, again)
+
+
 @pytest.mark.parametrize("rows,width,outputs", [(1, 4096, 300), (20, 288, 200), (300, 2080, 520)])
 def test_linear_forms(ops, rows, width, outputs):
     """A matrix that was quantised before gives the same bits; outputs of the other type; part of a larger scratch; strided outputs."""
