@@ -7,6 +7,8 @@
 // are exact but for that rounding.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "../tma.h"
 #include "kv_common.cuh"
 #include "mx4.cuh"
@@ -14,6 +16,8 @@
 namespace ivb {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 // Eight values as codes, the first in the lowest four bits.
 __device__ __forceinline__ uint32_t mx4_codes(const float (&f)[8]) {
@@ -141,10 +145,11 @@ bool rows_vec(const void *p, long long stride) { return reinterpret_cast<uintptr
 // applies the blocks' scales itself, 128 weight rows (a lane of TMEM each) by TN
 // tokens (a column each) by 64 of the width an instruction, sums in f32.
 //
-// A tile is 128 weight rows x TN tokens; its units are stages of 256 of the width.
-// The units are divided over the CTAs, one an SM, evenly (few tiles: a tile is cut
-// over CTAs, its parts are joined by the last of them to arrive, in their order) or
-// by whole tiles.
+// A tile is 128 weight rows (or twice that) x TN tokens, in stages of 256 of the width.  A
+// CTA, one an SM, has some tiles; or, where tiles are fewer than SMs, the CTAs of a
+// cluster have a part of one's stages each, and add the parts up out of one another's
+// shared memory.  (Parts left in global memory for the last CTA: 38 us for 50 tokens x
+// 4096 -> 6144, two weight tiles, against 13 without parts; an SM reads too slowly.)
 //   warp 0     brings a stage's codes (TMA, 128-byte swizzled lines) and scales (as they
 //              lie in memory: 512 bytes for 128 rows x 128 of the width)
 //   warp 1     copies a stage's scales into TMEM and issues its products
@@ -152,10 +157,11 @@ bool rows_vec(const void *p, long long stride) { return reinterpret_cast<uintptr
 // Two sets of accumulators: a tile's products run while the one before it goes out.
 //
 // Every wait is bounded: a timeout sets the status word and an abort flag, all
-// roles run out, and parts of cut tiles are counted all the same.
+// roles run out.
 constexpr int kMm = 128;             // weight rows of an instruction
 constexpr int kStageK = 256;         // of the width
-constexpr int kFuseWarps = 4;
+constexpr int kFuseWarps = 4, kFuseTokens = 6;  // (warps that quantise tokens on the way, and how many tokens there may be)
+constexpr int kMostSplit = 8;          // CTAs of a cluster that share a tile
 
 // MT: weight tiles of 128 rows that share a stage's tokens.  What an SM gets from the L2 in
 // a clock (some 38 bytes when all ask) bounds products with many tokens, and weights,
@@ -170,7 +176,7 @@ struct Tile {
   // Up to 64 tokens two CTAs fit on an SM: the next launch's CTAs set themselves up, and ask for
   // their weights, while this one's end.
   static constexpr int kCtas = TN <= 64 && MT == 1 ? 2 : 1;
-  static constexpr int kStages = MT == 2 ? (TN == 64 ? 5 : 3) : TN == 16 ? 5 : TN <= 64 ? 4 : TN == 128 ? 6 : 5;
+  static constexpr int kStages = MT == 2 ? (TN > 64 ? 3 : 5) : TN == 16 ? 5 : TN <= 64 ? 4 : TN == 128 ? 6 : 5;
   static constexpr int kD = TN < 32 ? 32 : TN;             // columns of an accumulator
   // Two sets of accumulators where they fit.  (256 x 192: one; the loads go on while it is emptied.)
   static constexpr int kBufs = MT == 2 && TN > 64 ? 1 : 2;
@@ -183,6 +189,7 @@ struct Tile {
   static constexpr bool kSwap = MT == 2 && TN > 64;
   static_assert(kBufs * MT * kD + kStages * kScaleCols <= kTmem, "TMEM");
   static_assert(kSmem * kCtas <= 224 << 10, "shared memory");
+  static_assert(kSwap || kRows * TN * 4 <= kStage * kStages, "a part fits into the ring");
 };
 
 struct LinearArgs {
@@ -197,43 +204,35 @@ struct LinearArgs {
   long long chunks;         // 128-wide scale pieces of a row
   int rows, outputs, width;
   int m_tiles, ks;          // tiles of lanes; stages of a tile
-  uint32_t units, size;     // in all; of a CTA's share
+  uint32_t tiles, each;     // in all; of a CTA (or cluster)
+  int split;                // CTAs of a cluster that share a tile
   int fresh;
-  float *slots;
-  unsigned *counters;
   int *status;
 };
 
-// A CTA's share, tile by tile: stages k0 .. k1 - 1 of tile (m, t).
+// A CTA's tiles (m, t), one after the other; or, where `split` CTAs of a cluster have a
+// tile, the CTA's part of its stages: k0 .. k1 - 1.
 struct LinearWalk {
-  uint32_t u, end;
+  uint32_t i, end;
   int m, t, k0, k1;
-  int first_cta, last_cta;
   __device__ __forceinline__ LinearWalk(const LinearArgs &a) {
-    u = min(a.units, blockIdx.x * a.size);
-    end = min(a.units, u + a.size);
+    i = blockIdx.x / (uint32_t)a.split * a.each;
+    end = min(a.tiles, i + a.each);
+    const int rank = (int)(blockIdx.x % (uint32_t)a.split);
+    k0 = rank * a.ks / a.split;
+    k1 = (rank + 1) * a.ks / a.split;
   }
   __device__ __forceinline__ bool next(const LinearArgs &a) {
-    if (u >= end) return false;
-    const uint32_t ks = (uint32_t)a.ks, tile = u / ks, begin = tile * ks;
-    m = (int)(tile % (uint32_t)a.m_tiles);
-    t = (int)(tile / (uint32_t)a.m_tiles);
-    k0 = (int)(u - begin);
-    k1 = (int)(min(end, begin + ks) - begin);
-    first_cta = (int)(begin / a.size);
-    last_cta = (int)((begin + ks - 1) / a.size);
-    u = begin + (uint32_t)k1;
+    if (i >= end) return false;
+    m = (int)(i % (uint32_t)a.m_tiles);
+    t = (int)(i / (uint32_t)a.m_tiles);
+    ++i;
     return true;
   }
 };
 
 __device__ __forceinline__ void prefetch_2d(const void *map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ unsigned count_acq_rel(unsigned *p) {  // (what the block's barrier has put before it is released too)
-  unsigned v;
-  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
-  return v;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
@@ -281,10 +280,10 @@ __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWar
   __shared__ uint64_t full[S::kStages], empty[S::kStages], accfull[2], accempty[2], drained;
   __shared__ uint32_t tmem_sh;
   __shared__ volatile int abort_sh;
-  __shared__ int last_sh[MT];
   constexpr long long kLimit = kConvWaitLimitDefault;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  float *const parts = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)));  // [columns][128 rows], where a cluster has a tile
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&full[i]), FUSE ? 2 : 1), mbar_init(smem_u32(&empty[i]), 1);
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&accfull[i]), 1), mbar_init(smem_u32(&accempty[i]), 4 * MT);
@@ -483,7 +482,6 @@ __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWar
   } else {
     // ---- results: thread = weight row, four warps the four lane quarters
     const int quarter = warp & 3, row = quarter * 32 + lane, mt = (warp - 2) >> 2;
-    auto team_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + mt) : "memory"); };
     pdl_wait();
     uint32_t tile = 0;
     LinearWalk w(a);
@@ -497,56 +495,22 @@ __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWar
       const uint32_t d = tmem + (buf * MT + mt) * S::kD + ((uint32_t)quarter << 21);
       const int t0 = w.t * TN, count = min(TN, (S::kSwap ? a.outputs : a.rows) - t0);
       const long long n = (long long)w.m * S::kRows + mt * kMm + row;
-      const bool whole = w.k0 == 0 && w.k1 == a.ks;
       // (swapped: the lanes are tokens, the columns outputs)
       const long long lanes = S::kSwap ? a.rows : a.outputs;
       uint16_t *out = S::kSwap ? a.out + n * a.stride + t0 : a.out + (long long)t0 * a.stride + n;
-      bool last = false;
-      if (!whole) {
-        float *slot = a.slots + ((size_t)(2 * blockIdx.x + (w.k0 == 0)) * MT + mt) * (kMm * TN);
-        if (ok) {
-#pragma unroll 1
-          for (int c = 0; c < count; c += kStep) {
-            uint32_t r[16];
-            tmem_ld16(d + c, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < kStep; ++i)
-              if (c + i < count) __stcg(&slot[(c + i) * kMm + row], __uint_as_float(r[i]));
-          }
-        }
-        team_sync();
-        if (quarter == 0 && lane == 0) {
-          const unsigned parts = (unsigned)(w.last_cta - w.first_cta + 1);
-          const bool done = count_acq_rel(&a.counters[w.first_cta * MT + mt]) == parts - 1;
-          if (done) atomicExch(&a.counters[w.first_cta * MT + mt], 0u);
-          last_sh[mt] = done;
-        }
-        team_sync();
-        last = last_sh[mt] != 0;
-      }
-      if (ok && (whole || last)) {
+      if (ok) {
 #pragma unroll 1
         for (int c = 0; c < count; c += kStep) {
+          uint32_t r[16];
+          tmem_ld16(d + c, r);
+          tmem_ld_wait();
           float v[kStep];
-          if (whole) {
-            uint32_t r[16];
-            tmem_ld16(d + c, r);
-            tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) v[i] = __uint_as_float(r[i]);
-          } else {
+          for (int i = 0; i < kStep; ++i) v[i] = __uint_as_float(r[i]);
+          if (a.split > 1) {  // (all products have read their operands: the ring is free)
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) v[i] = 0.f;
-#pragma unroll 4
-            for (int z = w.first_cta; z <= w.last_cta; ++z) {
-              const float *slot = a.slots + ((size_t)(2 * z + (z == w.first_cta)) * MT + mt) * (kMm * TN);
-#pragma unroll
-              for (int i = 0; i < kStep; ++i)
-                if (c + i < count) v[i] += __ldcg(&slot[(c + i) * kMm + row]);
-            }
-          }
-          if (n < lanes) {
+            for (int i = 0; i < kStep; ++i) parts[(mt * TN + c + i) * kMm + row] = v[i];
+          } else if (n < lanes) {
             if constexpr (S::kSwap) {
               store_outputs<BF16>(out + c, v, count - c, a.out_vec);
             } else {
@@ -561,7 +525,6 @@ __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWar
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&accempty[buf]));
-      if (!whole) team_sync();  // (last_sh has been read)
       ++tile;
     }
   }
@@ -569,41 +532,109 @@ __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWar
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, S::kTmem);
+  if constexpr (!S::kSwap) {
+    if (a.split > 1) {
+      // the cluster's parts, added up in the order of their stages: a CTA some of the columns
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      if (warp >= 2 && warp < 2 + 4 * MT) {
+        const int row = (warp & 3) * 32 + lane, mt = (warp - 2) >> 2;
+        LinearWalk w(a);
+        w.next(a);
+        const int t0 = w.t * TN, count = min(TN, a.rows - t0), per = (count + a.split - 1) / a.split;
+        const int c0 = (int)(blockIdx.x % (uint32_t)a.split) * per, c1 = min(count, c0 + per);
+        const long long n = (long long)w.m * S::kRows + mt * kMm + row;
+        const float *from[kMostSplit];
+#pragma unroll
+        for (int q = 0; q < kMostSplit; ++q) from[q] = cluster.map_shared_rank(parts, min(q, a.split - 1)) + mt * TN * kMm + row;
+        constexpr int kCols = TN <= 32 ? 2 : 8;  // columns whose parts are asked for together
+        for (int c = c0; c < c1; c += kCols) {
+          float v[kCols][kMostSplit];
+#pragma unroll
+          for (int q = 0; q < kMostSplit; ++q)
+            if (q < a.split)
+#pragma unroll
+              for (int i = 0; i < kCols; ++i) v[i][q] = c + i < c1 ? from[q][(c + i) * kMm] : 0.f;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            float sum = v[i][0];
+#pragma unroll
+            for (int q = 1; q < kMostSplit; ++q)
+              if (q < a.split) sum += v[i][q];
+            if (c + i < c1 && n < a.outputs) a.out[(t0 + c + i) * a.stride + n] = (uint16_t)pack2<BF16>(sum, sum);
+          }
+        }
+      }
+      cluster.sync();  // (the parts have been read)
+    }
+  }
 }
 
-// How a product is divided: tokens and weight tiles of a tile, and whether tiles are cut over CTAs.
+// How a product is divided: tokens and weight tiles of a tile, CTAs that share one (or tiles that one CTA has).
 struct LinearPlan {
-  int tn, mt;
-  uint32_t units, size;
-  int grid;
+  int tn, mt, split;
+  uint32_t tiles, each;
 };
+
+// How many clusters of `split` CTAs run at a time (asked once for a device: SMs come in
+// groups, and a cluster lies in one of them).
+int linear_clusters(int device, int mt, int split) {
+  static std::atomic<int> known[kAttrMaxDevices][2][kMostSplit + 1];
+  const bool tracked = device >= 0 && device < kAttrMaxDevices;
+  int n = tracked ? known[device][mt - 1][split].load(std::memory_order_relaxed) : 0;
+  if (n) return n - 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)split);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto ask = [&](auto kernel, int threads, int bytes) {
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)bytes;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+  };
+  if (mt == 2)
+    ask(mx4_linear_k<64, 2, false, 0>, Tile<64, 2>::kThreads, Tile<64, 2>::kSmem);
+  else  // (alone on its SM, as if others' blocks had the second places)
+    ask(mx4_linear_k<128, 1, false, 0>, Tile<128, 1>::kThreads, Tile<128, 1>::kSmem);
+  if (tracked) known[device][mt - 1][split].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 LinearPlan linear_plan(const Mx4Linear &l) {
   const long long ks = (l.w.width + kStageK - 1) / kStageK;
   LinearPlan best{};
   double least = 1e300;
+  const double memory = l.w.rows * l.w.width * 17.0 / 32 / 6.2e6;
   struct Form {
     int tn, mt;
   };
-  for (const Form f : {Form{16, 1}, Form{32, 1}, Form{64, 1}, Form{64, 2}, Form{128, 1}, Form{192, 1}, Form{192, 2}}) {
+  for (const Form f : {Form{16, 1}, Form{16, 2}, Form{32, 1}, Form{32, 2}, Form{64, 1}, Form{64, 2}, Form{128, 1}, Form{192, 1}, Form{192, 2}}) {
     const int tn = f.tn, mt = f.mt;
     if (tn < 64 && l.x.rows > tn) continue;
-    if (least < 1e300 && tn / 2 >= l.x.rows && tn > 64) continue;
+    if (tn > 16 && tn / 2 >= l.x.rows) continue;
     const bool swap = mt == 2 && tn > 64;  // (Tile::kSwap)
     const long long lanes = swap ? l.x.rows : l.w.rows, columns = swap ? l.w.rows : l.x.rows;
     const long long tiles = (lanes + 128 * mt - 1) / (128 * mt) * ((columns + tn - 1) / tn);
-    if (tiles * ks > 0x7fffffffLL) continue;
-    // Us of a stage: bytes that come from the L2 (some 73 GB/s to an SM), the weights' from
-    // memory (44 GB/s).
-    const double weights = mt * kMm * 136.0, tokens = tn * 128.0 + 1024;
-    const double stage = tn < 128 ? weights / 44e3 + tokens / 46e3 : (weights + tokens) / 73e3;
-    const long long turns = (tiles + l.sms - 1) / l.sms;
-    for (int cut = 0; cut < (mt == 2 && tn > 64 ? 1 : 2); ++cut) {
-      const long long size = cut ? (tiles * ks + l.sms - 1) / l.sms : turns * ks;
-      if (cut && size >= turns * ks) continue;
-      const double us = size * stage + (cut ? 2.5 + 0.03 * tn : 0.0);
+    if (tiles > 0x7fffffffLL) continue;
+    // Us, from measurements at 1 to 4001 tokens (within some 10 %): a stage's bytes into an
+    // SM, weights slower than tokens, or all weights out of memory; starting and ending; a tile's results where nothing else runs meanwhile, or a cluster's gathering.
+    const double weights = mt * kMm * 136.0, tokens = tn * 136.0;
+    for (int split = 1; split <= (swap ? 1 : kMostSplit); ++split) {
+      if (split > 1 && (split > ks || tiles > linear_clusters(l.device, mt, split))) continue;
+      const long long each = split > 1 ? 1 : (tiles + l.sms - 1) / l.sms;
+      const double stages = each * ((ks + split - 1) / split) * (weights / (mt == 2 ? 85e3 : 64e3) + tokens / 100e3);
+      const double us = 4.0 + std::max(stages, memory) + each * (swap ? 2.0 : 0.0) + (each - 1) * 1.5 + (split > 1 ? 1.0 + 0.03 * tn * mt : 0.0);
       if (us < least) {
         least = us;
-        best = LinearPlan{tn, mt, (uint32_t)(tiles * ks), (uint32_t)size, (int)((tiles * ks + size - 1) / size)};
+        best = LinearPlan{tn, mt, split, (uint32_t)tiles, (uint32_t)each};
       }
     }
   }
@@ -630,35 +661,59 @@ cudaError_t linear_tiles(const Mx4Linear &l, const LinearPlan &plan, cudaStream_
   a.rows = (int)l.x.rows, a.outputs = (int)l.w.rows, a.width = (int)l.w.width;
   a.m_tiles = (int)((lanes.rows + S::kRows - 1) / S::kRows);
   a.ks = (int)((l.w.width + kStageK - 1) / kStageK);
-  a.units = plan.units;
-  a.size = plan.size;
+  a.tiles = plan.tiles;
+  a.each = plan.each;
+  a.split = plan.split;
   a.fresh = l.rows && !FUSE && !S::kSwap;
-  a.counters = static_cast<unsigned *>(l.workspace);
-  a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(l.workspace) + kKvCounterBytes);
   a.status = l.status;
   static std::atomic<bool> attr_set[kAttrMaxDevices];
   const cudaError_t e = ensure_dynamic_smem(mx4_linear_k<TN, MT, BF16, FUSE>, S::kSmem, attr_set);
   if (e != cudaSuccess) return e;
-  return launch_kernel(mx4_linear_k<TN, MT, BF16, FUSE>, dim3((unsigned)plan.grid), dim3(S::kThreads + (FUSE ? 32 * kFuseWarps : 0)),
-                       (size_t)S::kSmem, st, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((plan.tiles + plan.each - 1) / plan.each * (unsigned)plan.split);
+  cfg.blockDim = dim3(S::kThreads + (FUSE ? 32 * kFuseWarps : 0));
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (plan.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)plan.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (g_launch_pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = (unsigned)n;
+  return cudaLaunchKernelEx(&cfg, mx4_linear_k<TN, MT, BF16, FUSE>, a);
 }
 
 template <bool BF16>
 cudaError_t linear_rows(const Mx4Linear &l, cudaStream_t st) {
   const LinearPlan p = linear_plan(l);
   if (!p.tn) return cudaErrorInvalidValue;
-  if (p.tn == 16 && l.rows && l.x.rows <= 16)
+  // (one launch / two: 4096 -> 6144, 1 token 7.4 / 8.9 us, 4 8.0 / 9.4, 8 9.6 / 9.7, 16 13.8 / 10.3;
+  // 8192 -> 28672, 1 22.6 / 24.6, 4 23.3 / 24.5, 8 27.2 / 24.6)
+  if (p.tn == 16 && l.rows && l.x.rows <= kFuseTokens) {
+    if (p.mt == 2) return l.x_bf16 ? linear_tiles<16, 2, BF16, 2>(l, p, st) : linear_tiles<16, 2, BF16, 1>(l, p, st);
     return l.x_bf16 ? linear_tiles<16, 1, BF16, 2>(l, p, st) : linear_tiles<16, 1, BF16, 1>(l, p, st);
+  }
   if (l.rows) {
     const cudaError_t e = launch_mx4_quantize(l.x_bf16, l.rows, l.x.rows, l.x_stride, l.x, st);
     if (e != cudaSuccess) return e;
   }
-  switch (p.tn * p.mt) {
-    case 16: return linear_tiles<16, 1, BF16, 0>(l, p, st);
-    case 32: return linear_tiles<32, 1, BF16, 0>(l, p, st);
-    case 64: return linear_tiles<64, 1, BF16, 0>(l, p, st);
-    case 128: return p.mt == 2 ? linear_tiles<64, 2, BF16, 0>(l, p, st) : linear_tiles<128, 1, BF16, 0>(l, p, st);
-    case 192: return linear_tiles<192, 1, BF16, 0>(l, p, st);
+  switch (p.tn * 4 + p.mt) {
+    case 16 * 4 + 1: return linear_tiles<16, 1, BF16, 0>(l, p, st);
+    case 16 * 4 + 2: return linear_tiles<16, 2, BF16, 0>(l, p, st);
+    case 32 * 4 + 1: return linear_tiles<32, 1, BF16, 0>(l, p, st);
+    case 32 * 4 + 2: return linear_tiles<32, 2, BF16, 0>(l, p, st);
+    case 64 * 4 + 1: return linear_tiles<64, 1, BF16, 0>(l, p, st);
+    case 64 * 4 + 2: return linear_tiles<64, 2, BF16, 0>(l, p, st);
+    case 128 * 4 + 1: return linear_tiles<128, 1, BF16, 0>(l, p, st);
+    case 192 * 4 + 1: return linear_tiles<192, 1, BF16, 0>(l, p, st);
     default: return linear_tiles<192, 2, BF16, 0>(l, p, st);
   }
 }
@@ -699,9 +754,6 @@ cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long l
 cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st) {
   return bf16 ? read<true>(m, rows, out, stride, st) : read<false>(m, rows, out, stride, st);
 }
-
-// Counters (zero before the first call and after each), then two parts of tiles a CTA.
-size_t mx4_workspace_bytes(int sms) { return kKvCounterBytes + sizeof(float) * 2 * (size_t)sms * kMm * 192; }  // (most: 128 x 192)
 
 cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st) {
   return a.bf16 ? linear_rows<true>(a, st) : linear_rows<false>(a, st);

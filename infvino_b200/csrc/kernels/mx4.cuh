@@ -31,11 +31,9 @@ struct Mx4Linear {
   void *out;
   long long stride;
   bool bf16;
-  void *workspace;
   int *status;
-  int sms;
+  int sms, device;
 };
-size_t mx4_workspace_bytes(int sms);
 cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st);
 
 }  // namespace ivb

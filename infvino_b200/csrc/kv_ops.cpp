@@ -134,7 +134,7 @@ void *workspace(ivc_kv *h, cudaStream_t st) {
   const auto it = h->workspace.find(name.id);
   if (it != h->workspace.end()) return it->second;
   need(!name.captured, "a stream's first call cannot be captured: call ivc_kv_reserve before");
-  const size_t bytes = std::max(ivb::kv_workspace_bytes(h->sms), ivb::mx4_workspace_bytes(h->sms));
+  const size_t bytes = ivb::kv_workspace_bytes(h->sms);
   void *p = nullptr;
   cuda(cudaMalloc(&p, bytes), "workspace");
   try {
@@ -566,7 +566,6 @@ int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64
     need(rows <= a.x.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0 || a.w.rows == 0) return;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    a.workspace = workspace(h, st);
     a.rows = x;
     a.x_stride = x_stride;
     a.x_bf16 = x_dtype == IVC_BF16;
@@ -576,6 +575,7 @@ int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64
     a.bf16 = out_dtype == IVC_BF16;
     a.status = h->status;
     a.sms = h->sms;
+    a.device = h->device;
     cuda(ivb::launch_mx4_linear(a, st), "launch");
   });
 }
