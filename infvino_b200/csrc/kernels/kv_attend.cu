@@ -129,7 +129,8 @@ struct StepShared {
   long long base;
   int seq;
   int last;
-  unsigned items, each;  // of kRest: items, and blocks of one
+  long long scan_items[kStepWarps];  // of kRest
+  int most[kStepWarps];
 };
 
 // NT: 8-row tiles of queries that share the codes of an item.
@@ -151,23 +152,26 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   const int per = (a.seqs.batch + kStepThreads - 1) / kStepThreads;
   long long mine = 0;
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
-  if (MODE == kRest) {
-    if (threadIdx.x == 0) sh.items = 0;
-    __syncthreads();
-  }
+  long long my_items = 0;
+  int most = 0;
   for (int b = b_lo; b < b_hi; ++b) {
     const KvSpan s = kv_span<MODE>(a, b);
-    const int tiles = (s.n * a.group + kRows - 1) / kRows;
-    mine += (long long)s.blocks * tiles * a.cache.heads;
-    if (MODE == kRest && tiles) atomicAdd(&sh.items, (unsigned)(tiles * a.cache.heads));
+    const long long items = (long long)((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
+    mine += s.blocks * items;
+    if (MODE == kRest) my_items += items, most = max(most, s.blocks);
   }
-  long long incl = mine;
+  long long incl = mine, incl_items = my_items;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const long long w = MODE == kRest ? __shfl_up_sync(0xffffffffu, incl_items, o) : 0;
+    if (lane >= o) incl += v, incl_items += w;
   }
   if (lane == 31) sh.scan[warp] = incl;
+  if (MODE == kRest) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) sh.scan_items[warp] = incl_items, sh.most[warp] = most;
+  }
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -176,26 +180,40 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     total += sh.scan[w];
   }
   if (total == 0) return;
-  // (what a sequence has of its own may be a block or two: a share is an item then, not several in turn)
-  if (MODE == kRest && threadIdx.x == 0) sh.each = (uint32_t)min(total / max(sh.items, 1u) + 1, (long long)kStepMinBlocks);
-  if (MODE == kRest) __syncthreads();
   if (total > 0x7fffffffLL) {  // (hours of work; units are counted in 32 bits from here)
     if (threadIdx.x == 0) kv_flag(a.status, kStatusKvSeqs);
     return;
   }
   uint32_t at_least = kStepMinBlocks;
-  if (MODE == kRest) at_least = min(at_least, sh.each);
+  bool by_item = false;  // a share is some whole items
+  long long excl = before + incl - mine;
+  if (MODE == kRest) {
+    // What sequences have of their own is often a few blocks.  Where whole items
+    // divide about as evenly as blocks, nothing is cut (64 sequences of up to 500 keys of
+    // their own, 8 heads: 25 us against 28); else a share is no more than an item.
+    long long items_before = 0, items = 0;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      if (w < warp) items_before += sh.scan_items[w];
+      items += sh.scan_items[w];
+      most = max(most, sh.most[w]);
+    }
+    const long long turns = (items + gridDim.x - 1) / gridDim.x;
+    by_item = most * turns <= 2 * ((total + gridDim.x - 1) / gridDim.x) + 24;
+    at_least = by_item ? 1u : (uint32_t)min(total / max(items, 1ll) + 1, (long long)kStepMinBlocks);
+    if (by_item) total = items, mine = my_items, excl = items_before + incl_items - my_items;
+  }
+  auto units_of = [&](const KvSpan &s) { return MODE == kRest && by_item ? 1u : (uint32_t)s.blocks; };
   const uint32_t size = max(at_least, ((uint32_t)total + gridDim.x - 1) / gridDim.x);  // units of a share
   uint32_t u = blockIdx.x * size;
   if (u >= (uint32_t)total) return;
   const uint32_t u_end = min((uint32_t)total, u + size);
-  const long long excl = before + incl - mine;
   if (u >= excl && u < excl + mine) {
     long long at = excl;
     int b = b_lo;
     for (;; ++b) {
       const KvSpan s = kv_span<MODE>(a, b);
-      const long long w = (long long)s.blocks * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
+      const long long w = (long long)units_of(s) * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
       if (u < at + w) break;
       at += w;
     }
@@ -223,18 +241,18 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   float2 sc_mine = make_float2(0.f, -INFINITY);
   auto locate = [&]() {
     for (;;) {
-      const uint32_t units = (uint32_t)s.blocks * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
+      const uint32_t units = units_of(s) * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
       if (u < base + units) break;
       base += units;
       s = kv_span<MODE>(a, ++b);  // (units are left, so there is a next sequence)
       row_tiles = (s.n * a.group + kRows - 1) / kRows;
     }
-    const uint32_t item = (u - base) / (uint32_t)s.blocks;
+    const uint32_t item = (u - base) / units_of(s);
     head = (int)(item / (uint32_t)row_tiles);
     rt = (int)item - head * row_tiles;
-    item_begin = base + item * (uint32_t)s.blocks;
-    k0 = (int)(u - item_begin);
-    k1 = (int)(min(u_end, item_begin + (uint32_t)s.blocks) - item_begin);
+    item_begin = base + item * units_of(s);
+    k0 = MODE == kRest && by_item ? 0 : (int)(u - item_begin);
+    k1 = MODE == kRest && by_item ? s.blocks : (int)(min(u_end, item_begin + (uint32_t)s.blocks) - item_begin);
     count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
     looked = 0;
   };
@@ -514,7 +532,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     const int n = s.n, first = s.first, head_now = head, rt_now = rt;
     const bool begins = k0 == 0, whole = begins && k1 == s.blocks, joins = MODE == kRest && s.first_block > 0;
     const int first_cta = (int)(item_begin / size), last_cta = (int)((item_begin + (uint32_t)s.blocks - 1u) / size);
-    u += (uint32_t)(k1 - k0);
+    u += MODE == kRest && by_item ? 1u : (uint32_t)(k1 - k0);
     const bool more = u < u_end;
     if (more) {
       locate();
