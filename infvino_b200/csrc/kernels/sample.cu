@@ -38,30 +38,32 @@ constexpr int kMaxRanks = 8;
 constexpr int kWindow = 16;  // bins around a guess
 constexpr double kFar = 41.588830833596715;  // 60 ln 2: what is further below the largest has no weight
 
-// 2^(j / 64), j below 64, by the first threads of a block.
-constexpr int kPowers = 64;
+// 2^(j / 1024), j below 1024.
+constexpr int kPowers = 1024;
 __device__ __forceinline__ void fill_powers(double *powers) {
-  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2(threadIdx.x / (double)kPowers);
+  for (int j = threadIdx.x; j < kPowers; j += blockDim.x) powers[j] = exp2(j / (double)kPowers);
 }
-// e^((v - top) / T) with by = 64 log2(e) / T: 2^(n / 64) from the table, and the first
-// terms of the series of 2^(r / 64), r at most a half (the rest is below 2^-44 of it).
-__device__ __forceinline__ double weight_of(float v, float top, double by, const double *powers) {
-  if (v == top) return 1.0;
-  const double t = ((double)v - (double)top) * by;
-  if (!(t > -60.0 * kPowers)) return 0.0;
-  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: what is added to it is rounded to a whole number
-  const double s = t + kRound;
-  const double r = t - (s - kRound);
-  const int n = __double2loint(s);
-  constexpr double c = 0.6931471805599453 / kPowers;
-  double p = c * c * c * c / 24.0;
-  p = fma(p, r, c * c * c / 6.0);
-  p = fma(p, r, c * c / 2.0);
-  p = fma(p, r, c);
-  p = fma(p, r, 1.0);
-  const double w = p * powers[n & (kPowers - 1)];
-  return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
-}
+// e^((v - top) / T) = 2^(n / 1024) 2^(r / 1024), |r| at most a half: the first from the
+// table, of the second the first terms of its series (the rest is below 2^-37 of it).
+struct Weights {
+  float top, by32;
+  double by;  // 1024 log2(e) / T
+  const double *powers;
+  __device__ __forceinline__ void set(float t, float temperature) {
+    top = t;
+    by = fmin(kPowers * 1.4426950408889634 / (double)temperature, 1e300);
+    by32 = (float)fmin(by, 3e38);
+  }
+  __device__ __forceinline__ double operator()(float v) const {
+    if (!((v - top) * by32 > -60.f * kPowers)) return v == top ? 1.0 : 0.0;  // (the largest may be +inf)
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: what is added to it is rounded to a whole number
+    constexpr double c = 0.6931471805599453 / kPowers;
+    const double d = (double)v - (double)top, s = fma(d, by, kRound), r = fma(d, by, kRound - s);
+    const int n = __double2loint(s);
+    const double w = fma(fma(c * c / 2.0, r, c), r, 1.0) * powers[n & (kPowers - 1)];
+    return __hiloint2double(__double2hiint(w) + (n >> 10) * (1 << 20), __double2loint(w));
+  }
+};
 
 struct Cut {  // kept: x > this one's, or x equal and number at most this one's
   float x;
@@ -128,11 +130,11 @@ struct Row {
   int n, first;    // its length, the number of its first token
   int ranks, rank;
   float top;       // the largest logit
-  double by;       // 64 log2(e) / T
+  Weights weight;
   Cut cut;
   int turn = 0;    // of `part`
 
-  __device__ Row(SampleShared &s) : sh(s) {}
+  __device__ Row(SampleShared &s) : sh(s) { weight.powers = s.powers; }
 
   __device__ __forceinline__ void sync() {
     if (ranks > 1)
@@ -145,7 +147,6 @@ struct Row {
     return ranks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
   }
 
-  __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, by, sh.powers); }
   __device__ __forceinline__ bool keeps(float v, int i) const { return v > cut.x || (v == cut.x && i <= cut.i); }
 
   // Sum (or maximum) of a and b over the cluster, to all its threads.
@@ -609,7 +610,7 @@ struct Row {
       }
       return;
     }
-    by = kPowers * 1.4426950408889634 / (double)want.t;
+    weight.set(top, want.t);
     cut = Cut{-INFINITY, -1};  // (-inf weighs nothing)
     // logits below this have no weight
     const float least = high == INFINITY ? top : (float)fmax(-low, high - kFar * (double)want.t);
@@ -864,13 +865,12 @@ struct Counter {
   const T *x;
   int vocab, skip;            // skip: how many elements before the row its first 16-byte piece begins
   float top;
-  double by;
+  Weights weight;
   uint32_t cut = kDead - 1;   // kept: smaller keys, and the first `room` (by number) of this one
   unsigned room = 0xffffffffu;
 
-  __device__ Counter(CountShared &s) : sh(s) {}
+  __device__ Counter(CountShared &s) : sh(s) { weight.powers = s.powers; }
 
-  __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, by, sh.powers); }
   __device__ __forceinline__ double weight_at(uint32_t k) const { return weight(Key<T>::value(k)); }
 
   // The keys of piece c of the row (16 bytes, in order).
@@ -1345,6 +1345,8 @@ struct Counter {
       const double w = weight(v);
       return want.enough(w, v == top) ? w : 0.0;
     };
+    const uint32_t k0 = first >> 16, end = cut >> 16;
+    const bool table = !kWide && end - k0 <= sizeof(sh.hist) / sizeof(double);
     __syncthreads();
     for (int e = threadIdx.x; e < kGroups; e += kCountThreads) sh.sum[e] = 0.0, sh.cnt[e] = 0;
     if constexpr (kWide) {
@@ -1386,7 +1388,7 @@ struct Counter {
           if (lane == 0) sh.sum[e0 + q * kCountWarps] = s, sh.cnt[e0 + q * kCountWarps] = cut_counts ? equal : 0u;
         }
       }
-    } else if ((cut >> 16) - (first >> 16) > sizeof(sh.hist) / sizeof(double)) {
+    } else if (!table) {
       // more values than a table holds (or everything) is kept: weights from the logits as they are
       __syncthreads();
       constexpr int kAtOnce = 4;
@@ -1426,13 +1428,12 @@ struct Counter {
         }
       }
     } else {
-      // the weights of the first kept values, in the counters' place
-      const uint32_t k0 = first >> 16, end = cut >> 16;  // (k0 .. end are kept)
-      double *const table = reinterpret_cast<double *>(sh.hist);
-      for (uint32_t i = threadIdx.x; k0 + i < end; i += kCountThreads) table[i] = before_cut((k0 + i) << 16);
+      // the weights of the kept values, in the counters' place
+      double *const weights = reinterpret_cast<double *>(sh.hist);
+      for (uint32_t i = threadIdx.x; k0 + i < end; i += kCountThreads) weights[i] = before_cut((k0 + i) << 16);
       __syncthreads();
       auto weigh = [&](uint32_t k, double &s, unsigned &equal) {
-        if (k < end) s += table[k - k0];
+        if (k < end) s += weights[k - k0];
         equal += k == end;
       };
       constexpr int kAtOnce = 4;
@@ -1592,7 +1593,7 @@ __global__ void __launch_bounds__(kCountThreads, 1) sample_count_k(const __grid_
     return;
   }
   c.top = Key<T>::value(first);
-  c.by = want.t > 0.f ? kPowers * 1.4426950408889634 / (double)want.t : 0.0;
+  c.weight.set(c.top, want.t > 0.f ? want.t : 1.f);
   if (!(want.t > 0.f)) {  // the first of the largest
     c.cut = first;
     c.room = 1;
