@@ -38,16 +38,16 @@ constexpr int kMaxRanks = 8;
 constexpr int kWindow = 16;  // bins around a guess
 constexpr double kFar = 41.588830833596715;  // 60 ln 2: what is further below the largest has no weight
 
-// 2^(j / 1024), j below 1024.
-constexpr int kPowers = 1024;
+// 2^(j / 256), j below 256.
+constexpr int kPowers = 256;
 __device__ __forceinline__ void fill_powers(double *powers) {
   for (int j = threadIdx.x; j < kPowers; j += blockDim.x) powers[j] = exp2(j / (double)kPowers);
 }
-// e^((v - top) / T) = 2^(n / 1024) 2^(r / 1024), |r| at most a half: the first from the
-// table, of the second the first terms of its series (the rest is below 2^-37 of it).
+// e^((v - top) / T) = 2^(n / 256) 2^(r / 256), |r| at most a half: the first from the
+// table, of the second the first terms of its series (the rest is below 2^-42 of it).
 struct Weights {
   float top, by32;
-  double by;  // 1024 log2(e) / T
+  double by;  // 256 log2(e) / T
   const double *powers;
   __device__ __forceinline__ void set(float t, float temperature) {
     top = t;
@@ -60,8 +60,8 @@ struct Weights {
     constexpr double c = 0.6931471805599453 / kPowers;
     const double d = (double)v - (double)top, s = fma(d, by, kRound), r = fma(d, by, kRound - s);
     const int n = __double2loint(s);
-    const double w = fma(fma(c * c / 2.0, r, c), r, 1.0) * powers[n & (kPowers - 1)];
-    return __hiloint2double(__double2hiint(w) + (n >> 10) * (1 << 20), __double2loint(w));
+    const double w = fma(fma(fma(c * c * c / 6.0, r, c * c / 2.0), r, c), r, 1.0) * powers[n & (kPowers - 1)];
+    return __hiloint2double(__double2hiint(w) + (n >> 8) * (1 << 20), __double2loint(w));
   }
 };
 
