@@ -470,10 +470,11 @@ struct Row {
 
   // Cuts where `target` is reached: of how many are kept (COUNT) or of what they weigh.
   template <bool COUNT>
-  __device__ void select(double target, float least, int vocab, bool counted) {
+  // counted: the bins from the largest logit down to `least` have been; guessed_bin: and the guess is this one (below 0: not made).
+  __device__ void select(double target, float least, int vocab, bool counted, int guessed_bin) {
     float hi = top, lo = least;
     double base = 0;
-    for (;; counted = false) {
+    for (;; counted = false, guessed_bin = -1) {
       if (!(lo < hi)) {
         // equal ones: as many as it takes
         const double w = COUNT ? 1.0 : weight(hi);
@@ -494,8 +495,11 @@ struct Row {
         // a guess by the weights of the bins' middles; then the weights up to a window
         // around it are added up one by one
         auto guess = [&](int k) { return sh.hist[k] ? sh.hist[k] * weight(bins.middle(k)) : 0.0; };
-        find(target - base, guess);
-        b = sh.found;
+        b = guessed_bin;
+        if (b < 0) {
+          find(target - base, guess);
+          b = sh.found;
+        }
         int from = 0, to = kBins - 1;  // the bin is one of these
         for (;;) {
           const int w0 = max(from, min(b - kWindow / 2, to + 1 - kWindow));
@@ -555,14 +559,20 @@ struct Row {
           if (COUNT) {
             at = (unsigned)(target - base) - 1;
           } else {
-            for (unsigned e = threadIdx.x; e < listed; e += kThreads) sh.mass[e] = weight(from_falling((uint32_t)(sh.key[e] >> 32)));
-            __syncthreads();
-            if (threadIdx.x == 0) {
-              double s = base;
-              unsigned e = 0;
-              while (e + 1 < listed && (s += sh.mass[e]) < target) ++e;
-              sh.found = (int)e;
+            double c[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const unsigned e = kPer * threadIdx.x + i;
+              c[i] = e < listed ? weight(from_falling((uint32_t)(sh.key[e] >> 32))) : 0.0;
             }
+            if (threadIdx.x == 0) sh.found = (int)listed - 1;
+            scan(c);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+              if (kPer * threadIdx.x + i < listed && base + c[i] >= target) {
+                atomicMin(&sh.found, (int)(kPer * threadIdx.x) + i);
+                break;
+              }
             __syncthreads();
             at = (unsigned)sh.found;
           }
@@ -620,6 +630,7 @@ struct Row {
       reduce<false>(mass, none);
     }
     bool counted = false;
+    int guess = -1;
     if ((want.p < 1.f || want.k) && want.k <= kList && least < top) {
       // what is kept, if it is not much, goes through one list
       const Bins bins(top, least);
@@ -632,6 +643,7 @@ struct Row {
       int b = sh.found;
       unsigned many = sh.before + sh.in_bin;
       if (!want.k) {  // (the bins' middles are a guess: two more)
+        guess = b;
         for (int more = 0; more < 2 && b + 1 < kBins; ++more) many += sh.hist[++b];
       }
       __syncthreads();
@@ -645,14 +657,14 @@ struct Row {
         if (sh.reached) return;
       }
     }
-    if (want.k) select<true>((double)want.k, least, a.vocab, counted);
+    if (want.k) select<true>((double)want.k, least, a.vocab, counted, -1);
     if (want.p < 1.f) {
       if (want.k) {
         mass = 0;
         each([&](float v, int i) { mass += keeps(v, i) ? weight(v) : 0.0; });
         reduce<false>(mass, none);
       }
-      select<false>((double)want.p * mass, least, a.vocab, counted && !want.k);
+      select<false>((double)want.p * mass, least, a.vocab, counted && !want.k, guess);
     }
     // ---- running sums, by number: a warp has a piece of the slice, in steps of 128
     const float lowest = want.floor(top);
