@@ -46,16 +46,22 @@ __device__ __forceinline__ void fill_powers(double *powers) {
 // e^((v - top) / T) = 2^(n / 256) 2^(r / 256), |r| at most a half: the first from the
 // table, of the second the first terms of its series (the rest is below 2^-42 of it).
 struct Weights {
-  float top, by32;
+  float top;
+  // Whether a weight is 0 is asked in 32 bits: (v times - top_times) by32, where neither
+  // the difference of the largest numbers nor a division by the smallest runs over.
+  float times, top_times, by32;
   double by;  // 256 log2(e) / T
   const double *powers;
   __device__ __forceinline__ void set(float t, float temperature) {
     top = t;
-    by = fmin(kPowers * 1.4426950408889634 / (double)temperature, 1e300);
-    by32 = (float)fmin(by, 3e38);
+    by = kPowers * 1.4426950408889634 / (double)temperature;
+    const bool small = by > 0x1p126 && fabsf(top) < 0x1p27f;  // (a larger one is by more than 60 bits above the next)
+    times = small ? 0x1p100f : 0.5f;
+    top_times = top * times;
+    by32 = (float)(by / (double)times);
   }
   __device__ __forceinline__ double operator()(float v) const {
-    if (!((v - top) * by32 > -60.f * kPowers)) return v == top ? 1.0 : 0.0;  // (the largest may be +inf)
+    if (!(fmaf(v, times, -top_times) * by32 > -60.f * kPowers)) return v == top ? 1.0 : 0.0;  // (the largest may be +inf)
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: what is added to it is rounded to a whole number
     constexpr double c = 0.6931471805599453 / kPowers;
     const double d = (double)v - (double)top, s = fma(d, by, kRound), r = fma(d, by, kRound - s);

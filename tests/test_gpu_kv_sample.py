@@ -255,3 +255,18 @@ def test_refusals(ops):
             ops.sample(stream=stream(), **args)
     with pytest.raises(ivb.NativeError):
         ops.sample(torch.empty((1, 500001), dtype=torch.float16, device="cuda"), u[:1], t[:1], stream=stream())
+
+
+@pytest.mark.parametrize("rows", [2, 120])
+def test_extreme_temperatures(ops, rows):
+    """Logits and temperatures whose difference or quotient does not fit into 32 bits."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    u, low = uniform(rows, 11), torch.finfo(torch.float32).min
+    x = torch.rand((rows, 3001), generator=g, device="cuda")
+    for y, t in (((x * 6 - 3) * 1e38, 1e38), ((x * 6 - 3) * 1e38, 3e38), (x * 2e-37, 1e-38), (x * -4e-44, 1e-44), (x * 1e-30, 1e-40), (x - 2.0 ** 28, 1e-40),
+                 (torch.where(x > 0.5, low, -low), 3e38), (torch.where(x > 0.5, low, -low), INF)):
+        for k, p in ((None, None), (40, None), (None, 0.6)):
+            check(ops, y, u, temperature=[t] * rows, top_k=None if k is None else [k] * rows, top_p=None if p is None else [p] * rows)
+    z = (x * 1.2e5 - 6e4).to(torch.float16)
+    check(ops, z, u, temperature=[3e4] * rows, top_p=[0.7] * rows)
+    check(ops, ((x * 6 - 3) * 1e38).to(torch.bfloat16), u, temperature=[1e38] * rows, top_p=[0.7] * rows)
