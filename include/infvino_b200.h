@@ -228,8 +228,9 @@ void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
 
 /* ------------------------------------------------------------------------
  * Language-model operators: rotary positions, a paged key/value cache held in
- * 8 bits, and the attention over it, for a decoder that follows a network of
- * this library (its outputs become tokens).  Inference only.
+ * 8 bits, the attention over it, products in microscaled 4-bit numbers and the
+ * choice of tokens, for a decoder that follows a network of this library (its
+ * outputs become tokens).  Inference only.
  *
  * All tensors are device memory of the handle's device; nothing is copied and
  * no call waits for the device.  `stream` is a cudaStream_t; NULL is the
@@ -243,12 +244,13 @@ void ivc_f16_to_f32(const uint16_t *in, float *out, size_t n);
  * whose offsets or length do not fit, and the keys in a page outside the cache,
  * as if they were hidden.  The others of the call are as they would be alone.
  *
- * Calls may be captured into a CUDA graph once the stream has had one call of
- * ivc_kv_attend or ivc_kv_reserve (each stream has its own workspace, so calls
- * on several streams may run at the same time; cudaStreamPerThread is another
- * stream in every thread).  A graph uses the workspace of the stream that it
- * was captured on: its replays must not overlap one another, other graphs'
- * from that stream, or eager calls on it. */
+ * Calls may be captured into a CUDA graph, ivc_kv_attend and
+ * ivc_kv_attend_shared once the stream has had one call of either or of
+ * ivc_kv_reserve (each stream has its own workspace, so calls on several streams
+ * may run at the same time; cudaStreamPerThread is another stream in every
+ * thread).  A graph with one of these uses the workspace of the stream that it
+ * was captured on: its replays must not overlap one another, other graphs' from
+ * that stream, or eager calls on it. */
 typedef struct ivc_kv ivc_kv;
 
 typedef enum ivc_dtype { IVC_F16 = 0, IVC_BF16 = 1, IVC_F32 = 2 /* logits only */ } ivc_dtype;
@@ -431,8 +433,9 @@ int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64
 int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *out, int64_t out_stride, void *stream);
 /* out [rows][w->rows] = X W^T, summed in f32 and rounded once: W is w; X is the
  * first `rows` rows of xq if x is NULL, else x [rows][width] (x_dtype), quantised as
- * ivc_kv_mx4_quantize does it: xq is room for that then, and what it holds
- * afterwards is not defined.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
+ * ivc_kv_mx4_quantize does it: xq is room for that then, of nobody else until
+ * the call has run, and what it holds afterwards is not defined.  out shares no
+ * memory with the others.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
 int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
                       const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream);
 

@@ -154,7 +154,7 @@ bool rows_vec(const void *p, long long stride) { return reinterpret_cast<uintptr
 //              lie in memory: 512 bytes for 128 rows x 128 of the width)
 //   warp 1     copies a stage's scales into TMEM and issues its products
 //   warps 2 .. take a finished tile out of TMEM: a thread a weight row
-// Two sets of accumulators: a tile's products run while the one before it goes out.
+// Where TMEM has two sets of accumulators a tile's products run while the one before it goes out.
 //
 // Every wait is bounded: a timeout sets the status word and an abort flag, all
 // roles run out.
@@ -166,7 +166,8 @@ constexpr int kMostSplit = 8;          // CTAs of a cluster that share a tile
 // MT: weight tiles of 128 rows that share a stage's tokens.  What an SM gets from the L2 in
 // a clock (some 38 bytes when all ask) bounds products with many tokens, and weights,
 // from memory, queue up behind tokens in the copies of those with some: two weight tiles
-// halve the tokens' part.
+// halve the tokens' part.  (4001 tokens x 4096 -> 14336: 121 us with 256 x 192 tiles, 1.18 GB
+// into the SMs, the tensor cores 45 % of the time at work; the loads alone 93.)
 template <int TN, int MT>
 struct Tile {
   static constexpr int kRows = 128 * MT;                   // weight rows of a tile
@@ -252,9 +253,6 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
       : "memory");
 }
 
-// FUSE: 0: X comes from memory in 4 bits; 1, 2: from halves / bf16 rows, which the CTA
-// quantises itself, with kFuseWarps more warps.  Few rows: every CTA does it for its
-// stages again, but a launch is saved, and the weights are on their way meanwhile.
 // Sixteen outputs of a token, the first n of them.
 template <bool BF16>
 __device__ __forceinline__ void store_outputs(uint16_t *out, const float (&v)[16], int n, bool vec) {
@@ -272,6 +270,9 @@ __device__ __forceinline__ void store_outputs(uint16_t *out, const float (&v)[16
     if (i < n) out[i] = (uint16_t)pack2<BF16>(v[i], v[i]);
 }
 
+// FUSE: 0: X comes from memory in 4 bits; 1, 2: from halves / bf16 rows, which the CTA
+// quantises itself, with kFuseWarps more warps.  Few rows: every CTA does it for its
+// stages again, but a launch is saved, and the weights are on their way meanwhile.
 template <int TN, int MT, bool BF16, int FUSE>
 __global__ void __launch_bounds__(Tile<TN, MT>::kThreads + (FUSE ? 32 * kFuseWarps : 0), Tile<TN, MT>::kCtas)
     mx4_linear_k(const __grid_constant__ LinearArgs a) {
@@ -625,7 +626,8 @@ LinearPlan linear_plan(const Mx4Linear &l) {
     const long long tiles = (lanes + 128 * mt - 1) / (128 * mt) * ((columns + tn - 1) / tn);
     if (tiles > 0x7fffffffLL) continue;
     // Us, from measurements at 1 to 4001 tokens (within some 10 %): a stage's bytes into an
-    // SM, weights slower than tokens, or all weights out of memory; starting and ending; a tile's results where nothing else runs meanwhile, or a cluster's gathering.
+    // SM, weights slower than tokens, or all weights out of memory; starting and ending; a
+    // tile's results where nothing else runs meanwhile, or a cluster's gathering.
     const double weights = mt * kMm * 136.0, tokens = tn * 136.0;
     for (int split = 1; split <= (swap ? 1 : kMostSplit); ++split) {
       if (split > 1 && (split > ks || tiles > linear_clusters(l.device, mt, split))) continue;

@@ -263,6 +263,17 @@ ivb::Mx4 check_mx4(const ivc_mx4 *m) {
   return ivb::Mx4{m->codes, m->scales, m->rows, m->width};
 }
 
+bool apart(const ivb::Mx4 &a, const ivb::Mx4 &b) {
+  auto disjoint = [](const uint8_t *p, int64_t n, const uint8_t *q, int64_t m) {
+    const auto x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return x + n <= y || y + m <= x;
+  };
+  auto codes = [](const ivb::Mx4 &m) { return m.rows * (m.width / 2); };
+  auto scales = [](const ivb::Mx4 &m) { return (m.rows + 127) / 128 * ((m.width + 127) / 128) * 512; };
+  return disjoint(a.codes, codes(a), b.codes, codes(b)) && disjoint(a.codes, codes(a), b.scales, scales(b)) &&
+         disjoint(a.scales, scales(a), b.codes, codes(b)) && disjoint(a.scales, scales(a), b.scales, scales(b));
+}
+
 void check_matrix(int dtype, const void *p, int64_t rows, int64_t width, int64_t stride, bool written) {
   check_dtype(dtype);
   need(rows >= 0 && rows <= kMaxTokens, "rows out of range");
@@ -565,11 +576,13 @@ int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64
     if (x) check_matrix(x_dtype, x, rows, a.x.width, x_stride, false);
     need(rows <= a.x.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0 || a.w.rows == 0) return;
+    a.x.rows = rows;
+    need(!x || apart(a.x, a.w), "the room for x in 4 bits overlaps the weights");
+    need(x != out, "out is x");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     a.rows = x;
     a.x_stride = x_stride;
     a.x_bf16 = x_dtype == IVC_BF16;
-    a.x.rows = rows;
     a.out = out;
     a.stride = out_stride;
     a.bf16 = out_dtype == IVC_BF16;

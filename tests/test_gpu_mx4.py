@@ -314,3 +314,21 @@ def test_refusals(ops):
     ops.mx4_quantize(x[:0], m, stream=stream())
     ops.mx4_read(m, x[:0], stream=stream())
     ops.mx4_linear(x[:0], m, out[:0], scratch=m, stream=stream())
+
+
+def test_shared_memory_is_refused(ops):
+    """Room for x inside the weights, or the output in x's place, would be read and written at once."""
+    big, s = empty(256, 64)
+    w, x = ivb.Mx4(big[:64], s[:1]), torch.zeros((16, 64), dtype=torch.float16, device="cuda")
+    out = torch.zeros((16, 64), dtype=torch.float16, device="cuda")
+    for room in ((big[48:64], s[1:]), (big[63:80], s[1:]), (big[128:144], s[:1])):
+        with pytest.raises(ivb.NativeError):
+            ops.mx4_linear(x, w, out, scratch=ivb.Mx4(*room), stream=stream())
+    with pytest.raises(ivb.NativeError):
+        ops.mx4_linear(x, w, x, scratch=ivb.Mx4(big[64:80], s[1:]), stream=stream())
+    ops.mx4_quantize(torch.ones((64, 64), dtype=torch.float16, device="cuda"), w, stream=stream())
+    ops.mx4_linear(x + 1, w, out, scratch=ivb.Mx4(big[64:80], s[1:]), stream=stream())
+    xq = ivb.Mx4(big[48:64], torch.zeros_like(s[:1]))
+    ops.mx4_linear(xq, w, out.clone(), stream=stream())  # (what is only read may be shared)
+    ops.synchronize(stream())
+    assert (out == 64).all()
