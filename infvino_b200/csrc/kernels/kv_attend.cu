@@ -47,6 +47,7 @@ namespace ivb {
 namespace {
 
 constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps;
+constexpr unsigned kStepItemCost = 8;  // of items that are not cut: start and join, in blocks
 constexpr int kStepStages = 4;  // blocks of a warp's ring; two are worked on at once
 // A CTA's share is at least this: four blocks for each warp (777 keys, 4 kv
 // heads: 12.2 us; one block 14.1, two 12.6, eight 15.3: joining against reading).
@@ -133,6 +134,13 @@ struct StepShared {
   int most[kStepWarps];
 };
 
+// Of kRest: what sequences are, behind the above, where there is one for each thread
+// at most.  (Looked up again, each has a chain of three loads: 98 us for a call of 96
+// sequences in 6 groups, 94 so.)
+struct StepKept {
+  int first, n, len, first_block, blocks;
+};
+
 // NT: 8-row tiles of queries that share the codes of an item.
 template <bool BF16, int DIM, int NT, int MODE>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
@@ -146,7 +154,10 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   constexpr int kTile = kKvBlock * DIM;  // bytes of a block's keys or values
   constexpr int kZ = 2;                  // blocks worked on at once
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  pdl_wait_and_release();
+  // (kRest: its launch begins when every CTA of the one before, which works on the
+  // beginning, has; that one's results are wanted, and its place in the workspace is free,
+  // only at a segment's end)
+  if (MODE != kRest) pdl_wait_and_release();
 
   // ---- all units, and the sequence where this CTA's share begins
   const int per = (a.seqs.batch + kStepThreads - 1) / kStepThreads;
@@ -154,8 +165,18 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   const int b_lo = min(a.seqs.batch, (int)threadIdx.x * per), b_hi = min(a.seqs.batch, b_lo + per);
   long long my_items = 0;
   int most = 0;
+  StepKept *const kept = reinterpret_cast<StepKept *>(smem_raw + sizeof(StepShared<DIM, NT>));
+  auto span_of = [&](int b) {
+    if (MODE != kRest || per > 1) return kv_span<MODE>(a, b);
+    const StepKept k = kept[b];
+    KvSpan s;
+    s.first = k.first, s.n = k.n, s.len = k.len, s.first_block = k.first_block, s.blocks = k.blocks;
+    s.sink_blocks = s.lead = s.common = 0;
+    return s;
+  };
   for (int b = b_lo; b < b_hi; ++b) {
     const KvSpan s = kv_span<MODE>(a, b);
+    if (MODE == kRest && per == 1) kept[b] = StepKept{s.first, s.n, s.len, s.first_block, s.blocks};
     const long long items = (long long)((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
     mine += s.blocks * items;
     if (MODE == kRest) my_items += items, most = max(most, s.blocks);
@@ -179,18 +200,24 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
-  if (total == 0) return;
+  // (no CTA ends before the launch before: what follows relies on that)
+  if (total == 0) {
+    if (MODE == kRest) pdl_wait_and_release();
+    return;
+  }
   if (total > 0x7fffffffLL) {  // (hours of work; units are counted in 32 bits from here)
     if (threadIdx.x == 0) kv_flag(a.status, kStatusKvSeqs);
+    if (MODE == kRest) pdl_wait_and_release();
     return;
   }
   uint32_t at_least = kStepMinBlocks;
-  bool by_item = false;  // a share is some whole items
+  bool by_item = false;  // a share is the items that begin in it, whole
   long long excl = before + incl - mine;
+  uint32_t cost = 0;  // units of an item beside its blocks
   if (MODE == kRest) {
-    // What sequences have of their own is often a few blocks.  Where whole items
-    // divide about as evenly as blocks, nothing is cut (64 sequences of up to 500 keys of
-    // their own, 8 heads: 25 us against 28); else a share is no more than an item.
+    // What sequences have of their own is often a few blocks.  Where no item is much more
+    // than a share, nothing is cut (64 sequences of up to 500 keys of their own, 8 heads:
+    // 25 us for this launch alone against 28); else a share is no more than an item.
     long long items_before = 0, items = 0;
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w) {
@@ -198,21 +225,26 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       items += sh.scan_items[w];
       most = max(most, sh.most[w]);
     }
-    const long long turns = (items + gridDim.x - 1) / gridDim.x;
-    by_item = most * turns <= 2 * ((total + gridDim.x - 1) / gridDim.x) + 24;
+    by_item = most <= (total + gridDim.x - 1) / gridDim.x + 24 && total + kStepItemCost * items <= 0x7fffffffLL;
     at_least = by_item ? 1u : (uint32_t)min(total / max(items, 1ll) + 1, (long long)kStepMinBlocks);
-    if (by_item) total = items, mine = my_items, excl = items_before + incl_items - my_items;
+    if (by_item) {
+      cost = kStepItemCost;
+      total += cost * items, mine += cost * my_items, excl += cost * (items_before + incl_items - my_items);
+    }
   }
-  auto units_of = [&](const KvSpan &s) { return MODE == kRest && by_item ? 1u : (uint32_t)s.blocks; };
+  auto units_of = [&](const KvSpan &s) { return MODE == kRest ? (uint32_t)s.blocks + cost : (uint32_t)s.blocks; };
   const uint32_t size = max(at_least, ((uint32_t)total + gridDim.x - 1) / gridDim.x);  // units of a share
   uint32_t u = blockIdx.x * size;
-  if (u >= (uint32_t)total) return;
+  if (u >= (uint32_t)total) {
+    if (MODE == kRest) pdl_wait_and_release();
+    return;
+  }
   const uint32_t u_end = min((uint32_t)total, u + size);
   if (u >= excl && u < excl + mine) {
     long long at = excl;
     int b = b_lo;
     for (;; ++b) {
-      const KvSpan s = kv_span<MODE>(a, b);
+      const KvSpan s = span_of(b);
       const long long w = (long long)units_of(s) * ((s.n * a.group + kRows - 1) / kRows) * a.cache.heads;
       if (u < at + w) break;
       at += w;
@@ -223,8 +255,16 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
   __syncthreads();
   int b = sh.seq;
   uint32_t base = (uint32_t)sh.base;  // first unit of sequence b
-  KvSpan s = kv_span<MODE>(a, b);
+  KvSpan s = span_of(b);
   int row_tiles = (s.n * a.group + kRows - 1) / kRows;
+  if (MODE == kRest && by_item) {  // from the first item that begins here
+    const uint32_t into = (u - base) % units_of(s);
+    if (into) u += units_of(s) - into;
+    if (u >= u_end) {
+      pdl_wait_and_release();
+      return;
+    }
+  }
 
   // ---- this lane's places in a tile of codes
   const uint32_t ring = smem_u32(&sh.ring[warp][0][0][0]);
@@ -244,14 +284,14 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       const uint32_t units = units_of(s) * (uint32_t)row_tiles * (uint32_t)a.cache.heads;
       if (u < base + units) break;
       base += units;
-      s = kv_span<MODE>(a, ++b);  // (units are left, so there is a next sequence)
+      s = span_of(++b);  // (units are left, so there is a next sequence)
       row_tiles = (s.n * a.group + kRows - 1) / kRows;
     }
     const uint32_t item = (u - base) / units_of(s);
     head = (int)(item / (uint32_t)row_tiles);
     rt = (int)item - head * row_tiles;
     item_begin = base + item * units_of(s);
-    k0 = MODE == kRest && by_item ? 0 : (int)(u - item_begin);
+    k0 = (int)(u - item_begin);
     k1 = MODE == kRest && by_item ? s.blocks : (int)(min(u_end, item_begin + (uint32_t)s.blocks) - item_begin);
     count = k1 - k0 > warp ? (k1 - k0 - warp + kStepWarps - 1) / kStepWarps : 0;
     looked = 0;
@@ -268,12 +308,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
         if (it + lane < count) {
           const int key = s.block(k0 + warp + (it + lane) * kStepWarps) * kKvBlock;
           if (key < s.len) {
-            const int at = fast_div(key, a.by_page), page = a.seqs.pages[kv_page_at<MODE>(a, s, b, key, at)];
+            const int at = fast_div(key, a.by_page), page = kv_get<MODE>(a.seqs.pages + kv_page_at<MODE>(a, s, b, key, at));
             if ((unsigned)page < (unsigned long long)a.cache.pages) {
               const int slot = key - at * a.cache.page;
               where = kv_code_at(a.cache, page, head, slot);
               const long long sa = kv_scale_at(a.cache, page, head, slot);
-              sc_mine = make_float2(a.cache.ks[sa], fmaxf(log2_of(a.cache.vs[sa]), kNoValue));
+              sc_mine = make_float2(kv_get<MODE>(a.cache.ks + sa), fmaxf(log2_of(kv_get<MODE>(a.cache.vs + sa)), kNoValue));
             } else {
               kv_flag(a.status, kStatusKvPage);
             }
@@ -319,8 +359,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
       uint32_t w[2 * kTiles];
 #pragma unroll
       for (int c = 0; c < DIM / 64; ++c) {
-        const uint4 x = i < s.n ? load8(row + 64 * c + 16 * t4, a.q.vec) : make_uint4(0, 0, 0, 0);
-        const uint4 y = i < s.n ? load8(row + 64 * c + 16 * t4 + 8, a.q.vec) : make_uint4(0, 0, 0, 0);
+        const uint4 x = i < s.n ? load8<MODE == kRest>(row + 64 * c + 16 * t4, a.q.vec) : make_uint4(0, 0, 0, 0);
+        const uint4 y = i < s.n ? load8<MODE == kRest>(row + 64 * c + 16 * t4 + 8, a.q.vec) : make_uint4(0, 0, 0, 0);
         w[8 * c] = x.x, w[8 * c + 1] = x.y, w[8 * c + 2] = x.z, w[8 * c + 3] = x.w;
         w[8 * c + 4] = y.x, w[8 * c + 5] = y.y, w[8 * c + 6] = y.z, w[8 * c + 7] = y.w;
       }
@@ -532,13 +572,15 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
     const int n = s.n, first = s.first, head_now = head, rt_now = rt;
     const bool begins = k0 == 0, whole = begins && k1 == s.blocks, joins = MODE == kRest && s.first_block > 0;
     const int first_cta = (int)(item_begin / size), last_cta = (int)((item_begin + (uint32_t)s.blocks - 1u) / size);
-    u += MODE == kRest && by_item ? 1u : (uint32_t)(k1 - k0);
+    u += (uint32_t)(k1 - k0) + cost;
     const bool more = u < u_end;
     if (more) {
       locate();
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) fetch(i);
     }
+
+    if (MODE == kRest) pdl_wait_and_release();
 
     // ---- join the warps: row maxima, then sums in a common scale
 #pragma unroll
@@ -667,7 +709,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(DIM, NT))
 template <bool BF16, int DIM, int NT, int MODE>
 cudaError_t launch_step(const KvAttend &a, void *workspace, int sms, cudaStream_t st) {
   static std::atomic<bool> attr_set[kAttrMaxDevices];
-  const int bytes = (int)sizeof(StepShared<DIM, NT>);
+  const int bytes = (int)(sizeof(StepShared<DIM, NT>) + (MODE == kRest ? sizeof(StepKept) * kStepThreads : 0));
   const cudaError_t e = ensure_dynamic_smem(kv_step_k<BF16, DIM, NT, MODE>, bytes, attr_set);
   if (e != cudaSuccess) return e;
   const int grid = sms * step_ctas(DIM, NT);

@@ -67,16 +67,25 @@ struct KvSpan {
 // those results joined in; or both in one pass, each sequence reading the beginning.
 enum KvMode { kWhole = 0, kBegin = 1, kRest = 2, kOne = 3 };
 
+// What a launch reads.  The step kernel of kRest begins while the launch before it, of
+// the same call, still works on the beginning: what was written before that launch is in
+// the L2 by then, but an SM's own cache may hold it as it was earlier.
+template <int MODE, class T>
+__device__ __forceinline__ T kv_get(const T *p) {
+  return MODE == kRest ? __ldcg(p) : *p;
+}
+
 // A group's sequences s0 .. s1 - 1, its packed tokens o .. e - 1, and how many are common; false (status set) if that does not fit.
 struct KvGroup {
   int s0, s1, o, e, len;
 };
+template <int MODE>
 __device__ __forceinline__ bool kv_group(const KvAttend &a, int g, KvGroup &r) {
-  r.s0 = a.first[g], r.s1 = a.first[g + 1], r.len = a.shared[g];
+  r.s0 = kv_get<MODE>(a.first + g), r.s1 = kv_get<MODE>(a.first + g + 1), r.len = kv_get<MODE>(a.shared + g);
   bool fits = r.s0 >= 0 && r.s1 >= r.s0 && r.s1 <= a.sequences && r.len >= 0 && r.len <= (long long)a.seqs.pps * a.cache.page &&
               r.len == fast_div(r.len, a.by_page) * a.cache.page;
   if (fits) {
-    r.o = a.seqs.offsets[r.s0], r.e = a.seqs.offsets[r.s1];
+    r.o = kv_get<MODE>(a.seqs.offsets + r.s0), r.e = kv_get<MODE>(a.seqs.offsets + r.s1);
     fits = r.o >= 0 && r.e >= r.o && r.e <= a.seqs.tokens;
   }
   if (!fits) kv_flag(a.status, kStatusKvSeqs);
@@ -92,7 +101,7 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
   if (MODE == kBegin) {
     KvGroup r;
     s.first = s.n = s.len = 0;
-    if (!kv_group(a, b, r) || r.o == r.e || r.len == 0) return s;
+    if (!kv_group<MODE>(a, b, r) || r.o == r.e || r.len == 0) return s;
     s.first = r.o;
     s.n = r.e - r.o;
     s.lead = r.s0;
@@ -100,9 +109,9 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
     s.blocks = r.len / kKvBlock;
     return s;
   }
-  const int o = a.seqs.offsets[b], e = a.seqs.offsets[b + 1];
+  const int o = kv_get<MODE>(a.seqs.offsets + b), e = kv_get<MODE>(a.seqs.offsets + b + 1);
   s.first = o;
-  s.len = a.seqs.at[b];
+  s.len = kv_get<MODE>(a.seqs.at + b);
   s.n = e - o;
   if (o < 0 || e < o || e > a.seqs.tokens || s.n > a.max_new || s.len < 0 ||
       s.len > (long long)a.seqs.pps * a.cache.page) {
@@ -116,14 +125,14 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttend &a, int b) {
     int g = 0, end = a.groups;  // the last group that begins at or before b
     while (end - g > 1) {
       const int mid = (g + end) / 2;
-      if (a.first[mid] <= b)
+      if (kv_get<MODE>(a.first + mid) <= b)
         g = mid;
       else
         end = mid;
     }
     // (its tokens are the group's: their results over the beginning are there)
     KvGroup r;
-    if (!kv_group(a, g, r) || b < r.s0 || b >= r.s1 || o < r.o || e > r.e || s.len - s.n < r.len) {
+    if (!kv_group<MODE>(a, g, r) || b < r.s0 || b >= r.s1 || o < r.o || e > r.e || s.len - s.n < r.len) {
       kv_flag(a.status, kStatusKvSeqs);
       s.n = 0;
       return s;

@@ -35,13 +35,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // Eight consecutive 16-bit elements; element by element (a small loop, so that
 // every use does not carry eight copies) where the row is not on 16 bytes.
+template <bool L2 = false>  // (past the SM's own cache)
 __device__ __forceinline__ uint4 load8(const uint16_t *p, bool vec) {
-  if (vec) return *reinterpret_cast<const uint4 *>(p);
+  if (vec) return L2 ? __ldcg(reinterpret_cast<const uint4 *>(p)) : *reinterpret_cast<const uint4 *>(p);
   uint64_t lo = 0, hi = 0;
 #pragma unroll 1
   for (int i = 7; i >= 0; --i) {
     hi = (hi << 16) | (lo >> 48);
-    lo = (lo << 16) | p[i];
+    lo = (lo << 16) | (L2 ? __ldcg(p + i) : p[i]);
   }
   return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
