@@ -76,6 +76,28 @@ struct Cut {  // kept: x > this one's, or x equal and number at most this one's
   int i;
 };
 
+// Weights summed up in kWindow bins as whole numbers of 2^-44, so that their order does not
+// matter: in four pieces of 12 bits (a row has less than 2^19 tokens), since shared memory
+// adds 32 bits at once, and 64 by trying until nobody interferes.
+struct Window {
+  unsigned piece[4][kWindow];
+  __device__ __forceinline__ void clear() {
+    if (threadIdx.x < 4 * kWindow) (&piece[0][0])[threadIdx.x] = 0;
+  }
+  __device__ __forceinline__ void add(unsigned k, double w) {
+    const unsigned long long f = __double2ull_rn(w * 0x1p44);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) atomicAdd(&piece[q][k], (unsigned)(f >> (12 * q)) & 0xfffu);
+  }
+  __device__ __forceinline__ unsigned long long sum(unsigned k) const {
+    unsigned long long f = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f += (unsigned long long)piece[q][k] << (12 * q);
+    return f;
+  }
+};
+static_assert(kSampleMaxVocab < 1 << 19, "pieces of a sum");
+
 struct SampleShared {
   double powers[kPowers];
   unsigned hist[kBins];
@@ -84,12 +106,12 @@ struct SampleShared {
   double part[2][kMaxRanks][2];   // what CTAs tell one another, two exchanges in turn
   double red[2][kMostWarps];
   unsigned cnt[kMostWarps];
-  unsigned listed;
+  unsigned listed, staged, place;
   int found, kept, reached;
   unsigned before, in_bin;
   Cut cut;
   double seg[kMostWarps];
-  unsigned long long window[kWindow];
+  Window window;
 };
 
 // Order of floats as unsigned numbers, falling (no NaN, no -0).
@@ -215,12 +237,19 @@ struct Row {
   // Counts into sh.hist, over the cluster, what bin(logit, number) says (below 0: nothing).
   template <class F>
   __device__ void count(F &&bin) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
-    __syncthreads();
+    clear();
     each([&](float v, int i) {
       const int b = bin(v, i);
       if (b >= 0) atomicAdd(&sh.hist[b], 1u);
     });
+    merge();
+  }
+  __device__ void clear() {
+    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
+    __syncthreads();
+  }
+  // The CTAs' counts become the cluster's.
+  __device__ void merge() {
     if (ranks == 1) {
       __syncthreads();
       return;
@@ -301,42 +330,72 @@ struct Row {
     return m;
   }
 
-  // Puts those of which in(logit, number) holds (at most kList) in order, in CTA 0: sh.key; how many there are is returned there.
+  // Collects those of which in(logit, number) holds, in CTA 0's sh.key and sh.listed (more
+  // than kList: not all).  A CTA collects its own first (all counting in CTA 0: up to 6000
+  // clocks more for 1000 of 131072).
   template <class F>
-  __device__ unsigned gather(F &&in) {
-    if (threadIdx.x == 0) sh.listed = 0;
+  __device__ void collect(F &&in) {
+    if (threadIdx.x == 0) sh.listed = 0, sh.staged = 0;
     sync();
-    unsigned *listed = at(&sh.listed, 0);
-    unsigned long long *key = at(sh.key, 0);
+    unsigned long long *const stage = ranks > 1 ? reinterpret_cast<unsigned long long *>(sh.mass) : sh.key;
+    unsigned *const counter = ranks > 1 ? &sh.staged : &sh.listed;
     each([&](float v, int i) {
       if (!in(v, i)) return;
-      const unsigned p = atomicAdd(listed, 1u);
-      if (p < kList) key[p] = ((unsigned long long)falling(v) << 32) | (unsigned)i;
+      const unsigned p = atomicAdd(counter, 1u);
+      if (p < kList) stage[p] = ((unsigned long long)falling(v) << 32) | (unsigned)i;
     });
+    __syncthreads();
+    if (ranks == 1) return;
+    if (threadIdx.x == 0 && sh.staged) sh.place = atomicAdd(at(&sh.listed, 0), sh.staged);
+    __syncthreads();
+    unsigned long long *const key = at(sh.key, 0);
+    for (unsigned e = threadIdx.x; e < min(sh.staged, (unsigned)kList) && sh.place + e < kList; e += kThreads) key[sh.place + e] = stage[e];
     sync();
+  }
+  // Those, at most kList, in order; how many there are is returned in CTA 0.
+  template <class F>
+  __device__ unsigned gather(F &&in) {
+    collect(in);
     const unsigned n = min(sh.listed, (unsigned)kList);
     if (rank == 0) sort(n);
     return n;
   }
 
-  // Rising, padded with ~0 to a power of two.  Steps over at most 32 stay inside a warp's 64 keys.
+  // The n keys in rising order: two neighbours a thread, exchanged in registers but for steps
+  // of 64 and more.  (All steps in shared memory: some 6000 clocks more for 1024 keys.)
   __device__ void sort(unsigned n) {
+    using Key = unsigned long long;
     unsigned size = 2;
     while (size < n) size <<= 1;
-    for (unsigned e = n + threadIdx.x; e < size; e += kThreads) sh.key[e] = ~0ull;
-    __syncthreads();
-    for (unsigned k = 2; k <= size; k <<= 1)
-      for (unsigned j = k >> 1; j; j >>= 1) {
-        for (unsigned e = threadIdx.x; e < size / 2; e += kThreads) {
-          const unsigned a = 2 * e - (e & (j - 1)), b = a + j;
-          const unsigned long long s = sh.key[a], t = sh.key[b];
-          if ((s > t) == ((a & k) == 0)) sh.key[a] = t, sh.key[b] = s;
+    const unsigned e = 2 * threadIdx.x;
+    const bool works = 2 * (threadIdx.x & ~31u) < size;
+    Key a = works && e < n ? sh.key[e] : ~0ull, b = works && e + 1 < n ? sh.key[e + 1] : ~0ull;
+    auto keep = [](Key &x, Key y, bool less) { x = (y < x) == less ? y : x; };
+    for (unsigned k = 2; k <= size; k <<= 1) {
+      const bool up = (e & k) == 0;
+      unsigned j = k >> 1;
+      for (; j >= 64; j >>= 1) {
+        if (works) sh.key[e] = a, sh.key[e + 1] = b;
+        __syncthreads();
+        if (works) {
+          const bool less = ((e & j) == 0) == up;
+          keep(a, sh.key[e ^ j], less);
+          keep(b, sh.key[(e + 1) ^ j], less);
         }
-        if (j > 32 || (j == 1 && k >= 64))
-          __syncthreads();
-        else
-          __syncwarp();
+        __syncthreads();
       }
+      if (!works) continue;
+      for (; j >= 2; j >>= 1) {
+        const bool less = ((e & j) == 0) == up;
+        keep(a, __shfl_xor_sync(0xffffffffu, a, j >> 1), less);
+        keep(b, __shfl_xor_sync(0xffffffffu, b, j >> 1), less);
+      }
+      if ((a > b) == up) {
+        const Key t = a;
+        a = b, b = t;
+      }
+    }
+    if (works) sh.key[e] = a, sh.key[e + 1] = b;
     __syncthreads();
   }
 
@@ -428,6 +487,28 @@ struct Row {
     return true;
   }
 
+  // Of the n logits in sh.key, in order, behind others that weigh `base`: the first where
+  // the sum reaches the target; n, if none.
+  __device__ unsigned reach(unsigned n, double base, double target) {
+    double c[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const unsigned e = kPer * threadIdx.x + i;
+      c[i] = e < n ? weight(from_falling((uint32_t)(sh.key[e] >> 32))) : 0.0;
+    }
+    if (threadIdx.x == 0) sh.found = (int)n;
+    scan(c);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (kPer * threadIdx.x + i < n && base + c[i] >= target) {
+        atomicMin(&sh.found, (int)(kPer * threadIdx.x) + i);
+        break;
+      }
+    __syncthreads();
+    return (unsigned)sh.found;
+  }
+
+  static constexpr int kMissed = -7;  // as a cut's number: there is none
   // CTA 0's choice becomes every CTA's cut.
   __device__ void publish(bool chooses, Cut c) {
     if (rank == 0 && chooses)
@@ -506,11 +587,49 @@ struct Row {
           find(target - base, guess);
           b = sh.found;
         }
+        // (what comes before some bins around it is added up, and these are listed, in one pass;
+        // mostly the sum is reached in the list)
+        if (sh.hist[b] <= kList) {
+          int w0 = b, w1 = b;
+          unsigned many = sh.hist[b];
+          for (int more = 0; more < kWindow / 2; ++more) {
+            if (w1 + 1 < kBins && many + sh.hist[w1 + 1] <= kList) many += sh.hist[++w1];
+            if (w0 > 0 && many + sh.hist[w0 - 1] <= kList) many += sh.hist[--w0];
+          }
+          double a = 0, none = 0;
+          collect([&](float v, int i) {
+            const int k = bin(v, i);
+            if (k >= 0 && k < w0) a += weight(v);
+            return k >= w0 && k <= w1;
+          });
+          reduce<false>(a, none);
+          if (rank == 0) {
+            const unsigned listed = min(sh.listed, (unsigned)kList);
+            sort(listed);
+            unsigned at = listed ? reach(listed, base + a, target) : 0u;
+            const bool ends = w1 == kBins - 1 && listed;  // (sums in another order may fall short by a rounding)
+            if (at == listed && ends) at = listed - 1;
+            Cut c{0.f, kMissed};
+            if (at < listed && (w0 == 0 || base + a < target)) {
+              const unsigned long long k = sh.key[at];
+              c = Cut{from_falling((uint32_t)(k >> 32)), (int)(uint32_t)k};
+            }
+            const Cut before = cut;
+            publish(threadIdx.x == 0, c);
+            if (c.i != kMissed) return;
+            cut = before;
+          } else {
+            const Cut before = cut;
+            publish(false, Cut{});
+            if (cut.i != kMissed) return;
+            cut = before;
+          }
+        }
         int from = 0, to = kBins - 1;  // the bin is one of these
         for (;;) {
           const int w0 = max(from, min(b - kWindow / 2, to + 1 - kWindow));
           __syncthreads();
-          if (threadIdx.x < kWindow) sh.window[threadIdx.x] = 0;
+          sh.window.clear();
           __syncthreads();
           double a = 0, none = 0;
           each([&](float v, int i) {
@@ -520,12 +639,12 @@ struct Row {
             if (k < 0)
               a += w;
             else
-              atomicAdd(&sh.window[k], __double2ull_rn(w * 0x1p44));  // (whole numbers: the order does not matter)
+              sh.window.add(k, w);
           });
           reduce<false>(a, none);  // (and the windows are complete)
           if (threadIdx.x < kWindow) {
             unsigned long long u = 0;
-            for (int r = 0; r < ranks; ++r) u += *at(&sh.window[threadIdx.x], r);
+            for (int r = 0; r < ranks; ++r) u += at(&sh.window, r)->sum(threadIdx.x);
             sh.mass[threadIdx.x] = (double)u * 0x1p-44;
           }
           __syncthreads();
@@ -565,22 +684,7 @@ struct Row {
           if (COUNT) {
             at = (unsigned)(target - base) - 1;
           } else {
-            double c[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const unsigned e = kPer * threadIdx.x + i;
-              c[i] = e < listed ? weight(from_falling((uint32_t)(sh.key[e] >> 32))) : 0.0;
-            }
-            if (threadIdx.x == 0) sh.found = (int)listed - 1;
-            scan(c);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-              if (kPer * threadIdx.x + i < listed && base + c[i] >= target) {
-                atomicMin(&sh.found, (int)(kPer * threadIdx.x) + i);
-                break;
-              }
-            __syncthreads();
-            at = (unsigned)sh.found;
+            at = reach(listed, base, target);
           }
           const unsigned long long k = sh.key[min(at, listed - 1)];
           publish(threadIdx.x == 0, Cut{from_falling((uint32_t)(k >> 32)), (int)(uint32_t)k});
@@ -602,7 +706,8 @@ struct Row {
 
   // The row's token.  x, n, first, ranks and rank are set, sh.powers filled, high the
   // largest logit and low the smallest above -inf negated, of the whole row.
-  __device__ void run(const Sample &a, long long r, double high, double low) {
+  // mine: the largest that this thread has seen, of logits that no other one has seen.
+  __device__ void run(const Sample &a, long long r, double high, double low, float mine) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     top = (float)high;
     const bool writes = rank == 0 && threadIdx.x == 0;
@@ -631,16 +736,53 @@ struct Row {
     // logits below this have no weight
     const float least = high == INFINITY ? top : (float)fmax(-low, high - kFar * (double)want.t);
     double mass = 0, none = 0;
-    if (want.p < 1.f && !want.k) {
-      each([&](float v, int) { mass += v > -INFINITY ? weight(v) : 0.0; });
-      reduce<false>(mass, none);
-    }
     bool counted = false;
     int guess = -1;
+    if (want.p < 1.f && !want.k) {
+      if (least < top) {  // (with the count that follows)
+        const Bins bins(top, least);
+        count([&](float v, int) {
+          const int b = bins(v);
+          if (b >= 0) mass += weight(v);
+          return b;
+        });
+        counted = true;
+      } else {
+        each([&](float v, int) { mass += v > -INFINITY ? weight(v) : 0.0; });
+      }
+      reduce<false>(mass, none);
+    }
     if ((want.p < 1.f || want.k) && want.k <= kList && least < top) {
       // what is kept, if it is not much, goes through one list
       const Bins bins(top, least);
-      count([&](float v, int) { return bins(v); });
+      // At least k logits are no smaller than the k-th of the threads' largest, and of n
+      // threads' mostly no more than n log(1 / (1 - k / n)).  That k-th is found with one
+      // count a thread (a row of 131072, k = 50: 46000 clocks in all, against 53000 or more
+      // with a count of every logit).
+      const float threads = (float)(ranks * kThreads);
+      if (want.k && want.k < threads && -threads * log1pf(-want.k / threads) < 0.85f * kList) {
+        clear();
+        const int own = bins(mine);
+        if (own >= 0) atomicAdd(&sh.hist[own], 1u);
+        merge();
+        find((double)want.k, [&](int b) { return (double)sh.hist[b]; });
+        const int b = sh.found;
+        const bool there = sh.before + sh.in_bin >= (unsigned)want.k;
+        __syncthreads();
+        if (there) {
+          collect([&](float v, int) { return (unsigned)bins(v) <= (unsigned)b; });
+          const unsigned n = *at(&sh.listed, 0);
+          sync();  // (all have read it)
+          if (n <= kList) {
+            if (rank == 0) {
+              sort(n);
+              finish(n, want, mass, a, r);
+            }
+            return;
+          }
+        }
+      }
+      if (want.k) count([&](float v, int) { return bins(v); });
       counted = true;
       if (want.k)
         find((double)want.k, [&](int b) { return (double)sh.hist[b]; });
@@ -681,16 +823,16 @@ struct Row {
     };
     const int piece = (a.slice + 128 * kWarps - 1) / (128 * kWarps) * 128;
     const int j0 = min(warp * piece, n), j1 = min(j0 + piece, n);
-    double mine = 0;
+    double weighs = 0;
     for (int j = j0 + 4 * lane; j < j1; j += 128) {
       float v[4];
       load4(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine += kept(v[i], first + j + i);
+      for (int i = 0; i < 4; ++i) weighs += kept(v[i], first + j + i);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sh.seg[warp] = mine;
+    for (int o = 16; o; o >>= 1) weighs += __shfl_xor_sync(0xffffffffu, weighs, o);
+    if (lane == 0) sh.seg[warp] = weighs;
     __syncthreads();
     mass = threadIdx.x < kWarps ? sh.seg[threadIdx.x] : 0.0;
     reduce<false>(mass, none);
@@ -811,7 +953,7 @@ __global__ void __launch_bounds__(kClusterThreads, 2) sample_k(const __grid_cons
   if (a.resident) row.x = slice, row.vec = true;
   double h = high, l = low;
   row.template reduce<true>(h, l);  // (and the slice is in place)
-  row.run(a, r, h, l);
+  row.run(a, r, h, l, high);
 }
 
 // ---------------------------------------------------------------- by counting values
@@ -833,7 +975,7 @@ struct CountShared {
   double sum[kGroups];
   unsigned cnt[kGroups];
   double powers[kPowers];
-  unsigned long long window[kWindow];
+  Window window;
   double red[kCountWarps];
   unsigned redc[kCountWarps];
   unsigned bin, before;
@@ -1289,7 +1431,7 @@ struct Counter {
     for (;;) {
       const uint32_t from = min(max(b > kWindow / 2 ? b - kWindow / 2 : 0u, lo), max(lo, hi + 1 > kWindow ? hi + 1 - kWindow : 0u));
       __syncthreads();
-      if (threadIdx.x < kWindow) sh.window[threadIdx.x] = 0;
+      sh.window.clear();
       __syncthreads();
       double below = 0, above = 0;
       each([&](const uint32_t(&k)[kEach]) {
@@ -1303,7 +1445,7 @@ struct Counter {
             else if (at >= kWindow)
               above += w;
             else
-              atomicAdd(&sh.window[at], __double2ull_rn(w * 0x1p44));  // (whole numbers: the order does not matter)
+              sh.window.add(at, w);
           }
       });
       below = total(below);
@@ -1311,7 +1453,7 @@ struct Counter {
       double in[kWindow], all = below + above + room * wc;
       if (!(cut < kDead - 1)) all = below + above;
 #pragma unroll
-      for (int i = 0; i < kWindow; ++i) in[i] = (double)sh.window[i] * 0x1p-44, all += in[i];
+      for (int i = 0; i < kWindow; ++i) in[i] = (double)sh.window.sum(i) * 0x1p-44, all += in[i];
       const uint32_t at = (cut >> 16) - from;
       target = fmax((double)want.p * all, kLeast);
       if (target <= below && from > lo) {  // (the next guess begins at the window's edge, where the sum is known)
@@ -1634,8 +1776,9 @@ __global__ void __launch_bounds__(kCountThreads, 1) sample_count_k(const __grid_
   row.each([&](float v, int) {
     if (v > -INFINITY) high = fmax(high, (double)v), low = fmax(low, -(double)v);
   });
+  const float mine = (float)high;
   row.template reduce<true>(high, low);
-  row.run(a, r, high, low);
+  row.run(a, r, high, low, mine);
 }
 
 template <class T>
