@@ -1796,9 +1796,9 @@ template <class T>
 cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
   // A CTA a row is enough where there are many.  Us in a cluster / by counting, rows of
-  // 131072, with top p / with top k, top p and min p: 16-bit logits, 16 rows 82/68 and
-  // 66/45, 64 rows 154/68 and 123/47; 32 bits, 64 rows 153/156 and 87/170, 148 rows
-  // 285/160 and 164/156.  (One row of 32003: 21/23 and 21/23.)
+  // 131072, with top p / with top k, top p and min p: 16-bit logits, 1 row 25/43 and 25/43,
+  // 16 rows 84/73 and 51/55, 64 rows 166/74 and 138/55; 32 bits, 64 rows 155/154 and 98/168,
+  // 148 rows 250/159 and 137/156.
   if (a.rows >= (sizeof(T) == 2 ? 24 : 100)) return launch_count<T>(a, st);
   Sample s = a;
   const long long bytes = (long long)a.vocab * sizeof(T);
