@@ -313,3 +313,73 @@ def test_refusals(ops):
         ops.attend_shared(**{**a, "max_new": 0}, stream=stream())
     empty = c.q[:0]
     ops.attend_shared(**{**a, "q": empty, "out": empty, "offsets": ints([0, 0, 0, 0])}, stream=stream())
+
+
+def widened(c):
+    """The same pages in a table with so many columns that the beginning is worth a pass of its own."""
+    columns = (48 << 20) // (c.batch * c.page * c.heads * 2 * c.dim) + 2
+    return ints(np.pad(c.table, ((0, 0), (0, max(0, columns - c.table.shape[1]))), constant_values=-1))
+
+
+@pytest.mark.parametrize("dtype,dim,heads,group,page", [("f16", 128, 2, 4, 16), ("bf16", 64, 3, 1, 32), ("f16", 64, 1, 17, 48), ("bf16", 128, 1, 7, 16)])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_two_passes(ops, form, dtype, dim, heads, group, page):
+    c = Case(FORMS[form], heads, group, dim, page, dtype, seed=form)
+    c.check(ops, pages=widened(c))
+
+
+@pytest.mark.parametrize("groups", [[(5, [(7, 1)] * 4)] * 40, [(20, [(3 * i, 1 + i % 3) for i in range(130)])], [(6, [(0, 1)] * 200), (8, [(700, 1)])],
+                                    [(3, [(5, 1)] * 129), (40, [(900, 2)] * 3)]])
+def test_many_sequences_in_two_passes(ops, groups):
+    c = Case(groups, 2, 4, 128, 16, "bf16", seed=len(groups))
+    c.check(ops, pages=widened(c))
+
+
+@pytest.mark.parametrize("groups", [[(40, [(3 * i, 1) for i in range(12)])], [(30, [(20, 2)] * 40), (9, [(1, 1)] * 5)], [(25, [(10, 70)] * 3)]])
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_that_follow_at_once(ops, groups, captured):
+    """Queries, lengths, tables, codes and scales that change right before each call, and outputs read right after it."""
+    c = Case(groups, 2, 4, 128, 64, "f16", seed=7)
+    wide, steps = widened(c), 10
+    a = c.args(pages=wide.clone())
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = [torch.randn(c.q.shape, generator=g, device="cuda").half() for _ in range(steps)]
+    new = [[t[torch.randperm(t.shape[0], generator=g, device="cuda")] for t in c.cache_t] for _ in range(steps)]
+    tables = [wide.roll(0) if i % 2 else torch.where(wide >= 0, wide.max() - wide, wide) for i in range(steps)]
+    lens0, lens = ints(c.lens), a["lens"]
+
+    def run(st, wait):
+        outs = []
+        lens.copy_(lens0)
+        for i in range(steps):
+            c.q.copy_(q[i])
+            for t, u in zip(c.cache_t, new[i]):
+                t.copy_(u)
+            a["pages"].copy_(tables[i])
+            lens.add_(1)
+            if wait:
+                torch.cuda.synchronize()
+            ops.attend_shared(**a, stream=st)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(c.out.clone())
+            c.out.fill_(math.nan)
+        return torch.stack(outs)
+
+    want = run(stream(), True)
+    assert torch.isfinite(want).all()
+    if captured:
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        ops.reserve(side.cuda_stream)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            got = run(side.cuda_stream, False)
+        for _ in range(20):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        ops.release(side.cuda_stream)
+    else:
+        for _ in range(20):
+            assert torch.equal(run(stream(), False), want)
+    ops.synchronize(stream())
