@@ -100,7 +100,7 @@ static_assert(kSampleMaxVocab < 1 << 19, "pieces of a sum");
 
 struct SampleShared {
   double powers[kPowers];
-  unsigned hist[kBins];
+  alignas(16) unsigned hist[kBins];
   unsigned long long key[kList];  // (order of x, number), rising
   double mass[kList], wt[kList];  // running sums, weights
   double part[2][kMaxRanks][2];   // what CTAs tell one another, two exchanges in turn
@@ -255,16 +255,24 @@ struct Row {
       return;
     }
     sync();
-    unsigned sum[kBins / kThreads];
+    // A CTA adds up its part of the bins, and gives it to all (all parts in every CTA: 64 rows
+    // of 131072 78 us, 75 so).
+    static_assert(kBins % (4 * kMaxRanks) == 0 && kBins / 8 <= kClusterThreads, "bins");
+    const int part = kBins / 4 / ranks;  // (fours)
+    uint4 sum = make_uint4(0, 0, 0, 0);
+    const int four = rank * part + (int)threadIdx.x;
+    const bool mine = (int)threadIdx.x < part;
+    if (mine) {
+      uint4 u[kMaxRanks];
 #pragma unroll
-    for (int k = 0; k < kBins / kThreads; ++k) {
-      sum[k] = 0;
-      for (int r = 0; r < ranks; ++r) sum[k] += at(sh.hist, r)[threadIdx.x + k * kThreads];
+      for (int r = 0; r < kMaxRanks; ++r) u[r] = r < ranks ? reinterpret_cast<const uint4 *>(at(sh.hist, r))[four] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kMaxRanks; ++r) sum.x += u[r].x, sum.y += u[r].y, sum.z += u[r].z, sum.w += u[r].w;
     }
     sync();
-#pragma unroll
-    for (int k = 0; k < kBins / kThreads; ++k) sh.hist[threadIdx.x + k * kThreads] = sum[k];
-    __syncthreads();
+    if (mine)
+      for (int r = 0; r < ranks; ++r) reinterpret_cast<uint4 *>(at(sh.hist, r))[four] = sum;
+    sync();
   }
 
   // The first bin where value(b) summed up to it reaches `target` (the last one, if none), into sh.found; counts before it into sh.before.
