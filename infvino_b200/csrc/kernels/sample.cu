@@ -275,9 +275,11 @@ struct Row {
     sync();
   }
 
-  // The first bin where value(b) summed up to it reaches `target` (the last one, if none), into sh.found; counts before it into sh.before.
+  // The first bin where value(b) summed up to it reaches `target` (the last one, if none),
+  // into sh.found; counts before it into sh.before.  With `more`, the target is higher by
+  // what all values are beyond that.
   template <class F>
-  __device__ void find(double target, F &&value) {
+  __device__ void find(double target, F &&value, double more = -1) {
     constexpr int kEach = kBins / kThreads;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     double v[kEach], mine = 0;
@@ -299,9 +301,13 @@ struct Row {
     if (lane == 31) sh.red[0][warp] = incl, sh.cnt[warp] = ci;
     if (threadIdx.x == 0) sh.found = kBins - 1;
     __syncthreads();
-    double before = 0;
+    double before = 0, all = 0;
     unsigned cb = 0;
-    for (int w = 0; w < warp; ++w) before += sh.red[0][w], cb += sh.cnt[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.red[0][w], cb += sh.cnt[w];
+      all += sh.red[0][w];
+    }
+    if (more >= 0) target += all - more;
     before += incl - mine;
     cb += ci - c;
 #pragma unroll
@@ -794,8 +800,8 @@ struct Row {
       counted = true;
       if (want.k)
         find((double)want.k, [&](int b) { return (double)sh.hist[b]; });
-      else
-        find((double)want.p * mass, [&](int b) { return sh.hist[b] ? sh.hist[b] * weight(bins.middle(b)) : 0.0; });
+      else  // by the bins' middles: that their sum is not the logits' comes from the first bins above all, before the cut
+        find((double)want.p * mass, [&](int b) { return sh.hist[b] ? sh.hist[b] * weight(bins.middle(b)) : 0.0; }, mass);
       int b = sh.found;
       unsigned many = sh.before + sh.in_bin;
       if (!want.k) {  // (the bins' middles are a guess: two more)
