@@ -1811,9 +1811,9 @@ cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
   // A CTA a row is enough where there are many.  Us in a cluster / by counting, rows of
   // 131072, with top p / with top k, top p and min p: 16-bit logits, 1 row 25/43 and 25/43,
-  // 16 rows 84/73 and 51/55, 64 rows 166/74 and 138/55; 32 bits, 64 rows 155/154 and 98/168,
-  // 148 rows 250/159 and 137/156.
-  if (a.rows >= (sizeof(T) == 2 ? 24 : 100)) return launch_count<T>(a, st);
+  // 32 rows 66/72 and 61/54, 48 rows 113/73 and 84/55; 32 bits, 16 rows 59/190 and 53/131,
+  // 100 rows 175/156 and 100/190, 148 rows 234/158 and 132/154.
+  if (a.rows >= (sizeof(T) == 2 ? 40 : 148)) return launch_count<T>(a, st);
   Sample s = a;
   const long long bytes = (long long)a.vocab * sizeof(T);
   s.ranks = 1;

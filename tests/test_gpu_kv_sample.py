@@ -257,7 +257,7 @@ def test_refusals(ops):
         ops.sample(torch.empty((1, 500001), dtype=torch.float16, device="cuda"), u[:1], t[:1], stream=stream())
 
 
-@pytest.mark.parametrize("rows", [2, 120])
+@pytest.mark.parametrize("rows", [2, 120, 150])
 def test_extreme_temperatures(ops, rows):
     """Logits and temperatures whose difference or quotient does not fit into 32 bits."""
     g = torch.Generator(device="cuda").manual_seed(rows)
@@ -270,3 +270,58 @@ def test_extreme_temperatures(ops, rows):
     z = (x * 1.2e5 - 6e4).to(torch.float16)
     check(ops, z, u, temperature=[3e4] * rows, top_p=[0.7] * rows)
     check(ops, ((x * 6 - 3) * 1e38).to(torch.bfloat16), u, temperature=[1e38] * rows, top_p=[0.7] * rows)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_masked_and_not_finite_in_many_rows(ops, dtype):
+    vocab, times = 5003, 17
+    x = logits(9, vocab, dtype, 3)
+    x[0] = -INF
+    x[1] = -INF
+    x[1, 4999] = -3.0
+    x[2, ::2] = -INF
+    x[3] = torch.finfo(x.dtype).min
+    x[3, 100:110] = 1.0
+    x[4, 17] = NAN
+    x[4, 5:9] = -NAN
+    x[5] = NAN
+    x[6, [30, 4000]] = INF
+    x[7] = INF
+    x[8] = torch.finfo(x.dtype).min
+    x, rows = x.repeat(times, 1), 9 * times
+    u = uniform(rows, 1)
+    got = check(ops, x, u)
+    assert got[::9] == [-1] * times and got[1::9] == [4999] * times and got[5::9] == [-1] * times
+    check(ops, x, u, top_k=[20] * rows, top_p=[0.8] * rows, min_p=[0.01] * rows)
+    check(ops, x, u, top_k=[3000] * rows, top_p=[0.99] * rows)
+    check(ops, x, u, temperature=[0.0, INF, NAN] * (rows // 3), top_p=[NAN] * rows, min_p=[NAN] * rows)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [40, 70000])
+def test_ties_in_many_rows(ops, dtype, vocab):
+    """Few distinct logits, some more than 65535 times in a row."""
+    times = 25
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randint(-2, 3, (6, vocab), generator=g, device="cuda").to(TYPES[dtype])
+    x[1] = 1.5
+    x[2] = -0.0
+    x[2, ::2] = 0.0
+    x[3, 1:] = NAN
+    x[4, 2:] = -0.0
+    x, rows = x.repeat(times, 1), 6 * times
+    r, u = np.random.default_rng(1), uniform(rows, 5)
+    check(ops, x, u)
+    check(ops, x, u, top_k=r.integers(1, vocab, rows))
+    check(ops, x, u, temperature=r.random(rows) + 0.5, top_k=r.integers(1, vocab, rows), top_p=r.random(rows), min_p=r.random(rows) * 0.5)
+    check(ops, x, u, top_p=r.random(rows))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("spread", [0.05, 2.0, 5.0])
+def test_cuts_far_down(ops, dtype, spread):
+    """Cuts behind thousands of tokens, whose bins are guessed."""
+    x, u = logits(10, 150001, dtype, 21, spread), uniform(10, 21)
+    p = [0.3, 0.6, 0.9, 0.97, 0.99, 0.999, 0.9999, 0.99999, 1 - 2.0 ** -23, 0.5]
+    check(ops, x, u, top_p=p)
+    check(ops, x, u, top_p=p, temperature=[1.3] * 10, top_k=[100000, 800, 900, 1024, 1025, 5000, 0, 0, 0, 0])
