@@ -919,6 +919,9 @@ __global__ void __launch_bounds__(kClusterThreads, 2) sample_k(const __grid_cons
   const long long r = blockIdx.x / a.ranks;
   row.first = min(row.rank * a.slice, a.vocab);
   row.n = min(a.slice, a.vocab - row.first);
+  // (a CTA's shared memory is there for others once it runs: the wait for that is below,
+  // before the first exchange, so that it passes under the loads)
+  if (a.ranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   fill_powers(sh.powers);
   pdl_wait_and_release();
   const T *x = static_cast<const T *>(a.x) + r * a.stride + row.first;
@@ -966,6 +969,7 @@ __global__ void __launch_bounds__(kClusterThreads, 2) sample_k(const __grid_cons
   }
   if (a.resident) row.x = slice, row.vec = true;
   double h = high, l = low;
+  if (a.ranks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   row.template reduce<true>(h, l);  // (and the slice is in place)
   row.run(a, r, h, l, high);
 }

@@ -325,3 +325,23 @@ def test_cuts_far_down(ops, dtype, spread):
     p = [0.3, 0.6, 0.9, 0.97, 0.99, 0.999, 0.9999, 0.99999, 1 - 2.0 ** -23, 0.5]
     check(ops, x, u, top_p=p)
     check(ops, x, u, top_p=p, temperature=[1.3] * 10, top_k=[100000, 800, 900, 1024, 1025, 5000, 0, 0, 0, 0])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_rows_of_clusters_that_follow_at_once(ops, dtype):
+    """Rows of eight CTAs, small ones: launches of several streams, one behind the other, whose CTAs begin while others end."""
+    shapes = [(18, 16500), (3, 33000), (1, 20011), (30, 17001)]
+    x = [logits(*s, dtype, i) for i, s in enumerate(shapes)]
+    u = [torch.tensor(uniform(r, i), device="cuda") for i, (r, _) in enumerate(shapes)]
+    p = [torch.full((r,), 0.9, device="cuda") for r, _ in shapes]
+    side = [torch.cuda.Stream() for _ in range(3)]
+    out = [[torch.full((100, r), -7, dtype=torch.int32, device="cuda") for r, _ in shapes] for _ in side]
+    torch.cuda.synchronize()
+    for n in range(100):
+        for st, o in zip(side, out):
+            for i in range(len(shapes)):
+                ops.sample(x[i], u[i], o[i][n], top_p=p[i], stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for i, (rows, _) in enumerate(shapes):
+        want = torch.tensor(check(ops, x[i], u[i].cpu().numpy(), top_p=[0.9] * rows), dtype=torch.int32, device="cuda")
+        assert all((o[i] == want).all() for o in out)
