@@ -143,6 +143,7 @@ struct Want {
   // Logits below this weigh less than min_p, by more than any rounding.
   __device__ __forceinline__ float floor(float top) const {
     if (!(min_p > 0.f) || !(t > 0.f)) return -INFINITY;
+    if (top == INFINITY) return top;  // (the others weigh nothing)
     const double x = (double)top + (fmin(log((double)min_p), 0.0) - 1e-6) * (double)t;
     return (float)(x - 2e-7 * fabs(x));
   }
@@ -1588,7 +1589,7 @@ struct Counter {
           auto weigh = [&](float v) {
             if (!(v > last)) {
               equal += v == last;
-            } else if (!bounded || v >= lowest) {
+            } else if (!(v < lowest)) {
               const double w = weight(v);
               s += !bounded || want.enough(w, v == top) ? w : 0.0;
             }

@@ -345,3 +345,21 @@ def test_rows_of_clusters_that_follow_at_once(ops, dtype):
     for i, (rows, _) in enumerate(shapes):
         want = torch.tensor(check(ops, x[i], u[i].cpu().numpy(), top_p=[0.9] * rows), dtype=torch.int32, device="cuda")
         assert all((o[i] == want).all() for o in out)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [3, 153])
+def test_infinite_logits_under_min_p(ops, dtype, rows):
+    """Where logits are +inf only these have a weight, whatever min_p and the cut are."""
+    x, u, every = logits(rows, 5003, dtype, 4), uniform(rows, 4), np.arange(rows)
+    x[::3, [30, 4000]] = INF
+    x[1::3, 2500:] = INF
+    x[2::9, 1] = INF
+    x[5::9] = -INF
+    x[5::9, 4999] = INF
+    for f in (dict(), dict(top_k=[3000] * rows), dict(top_k=[1] * rows), dict(top_p=[0.99] * rows), dict(temperature=[0.5] * rows), dict(temperature=[INF] * rows),
+              dict(top_k=[3000] * rows, top_p=[0.9] * rows)):
+        for least in (0.01, 1.0):
+            got = np.array(check(ops, x, u, min_p=[least] * rows, **f))
+            assert np.isin(got[every % 3 == 0], [30, 4000]).all() and (got[every % 3 == 1] >= 2500).all()
+            assert (got[2::9] == 1).all() and (got[5::9] == 4999).all()
