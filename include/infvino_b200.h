@@ -426,7 +426,7 @@ typedef struct ivc_mx4 {
  * first `rows` rows: e - 127 is the exponent of a block's largest magnitude less 2
  * (at least -127), and codes are x 2^(127 - e), rounded to the nearest, ties to
  * even, at most 6.  NaN is held as 0, an infinity as the largest code of its sign;
- * neither takes part in e. */
+ * neither takes part in e.  The matrix's rows behind these stay as they are. */
 int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *m,
                         void *stream);
 /* out = the values of m's first `rows` rows, rounded once (out_stride elements apart). */

@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quantize_k(const uint16_t *
       word = (uint32_t)e << (8 * ((lane >> 2) & 3));
       word |= __shfl_xor_sync(0xffffffffu, word, 4);
       word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      if ((lane & 15) == 0 && c0 + 256 * q < chunks * 128) *reinterpret_cast<uint32_t *>(scales + 1024 * q) = word;
+      // (0 where there is no row; the matrix's rows behind the call's keep theirs)
+      if ((lane & 15) == 0 && (r < rows || r >= m.rows) && c0 + 256 * q < chunks * 128) *reinterpret_cast<uint32_t *>(scales + 1024 * q) = word;
     }
   }
 }

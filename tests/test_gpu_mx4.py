@@ -332,3 +332,23 @@ def test_shared_memory_is_refused(ops):
     ops.mx4_linear(xq, w, out.clone(), stream=stream())  # (what is only read may be shared)
     ops.synchronize(stream())
     assert (out == 64).all()
+
+
+@pytest.mark.parametrize("rows,more", [(1, 0), (40, 60), (100, 127), (130, 200), (128, 128), (7, 121)])
+@pytest.mark.parametrize("width", [96, 4096])
+def test_quantize_leaves_the_rows_behind_alone(ops, rows, more, width):
+    """The first rows of a matrix that holds others: codes and scales of those stay, scale bytes without a row are 0."""
+    whole, x = inputs(rows + more, width, "f16", 5), inputs(rows, width, "bf16", 6)
+    c, s = empty(rows + more, width)
+    m = ivb.Mx4(c, s)
+    ops.mx4_quantize(whole, m, stream=stream())
+    ops.mx4_quantize(x, m, stream=stream())
+    (codes, e), (first, f) = quantized(whole), quantized(x)
+    codes[:rows], e[:rows] = first, f
+    assert torch.equal(c.cpu(), packed(codes)) and torch.equal(s.cpu(), spread(e))
+    c, s = empty(rows + more, width)
+    ops.mx4_quantize(x, ivb.Mx4(c, s), stream=stream())
+    want = spread(torch.cat([torch.nn.functional.pad(f, (0, -(width // 32) % 4)), torch.full((more, -(-width // 128) * 4), 0xAA)]))
+    touched = (rows + 127) // 128  # (128-row pieces that no row of the call is in are not looked at)
+    assert torch.equal(s[:touched].cpu(), want[:touched]) and (s[touched:] == 0xAA).all()
+    assert torch.equal(c[:rows].cpu(), packed(first)) and (c[rows:] == 0xAA).all()
