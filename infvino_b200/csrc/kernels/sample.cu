@@ -76,24 +76,28 @@ struct Cut {  // kept: x > this one's, or x equal and number at most this one's
   int i;
 };
 
-// Weights summed up in kWindow bins as whole numbers of 2^-44, so that their order does not
-// matter: in four pieces of 12 bits (a row has less than 2^19 tokens), since shared memory
-// adds 32 bits at once, and 64 by trying until nobody interferes.
+// Weights summed up in kWindow bins as whole numbers of 2^-63, so that their order does not
+// matter: in six pieces of 11 bits (a row has less than 2^19 tokens), since shared memory
+// adds 32 bits at once, and 64 by trying until nobody interferes.  A sum is off by 2^-45 at
+// most.  top_p, in 32 bits, leaves 2^-24 of the weight or more behind a cut, so that where
+// one lies tokens weigh 2^-43 and more.  (With numbers of 2^-44 a cut at the end of 60000
+// equal tokens of e^-20 came out past it.)
 struct Window {
-  unsigned piece[4][kWindow];
+  static constexpr int kPieces = 6, kBits = 11;
+  unsigned piece[kPieces][kWindow];
   __device__ __forceinline__ void clear() {
-    if (threadIdx.x < 4 * kWindow) (&piece[0][0])[threadIdx.x] = 0;
+    if (threadIdx.x < kPieces * kWindow) (&piece[0][0])[threadIdx.x] = 0;
   }
   __device__ __forceinline__ void add(unsigned k, double w) {
-    const unsigned long long f = __double2ull_rn(w * 0x1p44);
+    const unsigned long long f = __double2ull_rn(w * 0x1p63);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) atomicAdd(&piece[q][k], (unsigned)(f >> (12 * q)) & 0xfffu);
+    for (int q = 0; q < kPieces; ++q) atomicAdd(&piece[q][k], (unsigned)(f >> (kBits * q)) & ((1u << kBits) - 1u));
   }
-  __device__ __forceinline__ unsigned long long sum(unsigned k) const {
-    unsigned long long f = 0;
+  __device__ __forceinline__ double sum(unsigned k) const {
+    double f = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) f += (unsigned long long)piece[q][k] << (12 * q);
-    return f;
+    for (int q = 0; q < kPieces; ++q) f = f * 0x1p-11 + (double)piece[q][k];
+    return f * 0x1p-8;  // (the last piece counts 2^55)
   }
 };
 static_assert(kSampleMaxVocab < 1 << 19, "pieces of a sum");
@@ -658,9 +662,9 @@ struct Row {
           });
           reduce<false>(a, none);  // (and the windows are complete)
           if (threadIdx.x < kWindow) {
-            unsigned long long u = 0;
+            double u = 0;
             for (int r = 0; r < ranks; ++r) u += at(&sh.window, r)->sum(threadIdx.x);
-            sh.mass[threadIdx.x] = (double)u * 0x1p-44;
+            sh.mass[threadIdx.x] = u;
           }
           __syncthreads();
           double sum = base + a;
@@ -689,9 +693,15 @@ struct Row {
           }
         }
       }
+      // (a sum in another order may be short of what one before it has shown, or above it, by a
+      // rounding: of no tokens then, and what comes before them is kept whole)
+      if (!COUNT && sh.hist[b] == 0) {
+        while (b > 0 && sh.hist[b] == 0) --b;
+        target = INFINITY;
+      }
       const unsigned in_bin = sh.hist[b];
       __syncthreads();
-      if (in_bin == 0) return;  // (sums in another order fell short by a rounding)
+      if (in_bin == 0) return;
       if (in_bin <= kList) {
         const unsigned listed = gather([&](float v, int i) { return bin(v, i) == b; });
         if (rank == 0) {
@@ -1402,6 +1412,9 @@ struct Counter {
     return least;
   }
 
+  // All of bin b is kept, and nothing behind it (b < 0xffff).
+  __device__ __forceinline__ void cut_behind(uint32_t b) { cut = b << 16 | 0xffffu, room = 0xffffffffu; }
+
   // The cut.  False: a counter ran over, or a guess was too far off.
   __device__ bool select(const Want &want, unsigned live, uint32_t first) {
     auto upper = [](uint32_t b) { return b << 16; };
@@ -1472,7 +1485,7 @@ struct Counter {
       double in[kWindow], all = below + above + room * wc;
       if (!(cut < kDead - 1)) all = below + above;
 #pragma unroll
-      for (int i = 0; i < kWindow; ++i) in[i] = (double)sh.window.sum(i) * 0x1p-44, all += in[i];
+      for (int i = 0; i < kWindow; ++i) in[i] = sh.window.sum(i), all += in[i];
       const uint32_t at = (cut >> 16) - from;
       target = fmax((double)want.p * all, kLeast);
       if (target <= below && from > lo) {  // (the next guess begins at the window's edge, where the sum is known)
@@ -1490,7 +1503,11 @@ struct Counter {
       }
       if (hit < 0) {
         lo = from + kWindow;
-        if (lo > min(hi, cut >> 16)) return true;  // (p is 1, but for a rounding)
+        if (lo > min(hi, cut >> 16)) {
+          // (sums in another order have shown that it is no later than hi)
+          if (hi < cut >> 16 && hi < 0xffffu) cut_behind(hi);
+          return true;
+        }
         b = locate<true>(weight_before(lo, middle) + (target - base), middle) ? sh.bin : hi;
         continue;
       }
@@ -1499,7 +1516,10 @@ struct Counter {
       if (in_bin == 0 || !count_inside(bin, in_bin)) return false;
       auto inside = [bin](uint32_t l) { return bin << 16 | l; };
       group_weights(inside);
-      if (!locate<true>(target - base, inside)) return true;
+      if (!locate<true>(target - base, inside)) {  // (short of it by a rounding)
+        if (bin < cut >> 16) cut_behind(bin);
+        return true;
+      }
       const uint32_t key = bin << 16 | sh.bin;
       if (key > cut) return true;
       const unsigned r = enough(target - base, sh.mass, weight_at(key), counter(sh.bin));

@@ -363,3 +363,61 @@ def test_infinite_logits_under_min_p(ops, dtype, rows):
             got = np.array(check(ops, x, u, min_p=[least] * rows, **f))
             assert np.isin(got[every % 3 == 0], [30, 4000]).all() and (got[every % 3 == 1] >= 2500).all()
             assert (got[2::9] == 1).all() and (got[5::9] == 4999).all()
+
+
+@pytest.mark.parametrize("rows", [30, 150])
+def test_cuts_at_the_end_of_a_long_run(ops, rows):
+    """top_p ends within the last token of 60000 equal ones, some e^-20 of the largest each, with others behind them."""
+    n, tail = 60000, 10000
+    r = np.random.default_rng(7)
+    near = np.float32(r.uniform(-20.3, -19.9, rows))
+    w, p, u = np.exp(near.astype(np.float64)), 1 - 2.0 ** -20, [1 - 2.0 ** -24] * rows
+    # p (1 + n w + tail) is what comes before the run's end but for a part of its last token
+    part = np.linspace(0.05, 0.95, rows)
+    far = np.float32(np.log(((1 + (n - part) * w) / p - 1 - n * w) / tail))
+    x = np.full((rows, 1 + n + tail), 0, np.float32)
+    x[:, 1:] = far[:, None]
+    places = 1 + r.permutation(n + tail)[:n]
+    x[:, places] = near[:, None]
+    x[:, places[0]], x[:, 0] = 0, near  # (the largest is somewhere)
+    got = check(ops, torch.tensor(x, device="cuda"), u, top_p=[p] * rows)
+    assert (x[np.arange(rows), got] >= near).all()  # (what is behind the run is not kept)
+
+
+@pytest.mark.parametrize("rows", [3, 150])
+def test_cuts_in_long_runs_of_small_weights(ops, rows):
+    """top_p ends inside 400000 equal tokens of some e^-25 each: the cut goes by sums in 64 bits."""
+    n, tail = 400000, 90000
+    near = np.float32(-25 + np.random.default_rng(3).uniform(-0.05, 0.05, rows))
+    w, v = np.exp(near.astype(np.float64)), np.exp(np.float64(np.float32(-25.3)))
+    x = torch.full((rows, 1 + n + tail), -25.3, device="cuda")
+    x[:, 0] = 0
+    x[:, 1:1 + n] = torch.tensor(near, device="cuda")[:, None]
+    p, u = 1 - 2.0 ** -18, 1 - 2.0 ** -24
+    all_ = 1 + n * w + tail * v
+    kept = np.ceil((p * all_ - 1) / w)      # of the run
+    assert ((kept > 1000) & (kept < n - 1000)).all()
+    want = np.floor((u * (1 + kept * w) - 1) / w) + 1
+    got = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    ops.sample(x, torch.full((rows,), u, device="cuda"), got, top_p=torch.full((rows,), p, device="cuda"), stream=stream())
+    # three sums (all, up to the cut, up to the token), each off by at most n 2^-53 whatever its order, weights by 2^-52 of
+    # themselves, and one token more or less for each border
+    off = (3 * x.shape[1] * 2.0 ** -53) / w + 2 * n * 2.0 ** -52 + 2
+    assert (np.abs(got.cpu().numpy() - want) <= off).all(), np.abs(got.cpu().numpy() - want).max()
+
+
+def test_cuts_in_long_runs_of_near_weights(ops):
+    """The same where eight values share the run, in rows enough that values are counted."""
+    n, tail, distinct, times, p, u = 400000, 90000, 8, 19, 1 - 2.0 ** -19, 1 - 2.0 ** -20
+    near = np.float32(-25 + np.random.default_rng(5).uniform(-0.01, 0.01, distinct))
+    x = np.full((distinct, 1 + n + tail), -26.2, np.float32)
+    x[:, 0] = 0
+    x[:, 1:1 + n] = near[:, None] - np.float32(0.125) * (np.arange(n, dtype=np.float32) % 8)
+    want = [choose(x[r].astype(np.float64), u, p=p)[0] for r in range(distinct)]
+    rows = distinct * times
+    got = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    ops.sample(torch.tensor(x, device="cuda").repeat(times, 1), torch.full((rows,), u, device="cuda"), got, top_p=torch.full((rows,), p, device="cuda"),
+               stream=stream())
+    # as above, on both sides; an eighth of the run at least is kept, so that so many tokens are at most eight times as far in numbers
+    off = 8 * (2 * (3 * x.shape[1] * 2.0 ** -53) / math.exp(-25.9) + 2 * n * 2.0 ** -52 + 2)
+    assert (np.abs(got.view(times, distinct).cpu().numpy() - np.array(want)) <= off).all(), (got[:distinct], want)
