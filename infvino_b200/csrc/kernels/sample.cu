@@ -1234,7 +1234,9 @@ struct Counter {
     for (int w = 0; w < warp; ++w) before += sh.red[w], nb += sh.redc[w];
     before += s - s0;
     nb += n - n0;
-    const int at = before + m[0] >= target ? 0 : before + m[0] + m[1] >= target ? 1 : 2;
+    // (an empty group may seem to be the first: what is before it is added up in another order
+    // than by the threads before this one)
+    const int at = c[0] && before + m[0] >= target ? 0 : c[1] && before + m[0] + m[1] >= target ? 1 : 2;
     if (at < 2) atomicMin(&sh.bin, (unsigned)(g0 + at));
     __syncthreads();
     const unsigned g = sh.bin;

@@ -421,3 +421,31 @@ def test_cuts_in_long_runs_of_near_weights(ops):
     # as above, on both sides; an eighth of the run at least is kept, so that so many tokens are at most eight times as far in numbers
     off = 8 * (2 * (3 * x.shape[1] * 2.0 ** -53) / math.exp(-25.9) + 2 * n * 2.0 ** -52 + 2)
     assert (np.abs(got.view(times, distinct).cpu().numpy() - np.array(want)) <= off).all(), (got[:distinct], want)
+
+
+@pytest.mark.parametrize("seed", [10, 14, 25])
+def test_a_cut_between_sums_in_two_orders(ops, seed):
+    """Rows whose top_p lies, in steps of half a unit in the last place, around the weight of the same 60 tokens: sums up to
+    there that are added in another order are above it or below."""
+    r = np.random.default_rng(seed)
+    head = np.sort(np.float16(r.uniform(3, 8, 60)))[::-1].astype(np.float64)
+    top, rows = head[0], 4096
+    left, tail = np.exp(head - top).sum() * (1 - 2.0 ** -42), []  # what comes behind weighs as much (p is a half)
+    for y in np.arange(2.9, -22, -0.1).astype(np.float16).astype(np.float64):
+        w = np.exp(y - top)
+        tail += [y] * int(left / w)
+        left -= int(left / w) * w
+    fine = np.float64(np.float16(top - 49 * math.log(2)))
+    one = np.concatenate([head, tail, np.full(rows, -INF)])
+    x = np.repeat(one[None].astype(np.float16), rows, 0)
+    for i in range(rows):
+        x[i, len(one) - rows:len(one) - rows + i] = fine
+    order = r.permutation(len(one))
+    x = np.ascontiguousarray(x[:, order])
+    tokens, probs = torch.full((rows,), -7, dtype=torch.int32, device="cuda"), torch.full((rows,), NAN, device="cuda")
+    u = torch.full((rows,), 0.5, device="cuda")
+    ops.sample(torch.tensor(x, device="cuda"), u, tokens, probs, top_p=u, stream=stream())
+    # (one token more or less is kept by a rounding)
+    may = [choose(x[0].astype(np.float64), 0.5, p=p)[:2] for p in (0.5 - 1e-9, 0.5 + 1e-9)]
+    for got in zip(tokens.tolist(), probs.tolist()):
+        assert any(got[0] == t and abs(got[1] - s) <= 2.0 ** -23 * s for t, s in may), (got, may)
