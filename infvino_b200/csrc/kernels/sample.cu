@@ -44,7 +44,7 @@ __device__ __forceinline__ void fill_powers(double *powers) {
   for (int j = threadIdx.x; j < kPowers; j += blockDim.x) powers[j] = exp2(j / (double)kPowers);
 }
 // e^((v - top) / T) = 2^(n / 256) 2^(r / 256), |r| at most a half: the first from the
-// table, of the second the first terms of its series (the rest is below 2^-42 of it).
+// table, of the second the first terms of its series (the rest is below 2^-54 of it).
 struct Weights {
   float top;
   // Whether a weight is 0 is asked in 32 bits: (v times - top_times) by32, where neither
@@ -66,7 +66,7 @@ struct Weights {
     constexpr double c = 0.6931471805599453 / kPowers;
     const double d = (double)v - (double)top, s = fma(d, by, kRound), r = fma(d, by, kRound - s);
     const int n = __double2loint(s);
-    const double w = fma(fma(fma(c * c * c / 6.0, r, c * c / 2.0), r, c), r, 1.0) * powers[n & (kPowers - 1)];
+    const double w = fma(fma(fma(fma(c * c * c * c / 24.0, r, c * c * c / 6.0), r, c * c / 2.0), r, c), r, 1.0) * powers[n & (kPowers - 1)];
     return __hiloint2double(__double2hiint(w) + (n >> 8) * (1 << 20), __double2loint(w));
   }
 };

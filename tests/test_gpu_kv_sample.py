@@ -449,3 +449,24 @@ def test_a_cut_between_sums_in_two_orders(ops, seed):
     may = [choose(x[0].astype(np.float64), 0.5, p=p)[:2] for p in (0.5 - 1e-9, 0.5 + 1e-9)]
     for got in zip(tokens.tolist(), probs.tolist()):
         assert any(got[0] == t and abs(got[1] - s) <= 2.0 ** -23 * s for t, s in may), (got, may)
+
+
+@pytest.mark.parametrize("rows", [100, 1000])
+def test_weights_have_the_bits_of_64(ops, rows):
+    """Rows whose largest logit weighs half of all but for 2^-48 to 2^-45: u = 0.5 is at its border."""
+    r, y = np.random.default_rng(2), np.float32(-0.37 * np.arange(3, 96))
+    small = np.exp(y.astype(np.longdouble))
+    x, first = np.full((rows, 2 + len(y)), -INF, np.float32), np.zeros(rows, bool)
+    for i in range(rows):
+        x[i, 0], x[i, 1] = 0, r.uniform(-0.6, -0.1)
+        total = 1 + np.exp(x[i, 1].astype(np.longdouble))
+        want = 2 + r.choice([-1, 1]) * r.uniform(2.0 ** -47, 2.0 ** -45)
+        for j in range(len(y)):
+            if total + small[j] < want:
+                total, x[i, 2 + j] = total + small[j], y[j]
+        # (64-bit weights and sums of them: some ten roundings of 2^-53 each)
+        assert 2.0 ** -48 < abs(total - 2) < 2.0 ** -44.9
+        first[i] = total < 2
+    got = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    ops.sample(torch.tensor(x, device="cuda"), torch.full((rows,), 0.5, device="cuda"), got, stream=stream())
+    assert (got.cpu().numpy() == np.where(first, 0, 1)).all()
