@@ -376,7 +376,8 @@ typedef struct ivc_kv_groups {
  * first shared[g] tokens are not looked at.  A group whose sequences, or whose
  * shared[g], do not fit is skipped, as is a sequence that ends inside the
  * beginning.  scratch: at least tokens * q_heads * (head_dim + 2) floats, 16-byte
- * aligned, of nobody else until the call has run. */
+ * aligned, of nobody else until the call has run (memory of q, out or the cache's
+ * codes and scales is refused). */
 int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, const ivc_kv_groups *groups,
                          int dtype, int q_heads, int max_new, const ivc_rows *q, const ivc_rows *out, float scale,
                          float *scratch, int64_t scratch_floats, void *stream);
@@ -426,16 +427,18 @@ typedef struct ivc_mx4 {
  * first `rows` rows: e - 127 is the exponent of a block's largest magnitude less 2
  * (at least -127), and codes are x 2^(127 - e), rounded to the nearest, ties to
  * even, at most 6.  NaN is held as 0, an infinity as the largest code of its sign;
- * neither takes part in e.  The matrix's rows behind these stay as they are. */
+ * neither takes part in e.  The matrix's rows behind these stay as they are.  m
+ * shares no memory with x. */
 int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *m,
                         void *stream);
-/* out = the values of m's first `rows` rows, rounded once (out_stride elements apart). */
+/* out = the values of m's first `rows` rows, rounded once (out_stride elements
+ * apart; it shares no memory with m). */
 int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *out, int64_t out_stride, void *stream);
 /* out [rows][w->rows] = X W^T, summed in f32 and rounded once: W is w; X is the
  * first `rows` rows of xq if x is NULL, else x [rows][width] (x_dtype), quantised as
  * ivc_kv_mx4_quantize does it: xq is room for that then, of nobody else until
- * the call has run, and what it holds afterwards is not defined.  out shares no
- * memory with the others.  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
+ * the call has run, and what it holds afterwards is not defined.  out, and the room
+ * for x, share no memory with the others (rows may lie between one another's).  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
 int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
                       const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream);
 

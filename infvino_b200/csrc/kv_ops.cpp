@@ -263,15 +263,55 @@ ivb::Mx4 check_mx4(const ivc_mx4 *m) {
   return ivb::Mx4{m->codes, m->scales, m->rows, m->width};
 }
 
-bool apart(const ivb::Mx4 &a, const ivb::Mx4 &b) {
-  auto disjoint = [](const uint8_t *p, int64_t n, const uint8_t *q, int64_t m) {
-    const auto x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-    return x + n <= y || y + m <= x;
-  };
-  auto codes = [](const ivb::Mx4 &m) { return m.rows * (m.width / 2); };
-  auto scales = [](const ivb::Mx4 &m) { return (m.rows + 127) / 128 * ((m.width + 127) / 128) * 512; };
-  return disjoint(a.codes, codes(a), b.codes, codes(b)) && disjoint(a.codes, codes(a), b.scales, scales(b)) &&
-         disjoint(a.scales, scales(a), b.codes, codes(b)) && disjoint(a.scales, scales(a), b.scales, scales(b));
+// Memory that a call reads or writes: n pieces of `bytes` each, `stride` bytes apart.
+struct Memory {
+  int64_t at, n, stride, bytes;
+  Memory(const void *p, int64_t count, int64_t apart, int64_t each)
+      : at((int64_t)reinterpret_cast<uintptr_t>(p)), n(each > 0 ? count : 0), stride(count > 1 ? apart : 0), bytes(each) {
+    if (stride < 0) at += stride * (n - 1), stride = -stride;
+  }
+  Memory(const void *p, int64_t all) : Memory(p, 1, 0, all) {}
+  int64_t end() const { return at + stride * (n - 1) + bytes; }
+};
+// Whether one of m's pieces has a byte of lo .. hi - 1.
+bool meets(const Memory &m, int64_t lo, int64_t hi) {
+  // the first piece that ends behind lo
+  const int64_t i = m.at + m.bytes > lo || m.stride == 0 ? 0 : (lo - m.bytes - m.at) / m.stride + 1;
+  return i < m.n && m.at + i * m.stride + m.bytes > lo && m.at + i * m.stride < hi;
+}
+// Rows that lie between one another (columns of one buffer) do not meet.
+bool meet(const Memory &a, const Memory &b) {
+  if (a.n == 0 || b.n == 0 || a.end() <= b.at || b.end() <= a.at) return false;
+  const Memory &few = a.n < b.n ? a : b, &many = a.n < b.n ? b : a;
+  if (few.stride == many.stride) {  // (as the rows of the one, seen from every row of the other)
+    Memory all = many;
+    all.at -= few.stride * (few.n - 1);
+    all.n += few.n - 1;
+    return meets(all, few.at, few.at + few.bytes);
+  }
+  for (int64_t i = 0; i < few.n; ++i)
+    if (meets(many, few.at + i * few.stride, few.at + i * few.stride + few.bytes)) return true;
+  return false;
+}
+
+Memory codes_of(const ivb::Mx4 &m) { return Memory(m.codes, m.rows * (m.width / 2)); }
+Memory scales_of(const ivb::Mx4 &m) { return Memory(m.scales, (m.rows + 127) / 128 * ((m.width + 127) / 128) * 512); }
+Memory matrix(const void *p, int64_t rows, int64_t width, int64_t stride) { return Memory(p, rows, 2 * stride, 2 * width); }
+ivb::Mx4 first_rows(ivb::Mx4 m, int64_t rows) { return m.rows = rows, m; }
+bool apart(const Memory &a, const ivb::Mx4 &m) { return !meet(a, codes_of(m)) && !meet(a, scales_of(m)); }
+bool apart(const ivb::Mx4 &a, const ivb::Mx4 &b) { return apart(codes_of(a), b) && apart(scales_of(a), b); }
+
+// Whether rows of [tokens][heads][dim] meet m.
+bool meet(const ivb::KvRows &r, int64_t tokens, int heads, int dim, const Memory &m) {
+  const Memory head(r.p, tokens, 2 * r.ts, 2 * dim);
+  const int64_t span = 2 * r.hs * (heads - 1);
+  if (head.end() + std::max<int64_t>(span, 0) <= m.at || m.end() <= head.at + std::min<int64_t>(span, 0)) return false;
+  for (int h = 0; h < heads; ++h) {
+    Memory one = head;
+    one.at += 2 * r.hs * h;
+    if (meet(one, m)) return true;
+  }
+  return false;
 }
 
 void check_matrix(int dtype, const void *p, int64_t rows, int64_t width, int64_t stride, bool written) {
@@ -507,6 +547,13 @@ int ivc_kv_attend_shared(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs
          "scratch: at least tokens * q_heads * (head_dim + 2) floats");
     need(a.seqs.tokens * a.group < (1LL << 30), "tokens * q_heads / kv_heads out of range");
     if (a.seqs.tokens == 0) return;
+    const Memory room(scratch, 4 * a.seqs.tokens * q_heads * (a.cache.dim + 2));
+    const int64_t blocks = a.cache.pages * a.cache.heads * (a.cache.page / IVC_KV_BLOCK);
+    need(!meet(a.q, a.seqs.tokens, q_heads, a.cache.dim, room) && !meet(a.out, a.seqs.tokens, q_heads, a.cache.dim, room),
+         "scratch overlaps q or out");
+    for (const void *p : {(const void *)a.cache.k, (const void *)a.cache.v})
+      need(!meet(room, Memory(p, blocks * IVC_KV_BLOCK * a.cache.dim)), "scratch overlaps the cache");
+    for (const void *p : {(const void *)a.cache.ks, (const void *)a.cache.vs}) need(!meet(room, Memory(p, 4 * blocks)), "scratch overlaps the cache");
     a.first = groups->first;
     a.shared = groups->shared;
     a.groups = groups->count;
@@ -550,6 +597,7 @@ int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64
     check_matrix(dtype, x, rows, q.width, x_stride, false);
     need(rows <= q.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0) return;
+    need(apart(matrix(x, rows, q.width, x_stride), first_rows(q, rows)), "the 4-bit matrix overlaps x");
     cuda(ivb::launch_mx4_quantize(dtype == IVC_BF16, x, rows, x_stride, q, static_cast<cudaStream_t>(stream)), "launch");
   });
 }
@@ -560,6 +608,7 @@ int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *
     check_matrix(dtype, out, rows, q.width, out_stride, true);
     need(rows <= q.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0) return;
+    need(apart(matrix(out, rows, q.width, out_stride), first_rows(q, rows)), "out overlaps the 4-bit matrix");
     cuda(ivb::launch_mx4_read(dtype == IVC_BF16, q, rows, out, out_stride, static_cast<cudaStream_t>(stream)), "launch");
   });
 }
@@ -577,8 +626,9 @@ int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64
     need(rows <= a.x.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0 || a.w.rows == 0) return;
     a.x.rows = rows;
-    need(!x || apart(a.x, a.w), "the room for x in 4 bits overlaps the weights");
-    need(x != out, "out is x");
+    const Memory input = matrix(x, x ? rows : 0, a.x.width, x_stride), output = matrix(out, rows, a.w.rows, out_stride);
+    need(!x || (apart(a.x, a.w) && apart(input, a.x)), "the room for x in 4 bits overlaps x or the weights");
+    need(!meet(output, input) && apart(output, a.x) && apart(output, a.w), "out overlaps x, its room or the weights");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     a.rows = x;
     a.x_stride = x_stride;

@@ -383,3 +383,32 @@ def test_calls_that_follow_at_once(ops, groups, captured):
         for _ in range(20):
             assert torch.equal(run(stream(), False), want)
     ops.synchronize(stream())
+
+
+def test_scratch_in_others_memory_is_refused(ops):
+    """Scratch that shares a byte with queries, outputs or the cache is refused; scratch between rows is not."""
+    c = Case(FORMS[1], 2, 4, 64, 16)
+    a = c.args()
+    t, h, d = c.q.shape
+    need = a["scratch"].shape[0]
+    both = torch.zeros(need + t * h * d, device="cuda")  # scratch, then rows
+    rows = both.view(torch.float16)[2 * need:2 * need + t * h * d].view(t, h, d)
+    near = both.view(torch.float16)[2 * need - 8:2 * need - 8 + t * h * d].view(t, h, d)
+    for name in ("q", "out"):
+        with pytest.raises(ivb.NativeError):
+            ops.attend_shared(**{**a, "scratch": both[:need], name: near}, stream=stream())
+        with pytest.raises(ivb.NativeError):
+            ops.attend_shared(**{**a, "scratch": both[:need], name: near.view(h, t, d).transpose(0, 1)}, stream=stream())
+    codes = torch.zeros(4 * need + c.cache_t[0].numel(), dtype=torch.int8, device="cuda")
+    k = codes[4 * need - 16:][:c.cache_t[0].numel()].view(c.cache_t[0].shape)
+    scale = torch.zeros(need + c.cache_t[2].numel(), device="cuda")
+    for at, t_ in ((0, k), (1, k), (2, scale[need - 4:][:c.cache_t[2].numel()].view(c.cache_t[2].shape)), (3, scale[need - 4:][:c.cache_t[2].numel()].view(c.cache_t[2].shape))):
+        cache = list(c.cache_t)
+        cache[at] = t_
+        with pytest.raises(ivb.NativeError):
+            ops.attend_shared(**{**a, "cache": ivb.KvCache(*cache), "scratch": codes[:4 * need].view(torch.float32) if at < 2 else scale[:need]}, stream=stream())
+    rows.copy_(c.q)
+    c.q = rows
+    between = torch.zeros((t, need + h * d // 2), device="cuda")  # a token's rows, and room for all before the next one's
+    c.q = between.view(torch.float16)[:, :h * d].view(t, h, d).copy_(rows)
+    c.check(ops, scratch=between[1, h * d // 2:])

@@ -352,3 +352,42 @@ def test_quantize_leaves_the_rows_behind_alone(ops, rows, more, width):
     touched = (rows + 127) // 128  # (128-row pieces that no row of the call is in are not looked at)
     assert torch.equal(s[:touched].cpu(), want[:touched]) and (s[touched:] == 0xAA).all()
     assert torch.equal(c[:rows].cpu(), packed(first)) and (c[rows:] == 0xAA).all()
+
+
+def test_memory_that_is_read_and_written_is_refused(ops):
+    """Any byte that a call both reads and writes, or writes twice; rows that lie between one another are not refused."""
+    def refused(call, *args, **more):
+        with pytest.raises(ivb.NativeError):
+            call(*args, stream=stream(), **more)
+
+    rows, width = 16, 64
+    buf = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")
+    byte = buf.view(torch.uint8)
+    x = buf[:rows * width].view(rows, width)
+    w, room = ivb.Mx4(*empty(64, width, fill=0)), ivb.Mx4(*empty(rows, width, fill=0))
+    for at in (0, 1, rows * width - 1):  # the output in x, or one element into it
+        refused(ops.mx4_linear, x, w, buf[at:at + rows * 64].view(rows, 64), scratch=room)
+    refused(ops.mx4_linear, x[1:], w, buf[:15 * 64].view(15, 64), scratch=room)
+    refused(ops.mx4_linear, x[:8], w, torch.as_strided(buf, (8, 64), (96, 1), 511), scratch=room)
+    wide = buf[:rows * 200].view(rows, 200)
+    refused(ops.mx4_linear, wide[:, :64], w, wide[:, 63:127], scratch=room)
+    refused(ops.mx4_linear, wide[:, :64], w, torch.as_strided(buf, (rows, 64), (264, 1), 64), scratch=room)  # (other strides: they meet further down)
+    inside = ivb.Mx4(byte[1024:1024 + rows * 32].view(rows, 32), empty(rows, width)[1])
+    scales = ivb.Mx4(empty(rows, width)[0], byte[512:1024].view(1, 1, 32, 4, 4))
+    for m in (inside, scales):
+        refused(ops.mx4_linear, x, w, torch.empty_like(x), scratch=m)                       # the room in x
+        refused(ops.mx4_linear, torch.zeros_like(x), w, x, scratch=m)                       # the room in the output
+        refused(ops.mx4_linear, m, w, x)                                                    # x in 4 bits in the output
+        refused(ops.mx4_linear, torch.zeros_like(x), m, buf[256 if m is scales else 512:][:rows * rows].view(rows, rows), scratch=room)  # the weights
+        refused(ops.mx4_quantize, x, m)
+        refused(ops.mx4_read, m, x)
+    # columns of one buffer, and a matrix behind the rows
+    ops.mx4_quantize(torch.ones((64, width), dtype=torch.float16, device="cuda"), w, stream=stream())
+    wide[:, :64] = 1
+    ops.mx4_linear(wide[:, :64], w, wide[:, 64:128], scratch=room, stream=stream())
+    assert (wide[:, 64:128] == 64).all() and (wide[:, :64] == 1).all() and (wide[:, 128:] == 0).all()
+    ops.mx4_linear(wide[::2, :64], w, wide[::2, 128:192], scratch=room, stream=stream())
+    ops.mx4_linear(wide[:4, :64], w, torch.as_strided(buf, (4, 64), (400, 1), 264), scratch=room, stream=stream())  # (every second row, the columns between)
+    assert (wide[::2, 128:192] == 64).all() and (wide[1:9:2, 64:128] == 64).all() and (wide[:, :64] == 1).all()
+    ops.mx4_quantize(x, ivb.Mx4(byte[2 * rows * width:2 * rows * width + rows * 32].view(rows, 32), empty(rows, width)[1]), stream=stream())
+    ops.synchronize(stream())
