@@ -412,3 +412,199 @@ def test_scratch_in_others_memory_is_refused(ops):
     between = torch.zeros((t, need + h * d // 2), device="cuda")  # a token's rows, and room for all before the next one's
     c.q = between.view(torch.float16)[:, :h * d].view(t, h, d).copy_(rows)
     c.check(ops, scratch=between[1, h * d // 2:])
+
+
+def wide(c, table):
+    """`table` with the columns of `widened`."""
+    columns = widened(c).shape[1]
+    return ints(np.pad(table, ((0, 0), (0, columns - table.shape[1])), constant_values=-1))
+
+
+# Beginnings of few rows and of many, items that are cut and whole; a sequence's own keys always for the kernel of few rows.
+TWO = {n: FORMS[n] for n in (1, 3, 4, 6, 7, 8)}
+TWO["long"] = [(60, [(10 * i, 1) for i in range(24)]), (40, [(5 * i, 1) for i in range(24)])]  # (the parts of cut items are added up by a launch of their own)
+
+
+@pytest.mark.parametrize("form", list(TWO))
+@pytest.mark.parametrize("dtype,dim,group", [("bf16", 64, 4), ("f16", 128, 4), ("bf16", 128, 17)])
+@pytest.mark.parametrize("low,high", [(-30, 20), (20, -30)])
+def test_scales_far_apart_in_two_passes(ops, form, dtype, dim, group, low, high):
+    c = Case(TWO[form], 2, group, dim, 16, dtype, seed=7)
+    for n, p in enumerate(c.common):
+        c.cache_t[3][torch.from_numpy(c.full[c.first[n], :p // c.page]).long()] *= 2.0 ** low
+        for b in range(c.first[n], c.first[n + 1]):
+            own = c.full[b, p // c.page:]
+            c.cache_t[3][torch.from_numpy(own[own >= 0]).long()] *= 2.0 ** high
+    if dtype == "f16":  # (what is in the type's range)
+        c.cache_t[3].mul_(2.0 ** -20)
+    c.check(ops, pages=widened(c))
+
+
+@pytest.mark.parametrize("form", list(TWO))
+def test_zero_value_scales_in_two_passes(ops, form):
+    """A beginning, or a sequence's own keys, whose values are 0."""
+    for common in (True, False):
+        c = Case(TWO[form], 2, 4, 64, 16, "bf16", seed=7)
+        for n, p in enumerate(c.common):
+            for b in range(c.first[n], c.first[n + 1]):
+                some = c.full[b, :p // c.page] if common else c.full[b, p // c.page:]
+                c.cache_t[3][torch.from_numpy(some[some >= 0]).long()] = 0
+        c.check(ops, pages=widened(c))
+
+
+@pytest.mark.parametrize("form", [3, 4, 7, "long"])
+@pytest.mark.parametrize("layout", ["sliced", "odd_offset", "heads_first"])
+def test_layouts_in_two_passes(ops, form, layout):
+    c = Case(TWO[form], 2, 4, 64, 16, "f16", seed=1)
+    t, h, d = c.q.shape
+    if layout == "sliced":
+        q, out = (torch.zeros((t, 3 * h, d), dtype=c.q.dtype, device="cuda")[:, h:2 * h] for _ in range(2))
+    elif layout == "odd_offset":
+        q, out = (torch.zeros(t * h * d + 1, dtype=c.q.dtype, device="cuda")[1:].view(t, h, d) for _ in range(2))
+    else:
+        q, out = (torch.zeros((h, t, d), dtype=c.q.dtype, device="cuda").transpose(0, 1) for _ in range(2))
+    q.copy_(c.q)
+    c.q, c.out = q, out
+    c.check(ops, pages=widened(c))
+
+
+@pytest.mark.parametrize("form", [1, 3, 4, 7, "long"])
+def test_not_finite_query_stays_in_its_row_in_two_passes(ops, form):
+    c = Case(TWO[form], 2, 4, 64, 16, "f16", seed=3)
+    clean = c.run(ops, pages=widened(c)).clone()
+    c.q[1, 3, 7], c.q[-1, 0, 0] = math.nan, math.inf
+    got = c.run(ops, pages=widened(c))
+    same = torch.ones(c.q.shape[:2], dtype=torch.bool)
+    same[1, 3] = same[-1, 0] = False
+    assert torch.equal(got.cpu()[same], clean.cpu()[same]) and got[1, 3].isnan().all()
+
+
+@pytest.mark.parametrize("form", [3, 4, 7, "long"])
+def test_a_row_does_not_depend_on_its_neighbours_in_two_passes(ops, form):
+    c = Case(TWO[form], 2, 4, 64, 16, "f16", seed=4)
+    want = c.run(ops, pages=widened(c))[:1].clone()
+    c.q[1:] = c.q[1:].flip(0) * 3
+    assert torch.equal(c.run(ops, pages=widened(c))[:1], want)
+
+
+@pytest.mark.parametrize("what", ["length", "offsets", "common", "part_of_a_page", "negative", "first", "last", "not_covered", "page", "own_page", "max_new", "all"])
+@pytest.mark.parametrize("form", [3, 4, 8, "long"])
+def test_device_side_errors_are_reported_in_two_passes(ops, what, form):
+    """What does not fit is skipped and reported; the other groups are as they would be alone, and so is the next call."""
+    c = Case(TWO[form], 2, 4, 64, 16, "f16", seed=6)
+    table = widened(c)
+    want = c.run(ops, pages=table).clone()
+    a = c.args(pages=table.clone())
+    tokens = np.cumsum([0] + c.new)
+    skipped, wrong = np.zeros(tokens[-1], bool), np.zeros(tokens[-1], bool)  # rows that stay as they were; rows of which nothing is said
+    group0 = slice(0, tokens[c.first[1]])
+    if what == "length":
+        a["lens"][0] = c.common[0] + c.new[0] - 1
+        skipped[:c.new[0]] = True
+    elif what == "offsets":
+        a["offsets"][1] = 1 << 20
+        wrong[group0] = True
+    elif what in ("common", "part_of_a_page", "negative"):
+        a["shared"][0] = {"common": 1 << 20, "part_of_a_page": c.common[0] - 1, "negative": -16}[what]
+        skipped[group0] = True
+    elif what == "first":
+        a["groups"][0] = -1
+        skipped[group0] = True
+    elif what == "last":  # the last sequence is in no group
+        a["groups"][-1] -= 1
+        skipped[tokens[-2]:] = True
+    elif what == "not_covered":
+        a["groups"][0], a["pages"] = 1, wide(c, c.full)
+        skipped[:c.new[0]] = True
+    elif what == "page":
+        a["pages"][0, 0] = 1 << 20
+        wrong[group0] = True
+    elif what == "own_page":
+        a["pages"][0, c.common[0] // c.page] = 1 << 20
+        wrong[:c.new[0]] = True
+    elif what == "max_new":
+        a["max_new"] = max(c.new) - 1
+        for b, n in enumerate(c.new):
+            skipped[tokens[b]:tokens[b + 1]] = n == max(c.new)
+    else:  # no group fits: the second pass has nothing to do
+        a["shared"].fill_(-16)
+        skipped[:] = True
+    c.out.fill_(5.0)
+    if a["max_new"] == 0:
+        with pytest.raises(ivb.NativeError):
+            ops.attend_shared(**a, stream=stream())
+        return
+    ops.attend_shared(**a, stream=stream())
+    with pytest.raises(ivb.NativeError):
+        ops.synchronize(stream())
+    ops.synchronize(stream())
+    exact, bound = c.definition()
+    near = ((c.out.double().cpu() - exact).abs() <= bound * 1.01 + HALF_ULP["f16"] * exact.abs() + TINY["f16"]).all((1, 2)).numpy()
+    assert near[~skipped & ~wrong].all() and (c.out.cpu().numpy()[skipped] == 5.0).all()
+    # calls one behind the other, an erroneous one between
+    outs = []
+    for args in (c.args(pages=table), a, c.args(pages=table)):
+        c.out.fill_(math.nan)
+        ops.attend_shared(**args, stream=stream())
+        outs.append(c.out.clone())
+    with pytest.raises(ivb.NativeError):
+        ops.synchronize(stream())
+    assert torch.equal(outs[0], want) and torch.equal(outs[2], want)
+
+
+@pytest.mark.parametrize("groups", [[(3, [(7, 1), (90, 2)])], [(6, [(5 + i, 1) for i in range(9)])], [(3, [(70, 90), (3, 20)])]])
+def test_offsets_past_32_bits_in_two_passes(ops, groups):
+    """Common and own pages beyond 2^31 codes: a beginning for the kernel of few rows, of many, and both passes for that one."""
+    page, heads, dim, pages = 128, 8, 128, 17000
+    codes = [torch.zeros((pages, heads, page, dim), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros((pages, heads, page // BLOCK), device="cuda") for _ in range(2)]
+    c = Case(groups, heads, 8, dim, page, "f16", seed=8)
+    many = c.cache_t[0].shape[0]
+    far = np.arange(pages - many, pages)
+    for big, small in zip((*codes, *scales), c.cache_t):
+        big[torch.from_numpy(far).long()] = small
+    want = c.run(ops, pages=wide(c, c.table)).clone()
+    got = c.run(ops, cache=ivb.KvCache(*codes, *scales), pages=wide(c, np.where(c.table >= 0, far[c.table], -1)))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("form", [3, 4, 7, "long"])
+def test_same_bits_again_and_in_a_graph_in_two_passes(ops, form):
+    c = Case(TWO[form], 2, 4, 128, 16, "f16", seed=7)
+    table = widened(c)
+    want = c.run(ops, pages=table).clone()
+    for _ in range(4):
+        c.out.fill_(math.nan)
+        assert torch.equal(c.run(ops, pages=table), want)
+    a, side = c.args(pages=table), torch.cuda.Stream()
+    ops.reserve(side.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.attend_shared(**a, stream=side.cuda_stream)
+    for times in (1.0, 0.5):
+        c.q.mul_(times)
+        c.out.fill_(math.nan)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        again = c.out.clone()
+        assert torch.equal(c.run(ops, pages=table), again)
+    ops.release(side.cuda_stream)
+
+
+def test_streams_at_once_in_two_passes(ops):
+    cases = [Case(TWO[f], 2, 4, 64, 16, "f16", seed=7) for f in (3, 4, 7, 8, "long")]
+    args = [c.args(pages=widened(c)) for c in cases]
+    wants = [c.run(ops, pages=widened(c)).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[torch.empty_like(c.q) for _ in range(20)] for c in cases]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for a, st, o in zip(args, streams, outs):
+            ops.attend_shared(**{**a, "out": o[i]}, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for want, o in zip(wants, outs):
+        assert all(torch.equal(x, want) for x in o)
+    for st in streams:
+        ops.release(st.cuda_stream)
