@@ -141,6 +141,7 @@ struct Want {
     p = a.top_p && t > 0.f ? fmaxf(a.top_p[r], 0.f) : 1.f;
     if (!(a.top_p && a.top_p[r] < 1.f)) p = 1.f;
     min_p = a.min_p ? a.min_p[r] : 0.f;
+    if (min_p > 1.f && a.vocab > 1) k = 1;  // (no weight is as large: the first alone)
     u = a.u[r];
     u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   }

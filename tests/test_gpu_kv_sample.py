@@ -470,3 +470,24 @@ def test_weights_have_the_bits_of_64(ops, rows):
     got = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
     ops.sample(torch.tensor(x, device="cuda"), torch.full((rows,), 0.5, device="cuda"), got, stream=stream())
     assert (got.cpu().numpy() == np.where(first, 0, 1)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [4, 152])
+def test_min_p_above_every_weight(ops, dtype, rows):
+    """The first token in order alone, of several equal ones too."""
+    x = logits(rows, 3001, dtype, 6)
+    x[::2, [2000, 2001, 17, 900]] = 30.0
+    x[1::4] = 1.0
+    x[3::8, [5, 6]] = INF
+    x[7::16] = -INF
+    x[7::16, 3000] = 0
+    want = [int(np.argmax(v)) for v in x.double().cpu().numpy()]
+    for f in (dict(), dict(top_k=[50] * rows), dict(top_p=[0.9] * rows), dict(temperature=[1.7] * rows)):
+        tokens, probs = torch.full((rows,), -7, dtype=torch.int32, device="cuda"), torch.full((rows,), NAN, device="cuda")
+        more = {n: torch.tensor(v, device="cuda", dtype=torch.int32 if n == "top_k" else torch.float32) for n, v in f.items()}
+        ops.sample(x, torch.tensor(uniform(rows, 3), device="cuda"), tokens, probs, min_p=torch.tensor([1.5, INF] * (rows // 2), device="cuda"), stream=stream(), **more)
+        assert tokens.tolist() == want and (probs == 1).all()
+    one = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    ops.sample(x[:, :1], torch.rand(rows, device="cuda"), one, min_p=torch.full((rows,), 2.0, device="cuda"), stream=stream())
+    assert (one == torch.where(x[:, 0] == -INF, -1, 0)).all()
