@@ -1462,7 +1462,9 @@ struct Counter {
     }
     // The middles gave a guess of the bin; the weights up to a window around it are added up one by one.
     uint32_t b = locate<true>(target, middle) ? sh.bin : 0xffffu;
-    uint32_t lo = 0, hi = 0xffffu;  // the bin is one of these
+    // (top_k's cut lies in the last of them: its bin is in the window or behind it, so that what
+    // there is room for counts)
+    uint32_t lo = 0, hi = cut >> 16;  // the bin is one of these
     for (;;) {
       const uint32_t from = min(max(b > kWindow / 2 ? b - kWindow / 2 : 0u, lo), max(lo, hi + 1 > kWindow ? hi + 1 - kWindow : 0u));
       __syncthreads();
@@ -1506,9 +1508,9 @@ struct Counter {
       }
       if (hit < 0) {
         lo = from + kWindow;
-        if (lo > min(hi, cut >> 16)) {
+        if (lo > hi) {
           // (sums in another order have shown that it is no later than hi)
-          if (hi < cut >> 16 && hi < 0xffffu) cut_behind(hi);
+          if (hi < cut >> 16) cut_behind(hi);
           return true;
         }
         b = locate<true>(weight_before(lo, middle) + (target - base), middle) ? sh.bin : hi;

@@ -491,3 +491,19 @@ def test_min_p_above_every_weight(ops, dtype, rows):
     one = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
     ops.sample(x[:, :1], torch.rand(rows, device="cuda"), one, min_p=torch.full((rows,), 2.0, device="cuda"), stream=stream())
     assert (one == torch.where(x[:, 0] == -INF, -1, 0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [6, 42, 153])
+@pytest.mark.parametrize("vocab", [1001, 20252])
+def test_top_p_inside_the_run_that_top_k_cuts(ops, dtype, rows, vocab):
+    """Equal logits behind a larger one or a few: top_k ends among them, and top_p before that."""
+    r = np.random.default_rng(vocab + rows)
+    x = np.repeat(r.uniform(-6, 2, (rows, 1)), vocab, 1)
+    for i in range(rows):
+        x[i, r.integers(0, vocab, 1 + i % 3)] += r.uniform(0.5, 12, 1 + i % 3)
+    x, u = torch.tensor(x, device="cuda").to(TYPES[dtype]), uniform(rows, 9)
+    for k in ([vocab - 1] * rows, [vocab - 7] * rows, r.integers(5, vocab, rows)):
+        for p in ([0.9999] * rows, [0.99] * rows, r.random(rows)):
+            check(ops, x, u, top_k=k, top_p=p)
+            check(ops, x, np.float32(1) - u * np.float32(1e-4), top_k=k, top_p=p)
