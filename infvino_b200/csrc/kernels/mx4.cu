@@ -705,7 +705,7 @@ cudaError_t linear_rows(const Mx4Linear &l, cudaStream_t st) {
     return l.x_bf16 ? linear_tiles<16, 1, BF16, 2>(l, p, st) : linear_tiles<16, 1, BF16, 1>(l, p, st);
   }
   if (l.rows) {
-    const cudaError_t e = launch_mx4_quantize(l.x_bf16, l.rows, l.x.rows, l.x_stride, l.x, st);
+    const cudaError_t e = launch_mx4_quantize(l.x_bf16, l.rows, l.x.rows, l.x_stride, l.x, l.sms, st);
     if (e != cudaSuccess) return e;
   }
   switch (p.tn * 4 + p.mt) {
@@ -722,26 +722,26 @@ cudaError_t linear_rows(const Mx4Linear &l, cudaStream_t st) {
 }
 
 // Pieces of a warp, and the grid: few values go to many warps.
-dim3 quant_grid(long long width, long long rows, bool &four) {
+dim3 quant_grid(long long width, long long rows, int sms, bool &four) {
   const long long blocks = (rows + kQuantRows - 1) / kQuantRows;
-  four = width > 256 && blocks * ((width + 1023) / 1024) >= 148 * 2;
+  four = width > 256 && blocks * ((width + 1023) / 1024) >= sms * 2;
   const long long x = (width + (four ? 1023 : 255)) / (four ? 1024 : 256);
-  return dim3((unsigned)x, (unsigned)std::min(blocks, std::max(1ll, 148 * 8 / x)));
+  return dim3((unsigned)x, (unsigned)std::min(blocks, std::max(1ll, sms * 8 / x)));
 }
 
 template <bool BF16>
-cudaError_t quantize(const void *x, long long rows, long long stride, const Mx4 &m, cudaStream_t st) {
+cudaError_t quantize(const void *x, long long rows, long long stride, const Mx4 &m, int sms, cudaStream_t st) {
   const long long padded = (rows + 127) / 128 * 128;  // (scale bytes of rows that are not there are 0)
   bool four;
-  const dim3 grid = quant_grid(m.width, padded, four);
+  const dim3 grid = quant_grid(m.width, padded, sms, four);
   const uint16_t *p = static_cast<const uint16_t *>(x);
   if (four) return launch_kernel(mx4_quantize_k<BF16, 4>, grid, dim3(kQuantThreads), 0, st, p, rows, padded, stride, (int)rows_vec(x, stride), m);
   return launch_kernel(mx4_quantize_k<BF16, 1>, grid, dim3(kQuantThreads), 0, st, p, rows, padded, stride, (int)rows_vec(x, stride), m);
 }
 template <bool BF16>
-cudaError_t read(const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st) {
+cudaError_t read(const Mx4 &m, long long rows, void *out, long long stride, int sms, cudaStream_t st) {
   bool four;
-  const dim3 grid = quant_grid(m.width, rows, four);
+  const dim3 grid = quant_grid(m.width, rows, sms, four);
   uint16_t *p = static_cast<uint16_t *>(out);
   if (four) return launch_kernel(mx4_read_k<BF16, 4>, grid, dim3(kQuantThreads), 0, st, m, rows, p, stride, (int)rows_vec(out, stride));
   return launch_kernel(mx4_read_k<BF16, 1>, grid, dim3(kQuantThreads), 0, st, m, rows, p, stride, (int)rows_vec(out, stride));
@@ -749,13 +749,13 @@ cudaError_t read(const Mx4 &m, long long rows, void *out, long long stride, cuda
 
 }  // namespace
 
-cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long long stride, const Mx4 &m,
+cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long long stride, const Mx4 &m, int sms,
                                 cudaStream_t st) {
-  return bf16 ? quantize<true>(x, rows, stride, m, st) : quantize<false>(x, rows, stride, m, st);
+  return bf16 ? quantize<true>(x, rows, stride, m, sms, st) : quantize<false>(x, rows, stride, m, sms, st);
 }
 
-cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st) {
-  return bf16 ? read<true>(m, rows, out, stride, st) : read<false>(m, rows, out, stride, st);
+cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, int sms, cudaStream_t st) {
+  return bf16 ? read<true>(m, rows, out, stride, sms, st) : read<false>(m, rows, out, stride, sms, st);
 }
 
 cudaError_t launch_mx4_linear(const Mx4Linear &a, cudaStream_t st) {

@@ -20,9 +20,9 @@ __host__ __device__ inline long long mx4_scale_at(long long r, long long b, long
   return ((r >> 7) * chunks + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
 }
 
-cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long long stride, const Mx4 &m,
+cudaError_t launch_mx4_quantize(bool bf16, const void *x, long long rows, long long stride, const Mx4 &m, int sms,
                                 cudaStream_t st);
-cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, cudaStream_t st);
+cudaError_t launch_mx4_read(bool bf16, const Mx4 &m, long long rows, void *out, long long stride, int sms, cudaStream_t st);
 struct Mx4Linear {
   Mx4 x, w;         // x.rows: the rows that are used
   const void *rows;  // if not null: 16-bit rows that X is quantised from, x is room for it

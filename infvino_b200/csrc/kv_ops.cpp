@@ -598,7 +598,7 @@ int ivc_kv_mx4_quantize(ivc_kv *h, int dtype, const void *x, int64_t rows, int64
     need(rows <= q.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0) return;
     need(apart(matrix(x, rows, q.width, x_stride), first_rows(q, rows)), "the 4-bit matrix overlaps x");
-    cuda(ivb::launch_mx4_quantize(dtype == IVC_BF16, x, rows, x_stride, q, static_cast<cudaStream_t>(stream)), "launch");
+    cuda(ivb::launch_mx4_quantize(dtype == IVC_BF16, x, rows, x_stride, q, h->sms, static_cast<cudaStream_t>(stream)), "launch");
   });
 }
 
@@ -609,7 +609,7 @@ int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *
     need(rows <= q.rows, "the 4-bit matrix has fewer rows");
     if (rows == 0) return;
     need(apart(matrix(out, rows, q.width, out_stride), first_rows(q, rows)), "out overlaps the 4-bit matrix");
-    cuda(ivb::launch_mx4_read(dtype == IVC_BF16, q, rows, out, out_stride, static_cast<cudaStream_t>(stream)), "launch");
+    cuda(ivb::launch_mx4_read(dtype == IVC_BF16, q, rows, out, out_stride, h->sms, static_cast<cudaStream_t>(stream)), "launch");
   });
 }
 
