@@ -357,7 +357,9 @@ int ivc_kv_read(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, i
  * the keys j <= p, with window > 0 only those with p - j < window or
  * j < sinks.  q_heads is a multiple of kv_heads; query head h reads kv head
  * h / (q_heads / kv_heads).  A row that sees nothing gives 0.  max_new: at
- * least the largest number of new tokens of one sequence. */
+ * least the largest number of new tokens of one sequence.  Scores, maxima and
+ * sums are in f32; a weight meets the values as a half, with 11 bits down to
+ * 2^-22 of a row's largest weight times value scale and fewer below. */
 int ivc_kv_attend(ivc_kv *h, const ivc_kv_cache *cache, const ivc_kv_seqs *seqs, int dtype, int q_heads, int max_new,
                   const ivc_rows *q, const ivc_rows *out, float scale, int window, int sinks, void *stream);
 
@@ -371,7 +373,7 @@ typedef struct ivc_kv_groups {
 } ivc_kv_groups;
 /* ivc_kv_attend without a window, for groups of sequences with a common
  * beginning (samples or questions over the same frames): its keys and values are
- * read once for all of a group's queries.  Every sequence's new tokens come
+ * read once for all of a group's queries, with ivc_kv_attend's roundings.  Every sequence's new tokens come
  * after it (lens[b] - new tokens >= shared[g]); a sequence's own pages for the
  * first shared[g] tokens are not looked at.  A group whose sequences, or whose
  * shared[g], do not fit is skipped, as is a sequence that ends inside the
@@ -405,8 +407,11 @@ typedef struct ivc_sampling {
  * all kept ones, probs[row] (NULL: not wanted) its share of that.  With a
  * temperature that is not above 0 it is the first in order, with probability 1.
  * A logit of NaN counts as -inf; where one is +inf, only those have a weight; a
- * row of -inf alone gives token -1 with probability 0.  Sums are in 64 bits;
- * weights below 2^-60 count as 0.  u is taken into [0, 1) (NaN: 0). */
+ * row of -inf alone gives token -1 with probability 0.  Weights and sums are in 64
+ * bits; weights below 2^-60 count as 0.  u is taken into [0, 1) (NaN: 0).  The order
+ * of the sums goes by vocab, the number of rows, the device and the row's address
+ * modulo 16: with these the same, so is every bit; otherwise a row within a rounding
+ * of a border may get a neighbouring cut or token. */
 int ivc_kv_sample(ivc_kv *h, const ivc_logits *logits, const ivc_sampling *how, int32_t *tokens, float *probs,
                   void *stream);
 
@@ -438,7 +443,8 @@ int ivc_kv_mx4_read(ivc_kv *h, const ivc_mx4 *m, int64_t rows, int dtype, void *
  * first `rows` rows of xq if x is NULL, else x [rows][width] (x_dtype), quantised as
  * ivc_kv_mx4_quantize does it: xq is room for that then, of nobody else until
  * the call has run, and what it holds afterwards is not defined.  out, and the room
- * for x, share no memory with the others (rows may lie between one another's).  Outputs of out_dtype (IVC_F16 or IVC_BF16). */
+ * for x, share no memory with the others (rows may lie between one another's).
+ * Outputs of out_dtype (IVC_F16 or IVC_BF16). */
 int ivc_kv_mx4_linear(ivc_kv *h, int x_dtype, const void *x, int64_t rows, int64_t x_stride, const ivc_mx4 *xq,
                       const ivc_mx4 *w, int out_dtype, void *out, int64_t out_stride, void *stream);
 

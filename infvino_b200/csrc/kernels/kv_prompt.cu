@@ -311,6 +311,7 @@ __device__ __noinline__ void count_rest(const KvAttend &a, Shared &sh, unsigned 
         count_part(&counters[2 * g.first_cta + i], g.first_cta, g.last_cta);
 }
 
+// (128 registers a thread; kRest, which holds the join's shares too, spills up to 112 bytes, the others up to 52.)
 template <bool BF16, int DIM, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_prompt_k(const __grid_constant__ KvAttend a, PromptSlot *slots, unsigned *counters) {

@@ -6,7 +6,8 @@
 // a cut: the last (logit, number) that is kept.  The token is then the first, by
 // number, where the running sum of kept weights passes u times their sum.  Which
 // one that is goes by sums next to a border, so weights and sums are in 64 bits,
-// added in an order that is fixed for a size and a number of rows.
+// added in an order that is fixed for a size, a number of rows, a device and a row's
+// address (modulo 16 bytes): a token next to a border may be another one elsewhere.
 //
 // Two kernels.  sample_count_k, for logits in 16 bits: a CTA a row counts how often
 // each of the 65536 values occurs, in shared memory.  A value's weight is then worked
@@ -920,6 +921,7 @@ struct Row {
   }
 };
 
+// (Two CTAs an SM, so 64 registers a thread: some 340 bytes spill.)
 template <class T>
 __global__ void __launch_bounds__(kClusterThreads, 2) sample_k(const __grid_constant__ Sample a) {
   extern __shared__ __align__(16) uint8_t slice_raw[];
@@ -1839,8 +1841,9 @@ cudaError_t launch_count(const Sample &a, cudaStream_t st) {
 template <class T>
 cudaError_t launch(const Sample &a, int sms, cudaStream_t st) {
   constexpr int kResident = 184 << 10;  // bytes of a slice that is kept
-  // A CTA a row is enough where there are many.  Us in a cluster / by counting, rows of
-  // 131072, with top p / with top k, top p and min p: 16-bit logits, 1 row 25/43 and 25/43,
+  // A CTA a row is enough where there are many.  (Measured at one width; top p alone is faster
+  // by counting from fewer rows on, which this does not look at.)  Us in a cluster / by
+  // counting, rows of 131072, with top p / with top k, top p and min p: 16-bit logits, 1 row 25/43 and 25/43,
   // 32 rows 66/72 and 61/54, 48 rows 113/73 and 84/55; 32 bits, 16 rows 59/190 and 53/131,
   // 100 rows 175/156 and 100/190, 148 rows 234/158 and 132/154.
   if (a.rows >= (sizeof(T) == 2 ? 40 : 148)) return launch_count<T>(a, st);

@@ -292,7 +292,8 @@ class KvOps:
         groups[g] .. groups[g + 1] - 1 (groups int32 [count + 1], from 0 to batch)
         have their first shared[g] tokens (int32 [count], whole pages) in common, in
         the pages of the group's first sequence, and those are read once for all of
-        the group.  scratch: float32, at least tokens * q_heads * (head_dim + 2)."""
+        the group.  scratch: float32, at least tokens * q_heads * (head_dim + 2), in
+        nobody else's memory."""
         name, sh, d = _kind(q, "q"), q.shape, self.device
         tokens, heads, dim = sh
         if dim != cache.head_dim:
@@ -346,7 +347,7 @@ class KvOps:
         return p, rows, st, dt
 
     def mx4_quantize(self, x, m: Mx4, stream: int = 0) -> None:
-        """The first rows of m = x [rows, width] (float16 or bfloat16), width m's, rows at most m's."""
+        """The first rows of m = x [rows, width] (float16 or bfloat16), width m's, rows at most m's; the others stay."""
         p, rows, st, dt = self._rows_of(x, "x", m)
         st = self._quantize(self._h, dt, p, rows, st, m._m, stream)
         if st:
@@ -363,7 +364,8 @@ class KvOps:
         """out [rows, w.rows] = x w^T with both in 4 bits: x is an `Mx4`, or a
         float16 / bfloat16 tensor [rows, width], which is quantised on the way;
         `scratch` is room for that (an Mx4 of at least as many rows, whose contents
-        are not defined afterwards).  Sums are in 32 bits."""
+        are not defined afterwards).  out and scratch lie apart from the others.  Sums
+        are in 32 bits."""
         d, width = self.device, w.width
         rows = out.shape[0]
         o, ost, odt = _matrix(out, "out", d, rows, w.rows)
